@@ -226,6 +226,7 @@ int64_t bounds_error(bool reset) {
 
 void register_gemm(pybind11::module& m);
 void register_comm(pybind11::module& m);
+void register_fp8(pybind11::module& m);
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "nanovllm_self_b200 sm_100a kernels";
@@ -255,4 +256,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.attr("BOUNDS_CHECK") = (int64_t)nvb::bounds_check_enabled();
   register_gemm(m);
   register_comm(m);
+  register_fp8(m);
 }

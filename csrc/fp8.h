@@ -1,0 +1,44 @@
+// Host interface of the fp8 (e4m3) layer kernels: quantisation, norm and matrix products with
+// block scales (raw pointers, no torch types).
+#pragma once
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace nvb {
+
+constexpr int FP8_GROUP = 128;  // channels of one activation scale; side of one weight scale's block
+
+// q[T, K] (e4m3) and s (one fp32 scale per token and 128 channels, s[g * lds + t]) of x[T, K] (bf16,
+// row stride ldx).  K % 16 == 0, ldx % 8 == 0, 16-byte aligned x, 8-byte aligned q.
+cudaError_t launch_quant_fp8(const void* x, int64_t ldx, void* q, float* s, int64_t lds, int T, int K,
+                             cudaStream_t stream);
+
+// r = bf16(x + residual) (written back to `residual`), or x where residual is null;
+// (q, s) = quantised rmsnorm(r) * w.  K % 16 == 0, K <= 16384.
+cudaError_t launch_add_rmsnorm_fp8(const void* x, int64_t ldx, void* residual, const void* w, void* q, float* s,
+                                   int64_t lds, int T, int K, float eps, cudaStream_t stream);
+
+// Y[T, N] = sum over 128-blocks b of k of xs[b * ldxs + t] ws[(n / 128) * ldws + b] sum_k xq wq.
+struct Fp8Gemm {
+  const void* xq;    // e4m3 [T, K], row stride ldx (bytes, a multiple of 16), 16-byte aligned
+  const float* xs;   // [K / 128][T], row stride ldxs (a multiple of 4), 16-byte aligned
+  const void* wq;    // e4m3 [N, K], row stride ldw
+  const float* ws;   // [N / 128][K / 128], row stride ldws
+  int64_t ldx, ldxs, ldw, ldws;
+  int T, N, K;
+  // act = 0: out is bf16 [T, N], row stride ldo.  act = 1 (SiLU-and-mul): W's rows are alternating
+  // blocks of 128 gate rows and the 128 matching up rows; out is e4m3 [T, features], row stride
+  // ldo (a multiple of 16), and os (os[g * ldos + t]) its scales.
+  int act;
+  int features;
+  void* out;
+  int64_t ldo;
+  float* os;
+  int64_t ldos;
+};
+cudaError_t gemm_fp8(const Fp8Gemm& g, int num_sms, cudaStream_t stream);
+
+// Error word written by an fp8 GEMM that gave up on a bounded wait (0 = none).
+int gemm_fp8_error_code(int reset);
+
+}  // namespace nvb

@@ -1,0 +1,152 @@
+// bf16 -> e4m3 with one scale per token and 128 channels, alone and behind residual add + RMSNorm.
+//
+// No counterpart in the reference (its products are all 16-bit); the norm is its RMSNorm
+// (nanovllm/layers/RMSNorm.py:11-17) with the 8-bit rounding of the next product's input fused in.
+// Both are bound by memory traffic: 3 bytes per value for the quantisation (2 read, 1 written), 7
+// for the norm (x and the residual read, the residual and the 8-bit value written).
+#include "fp8_quant.cuh"
+
+namespace nvb {
+namespace {
+
+constexpr int QROWS = 16;   // rows per CTA: one half-warp each
+constexpr int QGROUPS = 4;  // groups per half-warp, all of whose loads are in flight together
+
+// A half-warp holds a group of 128 as 16 lanes x 8 values.  The 16 half-warps of a CTA take 16
+// consecutive tokens of the same groups, so that a group's scales leave as 64 contiguous bytes
+// (scales are stored token-contiguous, the order in which the products read them).
+__global__ void __launch_bounds__(QROWS * 16) quant_fp8_kernel(const __nv_bfloat16* __restrict__ x, int64_t ldx,
+                                                               uint8_t* __restrict__ q, float* __restrict__ s,
+                                                               int64_t lds, int T, int K) {
+  pdl_wait();     // inputs come from the previous kernel in the stream
+  pdl_trigger();  // the next kernel may start its prologue
+  const int hw = threadIdx.x >> 4, l = threadIdx.x & 15;
+  const int kb = (K + FP8_GROUP - 1) / FP8_GROUP;
+  const int chunks = (kb + QGROUPS - 1) / QGROUPS;
+  const int t = (int)(blockIdx.x / chunks) * QROWS + hw;
+  const int g0 = (int)(blockIdx.x % chunks) * QGROUPS;
+  uint4 v[QGROUPS];
+#pragma unroll
+  for (int i = 0; i < QGROUPS; ++i) {
+    const int c = (g0 + i) * FP8_GROUP + l * 8;
+    v[i] = make_uint4(0, 0, 0, 0);
+    if (t < T && c < K) v[i] = *reinterpret_cast<const uint4*>(x + (int64_t)t * ldx + c);
+  }
+#pragma unroll
+  for (int i = 0; i < QGROUPS; ++i) {
+    // |bf16| as 16-bit integers, two per word
+    uint32_t m = __vmaxu2(__vmaxu2(v[i].x & 0x7fff7fffu, v[i].y & 0x7fff7fffu),
+                          __vmaxu2(v[i].z & 0x7fff7fffu, v[i].w & 0x7fff7fffu));
+    m = max(m & 0xffff0000u, m << 16);  // as an fp32 magnitude
+    const Fp8Scale sc = fp8_scale(half_warp_umax(m));
+    const int c = (g0 + i) * FP8_GROUP + l * 8;
+    if (t < T && c < K) {
+      float f[8];
+      bf16x8_to_f32(v[i], f);
+      *reinterpret_cast<uint2*>(q + (int64_t)t * K + c) = f32x8_to_e4m3(f, sc.inv);
+    }
+    if (l == 0 && t < T && g0 + i < kb) s[(g0 + i) * lds + t] = sc.scale;
+  }
+}
+
+// One CTA per row, 8 values per thread and step; a group of 128 is the 16 lanes of a half-warp.
+template <int NI>
+__global__ void __launch_bounds__(256) add_rmsnorm_fp8_kernel(const __nv_bfloat16* __restrict__ x, int64_t ldx,
+                                                              __nv_bfloat16* __restrict__ residual,
+                                                              const __nv_bfloat16* __restrict__ w,
+                                                              uint8_t* __restrict__ q, float* __restrict__ s,
+                                                              int64_t lds, int K, float eps) {
+  pdl_wait();     // inputs come from the previous kernel in the stream
+  pdl_trigger();  // the next kernel may start its prologue
+  const int row = blockIdx.x;
+  const int nvec = K >> 3;
+  const uint4* xr = reinterpret_cast<const uint4*>(x + (int64_t)row * ldx);
+  uint4* rr = reinterpret_cast<uint4*>(residual + (int64_t)row * K);
+  float v[NI][8];
+  float ss = 0.f;
+#pragma unroll
+  for (int i = 0; i < NI; ++i) {
+    const int c = threadIdx.x + i * blockDim.x;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
+    if (c < nvec) {
+      bf16x8_to_f32(xr[c], v[i]);
+      if (residual) {
+        // the residual stream stays bf16, as an eager bf16 add keeps it
+        float r[8];
+        bf16x8_to_f32(rr[c], r);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[i][j] = bf16_round(v[i][j] + r[j]);
+        rr[c] = f32_to_bf16x8(v[i]);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) ss += v[i][j] * v[i][j];
+  }
+  __shared__ float red[8];
+  ss = warp_sum(ss);
+  const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  if (lane == 0) red[wid] = ss;
+  __syncthreads();
+  float tot = 0.f;
+  for (int i = 0; i < warps; ++i) tot += red[i];
+  const float inv_rms = rsqrtf(tot / (float)K + eps);
+  const uint4* wr = reinterpret_cast<const uint4*>(w);
+#pragma unroll
+  for (int i = 0; i < NI; ++i) {
+    const int c = threadIdx.x + i * blockDim.x;
+    uint32_t m = 0;
+    float o[8];
+    if (c < nvec) {
+      float wf[8];
+      bf16x8_to_f32(wr[c], wf);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        o[j] = v[i][j] * inv_rms * wf[j];
+        m = max(m, __float_as_uint(o[j]) & 0x7fffffffu);
+      }
+    }
+    const Fp8Scale sc = fp8_scale(half_warp_umax(m));
+    if (c < nvec) {
+      *reinterpret_cast<uint2*>(q + (int64_t)row * K + c * 8) = f32x8_to_e4m3(o, sc.inv);
+      if ((c & 15) == 0) s[(int64_t)(c >> 4) * lds + row] = sc.scale;
+    }
+  }
+}
+
+}  // namespace
+
+cudaError_t launch_quant_fp8(const void* x, int64_t ldx, void* q, float* s, int64_t lds, int T, int K,
+                             cudaStream_t stream) {
+  if (T == 0) return cudaSuccess;
+  const int kb = (K + FP8_GROUP - 1) / FP8_GROUP;
+  const int64_t ctas = (int64_t)((T + QROWS - 1) / QROWS) * ((kb + QGROUPS - 1) / QGROUPS);
+  if (K % 16 || ldx % 8 || ctas > 0x7fffffff) return cudaErrorInvalidValue;
+  launch_pdl(quant_fp8_kernel, dim3((unsigned)ctas), dim3(QROWS * 16), 0, stream,
+             static_cast<const __nv_bfloat16*>(x), ldx, static_cast<uint8_t*>(q), s, lds, T, K);
+  NVB_LAUNCH_CHECK();
+  return cudaSuccess;
+}
+
+cudaError_t launch_add_rmsnorm_fp8(const void* x, int64_t ldx, void* residual, const void* w, void* q, float* s,
+                                   int64_t lds, int T, int K, float eps, cudaStream_t stream) {
+  if (T == 0) return cudaSuccess;
+  if (K % 16 || ldx % 8 || K > 8 * 256 * 8) return cudaErrorInvalidValue;
+  const int nvec = K / 8;
+  const int threads = nvec >= 256 ? 256 : (nvec + 31) / 32 * 32;
+  const int ni = (nvec + threads - 1) / threads;
+  auto X = static_cast<const __nv_bfloat16*>(x);
+  auto R = static_cast<__nv_bfloat16*>(residual);
+  auto W = static_cast<const __nv_bfloat16*>(w);
+  auto Q = static_cast<uint8_t*>(q);
+  auto go = [&](auto kern) { launch_pdl(kern, dim3(T), dim3(threads), 0, stream, X, ldx, R, W, Q, s, lds, K, eps); };
+  if (ni == 1) go(add_rmsnorm_fp8_kernel<1>);
+  else if (ni == 2) go(add_rmsnorm_fp8_kernel<2>);
+  else if (ni == 3) go(add_rmsnorm_fp8_kernel<3>);
+  else if (ni == 4) go(add_rmsnorm_fp8_kernel<4>);
+  else go(add_rmsnorm_fp8_kernel<8>);
+  NVB_LAUNCH_CHECK();
+  return cudaSuccess;
+}
+
+}  // namespace nvb

@@ -1,0 +1,366 @@
+// fp8 (e4m3) matrix product with block scales on the 5th-generation tensor cores, sm_100a.
+//
+//   Y[t, n] = sum_b xs[t, b] ws[n / 128, b] sum_{k in block b} xq[t, k] wq[n, k]
+//
+// b runs over blocks of 128 channels: activations carry a scale per token and block, weights one
+// per 128 x 128 block.  The scales are arbitrary fp32 numbers, so the tensor core cannot apply
+// them: every block's product is a separate MMA accumulation in TMEM, and the epilogue warps add it,
+// scaled, to fp32 accumulators in registers while the tensor core works on the next block (two TMEM
+// buffers).
+//
+// No counterpart in the reference, whose linear layers are 16-bit (nanovllm/models/qwen3.py:96-134).
+//
+// gemm_fp8_tokens_kernel: tiles of 128 tokens (MMA M, one TMEM lane each) x 256 features (MMA N).
+// A thread of the epilogue owns one token and 64 + 64 features, [64 w, 64 w + 64) of both 128-row
+// weight blocks of the tile: both scales are then one number per thread and k-block (no scale
+// vector to load), and with gate and up rows in alternating blocks of 128 the thread holds matching
+// gate / up pairs, so SiLU-and-mul needs no exchange and the tile is one whole group of 128 of the
+// 8-bit output.
+//
+// Every wait is bounded; on expiry the kernel records an error code, drains its copies, frees TMEM
+// and returns.
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
+#include "fp8_quant.cuh"
+#include "tcgen05.cuh"
+
+namespace nvb {
+
+__device__ int g_fp8_error = 0;
+
+namespace {
+
+using namespace tc;
+
+constexpr int BM = 128;                 // tokens per tile
+constexpr int BN = 256;                 // features per tile
+constexpr int BK = 128;                 // one scale block = one 128-byte swizzle row
+constexpr int STAGES = 4;
+constexpr int A_BYTES = BM * BK, B_BYTES = BN * BK, STAGE_BYTES = A_BYTES + B_BYTES;
+constexpr int THREADS = 320;            // TMA warp, MMA warp, 8 epilogue warps
+constexpr int EPI_THREADS = 256;
+constexpr int SMEM_TOKENS = 1024 + STAGES * STAGE_BYTES + 2 * 2 * BM * 4 + 8 * (2 * STAGES + 6) + 16;
+
+struct Params {
+  const float* xs;
+  const float* ws;
+  int64_t ldxs, ldws;
+  int T, N, num_kb, nb;      // nb: 128-row blocks of W
+  int tiles_m, tiles_n, group;
+  int act, features, vec;    // vec: bf16 rows allow 16-byte stores
+  void* out;
+  int64_t ldo;
+  float* os;
+  int64_t ldos;
+};
+
+// Tile order: groups of `group` token tiles walk the features together, so that CTAs which run at
+// the same time share operand tiles in L2.
+__device__ __forceinline__ void tile_coords(const Params& p, int t, int& tm, int& tn) {
+  const int per_group = p.group * p.tiles_n;
+  const int g = t / per_group;
+  const int first = g * p.group;
+  const int size = min(p.group, p.tiles_m - first);
+  const int r = t - g * per_group;
+  tm = first + r % size;
+  tn = r / size;
+}
+
+__device__ __forceinline__ float silu_f(float g) { return g / (1.f + expf(-g)); }
+
+// bf16 values [c, c + 64) of one row (accumulator pairs in `acc`).
+__device__ __forceinline__ void store_bf16_64(const Params& p, int row, int c, const uint64_t* acc) {
+  if (row >= p.T || c >= p.N) return;
+  __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(p.out) + (int64_t)row * p.ldo + c;
+  const int n = p.N - c;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    float f[8];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 v = unpack2(acc[4 * i + j]);
+      f[2 * j] = v.x;
+      f[2 * j + 1] = v.y;
+    }
+    if (p.vec && 8 * i + 8 <= n) {
+      *reinterpret_cast<uint4*>(dst + 8 * i) = f32_to_bf16x8(f);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (8 * i + j < n) dst[8 * i + j] = __float2bfloat16_rn(f[j]);
+    }
+  }
+}
+
+__global__ void __launch_bounds__(THREADS, 1)
+    gemm_fp8_tokens_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
+                           Params p) {
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint32_t* amax = reinterpret_cast<uint32_t*>(smem + STAGES * STAGE_BYTES);  // [tile parity][half][token]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(amax + 2 * 2 * BM);
+  const uint32_t bar0 = smem_u32(bars);
+  auto full = [&](int s) { return bar0 + 8u * s; };
+  auto empty = [&](int s) { return bar0 + 8u * (STAGES + s); };
+  auto tfull = [&](int b) { return bar0 + 8u * (2 * STAGES + b); };
+  auto tempty = [&](int b) { return bar0 + 8u * (2 * STAGES + 2 + b); };
+  const uint32_t final_bar = bar0 + 8u * (2 * STAGES + 4);
+  const uint32_t amax_bar = bar0 + 8u * (2 * STAGES + 5);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + 2 * STAGES + 6);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * STAGES + 6) + 1;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(full(s), 1);
+      mbar_init(empty(s), 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(tfull(b), 1);
+      mbar_init(tempty(b), EPI_THREADS / 32);
+    }
+    mbar_init(final_bar, 1);
+    mbar_init(amax_bar, EPI_THREADS / 32);
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 1) tmem_alloc(smem_u32(tmem_slot), 512);
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = *tmem_slot;
+  pdl_trigger();
+  pdl_wait();
+
+  const int tiles = p.tiles_m * p.tiles_n;
+  if (warp == 0 && lane == 0) {
+    // ------------------------------------------------------------------ producer
+    prefetch_map(&map_x);
+    prefetch_map(&map_w);
+    uint32_t it = 0;
+    bool ok = true;
+    for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+      int tm, tn;
+      tile_coords(p, t, tm, tn);
+      for (int kb = 0; kb < p.num_kb; ++kb, ++it) {
+        const int s = it % STAGES;
+        if (!mbar_wait(empty(s), ((it / STAGES) & 1) ^ 1, abort_flag, &g_fp8_error, 501)) {
+          ok = false;
+          break;
+        }
+        mbar_arrive_expect_tx(full(s), STAGE_BYTES);
+        const uint32_t st = smem_u32(smem + s * STAGE_BYTES);
+        tma_load_2d(st, &map_x, full(s), kb * BK, tm * BM);
+        tma_load_2d(st + A_BYTES, &map_w, full(s), kb * BK, tn * BN);
+      }
+    }
+    if (!ok) {
+      const uint32_t n = it < (uint32_t)STAGES ? it : (uint32_t)STAGES;
+      for (uint32_t j = it - n; j < it; ++j) mbar_drain(full(j % STAGES), (j / STAGES) & 1);
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------------ MMA issuer
+    const uint32_t tbase = __shfl_sync(FULL_MASK, tmem, 0);
+    uint32_t it = 0;
+    bool ok = true;
+    for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+      for (int kb = 0; kb < p.num_kb; ++kb, ++it) {
+        const int s = it % STAGES, b = it & 1;
+        int okw = 1;
+        if (lane == 0)
+          okw = mbar_wait(tempty(b), ((it >> 1) & 1) ^ 1, abort_flag, &g_fp8_error, 502) &&
+                mbar_wait(full(s), (it / STAGES) & 1, abort_flag, &g_fp8_error, 503);
+        ok = __shfl_sync(FULL_MASK, okw, 0);
+        if (!ok) break;
+        fence_after();
+        const uint32_t st = smem_u32(smem + s * STAGE_BYTES);
+        const uint64_t ad = sdesc(st), bd = sdesc(st + A_BYTES);
+        if (elect_one()) {
+#pragma unroll
+          for (int k = 0; k < BK / 32; ++k)
+            mma_f8(tbase + b * BN, ad + 2 * k, bd + 2 * k, idesc_f8(BM, BN), k > 0 ? 1u : 0u);
+          commit(empty(s));
+          commit(tfull(b));
+        }
+        __syncwarp();
+      }
+    }
+    if (elect_one()) commit(final_bar);
+    if (lane == 0) mbar_drain(final_bar, 0);
+    __syncwarp();
+  } else if (warp >= 2) {
+    // ------------------------------------------------------------------ epilogue
+    const int q4 = warp & 3, wg = (warp - 2) >> 2;
+    uint32_t it = 0, tile_parity = 0;
+    bool ok = true;
+    for (int t = blockIdx.x; t < tiles; t += gridDim.x, tile_parity ^= 1) {
+      int tm, tn;
+      tile_coords(p, t, tm, tn);
+      const int row = tm * BM + q4 * 32 + lane;
+      const float* xs = p.xs + row;
+      const float* ws0 = p.ws + (int64_t)(2 * tn) * p.ldws;
+      const float* ws1 = p.ws + (int64_t)min(2 * tn + 1, p.nb - 1) * p.ldws;
+      uint64_t acc[2][32];
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < 32; ++i) acc[h][i] = 0;
+      float x_n = row < p.T ? xs[0] : 0.f, w0_n = ws0[0], w1_n = ws1[0];
+      for (int kb = 0; kb < p.num_kb; ++kb, ++it) {
+        const float s0 = x_n * w0_n, s1 = x_n * w1_n;
+        const uint64_t sc[2] = {pack2(s0, s0), pack2(s1, s1)};
+        if (kb + 1 < p.num_kb) {
+          x_n = row < p.T ? xs[(int64_t)(kb + 1) * p.ldxs] : 0.f;
+          w0_n = ws0[kb + 1];
+          w1_n = ws1[kb + 1];
+        }
+        const int b = it & 1;
+        ok = mbar_wait(tfull(b), (it >> 1) & 1, abort_flag, &g_fp8_error, 504);
+        ok = __all_sync(FULL_MASK, ok);  // the warp stays together
+        if (!ok) break;
+        fence_after();
+        const uint32_t ta = tmem + ((uint32_t)(q4 * 32) << 16) + b * BN + wg * 64;
+        // 8 chunks of 16 columns (4 of each half), the next one in flight while one is added
+        uint32_t v[2][16];
+        tmem_ld16(ta, v[0]);
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          ld_wait(v[c & 1]);
+          if (c < 7) tmem_ld16(ta + ((c + 1) >> 2) * 128 + ((c + 1) & 3) * 16, v[(c + 1) & 1]);
+          if (c == 7) {  // this buffer has been read: the tensor core may overwrite it
+            fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(tempty(b));
+          }
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            uint64_t& a = acc[c >> 2][(c & 3) * 8 + i];
+            a = fma2(pack2(v[c & 1][2 * i], v[c & 1][2 * i + 1]), sc[c >> 2], a);
+          }
+        }
+      }
+      if (!ok) break;
+      if (!p.act) {
+        store_bf16_64(p, row, tn * BN + wg * 64, acc[0]);
+        store_bf16_64(p, row, tn * BN + 128 + wg * 64, acc[1]);
+      } else {
+        // the sums stay fp32 up to the 8-bit rounding
+        const int f0 = tn * 128 + wg * 64;
+        float h[64];
+        uint32_t m = 0;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          const float2 g = unpack2(acc[0][i]), u = unpack2(acc[1][i]);
+          h[2 * i] = f0 + 2 * i < p.features ? silu_f(g.x) * u.x : 0.f;
+          h[2 * i + 1] = f0 + 2 * i + 1 < p.features ? silu_f(g.y) * u.y : 0.f;
+          m = max(m, max(__float_as_uint(h[2 * i]) & 0x7fffffffu, __float_as_uint(h[2 * i + 1]) & 0x7fffffffu));
+        }
+        // the other half of the group of 128 belongs to the other warpgroup's thread of this token;
+        // two buffers: a warp may be one tile ahead of the reader of the one before
+        uint32_t* am = amax + tile_parity * 2 * BM + q4 * 32 + lane;
+        am[wg * BM] = m;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(amax_bar);
+        ok = mbar_wait(amax_bar, tile_parity, abort_flag, &g_fp8_error, 505);
+        ok = __all_sync(FULL_MASK, ok);
+        if (!ok) break;
+        const Fp8Scale sc = fp8_scale(max(m, am[(wg ^ 1) * BM]));
+        if (row < p.T) {
+          uint8_t* dst = static_cast<uint8_t*>(p.out) + (int64_t)row * p.ldo + f0;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            if (f0 + 16 * i < p.features) {
+              const uint2 a = f32x8_to_e4m3(h + 16 * i, sc.inv), b2 = f32x8_to_e4m3(h + 16 * i + 8, sc.inv);
+              *reinterpret_cast<uint4*>(dst + 16 * i) = make_uint4(a.x, a.y, b2.x, b2.y);
+            }
+          }
+          if (wg == 0) p.os[(int64_t)tn * p.ldos + row] = sc.scale;
+        }
+      }
+    }
+  }
+  __syncwarp();
+  fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+PFN_cuTensorMapEncodeTiled_v12000 get_encode() {
+  static std::atomic<PFN_cuTensorMapEncodeTiled_v12000> cached{nullptr};
+  auto fn = cached.load(std::memory_order_acquire);
+  if (!fn) {
+    cudaDriverEntryPointQueryResult q;
+    void* p = nullptr;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess) {
+      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+      cached.store(fn, std::memory_order_release);
+    }
+  }
+  return fn;
+}
+
+// e4m3 [rows, k] with row stride ld; boxes of 128 channels x box_rows, 128-byte swizzle; elements
+// outside are read as zero.
+bool make_map(CUtensorMap* m, const void* base, int rows, int k, int64_t ld, int box_rows) {
+  auto enc = get_encode();
+  if (!enc) return false;
+  cuuint64_t dims[2] = {(cuuint64_t)k, (cuuint64_t)rows};
+  cuuint64_t strides[1] = {(cuuint64_t)ld};
+  cuuint32_t box[2] = {(cuuint32_t)BK, (cuuint32_t)box_rows};
+  cuuint32_t estr[2] = {1, 1};
+  return enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
+             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+}  // namespace
+
+cudaError_t gemm_fp8(const Fp8Gemm& g, int num_sms, cudaStream_t stream) {
+  if (g.T == 0 || g.N == 0) return cudaSuccess;
+  CUtensorMap mx, mw;
+  if (!make_map(&mx, g.xq, g.T, g.K, g.ldx, BM) || !make_map(&mw, g.wq, g.N, g.K, g.ldw, BN))
+    return cudaErrorInvalidValue;
+  Params p;
+  p.xs = g.xs;
+  p.ws = g.ws;
+  p.ldxs = g.ldxs;
+  p.ldws = g.ldws;
+  p.T = g.T;
+  p.N = g.N;
+  p.num_kb = (g.K + BK - 1) / BK;
+  p.nb = (g.N + FP8_GROUP - 1) / FP8_GROUP;
+  p.tiles_m = (g.T + BM - 1) / BM;
+  p.tiles_n = (g.N + BN - 1) / BN;
+  p.group = 16;
+  p.act = g.act;
+  p.features = g.features;
+  p.out = g.out;
+  p.ldo = g.ldo;
+  p.os = g.os;
+  p.ldos = g.ldos;
+  p.vec = g.ldo % 8 == 0 && (reinterpret_cast<uintptr_t>(g.out) & 15) == 0;
+  const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n;
+  if (tiles > 0x7fffffff - 65536) return cudaErrorInvalidValue;
+  static std::atomic<uint64_t> done{0};
+  cudaError_t e = smem_opt_in(done, gemm_fp8_tokens_kernel, SMEM_TOKENS);
+  if (e != cudaSuccess) return e;
+  const int grid = tiles < num_sms ? (int)tiles : num_sms;
+  return launch_pdl(gemm_fp8_tokens_kernel, dim3(grid), dim3(THREADS), SMEM_TOKENS, stream, mx, mw, p);
+}
+
+int gemm_fp8_error_code(int reset) {
+  int v = 0;
+  cudaMemcpyFromSymbol(&v, g_fp8_error, sizeof(int));
+  if (reset) {
+    int z = 0;
+    cudaMemcpyToSymbol(g_fp8_error, &z, sizeof(int));
+  }
+  return v;
+}
+
+}  // namespace nvb

@@ -63,6 +63,20 @@ class TorchOps:
         """silu(gate) * up of x @ w^T, w in the interleaved gate/up layout."""
         return R.silu_mul_interleaved(R.linear(x, w_gate_up)).to(x.dtype)
 
+    def quant_fp8(self, x):
+        return R.quant_fp8(x)
+
+    def add_rmsnorm_fp8(self, x, residual, w, eps):
+        r = x if residual is None else residual.copy_((x.float() + residual.float()).to(x.dtype))
+        return R.quant_fp8(R.rmsnorm(r.float(), w, eps)), r
+
+    def linear_fp8(self, x, w, out=None, dtype=torch.bfloat16):
+        y = R.linear_fp8(x, w)
+        return y.to(dtype) if out is None else out.copy_(y)
+
+    def linear_silu_fp8(self, x, w, features=None):
+        return R.linear_silu_fp8(x, w, w[0].shape[0] // 2 if features is None else features)
+
     def sample(self, logits, temperatures, top_p=None, seeds=None, step=0, batch_greedy_compat=False,
                generator=None, use_top_p=True, col_offset=0):
         return R.sample(logits, temperatures, top_p, generator, batch_greedy_compat).to(torch.int32)

@@ -108,6 +108,37 @@ class CudaOps:
         self.launches += 1
         return out
 
+    # ------------------------------------------------- fp8 weights and activations
+    # An 8-bit activation is a pair (q, s): q [T, K] e4m3 and one fp32 scale per token and 128 channels,
+    # s [T, ceil(K / 128)], stored token-contiguous (strides (1, a multiple of 4)).  An 8-bit weight is
+    # a pair (q [N, K], s [ceil(N / 128), ceil(K / 128)]): ``torch_ref.quant_fp8_weight``.  K is a
+    # multiple of 16.  The kernels keep no workspace, so calls on different streams and replays of
+    # different graphs do not meet.
+    def quant_fp8(self, x):
+        """(q, s) of x [T, K] bf16 (any row stride that is a multiple of 8)."""
+        self.launches += 1
+        return self.C.quant_fp8(x)
+
+    def add_rmsnorm_fp8(self, x, residual, w, eps):
+        """((q, s) of rmsnorm(x + residual) * w, the residual, updated in place) - or, without a
+        residual, of rmsnorm(x) * w, and x."""
+        self.launches += 1
+        return self.C.add_rmsnorm_fp8(x, residual, w, float(eps)), x if residual is None else residual
+
+    def linear_fp8(self, x, w, out=None, dtype=torch.bfloat16):
+        """bf16 [T, N] of x @ w^T for 8-bit x and w."""
+        if dtype != torch.bfloat16:
+            raise ValueError(f"linear_fp8 returns bfloat16, not {dtype}")
+        self.launches += 1
+        return self.C.linear_fp8(x[0], x[1], w[0], w[1], out)
+
+    def linear_silu_fp8(self, x, w, features=None):
+        """(q, s) of silu(gate) * up, [T, features], for 8-bit x and a gate/up weight in the layout of
+        ``torch_ref.group_gate_up`` (features: the layout's rows / 2 unless given)."""
+        self.launches += 1
+        return self.C.linear_silu_fp8(x[0], x[1], w[0], w[1],
+                                      w[0].shape[0] // 2 if features is None else features)
+
     def _plan(self, m, n, k):
         key = (m, n, k)
         p = self._plans.get(key)

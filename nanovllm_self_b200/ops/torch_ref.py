@@ -163,6 +163,82 @@ def linear(x: torch.Tensor, w: torch.Tensor) -> torch.Tensor:
     return F.linear(x, w)
 
 
+FP8_GROUP = 128        # channels of one activation scale; side of one weight scale's block
+FP8_AMAX_MIN = 1e-30
+
+
+def _fp8_scale(a: torch.Tensor):
+    """(scale, its inverse) of groups with largest magnitude ``a`` (fp32)."""
+    a = a.clamp(min=FP8_AMAX_MIN)
+    m = torch.full_like(a, FP8_MAX)  # a tensor: IEEE divisions, no multiplication by a reciprocal
+    return a / m, m / a
+
+
+def quant_fp8(x: torch.Tensor):
+    """x [T, K] -> (q [T, K] e4m3, s [T, ceil(K / 128)] fp32), x ~ q * s per group of 128 channels:
+    s = max |x| / 448 (at least 1e-30 / 448), q = e4m3(x * (448 / max |x|)), saturating."""
+    t, k = x.shape
+    kb = -(-k // FP8_GROUP)
+    p = x.new_zeros(t, kb * FP8_GROUP, dtype=torch.float32)
+    p[:, :k] = x
+    p = p.view(t, kb, FP8_GROUP)
+    s, inv = _fp8_scale(p.abs().amax(-1))
+    q = torch.clamp(p * inv[..., None], -FP8_MAX, FP8_MAX).to(torch.float8_e4m3fn)
+    return q.view(t, kb * FP8_GROUP)[:, :k].contiguous(), s
+
+
+def dequant_fp8(q: torch.Tensor, s: torch.Tensor, dtype=torch.float32) -> torch.Tensor:
+    return q.to(dtype) * s.to(dtype).repeat_interleave(FP8_GROUP, 1)[:, :q.shape[1]]
+
+
+def quant_fp8_weight(w: torch.Tensor):
+    """w [N, K] -> (q [N, K] e4m3, s [ceil(N / 128), ceil(K / 128)] fp32): one scale per block of
+    128 x 128, by the rule of :func:`quant_fp8`."""
+    n, k = w.shape
+    g = FP8_GROUP
+    nb, kb = -(-n // g), -(-k // g)
+    p = w.new_zeros(nb * g, kb * g, dtype=torch.float32)
+    p[:n, :k] = w
+    p = p.view(nb, g, kb, g)
+    s, inv = _fp8_scale(p.abs().amax(dim=(1, 3)))
+    q = torch.clamp(p * inv[:, None, :, None], -FP8_MAX, FP8_MAX).to(torch.float8_e4m3fn)
+    return q.view(nb * g, kb * g)[:n, :k].contiguous(), s
+
+
+def dequant_fp8_weight(q: torch.Tensor, s: torch.Tensor, dtype=torch.float32) -> torch.Tensor:
+    g = FP8_GROUP
+    s = s.to(dtype).repeat_interleave(g, 0)[:q.shape[0]].repeat_interleave(g, 1)[:, :q.shape[1]]
+    return q.to(dtype) * s
+
+
+def group_gate_up(g: torch.Tensor, u: torch.Tensor) -> torch.Tensor:
+    """[I, H] gate and up weights -> [2 * 128 * ceil(I / 128), H]: blocks of 128 gate rows and the
+    128 matching up rows in turn, the last pair of blocks filled up with zero rows.  No block of
+    128 x 128 then mixes gate and up rows, and 256 output columns are one group of 128 of
+    silu(gate) * up."""
+    i, h = g.shape
+    b = -(-i // FP8_GROUP)
+    out = g.new_zeros(b, 2, FP8_GROUP, h)
+    for j, x in enumerate((g, u)):
+        p = g.new_zeros(b * FP8_GROUP, h)
+        p[:i] = x
+        out[:, j] = p.view(b, FP8_GROUP, h)
+    return out.view(2 * b * FP8_GROUP, h)
+
+
+def linear_fp8(x, w) -> torch.Tensor:
+    """x and w as (values, scales) -> fp32 x @ w^T."""
+    return F.linear(dequant_fp8(*x), dequant_fp8_weight(*w))
+
+
+def linear_silu_fp8(x, w, features: int):
+    """silu(gate) * up of x @ w^T, quantised; w in the layout of :func:`group_gate_up`."""
+    y = linear_fp8(x, w)
+    y = y.view(y.shape[0], -1, 2, FP8_GROUP)
+    h = (F.silu(y[:, :, 0]) * y[:, :, 1]).reshape(y.shape[0], -1)
+    return quant_fp8(h[:, :features])
+
+
 def embedding(ids: torch.Tensor, w: torch.Tensor, vocab_start: int = 0) -> torch.Tensor:
     """Rows of the (possibly vocab-sharded) table; ids outside the shard give zeros."""
     local = ids.long() - vocab_start

@@ -15,7 +15,7 @@ CSRC = os.path.join(ROOT, "csrc")
 SOURCES = [
     "bindings.cpp", "gemm_bind.cpp", "comm_bind.cpp",
     "norm_act.cu", "qkv_rope_kv.cu", "attention.cu", "sampling.cu", "gemm_tcgen05.cu", "comm.cu",
-    "attn_decode_noalloc.cu",
+    "attn_decode_noalloc.cu", "fp8_bind.cpp", "fp8_quant.cu", "gemm_fp8.cu",
 ]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
