@@ -36,7 +36,16 @@ struct Fp8Gemm {
   float* os;
   int64_t ldos;
 };
-cudaError_t gemm_fp8(const Fp8Gemm& g, int num_sms, cudaStream_t stream);
+
+// Which kernel computes a product, and in which shape.  np = 0: the kernel with the tokens on the
+// MMA's M side (any T).  np = 16, 32, 64, 128: the weights on the M side, np >= T tokens, mw = 1 or 2
+// tiles of 128 weight rows per CTA (2 with act), K split over clusters of `splits` (1 .. 8) CTAs.
+struct Fp8Plan {
+  int np = 0, mw = 0, splits = 1;
+};
+// The plan of a product, from its sizes alone (the same in every process and every call).
+Fp8Plan fp8_plan(int T, int N, int K, int act, int num_sms);
+cudaError_t gemm_fp8(const Fp8Gemm& g, const Fp8Plan& plan, int num_sms, cudaStream_t stream);
 
 // Error word written by an fp8 GEMM that gave up on a bounded wait (0 = none).
 int gemm_fp8_error_code(int reset);

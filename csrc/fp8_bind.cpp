@@ -116,10 +116,26 @@ nvb::Fp8Gemm gemm_args(const at::Tensor& xq, const at::Tensor& xs, const at::Ten
   return a;
 }
 
+// plan: empty (chosen from the sizes) or (np, mw, splits), see Fp8Plan.
+nvb::Fp8Plan plan_of(const nvb::Fp8Gemm& a, const std::vector<int64_t>& plan, int num_sms) {
+  if (plan.empty()) return nvb::fp8_plan(a.T, a.N, a.K, a.act, num_sms);
+  TORCH_CHECK(plan.size() == 3, "plan: (np, mw, splits)");
+  nvb::Fp8Plan p;
+  p.np = (int)plan[0];
+  p.mw = (int)plan[1];
+  p.splits = (int)plan[2];
+  return p;
+}
+
+std::vector<int64_t> fp8_plan(int64_t T, int64_t N, int64_t K, int64_t act, int64_t num_sms) {
+  const auto p = nvb::fp8_plan((int)T, (int)N, (int)K, (int)act, (int)num_sms);
+  return {p.np, p.mw, p.splits};
+}
+
 int sms() { return at::cuda::getCurrentDeviceProperties()->multiProcessorCount; }
 
 at::Tensor linear_fp8(const at::Tensor& xq, const at::Tensor& xs, const at::Tensor& wq, const at::Tensor& ws,
-                      const c10::optional<at::Tensor>& out) {
+                      const c10::optional<at::Tensor>& out, const std::vector<int64_t>& plan) {
   nvb::Fp8Gemm a = gemm_args(xq, xs, wq, ws, "linear_fp8");
   if (out.has_value()) {
     const at::Tensor& y = *out;
@@ -132,12 +148,12 @@ at::Tensor linear_fp8(const at::Tensor& xq, const at::Tensor& xs, const at::Tens
   at::Tensor y = out.has_value() ? *out : at::empty({a.T, a.N}, xq.options().dtype(at::kBFloat16));
   a.out = y.data_ptr();
   a.ldo = row_stride(y);
-  ok(nvb::gemm_fp8(a, sms(), stream()), "linear_fp8");
+  ok(nvb::gemm_fp8(a, plan_of(a, plan, sms()), sms(), stream()), "linear_fp8");
   return y;
 }
 
 Pair linear_silu_fp8(const at::Tensor& xq, const at::Tensor& xs, const at::Tensor& wq, const at::Tensor& ws,
-                     int64_t features) {
+                     int64_t features, const std::vector<int64_t>& plan) {
   nvb::Fp8Gemm a = gemm_args(xq, xs, wq, ws, "linear_silu_fp8");
   TORCH_CHECK(features > 0 && features % 16 == 0 && wq.size(0) == 2 * nvb::FP8_GROUP * groups(features),
               "linear_silu_fp8: features must be a positive multiple of 16 and w must hold 2 x ceil(features / 128) "
@@ -151,7 +167,7 @@ Pair linear_silu_fp8(const at::Tensor& xq, const at::Tensor& xs, const at::Tenso
   a.ldo = features;
   a.os = s.data_ptr<float>();
   a.ldos = s.stride(1);
-  ok(nvb::gemm_fp8(a, sms(), stream()), "linear_silu_fp8");
+  ok(nvb::gemm_fp8(a, plan_of(a, plan, sms()), sms(), stream()), "linear_silu_fp8");
   return {q, s};
 }
 
@@ -162,7 +178,10 @@ int64_t fp8_error(bool reset) { return nvb::gemm_fp8_error_code(reset ? 1 : 0); 
 void register_fp8(pybind11::module& m) {
   m.def("quant_fp8", &quant_fp8);
   m.def("add_rmsnorm_fp8", &add_rmsnorm_fp8);
-  m.def("linear_fp8", &linear_fp8);
-  m.def("linear_silu_fp8", &linear_silu_fp8);
+  m.def("linear_fp8", &linear_fp8, pybind11::arg("xq"), pybind11::arg("xs"), pybind11::arg("wq"), pybind11::arg("ws"),
+        pybind11::arg("out") = c10::nullopt, pybind11::arg("plan") = std::vector<int64_t>{});
+  m.def("linear_silu_fp8", &linear_silu_fp8, pybind11::arg("xq"), pybind11::arg("xs"), pybind11::arg("wq"),
+        pybind11::arg("ws"), pybind11::arg("features"), pybind11::arg("plan") = std::vector<int64_t>{});
+  m.def("fp8_plan", &fp8_plan);
   m.def("fp8_error", &fp8_error, pybind11::arg("reset") = false);
 }

@@ -17,7 +17,14 @@
 // gate / up pairs, so SiLU-and-mul needs no exchange and the tile is one whole group of 128 of the
 // 8-bit output.
 //
-// Every wait is bounded; on expiry the kernel records an error code, drains its copies, frees TMEM
+// gemm_fp8_weights_kernel: few tokens.  Tiles of 128 weight rows (MMA M) x NP tokens (MMA N), so a
+// step of one token moves 16 activation rows beside the weights instead of 128, and K split over the
+// CTAs of a cluster so that the weights of a small layer are streamed by the whole GPU.  A thread
+// owns one feature and all NP tokens; the K slices' fp32 sums meet in shared memory: every CTA stores
+// the sums of token c straight into CTA c mod splits (distributed shared memory), which adds them in
+// the order of the slices (the result does not depend on timing), finishes and stores the token.
+//
+// Neither kernel uses a global workspace.  Every wait is bounded; on expiry the kernel records an error code, drains its copies, frees TMEM
 // and returns.
 #include <cuda.h>
 #include <cudaTypedefs.h>
@@ -42,7 +49,38 @@ constexpr int THREADS = 320;            // TMA warp, MMA warp, 8 epilogue warps
 constexpr int EPI_THREADS = 256;
 constexpr int SMEM_TOKENS = 1024 + STAGES * STAGE_BYTES + 2 * 2 * BM * 4 + 8 * (2 * STAGES + 6) + 16;
 
+// Shape of one launch of gemm_fp8_weights_kernel<NP, MW>: NP tokens, MW tiles of 128 weight rows per
+// CTA (2 for SiLU-and-mul: the gate block and the up block of the same features).
+template <int NP, int MW>
+struct WeightsCfg {
+  static constexpr int THREADS = 64 + 128 * MW;
+  static constexpr int MIN_CTAS = MW == 1 && NP <= 64 ? 2 : 1; // CTAs per SM
+  static constexpr int ACC_BUFS = MW * NP <= 64 ? 4 : 2;       // TMEM buffers
+  static constexpr int TMEM_COLS = ACC_BUFS * MW * NP;         // 64 .. 512
+  static constexpr int W_BYTES = MW * 128 * BK, X_BYTES = NP * BK, STAGE = W_BYTES + X_BYTES;
+  // fp32 sums of the tokens this CTA finishes: splits x ceil(NP / splits) <= NP + 7 rows
+  static constexpr int EXCHANGE = (NP + 8) * MW * 128 * 4;
+  static constexpr bool OVER_RING = MW * NP > 128;             // too large to lie beside the ring
+  static constexpr int SLOT = NP * 4 < 128 ? 128 : NP * 4;     // activation scales of one k-block
+  static constexpr int BUDGET = MIN_CTAS == 2 ? 113 * 1024 : 226 * 1024;
+  // one slot more than stages and buffers together: see the producer
+  static constexpr int stages() {
+    int s = 8;
+    while (s > 2 && smem(s) > BUDGET) --s;
+    return s;
+  }
+  static constexpr int smem(int s) {
+    return 1024 + (OVER_RING ? (s * STAGE > EXCHANGE ? s * STAGE : EXCHANGE) : s * STAGE + EXCHANGE) + (s + ACC_BUFS + 1) * SLOT + bar_bytes(s);
+  }
+  static constexpr int bar_bytes(int s) { return 8 * (3 * s + 3 * ACC_BUFS + 2) + 16; }
+  static constexpr int STAGES = stages();
+  static constexpr int BAR_BYTES = bar_bytes(STAGES);
+  static constexpr int SLOTS = STAGES + ACC_BUFS + 1;
+  static constexpr int SMEM = smem(STAGES);
+};
+
 struct Params {
+  int splits, kb_per_split;  // weights kernel
   const float* xs;
   const float* ws;
   int64_t ldxs, ldws;
@@ -289,6 +327,253 @@ __global__ void __launch_bounds__(THREADS, 1)
   }
 }
 
+template <int NP, int MW>
+__global__ void __launch_bounds__(WeightsCfg<NP, MW>::THREADS, WeightsCfg<NP, MW>::MIN_CTAS)
+    gemm_fp8_weights_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
+                            const __grid_constant__ CUtensorMap map_s, Params p) {
+  using C = WeightsCfg<NP, MW>;
+  constexpr int S = C::STAGES, NB = C::ACC_BUFS, SL = C::SLOTS;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  // the same offset in every CTA of the cluster
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  float* exchange = reinterpret_cast<float*>(smem + (C::OVER_RING ? 0 : S * C::STAGE));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::SMEM - 1024 - C::BAR_BYTES);
+  uint8_t* slots = reinterpret_cast<uint8_t*>(bars) - SL * C::SLOT;
+  const uint32_t bar0 = smem_u32(bars);
+  auto full = [&](int s) { return bar0 + 8u * s; };
+  auto empty = [&](int s) { return bar0 + 8u * (S + s); };
+  auto tfull = [&](int b) { return bar0 + 8u * (2 * S + b); };
+  auto tempty = [&](int b) { return bar0 + 8u * (2 * S + NB + b); };
+  auto sfull = [&](int l) { return bar0 + 8u * (2 * S + 2 * NB + l); };
+  const uint32_t final_bar = bar0 + 8u * (2 * S + 2 * NB + SL);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + 2 * S + 2 * NB + SL + 1);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * S + 2 * NB + SL + 1) + 1;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = p.splits > 1 ? (int)cluster_rank() : 0;
+  const int tile = blockIdx.x / p.splits;
+  const int kb0 = rank * p.kb_per_split;
+  const int nkb = max(0, min(p.num_kb - kb0, p.kb_per_split));
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S; ++s) {
+      mbar_init(full(s), 1);
+      mbar_init(empty(s), 1);
+    }
+    for (int b = 0; b < NB; ++b) {
+      mbar_init(tfull(b), 1);
+      mbar_init(tempty(b), 4 * MW);
+    }
+    for (int l = 0; l < SL; ++l) mbar_init(sfull(l), 1);
+    mbar_init(final_bar, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 1) tmem_alloc(smem_u32(tmem_slot), C::TMEM_COLS);
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = *tmem_slot;
+  // this CTA's exchange area may be written: now, or once its ring is idle (waited on below)
+  if (!C::OVER_RING && p.splits > 1) cluster_arrive();
+  pdl_trigger();
+
+  if (warp == 0 && lane == 0) {
+    // ------------------------------------------------------------------ producer
+    prefetch_map(&map_w);
+    prefetch_map(&map_x);
+    prefetch_map(&map_s);
+    // Into L2 only, ahead of the previous kernel's end: whoever writes the weights writes there too
+    for (int i = 0; i < min(nkb, S); ++i) tma_prefetch_2d(&map_w, (kb0 + i) * BK, tile * MW * 128);
+    pdl_wait();
+    bool ok = true;
+    int i = 0;
+    for (; i < nkb; ++i) {
+      const int s = i % S, l = i % SL;
+      if (!mbar_wait(empty(s), ((i / S) & 1) ^ 1, abort_flag, &g_fp8_error, 511)) {
+        ok = false;
+        break;
+      }
+      const uint32_t st = smem_u32(smem + s * C::STAGE);
+      mbar_arrive_expect_tx(full(s), C::STAGE);
+      tma_load_2d(st, &map_w, full(s), (kb0 + i) * BK, tile * MW * 128);
+      tma_load_2d(st + C::W_BYTES, &map_x, full(s), (kb0 + i) * BK, 0);
+      // Slot l was last read for k-block i - SL.  Stage s is free, so k-block i - S has been
+      // multiplied, so the epilogue has emptied the buffer of k-block i - S - NB, and had by then
+      // read the scales of the one before, i - SL: no barrier of its own guards the slot.
+      mbar_arrive_expect_tx(sfull(l), NP * 4);
+      tma_load_2d(smem_u32(slots + l * C::SLOT), &map_s, sfull(l), 0, kb0 + i);
+    }
+    if (!ok) {
+      for (int j = max(0, i - S); j < i; ++j) {
+        mbar_drain(full(j % S), (j / S) & 1);
+        mbar_drain(sfull(j % SL), (j / SL) & 1);
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------------ MMA issuer
+    const uint32_t tbase = __shfl_sync(FULL_MASK, tmem, 0);
+    for (int i = 0; i < nkb; ++i) {
+      const int s = i % S, b = i % NB;
+      int okw = 1;
+      if (lane == 0)
+        okw = mbar_wait(tempty(b), ((i / NB) & 1) ^ 1, abort_flag, &g_fp8_error, 512) &&
+              mbar_wait(full(s), (i / S) & 1, abort_flag, &g_fp8_error, 513);
+      if (!__shfl_sync(FULL_MASK, okw, 0)) break;
+      fence_after();
+      const uint32_t st = smem_u32(smem + s * C::STAGE);
+      const uint64_t xd = sdesc(st + C::W_BYTES);
+      if (elect_one()) {
+#pragma unroll
+        for (int w = 0; w < MW; ++w) {
+          const uint64_t wd = sdesc(st + w * 128 * BK);
+#pragma unroll
+          for (int k = 0; k < BK / 32; ++k)
+            mma_f8(tbase + (b * MW + w) * NP, wd + 2 * k, xd + 2 * k, idesc_f8(128, NP), k > 0 ? 1u : 0u);
+        }
+        commit(empty(s));
+        commit(tfull(b));
+      }
+      __syncwarp();
+    }
+    if (elect_one()) commit(final_bar);
+    if (lane == 0) mbar_drain(final_bar, 0);
+    __syncwarp();
+  } else if (warp >= 2) {
+    // ------------------------------------------------------------------ epilogue
+    const int q4 = warp & 3, w = (warp - 2) >> 2;  // lane quarter, weight tile
+    const float* ws = p.ws + (int64_t)min(tile * MW + w, p.nb - 1) * p.ldws + kb0;
+    uint64_t acc[NP / 2];
+#pragma unroll
+    for (int i = 0; i < NP / 2; ++i) acc[i] = 0;
+    pdl_wait();
+    float w_n = nkb > 0 ? ws[0] : 0.f;
+    bool ok = true;
+    for (int i = 0; i < nkb; ++i) {
+      const uint64_t wsc = pack2(w_n, w_n);
+      if (i + 1 < nkb) w_n = ws[i + 1];
+      const int b = i % NB, l = i % SL;
+      ok = mbar_wait(sfull(l), (i / SL) & 1, abort_flag, &g_fp8_error, 514) &&
+           mbar_wait(tfull(b), (i / NB) & 1, abort_flag, &g_fp8_error, 515);
+      ok = __all_sync(FULL_MASK, ok);  // the warp stays together
+      if (!ok) break;
+      fence_after();
+      const uint32_t ta = tmem + ((uint32_t)(q4 * 32) << 16) + (b * MW + w) * NP;
+      const ulonglong2* xs = reinterpret_cast<const ulonglong2*>(slots + l * C::SLOT);
+      uint32_t v[2][16];
+      tmem_ld16(ta, v[0]);
+#pragma unroll
+      for (int c = 0; c < NP / 16; ++c) {
+        ld_wait(v[c & 1]);
+        if (c + 1 < NP / 16) {
+          tmem_ld16(ta + (c + 1) * 16, v[(c + 1) & 1]);
+        } else {  // this buffer has been read: the tensor core may overwrite it
+          fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(tempty(b));
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const ulonglong2 sx = xs[c * 4 + j];  // 4 tokens' scales, the same for every lane
+          uint64_t& a0 = acc[c * 8 + 2 * j];
+          uint64_t& a1 = acc[c * 8 + 2 * j + 1];
+          a0 = fma2(pack2(v[c & 1][4 * j], v[c & 1][4 * j + 1]), mul2(sx.x, wsc), a0);
+          a1 = fma2(pack2(v[c & 1][4 * j + 2], v[c & 1][4 * j + 3]), mul2(sx.y, wsc), a1);
+        }
+      }
+    }
+    // sums of token c to CTA c mod splits: [slice][c / splits][feature]
+    if (p.splits > 1) {
+      if (C::OVER_RING) cluster_arrive();  // the last MMA has completed: nothing reads the ring any more
+      cluster_wait();
+    }
+    const int f = w * 128 + q4 * 32 + lane;
+    const int per = (NP + p.splits - 1) / p.splits;
+    int owner = 0, tl = 0;
+    if (p.splits == 1) {
+#pragma unroll
+      for (int c = 0; c < NP; ++c)
+        if (c < p.T) {
+          const float2 a = unpack2(acc[c / 2]);
+          exchange[c * MW * 128 + f] = c & 1 ? a.y : a.x;
+        }
+    } else {
+#pragma unroll
+      for (int c = 0; c < NP; ++c)
+        if (c < p.T) {
+          const float2 a = unpack2(acc[c / 2]);
+          st_cluster_f32(cluster_map(smem_u32(exchange + (rank * per + tl) * MW * 128 + f), owner), c & 1 ? a.y : a.x);
+          if (++owner == p.splits) {
+            owner = 0;
+            ++tl;
+          }
+        }
+    }
+  }
+  __syncwarp();
+  fence_before();
+  if (p.splits > 1) {
+    if (warp < 2) {
+      if (C::OVER_RING) cluster_arrive();
+      cluster_wait();
+    }
+    cluster_arrive();
+    cluster_wait();  // every slice's sums have arrived
+  } else {
+    __syncthreads();
+  }
+  if (warp >= 2 && !*abort_flag) {
+    const int per = (NP + p.splits - 1) / p.splits;
+    const int mine = (p.T - rank + p.splits - 1) / p.splits;  // tokens rank, rank + splits, ...
+    const int wi = warp - 2;
+    if (!p.act) {
+      for (int it = wi; it < mine * MW; it += 4 * MW) {
+        const int tl = it / MW, blk = it % MW;
+        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int r = 0; r < p.splits; ++r) {
+          const float4 v = *reinterpret_cast<const float4*>(exchange + (r * per + tl) * MW * 128 + blk * 128 + lane * 4);
+          a.x += v.x; a.y += v.y; a.z += v.z; a.w += v.w;
+        }
+        const int n = (tile * MW + blk) * 128 + lane * 4;
+        __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(p.out) + (int64_t)(rank + tl * p.splits) * p.ldo + n;
+        const float o[4] = {a.x, a.y, a.z, a.w};
+        if (p.vec && n + 4 <= p.N) {
+          *reinterpret_cast<uint2*>(dst) = f32_to_bf16x4(o);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (n + e < p.N) dst[e] = __float2bfloat16_rn(o[e]);
+        }
+      }
+    } else if constexpr (MW == 2) {
+      for (int tl = wi; tl < mine; tl += 4 * MW) {
+        float4 g = make_float4(0.f, 0.f, 0.f, 0.f), u = g;
+        for (int r = 0; r < p.splits; ++r) {
+          const float4* row = reinterpret_cast<const float4*>(exchange + (r * per + tl) * 256);
+          const float4 a = row[lane], b = row[32 + lane];
+          g.x += a.x; g.y += a.y; g.z += a.z; g.w += a.w;
+          u.x += b.x; u.y += b.y; u.z += b.z; u.w += b.w;
+        }
+        const int f = tile * 128 + lane * 4;
+        const bool in = f < p.features;
+        const float h[4] = {in ? silu_f(g.x) * u.x : 0.f, in ? silu_f(g.y) * u.y : 0.f, in ? silu_f(g.z) * u.z : 0.f,
+                            in ? silu_f(g.w) * u.w : 0.f};
+        uint32_t m = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) m = max(m, __float_as_uint(h[e]) & 0x7fffffffu);
+        const Fp8Scale sc = fp8_scale(__reduce_max_sync(FULL_MASK, m));
+        const int t = rank + tl * p.splits;
+        const float o[4] = {h[0] * sc.inv, h[1] * sc.inv, h[2] * sc.inv, h[3] * sc.inv};
+        if (in) *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(p.out) + (int64_t)t * p.ldo + f) = f32x4_to_e4m3(o);
+        if (lane == 0) p.os[(int64_t)tile * p.ldos + t] = sc.scale;
+      }
+    }
+  }
+  if (warp == 1) {
+    fence_after();
+    tmem_dealloc(tmem, C::TMEM_COLS);
+  }
+}
+
 PFN_cuTensorMapEncodeTiled_v12000 get_encode() {
   static std::atomic<PFN_cuTensorMapEncodeTiled_v12000> cached{nullptr};
   auto fn = cached.load(std::memory_order_acquire);
@@ -318,14 +603,84 @@ bool make_map(CUtensorMap* m, const void* base, int rows, int k, int64_t ld, int
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// fp32 scales [blocks][tokens] with row stride ld; boxes of one block's scales of `box` tokens.
+bool make_scale_map(CUtensorMap* m, const float* base, int blocks, int tokens, int64_t ld, int box) {
+  auto enc = get_encode();
+  if (!enc) return false;
+  cuuint64_t dims[2] = {(cuuint64_t)tokens, (cuuint64_t)blocks};
+  cuuint64_t strides[1] = {(cuuint64_t)ld * 4};
+  cuuint32_t boxd[2] = {(cuuint32_t)box, 1};
+  cuuint32_t estr[2] = {1, 1};
+  return enc(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, const_cast<float*>(base), dims, strides, boxd, estr,
+             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int NP, int MW>
+cudaError_t run_weights(const Fp8Gemm& g, Params p, int splits, cudaStream_t stream) {
+  using C = WeightsCfg<NP, MW>;
+  if (splits < 1 || splits > 8 || g.T > NP || (g.act && MW != 2)) return cudaErrorInvalidValue;
+  CUtensorMap mx, mw, ms;
+  if (!make_map(&mx, g.xq, g.T, g.K, g.ldx, NP) || !make_map(&mw, g.wq, g.N, g.K, g.ldw, 128 * MW) ||
+      !make_scale_map(&ms, g.xs, p.num_kb, g.T, g.ldxs, NP))
+    return cudaErrorInvalidValue;
+  p.splits = splits;
+  p.kb_per_split = (p.num_kb + splits - 1) / splits;
+  auto kern = gemm_fp8_weights_kernel<NP, MW>;
+  static std::atomic<uint64_t> done{0};
+  cudaError_t e = smem_opt_in(done, kern, C::SMEM);
+  if (e != cudaSuccess) return e;
+  const int tiles = (g.N + 128 * MW - 1) / (128 * MW);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(tiles * splits);
+  cfg.blockDim = dim3(C::THREADS);
+  cfg.dynamicSmemBytes = C::SMEM;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = splits;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = splits > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kern, mx, mw, ms, p);
+}
+
+cudaError_t run_weights(const Fp8Gemm& g, const Params& p, const Fp8Plan& pl, cudaStream_t stream) {
+  switch (pl.np * 4 + pl.mw) {
+    case 16 * 4 + 1: return run_weights<16, 1>(g, p, pl.splits, stream);
+    case 32 * 4 + 1: return run_weights<32, 1>(g, p, pl.splits, stream);
+    case 64 * 4 + 1: return run_weights<64, 1>(g, p, pl.splits, stream);
+    case 128 * 4 + 1: return run_weights<128, 1>(g, p, pl.splits, stream);
+    case 16 * 4 + 2: return run_weights<16, 2>(g, p, pl.splits, stream);
+    case 32 * 4 + 2: return run_weights<32, 2>(g, p, pl.splits, stream);
+    case 64 * 4 + 2: return run_weights<64, 2>(g, p, pl.splits, stream);
+    case 128 * 4 + 2: return run_weights<128, 2>(g, p, pl.splits, stream);
+  }
+  return cudaErrorInvalidValue;
+}
+
 }  // namespace
 
-cudaError_t gemm_fp8(const Fp8Gemm& g, int num_sms, cudaStream_t stream) {
+Fp8Plan fp8_plan(int T, int N, int K, int act, int num_sms) {
+  Fp8Plan pl;
+  if (T > 128) return pl;
+  pl.np = T <= 16 ? 16 : T <= 32 ? 32 : T <= 64 ? 64 : 128;
+  pl.mw = act ? 2 : 1;
+  const int tiles = (N + 128 * pl.mw - 1) / (128 * pl.mw);
+  const int num_kb = (K + BK - 1) / BK;
+  const int slots = num_sms * (pl.mw == 1 && pl.np <= 64 ? 2 : 1);
+  pl.splits = 1;
+  for (int s = 2; s <= 8; ++s)
+    if (tiles * s <= slots && num_kb / s >= 2) pl.splits = s;
+  return pl;
+}
+
+cudaError_t gemm_fp8(const Fp8Gemm& g, const Fp8Plan& pl, int num_sms, cudaStream_t stream) {
   if (g.T == 0 || g.N == 0) return cudaSuccess;
-  CUtensorMap mx, mw;
-  if (!make_map(&mx, g.xq, g.T, g.K, g.ldx, BM) || !make_map(&mw, g.wq, g.N, g.K, g.ldw, BN))
-    return cudaErrorInvalidValue;
-  Params p;
+  Params p{};
   p.xs = g.xs;
   p.ws = g.ws;
   p.ldxs = g.ldxs;
@@ -344,6 +699,10 @@ cudaError_t gemm_fp8(const Fp8Gemm& g, int num_sms, cudaStream_t stream) {
   p.os = g.os;
   p.ldos = g.ldos;
   p.vec = g.ldo % 8 == 0 && (reinterpret_cast<uintptr_t>(g.out) & 15) == 0;
+  if (pl.np) return run_weights(g, p, pl, stream);
+  CUtensorMap mx, mw;
+  if (!make_map(&mx, g.xq, g.T, g.K, g.ldx, BM) || !make_map(&mw, g.wq, g.N, g.K, g.ldw, BN))
+    return cudaErrorInvalidValue;
   const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n;
   if (tiles > 0x7fffffff - 65536) return cudaErrorInvalidValue;
   static std::atomic<uint64_t> done{0};

@@ -135,6 +135,28 @@ __device__ __forceinline__ void ld_wait(uint32_t (&r)[16]) {
                : "memory");
 }
 
+// Cluster barrier, split so that work fits between its halves.  Every thread of every CTA of the
+// cluster executes both.
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+
+// Address of a shared-memory location of this CTA in CTA `rank` of the cluster.
+__device__ __forceinline__ uint32_t cluster_map(uint32_t local_addr, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(local_addr), "r"(rank));
+  return r;
+}
+
+__device__ __forceinline__ void st_cluster_f32(uint32_t addr, float v) {
+  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
+}
+
 // Two fp32 values in one 64-bit register (fma.rn.f32x2: one instruction for two products).
 __device__ __forceinline__ uint64_t pack2(float a, float b) {
   uint64_t r;

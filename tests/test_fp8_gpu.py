@@ -180,6 +180,49 @@ def test_linear_silu(ops, t, i, k):
     assert ((q.double() * sc - h).abs() <= h.abs() * (2.0 ** -4 + 2 * wide) + 1.1 * err + sc * 2.0 ** -10 * (1 + wide)).all()
 
 
+def _plans(t, act):
+    for np_ in (16, 32, 64, 128):
+        if np_ >= t:
+            for mw in (2,) if act else (1, 2):
+                for splits in (1, 2, 3, 5, 8):
+                    yield [np_, mw, splits]
+    yield [0, 0, 1]
+
+
+@pytest.mark.parametrize("t,n,k", [(1, 384, 272), (13, 100, 1712), (32, 640, 1040), (50, 250, 512), (128, 900, 2064)])
+def test_every_kernel_variant(ops, t, n, k):
+    """The variants differ in the order of fp32 additions alone."""
+    C = ops.C
+    x, w = ops.quant_fp8(_acts(t, k)), _weight(n, k)
+    want = _exact(x, w)
+    tol = want.abs() * 2.0 ** -8 + 1.01 * (_acc(k) + 8 * U) * _bound(x, w)
+    for plan in _plans(t, False):
+        y = C.linear_fp8(*x, *w, None, plan)
+        assert ((y.double() - want).abs() <= tol).all(), plan
+    i = (n + 15) // 16 * 16
+    g = torch.Generator(device=DEV).manual_seed(3)
+    gu = [torch.randn(i, k, device=DEV, generator=g) / k ** 0.5 for _ in range(2)]
+    w = R.quant_fp8_weight(R.group_gate_up(*gu))
+    q0, s0 = C.linear_silu_fp8(*x, *w, i, [0, 0, 1])
+    d0 = R.dequant_fp8(q0, s0, torch.float64)
+    for plan in _plans(t, True):
+        q, s = C.linear_silu_fp8(*x, *w, i, plan)
+        # scales agree up to the sums' rounding, values up to a step of e4m3
+        assert ((s - s0).abs() <= 1e-3 * s0).all(), plan
+        step = d0.abs() * 2.0 ** -3 + s0.double().repeat_interleave(128, 1)[:, :i] * 2.0 ** -9
+        assert ((R.dequant_fp8(q, s, torch.float64) - d0).abs() <= 1.01 * step + 1e-3 * d0.abs()).all(), plan
+        assert (_bits(q) == _bits(q0)).float().mean() > 0.99, plan
+
+
+def test_plans_refused(ops):
+    x, w = ops.quant_fp8(_acts(20, 256)), _weight(256, 256)
+    for plan in ([16, 1, 1], [32, 1, 9], [32, 3, 1], [24, 1, 1], [32, 1, 0], [32, 1]):
+        with pytest.raises(RuntimeError):
+            ops.C.linear_fp8(*x, *w, None, plan)
+    with pytest.raises(RuntimeError):
+        ops.C.linear_silu_fp8(*x, *w, 128, [32, 1, 1])
+
+
 @pytest.mark.parametrize("t", [1, 20, 200])
 def test_linear_nan_and_zero_rows_stay_their_own(ops, t):
     k, n = 512, 384
