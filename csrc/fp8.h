@@ -38,10 +38,10 @@ struct Fp8Gemm {
 };
 
 // Which kernel computes a product, and in which shape.  np = 0: the kernel with the tokens on the
-// MMA's M side (any T).  np = 16, 32, 64, 128: the weights on the M side, np >= T tokens, mw = 1 or 2
-// tiles of 128 weight rows per CTA (2 with act), K split over clusters of `splits` (1 .. 8) CTAs.
+// MMA's M side (any T).  np = 16, 32, 64, 128: the weights on the M side, np >= T tokens, K split over
+// `splits` CTAs of a cluster (1 .. 8, with act 1 .. 4).
 struct Fp8Plan {
-  int np = 0, mw = 0, splits = 1;
+  int np = 0, splits = 1;
 };
 // The plan of a product, from its sizes alone (the same in every process and every call).
 Fp8Plan fp8_plan(int T, int N, int K, int act, int num_sms);

@@ -116,20 +116,19 @@ nvb::Fp8Gemm gemm_args(const at::Tensor& xq, const at::Tensor& xs, const at::Ten
   return a;
 }
 
-// plan: empty (chosen from the sizes) or (np, mw, splits), see Fp8Plan.
+// plan: empty (chosen from the sizes) or (np, splits), see Fp8Plan.
 nvb::Fp8Plan plan_of(const nvb::Fp8Gemm& a, const std::vector<int64_t>& plan, int num_sms) {
   if (plan.empty()) return nvb::fp8_plan(a.T, a.N, a.K, a.act, num_sms);
-  TORCH_CHECK(plan.size() == 3, "plan: (np, mw, splits)");
+  TORCH_CHECK(plan.size() == 2, "plan: (np, splits)");
   nvb::Fp8Plan p;
   p.np = (int)plan[0];
-  p.mw = (int)plan[1];
-  p.splits = (int)plan[2];
+  p.splits = (int)plan[1];
   return p;
 }
 
 std::vector<int64_t> fp8_plan(int64_t T, int64_t N, int64_t K, int64_t act, int64_t num_sms) {
   const auto p = nvb::fp8_plan((int)T, (int)N, (int)K, (int)act, (int)num_sms);
-  return {p.np, p.mw, p.splits};
+  return {p.np, p.splits};
 }
 
 int sms() { return at::cuda::getCurrentDeviceProperties()->multiProcessorCount; }

@@ -49,38 +49,46 @@ constexpr int THREADS = 320;            // TMA warp, MMA warp, 8 epilogue warps
 constexpr int EPI_THREADS = 256;
 constexpr int SMEM_TOKENS = 1024 + STAGES * STAGE_BYTES + 2 * 2 * BM * 4 + 8 * (2 * STAGES + 6) + 16;
 
-// Shape of one launch of gemm_fp8_weights_kernel<NP, MW>: NP tokens, MW tiles of 128 weight rows per
-// CTA (2 for SiLU-and-mul: the gate block and the up block of the same features).
-template <int NP, int MW>
+// Shape of gemm_fp8_weights_kernel<NP> (NP tokens, rounded up).  Two CTAs fit on an SM, so that one
+// streams while the other fills its pipeline or finishes, and so that the next kernel's CTAs start early.
+template <int NP>
 struct WeightsCfg {
-  static constexpr int THREADS = 64 + 128 * MW;
-  static constexpr int MIN_CTAS = MW == 1 && NP <= 64 ? 2 : 1; // CTAs per SM
-  static constexpr int ACC_BUFS = MW * NP <= 64 ? 4 : 2;       // TMEM buffers
-  static constexpr int TMEM_COLS = ACC_BUFS * MW * NP;         // 64 .. 512
-  static constexpr int W_BYTES = MW * 128 * BK, X_BYTES = NP * BK, STAGE = W_BYTES + X_BYTES;
-  // fp32 sums of the tokens this CTA finishes: splits x ceil(NP / splits) <= NP + 7 rows
-  static constexpr int EXCHANGE = (NP + 8) * MW * 128 * 4;
-  static constexpr bool OVER_RING = MW * NP > 128;             // too large to lie beside the ring
+  static constexpr int COL_SPLIT = NP >= 64 ? 2 : 1;           // warps that share a quarter of the lanes
+  static constexpr int NC = NP / COL_SPLIT;                    // tokens per epilogue thread
+  static constexpr int CHUNK = NC == 32 ? 32 : 16;             // TMEM columns per load
+  static constexpr int EPI_WARPS = 4 * COL_SPLIT;
+  static constexpr int THREADS = 64 + 32 * EPI_WARPS;
+  static constexpr int ACC_BUFS = NP <= 64 ? 4 : 2;            // TMEM buffers
+  static constexpr int TMEM_COLS = ACC_BUFS * NP;              // 64 .. 256
+  static constexpr int W_BYTES = 128 * BK, X_BYTES = NP * BK, STAGE = W_BYTES + X_BYTES;
+  // fp32 sums of the tokens this CTA finishes: in all at most NP + 7 rows of 128; beside the ring
+  // where that leaves it deep enough, over it otherwise
+  static constexpr int EXCHANGE = (NP + 8) * 128 * 4;
+  static constexpr bool OVER_RING = NP > 32;
   static constexpr int SLOT = NP * 4 < 128 ? 128 : NP * 4;     // activation scales of one k-block
-  static constexpr int BUDGET = MIN_CTAS == 2 ? 113 * 1024 : 226 * 1024;
+  static constexpr int BUDGET = 113 * 1024;
+  static constexpr int bar_bytes(int s) { return 8 * (3 * s + 3 * ACC_BUFS + 2) + 16; }
+  static constexpr int ring_bytes(int s) {
+    return OVER_RING ? (s * STAGE > EXCHANGE ? s * STAGE : EXCHANGE) : s * STAGE + EXCHANGE;
+  }
   // one slot more than stages and buffers together: see the producer
+  static constexpr int smem(int s) { return 1024 + ring_bytes(s) + (s + ACC_BUFS + 1) * SLOT + bar_bytes(s); }
   static constexpr int stages() {
     int s = 8;
     while (s > 2 && smem(s) > BUDGET) --s;
     return s;
   }
-  static constexpr int smem(int s) {
-    return 1024 + (OVER_RING ? (s * STAGE > EXCHANGE ? s * STAGE : EXCHANGE) : s * STAGE + EXCHANGE) + (s + ACC_BUFS + 1) * SLOT + bar_bytes(s);
-  }
-  static constexpr int bar_bytes(int s) { return 8 * (3 * s + 3 * ACC_BUFS + 2) + 16; }
   static constexpr int STAGES = stages();
-  static constexpr int BAR_BYTES = bar_bytes(STAGES);
   static constexpr int SLOTS = STAGES + ACC_BUFS + 1;
+  static constexpr int BAR_BYTES = bar_bytes(STAGES);
   static constexpr int SMEM = smem(STAGES);
+  static_assert(SMEM <= BUDGET, "two CTAs per SM");
 };
 
 struct Params {
-  int splits, kb_per_split;  // weights kernel
+  // weights kernel: K slices, their length, CTAs per cluster (slices x halves: with SiLU-and-mul two
+  // CTAs share 128 gate and 128 up rows)
+  int splits, kb_per_split, cluster;
   const float* xs;
   const float* ws;
   int64_t ldxs, ldws;
@@ -261,11 +269,11 @@ __global__ void __launch_bounds__(THREADS, 1)
         const uint32_t ta = tmem + ((uint32_t)(q4 * 32) << 16) + b * BN + wg * 64;
         // 8 chunks of 16 columns (4 of each half), the next one in flight while one is added
         uint32_t v[2][16];
-        tmem_ld16(ta, v[0]);
+        tmem_ld(ta, v[0]);
 #pragma unroll
         for (int c = 0; c < 8; ++c) {
           ld_wait(v[c & 1]);
-          if (c < 7) tmem_ld16(ta + ((c + 1) >> 2) * 128 + ((c + 1) & 3) * 16, v[(c + 1) & 1]);
+          if (c < 7) tmem_ld(ta + ((c + 1) >> 2) * 128 + ((c + 1) & 3) * 16, v[(c + 1) & 1]);
           if (c == 7) {  // this buffer has been read: the tensor core may overwrite it
             fence_before();
             __syncwarp();
@@ -327,11 +335,14 @@ __global__ void __launch_bounds__(THREADS, 1)
   }
 }
 
-template <int NP, int MW>
-__global__ void __launch_bounds__(WeightsCfg<NP, MW>::THREADS, WeightsCfg<NP, MW>::MIN_CTAS)
+// A CTA's tile is 128 weight rows.  Plain: rows [128 j, 128 j + 128).  SiLU-and-mul: half h of the
+// pair of blocks j: gate rows 64 h .. and the matching up rows, so that two CTAs of one cluster hold
+// a whole group of 128 of the output.
+template <int NP>
+__global__ void __launch_bounds__(WeightsCfg<NP>::THREADS, 2)
     gemm_fp8_weights_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
                             const __grid_constant__ CUtensorMap map_s, Params p) {
-  using C = WeightsCfg<NP, MW>;
+  using C = WeightsCfg<NP>;
   constexpr int S = C::STAGES, NB = C::ACC_BUFS, SL = C::SLOTS;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   // the same offset in every CTA of the cluster
@@ -349,9 +360,10 @@ __global__ void __launch_bounds__(WeightsCfg<NP, MW>::THREADS, WeightsCfg<NP, MW
   volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + 2 * S + 2 * NB + SL + 1);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * S + 2 * NB + SL + 1) + 1;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int rank = p.splits > 1 ? (int)cluster_rank() : 0;
-  const int tile = blockIdx.x / p.splits;
-  const int kb0 = rank * p.kb_per_split;
+  const int rank = p.cluster > 1 ? (int)cluster_rank() : 0;
+  const int tile = blockIdx.x / p.cluster;
+  const int half = p.act ? rank & 1 : 0, slice = p.act ? rank >> 1 : rank;
+  const int kb0 = slice * p.kb_per_split;
   const int nkb = max(0, min(p.num_kb - kb0, p.kb_per_split));
 
   if (threadIdx.x == 0) {
@@ -361,7 +373,7 @@ __global__ void __launch_bounds__(WeightsCfg<NP, MW>::THREADS, WeightsCfg<NP, MW
     }
     for (int b = 0; b < NB; ++b) {
       mbar_init(tfull(b), 1);
-      mbar_init(tempty(b), 4 * MW);
+      mbar_init(tempty(b), C::EPI_WARPS);
     }
     for (int l = 0; l < SL; ++l) mbar_init(sfull(l), 1);
     mbar_init(final_bar, 1);
@@ -374,16 +386,20 @@ __global__ void __launch_bounds__(WeightsCfg<NP, MW>::THREADS, WeightsCfg<NP, MW
   fence_after();
   const uint32_t tmem = *tmem_slot;
   // this CTA's exchange area may be written: now, or once its ring is idle (waited on below)
-  if (!C::OVER_RING && p.splits > 1) cluster_arrive();
+  if (!C::OVER_RING && p.cluster > 1) cluster_arrive();
   pdl_trigger();
 
   if (warp == 0 && lane == 0) {
     // ------------------------------------------------------------------ producer
+    const int row_a = p.act ? tile * 256 + half * 64 : tile * 128, row_b = row_a + (p.act ? 128 : 64);
     prefetch_map(&map_w);
     prefetch_map(&map_x);
     prefetch_map(&map_s);
     // Into L2 only, ahead of the previous kernel's end: whoever writes the weights writes there too
-    for (int i = 0; i < min(nkb, S); ++i) tma_prefetch_2d(&map_w, (kb0 + i) * BK, tile * MW * 128);
+    for (int i = 0; i < min(nkb, S); ++i) {
+      tma_prefetch_2d(&map_w, (kb0 + i) * BK, row_a);
+      tma_prefetch_2d(&map_w, (kb0 + i) * BK, row_b);
+    }
     pdl_wait();
     bool ok = true;
     int i = 0;
@@ -395,7 +411,8 @@ __global__ void __launch_bounds__(WeightsCfg<NP, MW>::THREADS, WeightsCfg<NP, MW
       }
       const uint32_t st = smem_u32(smem + s * C::STAGE);
       mbar_arrive_expect_tx(full(s), C::STAGE);
-      tma_load_2d(st, &map_w, full(s), (kb0 + i) * BK, tile * MW * 128);
+      tma_load_2d(st, &map_w, full(s), (kb0 + i) * BK, row_a);
+      tma_load_2d(st + 64 * BK, &map_w, full(s), (kb0 + i) * BK, row_b);
       tma_load_2d(st + C::W_BYTES, &map_x, full(s), (kb0 + i) * BK, 0);
       // Slot l was last read for k-block i - SL.  Stage s is free, so k-block i - S has been
       // multiplied, so the epilogue has emptied the buffer of k-block i - S - NB, and had by then
@@ -421,15 +438,11 @@ __global__ void __launch_bounds__(WeightsCfg<NP, MW>::THREADS, WeightsCfg<NP, MW
       if (!__shfl_sync(FULL_MASK, okw, 0)) break;
       fence_after();
       const uint32_t st = smem_u32(smem + s * C::STAGE);
-      const uint64_t xd = sdesc(st + C::W_BYTES);
+      const uint64_t wd = sdesc(st), xd = sdesc(st + C::W_BYTES);
       if (elect_one()) {
 #pragma unroll
-        for (int w = 0; w < MW; ++w) {
-          const uint64_t wd = sdesc(st + w * 128 * BK);
-#pragma unroll
-          for (int k = 0; k < BK / 32; ++k)
-            mma_f8(tbase + (b * MW + w) * NP, wd + 2 * k, xd + 2 * k, idesc_f8(128, NP), k > 0 ? 1u : 0u);
-        }
+        for (int k = 0; k < BK / 32; ++k)
+          mma_f8(tbase + b * NP, wd + 2 * k, xd + 2 * k, idesc_f8(128, NP), k > 0 ? 1u : 0u);
         commit(empty(s));
         commit(tfull(b));
       }
@@ -440,11 +453,12 @@ __global__ void __launch_bounds__(WeightsCfg<NP, MW>::THREADS, WeightsCfg<NP, MW
     __syncwarp();
   } else if (warp >= 2) {
     // ------------------------------------------------------------------ epilogue
-    const int q4 = warp & 3, w = (warp - 2) >> 2;  // lane quarter, weight tile
-    const float* ws = p.ws + (int64_t)min(tile * MW + w, p.nb - 1) * p.ldws + kb0;
-    uint64_t acc[NP / 2];
+    const int q4 = warp & 3, cs = (warp - 2) >> 2;  // lane quarter, share of the tokens
+    const int blk = p.act ? 2 * tile + (q4 >> 1) : tile;  // this warp's 128-row block of W
+    const float* ws = p.ws + (int64_t)min(blk, p.nb - 1) * p.ldws + kb0;
+    uint64_t acc[C::NC / 2];
 #pragma unroll
-    for (int i = 0; i < NP / 2; ++i) acc[i] = 0;
+    for (int i = 0; i < C::NC / 2; ++i) acc[i] = 0;
     pdl_wait();
     float w_n = nkb > 0 ? ws[0] : 0.f;
     bool ok = true;
@@ -457,61 +471,57 @@ __global__ void __launch_bounds__(WeightsCfg<NP, MW>::THREADS, WeightsCfg<NP, MW
       ok = __all_sync(FULL_MASK, ok);  // the warp stays together
       if (!ok) break;
       fence_after();
-      const uint32_t ta = tmem + ((uint32_t)(q4 * 32) << 16) + (b * MW + w) * NP;
-      const ulonglong2* xs = reinterpret_cast<const ulonglong2*>(slots + l * C::SLOT);
-      uint32_t v[2][16];
-      tmem_ld16(ta, v[0]);
+      const uint32_t ta = tmem + ((uint32_t)(q4 * 32) << 16) + b * NP + cs * C::NC;
+      const ulonglong2* xs = reinterpret_cast<const ulonglong2*>(slots + l * C::SLOT) + cs * (C::NC / 4);
 #pragma unroll
-      for (int c = 0; c < NP / 16; ++c) {
-        ld_wait(v[c & 1]);
-        if (c + 1 < NP / 16) {
-          tmem_ld16(ta + (c + 1) * 16, v[(c + 1) & 1]);
-        } else {  // this buffer has been read: the tensor core may overwrite it
+      for (int c = 0; c < C::NC / C::CHUNK; ++c) {
+        uint32_t v[C::CHUNK];
+        tmem_ld(ta + c * C::CHUNK, v);
+        ld_wait(v);
+        if (c + 1 == C::NC / C::CHUNK) {  // this buffer has been read: the tensor core may overwrite it
           fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(tempty(b));
         }
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const ulonglong2 sx = xs[c * 4 + j];  // 4 tokens' scales, the same for every lane
-          uint64_t& a0 = acc[c * 8 + 2 * j];
-          uint64_t& a1 = acc[c * 8 + 2 * j + 1];
-          a0 = fma2(pack2(v[c & 1][4 * j], v[c & 1][4 * j + 1]), mul2(sx.x, wsc), a0);
-          a1 = fma2(pack2(v[c & 1][4 * j + 2], v[c & 1][4 * j + 3]), mul2(sx.y, wsc), a1);
+        for (int j = 0; j < C::CHUNK / 4; ++j) {
+          const ulonglong2 sx = xs[c * (C::CHUNK / 4) + j];  // 4 tokens' scales, the same for every lane
+          uint64_t& a0 = acc[c * (C::CHUNK / 2) + 2 * j];
+          uint64_t& a1 = acc[c * (C::CHUNK / 2) + 2 * j + 1];
+          a0 = fma2(pack2(v[4 * j], v[4 * j + 1]), mul2(sx.x, wsc), a0);
+          a1 = fma2(pack2(v[4 * j + 2], v[4 * j + 3]), mul2(sx.y, wsc), a1);
         }
       }
     }
-    // sums of token c to CTA c mod splits: [slice][c / splits][feature]
-    if (p.splits > 1) {
+    // sums of token c to CTA c mod cluster: [slice][c / cluster][feature of the cluster]
+    if (p.cluster > 1) {
       if (C::OVER_RING) cluster_arrive();  // the last MMA has completed: nothing reads the ring any more
       cluster_wait();
     }
-    const int f = w * 128 + q4 * 32 + lane;
-    const int per = (NP + p.splits - 1) / p.splits;
-    int owner = 0, tl = 0;
-    if (p.splits == 1) {
+    const int r = q4 * 32 + lane;
+    const int f = p.act ? (r >> 6) * 128 + half * 64 + (r & 63) : r;
+    const int width = p.act ? 256 : 128;
+    const int per = (NP + p.cluster - 1) / p.cluster;
+    int owner = (cs * C::NC) % p.cluster, tl = (cs * C::NC) / p.cluster;
 #pragma unroll
-      for (int c = 0; c < NP; ++c)
-        if (c < p.T) {
-          const float2 a = unpack2(acc[c / 2]);
-          exchange[c * MW * 128 + f] = c & 1 ? a.y : a.x;
+    for (int c = 0; c < C::NC; ++c)
+      if (cs * C::NC + c < p.T) {
+        const float2 a = unpack2(acc[c / 2]);
+        const float v = c & 1 ? a.y : a.x;
+        float* dst = exchange + (slice * per + tl) * width + f;
+        if (p.cluster > 1)
+          st_cluster_f32(cluster_map(smem_u32(dst), owner), v);
+        else
+          *dst = v;
+        if (++owner == p.cluster) {
+          owner = 0;
+          ++tl;
         }
-    } else {
-#pragma unroll
-      for (int c = 0; c < NP; ++c)
-        if (c < p.T) {
-          const float2 a = unpack2(acc[c / 2]);
-          st_cluster_f32(cluster_map(smem_u32(exchange + (rank * per + tl) * MW * 128 + f), owner), c & 1 ? a.y : a.x);
-          if (++owner == p.splits) {
-            owner = 0;
-            ++tl;
-          }
-        }
-    }
+      }
   }
   __syncwarp();
   fence_before();
-  if (p.splits > 1) {
+  if (p.cluster > 1) {
     if (warp < 2) {
       if (C::OVER_RING) cluster_arrive();
       cluster_wait();
@@ -522,20 +532,18 @@ __global__ void __launch_bounds__(WeightsCfg<NP, MW>::THREADS, WeightsCfg<NP, MW
     __syncthreads();
   }
   if (warp >= 2 && !*abort_flag) {
-    const int per = (NP + p.splits - 1) / p.splits;
-    const int mine = (p.T - rank + p.splits - 1) / p.splits;  // tokens rank, rank + splits, ...
-    const int wi = warp - 2;
-    if (!p.act) {
-      for (int it = wi; it < mine * MW; it += 4 * MW) {
-        const int tl = it / MW, blk = it % MW;
-        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+    const int per = (NP + p.cluster - 1) / p.cluster;
+    const int mine = (p.T - rank + p.cluster - 1) / p.cluster;  // tokens rank, rank + cluster, ...
+    for (int tl = warp - 2; tl < mine; tl += C::EPI_WARPS) {
+      const int t = rank + tl * p.cluster;
+      if (!p.act) {
+        float o[4] = {0.f, 0.f, 0.f, 0.f};
         for (int r = 0; r < p.splits; ++r) {
-          const float4 v = *reinterpret_cast<const float4*>(exchange + (r * per + tl) * MW * 128 + blk * 128 + lane * 4);
-          a.x += v.x; a.y += v.y; a.z += v.z; a.w += v.w;
+          const float4 v = reinterpret_cast<const float4*>(exchange + (r * per + tl) * 128)[lane];
+          o[0] += v.x; o[1] += v.y; o[2] += v.z; o[3] += v.w;
         }
-        const int n = (tile * MW + blk) * 128 + lane * 4;
-        __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(p.out) + (int64_t)(rank + tl * p.splits) * p.ldo + n;
-        const float o[4] = {a.x, a.y, a.z, a.w};
+        const int n = tile * 128 + lane * 4;
+        __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(p.out) + (int64_t)t * p.ldo + n;
         if (p.vec && n + 4 <= p.N) {
           *reinterpret_cast<uint2*>(dst) = f32_to_bf16x4(o);
         } else {
@@ -543,27 +551,28 @@ __global__ void __launch_bounds__(WeightsCfg<NP, MW>::THREADS, WeightsCfg<NP, MW
           for (int e = 0; e < 4; ++e)
             if (n + e < p.N) dst[e] = __float2bfloat16_rn(o[e]);
         }
-      }
-    } else if constexpr (MW == 2) {
-      for (int tl = wi; tl < mine; tl += 4 * MW) {
-        float4 g = make_float4(0.f, 0.f, 0.f, 0.f), u = g;
+      } else {
+        // the sums stay fp32 up to the 8-bit rounding
+        float g[4] = {0.f, 0.f, 0.f, 0.f}, u[4] = {0.f, 0.f, 0.f, 0.f};
         for (int r = 0; r < p.splits; ++r) {
           const float4* row = reinterpret_cast<const float4*>(exchange + (r * per + tl) * 256);
           const float4 a = row[lane], b = row[32 + lane];
-          g.x += a.x; g.y += a.y; g.z += a.z; g.w += a.w;
-          u.x += b.x; u.y += b.y; u.z += b.z; u.w += b.w;
+          g[0] += a.x; g[1] += a.y; g[2] += a.z; g[3] += a.w;
+          u[0] += b.x; u[1] += b.y; u[2] += b.z; u[3] += b.w;
         }
         const int f = tile * 128 + lane * 4;
-        const bool in = f < p.features;
-        const float h[4] = {in ? silu_f(g.x) * u.x : 0.f, in ? silu_f(g.y) * u.y : 0.f, in ? silu_f(g.z) * u.z : 0.f,
-                            in ? silu_f(g.w) * u.w : 0.f};
         uint32_t m = 0;
+        float h[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) m = max(m, __float_as_uint(h[e]) & 0x7fffffffu);
+        for (int e = 0; e < 4; ++e) {
+          h[e] = f < p.features ? silu_f(g[e]) * u[e] : 0.f;
+          m = max(m, __float_as_uint(h[e]) & 0x7fffffffu);
+        }
         const Fp8Scale sc = fp8_scale(__reduce_max_sync(FULL_MASK, m));
-        const int t = rank + tl * p.splits;
-        const float o[4] = {h[0] * sc.inv, h[1] * sc.inv, h[2] * sc.inv, h[3] * sc.inv};
-        if (in) *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(p.out) + (int64_t)t * p.ldo + f) = f32x4_to_e4m3(o);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) h[e] *= sc.inv;
+        if (f < p.features)
+          *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(p.out) + (int64_t)t * p.ldo + f) = f32x4_to_e4m3(h);
         if (lane == 0) p.os[(int64_t)tile * p.ldos + t] = sc.scale;
       }
     }
@@ -616,50 +625,75 @@ bool make_scale_map(CUtensorMap* m, const float* base, int blocks, int tokens, i
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int NP, int MW>
+template <int NP>
+cudaLaunchConfig_t weights_config(int tiles, int cluster, cudaLaunchAttribute* attr) {
+  using C = WeightsCfg<NP>;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(tiles * cluster);
+  cfg.blockDim = dim3(C::THREADS);
+  cfg.dynamicSmemBytes = C::SMEM;
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = cluster;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  return cfg;
+}
+
+template <int NP>
+cudaError_t weights_opt_in() {
+  static std::atomic<uint64_t> done{0};
+  return smem_opt_in(done, gemm_fp8_weights_kernel<NP>, WeightsCfg<NP>::SMEM);
+}
+
+// Clusters of this size that the GPU holds at once (they have to lie within one of its processing
+// clusters, so it is less than SMs x 2 / cluster).  Cached; entries are atomic, so threads that ask
+// at once store the same value.
+template <int NP>
+int weights_capacity(int cluster, int num_sms) {
+  static std::atomic<int> cache[9];
+  if (int c = cache[cluster].load(std::memory_order_relaxed)) return c;
+  cudaLaunchAttribute attr[2];
+  cudaLaunchConfig_t cfg = weights_config<NP>(64, cluster, attr);
+  cfg.numAttrs = 1;
+  int n = 0;
+  if (weights_opt_in<NP>() != cudaSuccess ||
+      cudaOccupancyMaxActiveClusters(&n, gemm_fp8_weights_kernel<NP>, &cfg) != cudaSuccess || n <= 0) {
+    cudaGetLastError();
+    return num_sms * 2 / cluster;
+  }
+  cache[cluster].store(n, std::memory_order_relaxed);
+  return n;
+}
+
+int weights_capacity(int np, int cluster, int num_sms) {
+  return np == 16   ? weights_capacity<16>(cluster, num_sms)
+         : np == 32 ? weights_capacity<32>(cluster, num_sms)
+         : np == 64 ? weights_capacity<64>(cluster, num_sms)
+                    : weights_capacity<128>(cluster, num_sms);
+}
+
+template <int NP>
 cudaError_t run_weights(const Fp8Gemm& g, Params p, int splits, cudaStream_t stream) {
-  using C = WeightsCfg<NP, MW>;
-  if (splits < 1 || splits > 8 || g.T > NP || (g.act && MW != 2)) return cudaErrorInvalidValue;
+  const int cluster = splits * (g.act ? 2 : 1);
+  if (splits < 1 || cluster > 8 || g.T > NP) return cudaErrorInvalidValue;
   CUtensorMap mx, mw, ms;
-  if (!make_map(&mx, g.xq, g.T, g.K, g.ldx, NP) || !make_map(&mw, g.wq, g.N, g.K, g.ldw, 128 * MW) ||
+  if (!make_map(&mx, g.xq, g.T, g.K, g.ldx, NP) || !make_map(&mw, g.wq, g.N, g.K, g.ldw, 64) ||
       !make_scale_map(&ms, g.xs, p.num_kb, g.T, g.ldxs, NP))
     return cudaErrorInvalidValue;
   p.splits = splits;
+  p.cluster = cluster;
   p.kb_per_split = (p.num_kb + splits - 1) / splits;
-  auto kern = gemm_fp8_weights_kernel<NP, MW>;
-  static std::atomic<uint64_t> done{0};
-  cudaError_t e = smem_opt_in(done, kern, C::SMEM);
+  cudaError_t e = weights_opt_in<NP>();
   if (e != cudaSuccess) return e;
-  const int tiles = (g.N + 128 * MW - 1) / (128 * MW);
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(tiles * splits);
-  cfg.blockDim = dim3(C::THREADS);
-  cfg.dynamicSmemBytes = C::SMEM;
-  cfg.stream = stream;
+  const int rows = g.act ? 256 : 128;
   cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = splits;
-  attr[1].val.clusterDim.y = 1;
-  attr[1].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = splits > 1 ? 2 : 1;
-  return cudaLaunchKernelEx(&cfg, kern, mx, mw, ms, p);
-}
-
-cudaError_t run_weights(const Fp8Gemm& g, const Params& p, const Fp8Plan& pl, cudaStream_t stream) {
-  switch (pl.np * 4 + pl.mw) {
-    case 16 * 4 + 1: return run_weights<16, 1>(g, p, pl.splits, stream);
-    case 32 * 4 + 1: return run_weights<32, 1>(g, p, pl.splits, stream);
-    case 64 * 4 + 1: return run_weights<64, 1>(g, p, pl.splits, stream);
-    case 128 * 4 + 1: return run_weights<128, 1>(g, p, pl.splits, stream);
-    case 16 * 4 + 2: return run_weights<16, 2>(g, p, pl.splits, stream);
-    case 32 * 4 + 2: return run_weights<32, 2>(g, p, pl.splits, stream);
-    case 64 * 4 + 2: return run_weights<64, 2>(g, p, pl.splits, stream);
-    case 128 * 4 + 2: return run_weights<128, 2>(g, p, pl.splits, stream);
-  }
-  return cudaErrorInvalidValue;
+  cudaLaunchConfig_t cfg = weights_config<NP>((g.N + rows - 1) / rows, cluster, attr);
+  cfg.stream = stream;
+  return cudaLaunchKernelEx(&cfg, gemm_fp8_weights_kernel<NP>, mx, mw, ms, p);
 }
 
 }  // namespace
@@ -668,13 +702,11 @@ Fp8Plan fp8_plan(int T, int N, int K, int act, int num_sms) {
   Fp8Plan pl;
   if (T > 128) return pl;
   pl.np = T <= 16 ? 16 : T <= 32 ? 32 : T <= 64 ? 64 : 128;
-  pl.mw = act ? 2 : 1;
-  const int tiles = (N + 128 * pl.mw - 1) / (128 * pl.mw);
+  const int halves = act ? 2 : 1;
+  const int tiles = (N + 128 * halves - 1) / (128 * halves);
   const int num_kb = (K + BK - 1) / BK;
-  const int slots = num_sms * (pl.mw == 1 && pl.np <= 64 ? 2 : 1);
-  pl.splits = 1;
-  for (int s = 2; s <= 8; ++s)
-    if (tiles * s <= slots && num_kb / s >= 2) pl.splits = s;
+  for (int s = 2; s * halves <= 8; ++s)
+    if (num_kb / s >= 2 && tiles <= weights_capacity(pl.np, s * halves, num_sms)) pl.splits = s;
   return pl;
 }
 
@@ -699,7 +731,14 @@ cudaError_t gemm_fp8(const Fp8Gemm& g, const Fp8Plan& pl, int num_sms, cudaStrea
   p.os = g.os;
   p.ldos = g.ldos;
   p.vec = g.ldo % 8 == 0 && (reinterpret_cast<uintptr_t>(g.out) & 15) == 0;
-  if (pl.np) return run_weights(g, p, pl, stream);
+  switch (pl.np) {
+    case 0: break;
+    case 16: return run_weights<16>(g, p, pl.splits, stream);
+    case 32: return run_weights<32>(g, p, pl.splits, stream);
+    case 64: return run_weights<64>(g, p, pl.splits, stream);
+    case 128: return run_weights<128>(g, p, pl.splits, stream);
+    default: return cudaErrorInvalidValue;
+  }
   CUtensorMap mx, mw;
   if (!make_map(&mx, g.xq, g.T, g.K, g.ldx, BM) || !make_map(&mw, g.wq, g.N, g.K, g.ldw, BN))
     return cudaErrorInvalidValue;
