@@ -37,9 +37,9 @@ struct Fp8Gemm {
   int64_t ldos;
 };
 
-// Which kernel computes a product, and in which shape.  np = 0: the kernel with the tokens on the
-// MMA's M side (any T).  np = 16, 32, 64, 128: the weights on the M side, np >= T tokens, K split over
-// `splits` CTAs of a cluster (1 .. 8, with act 1 .. 4).
+// Which kernel computes a product, and over how many CTAs of a cluster K is split.  np = 0: the kernel
+// with the tokens on the MMA's M side (any T; 1, 2, 4 or 8 splits).  np = 16, 32, 64: the weights on
+// the M side, np >= T tokens (1 .. 8 splits, with act 1 .. 4).
 struct Fp8Plan {
   int np = 0, splits = 1;
 };

@@ -29,6 +29,8 @@
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
+#include <algorithm>
+
 #include "fp8_quant.cuh"
 #include "tcgen05.cuh"
 
@@ -45,8 +47,14 @@ constexpr int BN = 256;                 // features per tile
 constexpr int BK = 128;                 // one scale block = one 128-byte swizzle row
 constexpr int STAGES = 4;
 constexpr int A_BYTES = BM * BK, B_BYTES = BN * BK, STAGE_BYTES = A_BYTES + B_BYTES;
-constexpr int THREADS = 320;            // TMA warp, MMA warp, 8 epilogue warps
 constexpr int EPI_THREADS = 256;
+constexpr int THREADS = 128 + EPI_THREADS;  // TMA warp, MMA warp, two idle ones; 8 epilogue warps
+// Registers: the 12 warps are launched with 168 each (65536 / 384); the control warps give theirs up
+// for the epilogue's, which hold 128 sums and two TMEM loads of 32 values.
+constexpr int LAUNCH_REGS = 168, CONTROL_REGS = 56, EPI_REGS = 224;
+static_assert(4 * CONTROL_REGS + 8 * EPI_REGS <= 12 * LAUNCH_REGS, "the launch's registers");
+constexpr int XLD = BN + 4;             // exchange row: 16-byte stores of 8 rows hit distinct banks
+static_assert(BM * XLD * 4 <= STAGES * STAGE_BYTES, "the exchange fits over the ring");
 constexpr int SMEM_TOKENS = 1024 + STAGES * STAGE_BYTES + 2 * 2 * BM * 4 + 8 * (2 * STAGES + 6) + 16;
 
 // Shape of gemm_fp8_weights_kernel<NP> (NP tokens, rounded up).  Two CTAs fit on an SM, so that one
@@ -86,9 +94,8 @@ struct WeightsCfg {
 };
 
 struct Params {
-  // weights kernel: K slices, their length, CTAs per cluster (slices x halves: with SiLU-and-mul two
-  // CTAs share 128 gate and 128 up rows)
-  int splits, kb_per_split, cluster;
+  int splits, kb_per_split;  // K slices and their length in k-blocks
+  int cluster;               // weights kernel: CTAs per cluster (slices x 2 with SiLU-and-mul)
   const float* xs;
   const float* ws;
   int64_t ldxs, ldws;
@@ -139,11 +146,51 @@ __device__ __forceinline__ void store_bf16_64(const Params& p, int row, int c, c
   }
 }
 
+// acc += s * 32 values (pairs).
+__device__ __forceinline__ void add32(uint64_t* acc, const uint32_t (&v)[32], uint64_t s) {
+#pragma unroll
+  for (int i = 0; i < 16; ++i) acc[i] = fma2(pack2(v[2 * i], v[2 * i + 1]), s, acc[i]);
+}
+
+// silu(gate) * up of 4 + 4 sums of the features [f, f + 4) of token t, one warp per token and group of
+// 128: the fp32 sums are rounded once, to 8 bits.
+__device__ __forceinline__ void finish_silu4(const Params& p, int t, int group, int lane, const float* g, const float* u) {
+  const int f = group * 128 + lane * 4;
+  uint32_t m = 0;
+  float h[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    h[e] = f < p.features ? silu_f(g[e]) * u[e] : 0.f;
+    m = max(m, __float_as_uint(h[e]) & 0x7fffffffu);
+  }
+  const Fp8Scale sc = fp8_scale(__reduce_max_sync(FULL_MASK, m));
+#pragma unroll
+  for (int e = 0; e < 4; ++e) h[e] *= sc.inv;
+  if (f < p.features)
+    *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(p.out) + (int64_t)t * p.ldo + f) = f32x4_to_e4m3(h);
+  if (lane == 0) p.os[(int64_t)group * p.ldos + t] = sc.scale;
+}
+
+// bf16 values [n, n + 4) of token t.
+__device__ __forceinline__ void finish_bf16x4(const Params& p, int t, int n, const float* o) {
+  __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(p.out) + (int64_t)t * p.ldo + n;
+  if (p.vec && n + 4 <= p.N) {
+    *reinterpret_cast<uint2*>(dst) = f32_to_bf16x4(o);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (n + e < p.N) dst[e] = __float2bfloat16_rn(o[e]);
+  }
+}
+
+// One tile per cluster of `splits` CTAs (each a slice of K), or, with splits = 1, a persistent CTA per
+// SM that walks the tiles.
 __global__ void __launch_bounds__(THREADS, 1)
     gemm_fp8_tokens_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
                            Params p) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  float* exchange = reinterpret_cast<float*>(smem);  // over the idle ring (splits > 1)
   uint32_t* amax = reinterpret_cast<uint32_t*>(smem + STAGES * STAGE_BYTES);  // [tile parity][half][token]
   uint64_t* bars = reinterpret_cast<uint64_t*>(amax + 2 * 2 * BM);
   const uint32_t bar0 = smem_u32(bars);
@@ -177,116 +224,147 @@ __global__ void __launch_bounds__(THREADS, 1)
   fence_after();
   const uint32_t tmem = *tmem_slot;
   pdl_trigger();
-  pdl_wait();
 
   const int tiles = p.tiles_m * p.tiles_n;
-  if (warp == 0 && lane == 0) {
-    // ------------------------------------------------------------------ producer
-    prefetch_map(&map_x);
-    prefetch_map(&map_w);
-    uint32_t it = 0;
-    bool ok = true;
-    for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
-      int tm, tn;
-      tile_coords(p, t, tm, tn);
-      for (int kb = 0; kb < p.num_kb; ++kb, ++it) {
-        const int s = it % STAGES;
-        if (!mbar_wait(empty(s), ((it / STAGES) & 1) ^ 1, abort_flag, &g_fp8_error, 501)) {
-          ok = false;
-          break;
-        }
-        mbar_arrive_expect_tx(full(s), STAGE_BYTES);
-        const uint32_t st = smem_u32(smem + s * STAGE_BYTES);
-        tma_load_2d(st, &map_x, full(s), kb * BK, tm * BM);
-        tma_load_2d(st + A_BYTES, &map_w, full(s), kb * BK, tn * BN);
+  const int slice = p.splits > 1 ? (int)cluster_rank() : 0;
+  const int t0 = blockIdx.x / p.splits, dt = gridDim.x / p.splits;
+  const int kb0 = slice * p.kb_per_split;
+  const int nkb = max(0, min(p.num_kb - kb0, p.kb_per_split));
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(CONTROL_REGS));
+    if (warp == 0 && lane == 0) {
+      // ---------------------------------------------------------------- producer
+      prefetch_map(&map_x);
+      prefetch_map(&map_w);
+      if (t0 < tiles) {  // into L2 only, ahead of the previous kernel's end
+        int tm, tn;
+        tile_coords(p, t0, tm, tn);
+        for (int i = 0; i < min(nkb, STAGES); ++i) tma_prefetch_2d(&map_w, (kb0 + i) * BK, tn * BN);
       }
-    }
-    if (!ok) {
-      const uint32_t n = it < (uint32_t)STAGES ? it : (uint32_t)STAGES;
-      for (uint32_t j = it - n; j < it; ++j) mbar_drain(full(j % STAGES), (j / STAGES) & 1);
-    }
-  } else if (warp == 1) {
-    // ------------------------------------------------------------------ MMA issuer
-    const uint32_t tbase = __shfl_sync(FULL_MASK, tmem, 0);
-    uint32_t it = 0;
-    bool ok = true;
-    for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
-      for (int kb = 0; kb < p.num_kb; ++kb, ++it) {
-        const int s = it % STAGES, b = it & 1;
-        int okw = 1;
-        if (lane == 0)
-          okw = mbar_wait(tempty(b), ((it >> 1) & 1) ^ 1, abort_flag, &g_fp8_error, 502) &&
-                mbar_wait(full(s), (it / STAGES) & 1, abort_flag, &g_fp8_error, 503);
-        ok = __shfl_sync(FULL_MASK, okw, 0);
-        if (!ok) break;
-        fence_after();
-        const uint32_t st = smem_u32(smem + s * STAGE_BYTES);
-        const uint64_t ad = sdesc(st), bd = sdesc(st + A_BYTES);
-        if (elect_one()) {
+      pdl_wait();
+      uint32_t it = 0;
+      bool ok = true;
+      for (int t = t0; t < tiles && ok; t += dt) {
+        int tm, tn;
+        tile_coords(p, t, tm, tn);
+        for (int i = 0; i < nkb; ++i, ++it) {
+          const int s = it % STAGES;
+          if (!mbar_wait(empty(s), ((it / STAGES) & 1) ^ 1, abort_flag, &g_fp8_error, 501)) {
+            ok = false;
+            break;
+          }
+          mbar_arrive_expect_tx(full(s), STAGE_BYTES);
+          const uint32_t st = smem_u32(smem + s * STAGE_BYTES);
+          tma_load_2d(st, &map_x, full(s), (kb0 + i) * BK, tm * BM);
+          tma_load_2d(st + A_BYTES, &map_w, full(s), (kb0 + i) * BK, tn * BN);
+        }
+      }
+      if (!ok) {
+        const uint32_t n = it < (uint32_t)STAGES ? it : (uint32_t)STAGES;
+        for (uint32_t j = it - n; j < it; ++j) mbar_drain(full(j % STAGES), (j / STAGES) & 1);
+      }
+    } else if (warp == 1) {
+      // ---------------------------------------------------------------- MMA issuer
+      const uint32_t tbase = __shfl_sync(FULL_MASK, tmem, 0);
+      uint32_t it = 0;
+      bool ok = true;
+      for (int t = t0; t < tiles && ok; t += dt) {
+        for (int i = 0; i < nkb; ++i, ++it) {
+          const int s = it % STAGES, b = it & 1;
+          int okw = 1;
+          if (lane == 0)  // the operands first: they are there early, and each wait costs about 200 clocks
+            okw = mbar_wait(full(s), (it / STAGES) & 1, abort_flag, &g_fp8_error, 503) &&
+                  mbar_wait(tempty(b), ((it >> 1) & 1) ^ 1, abort_flag, &g_fp8_error, 502);
+          ok = __shfl_sync(FULL_MASK, okw, 0);
+          if (!ok) break;
+          fence_after();
+          const uint32_t st = smem_u32(smem + s * STAGE_BYTES);
+          const uint64_t ad = sdesc(st), bd = sdesc(st + A_BYTES);
+          if (elect_one()) {
 #pragma unroll
-          for (int k = 0; k < BK / 32; ++k)
-            mma_f8(tbase + b * BN, ad + 2 * k, bd + 2 * k, idesc_f8(BM, BN), k > 0 ? 1u : 0u);
-          commit(empty(s));
-          commit(tfull(b));
+            for (int k = 0; k < BK / 32; ++k)
+              mma_f8(tbase + b * BN, ad + 2 * k, bd + 2 * k, idesc_f8(BM, BN), k > 0 ? 1u : 0u);
+            commit(empty(s));
+            commit(tfull(b));
+          }
+          __syncwarp();
         }
-        __syncwarp();
       }
+      if (elect_one()) commit(final_bar);
+      if (lane == 0) mbar_drain(final_bar, 0);
     }
-    if (elect_one()) commit(final_bar);
-    if (lane == 0) mbar_drain(final_bar, 0);
     __syncwarp();
-  } else if (warp >= 2) {
+    if (p.splits > 1) {
+      cluster_arrive();  // (the epilogue's phases, see there)
+      cluster_wait();
+      cluster_arrive();
+      cluster_wait();
+    }
+  } else {
     // ------------------------------------------------------------------ epilogue
-    const int q4 = warp & 3, wg = (warp - 2) >> 2;
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(EPI_REGS));
+    const int q4 = warp & 3, wg = (warp - 4) >> 2;
+    const int r = q4 * 32 + lane;  // this thread's token in the tile
+    const uint32_t ta0 = tmem + ((uint32_t)(q4 * 32) << 16) + wg * 64;
+    auto landed = [&](uint32_t it) {  // the product of k-block `it` is in its buffer
+      const bool ok = mbar_wait(tfull(it & 1), (it >> 1) & 1, abort_flag, &g_fp8_error, 504);
+      const bool all = __all_sync(FULL_MASK, ok);  // the warp stays together
+      fence_after();
+      return all;
+    };
+    uint64_t acc[2][32];
     uint32_t it = 0, tile_parity = 0;
     bool ok = true;
-    for (int t = blockIdx.x; t < tiles; t += gridDim.x, tile_parity ^= 1) {
+    pdl_wait();
+    for (int t = t0; t < tiles; t += dt, tile_parity ^= 1) {
       int tm, tn;
       tile_coords(p, t, tm, tn);
-      const int row = tm * BM + q4 * 32 + lane;
-      const float* xs = p.xs + row;
-      const float* ws0 = p.ws + (int64_t)(2 * tn) * p.ldws;
-      const float* ws1 = p.ws + (int64_t)min(2 * tn + 1, p.nb - 1) * p.ldws;
-      uint64_t acc[2][32];
+      const int row = tm * BM + r;
+      const float* xs = p.xs + (int64_t)kb0 * p.ldxs + row;
+      const float* ws0 = p.ws + (int64_t)(2 * tn) * p.ldws + kb0;
+      const float* ws1 = p.ws + (int64_t)min(2 * tn + 1, p.nb - 1) * p.ldws + kb0;
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int i = 0; i < 32; ++i) acc[h][i] = 0;
-      float x_n = row < p.T ? xs[0] : 0.f, w0_n = ws0[0], w1_n = ws1[0];
-      for (int kb = 0; kb < p.num_kb; ++kb, ++it) {
-        const float s0 = x_n * w0_n, s1 = x_n * w1_n;
-        const uint64_t sc[2] = {pack2(s0, s0), pack2(s1, s1)};
-        if (kb + 1 < p.num_kb) {
-          x_n = row < p.T ? xs[(int64_t)(kb + 1) * p.ldxs] : 0.f;
-          w0_n = ws0[kb + 1];
-          w1_n = ws1[kb + 1];
-        }
-        const int b = it & 1;
-        ok = mbar_wait(tfull(b), (it >> 1) & 1, abort_flag, &g_fp8_error, 504);
-        ok = __all_sync(FULL_MASK, ok);  // the warp stays together
+      if (nkb > 0) {
+        float x_n = row < p.T ? xs[0] : 0.f, w0_n = ws0[0], w1_n = ws1[0];
+        // 4 loads of 32 columns (2 of each half) per k-block, the next one in flight while one is added
+        uint32_t v[2][32];
+        ok = landed(it);
         if (!ok) break;
-        fence_after();
-        const uint32_t ta = tmem + ((uint32_t)(q4 * 32) << 16) + b * BN + wg * 64;
-        // 8 chunks of 16 columns (4 of each half), the next one in flight while one is added
-        uint32_t v[2][16];
-        tmem_ld(ta, v[0]);
-#pragma unroll
-        for (int c = 0; c < 8; ++c) {
-          ld_wait(v[c & 1]);
-          if (c < 7) tmem_ld(ta + ((c + 1) >> 2) * 128 + ((c + 1) & 3) * 16, v[(c + 1) & 1]);
-          if (c == 7) {  // this buffer has been read: the tensor core may overwrite it
-            fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(tempty(b));
+        tmem_ld(ta0 + (it & 1) * BN, v[0]);
+        for (int kb = 0; kb < nkb; ++kb, ++it) {
+          const float s0 = x_n * w0_n, s1 = x_n * w1_n;
+          const uint64_t sc[2] = {pack2(s0, s0), pack2(s1, s1)};
+          if (kb + 1 < nkb) {
+            x_n = row < p.T ? xs[(int64_t)(kb + 1) * p.ldxs] : 0.f;
+            w0_n = ws0[kb + 1];
+            w1_n = ws1[kb + 1];
           }
+          const uint32_t ta = ta0 + (it & 1) * BN;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            uint64_t& a = acc[c >> 2][(c & 3) * 8 + i];
-            a = fma2(pack2(v[c & 1][2 * i], v[c & 1][2 * i + 1]), sc[c >> 2], a);
+          for (int c = 0; c < 4; ++c) {
+            ld_wait(v[c & 1]);
+            if (c < 3) {
+              tmem_ld(ta + ((c + 1) >> 1) * 128 + ((c + 1) & 1) * 32, v[(c + 1) & 1]);
+            } else {  // this buffer has been read: the tensor core may overwrite it
+              fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(tempty(it & 1));
+              if (kb + 1 < nkb) {
+                ok = landed(it + 1);
+                if (!ok) break;
+                tmem_ld(ta0 + ((it + 1) & 1) * BN, v[0]);
+              }
+            }
+            add32(acc[c >> 1] + (c & 1) * 16, v[c & 1], sc[c >> 1]);
           }
+          if (!ok) break;
         }
+        if (!ok) break;
       }
-      if (!ok) break;
+      if (p.splits > 1) break;  // one tile per cluster; finished below
       if (!p.act) {
         store_bf16_64(p, row, tn * BN + wg * 64, acc[0]);
         store_bf16_64(p, row, tn * BN + 128 + wg * 64, acc[1]);
@@ -304,7 +382,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
         // the other half of the group of 128 belongs to the other warpgroup's thread of this token;
         // two buffers: a warp may be one tile ahead of the reader of the one before
-        uint32_t* am = amax + tile_parity * 2 * BM + q4 * 32 + lane;
+        uint32_t* am = amax + tile_parity * 2 * BM + r;
         am[wg * BM] = m;
         __syncwarp();
         if (lane == 0) mbar_arrive(amax_bar);
@@ -322,6 +400,47 @@ __global__ void __launch_bounds__(THREADS, 1)
             }
           }
           if (wg == 0) p.os[(int64_t)tn * p.ldos + row] = sc.scale;
+        }
+      }
+    }
+    __syncwarp();
+    if (p.splits > 1) {
+      // The slices' sums meet in shared memory, over the idle rings: token r of the tile goes to CTA
+      // r / per of the cluster, [slice][r mod per][feature], which adds them in the order of the slices.
+      const int per = BM / p.splits;
+      int tm, tn;
+      tile_coords(p, t0, tm, tn);
+      cluster_arrive();  // this CTA's last MMA has completed: nothing reads its ring any more
+      cluster_wait();
+      if (ok && tm * BM + r < p.T) {
+        const uint32_t dst = cluster_map(smem_u32(exchange + (slice * per + r % per) * XLD + wg * 64), r / per);
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float2 a = unpack2(acc[h][2 * i]), b = unpack2(acc[h][2 * i + 1]);
+            st_cluster_f32x4(dst + (h * 128 + 4 * i) * 4, make_float4(a.x, a.y, b.x, b.y));
+          }
+      }
+      cluster_arrive();
+      cluster_wait();  // every slice's sums have arrived
+      if (!*abort_flag) {
+        for (int tl = warp - 4; tl < per; tl += EPI_THREADS / 32) {
+          const int row = tm * BM + slice * per + tl;
+          if (row >= p.T) break;
+          float g[4] = {0.f, 0.f, 0.f, 0.f}, u[4] = {0.f, 0.f, 0.f, 0.f};
+          for (int s = 0; s < p.splits; ++s) {
+            const float4* src = reinterpret_cast<const float4*>(exchange + (s * per + tl) * XLD);
+            const float4 a = src[lane], b = src[32 + lane];
+            g[0] += a.x; g[1] += a.y; g[2] += a.z; g[3] += a.w;
+            u[0] += b.x; u[1] += b.y; u[2] += b.z; u[3] += b.w;
+          }
+          if (p.act) {
+            finish_silu4(p, row, tn, lane, g, u);
+          } else {
+            finish_bf16x4(p, row, tn * BN + lane * 4, g);
+            finish_bf16x4(p, row, tn * BN + 128 + lane * 4, u);
+          }
         }
       }
     }
@@ -542,17 +661,8 @@ __global__ void __launch_bounds__(WeightsCfg<NP>::THREADS, 2)
           const float4 v = reinterpret_cast<const float4*>(exchange + (r * per + tl) * 128)[lane];
           o[0] += v.x; o[1] += v.y; o[2] += v.z; o[3] += v.w;
         }
-        const int n = tile * 128 + lane * 4;
-        __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(p.out) + (int64_t)t * p.ldo + n;
-        if (p.vec && n + 4 <= p.N) {
-          *reinterpret_cast<uint2*>(dst) = f32_to_bf16x4(o);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (n + e < p.N) dst[e] = __float2bfloat16_rn(o[e]);
-        }
+        finish_bf16x4(p, t, tile * 128 + lane * 4, o);
       } else {
-        // the sums stay fp32 up to the 8-bit rounding
         float g[4] = {0.f, 0.f, 0.f, 0.f}, u[4] = {0.f, 0.f, 0.f, 0.f};
         for (int r = 0; r < p.splits; ++r) {
           const float4* row = reinterpret_cast<const float4*>(exchange + (r * per + tl) * 256);
@@ -560,20 +670,7 @@ __global__ void __launch_bounds__(WeightsCfg<NP>::THREADS, 2)
           g[0] += a.x; g[1] += a.y; g[2] += a.z; g[3] += a.w;
           u[0] += b.x; u[1] += b.y; u[2] += b.z; u[3] += b.w;
         }
-        const int f = tile * 128 + lane * 4;
-        uint32_t m = 0;
-        float h[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          h[e] = f < p.features ? silu_f(g[e]) * u[e] : 0.f;
-          m = max(m, __float_as_uint(h[e]) & 0x7fffffffu);
-        }
-        const Fp8Scale sc = fp8_scale(__reduce_max_sync(FULL_MASK, m));
-#pragma unroll
-        for (int e = 0; e < 4; ++e) h[e] *= sc.inv;
-        if (f < p.features)
-          *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(p.out) + (int64_t)t * p.ldo + f) = f32x4_to_e4m3(h);
-        if (lane == 0) p.os[(int64_t)tile * p.ldos + t] = sc.scale;
+        finish_silu4(p, t, tile, lane, g, u);
       }
     }
   }
@@ -625,13 +722,11 @@ bool make_scale_map(CUtensorMap* m, const float* base, int blocks, int tokens, i
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int NP>
-cudaLaunchConfig_t weights_config(int tiles, int cluster, cudaLaunchAttribute* attr) {
-  using C = WeightsCfg<NP>;
+cudaLaunchConfig_t cluster_config(int grid, int threads, int smem, int cluster, cudaLaunchAttribute* attr) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(tiles * cluster);
-  cfg.blockDim = dim3(C::THREADS);
-  cfg.dynamicSmemBytes = C::SMEM;
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = cluster;
   attr[0].val.clusterDim.y = 1;
@@ -643,37 +738,52 @@ cudaLaunchConfig_t weights_config(int tiles, int cluster, cudaLaunchAttribute* a
   return cfg;
 }
 
+// Shared-memory opt-in, and the check that the kernel is launched with the registers that its
+// warps redistribute (fewer would leave the epilogue waiting for them).
+cudaError_t tokens_opt_in() {
+  static std::atomic<uint64_t> done{0};
+  return once_per_device(done, []() -> cudaError_t {
+    cudaFuncAttributes a;
+    cudaError_t e = cudaFuncGetAttributes(&a, gemm_fp8_tokens_kernel);
+    if (e != cudaSuccess) return e;
+    if (a.numRegs < LAUNCH_REGS) return cudaErrorInvalidDeviceFunction;
+    return cudaFuncSetAttribute(gemm_fp8_tokens_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_TOKENS);
+  });
+}
+
 template <int NP>
 cudaError_t weights_opt_in() {
   static std::atomic<uint64_t> done{0};
   return smem_opt_in(done, gemm_fp8_weights_kernel<NP>, WeightsCfg<NP>::SMEM);
 }
 
-// Clusters of this size that the GPU holds at once (they have to lie within one of its processing
-// clusters, so it is less than SMs x 2 / cluster).  Cached; entries are atomic, so threads that ask
-// at once store the same value.
-template <int NP>
-int weights_capacity(int cluster, int num_sms) {
+// Clusters of `cluster` CTAs, one CTA per SM, that the GPU holds at once (a cluster lies within one of
+// its processing clusters).  Cached; entries are atomic, so threads that ask at once store the same value.
+int clusters_of_sms(int cluster, int num_sms) {
   static std::atomic<int> cache[9];
+  if (cluster == 1) return num_sms;
   if (int c = cache[cluster].load(std::memory_order_relaxed)) return c;
   cudaLaunchAttribute attr[2];
-  cudaLaunchConfig_t cfg = weights_config<NP>(64, cluster, attr);
+  cudaLaunchConfig_t cfg = cluster_config(64 * cluster, THREADS, SMEM_TOKENS, cluster, attr);
   cfg.numAttrs = 1;
   int n = 0;
-  if (weights_opt_in<NP>() != cudaSuccess ||
-      cudaOccupancyMaxActiveClusters(&n, gemm_fp8_weights_kernel<NP>, &cfg) != cudaSuccess || n <= 0) {
+  if (tokens_opt_in() != cudaSuccess ||
+      cudaOccupancyMaxActiveClusters(&n, gemm_fp8_tokens_kernel, &cfg) != cudaSuccess || n <= 0) {
     cudaGetLastError();
-    return num_sms * 2 / cluster;
+    return num_sms / cluster;
   }
   cache[cluster].store(n, std::memory_order_relaxed);
   return n;
 }
 
-int weights_capacity(int np, int cluster, int num_sms) {
-  return np == 16   ? weights_capacity<16>(cluster, num_sms)
-         : np == 32 ? weights_capacity<32>(cluster, num_sms)
-         : np == 64 ? weights_capacity<64>(cluster, num_sms)
-                    : weights_capacity<128>(cluster, num_sms);
+// The same with two CTAs per SM: an even cluster takes half as many SMs, and a smaller cluster fits
+// wherever a larger one does.
+int clusters_of_half_sms(int cluster, int num_sms) {
+  if (cluster == 1) return 2 * num_sms;
+  const int twice = 2 * clusters_of_sms(cluster, num_sms);
+  return std::max(twice, cluster & 1 ? (cluster < 7 ? clusters_of_half_sms(cluster + 1, num_sms)
+                                                    : clusters_of_sms(4, num_sms))
+                                     : clusters_of_sms(cluster / 2, num_sms));
 }
 
 template <int NP>
@@ -691,7 +801,8 @@ cudaError_t run_weights(const Fp8Gemm& g, Params p, int splits, cudaStream_t str
   if (e != cudaSuccess) return e;
   const int rows = g.act ? 256 : 128;
   cudaLaunchAttribute attr[2];
-  cudaLaunchConfig_t cfg = weights_config<NP>((g.N + rows - 1) / rows, cluster, attr);
+  cudaLaunchConfig_t cfg =
+      cluster_config((g.N + rows - 1) / rows * cluster, WeightsCfg<NP>::THREADS, WeightsCfg<NP>::SMEM, cluster, attr);
   cfg.stream = stream;
   return cudaLaunchKernelEx(&cfg, gemm_fp8_weights_kernel<NP>, mx, mw, ms, p);
 }
@@ -700,13 +811,18 @@ cudaError_t run_weights(const Fp8Gemm& g, Params p, int splits, cudaStream_t str
 
 Fp8Plan fp8_plan(int T, int N, int K, int act, int num_sms) {
   Fp8Plan pl;
-  if (T > 128) return pl;
-  pl.np = T <= 16 ? 16 : T <= 32 ? 32 : T <= 64 ? 64 : 128;
-  const int halves = act ? 2 : 1;
-  const int tiles = (N + 128 * halves - 1) / (128 * halves);
   const int num_kb = (K + BK - 1) / BK;
-  for (int s = 2; s * halves <= 8; ++s)
-    if (num_kb / s >= 2 && tiles <= weights_capacity(pl.np, s * halves, num_sms)) pl.splits = s;
+  if (T <= 64) {
+    pl.np = T <= 16 ? 16 : T <= 32 ? 32 : 64;
+    const int halves = act ? 2 : 1;
+    const int tiles = (N + 128 * halves - 1) / (128 * halves);
+    for (int s = 2; s * halves <= 8; ++s)
+      if (num_kb / s >= 2 && tiles <= clusters_of_half_sms(s * halves, num_sms)) pl.splits = s;
+  } else {
+    const int64_t tiles = (int64_t)((T + BM - 1) / BM) * ((N + BN - 1) / BN);
+    for (int s = 2; s <= 4; s *= 2)
+      if (num_kb / s >= 4 && tiles <= clusters_of_sms(s, num_sms)) pl.splits = s;
+  }
   return pl;
 }
 
@@ -736,19 +852,23 @@ cudaError_t gemm_fp8(const Fp8Gemm& g, const Fp8Plan& pl, int num_sms, cudaStrea
     case 16: return run_weights<16>(g, p, pl.splits, stream);
     case 32: return run_weights<32>(g, p, pl.splits, stream);
     case 64: return run_weights<64>(g, p, pl.splits, stream);
-    case 128: return run_weights<128>(g, p, pl.splits, stream);
     default: return cudaErrorInvalidValue;
   }
+  if (pl.splits != 1 && pl.splits != 2 && pl.splits != 4 && pl.splits != 8) return cudaErrorInvalidValue;
   CUtensorMap mx, mw;
   if (!make_map(&mx, g.xq, g.T, g.K, g.ldx, BM) || !make_map(&mw, g.wq, g.N, g.K, g.ldw, BN))
     return cudaErrorInvalidValue;
   const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n;
-  if (tiles > 0x7fffffff - 65536) return cudaErrorInvalidValue;
-  static std::atomic<uint64_t> done{0};
-  cudaError_t e = smem_opt_in(done, gemm_fp8_tokens_kernel, SMEM_TOKENS);
+  if (tiles > 0x7fffffff / 16) return cudaErrorInvalidValue;
+  p.splits = pl.splits;
+  p.kb_per_split = (p.num_kb + pl.splits - 1) / pl.splits;
+  cudaError_t e = tokens_opt_in();
   if (e != cudaSuccess) return e;
-  const int grid = tiles < num_sms ? (int)tiles : num_sms;
-  return launch_pdl(gemm_fp8_tokens_kernel, dim3(grid), dim3(THREADS), SMEM_TOKENS, stream, mx, mw, p);
+  const int grid = pl.splits > 1 ? (int)tiles * pl.splits : tiles < num_sms ? (int)tiles : num_sms;
+  cudaLaunchAttribute attr[2];
+  cudaLaunchConfig_t cfg = cluster_config(grid, THREADS, SMEM_TOKENS, pl.splits, attr);
+  cfg.stream = stream;
+  return cudaLaunchKernelEx(&cfg, gemm_fp8_tokens_kernel, mx, mw, p);
 }
 
 int gemm_fp8_error_code(int reset) {

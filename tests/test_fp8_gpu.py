@@ -181,14 +181,15 @@ def test_linear_silu(ops, t, i, k):
 
 
 def _plans(t, act):
-    for np_ in (16, 32, 64, 128):
+    for np_ in (16, 32, 64):
         if np_ >= t:
             for splits in (1, 2, 3, 4) if act else (1, 2, 3, 5, 8):
                 yield [np_, splits]
-    yield [0, 1]
+    for splits in (1, 2, 4, 8):
+        yield [0, splits]
 
 
-@pytest.mark.parametrize("t,n,k", [(1, 384, 272), (13, 100, 1712), (32, 640, 1040), (50, 250, 512), (128, 900, 2064)])
+@pytest.mark.parametrize("t,n,k", [(1, 384, 272), (13, 100, 1712), (32, 640, 1040), (50, 250, 512), (128, 900, 2064), (300, 260, 1312)])
 def test_every_kernel_variant(ops, t, n, k):
     """The variants differ in the order of fp32 additions alone."""
     C = ops.C
@@ -215,7 +216,7 @@ def test_every_kernel_variant(ops, t, n, k):
 
 def test_plans_refused(ops):
     x, w = ops.quant_fp8(_acts(20, 256)), _weight(256, 256)
-    for plan in ([16, 1], [32, 9], [24, 1], [32, 0], [32]):
+    for plan in ([16, 1], [32, 9], [128, 1], [24, 1], [32, 0], [32], [0, 3], [0, 16], [0, 0]):
         with pytest.raises(RuntimeError):
             ops.C.linear_fp8(*x, *w, None, plan)
     with pytest.raises(RuntimeError):
