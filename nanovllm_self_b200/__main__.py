@@ -34,6 +34,7 @@ def _parse(argv):
     ap.add_argument("--dtype", default="bf16")
     ap.add_argument("--tp", type=int, default=1, help="tensor-parallel size (launch with torchrun)")
     ap.add_argument("--kv", default="none", help="kv_cache_quant_mode: none, fp8, int8_mock")
+    ap.add_argument("--weights", default="none", help="weight_quant_mode: none, fp8")
     ap.add_argument("--max-model-len", type=int, default=4096)
     ap.add_argument("--block-size", type=int, default=256)
     ap.add_argument("--num-blocks", type=int, default=-1, help="-1 sizes the KV pool from free memory")
@@ -51,7 +52,8 @@ def main(argv=None) -> list:
     if not ids and not a.prompt:
         raise SystemExit("give --prompt or --prompt-ids")
     kw = dict(device=a.device, dtype=a.dtype, max_model_len=a.max_model_len, block_size=a.block_size,
-              num_blocks=a.num_blocks, kv_cache_quant_mode=a.kv, enforce_eager=a.eager)
+              num_blocks=a.num_blocks, kv_cache_quant_mode=a.kv, weight_quant_mode=a.weights,
+              enforce_eager=a.eager)
     results = []
     t0 = time.perf_counter()
     if a.hf:

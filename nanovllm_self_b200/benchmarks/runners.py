@@ -65,7 +65,8 @@ class _Timed:
 
 def _llm(args, **kw):
     base = dict(device=args.device, max_model_len=args.max_model_len, max_num_seqs=args.max_num_seqs,
-                block_size=args.block_size, kv_cache_quant_mode=args.kv, tensor_parallel_size=args.tp)
+                block_size=args.block_size, kv_cache_quant_mode=args.kv, weight_quant_mode=args.weights,
+                tensor_parallel_size=args.tp)
     base.update(kw)
     return LLM(args.model, **base)
 
@@ -96,6 +97,7 @@ def decode_sweep(args) -> dict:
     llm = _llm(args)
     vocab = llm.model_runner.arch.vocab_size
     out = {"bench": "decode_sweep", "model": args.model, "tp": args.tp, "context": args.context, "kv": args.kv,
+           "weights": args.weights,
            "gen": args.gen, "points": []}
     for bs in [int(b) for b in args.batches.split(",")]:
         rows = datasets.uniform_serving(bs, vocab, (args.context, args.context), (args.gen, args.gen), seed=bs)
@@ -168,7 +170,8 @@ def pd(args) -> dict:
     pool = PDPool(args.work_root, args.num_prefill, args.num_decode, args.pd_backend, args.model,
                   policy="affinity_load_aware", tp=args.tp,
                   worker_args=["--max-model-len", str(args.max_model_len), "--block-size", str(args.block_size),
-                               "--kv-cache-quant-mode", args.kv])
+                               "--kv-cache-quant-mode", args.kv,
+                               "--weight-quant-mode", args.weights])
     pool.start()
     try:
         s = pool.run(rows, concurrency=None, rate=args.rate)
@@ -384,6 +387,7 @@ def main(argv=None):
     ap.add_argument("--device", default="cuda")
     ap.add_argument("--tp", type=int, default=1)
     ap.add_argument("--kv", default="none")
+    ap.add_argument("--weights", default="none", help="weight_quant_mode: none, fp8")
     ap.add_argument("--max-model-len", type=int, default=9216)
     ap.add_argument("--max-num-seqs", type=int, default=256)
     ap.add_argument("--block-size", type=int, default=256)

@@ -62,6 +62,7 @@ def resolve_torch_dtype(dtype):
 
 
 KV_QUANT_MODES = ("none", "int8_mock", "fp8")
+WEIGHT_QUANT_MODES = ("none", "fp8")
 COMM_BACKENDS = ("fused", "nccl")
 
 
@@ -77,6 +78,11 @@ class EngineConfig:
     attention_compute_dtype: torch.dtype | str | None = "auto"
     kv_cache_quant_mode: str = "none"
     kv_cache_scale_dtype: torch.dtype | str = torch.float32
+    # "fp8": the decoder layers' weights are quantised to e4m3 as they are loaded, one fp32 scale per
+    # block of 128 x 128, and their inputs in every step, one scale per token and 128 channels (half
+    # the weight bytes per decode step; on a GPU dtype must be bf16).  Embedding, norms and lm_head
+    # stay in ``dtype``.
+    weight_quant_mode: str = "none"
 
     max_model_len: int = 4096
     max_num_seqs: int = 256
@@ -140,6 +146,12 @@ class EngineConfig:
         self.kv_cache_scale_dtype = resolve_torch_dtype(self.kv_cache_scale_dtype) or torch.float32
         if self.kv_cache_quant_mode not in KV_QUANT_MODES:
             raise ValueError(f"unsupported kv_cache_quant_mode: {self.kv_cache_quant_mode}")
+        if self.weight_quant_mode not in WEIGHT_QUANT_MODES:
+            raise ValueError(f"unsupported weight_quant_mode: {self.weight_quant_mode}")
+        if self.weight_quant_mode == "fp8" and self.is_cuda and self.dtype != torch.bfloat16:
+            raise ValueError(f"weight_quant_mode='fp8' needs dtype bf16 on a GPU, not {self.dtype}")
+        if self.weight_quant_mode == "fp8" and self.fused_reduce_scatter:
+            raise ValueError("fused_reduce_scatter needs 16-bit weights (weight_quant_mode='none')")
         if self.comm_backend not in COMM_BACKENDS:
             raise ValueError(f"unsupported comm_backend: {self.comm_backend}")
         if self.prefill_attention not in ("tcgen05", "mma"):

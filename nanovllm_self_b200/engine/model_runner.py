@@ -57,7 +57,8 @@ class ModelRunner:
         self.is_cuda = self.device.type == "cuda"
         self.arch = resolve_arch(config.model, config.model_path)
         dtype = config.dtype
-        self.model = Qwen3ForCausalLM(self.arch, self.tp.rank, self.tp.size, dtype=dtype, device=self.device)
+        self.model = Qwen3ForCausalLM(self.arch, self.tp.rank, self.tp.size, dtype=dtype, device=self.device,
+                                      weight_quant=config.weight_quant_mode)
         with torch.inference_mode():
             if has_checkpoint(config.model_path):
                 load_safetensors(self.model, config.model_path)

@@ -10,6 +10,8 @@
 * ``random_init``: every tensor drawn from N(0, std) with a generator seeded from
   ``(seed, tensor name)`` on the target device; norm weights are 1.  The full tensor is
   drawn and then sliced, so the weights are the same at every TP degree.
+* With fp8 weights (``model.fp8``) each layer's products are quantised as soon as the layer is
+  read, so that at most one layer is held in 16 bits.
 * ``save_hf_checkpoint``: writes the same random weights as an HF directory
   (``config.json`` + safetensors) so another engine can load identical weights.
 """
@@ -23,7 +25,7 @@ import zlib
 import torch
 
 from .configs import Qwen3Arch
-from ..ops.torch_ref import interleave_gate_up
+from ..ops.torch_ref import group_gate_up, interleave_gate_up, quant_fp8_weight
 from .qwen3 import Qwen3ForCausalLM
 
 _HF = "model.layers.{i}."
@@ -140,12 +142,16 @@ def _fill(model: Qwen3ForCausalLM, src) -> Qwen3ForCausalLM:
         L.k_norm = src.get(p + "self_attn.k_norm.weight", dt)
         g = src.get(p + "mlp.gate_proj.weight", dt, rows=(r * ni, (r + 1) * ni))
         u = src.get(p + "mlp.up_proj.weight", dt, rows=(r * ni, (r + 1) * ni))
-        # gate/up rows interleaved in groups of 16: the GEMM applies SiLU-and-mul in its epilogue
-        L.gate_up = interleave_gate_up(g, u).contiguous()
+        # gate/up rows interleaved (in groups of 16, with fp8 weights of 128): the GEMM applies
+        # SiLU-and-mul in its epilogue
+        L.gate_up = group_gate_up(g, u) if model.fp8 else interleave_gate_up(g, u).contiguous()
         del g, u
         L.down = src.get(p + "mlp.down_proj.weight", dt, cols=(r * ni, (r + 1) * ni))
         L.ln1 = src.get(p + "input_layernorm.weight", dt)
         L.ln2 = src.get(p + "post_attention_layernorm.weight", dt)
+        if model.fp8:
+            for name in ("qkv", "o", "gate_up", "down"):
+                setattr(L, name, quant_fp8_weight(getattr(L, name)))
     return model
 
 

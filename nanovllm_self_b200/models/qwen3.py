@@ -17,7 +17,10 @@ B200-first layout (not the reference's module-per-projection layout):
   all-gathers;
 * the embedding table and lm_head are vocab-parallel under TP (the reference keeps
   full replicas on every rank, ``:255-258,285``);
-* the final norm runs only on the rows that are sampled.
+* the final norm runs only on the rows that are sampled;
+* with ``weight_quant="fp8"`` the four products of a layer run on e4m3 weights and inputs with
+  block scales: the norms, the attention output and SiLU-and-mul are rounded to 8 bits where they
+  are produced (``add_rmsnorm_fp8``, ``quant_fp8``, ``linear_silu_fp8``), never stored in 16 bits.
 
 Ops are supplied by an ops object (``ops.get_ops(device)``): hand-written CUDA kernels
 on GPU, the plain-PyTorch oracle on CPU.
@@ -43,10 +46,17 @@ class Qwen3Layer:
 
 class Qwen3ForCausalLM:
     def __init__(self, arch: Qwen3Arch, tp_rank: int = 0, tp_size: int = 1,
-                 dtype: torch.dtype = torch.bfloat16, device="cpu"):
+                 dtype: torch.dtype = torch.bfloat16, device="cpu", weight_quant: str = "none"):
         a = arch
         if a.num_attention_heads % tp_size or a.num_key_value_heads % tp_size or a.intermediate_size % tp_size:
             raise ValueError(f"heads/kv_heads/intermediate must be divisible by tp={tp_size}")
+        self.fp8 = weight_quant == "fp8"
+        if self.fp8:
+            for what, k in (("hidden size", a.hidden_size),
+                            ("attention output per rank", a.num_attention_heads * a.head_dim // tp_size),
+                            ("intermediate size per rank", a.intermediate_size // tp_size)):
+                if k % 16:
+                    raise ValueError(f"fp8 weights need the {what} to be a multiple of 16, got {k}")
         self.arch = a
         self.tp_rank, self.tp_size = tp_rank, tp_size
         self.dtype = dtype
@@ -90,7 +100,8 @@ class Qwen3ForCausalLM:
         return self.num_kv_heads * self.head_dim
 
     def weight_bytes(self) -> int:
-        n = sum(t.numel() * t.element_size() for L in self.layers for t in L.tensors().values())
+        n = sum(t.numel() * t.element_size() for L in self.layers for v in L.tensors().values()
+                for t in (v if isinstance(v, tuple) else (v,)))  # an fp8 weight: (values, scales)
         n += self.embed.numel() * self.embed.element_size() + self.norm.numel() * self.norm.element_size()
         if self.lm_head is not self.embed:
             n += self.lm_head.numel() * self.lm_head.element_size()
@@ -109,9 +120,23 @@ class Qwen3ForCausalLM:
             return self.comm.allreduce_add_rmsnorm(h, residual, w, self.eps)
         return self.ops.add_rmsnorm(h, residual, w, self.eps)
 
+    def _norm_in(self, h, residual, w):
+        """``_reduce_norm`` as the input of a product: in 8 bits with fp8 weights."""
+        if not self.fp8:
+            return self._reduce_norm(h, residual, w)
+        if self.comm is not None and self.tp_size > 1:
+            x, residual = self._reduce_norm(h, residual, w)
+            return self.ops.quant_fp8(x), residual
+        return self.ops.add_rmsnorm_fp8(h, residual, w, self.eps)
+
+    def _linear(self, x, w, out=None):
+        if self.fp8:
+            return self.ops.linear_fp8(x, w, out=out, dtype=self.dtype)
+        return self.ops.linear(x, w, out=out)
+
     def _rs(self, T: int, k: int) -> bool:
         """Row-parallel GEMMs of this step store their rows at the owner rank (decode steps)."""
-        return self.comm is not None and self.tp_size > 1 and self.comm.rs_ok(T, k)
+        return not self.fp8 and self.comm is not None and self.tp_size > 1 and self.comm.rs_ok(T, k)
 
     def forward_hidden(self, input_ids: torch.Tensor, positions: torch.Tensor, ctx, kv_caches, kv_scales=None):
         """Run embedding + all layers.
@@ -133,25 +158,26 @@ class Qwen3ForCausalLM:
         x = None
         for i, L in enumerate(self.layers):
             if not rs or i == 0:
-                x, residual = self._reduce_norm(h, residual, L.ln1)
-            qkv = ops.linear(x, L.qkv)
+                x, residual = self._norm_in(h, residual, L.ln1)
+            qkv = self._linear(x, L.qkv)
             kc, vc = kv_caches[i]
             ks, vs = kv_scales[i] if kv_scales is not None else (None, None)
             q = ops.qkv_post(qkv, L.q_norm, L.k_norm, self.eps, positions, self.cos_sin, kc, vc,
                              ctx.slot_mapping, ks, vs, nq, nkv, d)
-            o = ops.attention(q, kc, vc, ctx, self.scale, ks, vs)
+            o = ops.attention(q, kc, vc, ctx, self.scale, ks, vs).view(T, nq * d)
             if rs:
-                x, residual = self.comm.linear_rs_norm(o.view(T, nq * d), L.o, L.ln2, self.eps)
+                x, residual = self.comm.linear_rs_norm(o, L.o, L.ln2, self.eps)
             else:
-                h = ops.linear(o.view(T, nq * d), L.o, out=self._reduce_in(T))
-                x, residual = self._reduce_norm(h, residual, L.ln2)
-            a = ops.linear_silu(x, L.gate_up)  # silu(gate) * up, fused into the GEMM epilogue
+                h = self._linear(ops.quant_fp8(o) if self.fp8 else o, L.o, out=self._reduce_in(T))
+                x, residual = self._norm_in(h, residual, L.ln2)
+            # silu(gate) * up, fused into the GEMM epilogue
+            a = ops.linear_silu_fp8(x, L.gate_up, self.intermediate) if self.fp8 else ops.linear_silu(x, L.gate_up)
             if rs:
                 # the next layer's ln1, or the final norm after the last layer
                 w_next = self.layers[i + 1].ln1 if i + 1 < n else self.norm
                 x, residual = self.comm.linear_rs_norm(a, L.down, w_next, self.eps)
             else:
-                h = ops.linear(a, L.down, out=self._reduce_in(T))
+                h = self._linear(a, L.down, out=self._reduce_in(T))
         if rs:
             return x, residual, True
         return h, residual, False

@@ -13,6 +13,24 @@ from ..ops import torch_ref as R
 from .qwen3 import Qwen3ForCausalLM
 
 
+def _linear(model, x, w):
+    if model.fp8:
+        return R.linear_fp8(R.quant_fp8(x), w).to(x.dtype)
+    return R.linear(x, w)
+
+
+def _mlp(model, h, L):
+    if model.fp8:  # SiLU-and-mul in fp32, rounded to 8 bits
+        a = R.linear_silu_fp8(R.quant_fp8(h), L.gate_up, model.intermediate)
+        return R.linear_fp8(a, L.down).to(h.dtype)
+    return R.linear(R.silu_mul_interleaved(R.linear(h, L.gate_up)).to(h.dtype), L.down)
+
+
+def _norm(model, x, w):
+    # with fp8 weights a norm is rounded once, to 8 bits
+    return R.rmsnorm(x.float() if model.fp8 else x, w, model.eps)
+
+
 @torch.inference_mode()
 def dense_logits(model: Qwen3ForCausalLM, token_ids: list[int]) -> torch.Tensor:
     """Logits [V] of the last position for one sequence (fp32)."""
@@ -23,18 +41,17 @@ def dense_logits(model: Qwen3ForCausalLM, token_ids: list[int]) -> torch.Tensor:
     nq, nkv, d = model.num_heads, model.num_kv_heads, model.head_dim
     x = R.embedding(ids, model.embed)
     for L in model.layers:
-        h = R.rmsnorm(x, L.ln1, model.eps)
-        qkv = R.linear(h, L.qkv)
+        h = _norm(model, x, L.ln1)
+        qkv = _linear(model, h, L.qkv).to(x.dtype)
         q = qkv[:, :nq * d].reshape(-1, nq, d)
         k = qkv[:, nq * d:(nq + nkv) * d].reshape(-1, nkv, d)
         v = qkv[:, (nq + nkv) * d:].reshape(-1, nkv, d)
         q = R.apply_rope(R.rmsnorm(q, L.q_norm, model.eps), pos, model.cos_sin)
         k = R.apply_rope(R.rmsnorm(k, L.k_norm, model.eps), pos, model.cos_sin)
         o = R.dense_causal_attention(q, k, v, model.scale).reshape(-1, nq * d)
-        x = (x.float() + R.linear(o, L.o).float()).to(x.dtype)
-        h = R.rmsnorm(x, L.ln2, model.eps)
-        a = R.silu_mul_interleaved(R.linear(h, L.gate_up)).to(x.dtype)
-        x = (x.float() + R.linear(a, L.down).float()).to(x.dtype)
+        x = (x.float() + _linear(model, o, L.o).float()).to(x.dtype)
+        h = _norm(model, x, L.ln2)
+        x = (x.float() + _mlp(model, h, L).to(x.dtype).float()).to(x.dtype)
     x = R.rmsnorm(x[-1:], model.norm, model.eps)
     return R.linear(x, model.lm_head)[0].float()
 

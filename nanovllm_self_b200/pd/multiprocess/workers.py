@@ -67,6 +67,7 @@ def add_common_args(ap: argparse.ArgumentParser) -> None:
     ap.add_argument("--max-num-batched-tokens", type=int, default=16384)
     ap.add_argument("--max-model-len", type=int, default=4096)
     ap.add_argument("--kv-cache-quant-mode", default="none")
+    ap.add_argument("--weight-quant-mode", default="none")
     ap.add_argument("--gpu-memory-utilization", type=float, default=0.85)
     ap.add_argument("--global-rank", type=int, default=0)
     ap.add_argument("--world-size", type=int, default=1)
@@ -92,7 +93,7 @@ def build_runner(args, kv_pool_ipc: bool = False) -> ModelRunner:
                        dtype=args.dtype, block_size=args.block_size, num_blocks=args.num_blocks,
                        max_num_seqs=args.max_num_seqs, max_num_batched_tokens=args.max_num_batched_tokens,
                        max_model_len=args.max_model_len, kv_cache_quant_mode=args.kv_cache_quant_mode,
-                       gpu_memory_utilization=args.gpu_memory_utilization, seed=args.seed,
+                       weight_quant_mode=args.weight_quant_mode, gpu_memory_utilization=args.gpu_memory_utilization, seed=args.seed,
                        enforce_eager=args.enforce_eager, tensor_parallel_size=args.tp,
                        comm_backend=args.comm_backend)
     if args.tp > 1:

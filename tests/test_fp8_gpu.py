@@ -256,3 +256,122 @@ def test_empty_and_single(ops):
     x = ops.quant_fp8(_acts(5, 256)[:0])
     assert ops.linear_fp8(x, w).shape == (0, 256)
     assert ops.linear_silu_fp8(x, w, 128)[0].shape == (0, 128)
+
+
+# --------------------------------------------------------------------------- streams and graphs
+def _layer(ops, x, res, w, norm):
+    """The fp8 part of a decoder layer in its order: norm, product, 8-bit form, product, norm, MLP."""
+    h, r = ops.add_rmsnorm_fp8(x, res, norm, 1e-6)
+    o = ops.quant_fp8(ops.linear_fp8(h, w["qkv"]))
+    y = ops.linear_fp8(o, w["o"])
+    h, r = ops.add_rmsnorm_fp8(y, r, norm, 1e-6)
+    return ops.linear_fp8(ops.linear_silu_fp8(h, w["gate_up"], 400), w["down"]), r
+
+
+def _layer_weights(k=512):
+    gu = [torch.randn(400, k, device=DEV, generator=torch.Generator(device=DEV).manual_seed(s)) / k ** 0.5
+          for s in (5, 6)]
+    return {"qkv": _weight(640, k, 1), "o": _weight(k, 640, 2), "gate_up": R.quant_fp8_weight(R.group_gate_up(*gu)),
+            "down": _weight(k, 400, 3)}
+
+
+@pytest.mark.parametrize("t", [1, 37, 300])
+def test_layer_matches_plain_layer(ops, t):
+    """The operators together, against the plain forms of the same steps run in fp32."""
+    from nanovllm_self_b200.ops import TorchOps
+    w, norm = _layer_weights(), (1 + 0.1 * torch.randn(512, device=DEV)).to(torch.bfloat16)
+    x, res = _acts(t, 512), _acts(t, 512, 9)
+    want, want_r = _layer(TorchOps(), x, res.clone(), w, norm)
+    got, got_r = _layer(ops, x, res.clone(), w, norm)
+    # each step differs by fp32 rounding alone; where that moves a value across the border of an
+    # e4m3 step, one operand of the next product moves by up to 2^-3: rare, and averaged over its sum
+    for a, b in ((got, want), (got_r, want_r)):
+        assert ((a.double() - b.double()).norm() <= 0.01 * b.double().norm())
+
+
+def test_side_stream_and_concurrent_graphs(ops):
+    """No state is shared between calls: two captured layers replayed on two streams at once give
+    what the same calls give one after the other."""
+    w, norm = _layer_weights(), torch.ones(512, device=DEV, dtype=torch.bfloat16)
+    ins = [(_acts(t, 512, t), _acts(t, 512, t + 1)) for t in (3, 200)]
+    want = [_layer(ops, x, r.clone(), w, norm)[0] for x, r in ins]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = _layer(ops, ins[0][0], ins[0][1].clone(), w, norm)[0]
+    torch.cuda.synchronize()
+    assert torch.equal(got, want[0])
+    graphs = []
+    for x, r in ins:
+        st = {"r0": r, "r": r.clone(), "x": x}
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            st["r"].copy_(st["r0"])
+            st["y"] = _layer(ops, st["x"], st["r"], w, norm)[0]
+        graphs.append((g, st))
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(20):
+        for (g, _), s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    for (_, st), y in zip(graphs, want):
+        assert torch.equal(st["y"], y)
+
+
+def test_weights_written_just_before_the_call(ops):
+    """The kernels start before the previous kernel ends; what it writes is still seen."""
+    x = ops.quant_fp8(_acts(9, 1024))
+    pool = [_weight(512, 1024, s) for s in range(6)]
+    want = [ops.linear_fp8(x, w) for w in pool]
+    q, s = torch.empty_like(pool[0][0]), torch.empty_like(pool[0][1])
+    for i in list(range(6)) * 5:
+        s.copy_(pool[i][1])
+        q.view(torch.uint8).copy_(pool[i][0].view(torch.uint8))
+        assert torch.equal(ops.linear_fp8(x, (q, s)), want[i])
+
+
+# --------------------------------------------------------------------------- engine
+def _llm(**kw):
+    from nanovllm_self_b200 import LLM
+    base = dict(device="cuda", max_model_len=1024, max_num_seqs=16, num_blocks=128, block_size=16, cuda_graph_max_bs=16,
+                weight_quant_mode="fp8")
+    base.update(kw)
+    return LLM("tiny-gpu", **base)
+
+
+def _prompts():
+    g = torch.Generator().manual_seed(1)
+    return [torch.randint(0, 2048, (n,), generator=g).tolist() for n in (17, 40, 64, 100)]
+
+
+@pytest.mark.parametrize("kv", ["none", "fp8"])
+def test_engine_logits_match_dense_oracle(kv):
+    from nanovllm_self_b200 import SamplingParams
+    from nanovllm_self_b200.engine.sequence import Sequence
+    from nanovllm_self_b200.models.reference import dense_logits
+    llm = _llm(kv_cache_quant_mode=kv)
+    r = llm.model_runner
+    for p in _prompts():
+        s = Sequence(0, p, SamplingParams(temperature=0, max_tokens=1), r.block_size)
+        r.block_manager.allocate(s)
+        s.num_new_tokens = len(p) - s.num_cached_tokens
+        got = r.logits([s])[0].float()
+        r.block_manager.deallocate(s)
+        ref = dense_logits(r.model, p)
+        cos = torch.nn.functional.cosine_similarity(got, ref, dim=0).item()
+        # The two differ by bf16 roundings, 2^-9 of a value, ahead of each rounding to e4m3, whose steps
+        # are 2^-3: one value in 2^-3 / 2^-9 = 2^6 moves by a step, so an operand carries noise of
+        # 2^-3 * sqrt(2^-6) = 2^-6 of itself, and each of the 8 products of the two layers adds as much:
+        # sqrt(8) * 2^-6 = 0.044 of the logits, twice that with a margin, cos = 1 - 0.088^2 / 2 = 0.996.
+        # The 8-bit cache's own noise (0.1, cos 0.995) adds in square: 1 - (0.088^2 + 0.1^2) / 2 = 0.991.
+        assert cos > (0.996 if kv == "none" else 0.991), cos
+
+
+def test_engine_graph_equals_eager():
+    from nanovllm_self_b200 import SamplingParams
+    sp = SamplingParams(temperature=0, max_tokens=16, ignore_eos=True)
+    out = [_llm(enforce_eager=e).generate(_prompts(), sp) for e in (False, True)]
+    assert out[0] == out[1]
