@@ -93,6 +93,12 @@ struct WeightsCfg {
   static_assert(SMEM <= BUDGET, "two CTAs per SM");
 };
 
+// A wait of a whole warp that stays together afterwards.  All lanes poll: electing one to do it costs
+// more (the divergent branch and the broadcast) than the 31 other polls of the same word.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int code) {
+  return __all_sync(FULL_MASK, mbar_wait(bar, parity, abort_flag, &g_fp8_error, code));
+}
+
 struct Params {
   int splits, kb_per_split;  // K slices and their length in k-blocks
   int cluster;               // weights kernel: CTAs per cluster (slices x 2 with SiLU-and-mul)
@@ -180,6 +186,49 @@ __device__ __forceinline__ void finish_bf16x4(const Params& p, int t, int n, con
 #pragma unroll
     for (int e = 0; e < 4; ++e)
       if (n + e < p.N) dst[e] = __float2bfloat16_rn(o[e]);
+  }
+}
+
+// Tokens [128 slice / S, 128 (slice + 1) / S) of a tile whose sums lie in the S CTAs of the cluster: added
+// in the order of the slices, finished and stored.  A warp takes a token's 256 sums of one slice as two
+// 512-byte rows (remote reads of whole rows; remote stores of each thread's own 16 bytes took 5 us per
+// tile) and has 16 of them in flight.
+template <int S>
+__device__ __forceinline__ void finish_rows(const Params& p, float* exchange, int slice, int tm, int tn, int w,
+                                            int lane) {
+  constexpr int PER = BM / S, G = 8 / S;
+  for (int tl = w * G; tl < PER; tl += EPI_THREADS / 32 * G) {
+    const int r0 = slice * PER + tl;
+    if (tm * BM + r0 >= p.T) break;
+    const uint32_t src = smem_u32(exchange + r0 * XLD + lane * 4);
+    float4 a[G][S], b[G][S];
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+      const uint32_t at = cluster_map(src, s);
+#pragma unroll
+      for (int i = 0; i < G; ++i) {
+        a[i][s] = ld_cluster_f32x4(at + i * XLD * 4);
+        b[i][s] = ld_cluster_f32x4(at + i * XLD * 4 + 512);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < G; ++i) {
+      float g[4] = {0.f, 0.f, 0.f, 0.f}, u[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int s = 0; s < S; ++s) {
+        g[0] += a[i][s].x; g[1] += a[i][s].y; g[2] += a[i][s].z; g[3] += a[i][s].w;
+        u[0] += b[i][s].x; u[1] += b[i][s].y; u[2] += b[i][s].z; u[3] += b[i][s].w;
+      }
+      const int row = tm * BM + r0 + i;
+      if (row < p.T) {  // the same for the whole warp
+        if (p.act) {
+          finish_silu4(p, row, tn, lane, g, u);
+        } else {
+          finish_bf16x4(p, row, tn * BN + lane * 4, g);
+          finish_bf16x4(p, row, tn * BN + 128 + lane * 4, u);
+        }
+      }
+    }
   }
 }
 
@@ -271,11 +320,8 @@ __global__ void __launch_bounds__(THREADS, 1)
       for (int t = t0; t < tiles && ok; t += dt) {
         for (int i = 0; i < nkb; ++i, ++it) {
           const int s = it % STAGES, b = it & 1;
-          int okw = 1;
-          if (lane == 0)  // the operands first: they are there early, and each wait costs about 200 clocks
-            okw = mbar_wait(full(s), (it / STAGES) & 1, abort_flag, &g_fp8_error, 503) &&
-                  mbar_wait(tempty(b), ((it >> 1) & 1) ^ 1, abort_flag, &g_fp8_error, 502);
-          ok = __shfl_sync(FULL_MASK, okw, 0);
+          ok = warp_wait(full(s), (it / STAGES) & 1, abort_flag, 503) &&
+               warp_wait(tempty(b), ((it >> 1) & 1) ^ 1, abort_flag, 502);
           if (!ok) break;
           fence_after();
           const uint32_t st = smem_u32(smem + s * STAGE_BYTES);
@@ -307,10 +353,9 @@ __global__ void __launch_bounds__(THREADS, 1)
     const int r = q4 * 32 + lane;  // this thread's token in the tile
     const uint32_t ta0 = tmem + ((uint32_t)(q4 * 32) << 16) + wg * 64;
     auto landed = [&](uint32_t it) {  // the product of k-block `it` is in its buffer
-      const bool ok = mbar_wait(tfull(it & 1), (it >> 1) & 1, abort_flag, &g_fp8_error, 504);
-      const bool all = __all_sync(FULL_MASK, ok);  // the warp stays together
+      const bool ok = warp_wait(tfull(it & 1), (it >> 1) & 1, abort_flag, 504);
       fence_after();
-      return all;
+      return ok;
     };
     uint64_t acc[2][32];
     uint32_t it = 0, tile_parity = 0;
@@ -386,8 +431,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         am[wg * BM] = m;
         __syncwarp();
         if (lane == 0) mbar_arrive(amax_bar);
-        ok = mbar_wait(amax_bar, tile_parity, abort_flag, &g_fp8_error, 505);
-        ok = __all_sync(FULL_MASK, ok);
+        ok = warp_wait(amax_bar, tile_parity, abort_flag, 505);
         if (!ok) break;
         const Fp8Scale sc = fp8_scale(max(m, am[(wg ^ 1) * BM]));
         if (row < p.T) {
@@ -405,44 +449,27 @@ __global__ void __launch_bounds__(THREADS, 1)
     }
     __syncwarp();
     if (p.splits > 1) {
-      // The slices' sums meet in shared memory, over the idle rings: token r of the tile goes to CTA
-      // r / per of the cluster, [slice][r mod per][feature], which adds them in the order of the slices.
-      const int per = BM / p.splits;
+      // Every CTA lays its sums out in its own shared memory, over its idle ring (the last MMA has
+      // completed), [token][feature]; after the cluster's barrier CTA s finishes 128 / splits tokens.
       int tm, tn;
       tile_coords(p, t0, tm, tn);
-      cluster_arrive();  // this CTA's last MMA has completed: nothing reads its ring any more
-      cluster_wait();
-      if (ok && tm * BM + r < p.T) {
-        const uint32_t dst = cluster_map(smem_u32(exchange + (slice * per + r % per) * XLD + wg * 64), r / per);
+      float* dst = exchange + r * XLD + wg * 64;
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+      for (int h = 0; h < 2; ++h)
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const float2 a = unpack2(acc[h][2 * i]), b = unpack2(acc[h][2 * i + 1]);
-            st_cluster_f32x4(dst + (h * 128 + 4 * i) * 4, make_float4(a.x, a.y, b.x, b.y));
-          }
+        for (int i = 0; i < 16; ++i) {
+          const float2 a = unpack2(acc[h][2 * i]), b = unpack2(acc[h][2 * i + 1]);
+          *reinterpret_cast<float4*>(dst + h * 128 + 4 * i) = make_float4(a.x, a.y, b.x, b.y);
+        }
+      cluster_arrive();
+      cluster_wait();  // every slice's sums are laid out
+      if (!*abort_flag) {
+        if (p.splits == 2) finish_rows<2>(p, exchange, slice, tm, tn, warp - 4, lane);
+        else if (p.splits == 4) finish_rows<4>(p, exchange, slice, tm, tn, warp - 4, lane);
+        else finish_rows<8>(p, exchange, slice, tm, tn, warp - 4, lane);
       }
       cluster_arrive();
-      cluster_wait();  // every slice's sums have arrived
-      if (!*abort_flag) {
-        for (int tl = warp - 4; tl < per; tl += EPI_THREADS / 32) {
-          const int row = tm * BM + slice * per + tl;
-          if (row >= p.T) break;
-          float g[4] = {0.f, 0.f, 0.f, 0.f}, u[4] = {0.f, 0.f, 0.f, 0.f};
-          for (int s = 0; s < p.splits; ++s) {
-            const float4* src = reinterpret_cast<const float4*>(exchange + (s * per + tl) * XLD);
-            const float4 a = src[lane], b = src[32 + lane];
-            g[0] += a.x; g[1] += a.y; g[2] += a.z; g[3] += a.w;
-            u[0] += b.x; u[1] += b.y; u[2] += b.z; u[3] += b.w;
-          }
-          if (p.act) {
-            finish_silu4(p, row, tn, lane, g, u);
-          } else {
-            finish_bf16x4(p, row, tn * BN + lane * 4, g);
-            finish_bf16x4(p, row, tn * BN + 128 + lane * 4, u);
-          }
-        }
-      }
+      cluster_wait();  // nobody reads this CTA's shared memory any more
     }
   }
   __syncwarp();
@@ -550,11 +577,9 @@ __global__ void __launch_bounds__(WeightsCfg<NP>::THREADS, 2)
     const uint32_t tbase = __shfl_sync(FULL_MASK, tmem, 0);
     for (int i = 0; i < nkb; ++i) {
       const int s = i % S, b = i % NB;
-      int okw = 1;
-      if (lane == 0)
-        okw = mbar_wait(tempty(b), ((i / NB) & 1) ^ 1, abort_flag, &g_fp8_error, 512) &&
-              mbar_wait(full(s), (i / S) & 1, abort_flag, &g_fp8_error, 513);
-      if (!__shfl_sync(FULL_MASK, okw, 0)) break;
+      if (!warp_wait(full(s), (i / S) & 1, abort_flag, 513) ||
+          !warp_wait(tempty(b), ((i / NB) & 1) ^ 1, abort_flag, 512))
+        break;
       fence_after();
       const uint32_t st = smem_u32(smem + s * C::STAGE);
       const uint64_t wd = sdesc(st), xd = sdesc(st + C::W_BYTES);
@@ -585,9 +610,7 @@ __global__ void __launch_bounds__(WeightsCfg<NP>::THREADS, 2)
       const uint64_t wsc = pack2(w_n, w_n);
       if (i + 1 < nkb) w_n = ws[i + 1];
       const int b = i % NB, l = i % SL;
-      ok = mbar_wait(sfull(l), (i / SL) & 1, abort_flag, &g_fp8_error, 514) &&
-           mbar_wait(tfull(b), (i / NB) & 1, abort_flag, &g_fp8_error, 515);
-      ok = __all_sync(FULL_MASK, ok);  // the warp stays together
+      ok = warp_wait(sfull(l), (i / SL) & 1, abort_flag, 514) && warp_wait(tfull(b), (i / NB) & 1, abort_flag, 515);
       if (!ok) break;
       fence_after();
       const uint32_t ta = tmem + ((uint32_t)(q4 * 32) << 16) + b * NP + cs * C::NC;
