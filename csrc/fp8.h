@@ -37,11 +37,12 @@ struct Fp8Gemm {
   int64_t ldos;
 };
 
-// Which kernel computes a product, and over how many CTAs of a cluster K is split.  np = 0: the kernel
-// with the tokens on the MMA's M side (any T; 1, 2, 4 or 8 splits).  np = 16, 32, 64: the weights on
-// the M side, np >= T tokens (1 .. 8 splits, with act 1 .. 4).
+// Which kernel computes a product, and over how many CTAs of a cluster K is split.  np = -1, -2: the
+// kernel with the tokens on the MMA's M side (any T), 1 or 2 CTAs per tile; splits x CTAs at most 8,
+// splits 1, 2, 4 or 8.  np = 16, 32, 64: the weights on the M side, np >= T tokens, 1 .. 8 splits
+// (with act 1 .. 4).
 struct Fp8Plan {
-  int np = 0, splits = 1;
+  int np = -1, splits = 1;
 };
 // The plan of a product, from its sizes alone (the same in every process and every call).
 Fp8Plan fp8_plan(int T, int N, int K, int act, int num_sms);

@@ -10,12 +10,13 @@
 //
 // No counterpart in the reference, whose linear layers are 16-bit (nanovllm/models/qwen3.py:96-134).
 //
-// gemm_fp8_tokens_kernel: tiles of 128 tokens (MMA M, one TMEM lane each) x 256 features (MMA N).
-// A thread of the epilogue owns one token and 64 + 64 features, [64 w, 64 w + 64) of both 128-row
-// weight blocks of the tile: both scales are then one number per thread and k-block (no scale
-// vector to load), and with gate and up rows in alternating blocks of 128 the thread holds matching
-// gate / up pairs, so SiLU-and-mul needs no exchange and the tile is one whole group of 128 of the
-// 8-bit output.
+// gemm_fp8_tokens_kernel<CTAS>: tiles of 128 tokens (MMA M, one TMEM lane each) x 256 features (MMA N)
+// per CTA; CTAS = 2: a pair of CTAs (tcgen05.mma.cta_group::2) shares the 256 weight rows of a tile of
+// 256 tokens, each staging 128 of them.  A thread of the epilogue owns one token and 64 + 64 features,
+// [64 w, 64 w + 64) of both 128-row weight blocks of the tile: both scales are then one number per
+// thread and k-block (no scale vector to load), and with gate and up rows in alternating blocks of 128
+// the thread holds matching gate / up pairs, so SiLU-and-mul needs no exchange and the tile is one whole
+// group of 128 of the 8-bit output.
 //
 // gemm_fp8_weights_kernel: few tokens.  Tiles of 128 weight rows (MMA M) x NP tokens (MMA N), so a
 // step of one token moves 16 activation rows beside the weights instead of 128, and K split over the
@@ -42,20 +43,28 @@ namespace {
 
 using namespace tc;
 
-constexpr int BM = 128;                 // tokens per tile
+constexpr int BM = 128;                 // tokens per CTA
 constexpr int BN = 256;                 // features per tile
 constexpr int BK = 128;                 // one scale block = one 128-byte swizzle row
-constexpr int STAGES = 4;
-constexpr int A_BYTES = BM * BK, B_BYTES = BN * BK, STAGE_BYTES = A_BYTES + B_BYTES;
+constexpr int BUFS = 2;                 // accumulator buffers (all of TMEM)
 constexpr int EPI_THREADS = 256;
-constexpr int THREADS = 128 + EPI_THREADS;  // TMA warp, MMA warp, two idle ones; 8 epilogue warps
+constexpr int THREADS = 128 + EPI_THREADS;  // TMA warp, MMA warp, two scale warps; 8 epilogue warps
 // Registers: the 12 warps are launched with 168 each (65536 / 384); the control warps give theirs up
 // for the epilogue's, which hold 128 sums and two TMEM loads of 32 values.
 constexpr int LAUNCH_REGS = 168, CONTROL_REGS = 56, EPI_REGS = 224;
 static_assert(4 * CONTROL_REGS + 8 * EPI_REGS <= 12 * LAUNCH_REGS, "the launch's registers");
 constexpr int XLD = BN + 4;             // exchange row: 16-byte stores of 8 rows hit distinct banks
-static_assert(BM * XLD * 4 <= STAGES * STAGE_BYTES, "the exchange fits over the ring");
-constexpr int SMEM_TOKENS = 1024 + STAGES * STAGE_BYTES + 2 * 2 * BM * 4 + 8 * (2 * STAGES + 6) + 16;
+
+template <int CTAS>
+struct TokensCfg {
+  static constexpr int B_ROWS = BN / CTAS;  // weight rows staged by one CTA
+  static constexpr int A_BYTES = BM * BK, STAGE = A_BYTES + B_ROWS * BK;  // 48 or 32 KB
+  static constexpr int STAGES = CTAS == 2 ? 6 : 4;
+  static constexpr int SLOTS = STAGES + BUFS + 1;  // activation scales of one k-block each: see the producer
+  static constexpr int BARS = 2 * STAGES + 2 * BUFS + SLOTS + 2;
+  static constexpr int SMEM = 1024 + STAGES * STAGE + SLOTS * BM * 4 + 4 * 2 * BM * 4 + 2 * 2 * BM * 4 + 8 * BARS + 16;
+  static_assert(BM * XLD * 4 <= STAGES * STAGE, "the exchange fits over the ring");
+};
 
 // Shape of gemm_fp8_weights_kernel<NP> (NP tokens, rounded up).  Two CTAs fit on an SM, so that one
 // streams while the other fills its pipeline or finishes, and so that the next kernel's CTAs start early.
@@ -102,9 +111,8 @@ __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatil
 struct Params {
   int splits, kb_per_split;  // K slices and their length in k-blocks
   int cluster;               // weights kernel: CTAs per cluster (slices x 2 with SiLU-and-mul)
-  const float* xs;
   const float* ws;
-  int64_t ldxs, ldws;
+  int64_t ldws;
   int T, N, num_kb, nb;      // nb: 128-row blocks of W
   int tiles_m, tiles_n, group;
   int act, features, vec;    // vec: bf16 rows allow 16-byte stores
@@ -126,37 +134,51 @@ __device__ __forceinline__ void tile_coords(const Params& p, int t, int& tm, int
   tn = r / size;
 }
 
-__device__ __forceinline__ float silu_f(float g) { return g / (1.f + expf(-g)); }
+// __expf is within 2 + 1.2 |g| units and __fdividef within 2: far inside the 8-bit rounding that follows.
+__device__ __forceinline__ float silu_f(float g) { return __fdividef(g, 1.f + __expf(-g)); }
 
-// bf16 values [c, c + 64) of one row (accumulator pairs in `acc`).
-__device__ __forceinline__ void store_bf16_64(const Params& p, int row, int c, const uint64_t* acc) {
+// bf16 values [c, c + 32) of one row.
+__device__ __forceinline__ void store_bf16_32(const Params& p, int row, int c, const float* acc) {
   if (row >= p.T || c >= p.N) return;
   __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(p.out) + (int64_t)row * p.ldo + c;
   const int n = p.N - c;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    float f[8];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float2 v = unpack2(acc[4 * i + j]);
-      f[2 * j] = v.x;
-      f[2 * j + 1] = v.y;
-    }
-    if (p.vec && 8 * i + 8 <= n) {
-      *reinterpret_cast<uint4*>(dst + 8 * i) = f32_to_bf16x8(f);
+  for (int i = 0; i < 32; i += 8) {
+    if (p.vec && i + 8 <= n) {
+      *reinterpret_cast<uint4*>(dst + i) = f32_to_bf16x8(acc + i);
     } else {
 #pragma unroll
       for (int j = 0; j < 8; ++j)
-        if (8 * i + j < n) dst[8 * i + j] = __float2bfloat16_rn(f[j]);
+        if (i + j < n) dst[i + j] = __float2bfloat16_rn(acc[i + j]);
     }
   }
 }
 
-// acc += s * 32 values (pairs).
-__device__ __forceinline__ void add32(uint64_t* acc, const uint32_t (&v)[32], uint64_t s) {
+// acc += s * 32 values.
+__device__ __forceinline__ void add32(float* acc, const uint32_t (&v)[32], float s) {
 #pragma unroll
-  for (int i = 0; i < 16; ++i) acc[i] = fma2(pack2(v[2 * i], v[2 * i + 1]), s, acc[i]);
+  for (int i = 0; i < 32; ++i) acc[i] = fmaf(__uint_as_float(v[i]), s, acc[i]);
 }
+
+// The scales of one 128-row block of W for k-blocks 0, 1, .. n - 1, asked for in this order by a whole
+// warp.  Lane l holds those of l, l + 32, ..: 32 per load, which is under way 32 k-blocks early (a load
+// per k-block, with one k-block to arrive in, held the epilogue up by 500 clocks each).
+struct WeightScales {
+  const float* w;
+  int n, lane;
+  float now, next;
+  __device__ __forceinline__ WeightScales(const float* w_, int n_, int lane_) : w(w_), n(n_), lane(lane_) {
+    now = lane < n ? w[lane] : 0.f;
+    next = lane + 32 < n ? w[lane + 32] : 0.f;
+  }
+  __device__ __forceinline__ float at(int kb) {
+    if ((kb & 31) == 0 && kb > 0) {
+      now = next;
+      next = kb + 32 + lane < n ? w[kb + 32 + lane] : 0.f;
+    }
+    return __shfl_sync(FULL_MASK, now, kb & 31);
+  }
+};
 
 // silu(gate) * up of 4 + 4 sums of the features [f, f + 4) of token t, one warp per token and group of
 // 128: the fp32 sums are rounded once, to 8 bits.
@@ -189,22 +211,22 @@ __device__ __forceinline__ void finish_bf16x4(const Params& p, int t, int n, con
   }
 }
 
-// Tokens [128 slice / S, 128 (slice + 1) / S) of a tile whose sums lie in the S CTAs of the cluster: added
-// in the order of the slices, finished and stored.  A warp takes a token's 256 sums of one slice as two
-// 512-byte rows (remote reads of whole rows; remote stores of each thread's own 16 bytes took 5 us per
-// tile) and has 16 of them in flight.
-template <int S>
-__device__ __forceinline__ void finish_rows(const Params& p, float* exchange, int slice, int tm, int tn, int w,
-                                            int lane) {
+// Tokens [128 slice / S, 128 (slice + 1) / S) of this CTA's 128, whose sums lie in S CTAs of the cluster
+// (ranks r, r + CTAS, ...): added in the order of the slices, finished and stored.  A warp takes a
+// token's 256 sums of one slice as two 512-byte rows (remote stores of each thread's own 16 bytes were
+// slower by half) and has 16 of them in flight.
+template <int CTAS, int S>
+__device__ __forceinline__ void finish_rows(const Params& p, float* exchange, int slice, int r, int row0, int tn,
+                                            int w, int lane) {
   constexpr int PER = BM / S, G = 8 / S;
   for (int tl = w * G; tl < PER; tl += EPI_THREADS / 32 * G) {
     const int r0 = slice * PER + tl;
-    if (tm * BM + r0 >= p.T) break;
+    if (row0 + r0 >= p.T) break;
     const uint32_t src = smem_u32(exchange + r0 * XLD + lane * 4);
     float4 a[G][S], b[G][S];
 #pragma unroll
     for (int s = 0; s < S; ++s) {
-      const uint32_t at = cluster_map(src, s);
+      const uint32_t at = cluster_map(src, s * CTAS + r);
 #pragma unroll
       for (int i = 0; i < G; ++i) {
         a[i][s] = ld_cluster_f32x4(at + i * XLD * 4);
@@ -219,7 +241,7 @@ __device__ __forceinline__ void finish_rows(const Params& p, float* exchange, in
         g[0] += a[i][s].x; g[1] += a[i][s].y; g[2] += a[i][s].z; g[3] += a[i][s].w;
         u[0] += b[i][s].x; u[1] += b[i][s].y; u[2] += b[i][s].z; u[3] += b[i][s].w;
       }
-      const int row = tm * BM + r0 + i;
+      const int row = row0 + r0 + i;
       if (row < p.T) {  // the same for the whole warp
         if (p.act) {
           finish_silu4(p, row, tn, lane, g, u);
@@ -232,51 +254,64 @@ __device__ __forceinline__ void finish_rows(const Params& p, float* exchange, in
   }
 }
 
-// One tile per cluster of `splits` CTAs (each a slice of K), or, with splits = 1, a persistent CTA per
-// SM that walks the tiles.
+// One tile per cluster of splits x CTAS CTAs (each group of CTAS a slice of K), or, with splits = 1,
+// persistent CTAs that walk the tiles.
+template <int CTAS>
 __global__ void __launch_bounds__(THREADS, 1)
     gemm_fp8_tokens_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
-                           Params p) {
+                           const __grid_constant__ CUtensorMap map_s, Params p) {
+  using C = TokensCfg<CTAS>;
+  constexpr int S = C::STAGES, SL = C::SLOTS;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
+  // the same offset in every CTA of the cluster
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   float* exchange = reinterpret_cast<float*>(smem);  // over the idle ring (splits > 1)
-  uint32_t* amax = reinterpret_cast<uint32_t*>(smem + STAGES * STAGE_BYTES);  // [tile parity][half][token]
+  float* slots = reinterpret_cast<float*>(smem + S * C::STAGE);
+  float* prods = slots + SL * BM;  // [k-block & 3][weight block][token]: activation scale x weight scale
+  uint32_t* amax = reinterpret_cast<uint32_t*>(prods + 4 * 2 * BM);  // [tile parity][half][token]
   uint64_t* bars = reinterpret_cast<uint64_t*>(amax + 2 * 2 * BM);
   const uint32_t bar0 = smem_u32(bars);
-  auto full = [&](int s) { return bar0 + 8u * s; };
-  auto empty = [&](int s) { return bar0 + 8u * (STAGES + s); };
-  auto tfull = [&](int b) { return bar0 + 8u * (2 * STAGES + b); };
-  auto tempty = [&](int b) { return bar0 + 8u * (2 * STAGES + 2 + b); };
-  const uint32_t final_bar = bar0 + 8u * (2 * STAGES + 4);
-  const uint32_t amax_bar = bar0 + 8u * (2 * STAGES + 5);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + 2 * STAGES + 6);
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * STAGES + 6) + 1;
+  auto full = [&](int s) { return bar0 + 8u * s; };   // (the even CTA's)
+  auto empty = [&](int s) { return bar0 + 8u * (S + s); };
+  auto tfull = [&](int b) { return bar0 + 8u * (2 * S + b); };
+  auto tempty = [&](int b) { return bar0 + 8u * (2 * S + BUFS + b); };  // (the even CTA's)
+  auto sfull = [&](int l) { return bar0 + 8u * (2 * S + 2 * BUFS + l); };
+  const uint32_t final_bar = bar0 + 8u * (2 * S + 2 * BUFS + SL);
+  const uint32_t amax_bar = final_bar + 8u;
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + C::BARS);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + C::BARS) + 1;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = p.splits * CTAS > 1 ? (int)cluster_rank() : 0;
+  const int r = rank % CTAS, slice = rank / CTAS;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < STAGES; ++s) {
+    for (int s = 0; s < S; ++s) {
       mbar_init(full(s), 1);
       mbar_init(empty(s), 1);
     }
-    for (int b = 0; b < 2; ++b) {
-      mbar_init(tfull(b), 1);
-      mbar_init(tempty(b), EPI_THREADS / 32);
+    for (int b = 0; b < BUFS; ++b) {
+      mbar_init(tfull(b), 1 + 2);  // the product's commit and the two scale warps
+      mbar_init(tempty(b), CTAS * EPI_THREADS / 32);
     }
+    for (int l = 0; l < SL; ++l) mbar_init(sfull(l), 1);
     mbar_init(final_bar, 1);
     mbar_init(amax_bar, EPI_THREADS / 32);
     *abort_flag = 0;
     fence_barrier_init();
   }
-  if (warp == 1) tmem_alloc(smem_u32(tmem_slot), 512);
+  if (warp == 1) tmem_alloc<CTAS>(smem_u32(tmem_slot), BUFS * BN);
   fence_before();
   __syncthreads();
+  if constexpr (CTAS == 2) {  // both CTAs' barriers are initialised before any load, commit or arrival reaches them
+    cluster_arrive();
+    cluster_wait();
+  }
   fence_after();
   const uint32_t tmem = *tmem_slot;
   pdl_trigger();
 
   const int tiles = p.tiles_m * p.tiles_n;
-  const int slice = p.splits > 1 ? (int)cluster_rank() : 0;
-  const int t0 = blockIdx.x / p.splits, dt = gridDim.x / p.splits;
+  const int t0 = blockIdx.x / (p.splits * CTAS), dt = gridDim.x / (p.splits * CTAS);
   const int kb0 = slice * p.kb_per_split;
   const int nkb = max(0, min(p.num_kb - kb0, p.kb_per_split));
   if (warp < 4) {
@@ -285,10 +320,11 @@ __global__ void __launch_bounds__(THREADS, 1)
       // ---------------------------------------------------------------- producer
       prefetch_map(&map_x);
       prefetch_map(&map_w);
+      prefetch_map(&map_s);
       if (t0 < tiles) {  // into L2 only, ahead of the previous kernel's end
         int tm, tn;
         tile_coords(p, t0, tm, tn);
-        for (int i = 0; i < min(nkb, STAGES); ++i) tma_prefetch_2d(&map_w, (kb0 + i) * BK, tn * BN);
+        for (int i = 0; i < min(nkb, S); ++i) tma_prefetch_2d(&map_w, (kb0 + i) * BK, tn * BN + r * C::B_ROWS);
       }
       pdl_wait();
       uint32_t it = 0;
@@ -296,48 +332,92 @@ __global__ void __launch_bounds__(THREADS, 1)
       for (int t = t0; t < tiles && ok; t += dt) {
         int tm, tn;
         tile_coords(p, t, tm, tn);
+        const int row0 = (tm * CTAS + r) * BM;
         for (int i = 0; i < nkb; ++i, ++it) {
-          const int s = it % STAGES;
-          if (!mbar_wait(empty(s), ((it / STAGES) & 1) ^ 1, abort_flag, &g_fp8_error, 501)) {
+          const int s = it % S, l = it % SL, k = (kb0 + i) * BK;
+          if (!mbar_wait(empty(s), ((it / S) & 1) ^ 1, abort_flag, &g_fp8_error, 501)) {
             ok = false;
             break;
           }
-          mbar_arrive_expect_tx(full(s), STAGE_BYTES);
-          const uint32_t st = smem_u32(smem + s * STAGE_BYTES);
-          tma_load_2d(st, &map_x, full(s), (kb0 + i) * BK, tm * BM);
-          tma_load_2d(st + A_BYTES, &map_w, full(s), (kb0 + i) * BK, tn * BN);
+          const uint32_t st = smem_u32(smem + s * C::STAGE);
+          if constexpr (CTAS == 1) {
+            mbar_arrive_expect_tx(full(s), C::STAGE);
+            tma_load_2d(st, &map_x, full(s), k, row0);
+            tma_load_2d(st + C::A_BYTES, &map_w, full(s), k, tn * BN);
+          } else {
+            if (r == 0) mbar_arrive_expect_tx(full(s), 2 * C::STAGE);
+            const uint32_t fb = cluster_map(full(s), rank - r);
+            tma_load_2d_pair(st, &map_x, fb, k, row0);
+            tma_load_2d_pair(st + C::A_BYTES, &map_w, fb, k, tn * BN + r * C::B_ROWS);
+          }
+          // Slot l was last read, by the scale warps, for k-block it - SL.  Stage s is free, so k-block
+          // it - S has been multiplied: its buffer was freed by the epilogue's reading k-block it - S -
+          // BUFS, for which the scale warps had arrived: no barrier of its own guards the slot.
+          mbar_arrive_expect_tx(sfull(l), BM * 4);
+          tma_load_2d(smem_u32(slots + l * BM), &map_s, sfull(l), row0, kb0 + i);
         }
       }
       if (!ok) {
-        const uint32_t n = it < (uint32_t)STAGES ? it : (uint32_t)STAGES;
-        for (uint32_t j = it - n; j < it; ++j) mbar_drain(full(j % STAGES), (j / STAGES) & 1);
-      }
-    } else if (warp == 1) {
-      // ---------------------------------------------------------------- MMA issuer
-      const uint32_t tbase = __shfl_sync(FULL_MASK, tmem, 0);
-      uint32_t it = 0;
-      bool ok = true;
-      for (int t = t0; t < tiles && ok; t += dt) {
-        for (int i = 0; i < nkb; ++i, ++it) {
-          const int s = it % STAGES, b = it & 1;
-          ok = warp_wait(full(s), (it / STAGES) & 1, abort_flag, 503) &&
-               warp_wait(tempty(b), ((it >> 1) & 1) ^ 1, abort_flag, 502);
-          if (!ok) break;
-          fence_after();
-          const uint32_t st = smem_u32(smem + s * STAGE_BYTES);
-          const uint64_t ad = sdesc(st), bd = sdesc(st + A_BYTES);
-          if (elect_one()) {
-#pragma unroll
-            for (int k = 0; k < BK / 32; ++k)
-              mma_f8(tbase + b * BN, ad + 2 * k, bd + 2 * k, idesc_f8(BM, BN), k > 0 ? 1u : 0u);
-            commit(empty(s));
-            commit(tfull(b));
-          }
-          __syncwarp();
+        const uint32_t n = it < (uint32_t)S ? it : (uint32_t)S;
+        for (uint32_t j = it - n; j < it; ++j) {
+          if (r == 0) mbar_drain(full(j % S), (j / S) & 1);
+          mbar_drain(sfull(j % SL), (j / SL) & 1);
         }
       }
-      if (elect_one()) commit(final_bar);
+    } else if (warp == 1 && r == 0) {
+      // ---------------------------------------------------------------- MMA issuer (a pair's even CTA)
+      const uint32_t tbase = __shfl_sync(FULL_MASK, tmem, 0);
+      const uint32_t both = 3u << (rank - r);  // the pair's ranks in the cluster
+      const uint32_t total = (uint32_t)nkb * (t0 < tiles ? (tiles - t0 + dt - 1) / dt : 0);
+      for (uint32_t it = 0; it < total; ++it) {
+        const int s = it % S, b = it % BUFS;
+        if (!warp_wait(full(s), (it / S) & 1, abort_flag, 503) ||
+            !warp_wait(tempty(b), ((it / BUFS) & 1) ^ 1, abort_flag, 502))
+          break;
+        fence_after();
+        const uint32_t st = smem_u32(smem + s * C::STAGE);
+        const uint64_t ad = sdesc(st), bd = sdesc(st + C::A_BYTES);
+        if (elect_one()) {
+#pragma unroll
+          for (int k = 0; k < BK / 32; ++k)
+            mma_f8<CTAS>(tbase + b * BN, ad + 2 * k, bd + 2 * k, idesc_f8(CTAS * BM, BN), k > 0 ? 1u : 0u);
+          commit<CTAS>(empty(s), both);
+          commit<CTAS>(tfull(b), both);
+        }
+        __syncwarp();
+      }
+      if (elect_one()) commit<CTAS>(final_bar, both);
       if (lane == 0) mbar_drain(final_bar, 0);
+    } else if (warp >= 2) {
+      // ---------------------------------------------------------------- scales of weight block warp - 2
+      // Each k-block's products of activation and weight scale, so that the epilogue has one barrier to
+      // wait for and one number per column half to load.
+      pdl_wait();
+      uint32_t it = 0;
+      int sl = 0, sp = 0;  // scale slot of k-block `it` and its phase
+      bool ok = true;
+      for (int t = t0; t < tiles && ok; t += dt) {
+        int tm, tn;
+        tile_coords(p, t, tm, tn);
+        WeightScales ws(p.ws + (int64_t)min(2 * tn + warp - 2, p.nb - 1) * p.ldws + kb0, nkb, lane);
+        for (int kb = 0; kb < nkb; ++kb, ++it) {
+          const float w = ws.at(kb);
+          // The product of k-block it - 2 has landed: the arrival below belongs to the next phase of its
+          // barrier, and the epilogue has read the scales of it - 4 (it freed that buffer for it - 2).
+          ok = warp_wait(sfull(sl), sp, abort_flag, 506) &&
+               (it < 2 || warp_wait(tfull(it & 1), ((it - 2) >> 1) & 1, abort_flag, 507));
+          if (!ok) break;
+          float4 x = reinterpret_cast<const float4*>(slots + sl * BM)[lane];
+          x.x *= w; x.y *= w; x.z *= w; x.w *= w;
+          reinterpret_cast<float4*>(prods + ((it & 3) * 2 + warp - 2) * BM)[lane] = x;
+          __syncwarp();
+          if (lane == 0) mbar_arrive_release(tfull(it & 1));
+          if (++sl == SL) {
+            sl = 0;
+            sp ^= 1;
+          }
+        }
+      }
     }
     __syncwarp();
     if (p.splits > 1) {
@@ -350,98 +430,95 @@ __global__ void __launch_bounds__(THREADS, 1)
     // ------------------------------------------------------------------ epilogue
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(EPI_REGS));
     const int q4 = warp & 3, wg = (warp - 4) >> 2;
-    const int r = q4 * 32 + lane;  // this thread's token in the tile
+    const int lt = q4 * 32 + lane;  // this thread's token of the CTA's 128
     const uint32_t ta0 = tmem + ((uint32_t)(q4 * 32) << 16) + wg * 64;
-    auto landed = [&](uint32_t it) {  // the product of k-block `it` is in its buffer
-      const bool ok = warp_wait(tfull(it & 1), (it >> 1) & 1, abort_flag, 504);
-      fence_after();
-      return ok;
-    };
-    uint64_t acc[2][32];
+    // (in the cluster's window for one CTA too: an arrival that returns no state is not waited for)
+    const uint32_t te0 = cluster_map(tempty(0), rank - r);
+    float acc[2][64];
     uint32_t it = 0, tile_parity = 0;
     bool ok = true;
     pdl_wait();
     for (int t = t0; t < tiles; t += dt, tile_parity ^= 1) {
       int tm, tn;
       tile_coords(p, t, tm, tn);
-      const int row = tm * BM + r;
-      const float* xs = p.xs + (int64_t)kb0 * p.ldxs + row;
-      const float* ws0 = p.ws + (int64_t)(2 * tn) * p.ldws + kb0;
-      const float* ws1 = p.ws + (int64_t)min(2 * tn + 1, p.nb - 1) * p.ldws + kb0;
+      const int row = (tm * CTAS + r) * BM + lt;
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int i = 0; i < 32; ++i) acc[h][i] = 0;
+        for (int i = 0; i < 64; ++i) acc[h][i] = 0.f;
       if (nkb > 0) {
-        float x_n = row < p.T ? xs[0] : 0.f, w0_n = ws0[0], w1_n = ws1[0];
-        // 4 loads of 32 columns (2 of each half) per k-block, the next one in flight while one is added
+        // A k-block is 4 loads of 32 columns, 2 of each half, through two register buffers.  The loads of
+        // the next half are issued between the additions of this one, across k-blocks too; the buffer goes
+        // back to the tensor core before its second half is added.
         uint32_t v[2][32];
-        ok = landed(it);
+        ok = warp_wait(tfull(it & 1), (it >> 1) & 1, abort_flag, 504);
         if (!ok) break;
+        fence_after();
+        float s0 = prods[(it & 3) * 2 * BM + lt], s1 = prods[(it & 3) * 2 * BM + BM + lt];
         tmem_ld(ta0 + (it & 1) * BN, v[0]);
+        tmem_ld(ta0 + (it & 1) * BN + 32, v[1]);
         for (int kb = 0; kb < nkb; ++kb, ++it) {
-          const float s0 = x_n * w0_n, s1 = x_n * w1_n;
-          const uint64_t sc[2] = {pack2(s0, s0), pack2(s1, s1)};
-          if (kb + 1 < nkb) {
-            x_n = row < p.T ? xs[(int64_t)(kb + 1) * p.ldxs] : 0.f;
-            w0_n = ws0[kb + 1];
-            w1_n = ws1[kb + 1];
+          const bool more = kb + 1 < nkb;
+          const uint32_t ta = ta0 + (it & 1) * BN + 128, nx = ta0 + ((it + 1) & 1) * BN;
+          const float sb = s1;
+          ld_wait(v[0]);
+          ld_wait(v[1]);
+          add32(acc[0], v[0], s0);
+          tmem_ld(ta, v[0]);
+          add32(acc[0] + 32, v[1], s0);
+          tmem_ld(ta + 32, v[1]);
+          ld_wait(v[0]);
+          ld_wait(v[1]);
+          fence_before();
+          __syncwarp();
+          // this buffer has been read: the tensor core may overwrite it
+          if (lane == 0) mbar_arrive_cluster(te0 + 8u * (it & 1));
+          add32(acc[1], v[0], sb);
+          if (more) {
+            ok = warp_wait(tfull((it + 1) & 1), ((it + 1) >> 1) & 1, abort_flag, 504);
+            if (!ok) break;
+            fence_after();
+            tmem_ld(nx, v[0]);
+            const float* pr = prods + ((it + 1) & 3) * 2 * BM + lt;
+            s0 = pr[0];
+            s1 = pr[BM];
           }
-          const uint32_t ta = ta0 + (it & 1) * BN;
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            ld_wait(v[c & 1]);
-            if (c < 3) {
-              tmem_ld(ta + ((c + 1) >> 1) * 128 + ((c + 1) & 1) * 32, v[(c + 1) & 1]);
-            } else {  // this buffer has been read: the tensor core may overwrite it
-              fence_before();
-              __syncwarp();
-              if (lane == 0) mbar_arrive(tempty(it & 1));
-              if (kb + 1 < nkb) {
-                ok = landed(it + 1);
-                if (!ok) break;
-                tmem_ld(ta0 + ((it + 1) & 1) * BN, v[0]);
-              }
-            }
-            add32(acc[c >> 1] + (c & 1) * 16, v[c & 1], sc[c >> 1]);
-          }
-          if (!ok) break;
+          add32(acc[1] + 32, v[1], sb);
+          if (more) tmem_ld(nx + 32, v[1]);
         }
         if (!ok) break;
       }
       if (p.splits > 1) break;  // one tile per cluster; finished below
       if (!p.act) {
-        store_bf16_64(p, row, tn * BN + wg * 64, acc[0]);
-        store_bf16_64(p, row, tn * BN + 128 + wg * 64, acc[1]);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          store_bf16_32(p, row, tn * BN + h * 128 + wg * 64, acc[h]);
+          store_bf16_32(p, row, tn * BN + h * 128 + wg * 64 + 32, acc[h] + 32);
+        }
       } else {
-        // the sums stay fp32 up to the 8-bit rounding
-        const int f0 = tn * 128 + wg * 64;
-        float h[64];
+        // SiLU-and-mul; the values stay fp32 up to the 8-bit rounding
+        const int f = tn * 128 + wg * 64;
         uint32_t m = 0;
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          const float2 g = unpack2(acc[0][i]), u = unpack2(acc[1][i]);
-          h[2 * i] = f0 + 2 * i < p.features ? silu_f(g.x) * u.x : 0.f;
-          h[2 * i + 1] = f0 + 2 * i + 1 < p.features ? silu_f(g.y) * u.y : 0.f;
-          m = max(m, max(__float_as_uint(h[2 * i]) & 0x7fffffffu, __float_as_uint(h[2 * i + 1]) & 0x7fffffffu));
+        for (int i = 0; i < 64; ++i) {
+          acc[0][i] = f + i < p.features ? silu_f(acc[0][i]) * acc[1][i] : 0.f;
+          m = max(m, __float_as_uint(acc[0][i]) & 0x7fffffffu);
         }
         // the other half of the group of 128 belongs to the other warpgroup's thread of this token;
         // two buffers: a warp may be one tile ahead of the reader of the one before
-        uint32_t* am = amax + tile_parity * 2 * BM + r;
+        uint32_t* am = amax + tile_parity * 2 * BM + lt;
         am[wg * BM] = m;
         __syncwarp();
-        if (lane == 0) mbar_arrive(amax_bar);
+        if (lane == 0) mbar_arrive_release(amax_bar);
         ok = warp_wait(amax_bar, tile_parity, abort_flag, 505);
         if (!ok) break;
         const Fp8Scale sc = fp8_scale(max(m, am[(wg ^ 1) * BM]));
         if (row < p.T) {
-          uint8_t* dst = static_cast<uint8_t*>(p.out) + (int64_t)row * p.ldo + f0;
+          uint8_t* dst = static_cast<uint8_t*>(p.out) + (int64_t)row * p.ldo + f;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            if (f0 + 16 * i < p.features) {
-              const uint2 a = f32x8_to_e4m3(h + 16 * i, sc.inv), b2 = f32x8_to_e4m3(h + 16 * i + 8, sc.inv);
-              *reinterpret_cast<uint4*>(dst + 16 * i) = make_uint4(a.x, a.y, b2.x, b2.y);
-            }
+          for (int i = 0; i < 64; i += 16) {
+            const uint2 a = f32x8_to_e4m3(acc[0] + i, sc.inv), b = f32x8_to_e4m3(acc[0] + i + 8, sc.inv);
+            if (f + i < p.features) *reinterpret_cast<uint4*>(dst + i) = make_uint4(a.x, a.y, b.x, b.y);
           }
           if (wg == 0) p.os[(int64_t)tn * p.ldos + row] = sc.scale;
         }
@@ -450,23 +527,23 @@ __global__ void __launch_bounds__(THREADS, 1)
     __syncwarp();
     if (p.splits > 1) {
       // Every CTA lays its sums out in its own shared memory, over its idle ring (the last MMA has
-      // completed), [token][feature]; after the cluster's barrier CTA s finishes 128 / splits tokens.
+      // completed), [token][feature]; after the cluster's barrier each slice finishes its share.
       int tm, tn;
       tile_coords(p, t0, tm, tn);
-      float* dst = exchange + r * XLD + wg * 64;
+      float* dst = exchange + lt * XLD + wg * 64;
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float2 a = unpack2(acc[h][2 * i]), b = unpack2(acc[h][2 * i + 1]);
-          *reinterpret_cast<float4*>(dst + h * 128 + 4 * i) = make_float4(a.x, a.y, b.x, b.y);
-        }
+        for (int i = 0; i < 64; i += 4)
+          *reinterpret_cast<float4*>(dst + h * 128 + i) =
+              make_float4(acc[h][i], acc[h][i + 1], acc[h][i + 2], acc[h][i + 3]);
       cluster_arrive();
       cluster_wait();  // every slice's sums are laid out
       if (!*abort_flag) {
-        if (p.splits == 2) finish_rows<2>(p, exchange, slice, tm, tn, warp - 4, lane);
-        else if (p.splits == 4) finish_rows<4>(p, exchange, slice, tm, tn, warp - 4, lane);
-        else finish_rows<8>(p, exchange, slice, tm, tn, warp - 4, lane);
+        const int row0 = (tm * CTAS + r) * BM;
+        if (p.splits == 2) finish_rows<CTAS, 2>(p, exchange, slice, r, row0, tn, warp - 4, lane);
+        else if (p.splits == 4) finish_rows<CTAS, 4>(p, exchange, slice, r, row0, tn, warp - 4, lane);
+        else finish_rows<CTAS, 8>(p, exchange, slice, r, row0, tn, warp - 4, lane);
       }
       cluster_arrive();
       cluster_wait();  // nobody reads this CTA's shared memory any more
@@ -475,9 +552,13 @@ __global__ void __launch_bounds__(THREADS, 1)
   __syncwarp();
   fence_before();
   __syncthreads();
+  if constexpr (CTAS == 2) {  // the pair's MMAs, loads, commits and arrivals are done before TMEM is freed
+    cluster_arrive();
+    cluster_wait();
+  }
   if (warp == 1) {
     fence_after();
-    tmem_dealloc(tmem, 512);
+    tmem_dealloc<CTAS>(tmem, BUFS * BN);
   }
 }
 
@@ -526,7 +607,7 @@ __global__ void __launch_bounds__(WeightsCfg<NP>::THREADS, 2)
     *abort_flag = 0;
     fence_barrier_init();
   }
-  if (warp == 1) tmem_alloc(smem_u32(tmem_slot), C::TMEM_COLS);
+  if (warp == 1) tmem_alloc<1>(smem_u32(tmem_slot), C::TMEM_COLS);
   fence_before();
   __syncthreads();
   fence_after();
@@ -586,35 +667,33 @@ __global__ void __launch_bounds__(WeightsCfg<NP>::THREADS, 2)
       if (elect_one()) {
 #pragma unroll
         for (int k = 0; k < BK / 32; ++k)
-          mma_f8(tbase + b * NP, wd + 2 * k, xd + 2 * k, idesc_f8(128, NP), k > 0 ? 1u : 0u);
-        commit(empty(s));
-        commit(tfull(b));
+          mma_f8<1>(tbase + b * NP, wd + 2 * k, xd + 2 * k, idesc_f8(128, NP), k > 0 ? 1u : 0u);
+        commit<1>(empty(s));
+        commit<1>(tfull(b));
       }
       __syncwarp();
     }
-    if (elect_one()) commit(final_bar);
+    if (elect_one()) commit<1>(final_bar);
     if (lane == 0) mbar_drain(final_bar, 0);
     __syncwarp();
   } else if (warp >= 2) {
     // ------------------------------------------------------------------ epilogue
     const int q4 = warp & 3, cs = (warp - 2) >> 2;  // lane quarter, share of the tokens
     const int blk = p.act ? 2 * tile + (q4 >> 1) : tile;  // this warp's 128-row block of W
-    const float* ws = p.ws + (int64_t)min(blk, p.nb - 1) * p.ldws + kb0;
-    uint64_t acc[C::NC / 2];
+    float acc[C::NC];
 #pragma unroll
-    for (int i = 0; i < C::NC / 2; ++i) acc[i] = 0;
+    for (int i = 0; i < C::NC; ++i) acc[i] = 0.f;
     pdl_wait();
-    float w_n = nkb > 0 ? ws[0] : 0.f;
+    WeightScales ws(p.ws + (int64_t)min(blk, p.nb - 1) * p.ldws + kb0, nkb, lane);
     bool ok = true;
     for (int i = 0; i < nkb; ++i) {
-      const uint64_t wsc = pack2(w_n, w_n);
-      if (i + 1 < nkb) w_n = ws[i + 1];
+      const float wsc = ws.at(i);
       const int b = i % NB, l = i % SL;
       ok = warp_wait(sfull(l), (i / SL) & 1, abort_flag, 514) && warp_wait(tfull(b), (i / NB) & 1, abort_flag, 515);
       if (!ok) break;
       fence_after();
       const uint32_t ta = tmem + ((uint32_t)(q4 * 32) << 16) + b * NP + cs * C::NC;
-      const ulonglong2* xs = reinterpret_cast<const ulonglong2*>(slots + l * C::SLOT) + cs * (C::NC / 4);
+      const float4* xs = reinterpret_cast<const float4*>(slots + l * C::SLOT) + cs * (C::NC / 4);
 #pragma unroll
       for (int c = 0; c < C::NC / C::CHUNK; ++c) {
         uint32_t v[C::CHUNK];
@@ -623,15 +702,16 @@ __global__ void __launch_bounds__(WeightsCfg<NP>::THREADS, 2)
         if (c + 1 == C::NC / C::CHUNK) {  // this buffer has been read: the tensor core may overwrite it
           fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(tempty(b));
+          if (lane == 0) mbar_arrive_cluster(cluster_map(tempty(b), rank));
         }
 #pragma unroll
         for (int j = 0; j < C::CHUNK / 4; ++j) {
-          const ulonglong2 sx = xs[c * (C::CHUNK / 4) + j];  // 4 tokens' scales, the same for every lane
-          uint64_t& a0 = acc[c * (C::CHUNK / 2) + 2 * j];
-          uint64_t& a1 = acc[c * (C::CHUNK / 2) + 2 * j + 1];
-          a0 = fma2(pack2(v[4 * j], v[4 * j + 1]), mul2(sx.x, wsc), a0);
-          a1 = fma2(pack2(v[4 * j + 2], v[4 * j + 3]), mul2(sx.y, wsc), a1);
+          const float4 sx = xs[c * (C::CHUNK / 4) + j];  // 4 tokens' scales, the same for every lane
+          float* a = acc + c * C::CHUNK + 4 * j;
+          a[0] = fmaf(__uint_as_float(v[4 * j]), sx.x * wsc, a[0]);
+          a[1] = fmaf(__uint_as_float(v[4 * j + 1]), sx.y * wsc, a[1]);
+          a[2] = fmaf(__uint_as_float(v[4 * j + 2]), sx.z * wsc, a[2]);
+          a[3] = fmaf(__uint_as_float(v[4 * j + 3]), sx.w * wsc, a[3]);
         }
       }
     }
@@ -648,13 +728,11 @@ __global__ void __launch_bounds__(WeightsCfg<NP>::THREADS, 2)
 #pragma unroll
     for (int c = 0; c < C::NC; ++c)
       if (cs * C::NC + c < p.T) {
-        const float2 a = unpack2(acc[c / 2]);
-        const float v = c & 1 ? a.y : a.x;
         float* dst = exchange + (slice * per + tl) * width + f;
         if (p.cluster > 1)
-          st_cluster_f32(cluster_map(smem_u32(dst), owner), v);
+          st_cluster_f32(cluster_map(smem_u32(dst), owner), acc[c]);
         else
-          *dst = v;
+          *dst = acc[c];
         if (++owner == p.cluster) {
           owner = 0;
           ++tl;
@@ -699,7 +777,7 @@ __global__ void __launch_bounds__(WeightsCfg<NP>::THREADS, 2)
   }
   if (warp == 1) {
     fence_after();
-    tmem_dealloc(tmem, C::TMEM_COLS);
+    tmem_dealloc<1>(tmem, C::TMEM_COLS);
   }
 }
 
@@ -763,14 +841,16 @@ cudaLaunchConfig_t cluster_config(int grid, int threads, int smem, int cluster, 
 
 // Shared-memory opt-in, and the check that the kernel is launched with the registers that its
 // warps redistribute (fewer would leave the epilogue waiting for them).
+template <int CTAS>
 cudaError_t tokens_opt_in() {
   static std::atomic<uint64_t> done{0};
   return once_per_device(done, []() -> cudaError_t {
     cudaFuncAttributes a;
-    cudaError_t e = cudaFuncGetAttributes(&a, gemm_fp8_tokens_kernel);
+    cudaError_t e = cudaFuncGetAttributes(&a, gemm_fp8_tokens_kernel<CTAS>);
     if (e != cudaSuccess) return e;
     if (a.numRegs < LAUNCH_REGS) return cudaErrorInvalidDeviceFunction;
-    return cudaFuncSetAttribute(gemm_fp8_tokens_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_TOKENS);
+    return cudaFuncSetAttribute(gemm_fp8_tokens_kernel<CTAS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                TokensCfg<CTAS>::SMEM);
   });
 }
 
@@ -787,11 +867,11 @@ int clusters_of_sms(int cluster, int num_sms) {
   if (cluster == 1) return num_sms;
   if (int c = cache[cluster].load(std::memory_order_relaxed)) return c;
   cudaLaunchAttribute attr[2];
-  cudaLaunchConfig_t cfg = cluster_config(64 * cluster, THREADS, SMEM_TOKENS, cluster, attr);
+  cudaLaunchConfig_t cfg = cluster_config(64 * cluster, THREADS, TokensCfg<1>::SMEM, cluster, attr);
   cfg.numAttrs = 1;
   int n = 0;
-  if (tokens_opt_in() != cudaSuccess ||
-      cudaOccupancyMaxActiveClusters(&n, gemm_fp8_tokens_kernel, &cfg) != cudaSuccess || n <= 0) {
+  if (tokens_opt_in<1>() != cudaSuccess ||
+      cudaOccupancyMaxActiveClusters(&n, gemm_fp8_tokens_kernel<1>, &cfg) != cudaSuccess || n <= 0) {
     cudaGetLastError();
     return num_sms / cluster;
   }
@@ -830,6 +910,31 @@ cudaError_t run_weights(const Fp8Gemm& g, Params p, int splits, cudaStream_t str
   return cudaLaunchKernelEx(&cfg, gemm_fp8_weights_kernel<NP>, mx, mw, ms, p);
 }
 
+template <int CTAS>
+cudaError_t run_tokens(const Fp8Gemm& g, Params p, int splits, int num_sms, cudaStream_t stream) {
+  using C = TokensCfg<CTAS>;
+  if ((splits != 1 && splits != 2 && splits != 4 && splits != 8) || splits * CTAS > 8)
+    return cudaErrorInvalidValue;
+  CUtensorMap mx, mw, ms;
+  if (!make_map(&mx, g.xq, g.T, g.K, g.ldx, BM) || !make_map(&mw, g.wq, g.N, g.K, g.ldw, C::B_ROWS) ||
+      !make_scale_map(&ms, g.xs, p.num_kb, g.T, g.ldxs, BM))
+    return cudaErrorInvalidValue;
+  p.tiles_m = (g.T + CTAS * BM - 1) / (CTAS * BM);
+  p.tiles_n = (g.N + BN - 1) / BN;
+  p.group = 16 / CTAS;
+  const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n;
+  if (tiles > 0x7fffffff / 16) return cudaErrorInvalidValue;
+  p.splits = splits;
+  p.kb_per_split = (p.num_kb + splits - 1) / splits;
+  cudaError_t e = tokens_opt_in<CTAS>();
+  if (e != cudaSuccess) return e;
+  const int64_t most = splits > 1 ? tiles : std::min<int64_t>(tiles, clusters_of_sms(CTAS, num_sms));
+  cudaLaunchAttribute attr[2];
+  cudaLaunchConfig_t cfg = cluster_config((int)most * splits * CTAS, THREADS, C::SMEM, splits * CTAS, attr);
+  cfg.stream = stream;
+  return cudaLaunchKernelEx(&cfg, gemm_fp8_tokens_kernel<CTAS>, mx, mw, ms, p);
+}
+
 }  // namespace
 
 Fp8Plan fp8_plan(int T, int N, int K, int act, int num_sms) {
@@ -842,9 +947,11 @@ Fp8Plan fp8_plan(int T, int N, int K, int act, int num_sms) {
     for (int s = 2; s * halves <= 8; ++s)
       if (num_kb / s >= 2 && tiles <= clusters_of_half_sms(s * halves, num_sms)) pl.splits = s;
   } else {
-    const int64_t tiles = (int64_t)((T + BM - 1) / BM) * ((N + BN - 1) / BN);
+    const int ctas = T > 128 ? 2 : 1;
+    pl.np = -ctas;
+    const int64_t tiles = (int64_t)((T + ctas * BM - 1) / (ctas * BM)) * ((N + BN - 1) / BN);
     for (int s = 2; s <= 4; s *= 2)
-      if (num_kb / s >= 4 && tiles <= clusters_of_sms(s, num_sms)) pl.splits = s;
+      if (num_kb / s >= 4 && tiles <= clusters_of_sms(s * ctas, num_sms)) pl.splits = s;
   }
   return pl;
 }
@@ -852,17 +959,12 @@ Fp8Plan fp8_plan(int T, int N, int K, int act, int num_sms) {
 cudaError_t gemm_fp8(const Fp8Gemm& g, const Fp8Plan& pl, int num_sms, cudaStream_t stream) {
   if (g.T == 0 || g.N == 0) return cudaSuccess;
   Params p{};
-  p.xs = g.xs;
   p.ws = g.ws;
-  p.ldxs = g.ldxs;
   p.ldws = g.ldws;
   p.T = g.T;
   p.N = g.N;
   p.num_kb = (g.K + BK - 1) / BK;
   p.nb = (g.N + FP8_GROUP - 1) / FP8_GROUP;
-  p.tiles_m = (g.T + BM - 1) / BM;
-  p.tiles_n = (g.N + BN - 1) / BN;
-  p.group = 16;
   p.act = g.act;
   p.features = g.features;
   p.out = g.out;
@@ -871,27 +973,13 @@ cudaError_t gemm_fp8(const Fp8Gemm& g, const Fp8Plan& pl, int num_sms, cudaStrea
   p.ldos = g.ldos;
   p.vec = g.ldo % 8 == 0 && (reinterpret_cast<uintptr_t>(g.out) & 15) == 0;
   switch (pl.np) {
-    case 0: break;
+    case -1: return run_tokens<1>(g, p, pl.splits, num_sms, stream);
+    case -2: return run_tokens<2>(g, p, pl.splits, num_sms, stream);
     case 16: return run_weights<16>(g, p, pl.splits, stream);
     case 32: return run_weights<32>(g, p, pl.splits, stream);
     case 64: return run_weights<64>(g, p, pl.splits, stream);
     default: return cudaErrorInvalidValue;
   }
-  if (pl.splits != 1 && pl.splits != 2 && pl.splits != 4 && pl.splits != 8) return cudaErrorInvalidValue;
-  CUtensorMap mx, mw;
-  if (!make_map(&mx, g.xq, g.T, g.K, g.ldx, BM) || !make_map(&mw, g.wq, g.N, g.K, g.ldw, BN))
-    return cudaErrorInvalidValue;
-  const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n;
-  if (tiles > 0x7fffffff / 16) return cudaErrorInvalidValue;
-  p.splits = pl.splits;
-  p.kb_per_split = (p.num_kb + pl.splits - 1) / pl.splits;
-  cudaError_t e = tokens_opt_in();
-  if (e != cudaSuccess) return e;
-  const int grid = pl.splits > 1 ? (int)tiles * pl.splits : tiles < num_sms ? (int)tiles : num_sms;
-  cudaLaunchAttribute attr[2];
-  cudaLaunchConfig_t cfg = cluster_config(grid, THREADS, SMEM_TOKENS, pl.splits, attr);
-  cfg.stream = stream;
-  return cudaLaunchKernelEx(&cfg, gemm_fp8_tokens_kernel, mx, mw, p);
 }
 
 int gemm_fp8_error_code(int reset) {
