@@ -60,9 +60,11 @@ struct TokensCfg {
   static constexpr int B_ROWS = BN / CTAS;  // weight rows staged by one CTA
   static constexpr int A_BYTES = BM * BK, STAGE = A_BYTES + B_ROWS * BK;  // 48 or 32 KB
   static constexpr int STAGES = CTAS == 2 ? 6 : 4;
+  static constexpr int STAGING = EPI_THREADS / 32 * 2048;
   static constexpr int SLOTS = STAGES + BUFS + 1;  // activation scales of one k-block each: see the producer
   static constexpr int BARS = 2 * STAGES + 2 * BUFS + SLOTS + 2;
-  static constexpr int SMEM = 1024 + STAGES * STAGE + SLOTS * BM * 4 + 4 * 2 * BM * 4 + 2 * 2 * BM * 4 + 8 * BARS + 16;
+  static constexpr int SMEM = 1024 + STAGES * STAGE + STAGING + SLOTS * BM * 4 + 4 * 2 * BM * 4 + 2 * 2 * BM * 4 + 8 * BARS + 16;
+  static_assert(SMEM <= 227 * 1024, "shared memory of a CTA");
   static_assert(BM * XLD * 4 <= STAGES * STAGE, "the exchange fits over the ring");
 };
 
@@ -115,7 +117,8 @@ struct Params {
   int64_t ldws;
   int T, N, num_kb, nb;      // nb: 128-row blocks of W
   int tiles_m, tiles_n, group;
-  int act, features, vec;    // vec: bf16 rows allow 16-byte stores
+  int act, features;
+  int vec, tma_out;          // bf16 rows allow 16-byte stores; the output is stored by TMA
   void* out;
   int64_t ldo;
   float* os;
@@ -134,8 +137,15 @@ __device__ __forceinline__ void tile_coords(const Params& p, int t, int& tm, int
   tn = r / size;
 }
 
-// __expf is within 2 + 1.2 |g| units and __fdividef within 2: far inside the 8-bit rounding that follows.
-__device__ __forceinline__ float silu_f(float g) { return __fdividef(g, 1.f + __expf(-g)); }
+// g / (1 + e^-g) with e^-g = 2^(-g log2 e), by the approximate base-2 exponential and reciprocal (relative
+// errors of 2^-22 and 2^-23; the product -g log2 e adds |g| 2^-24): far inside the 8-bit rounding that
+// follows.  Subnormal results count as zero.
+__device__ __forceinline__ float silu_f(float g) {
+  float e, q;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(g * -1.44269504f));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(q) : "f"(1.f + e));
+  return g * q;
+}
 
 // bf16 values [c, c + 32) of one row.
 __device__ __forceinline__ void store_bf16_32(const Params& p, int row, int c, const float* acc) {
@@ -259,14 +269,15 @@ __device__ __forceinline__ void finish_rows(const Params& p, float* exchange, in
 template <int CTAS>
 __global__ void __launch_bounds__(THREADS, 1)
     gemm_fp8_tokens_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
-                           const __grid_constant__ CUtensorMap map_s, Params p) {
+                           const __grid_constant__ CUtensorMap map_s, const __grid_constant__ CUtensorMap map_o, Params p) {
   using C = TokensCfg<CTAS>;
   constexpr int S = C::STAGES, SL = C::SLOTS;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   // the same offset in every CTA of the cluster
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   float* exchange = reinterpret_cast<float*>(smem);  // over the idle ring (splits > 1)
-  float* slots = reinterpret_cast<float*>(smem + S * C::STAGE);
+  uint8_t* staging = smem + S * C::STAGE;  // 2 KB per epilogue warp: 64 bytes of 32 rows on their way out
+  float* slots = reinterpret_cast<float*>(staging + C::STAGING);
   float* prods = slots + SL * BM;  // [k-block & 3][weight block][token]: activation scale x weight scale
   uint32_t* amax = reinterpret_cast<uint32_t*>(prods + 4 * 2 * BM);  // [tile parity][half][token]
   uint64_t* bars = reinterpret_cast<uint64_t*>(amax + 2 * 2 * BM);
@@ -489,21 +500,51 @@ __global__ void __launch_bounds__(THREADS, 1)
         if (!ok) break;
       }
       if (p.splits > 1) break;  // one tile per cluster; finished below
+      // Each warp stores pieces of 32 rows x 64 bytes through shared memory by TMA, which writes whole
+      // sectors and drops what lies outside (stores of each thread's own row took 9000 clocks per tile,
+      // a quarter of it, as long as nothing overlaps them).
+      const int row0 = (tm * CTAS + r) * BM + q4 * 32;
+      uint8_t* mine = staging + (warp - 4) * 2048;
+      auto piece = [&](const uint4* w4, int col) {
+        if (lane == 0) bulk_wait_read();  // the piece before has left
+        __syncwarp();
+#pragma unroll
+        for (int c = 0; c < 4; ++c)  // 64-byte swizzle: no bank conflicts
+          *reinterpret_cast<uint4*>(mine + lane * 64 + (c ^ ((lane >> 1) & 3)) * 16) = w4[c];
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) {
+          tma_store_2d(&map_o, smem_u32(mine), col, row0);
+          bulk_commit();
+        }
+      };
       if (!p.act) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          store_bf16_32(p, row, tn * BN + h * 128 + wg * 64, acc[h]);
-          store_bf16_32(p, row, tn * BN + h * 128 + wg * 64 + 32, acc[h] + 32);
-        }
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const int col = tn * BN + h * 128 + wg * 64 + c * 32;
+            const float* a = acc[h] + c * 32;
+            if (p.tma_out) {
+              const uint4 w4[4] = {f32_to_bf16x8(a), f32_to_bf16x8(a + 8), f32_to_bf16x8(a + 16), f32_to_bf16x8(a + 24)};
+              if (row0 < p.T && col < p.N) piece(w4, col);
+            } else {
+              store_bf16_32(p, row, col, a);
+            }
+          }
       } else {
         // SiLU-and-mul; the values stay fp32 up to the 8-bit rounding
         const int f = tn * 128 + wg * 64;
         uint32_t m = 0;
 #pragma unroll
-        for (int i = 0; i < 64; ++i) {
-          acc[0][i] = f + i < p.features ? silu_f(acc[0][i]) * acc[1][i] : 0.f;
-          m = max(m, __float_as_uint(acc[0][i]) & 0x7fffffffu);
+        for (int i = 0; i < 64; ++i) acc[0][i] = silu_f(acc[0][i]) * acc[1][i];
+        if (f + 64 > p.features) {
+#pragma unroll
+          for (int i = 0; i < 64; ++i)
+            if (f + i >= p.features) acc[0][i] = 0.f;
         }
+#pragma unroll
+        for (int i = 0; i < 64; ++i) m = max(m, __float_as_uint(acc[0][i]) & 0x7fffffffu);
         // the other half of the group of 128 belongs to the other warpgroup's thread of this token;
         // two buffers: a warp may be one tile ahead of the reader of the one before
         uint32_t* am = amax + tile_parity * 2 * BM + lt;
@@ -513,17 +554,17 @@ __global__ void __launch_bounds__(THREADS, 1)
         ok = warp_wait(amax_bar, tile_parity, abort_flag, 505);
         if (!ok) break;
         const Fp8Scale sc = fp8_scale(max(m, am[(wg ^ 1) * BM]));
-        if (row < p.T) {
-          uint8_t* dst = static_cast<uint8_t*>(p.out) + (int64_t)row * p.ldo + f;
+        uint4 w4[4];
 #pragma unroll
-          for (int i = 0; i < 64; i += 16) {
-            const uint2 a = f32x8_to_e4m3(acc[0] + i, sc.inv), b = f32x8_to_e4m3(acc[0] + i + 8, sc.inv);
-            if (f + i < p.features) *reinterpret_cast<uint4*>(dst + i) = make_uint4(a.x, a.y, b.x, b.y);
-          }
-          if (wg == 0) p.os[(int64_t)tn * p.ldos + row] = sc.scale;
+        for (int i = 0; i < 4; ++i) {
+          const uint2 a = f32x8_to_e4m3(acc[0] + 16 * i, sc.inv), b = f32x8_to_e4m3(acc[0] + 16 * i + 8, sc.inv);
+          w4[i] = make_uint4(a.x, a.y, b.x, b.y);
         }
+        if (row0 < p.T && f < p.features) piece(w4, f);
+        if (wg == 0 && row < p.T) p.os[(int64_t)tn * p.ldos + row] = sc.scale;
       }
     }
+    if (lane == 0) bulk_wait();  // every piece has been written
     __syncwarp();
     if (p.splits > 1) {
       // Every CTA lays its sums out in its own shared memory, over its idle ring (the last MMA has
@@ -889,6 +930,20 @@ int clusters_of_half_sms(int cluster, int num_sms) {
                                      : clusters_of_sms(cluster / 2, num_sms));
 }
 
+// The output of the token-major kernel: bf16 [T, N] or e4m3 [T, features], pieces of 64 bytes x 32 rows.
+bool make_out_map(CUtensorMap* m, const Fp8Gemm& g) {
+  auto enc = get_encode();
+  if (!enc) return false;
+  const int bytes = g.act ? 1 : 2;
+  cuuint64_t dims[2] = {(cuuint64_t)(g.act ? g.features : g.N), (cuuint64_t)g.T};
+  cuuint64_t strides[1] = {(cuuint64_t)g.ldo * bytes};
+  cuuint32_t box[2] = {(cuuint32_t)(64 / bytes), 32};
+  cuuint32_t estr[2] = {1, 1};
+  return enc(m, g.act ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, g.out, dims, strides, box,
+             estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <int NP>
 cudaError_t run_weights(const Fp8Gemm& g, Params p, int splits, cudaStream_t stream) {
   const int cluster = splits * (g.act ? 2 : 1);
@@ -928,11 +983,14 @@ cudaError_t run_tokens(const Fp8Gemm& g, Params p, int splits, int num_sms, cuda
   p.kb_per_split = (p.num_kb + splits - 1) / splits;
   cudaError_t e = tokens_opt_in<CTAS>();
   if (e != cudaSuccess) return e;
+  CUtensorMap mo = mx;  // not used without p.tma_out
+  p.tma_out = g.act || p.vec;
+  if (p.tma_out && !make_out_map(&mo, g)) return cudaErrorInvalidValue;
   const int64_t most = splits > 1 ? tiles : std::min<int64_t>(tiles, clusters_of_sms(CTAS, num_sms));
   cudaLaunchAttribute attr[2];
   cudaLaunchConfig_t cfg = cluster_config((int)most * splits * CTAS, THREADS, C::SMEM, splits * CTAS, attr);
   cfg.stream = stream;
-  return cudaLaunchKernelEx(&cfg, gemm_fp8_tokens_kernel<CTAS>, mx, mw, ms, p);
+  return cudaLaunchKernelEx(&cfg, gemm_fp8_tokens_kernel<CTAS>, mx, mw, ms, mo, p);
 }
 
 }  // namespace

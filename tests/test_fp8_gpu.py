@@ -167,9 +167,9 @@ def test_linear_silu(ops, t, i, k):
     y, b = _exact(x, w).view(t, -1, 2, 128), _bound(x, w).view(t, -1, 2, 128)
     gate, up, gb, ub = (v.reshape(t, -1)[:, :i] for v in (y[:, :, 0], y[:, :, 1], b[:, :, 0], b[:, :, 1]))
     h = gate * torch.sigmoid(gate) * up
-    # |d silu| <= 1.1 |d gate|, silu <= |gate|; __expf is off by 2 + 1.2 |gate| units of 2^-23, the
-    # division by 2, the sum and the product by 1 each
-    err = 1.01 * _acc(k) * (1.1 * gb * up.abs() + gate.abs() * ub) + (2 * (2 + 1.2 * gate.abs()) + 6) * U * h.abs()
+    # |d silu| <= 1.1 |d gate|, silu <= |gate|; the exponential's argument is off by |gate| U, it by 4 U,
+    # the sum by U, the reciprocal by 2 U, two products by U each
+    err = 1.01 * _acc(k) * (1.1 * gb * up.abs() + gate.abs() * ub) + (gate.abs() + 9) * U * h.abs()
     kb = -(-i // 128)
     p = h.new_zeros(2, t, kb * 128)
     p[0, :, :i], p[1, :, :i] = h.abs(), err
