@@ -62,7 +62,7 @@ struct TokensCfg {
   static constexpr int STAGES = CTAS == 2 ? 6 : 4;
   static constexpr int STAGING = EPI_THREADS / 32 * 2048;
   static constexpr int SLOTS = STAGES + BUFS + 1;  // activation scales of one k-block each: see the producer
-  static constexpr int BARS = 2 * STAGES + 2 * BUFS + SLOTS + 2;
+  static constexpr int BARS = 2 * STAGES + BUFS + SLOTS + 2;
   static constexpr int SMEM = 1024 + STAGES * STAGE + STAGING + SLOTS * BM * 4 + 4 * 2 * BM * 4 + 2 * 2 * BM * 4 + 8 * BARS + 16;
   static_assert(SMEM <= 227 * 1024, "shared memory of a CTA");
   static_assert(BM * XLD * 4 <= STAGES * STAGE, "the exchange fits over the ring");
@@ -282,12 +282,14 @@ __global__ void __launch_bounds__(THREADS, 1)
   uint32_t* amax = reinterpret_cast<uint32_t*>(prods + 4 * 2 * BM);  // [tile parity][half][token]
   uint64_t* bars = reinterpret_cast<uint64_t*>(amax + 2 * 2 * BM);
   const uint32_t bar0 = smem_u32(bars);
-  auto full = [&](int s) { return bar0 + 8u * s; };   // (the even CTA's)
+  // go (the even CTA's): the operands of the k-block in this stage have landed and the epilogue warps have
+  // emptied its accumulator buffer.  One barrier for both: a poll costs the MMA warp 200 clocks or more
+  // beside the epilogue's additions, even when its answer is yes.
+  auto go = [&](int s) { return bar0 + 8u * s; };
   auto empty = [&](int s) { return bar0 + 8u * (S + s); };
   auto tfull = [&](int b) { return bar0 + 8u * (2 * S + b); };
-  auto tempty = [&](int b) { return bar0 + 8u * (2 * S + BUFS + b); };  // (the even CTA's)
-  auto sfull = [&](int l) { return bar0 + 8u * (2 * S + 2 * BUFS + l); };
-  const uint32_t final_bar = bar0 + 8u * (2 * S + 2 * BUFS + SL);
+  auto sfull = [&](int l) { return bar0 + 8u * (2 * S + BUFS + l); };
+  const uint32_t final_bar = bar0 + 8u * (2 * S + BUFS + SL);
   const uint32_t amax_bar = final_bar + 8u;
   volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + C::BARS);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + C::BARS) + 1;
@@ -297,12 +299,11 @@ __global__ void __launch_bounds__(THREADS, 1)
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < S; ++s) {
-      mbar_init(full(s), 1);
+      mbar_init(go(s), 1 + CTAS * EPI_THREADS / 32);
       mbar_init(empty(s), 1);
     }
     for (int b = 0; b < BUFS; ++b) {
       mbar_init(tfull(b), 1 + 2);  // the product's commit and the two scale warps
-      mbar_init(tempty(b), CTAS * EPI_THREADS / 32);
     }
     for (int l = 0; l < SL; ++l) mbar_init(sfull(l), 1);
     mbar_init(final_bar, 1);
@@ -352,14 +353,14 @@ __global__ void __launch_bounds__(THREADS, 1)
           }
           const uint32_t st = smem_u32(smem + s * C::STAGE);
           if constexpr (CTAS == 1) {
-            mbar_arrive_expect_tx(full(s), C::STAGE);
-            tma_load_2d(st, &map_x, full(s), k, row0);
-            tma_load_2d(st + C::A_BYTES, &map_w, full(s), k, tn * BN);
+            mbar_arrive_expect_tx(go(s), C::STAGE);
+            tma_load_2d(st, &map_x, go(s), k, row0);
+            tma_load_2d(st + C::A_BYTES, &map_w, go(s), k, tn * BN);
           } else {
-            if (r == 0) mbar_arrive_expect_tx(full(s), 2 * C::STAGE);
-            const uint32_t fb = cluster_map(full(s), rank - r);
-            tma_load_2d_pair(st, &map_x, fb, k, row0);
-            tma_load_2d_pair(st + C::A_BYTES, &map_w, fb, k, tn * BN + r * C::B_ROWS);
+            if (r == 0) mbar_arrive_expect_tx(go(s), 2 * C::STAGE);
+            const uint32_t gb = cluster_map(go(s), rank - r);
+            tma_load_2d_pair(st, &map_x, gb, k, row0);
+            tma_load_2d_pair(st + C::A_BYTES, &map_w, gb, k, tn * BN + r * C::B_ROWS);
           }
           // Slot l was last read, by the scale warps, for k-block it - SL.  Stage s is free, so k-block
           // it - S has been multiplied: its buffer was freed by the epilogue's reading k-block it - S -
@@ -371,7 +372,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       if (!ok) {
         const uint32_t n = it < (uint32_t)S ? it : (uint32_t)S;
         for (uint32_t j = it - n; j < it; ++j) {
-          if (r == 0) mbar_drain(full(j % S), (j / S) & 1);
+          if (r == 0) mbar_drain(go(j % S), (j / S) & 1);
           mbar_drain(sfull(j % SL), (j / SL) & 1);
         }
       }
@@ -380,22 +381,26 @@ __global__ void __launch_bounds__(THREADS, 1)
       const uint32_t tbase = __shfl_sync(FULL_MASK, tmem, 0);
       const uint32_t both = 3u << (rank - r);  // the pair's ranks in the cluster
       const uint32_t total = (uint32_t)nkb * (t0 < tiles ? (tiles - t0 + dt - 1) / dt : 0);
+      const uint64_t ad0 = sdesc(smem_u32(smem)), bd0 = sdesc(smem_u32(smem) + C::A_BYTES);
+      int s = 0, phase = 0;
       for (uint32_t it = 0; it < total; ++it) {
-        const int s = it % S, b = it % BUFS;
-        if (!warp_wait(full(s), (it / S) & 1, abort_flag, 503) ||
-            !warp_wait(tempty(b), ((it / BUFS) & 1) ^ 1, abort_flag, 502))
-          break;
+        if (!warp_wait(go(s), phase, abort_flag, 503)) break;
         fence_after();
-        const uint32_t st = smem_u32(smem + s * C::STAGE);
-        const uint64_t ad = sdesc(st), bd = sdesc(st + C::A_BYTES);
+        const uint32_t off = s * (C::STAGE >> 4);  // the descriptors count in 16 bytes
+        const uint64_t ad = ad0 + off, bd = bd0 + off;
+        const uint32_t d = tbase + (it & 1) * BN;
         if (elect_one()) {
 #pragma unroll
           for (int k = 0; k < BK / 32; ++k)
-            mma_f8<CTAS>(tbase + b * BN, ad + 2 * k, bd + 2 * k, idesc_f8(CTAS * BM, BN), k > 0 ? 1u : 0u);
+            mma_f8<CTAS>(d, ad + 2 * k, bd + 2 * k, idesc_f8(CTAS * BM, BN), k > 0 ? 1u : 0u);
           commit<CTAS>(empty(s), both);
-          commit<CTAS>(tfull(b), both);
+          commit<CTAS>(tfull(it & 1), both);
         }
         __syncwarp();
+        if (++s == S) {
+          s = 0;
+          phase ^= 1;
+        }
       }
       if (elect_one()) commit<CTAS>(final_bar, both);
       if (lane == 0) mbar_drain(final_bar, 0);
@@ -444,7 +449,12 @@ __global__ void __launch_bounds__(THREADS, 1)
     const int lt = q4 * 32 + lane;  // this thread's token of the CTA's 128
     const uint32_t ta0 = tmem + ((uint32_t)(q4 * 32) << 16) + wg * 64;
     // (in the cluster's window for one CTA too: an arrival that returns no state is not waited for)
-    const uint32_t te0 = cluster_map(tempty(0), rank - r);
+    const uint32_t go0 = cluster_map(go(0), rank - r);
+    int gs = 2 % S;  // stage of the k-block that takes over the buffer of k-block `it`, it + BUFS
+    if (lane == 0) {
+      mbar_arrive_cluster(go0);  // both buffers are empty
+      mbar_arrive_cluster(go0 + 8u);
+    }
     float acc[2][64];
     uint32_t it = 0, tile_parity = 0;
     bool ok = true;
@@ -483,7 +493,8 @@ __global__ void __launch_bounds__(THREADS, 1)
           fence_before();
           __syncwarp();
           // this buffer has been read: the tensor core may overwrite it
-          if (lane == 0) mbar_arrive_cluster(te0 + 8u * (it & 1));
+          if (lane == 0) mbar_arrive_cluster(go0 + 8u * gs);
+          if (++gs == S) gs = 0;
           add32(acc[1], v[0], sb);
           if (more) {
             ok = warp_wait(tfull((it + 1) & 1), ((it + 1) >> 1) & 1, abort_flag, 504);
