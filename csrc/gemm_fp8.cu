@@ -18,12 +18,13 @@
 // the thread holds matching gate / up pairs, so SiLU-and-mul needs no exchange and the tile is one whole
 // group of 128 of the 8-bit output.
 //
-// gemm_fp8_weights_kernel: few tokens.  Tiles of 128 weight rows (MMA M) x NP tokens (MMA N), so a
+// gemm_fp8_weights_kernel<NP, MW>: few tokens.  Tiles of 128 weight rows (MMA M) x NP tokens (MMA N), so a
 // step of one token moves 16 activation rows beside the weights instead of 128, and K split over the
 // CTAs of a cluster so that the weights of a small layer are streamed by the whole GPU.  A thread
 // owns one feature and all NP tokens; the K slices' fp32 sums meet in shared memory: every CTA stores
 // the sums of token c straight into CTA c mod splits (distributed shared memory), which adds them in
-// the order of the slices (the result does not depend on timing), finishes and stores the token.
+// the order of the slices (the result does not depend on timing), finishes and stores the token.  For
+// SiLU-and-mul a CTA holds both tiles of a group: its gate rows and the matching up rows.
 //
 // Neither kernel uses a global workspace.  Every wait is bounded; on expiry the kernel records an error code, drains its copies, frees TMEM
 // and returns.
@@ -68,30 +69,33 @@ struct TokensCfg {
   static_assert(BM * XLD * 4 <= STAGES * STAGE, "the exchange fits over the ring");
 };
 
-// Shape of gemm_fp8_weights_kernel<NP> (NP tokens, rounded up).  Two CTAs fit on an SM, so that one
-// streams while the other fills its pipeline or finishes, and so that the next kernel's CTAs start early.
-template <int NP>
+// Shape of gemm_fp8_weights_kernel<NP, MW>: NP tokens (rounded up), MW = 1 or (SiLU-and-mul: a block of 128
+// gate rows and the matching up rows) 2 tiles of 128 weight rows per CTA.  Two CTAs fit on an SM, so
+// that one streams while the other fills its pipeline or finishes, and so that the next kernel's CTAs
+// start early.
+template <int NP, int MW>
 struct WeightsCfg {
   static constexpr int COL_SPLIT = NP >= 64 ? 2 : 1;           // warps that share a quarter of the lanes
   static constexpr int NC = NP / COL_SPLIT;                    // tokens per epilogue thread
   static constexpr int CHUNK = NC == 32 ? 32 : 16;             // TMEM columns per load
-  static constexpr int EPI_WARPS = 4 * COL_SPLIT;
+  static constexpr int EPI_WARPS = 4 * COL_SPLIT * MW;
   static constexpr int THREADS = 64 + 32 * EPI_WARPS;
-  static constexpr int ACC_BUFS = NP <= 64 ? 4 : 2;            // TMEM buffers
-  static constexpr int TMEM_COLS = ACC_BUFS * NP;              // 64 .. 256
-  static constexpr int W_BYTES = 128 * BK, X_BYTES = NP * BK, STAGE = W_BYTES + X_BYTES;
-  // fp32 sums of the tokens this CTA finishes: in all at most NP + 7 rows of 128; beside the ring
-  // where that leaves it deep enough, over it otherwise
-  static constexpr int EXCHANGE = (NP + 8) * 128 * 4;
-  static constexpr bool OVER_RING = NP > 32;
+  static constexpr int ACC_BUFS = MW == 2 ? 2 : 4;             // TMEM buffers (at most as many as stages)
+  static constexpr int TMEM_COLS = ACC_BUFS * MW * NP;         // 64 .. 256
+  static constexpr int ROWS = 128 * MW;
+  static constexpr int W_BYTES = ROWS * BK, X_BYTES = NP * BK, STAGE = W_BYTES + X_BYTES;
+  // fp32 sums of the tokens this CTA finishes: slices x ceil(NP / slices) <= NP + 7 rows; beside the
+  // ring where that leaves it deep enough, over it otherwise
+  static constexpr int EXCHANGE = (NP + 8) * ROWS * 4;
+  static constexpr bool OVER_RING = NP * MW >= 32 && !(NP == 32 && MW == 1);
   static constexpr int SLOT = NP * 4 < 128 ? 128 : NP * 4;     // activation scales of one k-block
   static constexpr int BUDGET = 113 * 1024;
-  static constexpr int bar_bytes(int s) { return 8 * (3 * s + 3 * ACC_BUFS + 2) + 16; }
+  static constexpr int bars(int s) { return 3 * s + 2 * ACC_BUFS + 2; }
   static constexpr int ring_bytes(int s) {
     return OVER_RING ? (s * STAGE > EXCHANGE ? s * STAGE : EXCHANGE) : s * STAGE + EXCHANGE;
   }
   // one slot more than stages and buffers together: see the producer
-  static constexpr int smem(int s) { return 1024 + ring_bytes(s) + (s + ACC_BUFS + 1) * SLOT + bar_bytes(s); }
+  static constexpr int smem(int s) { return 1024 + ring_bytes(s) + (s + ACC_BUFS + 1) * SLOT + 8 * bars(s) + 16; }
   static constexpr int stages() {
     int s = 8;
     while (s > 2 && smem(s) > BUDGET) --s;
@@ -99,9 +103,10 @@ struct WeightsCfg {
   }
   static constexpr int STAGES = stages();
   static constexpr int SLOTS = STAGES + ACC_BUFS + 1;
-  static constexpr int BAR_BYTES = bar_bytes(STAGES);
+  static constexpr int BARS = bars(STAGES);
   static constexpr int SMEM = smem(STAGES);
   static_assert(SMEM <= BUDGET, "two CTAs per SM");
+  static_assert(ACC_BUFS <= STAGES, "a stage's barrier takes the arrivals of one k-block at a time");
 };
 
 // A wait of a whole warp that stays together afterwards.  All lanes poll: electing one to do it costs
@@ -112,7 +117,6 @@ __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatil
 
 struct Params {
   int splits, kb_per_split;  // K slices and their length in k-blocks
-  int cluster;               // weights kernel: CTAs per cluster (slices x 2 with SiLU-and-mul)
   const float* ws;
   int64_t ldws;
   int T, N, num_kb, nb;      // nb: 128-row blocks of W
@@ -614,46 +618,40 @@ __global__ void __launch_bounds__(THREADS, 1)
   }
 }
 
-// A CTA's tile is 128 weight rows.  Plain: rows [128 j, 128 j + 128).  SiLU-and-mul: half h of the
-// pair of blocks j: gate rows 64 h .. and the matching up rows, so that two CTAs of one cluster hold
-// a whole group of 128 of the output.
-template <int NP>
-__global__ void __launch_bounds__(WeightsCfg<NP>::THREADS, 2)
+template <int NP, int MW>
+__global__ void __launch_bounds__(WeightsCfg<NP, MW>::THREADS, 2)
     gemm_fp8_weights_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
                             const __grid_constant__ CUtensorMap map_s, Params p) {
-  using C = WeightsCfg<NP>;
+  using C = WeightsCfg<NP, MW>;
   constexpr int S = C::STAGES, NB = C::ACC_BUFS, SL = C::SLOTS;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   // the same offset in every CTA of the cluster
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   float* exchange = reinterpret_cast<float*>(smem + (C::OVER_RING ? 0 : S * C::STAGE));
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::SMEM - 1024 - C::BAR_BYTES);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::SMEM - 1024 - 8 * C::BARS - 16);
   uint8_t* slots = reinterpret_cast<uint8_t*>(bars) - SL * C::SLOT;
   const uint32_t bar0 = smem_u32(bars);
-  auto full = [&](int s) { return bar0 + 8u * s; };
+  // go: the operands of the k-block in this stage have landed and the epilogue warps have emptied its
+  // accumulator buffer (one poll for both, see gemm_fp8_tokens_kernel)
+  auto go = [&](int s) { return bar0 + 8u * s; };
   auto empty = [&](int s) { return bar0 + 8u * (S + s); };
   auto tfull = [&](int b) { return bar0 + 8u * (2 * S + b); };
-  auto tempty = [&](int b) { return bar0 + 8u * (2 * S + NB + b); };
-  auto sfull = [&](int l) { return bar0 + 8u * (2 * S + 2 * NB + l); };
-  const uint32_t final_bar = bar0 + 8u * (2 * S + 2 * NB + SL);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + 2 * S + 2 * NB + SL + 1);
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * S + 2 * NB + SL + 1) + 1;
+  auto sfull = [&](int l) { return bar0 + 8u * (2 * S + NB + l); };
+  const uint32_t final_bar = bar0 + 8u * (2 * S + NB + SL);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + C::BARS);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + C::BARS) + 1;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int rank = p.cluster > 1 ? (int)cluster_rank() : 0;
-  const int tile = blockIdx.x / p.cluster;
-  const int half = p.act ? rank & 1 : 0, slice = p.act ? rank >> 1 : rank;
+  const int slice = p.splits > 1 ? (int)cluster_rank() : 0;
+  const int tile = blockIdx.x / p.splits;
   const int kb0 = slice * p.kb_per_split;
   const int nkb = max(0, min(p.num_kb - kb0, p.kb_per_split));
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < S; ++s) {
-      mbar_init(full(s), 1);
+      mbar_init(go(s), 1 + C::EPI_WARPS);
       mbar_init(empty(s), 1);
     }
-    for (int b = 0; b < NB; ++b) {
-      mbar_init(tfull(b), 1);
-      mbar_init(tempty(b), C::EPI_WARPS);
-    }
+    for (int b = 0; b < NB; ++b) mbar_init(tfull(b), 1);
     for (int l = 0; l < SL; ++l) mbar_init(sfull(l), 1);
     mbar_init(final_bar, 1);
     *abort_flag = 0;
@@ -665,20 +663,16 @@ __global__ void __launch_bounds__(WeightsCfg<NP>::THREADS, 2)
   fence_after();
   const uint32_t tmem = *tmem_slot;
   // this CTA's exchange area may be written: now, or once its ring is idle (waited on below)
-  if (!C::OVER_RING && p.cluster > 1) cluster_arrive();
+  if (!C::OVER_RING && p.splits > 1) cluster_arrive();
   pdl_trigger();
 
   if (warp == 0 && lane == 0) {
     // ------------------------------------------------------------------ producer
-    const int row_a = p.act ? tile * 256 + half * 64 : tile * 128, row_b = row_a + (p.act ? 128 : 64);
     prefetch_map(&map_w);
     prefetch_map(&map_x);
     prefetch_map(&map_s);
     // Into L2 only, ahead of the previous kernel's end: whoever writes the weights writes there too
-    for (int i = 0; i < min(nkb, S); ++i) {
-      tma_prefetch_2d(&map_w, (kb0 + i) * BK, row_a);
-      tma_prefetch_2d(&map_w, (kb0 + i) * BK, row_b);
-    }
+    for (int i = 0; i < min(nkb, S); ++i) tma_prefetch_2d(&map_w, (kb0 + i) * BK, tile * C::ROWS);
     pdl_wait();
     bool ok = true;
     int i = 0;
@@ -689,10 +683,9 @@ __global__ void __launch_bounds__(WeightsCfg<NP>::THREADS, 2)
         break;
       }
       const uint32_t st = smem_u32(smem + s * C::STAGE);
-      mbar_arrive_expect_tx(full(s), C::STAGE);
-      tma_load_2d(st, &map_w, full(s), (kb0 + i) * BK, row_a);
-      tma_load_2d(st + 64 * BK, &map_w, full(s), (kb0 + i) * BK, row_b);
-      tma_load_2d(st + C::W_BYTES, &map_x, full(s), (kb0 + i) * BK, 0);
+      mbar_arrive_expect_tx(go(s), C::STAGE);
+      tma_load_2d(st, &map_w, go(s), (kb0 + i) * BK, tile * C::ROWS);
+      tma_load_2d(st + C::W_BYTES, &map_x, go(s), (kb0 + i) * BK, 0);
       // Slot l was last read for k-block i - SL.  Stage s is free, so k-block i - S has been
       // multiplied, so the epilogue has emptied the buffer of k-block i - S - NB, and had by then
       // read the scales of the one before, i - SL: no barrier of its own guards the slot.
@@ -701,7 +694,7 @@ __global__ void __launch_bounds__(WeightsCfg<NP>::THREADS, 2)
     }
     if (!ok) {
       for (int j = max(0, i - S); j < i; ++j) {
-        mbar_drain(full(j % S), (j / S) & 1);
+        mbar_drain(go(j % S), (j / S) & 1);
         mbar_drain(sfull(j % SL), (j / SL) & 1);
       }
     }
@@ -710,16 +703,17 @@ __global__ void __launch_bounds__(WeightsCfg<NP>::THREADS, 2)
     const uint32_t tbase = __shfl_sync(FULL_MASK, tmem, 0);
     for (int i = 0; i < nkb; ++i) {
       const int s = i % S, b = i % NB;
-      if (!warp_wait(full(s), (i / S) & 1, abort_flag, 513) ||
-          !warp_wait(tempty(b), ((i / NB) & 1) ^ 1, abort_flag, 512))
-        break;
+      if (!warp_wait(go(s), (i / S) & 1, abort_flag, 513)) break;
       fence_after();
       const uint32_t st = smem_u32(smem + s * C::STAGE);
       const uint64_t wd = sdesc(st), xd = sdesc(st + C::W_BYTES);
       if (elect_one()) {
 #pragma unroll
-        for (int k = 0; k < BK / 32; ++k)
-          mma_f8<1>(tbase + b * NP, wd + 2 * k, xd + 2 * k, idesc_f8(128, NP), k > 0 ? 1u : 0u);
+        for (int m = 0; m < MW; ++m)
+#pragma unroll
+          for (int k = 0; k < BK / 32; ++k)
+            mma_f8<1>(tbase + (b * MW + m) * NP, wd + m * (128 * BK >> 4) + 2 * k, xd + 2 * k, idesc_f8(128, NP),
+                      k > 0 ? 1u : 0u);
         commit<1>(empty(s));
         commit<1>(tfull(b));
       }
@@ -730,13 +724,16 @@ __global__ void __launch_bounds__(WeightsCfg<NP>::THREADS, 2)
     __syncwarp();
   } else if (warp >= 2) {
     // ------------------------------------------------------------------ epilogue
-    const int q4 = warp & 3, cs = (warp - 2) >> 2;  // lane quarter, share of the tokens
-    const int blk = p.act ? 2 * tile + (q4 >> 1) : tile;  // this warp's 128-row block of W
+    // lane quarter, 128-row block of the tile, share of the tokens
+    const int q4 = warp & 3, m = ((warp - 2) >> 2) % MW, cs = ((warp - 2) >> 2) / MW;
+    const uint32_t go0 = cluster_map(go(0), slice);
+    if (lane == 0)
+      for (int b = 0; b < NB; ++b) mbar_arrive_cluster(go0 + 8u * b);  // every buffer is empty
     float acc[C::NC];
 #pragma unroll
     for (int i = 0; i < C::NC; ++i) acc[i] = 0.f;
     pdl_wait();
-    WeightScales ws(p.ws + (int64_t)min(blk, p.nb - 1) * p.ldws + kb0, nkb, lane);
+    WeightScales ws(p.ws + (int64_t)min(tile * MW + m, p.nb - 1) * p.ldws + kb0, nkb, lane);
     bool ok = true;
     for (int i = 0; i < nkb; ++i) {
       const float wsc = ws.at(i);
@@ -744,7 +741,7 @@ __global__ void __launch_bounds__(WeightsCfg<NP>::THREADS, 2)
       ok = warp_wait(sfull(l), (i / SL) & 1, abort_flag, 514) && warp_wait(tfull(b), (i / NB) & 1, abort_flag, 515);
       if (!ok) break;
       fence_after();
-      const uint32_t ta = tmem + ((uint32_t)(q4 * 32) << 16) + b * NP + cs * C::NC;
+      const uint32_t ta = tmem + ((uint32_t)(q4 * 32) << 16) + (b * MW + m) * NP + cs * C::NC;
       const float4* xs = reinterpret_cast<const float4*>(slots + l * C::SLOT) + cs * (C::NC / 4);
 #pragma unroll
       for (int c = 0; c < C::NC / C::CHUNK; ++c) {
@@ -754,7 +751,7 @@ __global__ void __launch_bounds__(WeightsCfg<NP>::THREADS, 2)
         if (c + 1 == C::NC / C::CHUNK) {  // this buffer has been read: the tensor core may overwrite it
           fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive_cluster(cluster_map(tempty(b), rank));
+          if (lane == 0) mbar_arrive_cluster(go0 + 8u * ((i + NB) % S));
         }
 #pragma unroll
         for (int j = 0; j < C::CHUNK / 4; ++j) {
@@ -767,25 +764,23 @@ __global__ void __launch_bounds__(WeightsCfg<NP>::THREADS, 2)
         }
       }
     }
-    // sums of token c to CTA c mod cluster: [slice][c / cluster][feature of the cluster]
-    if (p.cluster > 1) {
+    // sums of token c to CTA c mod splits: [slice][c / splits][feature]
+    if (p.splits > 1) {
       if (C::OVER_RING) cluster_arrive();  // the last MMA has completed: nothing reads the ring any more
       cluster_wait();
     }
-    const int r = q4 * 32 + lane;
-    const int f = p.act ? (r >> 6) * 128 + half * 64 + (r & 63) : r;
-    const int width = p.act ? 256 : 128;
-    const int per = (NP + p.cluster - 1) / p.cluster;
-    int owner = (cs * C::NC) % p.cluster, tl = (cs * C::NC) / p.cluster;
+    const int f = m * 128 + q4 * 32 + lane;
+    const int per = (NP + p.splits - 1) / p.splits;
+    int owner = (cs * C::NC) % p.splits, tl = (cs * C::NC) / p.splits;
 #pragma unroll
     for (int c = 0; c < C::NC; ++c)
       if (cs * C::NC + c < p.T) {
-        float* dst = exchange + (slice * per + tl) * width + f;
-        if (p.cluster > 1)
+        float* dst = exchange + (slice * per + tl) * C::ROWS + f;
+        if (p.splits > 1)
           st_cluster_f32(cluster_map(smem_u32(dst), owner), acc[c]);
         else
           *dst = acc[c];
-        if (++owner == p.cluster) {
+        if (++owner == p.splits) {
           owner = 0;
           ++tl;
         }
@@ -793,7 +788,7 @@ __global__ void __launch_bounds__(WeightsCfg<NP>::THREADS, 2)
   }
   __syncwarp();
   fence_before();
-  if (p.cluster > 1) {
+  if (p.splits > 1) {
     if (warp < 2) {
       if (C::OVER_RING) cluster_arrive();
       cluster_wait();
@@ -804,27 +799,21 @@ __global__ void __launch_bounds__(WeightsCfg<NP>::THREADS, 2)
     __syncthreads();
   }
   if (warp >= 2 && !*abort_flag) {
-    const int per = (NP + p.cluster - 1) / p.cluster;
-    const int mine = (p.T - rank + p.cluster - 1) / p.cluster;  // tokens rank, rank + cluster, ...
+    const int per = (NP + p.splits - 1) / p.splits;
+    const int mine = (p.T - slice + p.splits - 1) / p.splits;  // tokens slice, slice + splits, ...
     for (int tl = warp - 2; tl < mine; tl += C::EPI_WARPS) {
-      const int t = rank + tl * p.cluster;
-      if (!p.act) {
-        float o[4] = {0.f, 0.f, 0.f, 0.f};
-        for (int r = 0; r < p.splits; ++r) {
-          const float4 v = reinterpret_cast<const float4*>(exchange + (r * per + tl) * 128)[lane];
-          o[0] += v.x; o[1] += v.y; o[2] += v.z; o[3] += v.w;
+      const int t = slice + tl * p.splits;
+      float o[MW][4] = {};
+      for (int r = 0; r < p.splits; ++r) {
+        const float4* row = reinterpret_cast<const float4*>(exchange + (r * per + tl) * C::ROWS);
+#pragma unroll
+        for (int m = 0; m < MW; ++m) {
+          const float4 v = row[m * 32 + lane];
+          o[m][0] += v.x; o[m][1] += v.y; o[m][2] += v.z; o[m][3] += v.w;
         }
-        finish_bf16x4(p, t, tile * 128 + lane * 4, o);
-      } else {
-        float g[4] = {0.f, 0.f, 0.f, 0.f}, u[4] = {0.f, 0.f, 0.f, 0.f};
-        for (int r = 0; r < p.splits; ++r) {
-          const float4* row = reinterpret_cast<const float4*>(exchange + (r * per + tl) * 256);
-          const float4 a = row[lane], b = row[32 + lane];
-          g[0] += a.x; g[1] += a.y; g[2] += a.z; g[3] += a.w;
-          u[0] += b.x; u[1] += b.y; u[2] += b.z; u[3] += b.w;
-        }
-        finish_silu4(p, t, tile, lane, g, u);
       }
+      if constexpr (MW == 1) finish_bf16x4(p, t, tile * 128 + lane * 4, o[0]);
+      else finish_silu4(p, t, tile, lane, o[0], o[1]);
     }
   }
   if (warp == 1) {
@@ -906,10 +895,10 @@ cudaError_t tokens_opt_in() {
   });
 }
 
-template <int NP>
+template <int NP, int MW>
 cudaError_t weights_opt_in() {
   static std::atomic<uint64_t> done{0};
-  return smem_opt_in(done, gemm_fp8_weights_kernel<NP>, WeightsCfg<NP>::SMEM);
+  return smem_opt_in(done, gemm_fp8_weights_kernel<NP, MW>, WeightsCfg<NP, MW>::SMEM);
 }
 
 // Clusters of `cluster` CTAs, one CTA per SM, that the GPU holds at once (a cluster lies within one of
@@ -955,25 +944,22 @@ bool make_out_map(CUtensorMap* m, const Fp8Gemm& g) {
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int NP>
+template <int NP, int MW>
 cudaError_t run_weights(const Fp8Gemm& g, Params p, int splits, cudaStream_t stream) {
-  const int cluster = splits * (g.act ? 2 : 1);
-  if (splits < 1 || cluster > 8 || g.T > NP) return cudaErrorInvalidValue;
+  using C = WeightsCfg<NP, MW>;
+  if (splits < 1 || splits > 8 || g.T > NP) return cudaErrorInvalidValue;
   CUtensorMap mx, mw, ms;
-  if (!make_map(&mx, g.xq, g.T, g.K, g.ldx, NP) || !make_map(&mw, g.wq, g.N, g.K, g.ldw, 64) ||
+  if (!make_map(&mx, g.xq, g.T, g.K, g.ldx, NP) || !make_map(&mw, g.wq, g.N, g.K, g.ldw, C::ROWS) ||
       !make_scale_map(&ms, g.xs, p.num_kb, g.T, g.ldxs, NP))
     return cudaErrorInvalidValue;
   p.splits = splits;
-  p.cluster = cluster;
   p.kb_per_split = (p.num_kb + splits - 1) / splits;
-  cudaError_t e = weights_opt_in<NP>();
+  cudaError_t e = weights_opt_in<NP, MW>();
   if (e != cudaSuccess) return e;
-  const int rows = g.act ? 256 : 128;
   cudaLaunchAttribute attr[2];
-  cudaLaunchConfig_t cfg =
-      cluster_config((g.N + rows - 1) / rows * cluster, WeightsCfg<NP>::THREADS, WeightsCfg<NP>::SMEM, cluster, attr);
+  cudaLaunchConfig_t cfg = cluster_config((g.N + C::ROWS - 1) / C::ROWS * splits, C::THREADS, C::SMEM, splits, attr);
   cfg.stream = stream;
-  return cudaLaunchKernelEx(&cfg, gemm_fp8_weights_kernel<NP>, mx, mw, ms, p);
+  return cudaLaunchKernelEx(&cfg, gemm_fp8_weights_kernel<NP, MW>, mx, mw, ms, p);
 }
 
 template <int CTAS>
@@ -1011,10 +997,9 @@ Fp8Plan fp8_plan(int T, int N, int K, int act, int num_sms) {
   const int num_kb = (K + BK - 1) / BK;
   if (T <= (act ? 32 : 64)) {
     pl.np = T <= 16 ? 16 : T <= 32 ? 32 : 64;
-    const int halves = act ? 2 : 1;
-    const int tiles = (N + 128 * halves - 1) / (128 * halves);
-    for (int s = 2; s * halves <= 8; ++s)
-      if (num_kb / s >= 2 && tiles <= clusters_of_half_sms(s * halves, num_sms)) pl.splits = s;
+    const int rows = act ? 256 : 128, tiles = (N + rows - 1) / rows;
+    for (int s = 2; s <= 8; ++s)
+      if (num_kb / s >= 2 && tiles <= clusters_of_half_sms(s, num_sms)) pl.splits = s;
   } else {
     const int64_t tiles = (int64_t)((T + BM - 1) / BM) * ((N + BN - 1) / BN);
     for (int s = 2; s <= 4; s *= 2)
@@ -1043,9 +1028,9 @@ cudaError_t gemm_fp8(const Fp8Gemm& g, const Fp8Plan& pl, int num_sms, cudaStrea
   switch (pl.np) {
     case -1: return run_tokens<1>(g, p, pl.splits, num_sms, stream);
     case -2: return run_tokens<2>(g, p, pl.splits, num_sms, stream);
-    case 16: return run_weights<16>(g, p, pl.splits, stream);
-    case 32: return run_weights<32>(g, p, pl.splits, stream);
-    case 64: return run_weights<64>(g, p, pl.splits, stream);
+    case 16: return g.act ? run_weights<16, 2>(g, p, pl.splits, stream) : run_weights<16, 1>(g, p, pl.splits, stream);
+    case 32: return g.act ? run_weights<32, 2>(g, p, pl.splits, stream) : run_weights<32, 1>(g, p, pl.splits, stream);
+    case 64: return g.act ? cudaErrorInvalidValue : run_weights<64, 1>(g, p, pl.splits, stream);
     default: return cudaErrorInvalidValue;
   }
 }

@@ -182,9 +182,9 @@ def test_linear_silu(ops, t, i, k):
 
 
 def _plans(t, act):
-    for np_ in (16, 32, 64):
+    for np_ in (16, 32) if act else (16, 32, 64):
         if np_ >= t:
-            for splits in (1, 2, 3, 4) if act else (1, 2, 3, 5, 8):
+            for splits in (1, 2, 3, 5, 8):
                 yield [np_, splits]
     for ctas in (1, 2):
         for splits in (1, 2, 4, 8 // ctas):
@@ -222,7 +222,7 @@ def test_plans_refused(ops):
         with pytest.raises(RuntimeError):
             ops.C.linear_fp8(*x, *w, None, plan)
     with pytest.raises(RuntimeError):
-        ops.C.linear_silu_fp8(*x, *w, 128, [32, 5])
+        ops.C.linear_silu_fp8(*x, *w, 128, [64, 1])
 
 
 @pytest.mark.parametrize("t", [1, 20, 200])
