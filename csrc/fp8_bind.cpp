@@ -1,6 +1,7 @@
 // Python bindings of the fp8 layer kernels.  Each call checks its arguments, allocates its outputs and
 // launches on the current stream of the inputs' device; none keeps a workspace.
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
@@ -27,12 +28,17 @@ int64_t groups(int64_t k) { return (k + nvb::FP8_GROUP - 1) / nvb::FP8_GROUP; }
 
 bool aligned(const at::Tensor& t, uintptr_t a) { return (reinterpret_cast<uintptr_t>(t.data_ptr()) & (a - 1)) == 0; }
 
+// Outputs come straight from the caching allocator: the smallest calls are bound by the host, and the
+// dispatcher's way there costs as much as the launch.
+at::Tensor new_cuda(at::IntArrayRef size, at::ScalarType dtype, const at::Tensor& like) {
+  return at::Tensor(at::detail::empty_cuda(size, dtype, like.device(), c10::nullopt));
+}
+
 // e4m3 [t, k] and its scales [t, k / 128], token-contiguous (strides (1, t rounded up to 4)).
 Pair new_pair(const at::Tensor& like, int64_t t, int64_t k) {
-  auto q = at::empty({t, k}, like.options().dtype(at::kFloat8_e4m3fn));
-  auto s = at::empty_strided({t, groups(k)}, {1, std::max<int64_t>((t + 3) / 4 * 4, 4)},
-                             like.options().dtype(at::kFloat));
-  return {q, s};
+  const int64_t ld = std::max<int64_t>((t + 3) / 4 * 4, 4);
+  return {new_cuda({t, k}, at::kFloat8_e4m3fn, like),
+          at::Tensor(at::detail::empty_strided_cuda({t, groups(k)}, {1, ld}, at::kFloat, like.device()))};
 }
 
 // The device is checked last: every other refusal then also holds for CPU tensors.
@@ -153,7 +159,7 @@ at::Tensor linear_fp8(const at::Tensor& xq, const at::Tensor& xs, const at::Tens
   }
   check_cuda(xq, "linear_fp8");
   at::cuda::CUDAGuard g(xq.device());
-  at::Tensor y = out.has_value() ? *out : at::empty({a.T, a.N}, xq.options().dtype(at::kBFloat16));
+  at::Tensor y = out.has_value() ? *out : new_cuda({a.T, a.N}, at::kBFloat16, xq);
   a.out = y.data_ptr();
   a.ldo = row_stride(y);
   ok(nvb::gemm_fp8(a, plan_of(a, plan, sms()), sms(), stream()), "linear_fp8");
