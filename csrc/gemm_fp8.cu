@@ -10,13 +10,18 @@
 //
 // No counterpart in the reference, whose linear layers are 16-bit (nanovllm/models/qwen3.py:96-134).
 //
-// gemm_fp8_tokens_kernel<CTAS>: tiles of 128 tokens (MMA M, one TMEM lane each) x 256 features (MMA N)
-// per CTA; CTAS = 2: a pair of CTAs (tcgen05.mma.cta_group::2) shares the 256 weight rows of a tile of
-// 256 tokens, each staging 128 of them.  A thread of the epilogue owns one token and 64 + 64 features,
-// [64 w, 64 w + 64) of both 128-row weight blocks of the tile: both scales are then one number per
-// thread and k-block (no scale vector to load), and with gate and up rows in alternating blocks of 128
-// the thread holds matching gate / up pairs, so SiLU-and-mul needs no exchange and the tile is one whole
-// group of 128 of the 8-bit output.
+// gemm_fp8_tokens_kernel<CTAS, BN>: tiles of 128 tokens (MMA M, one TMEM lane each) x BN = 256 or 128
+// features (MMA N) per CTA; CTAS = 2: a pair of CTAs (tcgen05.mma.cta_group::2) shares the weight rows of
+// a tile of 256 tokens, each staging half of them.  A thread of the epilogue owns one token and 64
+// features of each 128-row weight block of the tile: each scale is then one number per thread and
+// k-block (no scale vector to load), and with gate and up rows in alternating blocks of 128 the thread
+// holds matching gate / up pairs, so SiLU-and-mul needs no exchange and a tile of 256 is one whole group
+// of 128 of the 8-bit output.
+//
+// What bounds it: per k-block and 256 features the tensor core needs 512 clocks, the chain MMA -> commit
+// -> poll -> TMEM load -> additions -> arrival -> poll -> MMA about 850 with both TMEM buffers in flight
+// (polls of 100 to 300 clocks each beside the additions), so large products reach 0.6 of the rate of
+// the MMAs alone, and there the 1000 W limit holds the clock at 1.5 GHz besides.
 //
 // gemm_fp8_weights_kernel<NP, MW>: few tokens.  Tiles of 128 weight rows (MMA M) x NP tokens (MMA N), so a
 // step of one token moves 16 activation rows beside the weights instead of 128, and K split over the
@@ -45,28 +50,32 @@ namespace {
 using namespace tc;
 
 constexpr int BM = 128;                 // tokens per CTA
-constexpr int BN = 256;                 // features per tile
 constexpr int BK = 128;                 // one scale block = one 128-byte swizzle row
-constexpr int BUFS = 2;                 // accumulator buffers (all of TMEM)
 constexpr int EPI_THREADS = 256;
 constexpr int THREADS = 128 + EPI_THREADS;  // TMA warp, MMA warp, two scale warps; 8 epilogue warps
 // Registers: the 12 warps are launched with 168 each (65536 / 384); the control warps give theirs up
 // for the epilogue's, which hold 128 sums and two TMEM loads of 32 values.
 constexpr int LAUNCH_REGS = 168, CONTROL_REGS = 56, EPI_REGS = 224;
 static_assert(4 * CONTROL_REGS + 8 * EPI_REGS <= 12 * LAUNCH_REGS, "the launch's registers");
-constexpr int XLD = BN + 4;             // exchange row: 16-byte stores of 8 rows hit distinct banks
 
-template <int CTAS>
+// CTAS CTAs share a tile of CTAS x 128 tokens x BN features.
+template <int CTAS, int BN>
 struct TokensCfg {
+  static constexpr int BUFS = 512 / BN;     // accumulator buffers: all of TMEM
+  static constexpr int BLOCKS = BN / 128;   // 128-row blocks of W in a tile, each with a scale of its own
   static constexpr int B_ROWS = BN / CTAS;  // weight rows staged by one CTA
   static constexpr int A_BYTES = BM * BK, STAGE = A_BYTES + B_ROWS * BK;  // 48 or 32 KB
-  static constexpr int STAGES = CTAS == 2 ? 6 : 4;
+  static constexpr int STAGES = STAGE == 48 * 1024 ? 4 : 6;
   static constexpr int STAGING = EPI_THREADS / 32 * 2048;
   static constexpr int SLOTS = STAGES + BUFS + 1;  // activation scales of one k-block each: see the producer
   static constexpr int BARS = 2 * STAGES + BUFS + SLOTS + 2;
-  static constexpr int SMEM = 1024 + STAGES * STAGE + STAGING + SLOTS * BM * 4 + 4 * 2 * BM * 4 + 2 * 2 * BM * 4 + 8 * BARS + 16;
+  static constexpr int PRODS = 2 * BUFS;    // k-blocks whose scale products are kept
+  static constexpr int XLD = BN + 4;        // exchange row: 16-byte stores of 8 rows hit distinct banks
+  static constexpr int SMEM = 1024 + STAGES * STAGE + STAGING + SLOTS * BM * 4 + PRODS * BLOCKS * BM * 4 +
+                              2 * 2 * BM * 4 + 8 * BARS + 16;
   static_assert(SMEM <= 227 * 1024, "shared memory of a CTA");
   static_assert(BM * XLD * 4 <= STAGES * STAGE, "the exchange fits over the ring");
+  static_assert(BUFS <= STAGES, "a stage's barrier takes the arrivals of one k-block at a time");
 };
 
 // Shape of gemm_fp8_weights_kernel<NP, MW>: NP tokens (rounded up), MW = 1 or (SiLU-and-mul: a block of 128
@@ -227,41 +236,42 @@ __device__ __forceinline__ void finish_bf16x4(const Params& p, int t, int n, con
 
 // Tokens [128 slice / S, 128 (slice + 1) / S) of this CTA's 128, whose sums lie in S CTAs of the cluster
 // (ranks r, r + CTAS, ...): added in the order of the slices, finished and stored.  A warp takes a
-// token's 256 sums of one slice as two 512-byte rows (remote stores of each thread's own 16 bytes were
-// slower by half) and has 16 of them in flight.
-template <int CTAS, int S>
+// token's sums of one slice and 128 features as one 512-byte row (remote stores of each thread's own 16
+// bytes were slower by half) and has 16 of them in flight.
+template <int CTAS, int BN, int S>
 __device__ __forceinline__ void finish_rows(const Params& p, float* exchange, int slice, int r, int row0, int tn,
                                             int w, int lane) {
-  constexpr int PER = BM / S, G = 8 / S;
+  constexpr int XLD = TokensCfg<CTAS, BN>::XLD, NB = BN / 128;
+  constexpr int PER = BM / S, G = 16 / NB / S;
   for (int tl = w * G; tl < PER; tl += EPI_THREADS / 32 * G) {
     const int r0 = slice * PER + tl;
     if (row0 + r0 >= p.T) break;
     const uint32_t src = smem_u32(exchange + r0 * XLD + lane * 4);
-    float4 a[G][S], b[G][S];
+    float4 a[G][S][NB];
 #pragma unroll
     for (int s = 0; s < S; ++s) {
       const uint32_t at = cluster_map(src, s * CTAS + r);
 #pragma unroll
-      for (int i = 0; i < G; ++i) {
-        a[i][s] = ld_cluster_f32x4(at + i * XLD * 4);
-        b[i][s] = ld_cluster_f32x4(at + i * XLD * 4 + 512);
-      }
+      for (int i = 0; i < G; ++i)
+#pragma unroll
+        for (int h = 0; h < NB; ++h) a[i][s][h] = ld_cluster_f32x4(at + (i * XLD + h * 128) * 4);
     }
 #pragma unroll
     for (int i = 0; i < G; ++i) {
-      float g[4] = {0.f, 0.f, 0.f, 0.f}, u[4] = {0.f, 0.f, 0.f, 0.f};
+      float o[NB][4] = {};
 #pragma unroll
-      for (int s = 0; s < S; ++s) {
-        g[0] += a[i][s].x; g[1] += a[i][s].y; g[2] += a[i][s].z; g[3] += a[i][s].w;
-        u[0] += b[i][s].x; u[1] += b[i][s].y; u[2] += b[i][s].z; u[3] += b[i][s].w;
-      }
+      for (int s = 0; s < S; ++s)
+#pragma unroll
+        for (int h = 0; h < NB; ++h) {
+          o[h][0] += a[i][s][h].x; o[h][1] += a[i][s][h].y; o[h][2] += a[i][s][h].z; o[h][3] += a[i][s][h].w;
+        }
       const int row = row0 + r0 + i;
       if (row < p.T) {  // the same for the whole warp
-        if (p.act) {
-          finish_silu4(p, row, tn, lane, g, u);
+        if (BN == 256 && p.act) {
+          finish_silu4(p, row, tn, lane, o[0], o[NB - 1]);
         } else {
-          finish_bf16x4(p, row, tn * BN + lane * 4, g);
-          finish_bf16x4(p, row, tn * BN + 128 + lane * 4, u);
+#pragma unroll
+          for (int h = 0; h < NB; ++h) finish_bf16x4(p, row, tn * BN + h * 128 + lane * 4, o[h]);
         }
       }
     }
@@ -270,20 +280,20 @@ __device__ __forceinline__ void finish_rows(const Params& p, float* exchange, in
 
 // One tile per cluster of splits x CTAS CTAs (each group of CTAS a slice of K), or, with splits = 1,
 // persistent CTAs that walk the tiles.
-template <int CTAS>
+template <int CTAS, int BN>
 __global__ void __launch_bounds__(THREADS, 1)
     gemm_fp8_tokens_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
                            const __grid_constant__ CUtensorMap map_s, const __grid_constant__ CUtensorMap map_o, Params p) {
-  using C = TokensCfg<CTAS>;
-  constexpr int S = C::STAGES, SL = C::SLOTS;
+  using C = TokensCfg<CTAS, BN>;
+  constexpr int S = C::STAGES, SL = C::SLOTS, BUFS = C::BUFS, XLD = C::XLD;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   // the same offset in every CTA of the cluster
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   float* exchange = reinterpret_cast<float*>(smem);  // over the idle ring (splits > 1)
   uint8_t* staging = smem + S * C::STAGE;  // 2 KB per epilogue warp: 64 bytes of 32 rows on their way out
   float* slots = reinterpret_cast<float*>(staging + C::STAGING);
-  float* prods = slots + SL * BM;  // [k-block & 3][weight block][token]: activation scale x weight scale
-  uint32_t* amax = reinterpret_cast<uint32_t*>(prods + 4 * 2 * BM);  // [tile parity][half][token]
+  float* prods = slots + SL * BM;  // [k-block % PRODS][weight block][token]: activation scale x weight scale
+  uint32_t* amax = reinterpret_cast<uint32_t*>(prods + C::PRODS * C::BLOCKS * BM);  // [tile parity][half][token]
   uint64_t* bars = reinterpret_cast<uint64_t*>(amax + 2 * 2 * BM);
   const uint32_t bar0 = smem_u32(bars);
   // go (the even CTA's): the operands of the k-block in this stage have landed and the epilogue warps have
@@ -307,7 +317,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       mbar_init(empty(s), 1);
     }
     for (int b = 0; b < BUFS; ++b) {
-      mbar_init(tfull(b), 1 + 2);  // the product's commit and the two scale warps
+      mbar_init(tfull(b), 1 + C::BLOCKS);  // the product's commit and the scale warps
     }
     for (int l = 0; l < SL; ++l) mbar_init(sfull(l), 1);
     mbar_init(final_bar, 1);
@@ -392,13 +402,13 @@ __global__ void __launch_bounds__(THREADS, 1)
         fence_after();
         const uint32_t off = s * (C::STAGE >> 4);  // the descriptors count in 16 bytes
         const uint64_t ad = ad0 + off, bd = bd0 + off;
-        const uint32_t d = tbase + (it & 1) * BN;
+        const uint32_t d = tbase + (it % BUFS) * BN;
         if (elect_one()) {
 #pragma unroll
           for (int k = 0; k < BK / 32; ++k)
             mma_f8<CTAS>(d, ad + 2 * k, bd + 2 * k, idesc_f8(CTAS * BM, BN), k > 0 ? 1u : 0u);
           commit<CTAS>(empty(s), both);
-          commit<CTAS>(tfull(it & 1), both);
+          commit<CTAS>(tfull(it % BUFS), both);
         }
         __syncwarp();
         if (++s == S) {
@@ -408,7 +418,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       }
       if (elect_one()) commit<CTAS>(final_bar, both);
       if (lane == 0) mbar_drain(final_bar, 0);
-    } else if (warp >= 2) {
+    } else if (warp >= 2 && warp - 2 < C::BLOCKS) {
       // ---------------------------------------------------------------- scales of weight block warp - 2
       // Each k-block's products of activation and weight scale, so that the epilogue has one barrier to
       // wait for and one number per column half to load.
@@ -419,19 +429,19 @@ __global__ void __launch_bounds__(THREADS, 1)
       for (int t = t0; t < tiles && ok; t += dt) {
         int tm, tn;
         tile_coords(p, t, tm, tn);
-        WeightScales ws(p.ws + (int64_t)min(2 * tn + warp - 2, p.nb - 1) * p.ldws + kb0, nkb, lane);
+        WeightScales ws(p.ws + (int64_t)min(C::BLOCKS * tn + warp - 2, p.nb - 1) * p.ldws + kb0, nkb, lane);
         for (int kb = 0; kb < nkb; ++kb, ++it) {
           const float w = ws.at(kb);
-          // The product of k-block it - 2 has landed: the arrival below belongs to the next phase of its
-          // barrier, and the epilogue has read the scales of it - 4 (it freed that buffer for it - 2).
+          // The product of k-block it - BUFS has landed: the arrival below belongs to the next phase of its
+          // barrier, and the epilogue has read the scales of it - 2 BUFS (it freed that buffer for it - BUFS).
           ok = warp_wait(sfull(sl), sp, abort_flag, 506) &&
-               (it < 2 || warp_wait(tfull(it & 1), ((it - 2) >> 1) & 1, abort_flag, 507));
+               (it < BUFS || warp_wait(tfull(it % BUFS), (it / BUFS - 1) & 1, abort_flag, 507));
           if (!ok) break;
           float4 x = reinterpret_cast<const float4*>(slots + sl * BM)[lane];
           x.x *= w; x.y *= w; x.z *= w; x.w *= w;
-          reinterpret_cast<float4*>(prods + ((it & 3) * 2 + warp - 2) * BM)[lane] = x;
+          reinterpret_cast<float4*>(prods + ((it % C::PRODS) * C::BLOCKS + warp - 2) * BM)[lane] = x;
           __syncwarp();
-          if (lane == 0) mbar_arrive_release(tfull(it & 1));
+          if (lane == 0) mbar_arrive_release(tfull(it % BUFS));
           if (++sl == SL) {
             sl = 0;
             sp ^= 1;
@@ -454,12 +464,10 @@ __global__ void __launch_bounds__(THREADS, 1)
     const uint32_t ta0 = tmem + ((uint32_t)(q4 * 32) << 16) + wg * 64;
     // (in the cluster's window for one CTA too: an arrival that returns no state is not waited for)
     const uint32_t go0 = cluster_map(go(0), rank - r);
-    int gs = 2 % S;  // stage of the k-block that takes over the buffer of k-block `it`, it + BUFS
-    if (lane == 0) {
-      mbar_arrive_cluster(go0);  // both buffers are empty
-      mbar_arrive_cluster(go0 + 8u);
-    }
-    float acc[2][64];
+    int gs = BUFS % S;  // stage of the k-block that takes over the buffer of k-block `it`, it + BUFS
+    if (lane == 0)
+      for (int b = 0; b < BUFS; ++b) mbar_arrive_cluster(go0 + 8u * b);  // every buffer is empty
+    float acc[C::BLOCKS][64];
     uint32_t it = 0, tile_parity = 0;
     bool ok = true;
     pdl_wait();
@@ -468,48 +476,57 @@ __global__ void __launch_bounds__(THREADS, 1)
       tile_coords(p, t, tm, tn);
       const int row = (tm * CTAS + r) * BM + lt;
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
+      for (int h = 0; h < C::BLOCKS; ++h)
 #pragma unroll
         for (int i = 0; i < 64; ++i) acc[h][i] = 0.f;
       if (nkb > 0) {
-        // A k-block is 4 loads of 32 columns, 2 of each half, through two register buffers.  The loads of
+        // A k-block is 2 loads of 32 columns per block of W, through two register buffers.  The loads of
         // the next half are issued between the additions of this one, across k-blocks too; the buffer goes
-        // back to the tensor core before its second half is added.
+        // back to the tensor core before its last half is added.
         uint32_t v[2][32];
-        ok = warp_wait(tfull(it & 1), (it >> 1) & 1, abort_flag, 504);
+        float s[C::BLOCKS];
+        auto landed = [&](uint32_t it) {  // the product of k-block `it`; its scales
+          if (!warp_wait(tfull(it % BUFS), (it / BUFS) & 1, abort_flag, 504)) return false;
+          fence_after();
+          return true;
+        };
+        auto scales = [&](uint32_t it) {
+#pragma unroll
+          for (int h = 0; h < C::BLOCKS; ++h) s[h] = prods[((it % C::PRODS) * C::BLOCKS + h) * BM + lt];
+        };
+        ok = landed(it);
         if (!ok) break;
-        fence_after();
-        float s0 = prods[(it & 3) * 2 * BM + lt], s1 = prods[(it & 3) * 2 * BM + BM + lt];
-        tmem_ld(ta0 + (it & 1) * BN, v[0]);
-        tmem_ld(ta0 + (it & 1) * BN + 32, v[1]);
+        scales(it);
+        tmem_ld(ta0 + (it % BUFS) * BN, v[0]);
+        tmem_ld(ta0 + (it % BUFS) * BN + 32, v[1]);
         for (int kb = 0; kb < nkb; ++kb, ++it) {
           const bool more = kb + 1 < nkb;
-          const uint32_t ta = ta0 + (it & 1) * BN + 128, nx = ta0 + ((it + 1) & 1) * BN;
-          const float sb = s1;
+          const uint32_t ta = ta0 + (it % BUFS) * BN, nx = ta0 + ((it + 1) % BUFS) * BN;
+          const float last = s[C::BLOCKS - 1];
           ld_wait(v[0]);
           ld_wait(v[1]);
-          add32(acc[0], v[0], s0);
-          tmem_ld(ta, v[0]);
-          add32(acc[0] + 32, v[1], s0);
-          tmem_ld(ta + 32, v[1]);
-          ld_wait(v[0]);
-          ld_wait(v[1]);
+          if constexpr (C::BLOCKS == 2) {
+            add32(acc[0], v[0], s[0]);
+            tmem_ld(ta + 128, v[0]);
+            add32(acc[0] + 32, v[1], s[0]);
+            tmem_ld(ta + 160, v[1]);
+            ld_wait(v[0]);
+            ld_wait(v[1]);
+          }
           fence_before();
           __syncwarp();
           // this buffer has been read: the tensor core may overwrite it
           if (lane == 0) mbar_arrive_cluster(go0 + 8u * gs);
           if (++gs == S) gs = 0;
-          add32(acc[1], v[0], sb);
+          float* a = acc[C::BLOCKS - 1];
+          add32(a, v[0], last);
           if (more) {
-            ok = warp_wait(tfull((it + 1) & 1), ((it + 1) >> 1) & 1, abort_flag, 504);
+            ok = landed(it + 1);
             if (!ok) break;
-            fence_after();
             tmem_ld(nx, v[0]);
-            const float* pr = prods + ((it + 1) & 3) * 2 * BM + lt;
-            s0 = pr[0];
-            s1 = pr[BM];
+            scales(it + 1);
           }
-          add32(acc[1] + 32, v[1], sb);
+          add32(a + 32, v[1], last);
           if (more) tmem_ld(nx + 32, v[1]);
         }
         if (!ok) break;
@@ -533,9 +550,9 @@ __global__ void __launch_bounds__(THREADS, 1)
           bulk_commit();
         }
       };
-      if (!p.act) {
+      if (BN == 128 || !p.act) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+        for (int h = 0; h < C::BLOCKS; ++h)
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
             const int col = tn * BN + h * 128 + wg * 64 + c * 32;
@@ -552,7 +569,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         const int f = tn * 128 + wg * 64;
         uint32_t m = 0;
 #pragma unroll
-        for (int i = 0; i < 64; ++i) acc[0][i] = silu_f(acc[0][i]) * acc[1][i];
+        for (int i = 0; i < 64; ++i) acc[0][i] = silu_f(acc[0][i]) * acc[C::BLOCKS - 1][i];
         if (f + 64 > p.features) {
 #pragma unroll
           for (int i = 0; i < 64; ++i)
@@ -588,7 +605,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       tile_coords(p, t0, tm, tn);
       float* dst = exchange + lt * XLD + wg * 64;
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
+      for (int h = 0; h < C::BLOCKS; ++h)
 #pragma unroll
         for (int i = 0; i < 64; i += 4)
           *reinterpret_cast<float4*>(dst + h * 128 + i) =
@@ -597,9 +614,9 @@ __global__ void __launch_bounds__(THREADS, 1)
       cluster_wait();  // every slice's sums are laid out
       if (!*abort_flag) {
         const int row0 = (tm * CTAS + r) * BM;
-        if (p.splits == 2) finish_rows<CTAS, 2>(p, exchange, slice, r, row0, tn, warp - 4, lane);
-        else if (p.splits == 4) finish_rows<CTAS, 4>(p, exchange, slice, r, row0, tn, warp - 4, lane);
-        else finish_rows<CTAS, 8>(p, exchange, slice, r, row0, tn, warp - 4, lane);
+        if (p.splits == 2) finish_rows<CTAS, BN, 2>(p, exchange, slice, r, row0, tn, warp - 4, lane);
+        else if (p.splits == 4) finish_rows<CTAS, BN, 4>(p, exchange, slice, r, row0, tn, warp - 4, lane);
+        else finish_rows<CTAS, BN, 8>(p, exchange, slice, r, row0, tn, warp - 4, lane);
       }
       cluster_arrive();
       cluster_wait();  // nobody reads this CTA's shared memory any more
@@ -882,16 +899,16 @@ cudaLaunchConfig_t cluster_config(int grid, int threads, int smem, int cluster, 
 
 // Shared-memory opt-in, and the check that the kernel is launched with the registers that its
 // warps redistribute (fewer would leave the epilogue waiting for them).
-template <int CTAS>
+template <int CTAS, int BN>
 cudaError_t tokens_opt_in() {
   static std::atomic<uint64_t> done{0};
   return once_per_device(done, []() -> cudaError_t {
     cudaFuncAttributes a;
-    cudaError_t e = cudaFuncGetAttributes(&a, gemm_fp8_tokens_kernel<CTAS>);
+    cudaError_t e = cudaFuncGetAttributes(&a, gemm_fp8_tokens_kernel<CTAS, BN>);
     if (e != cudaSuccess) return e;
     if (a.numRegs < LAUNCH_REGS) return cudaErrorInvalidDeviceFunction;
-    return cudaFuncSetAttribute(gemm_fp8_tokens_kernel<CTAS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                TokensCfg<CTAS>::SMEM);
+    return cudaFuncSetAttribute(gemm_fp8_tokens_kernel<CTAS, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                TokensCfg<CTAS, BN>::SMEM);
   });
 }
 
@@ -908,11 +925,11 @@ int clusters_of_sms(int cluster, int num_sms) {
   if (cluster == 1) return num_sms;
   if (int c = cache[cluster].load(std::memory_order_relaxed)) return c;
   cudaLaunchAttribute attr[2];
-  cudaLaunchConfig_t cfg = cluster_config(64 * cluster, THREADS, TokensCfg<1>::SMEM, cluster, attr);
+  cudaLaunchConfig_t cfg = cluster_config(64 * cluster, THREADS, TokensCfg<1, 256>::SMEM, cluster, attr);
   cfg.numAttrs = 1;
   int n = 0;
-  if (tokens_opt_in<1>() != cudaSuccess ||
-      cudaOccupancyMaxActiveClusters(&n, gemm_fp8_tokens_kernel<1>, &cfg) != cudaSuccess || n <= 0) {
+  if (tokens_opt_in<1, 256>() != cudaSuccess ||
+      cudaOccupancyMaxActiveClusters(&n, gemm_fp8_tokens_kernel<1, 256>, &cfg) != cudaSuccess || n <= 0) {
     cudaGetLastError();
     return num_sms / cluster;
   }
@@ -962,10 +979,10 @@ cudaError_t run_weights(const Fp8Gemm& g, Params p, int splits, cudaStream_t str
   return cudaLaunchKernelEx(&cfg, gemm_fp8_weights_kernel<NP, MW>, mx, mw, ms, p);
 }
 
-template <int CTAS>
+template <int CTAS, int BN>
 cudaError_t run_tokens(const Fp8Gemm& g, Params p, int splits, int num_sms, cudaStream_t stream) {
-  using C = TokensCfg<CTAS>;
-  if ((splits != 1 && splits != 2 && splits != 4 && splits != 8) || splits * CTAS > 8)
+  using C = TokensCfg<CTAS, BN>;
+  if ((splits != 1 && splits != 2 && splits != 4 && splits != 8) || splits * CTAS > 8 || (g.act && BN != 256))
     return cudaErrorInvalidValue;
   CUtensorMap mx, mw, ms;
   if (!make_map(&mx, g.xq, g.T, g.K, g.ldx, BM) || !make_map(&mw, g.wq, g.N, g.K, g.ldw, C::B_ROWS) ||
@@ -978,7 +995,7 @@ cudaError_t run_tokens(const Fp8Gemm& g, Params p, int splits, int num_sms, cuda
   if (tiles > 0x7fffffff / 16) return cudaErrorInvalidValue;
   p.splits = splits;
   p.kb_per_split = (p.num_kb + splits - 1) / splits;
-  cudaError_t e = tokens_opt_in<CTAS>();
+  cudaError_t e = tokens_opt_in<CTAS, BN>();
   if (e != cudaSuccess) return e;
   CUtensorMap mo = mx;  // not used without p.tma_out
   p.tma_out = g.act || p.vec;
@@ -987,7 +1004,7 @@ cudaError_t run_tokens(const Fp8Gemm& g, Params p, int splits, int num_sms, cuda
   cudaLaunchAttribute attr[2];
   cudaLaunchConfig_t cfg = cluster_config((int)most * splits * CTAS, THREADS, C::SMEM, splits * CTAS, attr);
   cfg.stream = stream;
-  return cudaLaunchKernelEx(&cfg, gemm_fp8_tokens_kernel<CTAS>, mx, mw, ms, mo, p);
+  return cudaLaunchKernelEx(&cfg, gemm_fp8_tokens_kernel<CTAS, BN>, mx, mw, ms, mo, p);
 }
 
 }  // namespace
@@ -1001,10 +1018,28 @@ Fp8Plan fp8_plan(int T, int N, int K, int act, int num_sms) {
     for (int s = 2; s <= 8; ++s)
       if (num_kb / s >= 2 && tiles <= clusters_of_half_sms(s, num_sms)) pl.splits = s;
   } else {
-    const int64_t tiles = (int64_t)((T + BM - 1) / BM) * ((N + BN - 1) / BN);
-    for (int s = 2; s <= 4; s *= 2)
-      if (num_kb / s >= 4 && tiles <= clusters_of_sms(s, num_sms)) pl.splits = s;
-    pl.np = T > BM && pl.splits == 1 ? -2 : -1;
+    // Fewest nanoseconds by a model of one CTA's time: its k-blocks at 460 ns for a tile of 256 features
+    // and 310 ns for one of 128 (measured; below that the epilogue's latency per k-block is what
+    // remains), and the exchange of the slices' sums, 5.0 and 6.2 us for 2 and 4 slices of 256 features,
+    // 2.4 and 3.2 us of 128.  Examples of both sides, T x N x K: 256 x 4096 x 4096, 128 features in 2
+    // slices 11.6 us, 256 features in 4 slices 13.5 us, neither split 13.8 and 18.9 us; 512 x 6144 x
+    // 4096, 128 features 24.5 us, 256 features 20.2 us.  Where 256 features in one slice win and there
+    // are two rows of tiles or more, pairs of CTAs run them: 16384 x 24576 x 4096 with SiLU-and-mul
+    // 1572 us, single CTAs 1697 us; equal at 512 tokens.
+    int64_t best = -1;
+    for (int bn = 256; bn >= (act ? 256 : 128); bn /= 2) {
+      const int64_t tiles = (int64_t)((T + BM - 1) / BM) * ((N + bn - 1) / bn);
+      for (int s = 1; s <= 4; s *= 2) {
+        if (s > 1 && (num_kb / s < 4 || tiles > clusters_of_sms(s, num_sms))) continue;
+        const int64_t kbs = (num_kb + s - 1) / s * (s > 1 ? 1 : (tiles + num_sms - 1) / num_sms);
+        const int64_t exchange = s == 1 ? 0 : bn == 256 ? 3800 + 600 * s : 1600 + 400 * s;
+        const int64_t ns = kbs * (bn == 256 ? 460 : 310) + exchange;
+        if (best >= 0 && ns >= best) continue;
+        best = ns;
+        pl.np = bn == 128 ? -3 : s == 1 && T > BM ? -2 : -1;
+        pl.splits = s;
+      }
+    }
   }
   return pl;
 }
@@ -1026,8 +1061,9 @@ cudaError_t gemm_fp8(const Fp8Gemm& g, const Fp8Plan& pl, int num_sms, cudaStrea
   p.ldos = g.ldos;
   p.vec = g.ldo % 8 == 0 && (reinterpret_cast<uintptr_t>(g.out) & 15) == 0;
   switch (pl.np) {
-    case -1: return run_tokens<1>(g, p, pl.splits, num_sms, stream);
-    case -2: return run_tokens<2>(g, p, pl.splits, num_sms, stream);
+    case -1: return run_tokens<1, 256>(g, p, pl.splits, num_sms, stream);
+    case -2: return run_tokens<2, 256>(g, p, pl.splits, num_sms, stream);
+    case -3: return run_tokens<1, 128>(g, p, pl.splits, num_sms, stream);
     case 16: return g.act ? run_weights<16, 2>(g, p, pl.splits, stream) : run_weights<16, 1>(g, p, pl.splits, stream);
     case 32: return g.act ? run_weights<32, 2>(g, p, pl.splits, stream) : run_weights<32, 1>(g, p, pl.splits, stream);
     case 64: return g.act ? cudaErrorInvalidValue : run_weights<64, 1>(g, p, pl.splits, stream);
