@@ -38,8 +38,8 @@ struct Fp8Gemm {
 };
 
 // Which kernel computes a product, and over how many CTAs of a cluster K is split.  np = -1, -2, -3: the
-// kernel with the tokens on the MMA's M side (any T), 1 CTA per tile of 256 features, 2 CTAs per tile of
-// 256, 1 CTA per tile of 128 (not with act); splits 1, 2, 4 or 8, splits x CTAs at most 8.
+// kernel with the tokens on the MMA's M side (any T), 1 CTA per tile of 256 features (splits 1, 2, 4), 2
+// CTAs per tile of 256 (splits 1), 1 CTA per tile of 128 (splits 1, 2, 4; not with act).
 // np = 16, 32, 64 (with act 16, 32): the weights on the M side, np >= T tokens, 1 .. 8 splits.
 struct Fp8Plan {
   int np = -1, splits = 1;

@@ -234,14 +234,13 @@ __device__ __forceinline__ void finish_bf16x4(const Params& p, int t, int n, con
   }
 }
 
-// Tokens [128 slice / S, 128 (slice + 1) / S) of this CTA's 128, whose sums lie in S CTAs of the cluster
-// (ranks r, r + CTAS, ...): added in the order of the slices, finished and stored.  A warp takes a
+// Tokens [128 slice / S, 128 (slice + 1) / S) of a tile whose sums lie in the S CTAs of the cluster: added in the order of the slices, finished and stored.  A warp takes a
 // token's sums of one slice and 128 features as one 512-byte row (remote stores of each thread's own 16
 // bytes were slower by half) and has 16 of them in flight.
-template <int CTAS, int BN, int S>
-__device__ __forceinline__ void finish_rows(const Params& p, float* exchange, int slice, int r, int row0, int tn,
-                                            int w, int lane) {
-  constexpr int XLD = TokensCfg<CTAS, BN>::XLD, NB = BN / 128;
+template <int BN, int S>
+__device__ __forceinline__ void finish_rows(const Params& p, float* exchange, int slice, int row0, int tn, int w,
+                                            int lane) {
+  constexpr int XLD = TokensCfg<1, BN>::XLD, NB = BN / 128;
   constexpr int PER = BM / S, G = 16 / NB / S;
   for (int tl = w * G; tl < PER; tl += EPI_THREADS / 32 * G) {
     const int r0 = slice * PER + tl;
@@ -250,7 +249,7 @@ __device__ __forceinline__ void finish_rows(const Params& p, float* exchange, in
     float4 a[G][S][NB];
 #pragma unroll
     for (int s = 0; s < S; ++s) {
-      const uint32_t at = cluster_map(src, s * CTAS + r);
+      const uint32_t at = cluster_map(src, s);
 #pragma unroll
       for (int i = 0; i < G; ++i)
 #pragma unroll
@@ -278,8 +277,8 @@ __device__ __forceinline__ void finish_rows(const Params& p, float* exchange, in
   }
 }
 
-// One tile per cluster of splits x CTAS CTAs (each group of CTAS a slice of K), or, with splits = 1,
-// persistent CTAs that walk the tiles.
+// With one CTA per tile: one tile per cluster of splits CTAs, each a slice of K, or, with splits = 1,
+// persistent CTAs that walk the tiles.  With pairs: persistent pairs.
 template <int CTAS, int BN>
 __global__ void __launch_bounds__(THREADS, 1)
     gemm_fp8_tokens_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
@@ -308,8 +307,9 @@ __global__ void __launch_bounds__(THREADS, 1)
   volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + C::BARS);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + C::BARS) + 1;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int rank = p.splits * CTAS > 1 ? (int)cluster_rank() : 0;
-  const int r = rank % CTAS, slice = rank / CTAS;
+  const int rank = CTAS == 2 || p.splits > 1 ? (int)cluster_rank() : 0;
+  const int r = CTAS == 2 ? rank : 0, slice = CTAS == 2 ? 0 : rank;  // CTA of the pair; slice of K
+  const int splits = CTAS == 2 ? 1 : p.splits;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < S; ++s) {
@@ -337,7 +337,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   pdl_trigger();
 
   const int tiles = p.tiles_m * p.tiles_n;
-  const int t0 = blockIdx.x / (p.splits * CTAS), dt = gridDim.x / (p.splits * CTAS);
+  const int t0 = blockIdx.x / (splits * CTAS), dt = gridDim.x / (splits * CTAS);
   const int kb0 = slice * p.kb_per_split;
   const int nkb = max(0, min(p.num_kb - kb0, p.kb_per_split));
   if (warp < 4) {
@@ -372,7 +372,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             tma_load_2d(st + C::A_BYTES, &map_w, go(s), k, tn * BN);
           } else {
             if (r == 0) mbar_arrive_expect_tx(go(s), 2 * C::STAGE);
-            const uint32_t gb = cluster_map(go(s), rank - r);
+            const uint32_t gb = cluster_map(go(s), 0);
             tma_load_2d_pair(st, &map_x, gb, k, row0);
             tma_load_2d_pair(st + C::A_BYTES, &map_w, gb, k, tn * BN + r * C::B_ROWS);
           }
@@ -393,7 +393,6 @@ __global__ void __launch_bounds__(THREADS, 1)
     } else if (warp == 1 && r == 0) {
       // ---------------------------------------------------------------- MMA issuer (a pair's even CTA)
       const uint32_t tbase = __shfl_sync(FULL_MASK, tmem, 0);
-      const uint32_t both = 3u << (rank - r);  // the pair's ranks in the cluster
       const uint32_t total = (uint32_t)nkb * (t0 < tiles ? (tiles - t0 + dt - 1) / dt : 0);
       const uint64_t ad0 = sdesc(smem_u32(smem)), bd0 = sdesc(smem_u32(smem) + C::A_BYTES);
       int s = 0, phase = 0;
@@ -407,8 +406,8 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
           for (int k = 0; k < BK / 32; ++k)
             mma_f8<CTAS>(d, ad + 2 * k, bd + 2 * k, idesc_f8(CTAS * BM, BN), k > 0 ? 1u : 0u);
-          commit<CTAS>(empty(s), both);
-          commit<CTAS>(tfull(it % BUFS), both);
+          commit<CTAS>(empty(s));
+          commit<CTAS>(tfull(it % BUFS));
         }
         __syncwarp();
         if (++s == S) {
@@ -416,7 +415,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           phase ^= 1;
         }
       }
-      if (elect_one()) commit<CTAS>(final_bar, both);
+      if (elect_one()) commit<CTAS>(final_bar);
       if (lane == 0) mbar_drain(final_bar, 0);
     } else if (warp >= 2 && warp - 2 < C::BLOCKS) {
       // ---------------------------------------------------------------- scales of weight block warp - 2
@@ -450,7 +449,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       }
     }
     __syncwarp();
-    if (p.splits > 1) {
+    if (splits > 1) {
       cluster_arrive();  // (the epilogue's phases, see there)
       cluster_wait();
       cluster_arrive();
@@ -463,7 +462,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     const int lt = q4 * 32 + lane;  // this thread's token of the CTA's 128
     const uint32_t ta0 = tmem + ((uint32_t)(q4 * 32) << 16) + wg * 64;
     // (in the cluster's window for one CTA too: an arrival that returns no state is not waited for)
-    const uint32_t go0 = cluster_map(go(0), rank - r);
+    const uint32_t go0 = cluster_map(go(0), CTAS == 2 ? 0 : rank);
     int gs = BUFS % S;  // stage of the k-block that takes over the buffer of k-block `it`, it + BUFS
     if (lane == 0)
       for (int b = 0; b < BUFS; ++b) mbar_arrive_cluster(go0 + 8u * b);  // every buffer is empty
@@ -531,7 +530,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
         if (!ok) break;
       }
-      if (p.splits > 1) break;  // one tile per cluster; finished below
+      if (splits > 1) break;  // one tile per cluster; finished below
       // Each warp stores pieces of 32 rows x 64 bytes through shared memory by TMA, which writes whole
       // sectors and drops what lies outside (stores of each thread's own row took 9000 clocks per tile,
       // a quarter of it, as long as nothing overlaps them).
@@ -598,7 +597,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     }
     if (lane == 0) bulk_wait();  // every piece has been written
     __syncwarp();
-    if (p.splits > 1) {
+    if (splits > 1) {
       // Every CTA lays its sums out in its own shared memory, over its idle ring (the last MMA has
       // completed), [token][feature]; after the cluster's barrier each slice finishes its share.
       int tm, tn;
@@ -613,10 +612,8 @@ __global__ void __launch_bounds__(THREADS, 1)
       cluster_arrive();
       cluster_wait();  // every slice's sums are laid out
       if (!*abort_flag) {
-        const int row0 = (tm * CTAS + r) * BM;
-        if (p.splits == 2) finish_rows<CTAS, BN, 2>(p, exchange, slice, r, row0, tn, warp - 4, lane);
-        else if (p.splits == 4) finish_rows<CTAS, BN, 4>(p, exchange, slice, r, row0, tn, warp - 4, lane);
-        else finish_rows<CTAS, BN, 8>(p, exchange, slice, r, row0, tn, warp - 4, lane);
+        if (splits == 2) finish_rows<BN, 2>(p, exchange, slice, tm * BM, tn, warp - 4, lane);
+        else finish_rows<BN, 4>(p, exchange, slice, tm * BM, tn, warp - 4, lane);
       }
       cluster_arrive();
       cluster_wait();  // nobody reads this CTA's shared memory any more
@@ -982,8 +979,7 @@ cudaError_t run_weights(const Fp8Gemm& g, Params p, int splits, cudaStream_t str
 template <int CTAS, int BN>
 cudaError_t run_tokens(const Fp8Gemm& g, Params p, int splits, int num_sms, cudaStream_t stream) {
   using C = TokensCfg<CTAS, BN>;
-  if ((splits != 1 && splits != 2 && splits != 4 && splits != 8) || splits * CTAS > 8 || (g.act && BN != 256))
-    return cudaErrorInvalidValue;
+  if ((splits != 1 && (CTAS == 2 || (splits != 2 && splits != 4))) || (g.act && BN != 256)) return cudaErrorInvalidValue;
   CUtensorMap mx, mw, ms;
   if (!make_map(&mx, g.xq, g.T, g.K, g.ldx, BM) || !make_map(&mw, g.wq, g.N, g.K, g.ldw, C::B_ROWS) ||
       !make_scale_map(&ms, g.xs, p.num_kb, g.T, g.ldxs, BM))
@@ -1013,32 +1009,36 @@ Fp8Plan fp8_plan(int T, int N, int K, int act, int num_sms) {
   Fp8Plan pl;
   const int num_kb = (K + BK - 1) / BK;
   if (T <= (act ? 32 : 64)) {
+    // Few tokens: the weights are streamed once, by as many CTAs as the GPU holds.
     pl.np = T <= 16 ? 16 : T <= 32 ? 32 : 64;
     const int rows = act ? 256 : 128, tiles = (N + rows - 1) / rows;
     for (int s = 2; s <= 8; ++s)
-      if (num_kb / s >= 2 && tiles <= clusters_of_half_sms(s, num_sms)) pl.splits = s;
-  } else {
-    // Fewest nanoseconds by a model of one CTA's time: its k-blocks at 460 ns for a tile of 256 features
-    // and 310 ns for one of 128 (measured; below that the epilogue's latency per k-block is what
-    // remains), and the exchange of the slices' sums, 5.0 and 6.2 us for 2 and 4 slices of 256 features,
-    // 2.4 and 3.2 us of 128.  Examples of both sides, T x N x K: 256 x 4096 x 4096, 128 features in 2
-    // slices 11.6 us, 256 features in 4 slices 13.5 us, neither split 13.8 and 18.9 us; 512 x 6144 x
-    // 4096, 128 features 24.5 us, 256 features 20.2 us.  Where 256 features in one slice win and there
-    // are two rows of tiles or more, pairs of CTAs run them: 16384 x 24576 x 4096 with SiLU-and-mul
-    // 1572 us, single CTAs 1697 us; equal at 512 tokens.
-    int64_t best = -1;
-    for (int bn = 256; bn >= (act ? 256 : 128); bn /= 2) {
-      const int64_t tiles = (int64_t)((T + BM - 1) / BM) * ((N + bn - 1) / bn);
-      for (int s = 1; s <= 4; s *= 2) {
-        if (s > 1 && (num_kb / s < 4 || tiles > clusters_of_sms(s, num_sms))) continue;
-        const int64_t kbs = (num_kb + s - 1) / s * (s > 1 ? 1 : (tiles + num_sms - 1) / num_sms);
-        const int64_t exchange = s == 1 ? 0 : bn == 256 ? 3800 + 600 * s : 1600 + 400 * s;
-        const int64_t ns = kbs * (bn == 256 ? 460 : 310) + exchange;
-        if (best >= 0 && ns >= best) continue;
-        best = ns;
-        pl.np = bn == 128 ? -3 : s == 1 && T > BM ? -2 : -1;
-        pl.splits = s;
-      }
+      if (num_kb >= s && tiles <= clusters_of_half_sms(s, num_sms)) pl.splits = s;
+    // .. unless there is little to stream per tile: 61 x 7216 x 624 takes 8.3 us so, 5.3 us below
+    if (pl.np < 64 || pl.splits >= 4 || num_kb > 8) return pl;
+    pl = Fp8Plan{};
+  }
+  // Fewest nanoseconds by a model of one CTA's time: its k-blocks at 460 ns for a tile of 256 features
+  // and 310 ns for one of 128 (measured; below that the epilogue's latency per k-block is what
+  // remains), and the exchange of the slices' sums, 5.0 and 6.2 us for 2 and 4 slices of 256 features,
+  // 2.4 and 3.2 us of 128.  Examples of both sides, T x N x K: 256 x 4096 x 4096, 128 features in 2
+  // slices 11.6 us, 256 features in 4 slices 13.5 us, neither split 13.8 and 18.9 us; 512 x 6144 x
+  // 4096, 128 features 24.5 us, 256 features 20.2 us.  Where 256 features in one slice win and there
+  // are two rows of tiles or more, pairs of CTAs run them: 16384 x 24576 x 4096 with SiLU-and-mul
+  // 1572 us, single CTAs 1697 us; equal at 512 tokens; 612 x 7168 x 352 11.1 us against 7.6 us, so K
+  // has to fill 8 blocks.
+  int64_t best = -1;
+  for (int bn = 256; bn >= (act ? 256 : 128); bn /= 2) {
+    const int64_t tiles = (int64_t)((T + BM - 1) / BM) * ((N + bn - 1) / bn);
+    for (int s = 1; s <= 4; s *= 2) {
+      if (s > 1 && (num_kb / s < 4 || tiles > clusters_of_sms(s, num_sms))) continue;
+      const int64_t kbs = (num_kb + s - 1) / s * (s > 1 ? 1 : (tiles + num_sms - 1) / num_sms);
+      const int64_t exchange = s == 1 ? 0 : bn == 256 ? 3800 + 600 * s : 1600 + 400 * s;
+      const int64_t ns = kbs * (bn == 256 ? 460 : 310) + exchange;
+      if (best >= 0 && ns >= best) continue;
+      best = ns;
+      pl.np = bn == 128 ? -3 : s == 1 && T > BM && num_kb >= 8 ? -2 : -1;
+      pl.splits = s;
     }
   }
   return pl;

@@ -139,16 +139,16 @@ __device__ __forceinline__ void tmem_dealloc(uint32_t base, uint32_t cols) {
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(base), "r"(cols));
 }
 
-// Arrival on this barrier (of a pair: on the barrier at this offset in the cluster's CTAs of `mask`) once
-// every MMA issued so far by this thread has completed.
+// Arrival on this barrier (of a pair: on the barrier at this offset in both CTAs) once every MMA issued
+// so far by this thread has completed.
 template <int CTAS>
-__device__ __forceinline__ void commit(uint32_t bar, uint32_t mask = 0) {
+__device__ __forceinline__ void commit(uint32_t bar) {
   if constexpr (CTAS == 1)
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
   else
     asm volatile(
         "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
-        "h"((uint16_t)mask)
+        "h"((uint16_t)3)
         : "memory");
 }
 

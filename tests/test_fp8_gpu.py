@@ -186,9 +186,11 @@ def _plans(t, act):
         if np_ >= t:
             for splits in (1, 2, 3, 5, 8):
                 yield [np_, splits]
-    for kind, ctas in ((1, 1), (2, 2)) if act else ((1, 1), (2, 2), (3, 1)):
-        for splits in (1, 2, 4, 8 // ctas):
-            yield [-kind, splits]
+    yield [-2, 1]
+    for splits in (1, 2, 4):
+        yield [-1, splits]
+        if not act:
+            yield [-3, splits]
 
 
 @pytest.mark.parametrize("t,n,k", [(1, 384, 272), (13, 100, 1712), (32, 640, 1040), (50, 250, 512), (128, 900, 2064), (300, 260, 1312)])
@@ -218,7 +220,7 @@ def test_every_kernel_variant(ops, t, n, k):
 
 def test_plans_refused(ops):
     x, w = ops.quant_fp8(_acts(20, 256)), _weight(256, 256)
-    for plan in ([16, 1], [32, 9], [128, 1], [24, 1], [32, 0], [32], [-1, 3], [-1, 16], [-2, 8], [-1, 0], [0, 1], [-4, 1]):
+    for plan in ([16, 1], [32, 9], [128, 1], [24, 1], [32, 0], [32], [-1, 3], [-1, 8], [-2, 2], [-1, 0], [0, 1], [-4, 1]):
         with pytest.raises(RuntimeError):
             ops.C.linear_fp8(*x, *w, None, plan)
     with pytest.raises(RuntimeError):
