@@ -160,23 +160,6 @@ __device__ __forceinline__ float silu_f(float g) {
   return g * q;
 }
 
-// bf16 values [c, c + 32) of one row.
-__device__ __forceinline__ void store_bf16_32(const Params& p, int row, int c, const float* acc) {
-  if (row >= p.T || c >= p.N) return;
-  __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(p.out) + (int64_t)row * p.ldo + c;
-  const int n = p.N - c;
-#pragma unroll
-  for (int i = 0; i < 32; i += 8) {
-    if (p.vec && i + 8 <= n) {
-      *reinterpret_cast<uint4*>(dst + i) = f32_to_bf16x8(acc + i);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (i + j < n) dst[i + j] = __float2bfloat16_rn(acc[i + j]);
-    }
-  }
-}
-
 // acc += s * 32 values, two per instruction: half the issue slots of scalar additions (3% of the kernel).
 __device__ __forceinline__ void add32(float* acc, const uint32_t (&v)[32], float s) {
 #pragma unroll
@@ -537,16 +520,27 @@ __global__ void __launch_bounds__(THREADS, 1)
       const int row0 = (tm * CTAS + r) * BM + q4 * 32;
       uint8_t* mine = staging + (warp - 4) * 2048;
       auto piece = [&](const uint4* w4, int col) {
-        if (lane == 0) bulk_wait_read();  // the piece before has left
+        if (lane == 0 && p.tma_out) bulk_wait_read();  // the piece before has left
         __syncwarp();
 #pragma unroll
         for (int c = 0; c < 4; ++c)  // 64-byte swizzle: no bank conflicts
           *reinterpret_cast<uint4*>(mine + lane * 64 + (c ^ ((lane >> 1) & 3)) * 16) = w4[c];
-        fence_proxy_async();
-        __syncwarp();
-        if (lane == 0) {
-          tma_store_2d(&map_o, smem_u32(mine), col, row0);
-          bulk_commit();
+        if (p.tma_out) {
+          fence_proxy_async();
+          __syncwarp();
+          if (lane == 0) {
+            tma_store_2d(&map_o, smem_u32(mine), col, row0);
+            bulk_commit();
+          }
+        } else {  // bf16 rows that TMA cannot address: a lane per column, one row at a time
+          __syncwarp();
+          if (col + lane < p.N) {
+            __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(p.out) + (int64_t)row0 * p.ldo + col + lane;
+            const int n = min(32, p.T - row0);
+            for (int i = 0; i < n; ++i, dst += p.ldo)
+              *dst = *reinterpret_cast<const __nv_bfloat16*>(mine + i * 64 + ((lane >> 3) ^ ((i >> 1) & 3)) * 16 +
+                                                             (lane & 7) * 2);
+          }
         }
       };
       if (BN == 128 || !p.act) {
@@ -556,12 +550,8 @@ __global__ void __launch_bounds__(THREADS, 1)
           for (int c = 0; c < 2; ++c) {
             const int col = tn * BN + h * 128 + wg * 64 + c * 32;
             const float* a = acc[h] + c * 32;
-            if (p.tma_out) {
-              const uint4 w4[4] = {f32_to_bf16x8(a), f32_to_bf16x8(a + 8), f32_to_bf16x8(a + 16), f32_to_bf16x8(a + 24)};
-              if (row0 < p.T && col < p.N) piece(w4, col);
-            } else {
-              store_bf16_32(p, row, col, a);
-            }
+            const uint4 w4[4] = {f32_to_bf16x8(a), f32_to_bf16x8(a + 8), f32_to_bf16x8(a + 16), f32_to_bf16x8(a + 24)};
+            if (row0 < p.T && col < p.N) piece(w4, col);
           }
       } else {
         // SiLU-and-mul; the values stay fp32 up to the 8-bit rounding
