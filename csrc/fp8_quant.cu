@@ -14,8 +14,11 @@ constexpr int QGROUPS = 4;  // groups per half-warp, all of whose loads are in f
 
 // A half-warp holds a group of 128 as 16 lanes x 8 values.  The half-warps of a CTA take consecutive
 // tokens of the same groups, so that a group's scales leave as one 32-byte sector (scales are stored
-// token-contiguous, the order in which the products read them).  Measured, 16384 x 4096: 33.9 us
-// (6.0 TB/s); 16 rows 34.3 us, 2 groups 36.2 us, 8 groups 35.5 us, 16 groups 44 us.
+// token-contiguous, the order in which the products read them).  With a reduction and two divisions
+// per group in every lane the kernel was bound by its instructions (79% of the issue slots, 33.8 us at
+// 16384 x 4096); with the four groups' maxima and divisions spread over the lanes it is bound by
+// memory: 31.0 us, 6.5 TB/s.  2 groups per half-warp 35.7 us; 16 rows per CTA, 8 or 16 groups were
+// slower as well.
 __global__ void __launch_bounds__(QROWS * 16) quant_fp8_kernel(const __nv_bfloat16* __restrict__ x, int64_t ldx,
                                                                uint8_t* __restrict__ q, float* __restrict__ s,
                                                                int64_t lds, int T, int K) {
@@ -23,39 +26,45 @@ __global__ void __launch_bounds__(QROWS * 16) quant_fp8_kernel(const __nv_bfloat
   pdl_trigger();  // the next kernel may start its prologue
   const int hw = threadIdx.x >> 4, l = threadIdx.x & 15;
   const int kb = (K + FP8_GROUP - 1) / FP8_GROUP;
-  const int chunks = (kb + QGROUPS - 1) / QGROUPS;
-  const int t = (int)(blockIdx.x / chunks) * QROWS + hw;
-  const int g0 = (int)(blockIdx.x % chunks) * QGROUPS;
+  const int64_t t = ((int64_t)blockIdx.z * gridDim.y + blockIdx.y) * QROWS + hw;
+  const int g0 = (int)blockIdx.x * QGROUPS;
   uint4 v[QGROUPS];
 #pragma unroll
   for (int i = 0; i < QGROUPS; ++i) {
     const int c = (g0 + i) * FP8_GROUP + l * 8;
     v[i] = make_uint4(0, 0, 0, 0);
-    if (t < T && c < K) v[i] = *reinterpret_cast<const uint4*>(x + (int64_t)t * ldx + c);
+    if (t < T && c < K) v[i] = *reinterpret_cast<const uint4*>(x + t * ldx + c);
   }
+  uint32_t m[QGROUPS];
 #pragma unroll
   for (int i = 0; i < QGROUPS; ++i) {
     // |bf16| as 16-bit integers, two per word
-    uint32_t m = __vmaxu2(__vmaxu2(v[i].x & 0x7fff7fffu, v[i].y & 0x7fff7fffu),
-                          __vmaxu2(v[i].z & 0x7fff7fffu, v[i].w & 0x7fff7fffu));
-    m = max(m & 0xffff0000u, m << 16);  // as an fp32 magnitude
-    const Fp8Scale sc = fp8_scale(half_warp_umax(m));
+    m[i] = __vmaxu2(__vmaxu2(v[i].x & 0x7fff7fffu, v[i].y & 0x7fff7fffu),
+                    __vmaxu2(v[i].z & 0x7fff7fffu, v[i].w & 0x7fff7fffu));
+    m[i] = max(m[i] & 0xffff0000u, m[i] << 16);  // as an fp32 magnitude
+  }
+  constexpr int LPG = 16 / QGROUPS;  // lanes that hold a group's maximum
+  const Fp8Scale sc = fp8_scale(half_warp_umax(m));
+  if (l % LPG == 0 && t < T && g0 + l / LPG < kb) s[(g0 + l / LPG) * lds + t] = sc.scale;
+#pragma unroll
+  for (int i = 0; i < QGROUPS; ++i) {
+    const float inv = __shfl_sync(FULL_MASK, sc.inv, i * LPG, 16);
     const int c = (g0 + i) * FP8_GROUP + l * 8;
     if (t < T && c < K) {
       float f[8];
       bf16x8_to_f32(v[i], f);
-      *reinterpret_cast<uint2*>(q + (int64_t)t * K + c) = f32x8_to_e4m3(f, sc.inv);
+      *reinterpret_cast<uint2*>(q + t * K + c) = f32x8_to_e4m3(f, inv);
     }
-    if (l == 0 && t < T && g0 + i < kb) s[(g0 + i) * lds + t] = sc.scale;
   }
 }
 
 constexpr int TPR = 128;    // threads per row of the norm
 
 // One CTA of 128 threads per row, 8 values per thread and step; a group of 128 is the 16 lanes of a
-// half-warp.  The row is kept as bf16 between the two passes over them (the residual's rounding is
-// exact in it): half the registers of fp32, so that enough rows are in flight to cover the latency.  Measured, 8191 x
-// 5120: 48 us (6.1 TB/s); 256 threads per row 54 us, two rows per CTA 51 us, fp32 in between 63 us.
+// half-warp.  The row is kept as bf16 between the two passes over it (the residual's rounding is exact
+// in it): half the registers of fp32, so that enough rows are in flight to cover the latency.
+// Measured: 8191 x 5120 47.2 us (6.2 TB/s), 8192 x 8192 77.0 us; scales of one group at a time 47.9
+// and 83.8 us; 256 threads per row 54 us, two rows per CTA 51 us, fp32 in between 63 us (8191 x 5120).
 template <int NI>
 __global__ void __launch_bounds__(TPR) add_rmsnorm_fp8_kernel(const __nv_bfloat16* __restrict__ x, int64_t ldx,
                                                               __nv_bfloat16* __restrict__ residual,
@@ -117,25 +126,35 @@ __global__ void __launch_bounds__(TPR) add_rmsnorm_fp8_kernel(const __nv_bfloat1
   for (int i = 0; i < TPR / 32; ++i) ss += red[i];
   const float inv_rms = rsqrtf(ss / (float)K + eps);
   const uint4* wr = reinterpret_cast<const uint4*>(w);
+  constexpr int G = NI < 3 ? NI : 4;  // groups per half-warp whose scales are made at once
+  constexpr int LPG = 16 / G;
 #pragma unroll
-  for (int i = 0; i < NI; ++i) {
-    const int c = tid + i * TPR;
-    uint32_t m = 0;
-    float o[8];
-    bf16x8_to_f32(v[i], o);
-    if (c < nvec) {
-      float wf[8];
-      bf16x8_to_f32(wr[c], wf);
+  for (int i0 = 0; i0 < NI; i0 += G) {
+    uint32_t m[G];
+    float o[G][8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        o[j] = o[j] * inv_rms * wf[j];
-        m = max(m, __float_as_uint(o[j]) & 0x7fffffffu);
+    for (int g = 0; g < G; ++g) {
+      const int c = tid + (i0 + g) * TPR;
+      m[g] = 0;
+      if (i0 + g < NI && c < nvec) {
+        float wf[8];
+        bf16x8_to_f32(v[i0 + g], o[g]);
+        bf16x8_to_f32(wr[c], wf);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          o[g][j] = o[g][j] * inv_rms * wf[j];
+          m[g] = max(m[g], __float_as_uint(o[g][j]) & 0x7fffffffu);
+        }
       }
     }
     const Fp8Scale sc = fp8_scale(half_warp_umax(m));
-    if (c < nvec) {
-      *reinterpret_cast<uint2*>(q + (int64_t)row * K + c * 8) = f32x8_to_e4m3(o, sc.inv);
-      if ((c & 15) == 0) s[(int64_t)(c >> 4) * lds + row] = sc.scale;
+    const int cs = (tid & ~15) + (i0 + (tid & 15) / LPG) * TPR;  // first vector of this lane's group
+    if ((tid & 15) % LPG == 0 && i0 + (tid & 15) / LPG < NI && cs < nvec) s[(int64_t)(cs >> 4) * lds + row] = sc.scale;
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      const int c = tid + (i0 + g) * TPR;
+      const float inv = __shfl_sync(FULL_MASK, sc.inv, g * LPG, 16);
+      if (i0 + g < NI && c < nvec) *reinterpret_cast<uint2*>(q + (int64_t)row * K + c * 8) = f32x8_to_e4m3(o[g], inv);
     }
   }
 }
@@ -146,10 +165,12 @@ cudaError_t launch_quant_fp8(const void* x, int64_t ldx, void* q, float* s, int6
                              cudaStream_t stream) {
   if (T == 0) return cudaSuccess;
   const int kb = (K + FP8_GROUP - 1) / FP8_GROUP;
-  const int64_t ctas = (int64_t)((T + QROWS - 1) / QROWS) * ((kb + QGROUPS - 1) / QGROUPS);
-  if (K % 16 || ldx % 8 || ctas > 0x7fffffff) return cudaErrorInvalidValue;
-  return launch_pdl(quant_fp8_kernel, dim3((unsigned)ctas), dim3(QROWS * 16), 0, stream,
-             static_cast<const __nv_bfloat16*>(x), ldx, static_cast<uint8_t*>(q), s, lds, T, K);
+  const int64_t rows = ((int64_t)T + QROWS - 1) / QROWS;  // in CTAs; a grid's y goes to 65535 only
+  const int64_t ny = rows < 32768 ? rows : 32768, nz = (rows + ny - 1) / ny;
+  const int chunks = (kb + QGROUPS - 1) / QGROUPS;
+  if (K % 16 || ldx % 8 || nz > 65535) return cudaErrorInvalidValue;
+  return launch_pdl(quant_fp8_kernel, dim3(chunks, (unsigned)ny, (unsigned)nz), dim3(QROWS * 16), 0, stream,
+                    static_cast<const __nv_bfloat16*>(x), ldx, static_cast<uint8_t*>(q), s, lds, T, K);
 }
 
 cudaError_t launch_add_rmsnorm_fp8(const void* x, int64_t ldx, void* residual, const void* w, void* q, float* s,

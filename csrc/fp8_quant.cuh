@@ -24,11 +24,29 @@ __device__ __forceinline__ Fp8Scale fp8_scale(uint32_t amax_bits) {
   return {__fdiv_rn(a, FP8_E4M3_MAX), __fdiv_rn(FP8_E4M3_MAX, a)};
 }
 
-// Maximum over the 16 lanes of a half-warp (all 32 lanes call it).
-__device__ __forceinline__ uint32_t half_warp_umax(uint32_t v) {
+// Maxima over the 16 lanes of a half-warp, of G values per lane at once (all 32 lanes call it).  Each
+// step halves the values that a lane still holds, until lane l has that of value l / (16 / G); the
+// division that follows is then made once per lane instead of once per value.
+template <int G>
+__device__ __forceinline__ uint32_t half_warp_umax(const uint32_t (&v)[G]) {
+  static_assert(G == 1 || G == 2 || G == 4, "values per lane");
+  const int l = threadIdx.x & 15;
+  uint32_t m[G];
 #pragma unroll
-  for (int o = 8; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(FULL_MASK, v, o));
-  return v;
+  for (int i = 0; i < G; ++i) m[i] = v[i];
+  int o = 8;
+#pragma unroll
+  for (int n = G / 2; n > 0; n >>= 1, o >>= 1) {
+    const bool hi = l & o;
+#pragma unroll
+    for (int i = 0; i < n; ++i) {
+      const uint32_t send = hi ? m[i] : m[i + n], keep = hi ? m[i + n] : m[i];
+      m[i] = max(keep, __shfl_xor_sync(FULL_MASK, send, o));
+    }
+  }
+#pragma unroll
+  for (; o > 0; o >>= 1) m[0] = max(m[0], __shfl_xor_sync(FULL_MASK, m[0], o));
+  return m[0];
 }
 
 // 8 values as 8 bytes.
