@@ -379,6 +379,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       const uint32_t total = (uint32_t)nkb * (t0 < tiles ? (tiles - t0 + dt - 1) / dt : 0);
       const uint64_t ad0 = sdesc(smem_u32(smem)), bd0 = sdesc(smem_u32(smem) + C::A_BYTES);
       int s = 0, phase = 0;
+      pdl_wait();  // as in every role: the bounds of its waits do not count the previous kernel's time
       for (uint32_t it = 0; it < total; ++it) {
         if (!warp_wait(go(s), phase, abort_flag, 503)) break;
         fence_after();
@@ -613,6 +614,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   fence_before();
   __syncthreads();
   if constexpr (CTAS == 2) {  // the pair's MMAs, loads, commits and arrivals are done before TMEM is freed
+    if (r == 1 && threadIdx.x == 32) mbar_drain(final_bar, 0);  // the last commit has reached this CTA too
     cluster_arrive();
     cluster_wait();
   }
@@ -705,6 +707,7 @@ __global__ void __launch_bounds__(WeightsCfg<NP, MW>::THREADS, 2)
   } else if (warp == 1) {
     // ------------------------------------------------------------------ MMA issuer
     const uint32_t tbase = __shfl_sync(FULL_MASK, tmem, 0);
+    pdl_wait();  // as in every role: the bounds of its waits do not count the previous kernel's time
     for (int i = 0; i < nkb; ++i) {
       const int s = i % S, b = i % NB;
       if (!warp_wait(go(s), (i / S) & 1, abort_flag, 513)) break;
@@ -905,12 +908,18 @@ cudaError_t weights_opt_in() {
   return smem_opt_in(done, gemm_fp8_weights_kernel<NP, MW>, WeightsCfg<NP, MW>::SMEM);
 }
 
-// Clusters of `cluster` CTAs, one CTA per SM, that the GPU holds at once (a cluster lies within one of
-// its processing clusters).  Cached; entries are atomic, so threads that ask at once store the same value.
+// Clusters of `cluster` CTAs, one CTA per SM, that the current GPU holds at once (a cluster lies within
+// one of its processing clusters).  Cached per device; entries are atomic, so threads that ask at once
+// store the same value.
 int clusters_of_sms(int cluster, int num_sms) {
-  static std::atomic<int> cache[9];
+  static std::atomic<int> cache[64][9];
+  int dev = 0;
   if (cluster == 1) return num_sms;
-  if (int c = cache[cluster].load(std::memory_order_relaxed)) return c;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) {
+    cudaGetLastError();
+    return num_sms / cluster;
+  }
+  if (int c = cache[dev][cluster].load(std::memory_order_relaxed)) return c;
   cudaLaunchAttribute attr[2];
   cudaLaunchConfig_t cfg = cluster_config(64 * cluster, THREADS, TokensCfg<1, 256>::SMEM, cluster, attr);
   cfg.numAttrs = 1;
@@ -920,7 +929,7 @@ int clusters_of_sms(int cluster, int num_sms) {
     cudaGetLastError();
     return num_sms / cluster;
   }
-  cache[cluster].store(n, std::memory_order_relaxed);
+  cache[dev][cluster].store(n, std::memory_order_relaxed);
   return n;
 }
 

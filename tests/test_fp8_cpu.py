@@ -122,6 +122,38 @@ def test_tensor_parallel_shards_hold_the_same_blocks():
             assert torch.equal(bits(L.down[i]), bits(whole.down[i])[:, 2 * unit * r:2 * unit * (r + 1)])
 
 
+def _tp_worker(rank, world, port, path):
+    import json
+    import os
+    import torch.distributed as dist
+    os.environ.update(MASTER_ADDR="127.0.0.1", MASTER_PORT=str(port), RANK=str(rank), WORLD_SIZE=str(world),
+                      LOCAL_RANK=str(rank))
+    out = LLM("tiny-gpu", tensor_parallel_size=world, **_tp_kw()).generate(
+        _prompts(), SamplingParams(temperature=0, max_tokens=8, ignore_eos=True))
+    with open(f"{path}.{rank}", "w") as f:
+        json.dump(out, f)
+    dist.barrier()
+    os._exit(0)  # no teardown of the gloo group: its destructor can race with its own threads at exit
+
+
+def _tp_kw():
+    return dict(device="cpu", dtype="fp32", block_size=16, max_model_len=256, num_blocks=64, comm_backend="nccl",
+                weight_quant_mode="fp8")
+
+
+def test_tensor_parallel_engine_equals_one_rank(tmp_path):
+    import json
+    import socket
+    with socket.socket() as s:
+        s.bind(("127.0.0.1", 0))
+        port = s.getsockname()[1]
+    path = str(tmp_path / "tp")
+    torch.multiprocessing.spawn(_tp_worker, args=(2, port, path), nprocs=2, join=True)
+    outs = [json.load(open(f"{path}.{r}")) for r in range(2)]
+    want = LLM("tiny-gpu", **_tp_kw()).generate(_prompts(), SamplingParams(temperature=0, max_tokens=8, ignore_eos=True))
+    assert outs[0] == outs[1] == want
+
+
 # --------------------------------------------------------------------------- refusals
 def test_config_refusals():
     with pytest.raises(ValueError, match="weight_quant_mode"):

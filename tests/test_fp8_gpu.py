@@ -339,6 +339,97 @@ def test_weights_written_just_before_the_call(ops):
         assert torch.equal(ops.linear_fp8(x, (q, s)), want[i])
 
 
+def test_first_call_of_a_process_inside_a_capture():
+    """Nothing that a first call sets up (attributes, cached sizes) is refused while a stream is captured."""
+    import subprocess
+    import sys
+    code = """
+import torch
+from nanovllm_self_b200.ops import get_ops, torch_ref as R
+ops = get_ops("cuda")
+x = torch.randn(200, 512, device="cuda").bfloat16()
+r0 = torch.randn(200, 512, device="cuda").bfloat16()
+w = R.quant_fp8_weight(torch.randn(512, 512, device="cuda"))
+one = torch.ones(512, device="cuda").bfloat16()
+r = r0.clone()
+torch.cuda.synchronize()
+def step():
+    h, _ = ops.add_rmsnorm_fp8(x, r, one, 1e-6)
+    a = ops.linear_silu_fp8(h, w, 256)
+    few = ops.quant_fp8(x[:5])
+    return a[0].float(), ops.linear_fp8(h, w), ops.linear_fp8(few, w), ops.linear_silu_fp8(few, w, 256)[0].float()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    y = step()
+g.replay()
+torch.cuda.synchronize()
+r.copy_(r0)
+assert all(torch.equal(a, b) for a, b in zip(y, step()))
+"""
+    done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=120)
+    assert done.returncode == 0, done.stderr[-2000:]
+
+
+def test_norm_of_the_residual_itself(ops):
+    """x and the residual may be the same tensor: every value is read before it is written."""
+    x, w = _acts(37, 1040), torch.ones(1040, device=DEV, dtype=torch.bfloat16)
+    want = ops.add_rmsnorm_fp8(x, x.clone(), w, 1e-6)
+    got = ops.add_rmsnorm_fp8(x, x, w, 1e-6)
+    assert torch.equal(got[1], want[1])
+    _same_pair(got[0], want[0])
+
+
+# --------------------------------------------------------------------------- far offsets
+def _wide_fp8(n, k):
+    """[n, k] of e4m3 values, the bytes a cheap pattern without NaN."""
+    q = torch.empty(n, k, dtype=torch.uint8, device=DEV)
+    q.copy_((torch.arange(n, device=DEV) % 89)[:, None].to(torch.uint8))
+    q += (torch.arange(k, device=DEV) % 23).to(torch.uint8)
+    return q.view(torch.float8_e4m3fn)
+
+
+@pytest.mark.parametrize("t,k", [(262153, 16), (600001, 32), (524321, 4112)])
+def test_quant_and_norm_of_many_rows(ops, t, k):
+    """More rows than one dimension of a grid holds CTAs, and (the last) offsets past 2^31 values."""
+    x = torch.empty(t, k, dtype=torch.bfloat16, device=DEV)
+    x.copy_(((torch.arange(t, device=DEV) % 509) + 1)[:, None])
+    x *= ((torch.arange(k, device=DEV) % 7) - 3).to(torch.bfloat16)
+    w = torch.ones(k, device=DEV, dtype=torch.bfloat16)
+    for f in (ops.quant_fp8, lambda v: ops.add_rmsnorm_fp8(v, None, w, 1e-6)[0]):
+        got = f(x)
+        for rows in (slice(0, 40), slice(262140, 262153), slice(t - 33, t)):
+            _same_pair((got[0][rows], got[1][rows]), f(x[rows]))
+
+
+@pytest.mark.parametrize("t", [3, 200])
+def test_products_of_weights_past_2_gib(ops, t):
+    n, k = 524288 + 140, 4112
+    q = _wide_fp8(n, k)
+    s = torch.rand(-(-n // 128), -(-k // 128), device=DEV) + 0.5
+    x = ops.quant_fp8(_acts(t, k))
+    y = ops.linear_fp8(x, (q, s))
+    for a, b in ((0, 256), (n // 128 * 128 - 256, n)):    # whole blocks of rows, the last ones among them
+        part = (q[a:b], s[a // 128:-(-b // 128)])
+        want = _exact(x, part)
+        assert ((y[:, a:b].double() - want).abs() <= want.abs() * 2.0 ** -8 + 1.01 * _acc(k) * _bound(x, part)).all()
+
+
+@pytest.mark.parametrize("t,n,act", [(131200, 16640, False), (131200, 33280, True)])
+def test_products_with_outputs_past_2_gib(ops, t, n, act):
+    k = 32
+    x, w = ops.quant_fp8(_acts(t, k)), _weight(n, k)
+    rows = slice(t - 70, t)
+    few = ops.quant_fp8(_acts(t, k)[rows])
+    if act:
+        q, s = ops.linear_silu_fp8(x, w, n // 2)
+        want = ops.linear_silu_fp8(few, w, n // 2)
+        _same_pair((q[rows], s[rows]), want)
+    else:
+        want = _exact(few, w)
+        y = ops.linear_fp8(x, w)[rows]
+        assert ((y.double() - want).abs() <= want.abs() * 2.0 ** -8 + 1.01 * _acc(k) * _bound(few, w)).all()
+
+
 # --------------------------------------------------------------------------- engine
 def _llm(**kw):
     from nanovllm_self_b200 import LLM
