@@ -10,6 +10,9 @@
 //
 // No counterpart in the reference, whose linear layers are 16-bit (nanovllm/models/qwen3.py:96-134).
 //
+// The bf16 output is rounded once, from the fp32 sums: RoPE, attention and the residual addition behind
+// these products take bf16.  The 8-bit output of SiLU-and-mul is rounded once too, from fp32.
+//
 // gemm_fp8_tokens_kernel<CTAS, BN>: tiles of 128 tokens (MMA M, one TMEM lane each) x BN = 256 or 128
 // features (MMA N) per CTA; CTAS = 2: a pair of CTAs (tcgen05.mma.cta_group::2) shares the weight rows of
 // a tile of 256 tokens, each staging half of them.  A thread of the epilogue owns one token and 64
@@ -19,9 +22,12 @@
 // of 128 of the 8-bit output.
 //
 // What bounds it: per k-block and 256 features the tensor core needs 512 clocks, the chain MMA -> commit
-// -> poll -> TMEM load -> additions -> arrival -> poll -> MMA about 850 with both TMEM buffers in flight
-// (polls of 100 to 300 clocks each beside the additions), so large products reach 0.6 of the rate of
-// the MMAs alone, and there the 1000 W limit holds the clock at 1.5 GHz besides.
+// -> poll -> TMEM loads and additions -> arrival -> poll -> MMA 1540 with two TMEM buffers in flight, 770 per
+// k-block (the loads and additions alone, without a tensor core at work, take 320).  Large products run
+// at the 1000 W limit besides, which holds the clock at 1.5 GHz: 8192 x 4096 x 12288 425 us, 1.94 PFLOP/s;
+// gate / up of 16384 x 24576 x 4096 1.70 ms, 1.94 PFLOP/s.  16 epilogue warps of 32 features per block,
+// with half the registers each, were 10% slower (386 against 350 us beside each other); asking for the
+// next product's barrier ahead of the additions changed nothing.
 //
 // gemm_fp8_weights_kernel<NP, MW>: few tokens.  Tiles of 128 weight rows (MMA M) x NP tokens (MMA N), so a
 // step of one token moves 16 activation rows beside the weights instead of 128, and K split over the
@@ -31,8 +37,14 @@
 // the order of the slices (the result does not depend on timing), finishes and stores the token.  For
 // SiLU-and-mul a CTA holds both tiles of a group: its gate rows and the matching up rows.
 //
-// Neither kernel uses a global workspace.  Every wait is bounded; on expiry the kernel records an error code, drains its copies, frees TMEM
-// and returns.
+// What bounds it: the weights.  One token, 6144 x 4096: 6.75 us; 4096 x 12288: 10.9 us (4.6 TB/s); gate / up
+// of 2 x 12288 x 4096: 20.8 us in a graph (4.85 TB/s), of which 14.1 us are spent streaming at 7.1 TB/s, 1.7
+// pass until the first stage has landed, 2.3 until the slowest CTA is done, and 2 in the reduction and the
+// next launch.  Weights are prefetched into L2 for the first ring only, while the previous kernel ends:
+// two rings deep cost 2%, four 8%.
+//
+// Neither kernel uses a global workspace.  Every wait is bounded; on expiry the kernel records an error
+// code, drains its copies, frees TMEM and returns.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
@@ -217,9 +229,10 @@ __device__ __forceinline__ void finish_bf16x4(const Params& p, int t, int n, con
   }
 }
 
-// Tokens [128 slice / S, 128 (slice + 1) / S) of a tile whose sums lie in the S CTAs of the cluster: added in the order of the slices, finished and stored.  A warp takes a
-// token's sums of one slice and 128 features as one 512-byte row (remote stores of each thread's own 16
-// bytes were slower by half) and has 16 of them in flight.
+// Tokens [128 slice / S, 128 (slice + 1) / S) of a tile whose sums lie in the S CTAs of the cluster: added
+// in the order of the slices, finished and stored.  A warp takes a token's sums of one slice and 128
+// features as one 512-byte row (remote stores of each thread's own 16 bytes were slower by half) and has
+// 16 of them in flight.
 template <int BN, int S>
 __device__ __forceinline__ void finish_rows(const Params& p, float* exchange, int slice, int row0, int tn, int w,
                                             int lane) {
