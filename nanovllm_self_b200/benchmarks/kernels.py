@@ -29,7 +29,8 @@ NQ, NKV, D, HID, INTER, VOCAB = 32, 8, 128, 4096, 12288, 151936
 CASES = ("attn_decode", "attn_decode_fp8", "attn_prefill", "attn_prefill_mma", "attn_prefill_fp8",
          "attn_prefill_flash_attn", "gemm_prefill", "gemm_decode", "gemm_decode256", "gemm_gate_up_silu256", "qkv_post",
          "qkv_post_fp8", "add_rmsnorm", "silu_mul", "sample", "qkv_post256", "lm_head_sample256", "lm_head_logits_sample256",
-         "lm_head_sample256_t", "lm_head_logits_sample256_t", "lm_head_logits256")
+         "lm_head_sample256_t", "lm_head_logits_sample256_t", "lm_head_logits256", "fp8_quant", "fp8_norm",
+         "fp8_linear1", "fp8_linear256", "fp8_linear4096", "fp8_linear_silu1", "fp8_linear_silu256", "fp8_linear_silu4096")
 # Qwen3-8B decode GEMM shapes (n, k) for gemm_sweep: qkv, o_proj, gate_up, down_proj, lm_head
 DECODE_SHAPES = {"qkv": ((NQ + 2 * NKV) * D, HID), "o_proj": (HID, NQ * D), "gate_up": (2 * INTER, HID),
                  "down_proj": (HID, INTER), "lm_head": (VOCAB, HID)}
@@ -145,6 +146,25 @@ def build_case(name: str, ops: CudaOps, dev="cuda"):
         if name == "lm_head_logits256":
             return (lambda: ops.linear(x, w, out)), wbytes + 2 * m * VOCAB, 2 * m * VOCAB * HID
         return (lambda: ops.sample(ops.linear(x, w, out), t, step=st)), wbytes, 2 * m * VOCAB * HID
+    if name == "fp8_quant":
+        x = torch.randn(16384, HID, device=dev).to(torch.bfloat16)
+        return (lambda: ops.quant_fp8(x)), x.numel() * 3 + x.numel() // 32, None
+    if name == "fp8_norm":
+        x = torch.randn(16384, HID, device=dev).to(torch.bfloat16)
+        r = torch.randn_like(x)
+        w = torch.ones(HID, device=dev, dtype=torch.bfloat16)
+        return (lambda: ops.add_rmsnorm_fp8(x, r, w, 1e-6)), x.numel() * 7 + x.numel() // 32, None
+    if name.startswith("fp8_linear"):
+        # gate_up with SiLU-and-mul, or the down projection, on fp8 weights
+        from ..ops.torch_ref import quant_fp8_weight
+        silu = name.startswith("fp8_linear_silu")
+        m = int(name[len("fp8_linear_silu" if silu else "fp8_linear"):])
+        n, k = DECODE_SHAPES["gate_up" if silu else "down_proj"]
+        x = ops.quant_fp8(torch.randn(m, k, device=dev).to(torch.bfloat16))
+        w = quant_fp8_weight(torch.randn(n, k, device=dev) * 0.02)
+        if silu:
+            return (lambda: ops.linear_silu_fp8(x, w, INTER)), m * k + n * k + m * INTER, 2 * m * n * k
+        return (lambda: ops.linear_fp8(x, w)), m * k + n * k + 2 * m * n, 2 * m * n * k
     raise ValueError(f"unknown case {name!r}; one of {', '.join(CASES)}")
 
 
