@@ -1,6 +1,6 @@
 // Quantisation of groups of 128 channels to fp8 e4m3, shared by the norm, quantisation and GEMM
 // epilogue kernels:
-//   a = max(max |x|, 1e-30),  scale = a / 448,  q = e4m3(x * 448 / a)   (saturating, nearest even)
+//   a = max(max |x|, 1e-30),  scale = a / 448,  q = e4m3(x * (448 / a))   (saturating, nearest even)
 // so that scale * q is the value q stands for and the group's largest magnitude maps to e4m3's
 // largest, 448.  The floor keeps 448 / a finite for a group of zeros.  Maxima are taken over the
 // magnitude's bits as integers, which orders NaN above infinity above every finite value: a group
@@ -17,17 +17,6 @@ constexpr float FP8_AMAX_MIN = 1e-30f;
 struct Fp8Scale {
   float scale, inv;
 };
-
-// 448 / a in two parts.  One value in 200 of bf16 inputs lies exactly between two e4m3 values (x * 448 / a has
-// few enough digits where a's mantissa is a multiple of 7, or x's pattern makes up for it); the rounding of
-// hi alone pushed 15% of them off the tie.  With x * lo added ahead of the one rounding they stay ties.
-struct Fp8Inv {
-  float hi, lo;
-};
-__device__ __forceinline__ Fp8Inv fp8_inv(float a) {
-  const float hi = __fdiv_rn(FP8_E4M3_MAX, a);
-  return {hi, fmaf(-hi, a, FP8_E4M3_MAX) * (hi * (1.f / FP8_E4M3_MAX))};
-}
 
 __device__ __forceinline__ Fp8Scale fp8_scale(uint32_t amax_bits) {
   float a = __uint_as_float(amax_bits);
@@ -65,13 +54,6 @@ __device__ __forceinline__ uint2 f32x8_to_e4m3(const float* v, float inv) {
   float t[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) t[j] = v[j] * inv;
-  return make_uint2(f32x4_to_e4m3(t), f32x4_to_e4m3(t + 4));
-}
-
-__device__ __forceinline__ uint2 f32x8_to_e4m3(const float* v, Fp8Inv inv) {
-  float t[8];
-#pragma unroll
-  for (int j = 0; j < 8; ++j) t[j] = fmaf(v[j], inv.hi, v[j] * inv.lo);
   return make_uint2(f32x4_to_e4m3(t), f32x4_to_e4m3(t + 4));
 }
 

@@ -169,23 +169,21 @@ FP8_AMAX_MIN = 1e-30
 
 def _fp8_scale(a: torch.Tensor):
     """(scale, its inverse) of groups with largest magnitude ``a`` (fp32)."""
+    a = a.clamp(min=FP8_AMAX_MIN)
     m = torch.full_like(a, FP8_MAX)  # a tensor: IEEE divisions, no multiplication by a reciprocal
     return a / m, m / a
 
 
 def quant_fp8(x: torch.Tensor):
     """x [T, K] -> (q [T, K] e4m3, s [T, ceil(K / 128)] fp32), x ~ q * s per group of 128 channels:
-    s = max |x| / 448 (at least 1e-30 / 448), q = e4m3(x * 448 / max |x|), saturating; the quotient is
-    rounded to fp32 once."""
+    s = max |x| / 448 (at least 1e-30 / 448), q = e4m3(x * (448 / max |x|)), saturating."""
     t, k = x.shape
     kb = -(-k // FP8_GROUP)
     p = x.new_zeros(t, kb * FP8_GROUP, dtype=torch.float32)
     p[:, :k] = x
     p = p.view(t, kb, FP8_GROUP)
-    a = p.abs().amax(-1).clamp(min=FP8_AMAX_MIN)
-    v = (p.double() * FP8_MAX / a.double()[..., None]).float()
-    q = torch.clamp(v, -FP8_MAX, FP8_MAX).to(torch.float8_e4m3fn)
-    s = _fp8_scale(a)[0]
+    s, inv = _fp8_scale(p.abs().amax(-1))
+    q = torch.clamp(p * inv[..., None], -FP8_MAX, FP8_MAX).to(torch.float8_e4m3fn)
     return q.view(t, kb * FP8_GROUP)[:, :k].contiguous(), s
 
 
@@ -195,14 +193,14 @@ def dequant_fp8(q: torch.Tensor, s: torch.Tensor, dtype=torch.float32) -> torch.
 
 def quant_fp8_weight(w: torch.Tensor):
     """w [N, K] -> (q [N, K] e4m3, s [ceil(N / 128), ceil(K / 128)] fp32): one scale per block of
-    128 x 128, s = max |w| / 448 (at least 1e-30 / 448), q = e4m3(w * (448 / max |w|)), saturating."""
+    128 x 128, by the rule of :func:`quant_fp8`."""
     n, k = w.shape
     g = FP8_GROUP
     nb, kb = -(-n // g), -(-k // g)
     p = w.new_zeros(nb * g, kb * g, dtype=torch.float32)
     p[:n, :k] = w
     p = p.view(nb, g, kb, g)
-    s, inv = _fp8_scale(p.abs().amax(dim=(1, 3)).clamp(min=FP8_AMAX_MIN))
+    s, inv = _fp8_scale(p.abs().amax(dim=(1, 3)))
     q = torch.clamp(p * inv[:, None, :, None], -FP8_MAX, FP8_MAX).to(torch.float8_e4m3fn)
     return q.view(nb * g, kb * g)[:n, :k].contiguous(), s
 
