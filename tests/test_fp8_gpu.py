@@ -111,6 +111,15 @@ def test_norm(ops, t, k, residual):
     _check_quantised(q, s, y, ((64 + 13 + 2) / 2 + 8) * U)
 
 
+@pytest.mark.parametrize("t,k", [(64, 4096), (33, 1040)])
+def test_norm_values_are_those_of_r_times_w(ops, t, k):
+    """r * w is exact in fp32 and the root's factor cancels against the group's maximum, so the 8-bit
+    values are those of r * w bit for bit."""
+    x, res, w = _acts(t, k), _acts(t, k, 7), (1 + 0.2 * torch.randn(k, device=DEV)).to(torch.bfloat16)
+    (q, _), r = ops.add_rmsnorm_fp8(x, res, w, 1e-6)
+    assert torch.equal(_bits(q), _bits(R.quant_fp8(r.float() * w.float())[0]))
+
+
 def test_norm_zero_row_and_nan_row(ops):
     x = _acts(3, 256)
     x[1] = 0
