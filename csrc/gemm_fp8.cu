@@ -1035,21 +1035,25 @@ Fp8Plan fp8_plan(int T, int N, int K, int act, int num_sms) {
   // remains), and the exchange of the slices' sums, 5.0 and 6.2 us for 2 and 4 slices of 256 features,
   // 2.4 and 3.2 us of 128.  Examples of both sides, T x N x K: 256 x 4096 x 4096, 128 features in 2
   // slices 11.6 us, 256 features in 4 slices 13.5 us, neither split 13.8 and 18.9 us; 512 x 6144 x
-  // 4096, 128 features 24.5 us, 256 features 20.2 us.  Where 256 features in one slice win and there
-  // are two rows of tiles or more, pairs of CTAs run them: 16384 x 24576 x 4096 with SiLU-and-mul
-  // 1572 us, single CTAs 1697 us; equal at 512 tokens; 612 x 7168 x 352 11.1 us against 7.6 us, so K
-  // has to fill 8 blocks.
+  // 4096, 128 features 24.5 us, 256 features 20.2 us.  Where 256 features in one slice win, pairs of
+  // CTAs run them if that takes no more rounds of the GPU, and K fills 8 blocks or there are three rounds
+  // of it: 4699 x 6416 x 9456, pairs 284 us, single CTAs 404 us; 8192 x 8192 x 640 62 and 70 us; equal for
+  // one round of 512 x 6144 x 4096.  The other side: 300 x 12288 x 1024, pairs (two rounds) 14.6 us, single
+  // CTAs (one) 9.1 us; two rounds of 1024 x 8192 x 384 10.3 and 9.7 us.
   int64_t best = -1;
   for (int bn = 256; bn >= (act ? 256 : 128); bn /= 2) {
     const int64_t tiles = (int64_t)((T + BM - 1) / BM) * ((N + bn - 1) / bn);
     for (int s = 1; s <= 4; s *= 2) {
       if (s > 1 && (num_kb / s < 4 || tiles > clusters_of_sms(s, num_sms))) continue;
-      const int64_t kbs = (num_kb + s - 1) / s * (s > 1 ? 1 : (tiles + num_sms - 1) / num_sms);
+      const int64_t rounds = s > 1 ? 1 : (tiles + num_sms - 1) / num_sms, kbs = (num_kb + s - 1) / s * rounds;
       const int64_t exchange = s == 1 ? 0 : bn == 256 ? 3800 + 600 * s : 1600 + 400 * s;
       const int64_t ns = kbs * (bn == 256 ? 460 : 310) + exchange;
       if (best >= 0 && ns >= best) continue;
       best = ns;
-      pl.np = bn == 128 ? -3 : s == 1 && T > BM && num_kb >= 8 ? -2 : -1;
+      const int64_t pair_tiles = (int64_t)((T + 2 * BM - 1) / (2 * BM)) * ((N + bn - 1) / bn);
+      const int pairs = clusters_of_sms(2, num_sms);
+      const bool paired = s == 1 && T > BM && (pair_tiles + pairs - 1) / pairs <= rounds && (num_kb >= 8 || rounds >= 3);
+      pl.np = bn == 128 ? -3 : paired ? -2 : -1;
       pl.splits = s;
     }
   }
