@@ -111,6 +111,18 @@ def test_norm(ops, t, k, residual):
     _check_quantised(q, s, y, ((64 + 13 + 2) / 2 + 8) * U)
 
 
+@pytest.mark.parametrize("eps", [0.0, 1e-6])
+def test_norm_group_of_zero_weights_and_tiny_rows(ops, eps):
+    """A group below the floor beside ordinary ones, its factor past fp32's range without eps."""
+    x = (_acts(5, 512).float() * 1e-9).to(torch.bfloat16)
+    w = torch.ones(512, device=DEV, dtype=torch.bfloat16)
+    w[128:256] = 0
+    (q, s), _ = ops.add_rmsnorm_fp8(x, None, w, eps)
+    d = x.double()
+    _check_quantised(q, s, d / torch.sqrt(d.square().mean(1, keepdim=True) + eps) * w.double(), ((64 + 13 + 2) / 2 + 8) * U)
+    assert (q[:, 128:256].float() == 0).all()
+
+
 @pytest.mark.parametrize("t,k", [(64, 4096), (33, 1040)])
 def test_norm_values_are_those_of_r_times_w(ops, t, k):
     """r * w is exact in fp32 and the root's factor cancels against the group's maximum, so the 8-bit
