@@ -51,12 +51,9 @@ __device__ __forceinline__ void mbar_arrive_expect_tx(uint32_t bar, uint32_t byt
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
 
-// Arrivals that order nothing but what their caller has waited for or fenced (TMEM loads); a releasing
-// arrival also waits for the thread's other memory accesses (1000 clocks where it reaches another CTA).
-__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
-  asm volatile("mbarrier.arrive.relaxed.cta.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
-}
-// ... on a barrier of any CTA of the cluster (address in the cluster's window).
+// Arrival, on a barrier of any CTA of the cluster (address in the cluster's window), that orders nothing but
+// what its caller has waited for or fenced (TMEM loads); a releasing arrival also waits for the thread's
+// other memory accesses (1000 clocks where it reaches another CTA).
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar_cluster) {
   asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar_cluster) : "memory");
 }
