@@ -123,6 +123,73 @@ def test_norm_group_of_zero_weights_and_tiny_rows(ops, eps):
     assert (q[:, 128:256].float() == 0).all()
 
 
+def _norm_rel(k):
+    """Error of the row's factor and what follows it, relative: 8 squares per thread and step of 1024
+    channels are added in a row, then 5 + 4 sums; with a square's own rounding, the mean's division and eps
+    8 c + 12, half of which passes the root.  rsqrt is within 2 ulp (4 halves of one); up to two products by
+    the factor and w, the division by 448 or of it, and the product with its result."""
+    return (4 * -(-k // 1024) + 6 + 4 + 4) * U
+
+
+def _norm_exact(r, w, eps):
+    d = r.double()
+    return d / torch.sqrt(d.square().mean(1, keepdim=True) + eps) * w.double()
+
+
+# every number of vectors per thread that has a kernel of its own, with groups that end inside a step
+NORM_K = [256, 2048, 2064, 4096, 5120, 6144, 8192, 10000, 16384]
+
+
+@pytest.mark.parametrize("residual", [True, False])
+@pytest.mark.parametrize("eps", [0.0, 1e-12, 1e-10])
+@pytest.mark.parametrize("k", NORM_K)
+def test_norm_groups_of_tiny_values(ops, k, eps, residual):
+    """Groups between 1e-38 and 1e-18 in rows that a small eps scales up by as much as 1e18: 448 over a
+    group's largest |r w| alone would leave fp32's range."""
+    g = torch.Generator(device=DEV).manual_seed(k)
+    t, kb = 5, -(-k // 128)
+    mag = 10.0 ** (-38 + 20 * torch.rand(t, kb, device=DEV, generator=g, dtype=torch.float64))
+    mag[:, 0] = 1e-18
+    mag[1] = 1e-37                                  # eps alone makes this row's factor, where there is one
+    mag[1, 0] = 1e-37 if eps else 1e-18
+    v = torch.randn(t, k, device=DEV, generator=g, dtype=torch.float64) * mag.repeat_interleave(128, 1)[:, :k]
+    v[0, 128:132] = torch.tensor([1e-37, 5e-38, 0.0, 2e-38], device=DEV, dtype=torch.float64)
+    v[0, 132:256] = 0
+    x = v.to(torch.bfloat16)
+    w = (1 + 0.1 * torch.randn(k, device=DEV, generator=g)).to(torch.bfloat16)
+    res = torch.zeros_like(x) if residual else None
+    (q, s), _ = ops.add_rmsnorm_fp8(x, res, w, eps)
+    _check_quantised(q, s, _norm_exact(x, w, eps), _norm_rel(k))
+
+
+@pytest.mark.parametrize("k", NORM_K)
+def test_norm_weights_whose_product_with_the_row_overflows(ops, k):
+    """r w leaves fp32's range where the norm itself does not."""
+    x = (_acts(3, k).float() * 1e10).to(torch.bfloat16)
+    w = (1 + 0.1 * torch.randn(k, device=DEV, generator=torch.Generator(device=DEV).manual_seed(2))).to(torch.bfloat16)
+    w[128:256] *= 1e30
+    (q, s), _ = ops.add_rmsnorm_fp8(x, None, w, 1e-6)
+    _check_quantised(q, s, _norm_exact(x, w, 1e-6), _norm_rel(k))
+
+
+def test_norm_infinity_stays_in_its_group(ops):
+    x = _acts(2, 512)
+    x[0, 130] = float("inf")
+    w = torch.ones(512, device=DEV, dtype=torch.bfloat16)
+    d = R.dequant_fp8(*ops.add_rmsnorm_fp8(x, None, w, 1e-6)[0])
+    # finite values over an infinite root are zero; the group of the infinity itself is not a number
+    assert torch.isnan(d[0, 128:256]).all() and (d[0, :128] == 0).all() and (d[0, 256:] == 0).all()
+    assert torch.isfinite(d[1]).all()
+
+
+@pytest.mark.parametrize("k", NORM_K)
+def test_norm_within_its_own_error_bound(ops, k):
+    x, res = _acts(9, k), _acts(9, k, 7)
+    w = (1 + 0.1 * torch.randn(k, device=DEV, generator=torch.Generator(device=DEV).manual_seed(3))).to(torch.bfloat16)
+    (q, s), r = ops.add_rmsnorm_fp8(x, res, w, 1e-6)
+    _check_quantised(q, s, _norm_exact(r, w, 1e-6), _norm_rel(k))
+
+
 @pytest.mark.parametrize("t,k", [(64, 4096), (33, 1040)])
 def test_norm_values_are_those_of_r_times_w(ops, t, k):
     """r * w is exact in fp32 and the root's factor cancels against the group's maximum, so the 8-bit
