@@ -50,7 +50,7 @@ void check_rows(const at::Tensor& x, const char* what) {
   TORCH_CHECK(x.scalar_type() == at::kBFloat16, what, ": x must be bfloat16");
   TORCH_CHECK(x.dim() == 2 && (x.stride(1) == 1 || x.size(1) == 1), what, ": x must be [rows, K] with unit inner stride");
   TORCH_CHECK(x.size(1) > 0 && x.size(1) % 16 == 0, what, ": K must be a positive multiple of 16, got ", num(x.size(1)));
-  TORCH_CHECK(x.size(0) < (1LL << 31) - 65536, what, ": too many rows");
+  TORCH_CHECK(x.size(0) < (1LL << 31) - 65536 && x.size(1) < (1LL << 31) - 65536, what, ": too large");
   TORCH_CHECK(x.size(0) <= 1 || (x.stride(0) % 8 == 0 && x.stride(0) >= x.size(1)), what,
               ": x's row stride must be a multiple of 8 and at least K");
   TORCH_CHECK(aligned(x, 16), what, ": x must be 16-byte aligned");

@@ -204,6 +204,13 @@ def test_quant_and_norm_refusals(C):
     _refused(lambda: C.add_rmsnorm_fp8(_x(1, 16400), None, torch.ones(16400, dtype=torch.bfloat16), 1e-6), "16384")
 
 
+def test_sizes_that_do_not_fit_the_kernels_integers_are_refused(C):
+    """2^32 + 128 channels would be taken for 128 of them."""
+    for x in (torch.empty(0, 2 ** 32 + 128, dtype=torch.bfloat16), torch.empty(0, 2 ** 31, dtype=torch.bfloat16),
+              torch.empty(2 ** 32 + 1, 16, dtype=torch.bfloat16, device="meta")):
+        _refused(lambda: C.quant_fp8(x), "too large")
+
+
 def _operands(t=6, n=256, k=256):
     f8 = torch.float8_e4m3fn
     xs = torch.zeros(-(-k // 128), 8)[:, :t].t()
