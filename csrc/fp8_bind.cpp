@@ -134,7 +134,8 @@ nvb::Fp8Gemm gemm_args(const at::Tensor& xq, const at::Tensor& xs, const at::Ten
 // plan: empty (chosen from the sizes) or (np, splits), see Fp8Plan.
 nvb::Fp8Plan plan_of(const nvb::Fp8Gemm& a, const std::vector<int64_t>& plan, int num_sms) {
   if (plan.empty()) return nvb::fp8_plan(a.T, a.N, a.K, a.act, num_sms);
-  TORCH_CHECK(plan.size() == 2, "plan: (np, splits)");
+  TORCH_CHECK(plan.size() == 2 && plan[0] >= -3 && plan[0] <= 64 && plan[1] >= 1 && plan[1] <= 8,
+              "plan: (np, splits) with np from -3 to 64 and splits from 1 to 8");
   nvb::Fp8Plan p;
   p.np = (int)plan[0];
   p.splits = (int)plan[1];
@@ -142,6 +143,10 @@ nvb::Fp8Plan plan_of(const nvb::Fp8Gemm& a, const std::vector<int64_t>& plan, in
 }
 
 std::vector<int64_t> fp8_plan(int64_t T, int64_t N, int64_t K, int64_t act, int64_t num_sms) {
+  const int64_t most = (1LL << 31) - 65536;
+  TORCH_CHECK(T >= 0 && T < most && N >= 0 && N < most && K > 0 && K < most && (act == 0 || act == 1) && num_sms > 0 &&
+                  num_sms < 65536,
+              "fp8_plan: sizes from 0 (K: 1) to below 2^31 - 65536, act 0 or 1, and a GPU's number of SMs");
   const auto p = nvb::fp8_plan((int)T, (int)N, (int)K, (int)act, (int)num_sms);
   return {p.np, p.splits};
 }

@@ -930,7 +930,7 @@ int clusters_of_sms(int cluster, int num_sms) {
   if (cluster == 1) return num_sms;
   if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) {
     cudaGetLastError();
-    return num_sms / cluster;
+    return std::max(1, num_sms / cluster);
   }
   if (int c = cache[dev][cluster].load(std::memory_order_relaxed)) return c;
   cudaLaunchAttribute attr[2];
@@ -940,7 +940,7 @@ int clusters_of_sms(int cluster, int num_sms) {
   if (tokens_opt_in<1, 256>() != cudaSuccess ||
       cudaOccupancyMaxActiveClusters(&n, gemm_fp8_tokens_kernel<1, 256>, &cfg) != cudaSuccess || n <= 0) {
     cudaGetLastError();
-    return num_sms / cluster;
+    return std::max(1, num_sms / cluster);
   }
   cache[dev][cluster].store(n, std::memory_order_relaxed);
   return n;

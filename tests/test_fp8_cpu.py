@@ -244,3 +244,27 @@ def test_product_refusals(C):
     for features in (0, 120, 129, 64 * 1024):
         _refused(lambda: C.linear_silu_fp8(*a, features), "features")
     _refused(lambda: C.linear_silu_fp8(*a, 144), "features")  # w has one pair of blocks, not two
+
+
+def test_plans_of_any_gpu_size_and_their_refusals(C):
+    """In a process of its own: a plan for a GPU of no SMs, or one, divided by zero and ended the process."""
+    import subprocess
+    import sys
+    code = """
+from nanovllm_self_b200.ops._ext import load
+C = load()
+for sms in (1, 2, 3, 7, 148, 160):
+    for t, n, k, act in ((0, 0, 16, 0), (1, 16, 16, 0), (33, 256, 1040, 1), (200, 4096, 4096, 0), (9000, 24576, 4096, 1)):
+        np_, splits = C.fp8_plan(t, n, k, act, sms)
+        assert np_ in (-1, -2, -3) or t <= np_ <= 64
+        assert 1 <= splits <= 8
+for bad in ((-1, 16, 16, 0, 148), (1, -16, 16, 0, 148), (1, 16, 0, 0, 148), (200, 256, 256, 0, 0), (200, 256, 256, 0, -4),
+            (200, 256, 256, 2, 148), (2 ** 32 + 1, 256, 256, 0, 148), (1, 2 ** 33, 256, 0, 148), (1, 16, 2 ** 32 + 16, 0, 148)):
+    try:
+        C.fp8_plan(*bad)
+    except RuntimeError:
+        continue
+    raise SystemExit(f"not refused: {bad}")
+"""
+    done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=120)
+    assert done.returncode == 0, (done.returncode, done.stderr[-500:])
