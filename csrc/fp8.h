@@ -44,7 +44,8 @@ struct Fp8Gemm {
 struct Fp8Plan {
   int np = -1, splits = 1;
 };
-// The plan of a product, from its sizes alone (the same in every process and every call).
+// The plan of a product, from its sizes and the GPU's number of SMs alone (the same in every process and every
+// call, whatever the GPU): equal operands give equal bits on every GPU of one model.
 Fp8Plan fp8_plan(int T, int N, int K, int act, int num_sms);
 cudaError_t gemm_fp8(const Fp8Gemm& g, const Fp8Plan& plan, int num_sms, cudaStream_t stream);
 

@@ -145,7 +145,7 @@ nvb::Fp8Plan plan_of(const nvb::Fp8Gemm& a, const std::vector<int64_t>& plan, in
 std::vector<int64_t> fp8_plan(int64_t T, int64_t N, int64_t K, int64_t act, int64_t num_sms) {
   const int64_t most = (1LL << 31) - 65536;
   TORCH_CHECK(T >= 0 && T < most && N >= 0 && N < most && K > 0 && K < most && (act == 0 || act == 1) && num_sms > 0 &&
-                  num_sms < 65536,
+                  num_sms < 4096,
               "fp8_plan: sizes from 0 (K: 1) to below 2^31 - 65536, act 0 or 1, and a GPU's number of SMs");
   const auto p = nvb::fp8_plan((int)T, (int)N, (int)K, (int)act, (int)num_sms);
   return {p.np, p.splits};

@@ -921,40 +921,16 @@ cudaError_t weights_opt_in() {
   return smem_opt_in(done, gemm_fp8_weights_kernel<NP, MW>, WeightsCfg<NP, MW>::SMEM);
 }
 
-// Clusters of `cluster` CTAs, one CTA per SM, that the current GPU holds at once (a cluster lies within
-// one of its processing clusters).  Cached per device; entries are atomic, so threads that ask at once
-// store the same value.
-int clusters_of_sms(int cluster, int num_sms) {
-  static std::atomic<int> cache[64][9];
-  int dev = 0;
-  if (cluster == 1) return num_sms;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) {
-    cudaGetLastError();
-    return std::max(1, num_sms / cluster);
-  }
-  if (int c = cache[dev][cluster].load(std::memory_order_relaxed)) return c;
-  cudaLaunchAttribute attr[2];
-  cudaLaunchConfig_t cfg = cluster_config(64 * cluster, THREADS, TokensCfg<1, 256>::SMEM, cluster, attr);
-  cfg.numAttrs = 1;
-  int n = 0;
-  if (tokens_opt_in<1, 256>() != cudaSuccess ||
-      cudaOccupancyMaxActiveClusters(&n, gemm_fp8_tokens_kernel<1, 256>, &cfg) != cudaSuccess || n <= 0) {
-    cudaGetLastError();
-    return std::max(1, num_sms / cluster);
-  }
-  cache[dev][cluster].store(n, std::memory_order_relaxed);
-  return n;
-}
-
-// The same with two CTAs per SM: an even cluster takes half as many SMs, and a smaller cluster fits
-// wherever a larger one does.
-int clusters_of_half_sms(int cluster, int num_sms) {
-  if (cluster == 1) return 2 * num_sms;
-  const int twice = 2 * clusters_of_sms(cluster, num_sms);
-  return std::max(twice, cluster & 1 ? (cluster < 7 ? clusters_of_half_sms(cluster + 1, num_sms)
-                                                    : clusters_of_sms(4, num_sms))
-                                     : clusters_of_sms(cluster / 2, num_sms));
-}
+// Clusters of 1 .. 8 CTAs that a GPU of num_sms SMs holds at once, with one CTA per SM and with two: a cluster
+// lies within one of the GPU's processing clusters, so fewer fit than num_sms / cluster.  These are what
+// cudaOccupancyMaxActiveClusters answers on a B200 of 148 SMs, scaled to other sizes.  They are not asked of
+// the GPU at hand, on which parts of one model can differ: a plan fixes the order of the fp32 sums, and that
+// is the same wherever a size runs.  A GPU that holds fewer runs the rest in a second round: slower, with the
+// same result.
+constexpr int CLUSTERS_OF_SMS[9] = {0, 148, 74, 45, 33, 26, 22, 15, 15};
+constexpr int CLUSTERS_OF_HALF_SMS[9] = {0, 296, 148, 93, 71, 56, 45, 37, 33};
+int clusters_of_sms(int cluster, int num_sms) { return std::max(1, CLUSTERS_OF_SMS[cluster] * num_sms / 148); }
+int clusters_of_half_sms(int cluster, int num_sms) { return std::max(1, CLUSTERS_OF_HALF_SMS[cluster] * num_sms / 148); }
 
 // The output of the token-major kernel: bf16 [T, N] or e4m3 [T, features], pieces of 64 bytes x 32 rows.
 bool make_out_map(CUtensorMap* m, const Fp8Gemm& g) {

@@ -317,6 +317,26 @@ def test_plans_refused(ops):
         ops.C.linear_silu_fp8(*x, *w, 128, [-3, 1])
 
 
+def test_plans_are_those_of_a_process_without_a_gpu(ops):
+    """Equal sizes take equal plans, and so give equal bits, in every process."""
+    import json
+    import os
+    import random
+    import subprocess
+    import sys
+    rng = random.Random(0)
+    sizes = [(int(2 ** rng.uniform(0, 14)), 16 * int(2 ** rng.uniform(0, 11)), 16 * int(2 ** rng.uniform(0, 10)), rng.random() < 0.3)
+             for _ in range(400)] + [(1, 128 * n, 4096, 0) for n in range(1, 300)] + [(256, 128 * n, 8192, 0) for n in range(1, 100)]
+    sizes = [[t, -(-n // 256) * 256 if act else n, k, int(act)] for t, n, k, act in sizes]
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    code = ("import json, sys; from nanovllm_self_b200.ops._ext import load; C = load(); "
+            f"print(json.dumps([C.fp8_plan(*s, {sms}) for s in json.load(sys.stdin)]))")
+    done = subprocess.run([sys.executable, "-c", code], input=json.dumps(sizes), capture_output=True, text=True, timeout=120,
+                          env={**os.environ, "CUDA_VISIBLE_DEVICES": ""})
+    assert done.returncode == 0, done.stderr[-2000:]
+    assert json.loads(done.stdout) == [ops.C.fp8_plan(*s, sms) for s in sizes]
+
+
 @pytest.mark.parametrize("t", [1, 20, 200])
 def test_linear_nan_and_zero_rows_stay_their_own(ops, t):
     k, n = 512, 384
