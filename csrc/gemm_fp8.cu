@@ -1003,7 +1003,12 @@ Fp8Plan fp8_plan(int T, int N, int K, int act, int num_sms) {
     for (int s = 2; s <= 8; ++s)
       if (num_kb >= s && tiles <= clusters_of_half_sms(s, num_sms)) pl.splits = s;
     // .. unless there is little to stream per tile: 61 x 7216 x 624 takes 8.3 us so, 5.3 us below
-    if (pl.np < 64 || pl.splits >= 4 || num_kb > 8) return pl;
+    if (pl.np < 64 || pl.splits >= 4 || num_kb > 8) {
+      // as many slices as the length of the longest one leaves any work: 9 blocks in 8 slices are 5 of 2
+      const int per = (num_kb + pl.splits - 1) / pl.splits;
+      pl.splits = (num_kb + per - 1) / per;
+      return pl;
+    }
     pl = Fp8Plan{};
   }
   // Fewest nanoseconds by a model of one CTA's time: its k-blocks at 460 ns for a tile of 256 features

@@ -278,3 +278,13 @@ def test_plan_without_a_gpu_is_that_of_a_b200(C, sizes, plan):
     three lie where 35 or 36 tiles are to be split over clusters of 8, of which a B200 holds 33, and 72 over
     clusters of 4, of which it holds 71."""
     assert C.fp8_plan(*sizes, 148) == plan
+
+
+def test_every_slice_of_a_plan_has_work(C):
+    for t in (1, 16, 17, 33, 64, 65, 130, 256, 500, 2000):
+        for act in (0, 1):
+            for kb in list(range(1, 70)) + [96, 100, 128, 200]:
+                for n in (256, 768, 2048, 4608, 6144, 8960, 9216, 24576):
+                    splits = C.fp8_plan(t, n, kb * 128, act, 148)[1]
+                    per = -(-kb // splits)
+                    assert (splits - 1) * per < kb, (t, n, kb, act, splits)
