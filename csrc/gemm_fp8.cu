@@ -79,9 +79,12 @@ struct TokensCfg {
   static constexpr int A_BYTES = BM * BK, STAGE = A_BYTES + B_ROWS * BK;  // 48 or 32 KB
   static constexpr int STAGES = STAGE == 48 * 1024 ? 4 : 6;
   static constexpr int STAGING = EPI_THREADS / 32 * 2048;
-  static constexpr int SLOTS = STAGES + BUFS + 1;  // activation scales of one k-block each: see the producer
-  static constexpr int BARS = 2 * STAGES + BUFS + SLOTS + 2;
-  static constexpr int PRODS = 2 * BUFS;    // k-blocks whose scale products are kept
+  static constexpr int SLOTS = STAGES + BUFS + 1;  // activation scales of one k-block each
+  // K-blocks whose scale products are kept, in two halves: the epilogue gives them back by halves.  An
+  // arrival for each k-block cost 2-3% (8192 x 4096 x 12288 395 and 387 us beside each other).
+  static constexpr int PRODS = 8;
+  static constexpr int HALF = PRODS / 2;
+  static constexpr int BARS = 2 * STAGES + BUFS + 2 * SLOTS + 2 + 2;
   static constexpr int XLD = BN + 4;        // exchange row: 16-byte stores of 8 rows hit distinct banks
   static constexpr int SMEM = 1024 + STAGES * STAGE + STAGING + SLOTS * BM * 4 + PRODS * BLOCKS * BM * 4 +
                               2 * 2 * BM * 4 + 8 * BARS + 16;
@@ -111,11 +114,10 @@ struct WeightsCfg {
   static constexpr bool OVER_RING = NP * MW >= 32 && !(NP == 32 && MW == 1);
   static constexpr int SLOT = NP * 4 < 128 ? 128 : NP * 4;     // activation scales of one k-block
   static constexpr int BUDGET = 113 * 1024;
-  static constexpr int bars(int s) { return 3 * s + 2 * ACC_BUFS + 2; }
+  static constexpr int bars(int s) { return 4 * s + 3 * ACC_BUFS + 3; }
   static constexpr int ring_bytes(int s) {
     return OVER_RING ? (s * STAGE > EXCHANGE ? s * STAGE : EXCHANGE) : s * STAGE + EXCHANGE;
   }
-  // one slot more than stages and buffers together: see the producer
   static constexpr int smem(int s) { return 1024 + ring_bytes(s) + (s + ACC_BUFS + 1) * SLOT + 8 * bars(s) + 16; }
   static constexpr int stages() {
     int s = 8;
@@ -298,7 +300,10 @@ __global__ void __launch_bounds__(THREADS, 1)
   auto empty = [&](int s) { return bar0 + 8u * (S + s); };
   auto tfull = [&](int b) { return bar0 + 8u * (2 * S + b); };
   auto sfull = [&](int l) { return bar0 + 8u * (2 * S + BUFS + l); };
-  const uint32_t final_bar = bar0 + 8u * (2 * S + BUFS + SL);
+  // a slot's scales, and a half of the products of scales, have been read
+  auto sempty = [&](int l) { return bar0 + 8u * (2 * S + BUFS + SL + l); };
+  auto pempty = [&](int h) { return bar0 + 8u * (2 * S + BUFS + 2 * SL + h); };
+  const uint32_t final_bar = bar0 + 8u * (2 * S + BUFS + 2 * SL + 2);
   const uint32_t amax_bar = final_bar + 8u;
   volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + C::BARS);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + C::BARS) + 1;
@@ -315,7 +320,11 @@ __global__ void __launch_bounds__(THREADS, 1)
     for (int b = 0; b < BUFS; ++b) {
       mbar_init(tfull(b), 1 + C::BLOCKS);  // the product's commit and the scale warps
     }
-    for (int l = 0; l < SL; ++l) mbar_init(sfull(l), 1);
+    for (int l = 0; l < SL; ++l) {
+      mbar_init(sfull(l), 1);
+      mbar_init(sempty(l), C::BLOCKS);
+    }
+    for (int h = 0; h < 2; ++h) mbar_init(pempty(h), EPI_THREADS / 32);
     mbar_init(final_bar, 1);
     mbar_init(amax_bar, EPI_THREADS / 32);
     *abort_flag = 0;
@@ -357,7 +366,8 @@ __global__ void __launch_bounds__(THREADS, 1)
         const int row0 = (tm * CTAS + r) * BM;
         for (int i = 0; i < nkb; ++i, ++it) {
           const int s = it % S, l = it % SL, k = (kb0 + i) * BK;
-          if (!mbar_wait(empty(s), ((it / S) & 1) ^ 1, abort_flag, &g_fp8_error, 501)) {
+          if (!mbar_wait(empty(s), ((it / S) & 1) ^ 1, abort_flag, &g_fp8_error, 501) ||
+              !mbar_wait(sempty(l), ((it / SL) & 1) ^ 1, abort_flag, &g_fp8_error, 502)) {
             ok = false;
             break;
           }
@@ -372,9 +382,6 @@ __global__ void __launch_bounds__(THREADS, 1)
             tma_load_2d_pair(st, &map_x, gb, k, row0);
             tma_load_2d_pair(st + C::A_BYTES, &map_w, gb, k, tn * BN + r * C::B_ROWS);
           }
-          // Slot l was last read, by the scale warps, for k-block it - SL.  Stage s is free, so k-block
-          // it - S has been multiplied: its buffer was freed by the epilogue's reading k-block it - S -
-          // BUFS, for which the scale warps had arrived: no barrier of its own guards the slot.
           mbar_arrive_expect_tx(sfull(l), BM * 4);
           tma_load_2d(smem_u32(slots + l * BM), &map_s, sfull(l), row0, kb0 + i);
         }
@@ -429,15 +436,19 @@ __global__ void __launch_bounds__(THREADS, 1)
         for (int kb = 0; kb < nkb; ++kb, ++it) {
           const float w = ws.at(kb);
           // The product of k-block it - BUFS has landed: the arrival below belongs to the next phase of its
-          // barrier, and the epilogue has read the scales of it - 2 BUFS (it freed that buffer for it - BUFS).
+          // barrier.
           ok = warp_wait(sfull(sl), sp, abort_flag, 506) &&
-               (it < BUFS || warp_wait(tfull(it % BUFS), (it / BUFS - 1) & 1, abort_flag, 507));
+               (it < BUFS || warp_wait(tfull(it % BUFS), (it / BUFS - 1) & 1, abort_flag, 507)) &&
+               (it % C::HALF || warp_wait(pempty(it / C::HALF & 1), ((it / C::PRODS) & 1) ^ 1, abort_flag, 508));
           if (!ok) break;
           float4 x = reinterpret_cast<const float4*>(slots + sl * BM)[lane];
           x.x *= w; x.y *= w; x.z *= w; x.w *= w;
           reinterpret_cast<float4*>(prods + ((it % C::PRODS) * C::BLOCKS + warp - 2) * BM)[lane] = x;
           __syncwarp();
-          if (lane == 0) mbar_arrive_release(tfull(it % BUFS));
+          if (lane == 0) {
+            mbar_arrive_release(tfull(it % BUFS));
+            mbar_arrive_release(sempty(sl));
+          }
           if (++sl == SL) {
             sl = 0;
             sp ^= 1;
@@ -511,8 +522,11 @@ __global__ void __launch_bounds__(THREADS, 1)
           }
           fence_before();
           __syncwarp();
-          // this buffer has been read: the tensor core may overwrite it
-          if (lane == 0) mbar_arrive_cluster(go0 + 8u * gs);
+          // this buffer has been read: the tensor core may overwrite it, and the scale warps its products
+          if (lane == 0) {
+            mbar_arrive_cluster(go0 + 8u * gs);
+            if (it % C::HALF == C::HALF - 1) mbar_arrive_release(pempty(it / C::HALF & 1));
+          }
           if (++gs == S) gs = 0;
           float* a = acc[C::BLOCKS - 1];
           add32(a, v[0], last);
@@ -656,7 +670,8 @@ __global__ void __launch_bounds__(WeightsCfg<NP, MW>::THREADS, 2)
   auto empty = [&](int s) { return bar0 + 8u * (S + s); };
   auto tfull = [&](int b) { return bar0 + 8u * (2 * S + b); };
   auto sfull = [&](int l) { return bar0 + 8u * (2 * S + NB + l); };
-  const uint32_t final_bar = bar0 + 8u * (2 * S + NB + SL);
+  auto sempty = [&](int l) { return bar0 + 8u * (2 * S + NB + SL + l); };  // a slot's scales have been read
+  const uint32_t final_bar = bar0 + 8u * (2 * S + NB + 2 * SL);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + C::BARS);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + C::BARS) + 1;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -671,7 +686,10 @@ __global__ void __launch_bounds__(WeightsCfg<NP, MW>::THREADS, 2)
       mbar_init(empty(s), 1);
     }
     for (int b = 0; b < NB; ++b) mbar_init(tfull(b), 1);
-    for (int l = 0; l < SL; ++l) mbar_init(sfull(l), 1);
+    for (int l = 0; l < SL; ++l) {
+      mbar_init(sfull(l), 1);
+      mbar_init(sempty(l), C::EPI_WARPS);
+    }
     mbar_init(final_bar, 1);
     *abort_flag = 0;
     fence_barrier_init();
@@ -697,7 +715,8 @@ __global__ void __launch_bounds__(WeightsCfg<NP, MW>::THREADS, 2)
     int i = 0;
     for (; i < nkb; ++i) {
       const int s = i % S, l = i % SL;
-      if (!mbar_wait(empty(s), ((i / S) & 1) ^ 1, abort_flag, &g_fp8_error, 511)) {
+      if (!mbar_wait(empty(s), ((i / S) & 1) ^ 1, abort_flag, &g_fp8_error, 511) ||
+          !mbar_wait(sempty(l), ((i / SL) & 1) ^ 1, abort_flag, &g_fp8_error, 512)) {
         ok = false;
         break;
       }
@@ -705,9 +724,6 @@ __global__ void __launch_bounds__(WeightsCfg<NP, MW>::THREADS, 2)
       mbar_arrive_expect_tx(go(s), C::STAGE);
       tma_load_2d(st, &map_w, go(s), (kb0 + i) * BK, tile * C::ROWS);
       tma_load_2d(st + C::W_BYTES, &map_x, go(s), (kb0 + i) * BK, 0);
-      // Slot l was last read for k-block i - SL.  Stage s is free, so k-block i - S has been
-      // multiplied, so the epilogue has emptied the buffer of k-block i - S - NB, and had by then
-      // read the scales of the one before, i - SL: no barrier of its own guards the slot.
       mbar_arrive_expect_tx(sfull(l), NP * 4);
       tma_load_2d(smem_u32(slots + l * C::SLOT), &map_s, sfull(l), 0, kb0 + i);
     }
@@ -783,6 +799,8 @@ __global__ void __launch_bounds__(WeightsCfg<NP, MW>::THREADS, 2)
           a[3] = fmaf(__uint_as_float(v[4 * j + 3]), sx.w * wsc, a[3]);
         }
       }
+      __syncwarp();
+      if (lane == 0) mbar_arrive_release(sempty(l));
     }
     // sums of token c to CTA c mod splits: [slice][c / splits][feature]
     if (p.splits > 1) {

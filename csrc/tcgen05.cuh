@@ -51,14 +51,15 @@ __device__ __forceinline__ void mbar_arrive_expect_tx(uint32_t bar, uint32_t byt
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
 
-// Arrival, on a barrier of any CTA of the cluster (address in the cluster's window), that orders nothing but
-// what its caller has waited for or fenced (TMEM loads); a releasing arrival also waits for the thread's
-// other memory accesses (1000 clocks where it reaches another CTA).
+// Arrival, on a barrier of any CTA of the cluster (address in the cluster's window), that orders the TMEM loads
+// that its caller has waited for and fenced, and no other memory access: what the arriving warp has read from
+// shared memory is given back by an arrival that releases.  (A releasing arrival of the cluster's scope waits
+// for all of the thread's accesses, 1000 clocks where it reaches another CTA.)
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar_cluster) {
   asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar_cluster) : "memory");
 }
 
-// Arrival that publishes this thread's writes to whoever waits for the barrier.
+// Arrival that publishes this thread's writes to whoever waits for the barrier, after this thread's reads.
 __device__ __forceinline__ void mbar_arrive_release(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
