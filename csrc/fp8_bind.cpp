@@ -192,6 +192,11 @@ Pair linear_silu_fp8(const at::Tensor& xq, const at::Tensor& xs, const at::Tenso
 
 int64_t fp8_error(bool reset) { return nvb::gemm_fp8_error_code(reset ? 1 : 0); }
 
+void fp8_wait_check(int64_t budget_ns) {
+  TORCH_CHECK(budget_ns >= 0, "fp8_wait_check: the budget must not be negative");
+  ok(nvb::gemm_fp8_wait_check((uint64_t)budget_ns, stream()), "fp8_wait_check");
+}
+
 }  // namespace
 
 void register_fp8(pybind11::module& m) {
@@ -203,4 +208,5 @@ void register_fp8(pybind11::module& m) {
         pybind11::arg("ws"), pybind11::arg("features"), pybind11::arg("plan") = std::vector<int64_t>{});
   m.def("fp8_plan", &fp8_plan);
   m.def("fp8_error", &fp8_error, pybind11::arg("reset") = false);
+  m.def("fp8_wait_check", &fp8_wait_check, pybind11::arg("budget_ns") = 1000000);
 }

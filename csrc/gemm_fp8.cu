@@ -43,19 +43,20 @@
 // next launch.  Weights are prefetched into L2 for the first ring only, while the previous kernel ends:
 // two rings deep cost 2%, four 8%.
 //
-// Neither kernel uses a global workspace.  Every wait is bounded; on expiry the kernel records an error
-// code, drains its copies, frees TMEM and returns.
+// Neither kernel uses a global workspace.  Every wait on an mbarrier is bounded; on expiry the kernel records
+// an error code in a word of host memory, drains its copies, frees TMEM and returns, with an output that is
+// not valid: whoever reads the output back checks the word (fp8_error).  Cluster barriers, TMEM allocation and the wait
+// for the previous kernel have no bound of their own; every thread reaches them, on the error path too.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
 #include <algorithm>
+#include <mutex>
 
 #include "fp8_quant.cuh"
 #include "tcgen05.cuh"
 
 namespace nvb {
-
-__device__ int g_fp8_error = 0;
 
 namespace {
 
@@ -134,8 +135,8 @@ struct WeightsCfg {
 
 // A wait of a whole warp that stays together afterwards.  All lanes poll: electing one to do it costs
 // more (the divergent branch and the broadcast) than the 31 other polls of the same word.
-__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int code) {
-  return __all_sync(FULL_MASK, mbar_wait(bar, parity, abort_flag, &g_fp8_error, code));
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* word, int code) {
+  return __all_sync(FULL_MASK, mbar_wait(bar, parity, abort_flag, word, code));
 }
 
 struct Params {
@@ -150,6 +151,7 @@ struct Params {
   int64_t ldo;
   float* os;
   int64_t ldos;
+  int* error;                // the process's error word
 };
 
 // Tile order: groups of `group` token tiles walk the features together, so that CTAs which run at
@@ -366,8 +368,8 @@ __global__ void __launch_bounds__(THREADS, 1)
         const int row0 = (tm * CTAS + r) * BM;
         for (int i = 0; i < nkb; ++i, ++it) {
           const int s = it % S, l = it % SL, k = (kb0 + i) * BK;
-          if (!mbar_wait(empty(s), ((it / S) & 1) ^ 1, abort_flag, &g_fp8_error, 501) ||
-              !mbar_wait(sempty(l), ((it / SL) & 1) ^ 1, abort_flag, &g_fp8_error, 502)) {
+          if (!mbar_wait(empty(s), ((it / S) & 1) ^ 1, abort_flag, p.error, 501) ||
+              !mbar_wait(sempty(l), ((it / SL) & 1) ^ 1, abort_flag, p.error, 502)) {
             ok = false;
             break;
           }
@@ -401,7 +403,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       int s = 0, phase = 0;
       pdl_wait();  // as in every role: the bounds of its waits do not count the previous kernel's time
       for (uint32_t it = 0; it < total; ++it) {
-        if (!warp_wait(go(s), phase, abort_flag, 503)) break;
+        if (!warp_wait(go(s), phase, abort_flag, p.error, 503)) break;
         fence_after();
         const uint32_t off = s * (C::STAGE >> 4);  // the descriptors count in 16 bytes
         const uint64_t ad = ad0 + off, bd = bd0 + off;
@@ -437,9 +439,9 @@ __global__ void __launch_bounds__(THREADS, 1)
           const float w = ws.at(kb);
           // The product of k-block it - BUFS has landed: the arrival below belongs to the next phase of its
           // barrier.
-          ok = warp_wait(sfull(sl), sp, abort_flag, 506) &&
-               (it < BUFS || warp_wait(tfull(it % BUFS), (it / BUFS - 1) & 1, abort_flag, 507)) &&
-               (it % C::HALF || warp_wait(pempty(it / C::HALF & 1), ((it / C::PRODS) & 1) ^ 1, abort_flag, 508));
+          ok = warp_wait(sfull(sl), sp, abort_flag, p.error, 506) &&
+               (it < BUFS || warp_wait(tfull(it % BUFS), (it / BUFS - 1) & 1, abort_flag, p.error, 507)) &&
+               (it % C::HALF || warp_wait(pempty(it / C::HALF & 1), ((it / C::PRODS) & 1) ^ 1, abort_flag, p.error, 508));
           if (!ok) break;
           float4 x = reinterpret_cast<const float4*>(slots + sl * BM)[lane];
           x.x *= w; x.y *= w; x.z *= w; x.w *= w;
@@ -493,7 +495,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         uint32_t v[2][32];
         float s[C::BLOCKS];
         auto landed = [&](uint32_t it) {  // the product of k-block `it`; its scales
-          if (!warp_wait(tfull(it % BUFS), (it / BUFS) & 1, abort_flag, 504)) return false;
+          if (!warp_wait(tfull(it % BUFS), (it / BUFS) & 1, abort_flag, p.error, 504)) return false;
           fence_after();
           return true;
         };
@@ -600,7 +602,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         am[wg * BM] = m;
         __syncwarp();
         if (lane == 0) mbar_arrive_release(amax_bar);
-        ok = warp_wait(amax_bar, tile_parity, abort_flag, 505);
+        ok = warp_wait(amax_bar, tile_parity, abort_flag, p.error, 505);
         if (!ok) break;
         const Fp8Scale sc = fp8_scale(max(m, am[(wg ^ 1) * BM]));
         uint4 w4[4];
@@ -715,8 +717,8 @@ __global__ void __launch_bounds__(WeightsCfg<NP, MW>::THREADS, 2)
     int i = 0;
     for (; i < nkb; ++i) {
       const int s = i % S, l = i % SL;
-      if (!mbar_wait(empty(s), ((i / S) & 1) ^ 1, abort_flag, &g_fp8_error, 511) ||
-          !mbar_wait(sempty(l), ((i / SL) & 1) ^ 1, abort_flag, &g_fp8_error, 512)) {
+      if (!mbar_wait(empty(s), ((i / S) & 1) ^ 1, abort_flag, p.error, 511) ||
+          !mbar_wait(sempty(l), ((i / SL) & 1) ^ 1, abort_flag, p.error, 512)) {
         ok = false;
         break;
       }
@@ -739,7 +741,7 @@ __global__ void __launch_bounds__(WeightsCfg<NP, MW>::THREADS, 2)
     pdl_wait();  // as in every role: the bounds of its waits do not count the previous kernel's time
     for (int i = 0; i < nkb; ++i) {
       const int s = i % S, b = i % NB;
-      if (!warp_wait(go(s), (i / S) & 1, abort_flag, 513)) break;
+      if (!warp_wait(go(s), (i / S) & 1, abort_flag, p.error, 513)) break;
       fence_after();
       const uint32_t st = smem_u32(smem + s * C::STAGE);
       const uint64_t wd = sdesc(st), xd = sdesc(st + C::W_BYTES);
@@ -774,7 +776,7 @@ __global__ void __launch_bounds__(WeightsCfg<NP, MW>::THREADS, 2)
     for (int i = 0; i < nkb; ++i) {
       const float wsc = ws.at(i);
       const int b = i % NB, l = i % SL;
-      ok = warp_wait(sfull(l), (i / SL) & 1, abort_flag, 514) && warp_wait(tfull(b), (i / NB) & 1, abort_flag, 515);
+      ok = warp_wait(sfull(l), (i / SL) & 1, abort_flag, p.error, 514) && warp_wait(tfull(b), (i / NB) & 1, abort_flag, p.error, 515);
       if (!ok) break;
       fence_after();
       const uint32_t ta = tmem + ((uint32_t)(q4 * 32) << 16) + (b * MW + m) * NP + cs * C::NC;
@@ -858,6 +860,40 @@ __global__ void __launch_bounds__(WeightsCfg<NP, MW>::THREADS, 2)
     fence_after();
     tmem_dealloc<1>(tmem, C::TMEM_COLS);
   }
+}
+
+// The error word: pinned host memory that every GPU of the process can write, so that reading it after a
+// synchronisation costs no copy and covers all of them.  Null where it cannot be had.
+std::atomic<int*> g_error_word{nullptr};
+int* error_word() {
+  int* w = g_error_word.load(std::memory_order_acquire);
+  if (w) return w;
+  static std::mutex mu;
+  std::lock_guard<std::mutex> lock(mu);
+  if ((w = g_error_word.load(std::memory_order_acquire))) return w;
+  // the first call may lie inside a stream capture, which this allocation does not concern
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  if (cudaThreadExchangeStreamCaptureMode(&mode) != cudaSuccess) return nullptr;
+  void* m = nullptr;
+  const cudaError_t e = cudaHostAlloc(&m, sizeof(int), cudaHostAllocPortable | cudaHostAllocMapped);
+  cudaThreadExchangeStreamCaptureMode(&mode);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return nullptr;
+  }
+  w = static_cast<int*>(m);
+  *w = 0;
+  g_error_word.store(w, std::memory_order_release);
+  return w;
+}
+
+// A wait that nothing ends, given up after budget_ns.
+__global__ void wait_check_kernel(int* word, uint64_t budget_ns) {
+  __shared__ uint64_t bar;
+  __shared__ int abort_flag;
+  mbar_init(smem_u32(&bar), 1);
+  abort_flag = 0;
+  mbar_wait(smem_u32(&bar), 0, &abort_flag, word, 599, budget_ns);
 }
 
 PFN_cuTensorMapEncodeTiled_v12000 get_encode() {
@@ -1062,6 +1098,8 @@ Fp8Plan fp8_plan(int T, int N, int K, int act, int num_sms) {
 cudaError_t gemm_fp8(const Fp8Gemm& g, const Fp8Plan& pl, int num_sms, cudaStream_t stream) {
   if (g.T == 0 || g.N == 0) return cudaSuccess;
   Params p{};
+  p.error = error_word();
+  if (!p.error) return cudaErrorMemoryAllocation;
   p.ws = g.ws;
   p.ldws = g.ldws;
   p.T = g.T;
@@ -1087,13 +1125,16 @@ cudaError_t gemm_fp8(const Fp8Gemm& g, const Fp8Plan& pl, int num_sms, cudaStrea
 }
 
 int gemm_fp8_error_code(int reset) {
-  int v = 0;
-  cudaMemcpyFromSymbol(&v, g_fp8_error, sizeof(int));
-  if (reset) {
-    int z = 0;
-    cudaMemcpyToSymbol(g_fp8_error, &z, sizeof(int));
-  }
-  return v;
+  int* w = g_error_word.load(std::memory_order_acquire);
+  if (!w) return 0;  // no product was ever launched
+  return reset ? __atomic_exchange_n(w, 0, __ATOMIC_ACQ_REL) : __atomic_load_n(w, __ATOMIC_ACQUIRE);
+}
+
+cudaError_t gemm_fp8_wait_check(uint64_t budget_ns, cudaStream_t stream) {
+  int* w = error_word();
+  if (!w) return cudaErrorMemoryAllocation;
+  wait_check_kernel<<<1, 1, 0, stream>>>(w, std::min<uint64_t>(budget_ns, WAIT_BUDGET_NS));
+  return cudaGetLastError();
 }
 
 }  // namespace nvb

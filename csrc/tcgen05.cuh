@@ -23,17 +23,18 @@ __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
   return ok != 0;
 }
 
-// Bounded wait.  Returns false, after recording `code` in *word, once the budget has run out or
+// Bounded wait.  Returns false, after recording `code` in *word (host memory), once the budget has run out or
 // another role of this CTA has given up.
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* word,
-                                          int code) {
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* word, int code,
+                                          uint64_t budget_ns = WAIT_BUDGET_NS) {
   if (mbar_try(bar, parity)) return true;
   SpinBudget sb;
   while (true) {
     if (mbar_try(bar, parity)) return true;
     if (*abort_flag) return false;
-    if (sb.expired(WAIT_BUDGET_NS)) {
-      atomicCAS(word, 0, code);
+    if (sb.expired(budget_ns)) {
+      *reinterpret_cast<volatile int*>(word) = code;
+      __threadfence_system();
       *abort_flag = 1;
       return false;
     }

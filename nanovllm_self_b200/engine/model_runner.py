@@ -416,12 +416,24 @@ class ModelRunner:
         if n == 0:
             return []
         if not self.is_cuda:
-            return [int(x) for x in toks.tolist()]
-        self._out_pinned[:n].copy_(toks[:n], non_blocking=True)
-        self.d2h_bytes += n * 4
-        self._out_event.record()
-        self._out_event.synchronize()
-        return self._out_pinned[:n].tolist()
+            out = [int(x) for x in toks.tolist()]
+        else:
+            self._out_pinned[:n].copy_(toks[:n], non_blocking=True)
+            self.d2h_bytes += n * 4
+            self._out_event.record()
+            self._out_event.synchronize()
+            out = self._out_pinned[:n].tolist()
+        if self.model.fp8:
+            self._check_device_error()
+        return out
+
+    def _check_device_error(self) -> None:
+        """An fp8 product that gave up on a bounded wait leaves an output that is not valid: no token made
+        from it is returned, in this step or a later one (the KV cache may hold what came of it)."""
+        code = self.ops.device_error()
+        if code:
+            raise RuntimeError(f"an fp8 product gave up on a bounded wait (code {code}): this step's tokens and the "
+                               "KV cache are not valid")
 
     # ----------------------------------------------------------- cuda graphs
     @property

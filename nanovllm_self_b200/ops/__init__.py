@@ -77,6 +77,9 @@ class TorchOps:
     def linear_silu_fp8(self, x, w, features=None):
         return R.linear_silu_fp8(x, w, w[0].shape[0] // 2 if features is None else features)
 
+    def device_error(self):
+        return 0
+
     def sample(self, logits, temperatures, top_p=None, seeds=None, step=0, batch_greedy_compat=False,
                generator=None, use_top_p=True, col_offset=0):
         return R.sample(logits, temperatures, top_p, generator, batch_greedy_compat).to(torch.int32)

@@ -139,6 +139,11 @@ class CudaOps:
         return self.C.linear_silu_fp8(x[0], x[1], w[0], w[1],
                                       w[0].shape[0] // 2 if features is None else features)
 
+    def device_error(self) -> int:
+        """Code of an fp8 product that gave up on a bounded wait since the process began (0: none); its output
+        was not valid.  Reads host memory: call it once the product's stream has been synchronised."""
+        return self.C.fp8_error(False)
+
     def _plan(self, m, n, k):
         key = (m, n, k)
         p = self._plans.get(key)

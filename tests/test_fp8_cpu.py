@@ -103,6 +103,19 @@ def test_chunked_prefill_and_bf16_model_run_on_fp8_weights():
     assert [len(o) for o in out] == [len(p) + 4 for p in _prompts()]
 
 
+def test_engine_returns_no_token_of_a_product_that_gave_up(monkeypatch):
+    llm = _llm()
+    sp = SamplingParams(temperature=0, max_tokens=4, ignore_eos=True)
+    llm.generate(_prompts(), sp)
+    monkeypatch.setattr(llm.model_runner.ops, "device_error", lambda: 501)
+    for _ in range(2):   # it stays: the KV cache may hold what came of it
+        with pytest.raises(RuntimeError, match="bounded wait .code 501"):
+            llm.generate(_prompts(), sp)
+    other = _llm(weight_quant_mode="none")   # runs no fp8 product
+    assert other.model_runner.ops.device_error() == 501
+    assert [len(o) for o in other.generate(_prompts(), sp)] == [len(p) + 4 for p in _prompts()]
+
+
 ARCH = Qwen3Arch(vocab_size=256, hidden_size=128, intermediate_size=512, num_hidden_layers=1, num_attention_heads=4,
                  num_key_value_heads=2, head_dim=128, max_position_embeddings=256, tie_word_embeddings=False)
 

@@ -580,3 +580,21 @@ def test_engine_graph_equals_eager():
     sp = SamplingParams(temperature=0, max_tokens=16, ignore_eos=True)
     out = [_llm(enforce_eager=e).generate(_prompts(), sp) for e in (False, True)]
     assert out[0] == out[1]
+
+
+@pytest.mark.parametrize("eager", [True, False])
+def test_engine_reports_an_expired_wait(eager):
+    """A bounded wait that runs out on the GPU reaches the caller of the engine, and only until it is reset."""
+    from nanovllm_self_b200 import SamplingParams
+    from nanovllm_self_b200.ops._ext import load
+    C = load()
+    llm = _llm(enforce_eager=eager)
+    sp = SamplingParams(temperature=0, max_tokens=4, ignore_eos=True)
+    want = llm.generate(_prompts(), sp)
+    C.fp8_wait_check(1000000)     # nothing ends this wait: given up after a millisecond
+    torch.cuda.synchronize()
+    assert C.fp8_error() == 599
+    with pytest.raises(RuntimeError, match="code 599"):
+        llm.generate(_prompts(), sp)
+    assert C.fp8_error(True) == 599 and C.fp8_error() == 0
+    assert _llm(enforce_eager=eager).generate(_prompts(), sp) == want
