@@ -15,15 +15,6 @@ void ok(cudaError_t e, const char* what) { TORCH_CHECK(e == cudaSuccess, what, "
 
 cudaStream_t stream() { return at::cuda::getCurrentCUDAStream().stream(); }
 
-// Numbers and shapes of the messages, as strings: handing a number itself to TORCH_CHECK formats it
-// through a C++ stream, which ended the process (segmentation fault) in this extension.
-std::string num(int64_t v) { return std::to_string(v); }
-std::string shape(const at::Tensor& t) {
-  std::string s = "[";
-  for (int64_t i = 0; i < t.dim(); ++i) s += (i ? ", " : "") + num(t.size(i));
-  return s + "]";
-}
-
 int64_t groups(int64_t k) { return (k + nvb::FP8_GROUP - 1) / nvb::FP8_GROUP; }
 
 bool aligned(const at::Tensor& t, uintptr_t a) { return (reinterpret_cast<uintptr_t>(t.data_ptr()) & (a - 1)) == 0; }
@@ -49,7 +40,7 @@ void check_cuda(const at::Tensor& x, const char* what) {
 void check_rows(const at::Tensor& x, const char* what) {
   TORCH_CHECK(x.scalar_type() == at::kBFloat16, what, ": x must be bfloat16");
   TORCH_CHECK(x.dim() == 2 && (x.stride(1) == 1 || x.size(1) == 1), what, ": x must be [rows, K] with unit inner stride");
-  TORCH_CHECK(x.size(1) > 0 && x.size(1) % 16 == 0, what, ": K must be a positive multiple of 16, got ", num(x.size(1)));
+  TORCH_CHECK(x.size(1) > 0 && x.size(1) % 16 == 0, what, ": K must be a positive multiple of 16, got ", x.size(1));
   TORCH_CHECK(x.size(0) < (1LL << 31) - 65536 && x.size(1) < (1LL << 31) - 65536, what, ": too large");
   TORCH_CHECK(x.size(0) <= 1 || (x.stride(0) % 8 == 0 && x.stride(0) >= x.size(1)), what,
               ": x's row stride must be a multiple of 8 and at least K");
@@ -73,10 +64,10 @@ Pair quant_fp8(const at::Tensor& x) {
 Pair add_rmsnorm_fp8(const at::Tensor& x, const c10::optional<at::Tensor>& residual, const at::Tensor& w, double eps) {
   check_rows(x, "add_rmsnorm_fp8");
   const int64_t T = x.size(0), K = x.size(1);
-  TORCH_CHECK(K <= 16384, "add_rmsnorm_fp8: K must be at most 16384, got ", num(K));
+  TORCH_CHECK(K <= 16384, "add_rmsnorm_fp8: K must be at most 16384, got ", K);
   TORCH_CHECK(w.device() == x.device() && w.scalar_type() == at::kBFloat16 && w.is_contiguous() && w.numel() == K &&
                   aligned(w, 16),
-              "add_rmsnorm_fp8: w must be ", num(K), " contiguous bfloat16 values on x's device");
+              "add_rmsnorm_fp8: w must be ", K, " contiguous bfloat16 values on x's device");
   void* r = nullptr;
   if (residual.has_value()) {
     TORCH_CHECK(residual->device() == x.device() && residual->scalar_type() == at::kBFloat16 &&
@@ -103,19 +94,19 @@ nvb::Fp8Gemm gemm_args(const at::Tensor& xq, const at::Tensor& xs, const at::Ten
   TORCH_CHECK(xq.dim() == 2 && wq.dim() == 2 && xs.dim() == 2 && ws.dim() == 2, what, ": 2-D tensors required");
   const int64_t T = xq.size(0), K = xq.size(1), N = wq.size(0);
   TORCH_CHECK(K > 0 && K % 16 == 0 && wq.size(1) == K, what, ": x [T, K] and w [N, K] with K a multiple of 16, got ",
-              shape(xq), " and ", shape(wq));
+              xq.sizes(), " and ", wq.sizes());
   TORCH_CHECK(T < (1LL << 31) - 65536 && N < (1LL << 31) - 65536 && K < (1LL << 31) - 65536, what, ": too large");
   TORCH_CHECK(xq.stride(1) == 1 && wq.stride(1) == 1 && (T <= 1 || (xq.stride(0) % 16 == 0 && xq.stride(0) >= K)) &&
                   (N <= 1 || (wq.stride(0) % 16 == 0 && wq.stride(0) >= K)) && aligned(xq, 16) && aligned(wq, 16),
               what, ": x and w need unit inner strides, row strides that are multiples of 16 and 16-byte alignment");
   TORCH_CHECK(xs.size(0) == T && xs.size(1) == groups(K), what, ": x's scales must be [T, ceil(K / 128)], got ",
-              shape(xs));
+              xs.sizes());
   TORCH_CHECK((T <= 1 || xs.stride(0) == 1) &&
                   (xs.size(1) <= 1 || (xs.stride(1) % 4 == 0 && xs.stride(1) >= T)) && aligned(xs, 16),
               what, ": x's scales must be token-contiguous (strides (1, a multiple of 4)) and 16-byte aligned, as "
               "quant_fp8 returns them");
   TORCH_CHECK(ws.size(0) == groups(N) && ws.size(1) == groups(K) && (ws.size(1) <= 1 || ws.stride(1) == 1), what,
-              ": w's scales must be [ceil(N / 128), ceil(K / 128)] with unit inner stride, got ", shape(ws));
+              ": w's scales must be [ceil(N / 128), ceil(K / 128)] with unit inner stride, got ", ws.sizes());
   nvb::Fp8Gemm a{};
   a.xq = xq.data_ptr();
   a.xs = xs.data_ptr<float>();
@@ -160,7 +151,7 @@ at::Tensor linear_fp8(const at::Tensor& xq, const at::Tensor& xs, const at::Tens
     const at::Tensor& y = *out;
     TORCH_CHECK(y.device() == xq.device() && y.scalar_type() == at::kBFloat16 && y.dim() == 2 && y.size(0) == a.T &&
                     y.size(1) == a.N && (a.N <= 1 || y.stride(1) == 1) && (a.T <= 1 || y.stride(0) >= a.N),
-                "linear_fp8: out must be bfloat16 [", num(a.T), ", ", num(a.N), "] with unit inner stride on x's device");
+                "linear_fp8: out must be bfloat16 [", a.T, ", ", a.N, "] with unit inner stride on x's device");
   }
   check_cuda(xq, "linear_fp8");
   at::cuda::CUDAGuard g(xq.device());
@@ -176,7 +167,7 @@ Pair linear_silu_fp8(const at::Tensor& xq, const at::Tensor& xs, const at::Tenso
   nvb::Fp8Gemm a = gemm_args(xq, xs, wq, ws, "linear_silu_fp8");
   TORCH_CHECK(features > 0 && features % 16 == 0 && wq.size(0) == 2 * nvb::FP8_GROUP * groups(features),
               "linear_silu_fp8: features must be a positive multiple of 16 and w must hold 2 x ceil(features / 128) "
-              "blocks of 128 rows, got ", num(features), " features and ", num(wq.size(0)), " rows");
+              "blocks of 128 rows, got ", features, " features and ", wq.size(0), " rows");
   check_cuda(xq, "linear_silu_fp8");
   at::cuda::CUDAGuard g(xq.device());
   auto [q, s] = new_pair(xq, a.T, features);

@@ -23,6 +23,9 @@ NVCC_FLAGS = [
     "-U__CUDA_NO_HALF_OPERATORS__", "-U__CUDA_NO_HALF_CONVERSIONS__",
     "-U__CUDA_NO_BFLOAT16_CONVERSIONS__", "-U__CUDA_NO_HALF2_OPERATORS__",
 ]
+# The C++ library that torch uses, by its file: a compiler that finds only an archive of it would link a second
+# copy into the extension, whose streams look their facets up in torch's and crash at the first number.
+LINK_FLAGS = ["-l:libstdc++.so.6"]
 
 setup(
     name="nanovllm_self_b200_kernels",
@@ -31,6 +34,7 @@ setup(
             name="nanovllm_self_b200._C",
             sources=[os.path.join("csrc", s) for s in SOURCES if os.path.exists(os.path.join(CSRC, s))],
             extra_compile_args={"cxx": ["-O3", "-std=c++17"], "nvcc": NVCC_FLAGS},
+            extra_link_args=LINK_FLAGS,
         )
     ],
     cmdclass={"build_ext": BuildExtension.with_options(use_ninja=True)},

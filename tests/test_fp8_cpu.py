@@ -217,6 +217,32 @@ def test_quant_and_norm_refusals(C):
     _refused(lambda: C.add_rmsnorm_fp8(_x(1, 16400), None, torch.ones(16400, dtype=torch.bfloat16), 1e-6), "16384")
 
 
+def test_messages_hold_numbers_and_shapes(C):
+    """In a process of its own: with a second copy of the C++ library in the extension a number in a message ends
+    the process."""
+    import subprocess
+    import sys
+    code = """
+import torch
+from nanovllm_self_b200.ops._ext import load
+C = load()
+f8 = torch.float8_e4m3fn
+def message(f):
+    try:
+        f()
+    except RuntimeError as e:
+        return str(e)
+print(message(lambda: C.quant_fp8(torch.zeros(4, 40, dtype=torch.bfloat16))))
+xs = torch.zeros(2, 8)[:, :6].t()
+print(message(lambda: C.linear_fp8(torch.zeros(6, 256).to(f8), xs, torch.zeros(256, 240).to(f8), torch.zeros(2, 2))))
+"""
+    done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=120)
+    assert done.returncode == 0, (done.returncode, done.stderr[-500:])
+    assert "multiple of 16, got 40" in done.stdout and "[6, 256] and [256, 240]" in done.stdout
+    with open(C.__file__, "rb") as f:
+        assert b"\0libstdc++.so.6\0" in f.read()   # linked to the library that torch uses
+
+
 def test_sizes_that_do_not_fit_the_kernels_integers_are_refused(C):
     """2^32 + 128 channels would be taken for 128 of them."""
     for x in (torch.empty(0, 2 ** 32 + 128, dtype=torch.bfloat16), torch.empty(0, 2 ** 31, dtype=torch.bfloat16),
