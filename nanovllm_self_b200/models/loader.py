@@ -29,6 +29,7 @@ from ..ops.torch_ref import group_gate_up, interleave_gate_up, quant_fp8_weight
 from .qwen3 import Qwen3ForCausalLM
 
 _HF = "model.layers.{i}."
+_STORED_DTYPES = ("F64", "F32", "F16", "BF16")  # safetensors' names
 
 
 def _seed_for(seed: int, name: str) -> int:
@@ -108,6 +109,11 @@ class _SafetensorsSource:
 
     def get(self, name, dtype, rows=None, cols=None):
         sl = self.index[name].get_slice(name)
+        stored = sl.get_dtype()
+        if stored not in _STORED_DTYPES:
+            # 8-bit values mean nothing without their scales, which other tensors hold
+            raise ValueError(f"{name} is stored as {stored}: quantised checkpoints are not read, only "
+                             f"{', '.join(_STORED_DTYPES)} (weight_quant_mode='fp8' quantises those as they are loaded)")
         shape = sl.get_shape()
         if len(shape) == 1:
             t = sl[:]

@@ -5,6 +5,7 @@ import json
 import os
 import socket
 
+import pytest
 import torch
 import torch.multiprocessing as mp
 
@@ -60,3 +61,20 @@ def test_tp2_ranks_slice_the_checkpoint(tmp_path):
     out = str(tmp_path / "tok")
     mp.spawn(_rank, args=(_free_port(), path, out), nprocs=2, join=True)
     assert json.load(open(f"{out}.0")) == json.load(open(f"{out}.1")) == want
+
+
+@pytest.mark.parametrize("mode", ["none", "fp8"])
+@pytest.mark.parametrize("stored", [torch.float8_e4m3fn, torch.int8])
+def test_quantised_checkpoint_is_refused(tmp_path, mode, stored):
+    """Published 8-bit checkpoints hold their scales beside the values: the values alone are not the weights."""
+    from safetensors.torch import load_file, save_file
+    path = str(tmp_path / "ckpt")
+    save_hf_checkpoint(PRESETS["tiny"], path, seed=0, dtype=torch.float32)
+    f = os.path.join(path, "model-00000.safetensors")
+    t = load_file(f)
+    name = "model.layers.0.self_attn.q_proj.weight"
+    t[name + "_scale_inv"] = torch.ones(-(-t[name].shape[0] // 128), -(-t[name].shape[1] // 128))
+    t[name] = t[name].to(stored)
+    save_file(t, f, metadata={"format": "pt"})
+    with pytest.raises(ValueError, match="q_proj.weight is stored as .*not read"):
+        LLM(path, weight_quant_mode=mode, **KW)
