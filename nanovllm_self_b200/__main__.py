@@ -62,6 +62,8 @@ def main(argv=None) -> list:
         from .llm import HFLLM
         if not os.path.isdir(a.model):
             raise SystemExit("--hf needs a checkpoint directory")
+        if a.weights != "none":
+            raise SystemExit("--weights is the engine's: --hf runs the checkpoint's own weights")
         import glob
         has_tok = bool(glob.glob(os.path.join(a.model, "tokenizer*")))
         if a.prompt and not has_tok:

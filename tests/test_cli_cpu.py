@@ -49,3 +49,10 @@ def test_hf_loop_on_a_checkpoint_without_tokenizer(tmp_path):
     res = main(["--model", path, "--device", "cpu", "--dtype", "fp32", "--max-tokens", "4", "--hf",
                 "--prompt-ids", "5,17,300,9,44"])
     assert len(res) == 1 and len(res[0]["output_ids"]) == 4 and all(0 <= t < 1024 for t in res[0]["output_ids"])
+
+
+def test_hf_loop_refuses_the_engines_fp8_weights(tmp_path):
+    """It would run the checkpoint's own weights under that name."""
+    import pytest
+    with pytest.raises(SystemExit, match="--weights"):
+        main(["--model", str(tmp_path), "--device", "cpu", "--hf", "--weights", "fp8", "--prompt-ids", "1,2"])
