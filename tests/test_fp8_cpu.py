@@ -217,6 +217,17 @@ def test_quant_and_norm_refusals(C):
     _refused(lambda: C.add_rmsnorm_fp8(_x(1, 16400), None, torch.ones(16400, dtype=torch.bfloat16), 1e-6), "16384")
 
 
+def test_residual_over_other_rows_of_x_is_refused(C):
+    """Rows are read and written in any order: a residual over another row's input is not defined."""
+    w = torch.ones(256, dtype=torch.bfloat16)
+    big = _x(10, 256)
+    _refused(lambda: C.add_rmsnorm_fp8(big[:4], big[:4], w, 1e-6), "CUDA")     # the same rows: in place
+    _refused(lambda: C.add_rmsnorm_fp8(big[:4], big[4:8], w, 1e-6), "CUDA")
+    _refused(lambda: C.add_rmsnorm_fp8(big[1:5], big[:4], w, 1e-6), "in common")
+    _refused(lambda: C.add_rmsnorm_fp8(big[:8:2], big[:4], w, 1e-6), "in common")
+    _refused(lambda: C.add_rmsnorm_fp8(_x(), big[:4], big[2], 1e-6), "in common")
+
+
 def test_messages_hold_numbers_and_shapes(C):
     """In a process of its own: with a second copy of the C++ library in the extension a number in a message ends
     the process."""
