@@ -447,6 +447,34 @@ def test_weights_written_just_before_the_call(ops):
         assert torch.equal(ops.linear_fp8(x, (q, s)), want[i])
 
 
+@pytest.mark.parametrize("t", [9, 200, 600])
+def test_weights_of_a_kernel_that_lets_the_next_one_start_early(ops, t):
+    """quant_fp8 signals its dependents before it writes: the product that takes its 8-bit values as weights, and
+    starts beside it, sees all of them (one, several and paired CTAs per tile)."""
+    n, k = 4096, 2048
+    x = ops.quant_fp8(_acts(t, k))
+    srcs = [_acts(n, k, s) for s in (11, 12, 13)]
+    ws = torch.rand(n // 128, k // 128, device=DEV) + 0.5
+    want = []
+    for a in srcs:
+        q = ops.quant_fp8(a)[0].clone()
+        torch.cuda.synchronize()
+        want.append(ops.linear_fp8(x, (q, ws)))
+    torch.cuda.synchronize()
+    g, out = torch.cuda.CUDAGraph(), []
+    with torch.cuda.graph(g):
+        for a in srcs * 4:
+            # the last written values overwrite those of the call before in the same memory
+            q = ops.quant_fp8(a)[0]
+            out.append(ops.linear_fp8(x, (q, ws)))
+            del q
+    for _ in range(5):
+        g.replay()
+    torch.cuda.synchronize()
+    for i, y in enumerate(out):
+        assert torch.equal(y, want[i % 3]), i
+
+
 def test_first_call_of_a_process_inside_a_capture():
     """Nothing that a first call sets up (attributes, cached sizes) is refused while a stream is captured."""
     import subprocess
