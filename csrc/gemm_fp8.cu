@@ -80,18 +80,18 @@ struct TokensCfg {
   static constexpr int A_BYTES = BM * BK, STAGE = A_BYTES + B_ROWS * BK;  // 48 or 32 KB
   static constexpr int STAGES = STAGE == 48 * 1024 ? 4 : 6;
   static constexpr int STAGING = EPI_THREADS / 32 * 2048;
-  static constexpr int SLOTS = STAGES + BUFS + 1;  // activation scales of one k-block each
-  // K-blocks whose scale products are kept, in two halves: the epilogue gives them back by halves.  An
-  // arrival for each k-block cost 2-3% (8192 x 4096 x 12288 395 and 387 us beside each other).
-  static constexpr int PRODS = 8;
-  static constexpr int HALF = PRODS / 2;
-  static constexpr int BARS = 2 * STAGES + BUFS + 2 * SLOTS + 2 + 2;
+  // K-blocks whose scale products are kept, in two halves, which the epilogue gives back whole: an arrival for
+  // each k-block cost 2-3%.  As many barriers announce a product and its scales, so that the scale warps run
+  // ahead without looking at the products.
+  static constexpr int PRODS = 8, HALF = PRODS / 2;
+  static constexpr int BARS = 3 * STAGES + PRODS + 2 + 2;
   static constexpr int XLD = BN + 4;        // exchange row: 16-byte stores of 8 rows hit distinct banks
-  static constexpr int SMEM = 1024 + STAGES * STAGE + STAGING + SLOTS * BM * 4 + PRODS * BLOCKS * BM * 4 +
+  static constexpr int SMEM = 1024 + STAGES * STAGE + STAGING + STAGES * BM * 4 + PRODS * BLOCKS * BM * 4 +
                               2 * 2 * BM * 4 + 8 * BARS + 16;
   static_assert(SMEM <= 227 * 1024, "shared memory of a CTA");
   static_assert(BM * XLD * 4 <= STAGES * STAGE, "the exchange fits over the ring");
   static_assert(BUFS <= STAGES, "a stage's barrier takes the arrivals of one k-block at a time");
+  static_assert(BUFS <= PRODS, "a product's barrier takes the arrivals of one k-block at a time");
 };
 
 // Shape of gemm_fp8_weights_kernel<NP, MW>: NP tokens (rounded up), MW = 1 or (SiLU-and-mul: a block of 128
@@ -284,28 +284,29 @@ __global__ void __launch_bounds__(THREADS, 1)
     gemm_fp8_tokens_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
                            const __grid_constant__ CUtensorMap map_s, const __grid_constant__ CUtensorMap map_o, Params p) {
   using C = TokensCfg<CTAS, BN>;
-  constexpr int S = C::STAGES, SL = C::SLOTS, BUFS = C::BUFS, XLD = C::XLD;
+  constexpr int S = C::STAGES, BUFS = C::BUFS, XLD = C::XLD, PRODS = C::PRODS, HALF = C::HALF;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   // the same offset in every CTA of the cluster
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   float* exchange = reinterpret_cast<float*>(smem);  // over the idle ring (splits > 1)
   uint8_t* staging = smem + S * C::STAGE;  // 2 KB per epilogue warp: 64 bytes of 32 rows on their way out
-  float* slots = reinterpret_cast<float*>(staging + C::STAGING);
-  float* prods = slots + SL * BM;  // [k-block % PRODS][weight block][token]: activation scale x weight scale
-  uint32_t* amax = reinterpret_cast<uint32_t*>(prods + C::PRODS * C::BLOCKS * BM);  // [tile parity][half][token]
+  float* slots = reinterpret_cast<float*>(staging + C::STAGING);  // a stage's activation scales
+  float* prods = slots + S * BM;  // [k-block % PRODS][weight block][token]: activation scale x weight scale
+  uint32_t* amax = reinterpret_cast<uint32_t*>(prods + PRODS * C::BLOCKS * BM);  // [tile parity][half][token]
   uint64_t* bars = reinterpret_cast<uint64_t*>(amax + 2 * 2 * BM);
   const uint32_t bar0 = smem_u32(bars);
   // go (the even CTA's): the operands of the k-block in this stage have landed and the epilogue warps have
   // emptied its accumulator buffer.  One barrier for both: a poll costs the MMA warp 200 clocks or more
   // beside the epilogue's additions, even when its answer is yes.
   auto go = [&](int s) { return bar0 + 8u * s; };
+  // empty: the stage's product has read its operands, the scale warps its scales.  sfull: these have landed.
   auto empty = [&](int s) { return bar0 + 8u * (S + s); };
-  auto tfull = [&](int b) { return bar0 + 8u * (2 * S + b); };
-  auto sfull = [&](int l) { return bar0 + 8u * (2 * S + BUFS + l); };
-  // a slot's scales, and a half of the products of scales, have been read
-  auto sempty = [&](int l) { return bar0 + 8u * (2 * S + BUFS + SL + l); };
-  auto pempty = [&](int h) { return bar0 + 8u * (2 * S + BUFS + 2 * SL + h); };
-  const uint32_t final_bar = bar0 + 8u * (2 * S + BUFS + 2 * SL + 2);
+  auto sfull = [&](int s) { return bar0 + 8u * (2 * S + s); };
+  // tfull: the product of k-block % PRODS has landed, and the products of its scales are laid out.  pempty: the
+  // epilogue warps have read a half of these.
+  auto tfull = [&](int k) { return bar0 + 8u * (3 * S + k); };
+  auto pempty = [&](int h) { return bar0 + 8u * (3 * S + PRODS + h); };
+  const uint32_t final_bar = bar0 + 8u * (3 * S + PRODS + 2);
   const uint32_t amax_bar = final_bar + 8u;
   volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + C::BARS);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + C::BARS) + 1;
@@ -317,15 +318,10 @@ __global__ void __launch_bounds__(THREADS, 1)
   if (threadIdx.x == 0) {
     for (int s = 0; s < S; ++s) {
       mbar_init(go(s), 1 + CTAS * EPI_THREADS / 32);
-      mbar_init(empty(s), 1);
+      mbar_init(empty(s), 1 + C::BLOCKS);
+      mbar_init(sfull(s), 1);
     }
-    for (int b = 0; b < BUFS; ++b) {
-      mbar_init(tfull(b), 1 + C::BLOCKS);  // the product's commit and the scale warps
-    }
-    for (int l = 0; l < SL; ++l) {
-      mbar_init(sfull(l), 1);
-      mbar_init(sempty(l), C::BLOCKS);
-    }
+    for (int k = 0; k < PRODS; ++k) mbar_init(tfull(k), 1 + C::BLOCKS);
     for (int h = 0; h < 2; ++h) mbar_init(pempty(h), EPI_THREADS / 32);
     mbar_init(final_bar, 1);
     mbar_init(amax_bar, EPI_THREADS / 32);
@@ -367,9 +363,8 @@ __global__ void __launch_bounds__(THREADS, 1)
         tile_coords(p, t, tm, tn);
         const int row0 = (tm * CTAS + r) * BM;
         for (int i = 0; i < nkb; ++i, ++it) {
-          const int s = it % S, l = it % SL, k = (kb0 + i) * BK;
-          if (!mbar_wait(empty(s), ((it / S) & 1) ^ 1, abort_flag, p.error, 501) ||
-              !mbar_wait(sempty(l), ((it / SL) & 1) ^ 1, abort_flag, p.error, 502)) {
+          const int s = it % S, k = (kb0 + i) * BK;
+          if (!mbar_wait(empty(s), ((it / S) & 1) ^ 1, abort_flag, p.error, 501)) {
             ok = false;
             break;
           }
@@ -384,15 +379,15 @@ __global__ void __launch_bounds__(THREADS, 1)
             tma_load_2d_pair(st, &map_x, gb, k, row0);
             tma_load_2d_pair(st + C::A_BYTES, &map_w, gb, k, tn * BN + r * C::B_ROWS);
           }
-          mbar_arrive_expect_tx(sfull(l), BM * 4);
-          tma_load_2d(smem_u32(slots + l * BM), &map_s, sfull(l), row0, kb0 + i);
+          mbar_arrive_expect_tx(sfull(s), BM * 4);
+          tma_load_2d(smem_u32(slots + s * BM), &map_s, sfull(s), row0, kb0 + i);
         }
       }
       if (!ok) {
         const uint32_t n = it < (uint32_t)S ? it : (uint32_t)S;
         for (uint32_t j = it - n; j < it; ++j) {
           if (r == 0) mbar_drain(go(j % S), (j / S) & 1);
-          mbar_drain(sfull(j % SL), (j / SL) & 1);
+          mbar_drain(sfull(j % S), (j / S) & 1);
         }
       }
     } else if (warp == 1 && r == 0) {
@@ -413,7 +408,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           for (int k = 0; k < BK / 32; ++k)
             mma_f8<CTAS>(d, ad + 2 * k, bd + 2 * k, idesc_f8(CTAS * BM, BN), k > 0 ? 1u : 0u);
           commit<CTAS>(empty(s));
-          commit<CTAS>(tfull(it % BUFS));
+          commit<CTAS>(tfull(it % PRODS));
         }
         __syncwarp();
         if (++s == S) {
@@ -429,7 +424,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       // wait for and one number per column half to load.
       pdl_wait();
       uint32_t it = 0;
-      int sl = 0, sp = 0;  // scale slot of k-block `it` and its phase
+      int s = 0, phase = 0;
       bool ok = true;
       for (int t = t0; t < tiles && ok; t += dt) {
         int tm, tn;
@@ -437,23 +432,22 @@ __global__ void __launch_bounds__(THREADS, 1)
         WeightScales ws(p.ws + (int64_t)min(C::BLOCKS * tn + warp - 2, p.nb - 1) * p.ldws + kb0, nkb, lane);
         for (int kb = 0; kb < nkb; ++kb, ++it) {
           const float w = ws.at(kb);
-          // The product of k-block it - BUFS has landed: the arrival below belongs to the next phase of its
-          // barrier.
-          ok = warp_wait(sfull(sl), sp, abort_flag, p.error, 506) &&
-               (it < BUFS || warp_wait(tfull(it % BUFS), (it / BUFS - 1) & 1, abort_flag, p.error, 507)) &&
-               (it % C::HALF || warp_wait(pempty(it / C::HALF & 1), ((it / C::PRODS) & 1) ^ 1, abort_flag, p.error, 508));
+          // The half that holds k-block it - PRODS has been read: its products may be overwritten, and the
+          // barrier that announced it takes the arrival below.
+          ok = (it % HALF || warp_wait(pempty(it / HALF & 1), ((it / PRODS) & 1) ^ 1, abort_flag, p.error, 502)) &&
+               warp_wait(sfull(s), phase, abort_flag, p.error, 506);
           if (!ok) break;
-          float4 x = reinterpret_cast<const float4*>(slots + sl * BM)[lane];
+          float4 x = reinterpret_cast<const float4*>(slots + s * BM)[lane];
           x.x *= w; x.y *= w; x.z *= w; x.w *= w;
-          reinterpret_cast<float4*>(prods + ((it % C::PRODS) * C::BLOCKS + warp - 2) * BM)[lane] = x;
+          reinterpret_cast<float4*>(prods + ((it % PRODS) * C::BLOCKS + warp - 2) * BM)[lane] = x;
           __syncwarp();
           if (lane == 0) {
-            mbar_arrive_release(tfull(it % BUFS));
-            mbar_arrive_release(sempty(sl));
+            mbar_arrive_release(tfull(it % PRODS));
+            mbar_arrive_release(empty(s));
           }
-          if (++sl == SL) {
-            sl = 0;
-            sp ^= 1;
+          if (++s == S) {
+            s = 0;
+            phase ^= 1;
           }
         }
       }
@@ -495,13 +489,13 @@ __global__ void __launch_bounds__(THREADS, 1)
         uint32_t v[2][32];
         float s[C::BLOCKS];
         auto landed = [&](uint32_t it) {  // the product of k-block `it`; its scales
-          if (!warp_wait(tfull(it % BUFS), (it / BUFS) & 1, abort_flag, p.error, 504)) return false;
+          if (!warp_wait(tfull(it % PRODS), (it / PRODS) & 1, abort_flag, p.error, 504)) return false;
           fence_after();
           return true;
         };
         auto scales = [&](uint32_t it) {
 #pragma unroll
-          for (int h = 0; h < C::BLOCKS; ++h) s[h] = prods[((it % C::PRODS) * C::BLOCKS + h) * BM + lt];
+          for (int h = 0; h < C::BLOCKS; ++h) s[h] = prods[((it % PRODS) * C::BLOCKS + h) * BM + lt];
         };
         ok = landed(it);
         if (!ok) break;
@@ -527,7 +521,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           // this buffer has been read: the tensor core may overwrite it, and the scale warps its products
           if (lane == 0) {
             mbar_arrive_cluster(go0 + 8u * gs);
-            if (it % C::HALF == C::HALF - 1) mbar_arrive_release(pempty(it / C::HALF & 1));
+            if (it % HALF == HALF - 1) mbar_arrive_release(pempty(it / HALF & 1));
           }
           if (++gs == S) gs = 0;
           float* a = acc[C::BLOCKS - 1];

@@ -67,32 +67,32 @@ def wait(bar, parity):
     yield "went on"
 
 
-def tokens_kernel(rng, n, stages, bufs, blocks, warps, prods, slot_barriers=True, product_barriers=True):
-    """gemm_fp8_tokens_kernel: n k-blocks through `stages` operand stages, `bufs` accumulators, `blocks` scale
-    warps and `warps` epilogue warps; product barriers by halves of `prods` k-blocks."""
-    slots, half = stages + bufs + 1, prods // 2
+def tokens_kernel(rng, n, stages, bufs, blocks, warps, prods, product_barriers=True):
+    """gemm_fp8_tokens_kernel: n k-blocks through `stages` operand stages (with a slot of scales each), `bufs`
+    accumulators, `blocks` scale warps and `warps` epilogue warps; the products of scales are given back by
+    halves of `prods` k-blocks.  Without those barriers the scale warps wait for the product `bufs` k-blocks back
+    to have landed, which says that the epilogue has handed over the accumulator before it."""
+    half = prods // 2
     go = [Bar(1 + warps) for _ in range(stages)]
-    empty = [Bar(1) for _ in range(stages)]
-    tfull = [Bar(1 + blocks) for _ in range(bufs)]
-    sfull = [Bar(1) for _ in range(slots)]
-    sempty = [Bar(blocks) for _ in range(slots)]
+    empty = [Bar(1 + blocks) for _ in range(stages)]
+    sfull = [Bar(1) for _ in range(stages)]
+    tfull = [Bar(1 + blocks) for _ in range(prods if product_barriers else bufs)]
     pempty = [Bar(warps) for _ in range(2)]
-    slot, product = [None] * slots, [[None] * prods for _ in range(blocks)]
+    slot, product = [None] * stages, [[None] * prods for _ in range(blocks)]
     acc, stage = [None] * bufs, [None] * stages
     scale = [Thread(rng) for _ in range(blocks)]
     epi = [Thread(rng) for _ in range(warps)]
+    ring = len(tfull)
 
     def producer():
         for it in range(n):
-            s, l = it % stages, it % slots
+            s = it % stages
             yield from wait(empty[s], ((it // stages) & 1) ^ 1)
-            if slot_barriers:
-                yield from wait(sempty[l], ((it // slots) & 1) ^ 1)
             stage[s] = it
             go[s].arrive()
             yield "went on"
-            slot[l] = it
-            sfull[l].arrive()
+            slot[s] = it
+            sfull[s].arrive()
 
     def mma():
         for it in range(n):
@@ -102,29 +102,30 @@ def tokens_kernel(rng, n, stages, bufs, blocks, warps, prods, slot_barriers=True
             acc[it % bufs] = it
             empty[s].arrive()
             yield "went on"
-            tfull[it % bufs].arrive()
+            tfull[it % ring].arrive()
 
     def scales(b):
         for it in range(n):
-            l = it % slots
-            yield from wait(sfull[l], (it // slots) & 1)
-            if it >= bufs:
-                yield from wait(tfull[it % bufs], (it // bufs - 1) & 1)
-            if product_barriers and it % half == 0:
+            s = it % stages
+            if not product_barriers:
+                if it >= bufs:
+                    yield from wait(tfull[it % bufs], (it // bufs - 1) & 1)
+            elif it % half == 0:
                 yield from wait(pempty[it // half & 1], ((it // prods) & 1) ^ 1)
-            scale[b].read(slot, l, it)
+            yield from wait(sfull[s], (it // stages) & 1)
+            scale[b].read(slot, s, it)
             yield "went on"
             scale[b].perform()          # the product is made from it
             product[b][it % prods] = it
-            tfull[it % bufs].arrive()   # releases
+            tfull[it % ring].arrive()   # releases
             yield "went on"
-            sempty[l].arrive()
+            empty[s].arrive()
 
     def epilogue(w):
         for b in range(bufs):
             go[b].arrive()
         for it in range(n):
-            yield from wait(tfull[it % bufs], (it // bufs) & 1)
+            yield from wait(tfull[it % ring], (it // ring) & 1)
             assert acc[it % bufs] == it
             for b in range(blocks):
                 epi[w].read(product[b], it % prods, it)
@@ -239,6 +240,6 @@ def test_kernel_has_the_barriers_of_the_model():
     s = _source()
     tokens, weights = s[s.index("gemm_fp8_tokens_kernel(const"):s.index("template <int NP, int MW>\n__global__")], \
         s[s.index("gemm_fp8_weights_kernel(const"):]
-    assert "mbar_wait(sempty(l)" in tokens and "mbar_arrive_release(sempty(sl))" in tokens
+    assert "mbar_init(empty(s), 1 + C::BLOCKS)" in tokens and "mbar_arrive_release(empty(s))" in tokens
     assert "warp_wait(pempty(" in tokens and "mbar_arrive_release(pempty(" in tokens
     assert "mbar_wait(sempty(l)" in weights and "mbar_arrive_release(sempty(l))" in weights
