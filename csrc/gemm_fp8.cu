@@ -21,12 +21,13 @@
 // holds matching gate / up pairs, so SiLU-and-mul needs no exchange and a tile of 256 is one whole group
 // of 128 of the 8-bit output.
 //
-// What bounds it: per k-block and 256 features the tensor core needs 512 clocks, the chain MMA -> commit
-// -> poll -> TMEM loads and additions -> arrival -> poll -> MMA 1540 with two TMEM buffers in flight, 770 per
-// k-block (the loads and additions alone, without a tensor core at work, take 320).  Large products run
-// at the 1000 W limit besides, which holds the clock at 1.5 GHz: 8192 x 4096 x 12288 425 us, 1.94 PFLOP/s;
-// gate / up of 16384 x 24576 x 4096 1.70 ms, 1.94 PFLOP/s.  16 epilogue warps of 32 features per block,
-// with half the registers each, were 10% slower (386 against 350 us beside each other); asking for the
+// What bounds it: not one thing alone, as far as is known.  Per k-block and 256 features the tensor core needs 512
+// clocks.  Whole calls take 910 with 96 k-blocks per tile and 1010 with 32, the tile's end included: 8192 x
+// 4096 x 12288 434 us (1.90 PFLOP/s) and gate / up of 16384 x 24576 x 4096 1.77 ms (1.87), in a row at the 1000 W
+// limit, which holds the clock at 1.42 and 1.55 GHz.  In the loop the chain MMA -> commit -> poll -> TMEM loads and
+// additions -> arrival -> poll -> MMA took 1540 clocks, two of them in flight, when it was last timed by itself;
+// the loads and additions alone, without a tensor core at work, take 320.  16 epilogue warps of 32 features per
+// block, with half the registers each, were 10% slower (386 against 350 us beside each other); asking for the
 // next product's barrier ahead of the additions changed nothing.
 //
 // gemm_fp8_weights_kernel<NP, MW>: few tokens.  Tiles of 128 weight rows (MMA M) x NP tokens (MMA N), so a
@@ -37,16 +38,16 @@
 // the order of the slices (the result does not depend on timing), finishes and stores the token.  For
 // SiLU-and-mul a CTA holds both tiles of a group: its gate rows and the matching up rows.
 //
-// What bounds it: the weights.  One token, 6144 x 4096: 6.75 us; 4096 x 12288: 10.9 us (4.6 TB/s); gate / up
-// of 2 x 12288 x 4096: 20.8 us in a graph (4.85 TB/s), of which 14.1 us are spent streaming at 7.1 TB/s, 1.7
+// What bounds it: the weights.  One token, 6144 x 4096: 6.8 us; 4096 x 12288: 10.9 us (4.6 TB/s); gate / up
+// of 2 x 12288 x 4096: 21.2 us in a graph (4.75 TB/s), of which 14.1 us are spent streaming at 7.1 TB/s, 1.7
 // pass until the first stage has landed, 2.3 until the slowest CTA is done, and 2 in the reduction and the
 // next launch.  Weights are prefetched into L2 for the first ring only, while the previous kernel ends:
 // two rings deep cost 2%, four 8%.
 //
 // Neither kernel uses a global workspace.  Every wait on an mbarrier is bounded; on expiry the kernel records
 // an error code in a word of host memory, drains its copies, frees TMEM and returns, with an output that is
-// not valid: whoever reads the output back checks the word (fp8_error).  Cluster barriers, TMEM allocation and the wait
-// for the previous kernel have no bound of their own; every thread reaches them, on the error path too.
+// not valid: whoever reads the output back checks the word (fp8_error).  Cluster barriers, TMEM allocation and
+// the wait for the previous kernel have no bound of their own; every thread reaches them, on the error path too.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
@@ -168,7 +169,7 @@ __device__ __forceinline__ void tile_coords(const Params& p, int t, int& tm, int
 
 // g / (1 + e^-g) with e^-g = 2^(-g log2 e), by the approximate base-2 exponential and reciprocal (relative
 // errors of 2^-22 and 2^-23; the product -g log2 e adds |g| 2^-24): far inside the 8-bit rounding that
-// follows.  Subnormal results count as zero.
+// follows.  A reciprocal below 2^-126 counts as zero: gates below -87.3, where silu is under 1.1e-36 in magnitude.
 __device__ __forceinline__ float silu_f(float g) {
   float e, q;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(g * -1.44269504f));
@@ -1059,16 +1060,18 @@ Fp8Plan fp8_plan(int T, int N, int K, int act, int num_sms) {
     }
     pl = Fp8Plan{};
   }
-  // Fewest nanoseconds by a model of one CTA's time: its k-blocks at 460 ns for a tile of 256 features
-  // and 310 ns for one of 128 (measured; below that the epilogue's latency per k-block is what
-  // remains), and the exchange of the slices' sums, 5.0 and 6.2 us for 2 and 4 slices of 256 features,
-  // 2.4 and 3.2 us of 128.  Examples of both sides, T x N x K: 256 x 4096 x 4096, 128 features in 2
-  // slices 11.6 us, 256 features in 4 slices 13.5 us, neither split 13.8 and 18.9 us; 512 x 6144 x
-  // 4096, 128 features 24.5 us, 256 features 20.2 us.  Where 256 features in one slice win, pairs of
+  // Fewest nanoseconds by a model of one CTA's time: its k-blocks at 460 ns for a tile of 256 features and 310
+  // ns for one of 128, and the exchange of the slices' sums, 5.0 and 6.2 us for 2 and 4 slices of 256
+  // features, 2.4 and 3.2 us of 128.  (The slope over K is 440 and 296 ns with 32 CTAs at work, 430 in pairs, which
+  // load 32 KB per k-block and CTA instead of 48: it is the CTA's own chain, not the delivery of operands.  With all
+  // SMs at work it is 440-620 and 290-380, the more the longer K: power and memory.  What a call takes besides, 3.5 to
+  // 4.6 us, is the same for all.)  Examples of both sides, T x N x K: 256 x 4096 x 4096, 128 features in 2
+  // slices 11.3 us, 256 features in 4 slices 13.2 us, neither split 13.1 and 18.7 us; 512 x 6144 x
+  // 4096, 128 features 24.2 us, 256 features 19.3 us.  Where 256 features in one slice win, pairs of
   // CTAs run them if that takes no more rounds of the GPU, and K fills 8 blocks or there are three rounds
-  // of it: 4699 x 6416 x 9456, pairs 284 us, single CTAs 404 us; 8192 x 8192 x 640 62 and 70 us; equal for
-  // one round of 512 x 6144 x 4096.  The other side: 300 x 12288 x 1024, pairs (two rounds) 14.6 us, single
-  // CTAs (one) 9.1 us; two rounds of 1024 x 8192 x 384 10.3 and 9.7 us.
+  // of it: 4699 x 6416 x 9456, pairs 288 us, single CTAs 338 us; 8192 x 8192 x 640 61.7 and 62.5 us; equal for
+  // one round of 512 x 6144 x 4096.  The other side: 300 x 12288 x 1024, pairs (two rounds) 13.7 us, single
+  // CTAs (one) 8.8 us; two rounds of 1024 x 8192 x 384 9.9 and 9.3 us.
   int64_t best = -1;
   for (int bn = 256; bn >= (act ? 256 : 128); bn /= 2) {
     const int64_t tiles = (int64_t)((T + BM - 1) / BM) * ((N + bn - 1) / bn);

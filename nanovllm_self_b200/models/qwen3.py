@@ -19,8 +19,10 @@ B200-first layout (not the reference's module-per-projection layout):
   full replicas on every rank, ``:255-258,285``);
 * the final norm runs only on the rows that are sampled;
 * with ``weight_quant="fp8"`` the four products of a layer run on e4m3 weights and inputs with
-  block scales: the norms, the attention output and SiLU-and-mul are rounded to 8 bits where they
-  are produced (``add_rmsnorm_fp8``, ``quant_fp8``, ``linear_silu_fp8``), never stored in 16 bits.
+  block scales.  The norms and SiLU-and-mul are rounded once, to 8 bits, in the kernel that makes
+  them (``add_rmsnorm_fp8``, ``linear_silu_fp8``).  The attention output is stored in 16 bits and
+  read back by ``quant_fp8``; under tensor parallelism so is every norm, which is then rounded
+  twice: the all-reduce kernel's output is 16-bit.
 
 Ops are supplied by an ops object (``ops.get_ops(device)``): hand-written CUDA kernels
 on GPU, the plain-PyTorch oracle on CPU.
