@@ -47,21 +47,16 @@ void check_rows(const at::Tensor& x, const char* what) {
   TORCH_CHECK(aligned(x, 16), what, ": x must be 16-byte aligned");
 }
 
-// [first, last) byte of a tensor's elements.
-std::pair<uintptr_t, uintptr_t> span(const at::Tensor& t) {
-  const auto p = reinterpret_cast<uintptr_t>(t.data_ptr());
-  if (t.numel() == 0) return {p, p};
-  int64_t last = 0;
-  for (int64_t i = 0; i < t.dim(); ++i) last += (t.size(i) - 1) * t.stride(i);
-  return {p, p + (uintptr_t)((last + 1) * t.element_size())};
-}
-
-bool overlap(const at::Tensor& a, const at::Tensor& b) {
-  const auto x = span(a), y = span(b);
-  return x.first < y.second && y.first < x.second;
-}
-
 int64_t row_stride(const at::Tensor& x) { return x.size(0) > 1 ? x.stride(0) : x.size(1); }
+
+// Whether a row of x, [T, K] bf16 with any row stride, shares an element with the `n` bf16 values at `other`.
+bool rows_meet(const at::Tensor& x, const at::Tensor& other) {
+  const int64_t T = x.size(0), K = x.size(1), n = other.numel(), ld = row_stride(x);
+  if (T == 0 || n == 0) return false;
+  const int64_t d = (static_cast<const char*>(other.data_ptr()) - static_cast<const char*>(x.data_ptr())) / 2;
+  const int64_t i = d < K ? 0 : (d - K) / ld + 1;  // the first row that ends behind other's beginning
+  return i < T && i * ld < d + n;
+}
 
 Pair quant_fp8(const at::Tensor& x) {
   check_rows(x, "quant_fp8");
@@ -88,7 +83,7 @@ Pair add_rmsnorm_fp8(const at::Tensor& x, const c10::optional<at::Tensor>& resid
                     residual->sizes() == x.sizes() && residual->is_contiguous() && aligned(*residual, 16),
                 "add_rmsnorm_fp8: the residual must be contiguous bfloat16 of x's shape on x's device");
     // rows are read and written by CTAs of their own, in any order
-    TORCH_CHECK(!overlap(*residual, w) && (!overlap(x, *residual) ||
+    TORCH_CHECK(!rows_meet(*residual, w) && (!rows_meet(x, *residual) ||
                                            (x.data_ptr() == residual->data_ptr() && row_stride(x) == K)),
                 "add_rmsnorm_fp8: x and the residual must be the same memory or have none in common, and w none of the "
                 "residual's");

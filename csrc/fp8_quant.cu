@@ -67,7 +67,8 @@ constexpr int TPR = 128;    // threads per row of the norm
 // power of two and the product of two bf16 values are exact in fp32.  The mantissa is the same for the whole
 // row and enters the scales alone.  The power of two keeps the products in range whatever the row's
 // magnitude: between half of the normalised values and these, so that 448 over a group's largest one is
-// finite wherever that lies above the floor.
+// finite wherever that lies above the floor.  The squares are summed in fp32, as in the 16-bit norm: rows of a
+// root mean square below 1e-19 rest on eps, and rows above 1e19 come out as zeros.
 // Measured, inputs out of the cache and launches back to back: 8191 x 5120 48.4 us (6.1 TB/s), 8192 x 8192
 // 77.6 us; without the power of two 48.1 and 77.4 us.  Scales of one group at a time 83.8 us (8192 x 8192); 256
 // threads per row 54 us, two rows per CTA 51 us, fp32 in between 63 us (8191 x 5120).

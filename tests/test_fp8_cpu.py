@@ -226,6 +226,18 @@ def test_residual_over_other_rows_of_x_is_refused(C):
     _refused(lambda: C.add_rmsnorm_fp8(big[1:5], big[:4], w, 1e-6), "in common")
     _refused(lambda: C.add_rmsnorm_fp8(big[:8:2], big[:4], w, 1e-6), "in common")
     _refused(lambda: C.add_rmsnorm_fp8(_x(), big[:4], big[2], 1e-6), "in common")
+    _refused(lambda: C.add_rmsnorm_fp8(big[::8], big[1:3], w, 1e-6), "CUDA")   # between x's rows
+    # against every element's address, over all places of a few shapes
+    store = torch.zeros(64 * 16, dtype=torch.bfloat16)
+    at = store.data_ptr()
+    for t, ld in ((1, 16), (2, 16), (2, 48), (3, 24), (4, 64)):
+        x = store[16 * 20:].as_strided((t, 16), (ld, 1))
+        mine = {x.data_ptr() + 2 * (i * ld + j) for i in range(t) for j in range(16)}
+        for off in range(0, 64 * 16 - 16 * t, 8):
+            r = store[off:off + 16 * t].view(t, 16)
+            meets = any(at + 2 * (off + j) in mine for j in range(16 * t))
+            same = r.data_ptr() == x.data_ptr() and (ld == 16 or t == 1)
+            _refused(lambda: C.add_rmsnorm_fp8(x, r, w[:16], 1e-6), "in common" if meets and not same else "CUDA")
 
 
 def test_messages_hold_numbers_and_shapes(C):
