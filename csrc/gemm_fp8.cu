@@ -972,12 +972,15 @@ cudaError_t weights_opt_in() {
 
 // Clusters of 1 .. 8 CTAs that a GPU of num_sms SMs holds at once, with one CTA per SM and with two: a cluster
 // lies within one of the GPU's processing clusters, so fewer fit than num_sms / cluster.  These are what
-// cudaOccupancyMaxActiveClusters answers on a B200 of 148 SMs, scaled to other sizes.  They are not asked of
+// cudaOccupancyMaxActiveClusters answers on a B200 of 148 SMs, scaled to other sizes, but for 3 and 5 CTAs of two
+// per SM: 93 and 56 are its answers, and of launches behind one another 92 and 53 ran at once (1 x 4096 x 11904,
+// 93 tiles, in 3 slices 14.9 us, in 2 13.0; 7040, 55 tiles, in 5 slices 10.2, in 4 8.6; past the others' figures as
+// well: 9216, 72 tiles, in 4 slices 14.2, in 3 9.7).  They are not asked of
 // the GPU at hand, on which parts of one model can differ: a plan fixes the order of the fp32 sums, and that
 // is the same wherever a size runs.  A GPU that holds fewer runs the rest in a second round: slower, with the
 // same result.
 constexpr int CLUSTERS_OF_SMS[9] = {0, 148, 74, 45, 33, 26, 22, 15, 15};
-constexpr int CLUSTERS_OF_HALF_SMS[9] = {0, 296, 148, 93, 71, 56, 45, 37, 33};
+constexpr int CLUSTERS_OF_HALF_SMS[9] = {0, 296, 148, 92, 71, 53, 45, 37, 33};
 int clusters_of_sms(int cluster, int num_sms) { return std::max(1, CLUSTERS_OF_SMS[cluster] * num_sms / 148); }
 int clusters_of_half_sms(int cluster, int num_sms) { return std::max(1, CLUSTERS_OF_HALF_SMS[cluster] * num_sms / 148); }
 

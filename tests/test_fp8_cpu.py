@@ -333,12 +333,13 @@ for bad in ((-1, 16, 16, 0, 148), (1, -16, 16, 0, 148), (1, 16, 0, 0, 148), (200
 
 
 @pytest.mark.parametrize("sizes,plan", [((1, 4480, 4096, 0), [16, 7]), ((1, 9216, 4096, 0), [16, 3]),
+                                        ((1, 11904, 4096, 0), [16, 2]), ((1, 7040, 4096, 0), [16, 4]),
                                         ((1, 9216, 4096, 1), [16, 7]), ((256, 4096, 4096, 0), [-3, 2]),
                                         ((1024, 12288, 4096, 1), [-2, 1])])
 def test_plan_without_a_gpu_is_that_of_a_b200(C, sizes, plan):
-    """A plan fixes the order of the sums, so it must not depend on what the process can ask a GPU.  The first
-    three lie where 35 or 36 tiles are to be split over clusters of 8, of which a B200 holds 33, and 72 over
-    clusters of 4, of which it holds 71."""
+    """A plan fixes the order of the sums, so it must not depend on what the process can ask a GPU.  All
+    but the last two lie just past what a B200 holds: 35 or 36 tiles in clusters of 8 (33), 72 of 4 (71), 93 of 3
+    (92), 55 of 5 (53)."""
     assert C.fp8_plan(*sizes, 148) == plan
 
 
