@@ -141,7 +141,8 @@ class CudaOps:
 
     def device_error(self) -> int:
         """Code of an fp8 product that gave up on a bounded wait since the process began (0: none); its output
-        was not valid.  Reads host memory: call it once the product's stream has been synchronised."""
+        was not valid.  Reads host memory: call it once the product's stream has been synchronised.
+        ``C.fp8_error(True)`` clears it."""
         return self.C.fp8_error(False)
 
     def _plan(self, m, n, k):
