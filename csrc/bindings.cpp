@@ -227,6 +227,7 @@ int64_t bounds_error(bool reset) {
 void register_gemm(pybind11::module& m);
 void register_comm(pybind11::module& m);
 void register_fp8(pybind11::module& m);
+void register_tree(pybind11::module& m);
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "nanovllm_self_b200 sm_100a kernels";
@@ -257,4 +258,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   register_gemm(m);
   register_comm(m);
   register_fp8(m);
+  register_tree(m);
 }

@@ -18,6 +18,8 @@ B200-first layout (not the reference's module-per-projection layout):
 * the embedding table and lm_head are vocab-parallel under TP (the reference keeps
   full replicas on every rank, ``:255-258,285``);
 * the final norm runs only on the rows that are sampled;
+* with ``ctx.tree_mask`` set, the new tokens of a sequence are a tree of drafted tokens, and each of them
+  attends to its own ancestors only (``attention_tree``);
 * with ``weight_quant="fp8"`` the four products of a layer run on e4m3 weights and inputs with
   block scales.  The norms and SiLU-and-mul are rounded once, to 8 bits, in the kernel that makes
   them (``add_rmsnorm_fp8``, ``linear_silu_fp8``).  The attention output is stored in 16 bits and
@@ -166,7 +168,10 @@ class Qwen3ForCausalLM:
             ks, vs = kv_scales[i] if kv_scales is not None else (None, None)
             q = ops.qkv_post(qkv, L.q_norm, L.k_norm, self.eps, positions, self.cos_sin, kc, vc,
                              ctx.slot_mapping, ks, vs, nq, nkv, d)
-            o = ops.attention(q, kc, vc, ctx, self.scale, ks, vs).view(T, nq * d)
+            if ctx.tree_mask is None:
+                o = ops.attention(q, kc, vc, ctx, self.scale, ks, vs).view(T, nq * d)
+            else:
+                o = ops.attention_tree(q, kc, vc, ctx, ctx.tree_mask, self.scale, ks, vs).view(T, nq * d)
             if rs:
                 x, residual = self.comm.linear_rs_norm(o, L.o, L.ln2, self.eps)
             else:

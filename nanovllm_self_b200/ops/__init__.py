@@ -77,6 +77,25 @@ class TorchOps:
     def linear_silu_fp8(self, x, w, features=None):
         return R.linear_silu_fp8(x, w, w[0].shape[0] // 2 if features is None else features)
 
+    def tree_mask(self, parents, ctx):
+        return R.tree_mask(parents, ctx.cu_seqlens_q.tolist(), ctx.max_seqlen_q)
+
+    def attention_tree(self, q, k_cache, v_cache, ctx, mask, scale, k_scale=None, v_scale=None):
+        n, d = R.tree_words(ctx.max_seqlen_q), k_cache.shape[3]
+        if mask.dtype != torch.int64 or mask.dim() != 2 or mask.shape[0] != q.shape[0] or mask.shape[1] < n:
+            raise ValueError(f"attention_tree: mask must be int64 [{q.shape[0]}, {n} words or more]")
+        out = R.tree_attention(q.reshape(q.shape[0], -1, d), k_cache, v_cache, ctx.host_q_lens, ctx.host_k_lens,
+                               ctx.block_tables.tolist(), mask, scale, k_scale, v_scale)
+        return out.reshape(q.shape[0], -1)
+
+    def verify_tree(self, logits, tokens, parents, ctx, temperatures, uniforms, draw_uniforms, draft_probs=None):
+        return R.tree_verify(logits, tokens, parents, ctx.host_q_lens, ctx.max_seqlen_q, temperatures, uniforms,
+                             draw_uniforms, draft_probs)
+
+    def commit_tree(self, kv_cache, ctx, path, lengths, kv_scale_cache=None):
+        R.tree_commit(kv_cache, ctx.host_q_lens, ctx.host_k_lens, ctx.block_tables.tolist(), path, lengths,
+                      kv_scale_cache)
+
     def device_error(self):
         return 0
 

@@ -183,6 +183,40 @@ class CudaOps:
             self.launches += 1
         return out
 
+    # ------------------------------------------------- trees of drafted tokens
+    # A sequence's new tokens are the nodes of its tree (``torch_ref``'s section on them; up to 256): ``ctx`` is the
+    # step's Context, whose context_lens count them.  Workspaces come from the caching allocator, one per call.
+    def tree_mask(self, parents, ctx):
+        """(mask int64 [T, words], depth int32 [T]) of the trees with these parents (int32 [T]): each node's
+        ancestors and itself as bits, and how many ancestors it has (its position is that of the root plus this)."""
+        self.launches += 1
+        return self.C.tree_mask(parents, ctx.cu_seqlens_q, ctx.num_seqs, ctx.max_seqlen_q)
+
+    def attention_tree(self, q, k_cache, v_cache, ctx, mask, scale, k_scale=None, v_scale=None):
+        """[T, heads * 128] bf16: every node attends to the positions before its tree and to the nodes of its mask row
+        (``tree_mask``'s, or any other).  Rows behind the last sequence are not written."""
+        self.launches += 2
+        return self.C.tree_attention(q, k_cache, v_cache, k_scale, v_scale, mask, ctx.block_tables, ctx.cu_seqlens_q,
+                                     ctx.context_lens, ctx.num_seqs, ctx.max_seqlen_q, float(scale))
+
+    def verify_tree(self, logits, tokens, parents, ctx, temperatures, uniforms, draw_uniforms, draft_probs=None):
+        """(path int32 [B, max_seqlen_q], length int32 [B], next token int32 [B]): the walk through each tree by
+        rejection sampling from these random numbers (``torch_ref.tree_verify`` has the formulas).  logits [T, V]
+        bf16 or fp32, one row per node; tokens, parents int32 [T]; temperatures fp32 [B] (0 and below: greedy);
+        uniforms fp32 [T], draw_uniforms fp32 [B] in [0, 1); draft_probs fp32 [T, V], row i what i's children were
+        drawn from, or None where they were not drawn."""
+        self.launches += 1
+        return self.C.tree_verify(logits, tokens, parents, ctx.cu_seqlens_q, temperatures, uniforms, draw_uniforms,
+                                  draft_probs, ctx.num_seqs, ctx.max_seqlen_q)
+
+    def commit_tree(self, kv_cache, ctx, path, lengths, kv_scale_cache=None):
+        """Moves the K/V of ``verify_tree``'s paths to consecutive positions, in place, in every layer of the pool
+        [2, layers, blocks, KV heads, block size, 128] (bf16, or e4m3 with scales [2, layers, blocks, KV heads]).
+        A sequence's cached tokens then number context_len - nodes + length."""
+        self.launches += 1
+        self.C.tree_commit(kv_cache, path, lengths, ctx.block_tables, ctx.cu_seqlens_q, ctx.context_lens,
+                           kv_scale_cache, ctx.num_seqs, ctx.max_seqlen_q)
+
     # -------------------------------------------------------------- sampling
     sample_keys_cap = _SAMPLE_KEYS
 

@@ -268,6 +268,215 @@ def sample(logits: torch.Tensor, temperatures: torch.Tensor, top_p: torch.Tensor
     return torch.where(t > 0, drawn, greedy)
 
 
+# ------------------------------------------------------------------ trees of drafted tokens
+# A step that checks drafted tokens gives each sequence the nodes of a tree as its new tokens: node 0 is the
+# root (the last token that is known), ``parents`` holds each node's parent by its index within the tree, which
+# lies below the node's own, and node i's K/V lies at position context_len - nodes + i.  A node whose parent is no
+# index below its own has none.
+TREE_MAX_NODES = 256
+
+
+def tree_words(max_nodes: int) -> int:
+    """Words of a mask row for trees of up to ``max_nodes`` nodes (bit j % 64 of word j / 64 is node j)."""
+    if not 1 <= max_nodes <= TREE_MAX_NODES:
+        raise ValueError(f"trees have 1 to {TREE_MAX_NODES} nodes, got max_seqlen_q = {max_nodes}")
+    return -(-max_nodes // 64)
+
+
+def tree_mask(parents: torch.Tensor, cu_q: list, max_nodes: int):
+    """(mask int64 [T, words]: the ancestors of each node and itself; depth int32 [T]: how many ancestors)."""
+    words, t = tree_words(max_nodes), parents.shape[0]
+    mask = torch.zeros(t, words, dtype=torch.int64)
+    depth = torch.zeros(t, dtype=torch.int32)
+    host = parents.tolist()
+    for t0, t1 in zip(cu_q[:-1], cu_q[1:]):
+        see: list[int] = []
+        for i in range(min(t1 - t0, max_nodes)):
+            p = host[t0 + i]
+            see.append((see[p] if 0 <= p < i else 0) | 1 << i)
+            for w in range(words):
+                x = see[i] >> 64 * w & (1 << 64) - 1
+                mask[t0 + i, w] = x - (1 << 64) if x >> 63 else x
+            depth[t0 + i] = bin(see[i]).count("1") - 1
+    return mask.to(parents.device), depth.to(parents.device)
+
+
+def _gather_pages(cache: torch.Tensor, table: list, k_len: int, scale: torch.Tensor | None) -> torch.Tensor:
+    """``gather_kv`` with blocks outside of the pool or of the table read as zeros."""
+    nb = -(-k_len // cache.shape[2])
+    ids = (list(table) + [-1] * nb)[:nb]
+    ok = torch.tensor([0 <= i < cache.shape[0] for i in ids], device=cache.device)
+    x = gather_kv(cache, [i if 0 <= i < cache.shape[0] else 0 for i in ids], k_len, scale)
+    return torch.where(ok.repeat_interleave(cache.shape[2])[:k_len, None, None], x, 0.0)
+
+
+def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, q_lens: list, k_lens: list,
+                   block_tables: list, mask: torch.Tensor, scale: float, k_scale=None, v_scale=None) -> torch.Tensor:
+    """q [T, Hq, D] (each sequence's tree nodes) -> out [T, Hq, D]: node r sees the positions before the tree and
+    the nodes of its mask; a node that sees nothing gives zeros, and what a node does not see has no part in it,
+    an infinity or a NaN included."""
+    out = torch.zeros_like(q)
+    g = q.shape[1] // k_cache.shape[1]
+    t0 = 0
+    for b, (n, kl) in enumerate(zip(q_lens, k_lens)):
+        if n and kl > 0:
+            k = _gather_pages(k_cache, block_tables[b], kl, k_scale).repeat_interleave(g, dim=1)
+            v = _gather_pages(v_cache, block_tables[b], kl, v_scale).repeat_interleave(g, dim=1)
+            j = torch.arange(kl, device=q.device) - (kl - n)
+            word = mask[t0:t0 + n][:, (j // 64).clamp(0, mask.shape[1] - 1)]
+            see = (j < 0) | ((word >> (j % 64) & 1 == 1) & (j < 64 * mask.shape[1]))     # [n, kl]
+            s = torch.einsum("qhd,khd->hqk", q[t0:t0 + n].to(k.dtype), k) * scale
+            s = s.masked_fill(~see, float("-inf"))
+            m = s.amax(-1, keepdim=True)
+            p = torch.exp(s - m.masked_fill(m == float("-inf"), 0.0))
+            z = p.sum(-1, keepdim=True)
+            p = p / torch.where(z == 0, 1.0, z)
+            fine = torch.isfinite(v)
+            o = torch.einsum("hqk,khd->qhd", p, torch.where(fine, v, 0.0))
+            for i in torch.nonzero(~fine.all(-1).all(-1)).flatten().tolist():
+                part = p[:, :, i].t()[..., None] * torch.where(fine[i], 0.0, v[i])
+                o = o + torch.where(see[:, i, None, None], part, 0.0)
+            out[t0:t0 + n] = o.to(q.dtype)
+        t0 += n
+    return out
+
+
+def _tree_probs(row: torch.Tensor, temperature: float) -> torch.Tensor:
+    """float64 probabilities of a row of logits; all zero where no logit is above -inf (a NaN counts as -inf; less than
+    2^-1000 of the largest as nothing).  A temperature that is not above 0 puts all of it on the first maximum."""
+    z = row.double()
+    z = torch.where(torch.isnan(z), float("-inf"), z)
+    top = z.max()
+    if top == float("-inf"):
+        return torch.zeros_like(z)
+    if not temperature > 0:
+        p = torch.zeros_like(z)
+        p[int((z == top).int().argmax())] = 1.0
+        return p
+    w = (z == top).double() if top == float("inf") else torch.exp((z - top) / temperature)
+    w = torch.where(w < 2.0 ** -1000, 0.0, w)
+    return w / w.sum()
+
+
+def tree_verify(logits, tokens, parents, q_lens: list, max_nodes: int, temperatures, uniforms, draw_uniforms,
+                draft_probs=None):
+    """(path int32 [B, max_nodes], length int32 [B], next token int32 [B]) by the walk through each tree.
+
+    At a node with the target's probabilities p = softmax(logits / temperature), its children are tried in order.
+    Child c with token x is taken if ``uniforms[c] * q(x) < p(x)``, and the walk goes on there; else p becomes
+    ``max(p - q, 0)`` over its sum (p stays where that is nothing), and the next child is tried.  q is the node's
+    row of ``draft_probs``, from which its children were drawn independently, or, without them, 1 at x alone (p
+    loses x).  Behind the last child the next token is drawn from p: the first x whose cumulative sum is
+    above ``draw_uniforms[b]`` times the total.  At temperatures of 0 and below, a child is taken if its
+    token is the first maximum of the logits, which is the next token too.
+
+    ``path`` holds the nodes of the walk, the root first, then -1; ``length`` counts them: the tokens that the step
+    adds are those of path[1:] and the next one.  Without any logit above -inf the next token is 0; a sequence
+    without nodes has length 0 and next token -1."""
+    tree_words(max_nodes)
+    b, v = len(q_lens), logits.shape[1]
+    path = torch.full((b, max_nodes), -1, dtype=torch.int32)
+    length = torch.zeros(b, dtype=torch.int32)
+    draws = torch.full((b,), -1, dtype=torch.int32)
+    par, tok, u = parents.tolist(), tokens.tolist(), uniforms.double().tolist()
+    t0 = 0
+    for i, n in enumerate(q_lens):
+        n, step = min(n, max_nodes), n
+        temperature, node, walk = float(temperatures[i]), 0, [0]
+        while n:
+            p = _tree_probs(logits[t0 + node], temperature)
+            greedy, q = not temperature > 0, None
+            if draft_probs is not None and not greedy:
+                q = draft_probs[t0 + node].double()
+                q = torch.where(q > 0, q, 0.0)
+            took = None
+            for c in (c for c in range(node + 1, n) if par[t0 + c] == node):
+                x = tok[t0 + c]
+                if not 0 <= x < v:
+                    took_it = False
+                elif greedy:
+                    took_it = float(p[x]) > 0
+                else:
+                    took_it = u[t0 + c] * (1.0 if q is None else float(q[x])) < float(p[x])
+                if took_it:
+                    took = c
+                    break
+                if greedy:
+                    continue
+                if q is None:
+                    r = p.clone()
+                    if 0 <= x < v:
+                        r[x] = 0.0
+                else:
+                    r = (p - q).clamp(min=0.0)
+                if float(r.sum()) > 0:
+                    p = r / r.sum()
+            if took is None:
+                break
+            node = took
+            walk.append(node)
+        if n:
+            total = p.cumsum(0)
+            share = min(max(float(draw_uniforms[i].nan_to_num(0.0)), 0.0), 1.0)
+            above = torch.nonzero(total > share * total[-1]).flatten()
+            held = torch.nonzero(p > 0).flatten()
+            draws[i] = int(above[0]) if len(above) else int(held[-1]) if len(held) else 0
+            path[i, :len(walk)] = torch.tensor(walk, dtype=torch.int32)
+            length[i] = len(walk)
+        t0 += step
+    return tuple(x.to(logits.device) for x in (path, length, draws))
+
+
+def tree_commit(kv_cache: torch.Tensor, q_lens: list, k_lens: list, block_tables: list, path: torch.Tensor,
+                lengths: torch.Tensor, kv_scale_cache: torch.Tensor | None = None) -> None:
+    """Moves the K/V of each sequence's path to consecutive positions, in every layer of the pool [2, L, blocks,
+    heads, block size, D]: row ``context_len - nodes + path[j]`` to ``context_len - nodes + j``.
+
+    The path ends at ``lengths``, or at an entry that is not above the one before it or no node of the tree.  fp8:
+    a block whose first row is moved takes that row's scale (as :func:`store_kv` gives a first token); a row is
+    rounded again where the scales differ.  int8: rows move with their scales."""
+    bs, nb = kv_cache.shape[4], kv_cache.shape[2]
+    fp8 = kv_cache.dtype == torch.float8_e4m3fn
+    raw = kv_cache.view(torch.uint8) if fp8 else kv_cache
+    for b, (n, kl) in enumerate(zip(q_lens, k_lens)):
+        base, table = kl - n, block_tables[b]
+        nodes: list[int] = []
+        for i in path[b, :max(0, min(int(lengths[b]), path.shape[1]))].tolist():
+            if not (nodes[-1] if nodes else -1) < i < n:
+                break
+            nodes.append(i)
+        if base < 0:
+            continue
+
+        def at(pos):
+            blk = table[pos // bs] if pos // bs < len(table) else -1
+            return (blk, pos % bs) if 0 <= blk < nb else None
+
+        rows = []
+        for i in nodes:
+            w = at(base + i)
+            x = s = None
+            if w is not None:
+                x = raw[:, :, w[0], :, w[1]].clone()
+                if kv_scale_cache is not None:
+                    s = (kv_scale_cache[:, :, w[0]] if fp8 else kv_scale_cache[:, :, w[0], :, w[1]]).clone()
+            rows.append((x, s))
+        for j, (i, (x, s)) in enumerate(zip(nodes, rows)):
+            w = at(base + j)
+            if i == j or x is None or w is None:
+                continue
+            if fp8:
+                f = x.view(kv_cache.dtype).float() * s[..., None]
+                if w[1] == 0:
+                    kv_scale_cache[:, :, w[0]] = fp8_block_scale(f.abs().nan_to_num(0.0).amax(-1))
+                now = kv_scale_cache[:, :, w[0]][..., None]
+                y = torch.clamp(f / now, -FP8_MAX, FP8_MAX).to(kv_cache.dtype).view(torch.uint8)
+                x = torch.where(now == s[..., None], x, y)
+            elif s is not None:
+                kv_scale_cache[:, :, w[0], :, w[1]] = s
+            raw[:, :, w[0], :, w[1]] = x
+
+
 def dense_causal_attention(q, k, v, scale):
     """No-cache attention for one sequence: q [L, Hq, D], k/v [L, Hkv, D]."""
     g = q.shape[1] // k.shape[1]

@@ -11,7 +11,10 @@ Additions used by the B200 kernels:
   the prefix-aware prefill kernel;
 * ``logits_indices``: token row of the last token of each sampling sequence
   (``cu_seqlens_q[i + 1] - 1``), computed on the host;
-* ``positions`` is carried by the runner, not here.
+* ``positions`` is carried by the runner, not here;
+* ``tree_mask``: a step that checks drafted tokens gives every sequence the nodes of a tree as its new
+  tokens and this mask of their ancestors (``ops.tree_mask``): attention then follows the mask instead of
+  the order of the rows.
 """
 from __future__ import annotations
 
@@ -38,6 +41,7 @@ class Context:
     host_q_lens: list | None = None
     host_k_lens: list | None = None
     kv_scales: tuple | None = None
+    tree_mask: torch.Tensor | None = None
 
 
 def get_context(cu_seqlens_q=None, cu_seqlens_k=None, max_seqlen_q=0, max_seqlen_k=0, slot_mapping=None,
