@@ -34,12 +34,11 @@ struct TreeAttn {
   float softmax_scale;
 };
 struct TreeAttnPlan {
-  int rg;           // row groups of 16 (query node, head) rows per CTA
-  int row_tiles;    // CTAs that share a stretch of K/V tiles
-  int chunks;       // stretches
+  int rows_cap;  // (node, query head) rows per CTA
+  int chunks;    // CTAs
   int64_t ws_floats;
 };
-TreeAttnPlan tree_attn_plan(int num_seqs, int max_nodes, int nq, int nkv, int num_sms);
+TreeAttnPlan tree_attn_plan(int max_nodes, int nq, int nkv, int num_sms);
 cudaError_t launch_tree_attention(const TreeAttn& a, const TreeAttnPlan& p, cudaStream_t stream);
 // Error word of a kernel that gave up on a bounded wait (0 = none).
 int tree_attn_error_code(int reset);

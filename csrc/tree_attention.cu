@@ -2,38 +2,49 @@
 //
 // Row r = (node, query head) of a KV head sees the positions before the tree and the nodes of its mask:
 //   o_r = sum_j a_rj v_j,  a = softmax_j(scale q_r . k_j)   over j < base or (j - base) in mask(node).
-// All rows of a KV head (nodes x nq / nkv) share its keys, so a tree of 8 nodes and 4 heads per KV head does 32
-// rows' work on each key that decode attention would read for 4: HBM still bounds it up to some 64 rows.
+// All rows of a KV head (nodes x nq / nkv) share its keys.  One CTA takes up to 256 rows of a (sequence, KV head) and
+// tiles of 128 keys:
+//   S = Q K^T    tcgen05, Q and K in shared memory, S [128 rows x 128 keys] fp32 in TMEM
+//   P = exp2(S - m), rounded to bf16, written over S: one row per thread, no shuffles
+//   O += P V     tcgen05, P in TMEM, V in shared memory, O [128 x 128] fp32 in TMEM
+// Two groups of four warps, each with an S, an O, a running maximum and a running sum of its own, work on alternate
+// steps, so that one's products run beside the other's exponentials: with up to 128 rows they take every other key
+// tile and are joined at the end, with more they take 128 rows each of every tile.
+// An e4m3 cache is converted once per value by four more warps, to bf16 (exact); K's scale multiplies the scores, V's
+// the weights before they are rounded.
 //
-// One warp streams tiles of 64 keys with TMA into a ring; eight warps work on them: RG groups of 16 rows, the 8 / RG
-// warps of a group on different keys, each with running maxima, sums and outputs of its own (fp32) that are joined
-// through shared memory once per (sequence, KV head).  bf16 mma.sync tiles; an e4m3 cache is converted once per
-// value, by four further warps, into f16 tiles (exact; K's scale multiplies the scores, V's is carried by the
-// accumulator's unit), so all that follows is the same kernel on f16.
-//
-// Balance: the tiles of all (sequence, KV head) pairs are laid end to end and cut into equal stretches, one per CTA,
-// whatever the sequences' lengths.  A pair that is cut leaves partial sums (at most two per CTA), which the second
+// Balance: the tiles of all (sequence, 256 rows, KV head) are laid end to end and cut into equal stretches, one per
+// CTA, whatever the sequences' lengths.  One that is cut leaves partial sums (at most two per CTA), which a second
 // kernel joins in the order of the keys: no atomics, the same bits on every run.
 //
-// Masks: only tiles that reach into the tree look at them.  What a row does not see takes no part in it: scores are
-// replaced by -inf, and where a value that some row must not see is infinite or NaN (0 x inf), the tile's V is
-// cleaned in registers and such values are added row by row.
+// Masks: only tiles that reach into the tree look at them.  What a row does not see takes no part in it: its score is
+// -inf, and a value that is infinite or NaN (0 x inf) is taken out of such a tile in shared memory and added at the
+// end to the rows that see it.
 #include <cuda.h>
 #include <cudaTypedefs.h>
-#include <cuda_fp16.h>
 
 #include "common.cuh"
 #include "tcgen05.cuh"
 #include "tree.h"
 
+#include <algorithm>
+#include <type_traits>
+
 namespace nvb {
 namespace {
 
-constexpr int AD = 128;      // head dim
-constexpr int KT = 64;       // keys per tile
-constexpr int NWARP = 8;     // warps that work on tiles
+constexpr int AD = 128;                 // head dim
+constexpr int KT = 128;                 // keys per tile
+constexpr int HALF = KT * 128;          // bytes of 64 dims of a 128-row tile
+constexpr int TILE = 2 * HALF;          // a 128 x 128 tile of 16-bit values
+constexpr int RAW_TILE = KT * AD;       // of 8-bit values
 constexpr float LOG2E = 1.4426950408889634f;
-constexpr uint64_t WAIT_NS = 2000000000ull;
+constexpr float RAISE = 8.f;            // the running maximum follows once a row's grows by 2^8
+// First warp of each role; 0-7: softmax, whose rows up to 64 are with warps 0, 1, 4 and 5: the polling MMA warps share
+// the other warps' schedulers.
+constexpr int W_TMA = 8, W_Q = 9, W_MMA = 10, W_CONV = 12;
+constexpr int BAD_WORDS = TREE_MAX_NODES / 32;
+constexpr float NOTHING = -3e38f;       // below any score
 
 __device__ int g_tree_error = 0;
 
@@ -42,85 +53,51 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-__device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
-}
-__device__ __forceinline__ void ldsm4t(uint32_t addr, uint32_t (&r)[4]) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
-}
-// c += a b: 16 x 16 times 16 x 8, f16 or bf16 in, fp32 sums
-template <bool F16>
-__device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  if constexpr (F16)
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  else
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-template <bool F16>
-__device__ __forceinline__ uint32_t pack(float lo, float hi) {
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   uint32_t d;
-  if constexpr (F16)
-    asm("cvt.rn.f16x2.f32 %0, %2, %1;" : "=r"(d) : "f"(lo), "f"(hi));
-  else
-    asm("cvt.rn.bf16x2.f32 %0, %2, %1;" : "=r"(d) : "f"(lo), "f"(hi));
+  asm("cvt.rn.bf16x2.f32 %0, %2, %1;" : "=r"(d) : "f"(lo), "f"(hi));
   return d;
 }
-template <bool F16>
-__device__ __forceinline__ float2 unpack(uint32_t x) {
-  if constexpr (F16)
-    return __half22float2(*reinterpret_cast<__half2*>(&x));
-  else
-    return __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&x));
-}
-// Set in bits 15 and 31 where a half of x is infinite or NaN (its exponent is all ones).
-template <bool F16>
-__device__ __forceinline__ uint32_t odd_halves(uint32_t x) {
-  return ((x & 0x7fff7fffu) + (F16 ? 0x04000400u : 0x00800080u)) & 0x80008000u;
-}
+// Set in bits 15 and 31 where a bf16 half of x is infinite or NaN (its exponent is all ones).
+__device__ __forceinline__ uint32_t odd_halves(uint32_t x) { return ((x & 0x7fff7fffu) + 0x00800080u) & 0x80008000u; }
 
 struct Args {
   TreeAttn t;
-  int G, row_tiles, chunks, bs_shift;
-  int box_rows;     // rows per TMA box: min(64, block size)
+  int G, chunks, bs_shift;
+  int rows_cap;     // rows of a CTA: 128 or 256
+  int slots;        // tiles of the 16-bit ring (K and V in turn)
+  int raw_slots;    // and of the e4m3 ring
+  int box_rows;     // rows per TMA box: min(128, block size)
   int oob_row;      // a row behind the pool: reads as zeros
+  int q16;          // q's rows are 16-byte aligned
   float scale_log2;
 };
 
 // ------------------------------------------------------------------- the list of tiles
-// Sequence b with nodes has max(1, ceil(k_len / 64)) tiles for each of its KV heads (an empty context still writes
-// its zeros); tile i of the list belongs to the sequence, head and key tile that come from dividing through.
+// Sequence b with nodes has max(1, ceil(k_len / 128)) tiles for each KV head and stretch of rows (an empty context
+// still writes its zeros).  The list runs over sequences, stretches of rows, KV heads and tiles.
 __device__ __forceinline__ int seq_begin(const TreeAttn& t, int b) { return min(max(t.cu_q[b], 0), t.T); }
 __device__ __forceinline__ int seq_nodes(const TreeAttn& t, int b) { return min(t.cu_q[b + 1], t.T) - seq_begin(t, b); }
-__device__ __forceinline__ int seq_tiles(const TreeAttn& t, int b) {
-  return seq_nodes(t, b) > 0 ? max(1, (t.ctx_lens[b] + KT - 1) / KT) : 0;
+__device__ __forceinline__ int seq_rows(const Args& a, int b) { return min(seq_nodes(a.t, b), a.t.max_nodes) * a.G; }
+__device__ __forceinline__ int seq_tiles(const TreeAttn& t, int b) { return max(1, (t.ctx_lens[b] + KT - 1) / KT); }
+__device__ __forceinline__ int64_t seq_count(const Args& a, int b) {
+  const int rows = seq_rows(a, b);
+  return rows > 0 ? (int64_t)seq_tiles(a.t, b) * a.t.nkv * ((rows + a.rows_cap - 1) / a.rows_cap) : 0;
 }
 
-struct Where {
-  int b;        // sequence
-  int64_t rem;  // tiles between its first one and the place
-};
-
-// total number of tiles, and the sequences in which places `lo` and `hi` of chunk `c` lie.  All threads of the CTA.
+// Stretch [lo, hi) of the list, and the sequences in which its ends lie, with the tiles before them in it.
 struct Spot {
-  int64_t total, lo, hi;
-  Where at_lo, at_hi;
+  int64_t total, lo, hi, lo_rem, hi_rem;
+  int lo_seq, hi_seq;
 };
 
-__device__ void find_chunk(const Args& a, int c, Spot* out) {
-  __shared__ int64_t part[33];
+// All threads of the CTA.
+__device__ void find_chunk(const Args& a, int c, Spot* out, int64_t* part) {
   const int nt = blockDim.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, nw = nt >> 5;
   const int per = (a.t.num_seqs + nt - 1) / nt;
   const int b0 = min(a.t.num_seqs, (int)threadIdx.x * per), b1 = min(a.t.num_seqs, b0 + per);
   int64_t sum = 0;
-  for (int b = b0; b < b1; ++b) sum += (int64_t)seq_tiles(a.t, b) * a.t.nkv;
+  for (int b = b0; b < b1; ++b) sum += seq_count(a, b);
   int64_t incl = sum;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -129,45 +106,52 @@ __device__ void find_chunk(const Args& a, int c, Spot* out) {
   }
   if (lane == 31) part[warp] = incl;
   __syncthreads();
-  if (threadIdx.x == 0) {
-    int64_t s = 0;
-    for (int w = 0; w < nw; ++w) {
-      const int64_t x = part[w];
-      part[w] = s;
-      s += x;
-    }
-    part[32] = s;
-    out->total = s;
-    out->lo = s * c / a.chunks;
-    out->hi = s * (c + 1) / a.chunks;
-    out->at_lo.b = out->at_hi.b = a.t.num_seqs;
-    out->at_lo.rem = out->at_hi.rem = 0;
+  int64_t before = 0, total = 0;
+  for (int w = 0; w < nw; ++w) {
+    if (w < warp) before += part[w];
+    total += part[w];
   }
-  __syncthreads();
-  int64_t at = part[warp] + incl - sum;
-  const int64_t lo = out->lo, hi = out->hi;
+  const int64_t lo = total * c / a.chunks, hi = total * (c + 1) / a.chunks;
+  if (threadIdx.x == 0) {
+    out->total = total;
+    out->lo = lo;
+    out->hi = hi;
+  }
+  int64_t at = before + incl - sum;
   for (int b = b0; b < b1; ++b) {
-    const int64_t n = (int64_t)seq_tiles(a.t, b) * a.t.nkv;
-    if (lo >= at && lo < at + n) out->at_lo = {b, lo - at};
-    if (hi >= at && hi < at + n) out->at_hi = {b, hi - at};
+    const int64_t n = seq_count(a, b);
+    if (lo >= at && lo < at + n) {
+      out->lo_seq = b;
+      out->lo_rem = lo - at;
+    }
+    if (hi >= at && hi < at + n) {
+      out->hi_seq = b;
+      out->hi_rem = hi - at;
+    }
     at += n;
   }
   __syncthreads();
 }
 
-// Walks the (sequence, KV head) pairs of a stretch: tiles [t0, t1) of each.
+// Walks the items of a stretch: tiles [t0, t1) of KV head h and rows [row0, row0 + rows) of sequence b.
 struct Walk {
-  int b, h, t0, t1, tiles;
+  int b, rt, h, t0, t1, tiles, rts;
   int64_t left;
+  __device__ __forceinline__ void enter(const Args& a) {
+    tiles = seq_tiles(a.t, b);
+    rts = (seq_rows(a, b) + a.rows_cap - 1) / a.rows_cap;
+  }
   __device__ __forceinline__ Walk(const Args& a, const Spot& s) {
-    b = s.at_lo.b;
     left = s.hi - s.lo;
-    tiles = 0;
-    h = t0 = t1 = 0;
+    b = rt = h = t0 = t1 = tiles = rts = 0;
     if (left > 0) {
-      tiles = seq_tiles(a.t, b);
-      h = (int)(s.at_lo.rem / tiles);
-      t0 = (int)(s.at_lo.rem % tiles);
+      b = s.lo_seq;
+      enter(a);
+      const int per = tiles * a.t.nkv;  // below 2^31: k_len / 128 x nkv
+      rt = (int)(s.lo_rem / per);
+      const int r = (int)(s.lo_rem % per);
+      h = r / tiles;
+      t0 = r % tiles;
       t1 = (int)min((int64_t)tiles, t0 + left);
     }
   }
@@ -177,162 +161,666 @@ struct Walk {
     if (left <= 0) return;
     if (t1 == tiles && ++h == a.t.nkv) {
       h = 0;
-      do ++b;
-      while ((tiles = seq_tiles(a.t, b)) == 0);
+      if (++rt == rts) {
+        rt = 0;
+        do ++b;
+        while (seq_rows(a, b) <= 0);
+        enter(a);
+      }
     }
     t0 = 0;
     t1 = (int)min((int64_t)tiles, left);
   }
-  // rows of this pair in row tile rt
-  __device__ __forceinline__ int rows(const Args& a, int rt, int per_tile) const {
-    return min(per_tile, min(seq_nodes(a.t, b), a.t.max_nodes) * a.G - rt * per_tile);
-  }
+  __device__ __forceinline__ int rows(const Args& a) const { return min(a.rows_cap, seq_rows(a, b) - rt * a.rows_cap); }
 };
 
 // Partial sums of slot s (2 per CTA): rows x 128 outputs (not divided by the sum), then rows x (maximum, sum).
-__device__ __forceinline__ float* slot_o(const Args& a, int rows, int cta, int slot) {
-  return a.t.ws + (int64_t)(cta * 2 + slot) * rows * (AD + 2);
+__device__ __forceinline__ float* slot_o(const Args& a, int cta, int slot) {
+  return a.t.ws + (int64_t)(cta * 2 + slot) * a.rows_cap * (AD + 2);
 }
 
 // ------------------------------------------------------------------------ main kernel
-template <bool FP8>
-struct Cfg {
-  static constexpr int KV_BYTES = KT * AD * 2;        // one K or V tile in 16 bits
-  static constexpr int STAGE = 2 * KV_BYTES;
-  static constexpr int RING = FP8 ? 2 : 4;            // 16-bit stages
-  static constexpr int RAW = FP8 ? 5 : 0;             // e4m3 stages
-  static constexpr int RAW_STAGE = 2 * KT * AD;
-  static constexpr int CONV = FP8 ? 4 : 0;            // converting warps
-  static constexpr int THREADS = (NWARP + 1 + CONV) * 32;
-  static constexpr int MERGE = NWARP * 16 * AD * 4;   // the warps' outputs
-  static constexpr int SMEM = 1024 + RING * STAGE + RAW * RAW_STAGE + MERGE + NWARP * 16 * 8 + 512;
-};
-
-// Byte offset of (row, 16-byte chunk) in a 16-bit tile: [2 halves of 64 dims][64 rows][128 B], 128-byte swizzle.
+// Byte offset of (row, 16-byte chunk) in a tile: [2 halves of 64 dims][128 rows][128 B], 128-byte swizzle.
 __device__ __forceinline__ uint32_t tile_at(int r, int c16) {
-  return (uint32_t)((c16 >> 3) * (KT * 128) + r * 128 + (((c16 & 7) ^ (r & 7)) << 4));
+  return (uint32_t)((c16 >> 3) * HALF + r * 128 + (((c16 & 7) ^ (r & 7)) << 4));
 }
 
-template <bool FP8, int RG>
-__global__ void __launch_bounds__(Cfg<FP8>::THREADS, 1)
-    tree_attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, Args a) {
-  using C = Cfg<FP8>;
-  constexpr int SH = NWARP / RG;             // warps that share a row group
-  constexpr int KG = SH < 4 ? SH : 4;        // of them, on different keys of one tile
-  constexpr int TG = SH / KG;                // tiles worked on at a time
-  constexpr int KW = KT / KG;                // keys of a warp
-  constexpr int NT = KW / 8;                 // 8-key tiles of its scores
-  constexpr int ROWS = RG * 16;
-  pdl_wait();     // inputs come from the previous kernel in the stream
-  pdl_trigger();  // the next kernel may start its prologue
-  extern __shared__ __align__(1024) uint8_t raw_sm[];
-  uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw_sm) + 1023) & ~uintptr_t(1023));
-  uint8_t* ring = sm;
-  uint8_t* rawr = ring + C::RING * C::STAGE;
-  float* merge_o = reinterpret_cast<float*>(rawr + C::RAW * C::RAW_STAGE);
-  float2* merge_ml = reinterpret_cast<float2*>(reinterpret_cast<uint8_t*>(merge_o) + C::MERGE);
-  uint64_t* bars = reinterpret_cast<uint64_t*>(merge_ml + NWARP * 16);
-  volatile int* gave_up = reinterpret_cast<volatile int*>(bars + 2 * (C::RING + C::RAW));
-  __shared__ Spot spot;
-  __shared__ float2 unit_scale[C::RING][KT / 16];  // e4m3: (K, V) scales of 16 keys
-  const uint32_t bar0 = smem_u32(bars);
-  auto full = [&](int s) { return bar0 + 8u * s; };
-  auto empty = [&](int s) { return bar0 + 8u * (C::RING + s); };
-  auto raw_full = [&](int s) { return bar0 + 8u * (2 * C::RING + s); };
-  auto raw_empty = [&](int s) { return bar0 + 8u * (2 * C::RING + C::RAW + s); };
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int rt = blockIdx.x % a.row_tiles, chunk = blockIdx.x / a.row_tiles;
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < C::RING; ++s) {
-      tc::mbar_init(full(s), FP8 ? C::CONV * 32 : 1);
-      tc::mbar_init(empty(s), RG * KG);
-    }
-    for (int s = 0; s < C::RAW; ++s) {
-      tc::mbar_init(raw_full(s), 1);
-      tc::mbar_init(raw_empty(s), C::CONV);
-    }
-    *gave_up = 0;
-    tc::fence_barrier_init();
-  }
-  find_chunk(a, chunk, &spot);  // ends with a barrier
+struct Small {  // shared memory besides the tiles
+  uint64_t full[8], empty[8], raw_full[8], raw_empty[8];
+  uint64_t q_full, q_empty, s_full[2], p_ready[2], o_done[2], o_empty, drain[2];
+  uint64_t scale_full[4];
+  float2 ml[2][128];        // (maximum, sum) of the groups' rows
+  float2 scale[4][KT / 16];  // e4m3: (K, V) scales of 16 keys, of the last four tiles
+  uint32_t bad[2][BAD_WORDS];  // nodes whose values are not finite
+  int64_t part[16];
+  Spot spot;
+  uint32_t tmem;
+  int gave_up;
+};
 
-  // Bounded wait; on expiry every role goes on without waiting, and the outputs are not valid.
-  auto wait = [&](uint32_t bar, uint32_t parity, int code) -> bool {
-    if (tc::mbar_try(bar, parity)) return true;
-    SpinBudget sb;
-    while (!tc::mbar_try(bar, parity)) {
-      if (*gave_up) return false;
-      if (sb.expired(WAIT_NS)) {
-        atomicCAS(&g_tree_error, 0, code);
-        *gave_up = 1;
-        return false;
+__host__ __device__ constexpr int smem_bytes(int q_tiles, int slots, int raw_slots) {
+  return q_tiles * TILE + slots * TILE + raw_slots * RAW_TILE + (int)sizeof(Small);
+}
+
+// e4m3 x 4 -> bf16 x 4, exactly: the bits of exponent and mantissa are shifted into place, and a product with 2^120
+// makes up for the exponents' difference (subnormals too).  A NaN becomes 480, which no e4m3 value is.
+__device__ __forceinline__ void e4m3x4_to_bf16(uint32_t x, uint32_t& lo, uint32_t& hi) {
+  uint32_t a = __byte_perm(x, 0, 0x1404), b = __byte_perm(x, 0, 0x3424);
+  a = (a & 0x80008000u) | ((a >> 4) & 0x07f007f0u);
+  b = (b & 0x80008000u) | ((b >> 4) & 0x07f007f0u);
+  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(lo) : "r"(a), "r"(0x7b807b80u));
+  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(hi) : "r"(b), "r"(0x7b807b80u));
+}
+
+// A tile of e4m3 values (rows of 128 bytes) -> bf16 in a swizzled tile.  128 threads.
+__device__ __forceinline__ void convert_tile(const uint8_t* src, uint8_t* dst, int tid) {
+  uint4 x[8];
+#pragma unroll
+  for (int u = 0; u < 8; ++u) x[u] = *reinterpret_cast<const uint4*>(src + (tid + u * 128) * 16);
+#pragma unroll
+  for (int u = 0; u < 8; ++u) {
+    const int idx = tid + u * 128, r = idx >> 3, i = idx & 7;  // 16 values of row r
+    const uint32_t in[4] = {x[u].x, x[u].y, x[u].z, x[u].w};
+    uint32_t h[8], nan = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      e4m3x4_to_bf16(in[e], h[2 * e], h[2 * e + 1]);
+      nan |= (in[e] & 0x7f7f7f7fu) + 0x01010101u;
+    }
+    if (nan & 0x80808080u) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        if ((h[e] & 0x7fffu) == 0x43f0u) h[e] |= 0x7fffu;  // 480
+        if ((h[e] & 0x7fff0000u) == 0x43f00000u) h[e] |= 0x7fff0000u;
       }
     }
-    return true;
-  };
+    *reinterpret_cast<uint4*>(dst + tile_at(r, 2 * i)) = make_uint4(h[0], h[1], h[2], h[3]);
+    *reinterpret_cast<uint4*>(dst + tile_at(r, 2 * i + 1)) = make_uint4(h[4], h[5], h[6], h[7]);
+  }
+}
 
-  if (warp == NWARP) {
-    // ------------------------------------------------------------------ TMA producer
-    if (lane != 0) return;
-    tc::prefetch_map(&kmap);
-    tc::prefetch_map(&vmap);
-    constexpr int DEPTH = FP8 ? C::RAW : C::RING;
-    int i = 0;
-    bool ok = true;
-    for (Walk w(a, spot); w.more() && ok; w.next(a)) {
-      if (w.rows(a, rt, ROWS) <= 0) continue;
-      const int* bt = a.t.block_tables + w.b * a.t.bt_stride;
-      for (int t = w.t0; t < w.t1; ++t, ++i) {
-        const int s = i % DEPTH;
-        if (!wait(FP8 ? raw_empty(s) : empty(s), ((i / DEPTH) & 1) ^ 1, 1)) {
-          ok = false;
-          break;
-        }
-        const uint32_t bar = FP8 ? raw_full(s) : full(s);
-        uint8_t* kd = FP8 ? rawr + s * C::RAW_STAGE : ring + s * C::STAGE;
-        uint8_t* vd = kd + (FP8 ? C::RAW_STAGE : C::STAGE) / 2;
-        tc::mbar_arrive_expect_tx(bar, FP8 ? C::RAW_STAGE : C::STAGE);
-        for (int r = 0; r < KT; r += a.box_rows) {
-          const int tok = t * KT + r, bi = tok >> a.bs_shift;
-          int row = a.oob_row;
-          if (bi < a.t.W) {
-            const int blk = bt[bi];
-            if (blk >= 0 && blk < a.t.num_blocks)
-              row = ((blk * a.t.nkv + w.h) << a.bs_shift) + (tok & (a.t.block_size - 1));
+// Keys [key0, key0 + 64) that a row sees, as bits: those before the tree and its mask's, within the context.
+__device__ __forceinline__ uint64_t visible(const uint64_t (&mask)[TREE_WORDS], int key0, int base, int k_len) {
+  const int d = base - key0;
+  uint64_t see;
+  if (d >= 64) {
+    see = ~0ull;
+  } else if (d > 0) {
+    see = ((1ull << d) - 1) | (mask[0] << d);
+  } else {
+    const int word = -d >> 6, sh = -d & 63;
+    uint64_t lo = 0, hi = 0;
+#pragma unroll
+    for (int i = 0; i < TREE_WORDS; ++i) {
+      if (i == word) lo = mask[i];
+      if (i == word + 1) hi = mask[i];
+    }
+    see = sh ? lo >> sh | hi << (64 - sh) : lo;
+  }
+  const int valid = k_len - key0;
+  if (valid < 64) see &= valid > 0 ? (1ull << valid) - 1 : 0ull;
+  return see;
+}
+
+// 32 bytes of a row in one store: whole sectors.
+__device__ __forceinline__ void st32(void* p, const uint32_t (&v)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+               "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
+
+// With 512 threads (e4m3) the block starts with 128 registers per thread; the softmax warps take more from the other
+// warpgroups: 2 x 176 + 56 + 104 = 4 x 128.
+template <int N>
+__device__ __forceinline__ void regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+
+// (a, b) * f + c and (a, b) + (c, d) in one instruction each
+__device__ __forceinline__ float2 fma2(uint32_t a, uint32_t b, float f, float c) {
+  float2 r;
+  asm("{\n .reg .b64 x, y, z;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %4};\n mov.b64 z, {%5, %5};\n"
+      " fma.rn.f32x2 z, x, y, z;\n mov.b64 {%0, %1}, z;\n}\n"
+      : "=f"(r.x), "=f"(r.y)
+      : "r"(a), "r"(b), "f"(f), "f"(c));
+  return r;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n .reg .b64 x, y;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n add.rn.f32x2 x, x, y;\n mov.b64 {%0, %1}, x;\n}\n"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+
+// Bounded wait of a whole warp; on expiry every role goes on without waiting, and the outputs are not valid.  The same
+// answer in every lane.  One lane polls.
+__device__ __forceinline__ bool warp_poll(uint32_t bar, uint32_t parity, volatile int* gave_up, int code) {
+  int ok = 1;
+  if ((threadIdx.x & 31) == 0) {
+    SpinBudget sb;
+    while (!tc::mbar_try(bar, parity)) {
+      if (*gave_up) {
+        ok = 0;
+        break;
+      }
+      if (sb.expired(tc::WAIT_BUDGET_NS)) {
+        atomicCAS(&g_tree_error, 0, code);
+        *gave_up = 1;
+        ok = 0;
+        break;
+      }
+    }
+  }
+  ok = __shfl_sync(FULL_MASK, ok, 0);
+  if (ok) tc::mbar_try(bar, parity);  // the phase is complete: this orders the other lanes' accesses
+  return ok != 0;
+}
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* gave_up, int code) {
+  if (__all_sync(FULL_MASK, tc::mbar_try(bar, parity))) return true;
+  return warp_poll(bar, parity, gave_up, code);
+}
+
+// The part of nodes whose values were taken out of the products in a row that sees them, from the cache: the values
+// themselves (infinite or NaN), added to the row's outputs [d0, d0 + n) at `out`.
+template <bool FP8, typename T>
+__device__ __forceinline__ void add_bad(const Args& a, const Walk& w, const uint32_t* bad, int node, int d0, int n, T* out) {
+  const int qrow = seq_begin(a.t, w.b), nodes = seq_nodes(a.t, w.b), base = a.t.ctx_lens[w.b] - nodes;
+  for (int nd = 0; nd < min(nodes, min(TREE_WORDS, a.t.words) * 64); ++nd) {
+    if (!(bad[nd >> 5] >> (nd & 31) & 1) || !(a.t.mask[(int64_t)(qrow + node) * a.t.mask_stride + (nd >> 6)] >> (nd & 63) & 1))
+      continue;
+    const int pos = base + nd;
+    if (pos < w.t0 * KT || pos >= w.t1 * KT || (pos >> a.bs_shift) >= a.t.W) continue;
+    const int blk = a.t.block_tables[w.b * a.t.bt_stride + (pos >> a.bs_shift)];
+    if (blk < 0 || blk >= a.t.num_blocks) continue;
+    const int64_t at = ((((int64_t)blk * a.t.nkv + w.h) << a.bs_shift) + (pos & (a.t.block_size - 1))) * AD + d0;
+    for (int i = 0; i < n; ++i) {
+      float z;
+      if constexpr (FP8)
+        z = (static_cast<const uint8_t*>(a.t.v_cache)[at + i] & 0x7f) == 0x7f ? NAN : 0.f;
+      else
+        z = __bfloat162float(static_cast<const __nv_bfloat16*>(a.t.v_cache)[at + i]);
+      if (!(fabsf(z) < INFINITY)) {
+        if constexpr (sizeof(T) == 2)
+          out[i] = __float2bfloat16_rn(__bfloat162float(out[i]) + z);
+        else
+          out[i] += z;
+      }
+    }
+  }
+}
+
+// A place in a ring of S slots.
+struct Place {
+  int s = 0;
+  uint32_t ph = 0;
+  __device__ __forceinline__ void step(int by, int S) {  // by <= S
+    s += by;
+    if (s >= S) {
+      s -= S;
+      ph ^= 1;
+    }
+  }
+};
+
+template <bool FP8>
+__global__ void __launch_bounds__(FP8 ? 512 : 384, 1)
+    tree_attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, Args a) {
+  pdl_wait();     // inputs come from the previous kernel in the stream
+  pdl_trigger();  // the next kernel may start its prologue
+  extern __shared__ __align__(1024) uint8_t sm[];
+  const int q_tiles = a.rows_cap / 128, S = a.slots, RS = a.raw_slots;
+  uint8_t* sq = sm;
+  uint8_t* ring = sq + q_tiles * TILE;
+  uint8_t* rawr = ring + S * TILE;
+  Small& sh = *reinterpret_cast<Small*>(rawr + RS * RAW_TILE);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  auto bar = [](uint64_t& b) { return smem_u32(&b); };
+  if (smem_u32(sm) & 1023) {  // the swizzle goes by the address
+    if (threadIdx.x == 0) atomicCAS(&g_tree_error, 0, 9);
+    return;
+  }
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < 8; ++s) {
+      tc::mbar_init(bar(sh.full[s]), FP8 ? 4 : 1);
+      tc::mbar_init(bar(sh.empty[s]), 2);
+      tc::mbar_init(bar(sh.raw_full[s]), 1);
+      tc::mbar_init(bar(sh.raw_empty[s]), 4);
+    }
+    tc::mbar_init(bar(sh.q_full), 1);
+    tc::mbar_init(bar(sh.q_empty), 2);
+    for (int g = 0; g < 2; ++g) {
+      tc::mbar_init(bar(sh.s_full[g]), 1);
+      tc::mbar_init(bar(sh.p_ready[g]), 4);
+      tc::mbar_init(bar(sh.o_done[g]), 1);
+      tc::mbar_init(bar(sh.drain[g]), 1);
+    }
+    tc::mbar_init(bar(sh.o_empty), 8);
+    for (int s = 0; s < 4; ++s) tc::mbar_init(bar(sh.scale_full[s]), 1);
+    sh.gave_up = 0;
+    tc::fence_barrier_init();
+  }
+  if (threadIdx.x < 2 * BAD_WORDS) sh.bad[threadIdx.x / BAD_WORDS][threadIdx.x % BAD_WORDS] = 0;
+  if (warp == W_MMA) tc::tmem_alloc<1>(smem_u32(&sh.tmem), 512);
+  tc::fence_before();
+  find_chunk(a, blockIdx.x, &sh.spot, sh.part);  // ends with a barrier
+  tc::fence_after();
+  const uint32_t tmem = sh.tmem;
+  volatile int* gave_up = &sh.gave_up;
+
+  auto wait = [&](uint64_t& b, uint32_t parity, int code) { return warp_wait(bar(b), parity, &sh.gave_up, code); };
+
+  if (warp < W_TMA) {
+    // ------------------------------------------------------------------ softmax, outputs
+    if constexpr (FP8) regs_inc<176>();
+    const int g = warp >> 2, q4 = warp & 3, lr = q4 * 32 + lane;  // TMEM lane = row of the group
+    const uint32_t lanes = (uint32_t)(q4 * 32) << 16;
+    const uint32_t s_tm = tmem + g * 128u + lanes, o_tm = tmem + 256u + lanes;  // O of group k: + 128 k
+    uint32_t n_done = 0;  // steps of this group so far
+    // The groups make their weights in turn: left alone they fall into step, and then both wait for products at a
+    // time and share the exponentials' units at another.
+    auto turn_take = [&]() { asm volatile("bar.sync %0, 256;" ::"r"(2 + g) : "memory"); };
+    auto turn_pass = [&]() { asm volatile("bar.arrive %0, 256;" ::"r"(3 - g) : "memory"); };
+    if (g == 1) turn_pass();
+    int tile0 = 0, items = 0;  // tiles before this item
+    for (Walk w(a, sh.spot); w.more(); w.next(a), ++items) {
+      const int n = w.t1 - w.t0, rows = w.rows(a), two = rows > 128, steps = two ? 2 * n : n;
+      const int row = two ? g * 128 + lr : lr, R = w.rt * a.rows_cap + row;
+      const bool live = row < rows, work = __any_sync(FULL_MASK, live);
+      const int qrow = seq_begin(a.t, w.b), nodes = seq_nodes(a.t, w.b), k_len = a.t.ctx_lens[w.b], base = k_len - nodes;
+      const int node = live ? R / a.G : 0, head = w.h * a.G + (live ? R % a.G : 0);
+      uint64_t bits[TREE_WORDS];  // the row's mask
+#pragma unroll
+      for (int i = 0; i < TREE_WORDS; ++i)
+        bits[i] = i < a.t.words ? (uint64_t)a.t.mask[(int64_t)(qrow + node) * a.t.mask_stride + i] : 0ull;
+      float m = -INFINITY, l = 0.f;
+      int mine = 0;
+      for (int st = g; st < steps; st += 2, ++mine, ++n_done) {
+        const int j = two ? st >> 1 : st, t = w.t0 + j;
+        wait(sh.s_full[g], n_done & 1, 8);
+        tc::fence_after();
+        const bool masked = t * KT + KT > base;
+        const float2* scl = sh.scale[(tile0 + j) & 3];
+        // (not K's own barrier: its slot may have been filled again by now.  This one is filled for the fourth tile
+        // from here, once this one's weights are used.)
+        if constexpr (FP8) wait(sh.scale_full[(tile0 + j) & 3], ((tile0 + j) >> 2) & 1, 10);
+        auto softmax = [&](auto with_mask) {
+          constexpr bool MASK = decltype(with_mask)::value;
+          uint32_t see[4] = {~0u, ~0u, ~0u, ~0u}, x[2][16], p[64];
+          if constexpr (MASK) {
+            const uint64_t s0 = visible(bits, t * KT, base, k_len), s1 = visible(bits, t * KT + 64, base, k_len);
+            see[0] = (uint32_t)s0;
+            see[1] = (uint32_t)(s0 >> 32);
+            see[2] = (uint32_t)s1;
+            see[3] = (uint32_t)(s1 >> 32);
           }
-          if constexpr (FP8) {
-            tc::tma_load_2d(smem_u32(kd + r * AD), &kmap, bar, 0, row);
-            tc::tma_load_2d(smem_u32(vd + r * AD), &vmap, bar, 0, row);
+          // 16 columns (keys) at a time, the next ones on their way: f(column group, their scores in units of log2
+          // of weights, times K's scale)
+          auto columns = [&](auto&& f) {
+            tc::tmem_ld(s_tm, x[0]);
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+              tc::ld_wait(x[c & 1]);
+              if (c < 7) tc::tmem_ld(s_tm + 16 * (c + 1), x[(c + 1) & 1]);
+              f(c, x[c & 1]);
+            }
+          };
+          auto seen = [&](int c, int i) { return !MASK || (see[c >> 1] >> (16 * (c & 1) + i) & 1); };
+          auto factor = [&](int c) { return FP8 ? a.scale_log2 * scl[c].x : a.scale_log2; };
+          float2 ls[2];
+          float top;
+          // weights relative to `sub`, their sum, and the largest exponent
+          auto weights = [&](float sub) {
+            ls[0] = ls[1] = make_float2(0.f, 0.f);
+            float mx[2] = {-INFINITY, -INFINITY};
+            columns([&](int c, uint32_t(&v)[16]) {
+              const float f = factor(c);
+#pragma unroll
+              for (int i = 0; i < 16; i += 2) {
+                float2 y = fma2(v[i], v[i + 1], f, -sub);
+                if (!seen(c, i)) y.x = -INFINITY;
+                if (!seen(c, i + 1)) y.y = -INFINITY;
+                mx[0] = fmaxf(mx[0], y.x);
+                mx[1] = fmaxf(mx[1], y.y);
+                y = make_float2(ex2(y.x), ex2(y.y));
+                ls[i >> 1 & 1] = add2(ls[i >> 1 & 1], y);
+                if constexpr (FP8) {
+                  y.x *= scl[c].y;
+                  y.y *= scl[c].y;
+                }
+                // rounded by 2^-9 of a weight at most; the sum takes the weights as they were
+                p[8 * c + (i >> 1)] = pack_bf16(y.x, y.y);
+              }
+            });
+            top = fmaxf(mx[0], mx[1]);
+          };
+          if (mine == 0) {  // the first tile's maximum; later ones mostly stay within 2^RAISE of it
+            top = -INFINITY;
+            columns([&](int c, uint32_t(&v)[16]) {
+              float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+              for (int i = 0; i < 16; ++i)
+                if (seen(c, i)) mx[i & 1] = fmaxf(mx[i & 1], __uint_as_float(v[i]));
+              const float mc = fmaxf(mx[0], mx[1]);
+              if (mc > -INFINITY) top = fmaxf(top, mc * factor(c));
+            });
+            m = top;
+          }
+          weights(m == -INFINITY ? 0.f : m);
+          const bool raise = top > RAISE || (m == -INFINITY && top > -INFINITY);
+          if (mine > 0 && __any_sync(FULL_MASK, raise)) {
+            // the outputs so far move to the new maximum, and the weights are made again
+            const float nm = raise ? (m == -INFINITY ? top : m + top) : m, f = raise ? ex2(m - nm) : 1.f;
+            wait(sh.o_done[g], (n_done - 1) & 1, 11);
+            tc::fence_after();
+#pragma unroll 1
+            for (int c = 0; c < 8; ++c) {
+              uint32_t o[16];
+              tc::tmem_ld(o_tm + 128 * g + 16 * c, o);
+              tc::ld_wait(o);
+#pragma unroll
+              for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+              tc::tmem_st(o_tm + 128 * g + 16 * c, o);
+            }
+            l *= f;
+            m = nm;
+            weights(m == -INFINITY ? 0.f : m);
+          }
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            uint32_t(&pc)[16] = *reinterpret_cast<uint32_t(*)[16]>(p + 16 * c);
+            tc::tmem_st(s_tm + 16 * c, pc);  // over the scores
+          }
+          ls[0] = add2(ls[0], ls[1]);
+          l += ls[0].x + ls[0].y;
+          tc::st_wait();
+        };
+        turn_take();
+        if (work) {
+          if (masked)
+            softmax(std::true_type());
+          else
+            softmax(std::false_type());
+        }
+        turn_pass();
+        if (masked) {
+          // this group's threads look through V, a key each: positions behind the context hold any bits, and
+          // a node's infinities and NaN go to the rows that see it at the end.  (Where both groups use the tile, both
+          // do, since neither's product waits for the other's threads; they write the same.)
+          const int c = 2 * (tile0 + j) + 1, pos = t * KT + lr;
+          wait(sh.full[c % S], (c / S) & 1, 12);
+          uint8_t* v = ring + (c % S) * TILE;
+          if (pos >= base) {
+            bool odd = false;
+#pragma unroll 4
+            for (int i = 0; i < 16; ++i) {
+              uint4& x = *reinterpret_cast<uint4*>(v + tile_at(lr, i));
+              if (pos >= k_len) {
+                x = make_uint4(0, 0, 0, 0);
+                continue;
+              }
+              uint4 y = x;
+              const uint32_t o[4] = {odd_halves(y.x), odd_halves(y.y), odd_halves(y.z), odd_halves(y.w)};
+              if (o[0] | o[1] | o[2] | o[3]) {
+                odd = true;
+                y.x &= ~((o[0] >> 15) * 0xffffu);
+                y.y &= ~((o[1] >> 15) * 0xffffu);
+                y.z &= ~((o[2] >> 15) * 0xffffu);
+                y.w &= ~((o[3] >> 15) * 0xffffu);
+                x = y;
+              }
+            }
+            const int nd = pos - base;
+            if (odd && nd >= 0 && nd < TREE_MAX_NODES) atomicOr(&sh.bad[items & 1][nd >> 5], 1u << (nd & 31));
+          }
+          tc::fence_proxy_async();
+        }
+        tc::fence_before();
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive_release(bar(sh.p_ready[g]));
+      }
+      if (g == 1 && !two && (n & 1)) {  // the other group had a step more
+        turn_take();
+        turn_pass();
+      }
+      // ---- outputs
+      sh.ml[g][lr] = make_float2(m, l);
+      if (mine) wait(sh.o_done[g], (n_done - 1) & 1, 13);
+      tc::fence_before();
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      tc::fence_after();
+      const float2 ml0 = sh.ml[0][lr], ml1 = sh.ml[1][lr];
+      uint32_t any = 0;
+#pragma unroll
+      for (int i = 0; i < BAD_WORDS; ++i) any |= sh.bad[items & 1][i];
+      if (g == 0 && lr < BAD_WORDS) sh.bad[(items + 1) & 1][lr] = 0;
+      // the groups' sums by their weights: with more than 128 rows a group has rows of its own
+      float w0 = 0.f, w1 = 0.f, M = m, L = l;
+      bool has0, has1;
+      if (two) {
+        has0 = g == 0 && !(m == -INFINITY && l == 0.f);
+        has1 = g == 1 && !(m == -INFINITY && l == 0.f);
+        w0 = w1 = 1.f;
+      } else {
+        M = fmaxf(ml0.x, ml1.x);
+        const float mb = M == -INFINITY ? 0.f : M;
+        has0 = !(ml0.x == -INFINITY && ml0.y == 0.f);
+        has1 = steps > 1 && !(ml1.x == -INFINITY && ml1.y == 0.f);
+        L = 0.f;
+        if (has0) L += (w0 = ex2(ml0.x - mb)) * ml0.y;
+        if (has1) L += (w1 = ex2(ml1.x - mb)) * ml1.y;
+      }
+      const bool whole = w.t0 == 0 && w.t1 == w.tiles;
+      const float inv = whole ? (L != 0.f ? 1.f / L : 0.f) : 1.f;
+      float* slot = slot_o(a, blockIdx.x, w.t0 == 0);
+      if (work) {
+        const int c0 = two ? 0 : 4 * g, c1 = two ? 8 : 4 * g + 4;  // chunks of 16 dims
+        const bool r0 = !two || g == 0, r1 = two ? g == 1 : steps > 1;  // uniform
+        if (!has0) w0 = 0.f;
+        if (!has1) w1 = 0.f;
+        __nv_bfloat16* op = static_cast<__nv_bfloat16*>(a.t.out) + ((int64_t)(qrow + node) * a.t.nq + head) * AD;
+        float* po = slot + (int64_t)row * AD;
+#pragma unroll 1
+        for (int c = c0; c < c1; ++c) {
+          uint32_t x0[16], x1[16], v[8];
+          if (r0) tc::tmem_ld(o_tm + 16 * c, x0);
+          if (r1) tc::tmem_ld(o_tm + 128 + 16 * c, x1);
+          float o[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) o[i] = 0.f;
+          if (r0) {
+            tc::ld_wait(x0);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[i] = has0 ? w0 * __uint_as_float(x0[i]) : 0.f;
+          }
+          if (r1) {
+            tc::ld_wait(x1);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[i] += has1 ? w1 * __uint_as_float(x1[i]) : 0.f;
+          }
+          if (!live) continue;
+          if (whole) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = L == 0.f ? 0u : pack_bf16(o[2 * i] * inv, o[2 * i + 1] * inv);
+            st32(op + 16 * c, v);
           } else {
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-              const uint32_t off = half * (KT * 128) + r * 128;
-              tc::tma_load_2d(smem_u32(kd + off), &kmap, bar, half * 64, row);
-              tc::tma_load_2d(smem_u32(vd + off), &vmap, bar, half * 64, row);
+            for (int k = 0; k < 16; k += 8) {
+#pragma unroll
+              for (int i = 0; i < 8; ++i) v[i] = __float_as_uint(o[k + i]);
+              st32(po + 16 * c + k, v);
             }
           }
         }
+        if (any && live && k_len > 0) {
+          if (whole)
+            add_bad<FP8>(a, w, sh.bad[items & 1], node, 16 * c0, 16 * (c1 - c0), op + 16 * c0);
+          else
+            add_bad<FP8>(a, w, sh.bad[items & 1], node, 16 * c0, 16 * (c1 - c0), po + 16 * c0);
+        }
+        if (!whole && live && (two || g == 0))
+          *reinterpret_cast<float2*>(slot + (int64_t)a.rows_cap * AD + row * 2) = make_float2(M, L);
+      }
+      tc::fence_before();
+      asm volatile("bar.sync 1, 256;" ::: "memory");  // ml and bad have been read
+      if (lane == 0) tc::mbar_arrive_release(bar(sh.o_empty));
+      tile0 += n;
+    }
+    tc::fence_before();
+  } else if (warp < W_CONV) {
+    if constexpr (FP8) regs_dec<56>();
+    if (warp == W_TMA) {
+      // ---------------------------------------------------------------- TMA producer
+      if (lane == 0) {
+        tc::prefetch_map(&kmap);
+        tc::prefetch_map(&vmap);
+      }
+      const int depth = FP8 ? RS : S;
+      Place at;
+      int c = 0;  // tiles so far (K and V in turn)
+      bool ok = true;
+      for (Walk w(a, sh.spot); w.more() && ok; w.next(a)) {
+        const int* bt = a.t.block_tables + w.b * a.t.bt_stride;
+        for (int t = w.t0; t < w.t1 && ok; ++t) {
+          // one lane per box
+          int row = a.oob_row;
+          const int r = lane << (a.bs_shift < 7 ? a.bs_shift : 7);
+          if (r < KT) {
+            const int tok = t * KT + r, bi = tok >> a.bs_shift;
+            if (bi < a.t.W) {
+              const int blk = bt[bi];
+              if (blk >= 0 && blk < a.t.num_blocks) row = ((blk * a.t.nkv + w.h) << a.bs_shift) + (tok & (a.t.block_size - 1));
+            }
+          }
+          for (int kv = 0; kv < 2 && ok; ++kv, ++c) {
+            if (!wait(FP8 ? sh.raw_empty[at.s] : sh.empty[at.s], at.ph ^ 1, 1)) {
+              ok = false;
+              break;
+            }
+            const uint32_t full = bar(FP8 ? sh.raw_full[at.s] : sh.full[at.s]);
+            const uint32_t dst = FP8 ? smem_u32(rawr + at.s * RAW_TILE) : smem_u32(ring + at.s * TILE);
+            const CUtensorMap* map = kv ? &vmap : &kmap;
+            if (lane == 0) tc::mbar_arrive_expect_tx(full, FP8 ? RAW_TILE : TILE);
+            __syncwarp();
+            if (r < KT) {
+              tc::tma_load_2d(dst + r * 128, map, full, 0, row);
+              if (!FP8) tc::tma_load_2d(dst + HALF + r * 128, map, full, 64, row);
+            }
+            at.step(1, depth);
+          }
+        }
+      }
+      if (*gave_up)  // copies that nobody waited for may still be landing
+        for (int k = max(0, c - depth); k < c; ++k)
+          tc::mbar_drain(bar(FP8 ? sh.raw_full[k % depth] : sh.full[k % depth]), (k / depth) & 1);
+    } else if (warp >= W_MMA) {
+      // ---------------------------------------------------------------- MMA issuers, one per group
+      const int g = warp - W_MMA;
+      constexpr uint32_t id_qk = tc::idesc_bf16(128, 128, false), id_pv = tc::idesc_bf16(128, 128, true);
+      const uint32_t s_tm = tmem + g * 128u, o_tm = tmem + 256u + g * 128u;
+      const uint64_t ring_k = tc::sdesc(smem_u32(ring)), ring_v = tc::sdesc_mn(smem_u32(ring), HALF), q0 = tc::sdesc(smem_u32(sq));
+      bool ok = true;
+      uint32_t done = 0;  // steps so far
+      int items = 0;
+      Place begin;  // of the item's first K
+      for (Walk w(a, sh.spot); w.more() && ok; w.next(a), ++items) {
+        const int n = w.t1 - w.t0, two = w.rows(a) > 128;
+        const int mine = two ? n : (n + 1 - g) >> 1, by = two ? 2 : 4;  // this group's steps; their distance in the ring
+        const uint64_t qd = q0 + (two ? g * (TILE >> 4) : 0);
+        Place k_at = begin, v_at;
+        if (!two && g) k_at.step(2, S);
+        v_at = k_at;
+        v_at.step(1, S);
+        ok = wait(sh.q_full, items & 1, 2);
+        for (int i = 0; i <= mine && ok; ++i) {
+          if (i > 0) {  // P V of the step before
+            ok = wait(sh.p_ready[g], (done - 1) & 1, 3) && wait(sh.full[v_at.s], v_at.ph, 4) &&
+                 // the outputs of the item before have been read
+                 (i > 1 || items == 0 || wait(sh.o_empty, (items - 1) & 1, 5));
+            if (!ok) break;
+            tc::fence_after();
+            if (elect_one()) {
+              const uint64_t vd = ring_v + (uint64_t)v_at.s * (TILE >> 4);
+#pragma unroll
+              for (int k = 0; k < 8; ++k)  // 16 keys: packed columns 8 k of P, rows 16 k of V
+                tc::mma_bf16_ts(o_tm, s_tm + 8 * k, vd + k * (16 * 128 >> 4), id_pv, i > 1 || k > 0);
+              tc::commit<1>(bar(sh.o_done[g]));
+              tc::commit<1>(bar(sh.empty[v_at.s]));
+              if (!two) tc::commit<1>(bar(sh.empty[v_at.s]));
+            }
+            __syncwarp();
+            v_at.step(by, S);
+          }
+          if (i < mine) {
+            ok = wait(sh.full[k_at.s], k_at.ph, 6) &&
+                 (done == 0 || wait(sh.o_done[g], (done - 1) & 1, 7));  // S overwrites the P of this group's last step
+            if (!ok) break;
+            if (elect_one()) {
+              const uint64_t kd = ring_k + (uint64_t)k_at.s * (TILE >> 4);
+#pragma unroll
+              for (int k = 0; k < 8; ++k) {
+                const uint32_t at = ((k >> 2) * HALF + (k & 3) * 32) >> 4;
+                tc::mma_bf16_ss(s_tm, qd + at, kd + at, id_qk, k > 0);
+              }
+              tc::commit<1>(bar(sh.s_full[g]));
+              tc::commit<1>(bar(sh.empty[k_at.s]));
+              if (!two) tc::commit<1>(bar(sh.empty[k_at.s]));
+            }
+            __syncwarp();
+            k_at.step(by, S);
+            ++done;
+          }
+          if (i == mine - 1 || mine == 0) {  // Q has been read
+            if (elect_one()) tc::commit<1>(bar(sh.q_empty));
+            __syncwarp();
+          }
+        }
+        const int on = begin.s + 2 * n;
+        begin.ph ^= (uint32_t)(on / S) & 1;
+        begin.s = on % S;
+      }
+      if (elect_one()) tc::commit<1>(bar(sh.drain[g]));  // every MMA of this thread
+      __syncwarp();
+      if (lane == 0) tc::mbar_drain(bar(sh.drain[g]), 0);
+      __syncwarp();
+    } else {
+      static_assert(W_Q == W_TMA + 1 && W_MMA == W_Q + 1, "");
+      // ---------------------------------------------------------------- Q
+      int items = 0;
+      for (Walk w(a, sh.spot); w.more(); w.next(a), ++items) {
+        if (items > 0) wait(sh.q_empty, (items - 1) & 1, 14);  // the products of the item before have read theirs
+        const int rows = w.rows(a), R0 = w.rt * a.rows_cap;
+        const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(a.t.q) + (int64_t)seq_begin(a.t, w.b) * a.t.q_stride + (int64_t)w.h * a.G * AD;
+        for (int i = lane; i < rows * 16; i += 32) {
+          const int r = i >> 4, c = i & 15, R = R0 + r;
+          const __nv_bfloat16* src = q + (int64_t)(R / a.G) * a.t.q_stride + (R % a.G) * AD + c * 8;
+          const uint32_t dst = smem_u32(sq + (r >> 7) * TILE) + tile_at(r & 127, c);
+          if (a.q16) {
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst + 4 * e), "l"(src + 2 * e) : "memory");
+          }
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        tc::fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive_release(bar(sh.q_full));
       }
     }
-    // Do not leave while copies of this thread may still be landing.
-    for (int j = max(0, i - DEPTH); j < i; ++j)
-      tc::mbar_drain(FP8 ? raw_full(j % DEPTH) : full(j % DEPTH), (j / DEPTH) & 1);
-    return;
-  }
-
-  if constexpr (FP8) {
-    if (warp > NWARP) {
-      // ------------------------------------------------------------ e4m3 -> f16 tiles
-      const int tid = threadIdx.x - (NWARP + 1) * 32;
-      int i = 0;
-      for (Walk w(a, spot); w.more(); w.next(a)) {
-        if (w.rows(a, rt, ROWS) <= 0) continue;
-        const int* bt = a.t.block_tables + w.b * a.t.bt_stride;
-        const int k_len = a.t.ctx_lens[w.b];
-        for (int t = w.t0; t < w.t1; ++t, ++i) {
-          const int s = i % C::RAW, d = i % C::RING;
+  } else if constexpr (FP8) {
+    // ------------------------------------------------------------------ e4m3 -> bf16 tiles
+    regs_dec<104>();
+    const int tid = threadIdx.x - W_CONV * 32;
+    Place from, to;
+    int tile = 0;
+    for (Walk w(a, sh.spot); w.more(); w.next(a)) {
+      const int* bt = a.t.block_tables + w.b * a.t.bt_stride;
+      for (int t = w.t0; t < w.t1; ++t, ++tile)
+        for (int kv = 0; kv < 2; ++kv) {
           float2 sc = make_float2(0.f, 0.f);
-          if (tid < KT / 16) {
+          if (kv == 0 && tid < KT / 16) {
             const int bi = (t * KT + tid * 16) >> a.bs_shift;
             const int blk = bi < a.t.W ? bt[bi] : -1;
             if (blk >= 0 && blk < a.t.num_blocks) {
@@ -340,338 +828,602 @@ __global__ void __launch_bounds__(Cfg<FP8>::THREADS, 1)
               sc = make_float2(a.t.k_scale[at], a.t.v_scale[at]);
             }
           }
-          wait(raw_full(s), (i / C::RAW) & 1, 2);
-          wait(empty(d), ((i / C::RING) & 1) ^ 1, 3);
-          if (tid < KT / 16) unit_scale[d][tid] = sc;
-          const uint8_t* src = rawr + s * C::RAW_STAGE;
-          uint8_t* dst = ring + d * C::STAGE;
-#pragma unroll
-          for (int u = 0; u < 8; ++u) {
-            const int idx = tid + (u & 3) * 128, r = idx >> 3, c = idx & 7;  // 16 values of row r
-            uint4 x = *reinterpret_cast<const uint4*>(src + (u >> 2) * KT * AD + idx * 16);
-            // positions behind the context may hold any bytes, a NaN included
-            if (t * KT + r >= k_len) x = make_uint4(0, 0, 0, 0);
-            const uint32_t in[4] = {x.x, x.y, x.z, x.w};
-            uint32_t h[8];
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              asm("{\n .reg .b16 l, h;\n mov.b32 {l, h}, %2;\n cvt.rn.f16x2.e4m3x2 %0, l;\n cvt.rn.f16x2.e4m3x2 %1, h;\n}"
-                  : "=r"(h[2 * e]), "=r"(h[2 * e + 1])
-                  : "r"(in[e]));
-            uint8_t* to = dst + (u >> 2) * C::KV_BYTES;
-            *reinterpret_cast<uint4*>(to + tile_at(r, 2 * c)) = make_uint4(h[0], h[1], h[2], h[3]);
-            *reinterpret_cast<uint4*>(to + tile_at(r, 2 * c + 1)) = make_uint4(h[4], h[5], h[6], h[7]);
+          wait(sh.raw_full[from.s], from.ph, 15);
+          wait(sh.empty[to.s], to.ph ^ 1, 16);
+          if (kv == 0 && tid < 32) {
+            if (tid < KT / 16) sh.scale[tile & 3][tid] = sc;
+            __syncwarp();
+            if (tid == 0) tc::mbar_arrive_release(bar(sh.scale_full[tile & 3]));
           }
-          tc::mbar_arrive_release(full(d));
+          convert_tile(rawr + from.s * RAW_TILE, ring + to.s * TILE, tid);
+          tc::fence_proxy_async();
           __syncwarp();
-          if (lane == 0) tc::mbar_arrive_release(raw_empty(s));
+          if (lane == 0) {
+            tc::mbar_arrive_release(bar(sh.full[to.s]));
+            tc::mbar_arrive_release(bar(sh.raw_empty[from.s]));
+          }
+          from.step(1, RS);
+          to.step(1, S);
         }
-      }
-      return;
     }
   }
+  __syncthreads();
+  if (warp == W_MMA) {
+    tc::fence_after();
+    tc::tmem_dealloc<1>(tmem, 512);
+  }
+}
 
-  // -------------------------------------------------------------------- working warps
-  const int rg = warp % RG, kg = warp / RG % KG, tg = warp / (RG * KG);
-  const int key0 = kg * KW;  // this warp's keys in a tile
-  const int c2 = (lane & 3) * 2;
-  int i = 0;  // tiles so far
-  for (Walk w(a, spot); w.more(); w.next(a)) {
-    const int rows = w.rows(a, rt, ROWS);
-    if (rows <= 0) continue;
-    const int qrow = seq_begin(a.t, w.b), n_nodes = seq_nodes(a.t, w.b), k_len = a.t.ctx_lens[w.b];
-    const int base = k_len - n_nodes;
-    const int rr[2] = {rg * 16 + (lane >> 2), rg * 16 + (lane >> 2) + 8};  // this thread's rows in the tile
-    int node[2];
-    uint32_t qf[8][4];
-    float qmul[2];
+// ------------------------------------------------------------------ kernel for few rows
+// Up to 64 rows: keys on the products' M side, so that nothing is computed for rows that are not there.
+//   S^T = K Q^T     [128 keys x N rows], two buffers in TMEM
+//   P^T             one key per thread, N weights, as bf16 into shared memory (two buffers)
+//   O^T += V^T P^T  [128 dims x N rows] in TMEM, two buffers, one per item in turn
+// A row's maximum and sum run over threads: the maximum is taken from the first tile and raised only when a score
+// passes it by 2^8 (one vote per tile), the sums are kept per thread and added up at the item's end.
+struct Few {  // shared memory besides the tiles
+  uint64_t full[8], empty[8], raw_full[8], raw_empty[8];
+  uint64_t q_full[2], q_empty[2], s_full[2], p_ready[2], o_done[2], o_empty[2], scale_full[4], drain;
+  alignas(16) float mrow[64];  // maxima (units of log2); read four at a time
+  alignas(16) float inv[64];   // 1 / sums
+  alignas(16) float red[4][64];
+  float2 scale[4][KT / 16];
+  uint32_t bad[2][BAD_WORDS];
+  int64_t part[16];
+  Spot spot;
+  uint32_t tmem;
+  int gave_up;
+};
+
+__host__ __device__ constexpr int few_bytes(int n, int slots, int raw_slots) {
+  return 2 * n * 256 + 2 * HALF + slots * TILE + raw_slots * RAW_TILE + (int)sizeof(Few);
+}
+
+__device__ __forceinline__ bool vote_any(bool p) {  // over the 128 softmax threads
+  uint32_t r;
+  asm volatile(
+      "{\n .reg .pred p, q;\n setp.ne.b32 p, %1, 0;\n barrier.cta.red.or.pred q, 1, 128, p;\n selp.b32 %0, 1, 0, q;\n}\n"
+      : "=r"(r)
+      : "r"((int)p)
+      : "memory");
+  return r != 0;
+}
+// (a, b) * f - (c, d)
+__device__ __forceinline__ float2 fms2(uint32_t a, uint32_t b, float f, float c, float d) {
+  float2 r;
+  asm("{\n .reg .b64 x, y, z;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %4};\n mov.b64 z, {%5, %6};\n"
+      " fma.rn.f32x2 z, x, y, z;\n mov.b64 {%0, %1}, z;\n}\n"
+      : "=f"(r.x), "=f"(r.y)
+      : "r"(a), "r"(b), "f"(f), "f"(-c), "f"(-d));
+  return r;
+}
+
+template <bool FP8, int N>
+__global__ void __launch_bounds__(FP8 ? 384 : 256, 1)
+    tree_attn_few_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, Args a) {
+  pdl_wait();     // inputs come from the previous kernel in the stream
+  pdl_trigger();  // the next kernel may start its prologue
+  extern __shared__ __align__(1024) uint8_t sm[];
+  constexpr int QT = N * 256, QHALF = N * 128;
+  constexpr int F_TMA = 4, F_Q = 5, F_MMA = 6, F_CONV = 8;  // first warp of each role; 0-3: softmax
+  const int S = a.slots, RS = a.raw_slots;
+  uint8_t* ring = sm;
+  uint8_t* pbuf = ring + S * TILE;
+  uint8_t* rawr = pbuf + 2 * HALF;
+  uint8_t* sq = rawr + RS * RAW_TILE;
+  Few& sh = *reinterpret_cast<Few*>(sq + 2 * QT);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  auto bar = [](uint64_t& b) { return smem_u32(&b); };
+  if (smem_u32(sm) & 1023) {  // the swizzle goes by the address
+    if (threadIdx.x == 0) atomicCAS(&g_tree_error, 0, 9);
+    return;
+  }
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < 8; ++s) {
+      tc::mbar_init(bar(sh.full[s]), FP8 ? 4 : 1);
+      tc::mbar_init(bar(sh.empty[s]), 1);
+      tc::mbar_init(bar(sh.raw_full[s]), 1);
+      tc::mbar_init(bar(sh.raw_empty[s]), 4);
+    }
+    for (int k = 0; k < 2; ++k) {
+      tc::mbar_init(bar(sh.q_full[k]), 1);
+      tc::mbar_init(bar(sh.q_empty[k]), 1);
+      tc::mbar_init(bar(sh.s_full[k]), 1);
+      tc::mbar_init(bar(sh.p_ready[k]), 4);
+      tc::mbar_init(bar(sh.o_done[k]), 1);
+      tc::mbar_init(bar(sh.o_empty[k]), 4);
+    }
+    for (int k = 0; k < 4; ++k) tc::mbar_init(bar(sh.scale_full[k]), 1);
+    tc::mbar_init(bar(sh.drain), 1);
+    sh.gave_up = 0;
+    tc::fence_barrier_init();
+  }
+  if (threadIdx.x < 2 * BAD_WORDS) sh.bad[threadIdx.x / BAD_WORDS][threadIdx.x % BAD_WORDS] = 0;
+  if (warp == F_MMA) tc::tmem_alloc<1>(smem_u32(&sh.tmem), 256);
+  tc::fence_before();
+  find_chunk(a, blockIdx.x, &sh.spot, sh.part);  // ends with a barrier
+  tc::fence_after();
+  const uint32_t tmem = sh.tmem;  // S^T at 0 and 64, O^T at 128 and 192
+  volatile int* gave_up = &sh.gave_up;
+  auto wait = [&](uint64_t& b, uint32_t parity, int code) { return warp_wait(bar(b), parity, &sh.gave_up, code); };
+
+  if (warp < F_TMA) {
+    // ------------------------------------------------------------------ softmax, outputs
+    const int kq = threadIdx.x;  // TMEM lane: a key of the tile, a dim of the outputs
+    const uint32_t lanes = (uint32_t)(warp * 32) << 16;
+    uint32_t cnt = 0;  // tiles so far
+    int items = 0;
+    for (Walk w(a, sh.spot); w.more(); w.next(a), ++items) {
+      const int rows = w.rows(a);  // all of the tree's
+      const int qrow = seq_begin(a.t, w.b), nodes = seq_nodes(a.t, w.b), k_len = a.t.ctx_lens[w.b], base = k_len - nodes;
+      float l[N];
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const bool live = rr[e] < rows;
-      const int r = rt * ROWS + (live ? rr[e] : 0);
-      node[e] = r / a.G;
-      const uint32_t* qp = reinterpret_cast<const uint32_t*>(
-          static_cast<const __nv_bfloat16*>(a.t.q) + (int64_t)(qrow + node[e]) * a.t.q_stride + (w.h * a.G + r % a.G) * AD);
-#pragma unroll
-      for (int kk = 0; kk < 8; ++kk) {
-        qf[kk][e] = live ? qp[kk * 8 + (lane & 3)] : 0u;
-        qf[kk][2 + e] = live ? qp[kk * 8 + (lane & 3) + 4] : 0u;
-      }
-      qmul[e] = a.scale_log2;
-      if constexpr (FP8) {
-        // f16 holds 11 bits, but not bf16's range: the row by a power of two that brings it below 256
-        float m = 0.f;
-#pragma unroll
-        for (int kk = 0; kk < 8; ++kk) {
-          const float2 x = unpack<false>(qf[kk][e]), y = unpack<false>(qf[kk][2 + e]);
-          m = fmaxf(m, fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(y.x), fabsf(y.y))));
+      for (int i = 0; i < N; ++i) l[i] = 0.f;
+      for (int t = w.t0; t < w.t1; ++t, ++cnt) {
+        const int buf = cnt & 1, pos = t * KT + kq;
+        const bool masked = t * KT + KT > base;
+        uint64_t see = ~0ull;  // rows that see this thread's key
+        if (masked) {
+          see = pos < base ? ~0ull : 0ull;
+          const int nd = pos - base;
+          if (pos >= base && pos < k_len && nd >= 0 && (nd >> 6) < a.t.words) {
+            const int64_t* mw = a.t.mask + (int64_t)qrow * a.t.mask_stride + (nd >> 6);
+            const uint64_t ones = a.G >= 64 ? ~0ull : (1ull << a.G) - 1;
+#pragma unroll 4
+            for (int r = 0; r < rows; r += a.G, mw += a.t.mask_stride) see |= (*mw >> (nd & 63) & 1) ? ones << r : 0ull;
+          }
         }
-        m = fmaxf(m, __shfl_xor_sync(FULL_MASK, m, 1));
-        m = fmaxf(m, __shfl_xor_sync(FULL_MASK, m, 2));
-        const int ex = (int)(__float_as_uint(m) >> 23) - 127;  // m < 2^(ex + 1)
-        const int by = m > 0.f && ex < 128 ? max(-126, min(126, 7 - ex)) : 0;
-        const float f = __int_as_float((127 + by) << 23);
-        qmul[e] *= __int_as_float((127 - by) << 23);
+        wait(sh.s_full[buf], (cnt >> 1) & 1, 8);
+        tc::fence_after();
+        float f = a.scale_log2, vs = 1.f;
+        if constexpr (FP8) {
+          wait(sh.scale_full[cnt & 3], (cnt >> 2) & 1, 10);
+          const float2 sc = sh.scale[cnt & 3][kq >> 4];
+          f *= sc.x;
+          vs = sc.y;
+        }
+        const uint32_t s_tm = tmem + 64u * buf + lanes;
+        auto seen = [&](int r) { return (uint32_t)(see >> (r & 32)) >> (r & 31) & 1; };
+        // this key's scores, kept in registers where there are enough (e4m3 with 64 rows: read again each time)
+        constexpr bool KEEP = !(FP8 && N == 64);
+        uint32_t x[KEEP ? N / 16 : 2][16];
+        if constexpr (KEEP) {
 #pragma unroll
-        for (int kk = 0; kk < 8; ++kk) {
-          const float2 x = unpack<false>(qf[kk][e]), y = unpack<false>(qf[kk][2 + e]);
-          qf[kk][e] = pack<true>(x.x * f, x.y * f);
-          qf[kk][2 + e] = pack<true>(y.x * f, y.y * f);
+          for (int c = 0; c < N / 16; ++c) tc::tmem_ld(s_tm + 16 * c, x[c]);
+#pragma unroll
+          for (int c = 0; c < N / 16; ++c) tc::ld_wait(x[c]);
+        }
+        auto columns = [&](auto&& fn) {
+          if constexpr (KEEP) {
+#pragma unroll
+            for (int c = 0; c < N / 16; ++c) fn(c, x[c]);
+          } else {
+            tc::tmem_ld(s_tm, x[0]);
+#pragma unroll
+            for (int c = 0; c < N / 16; ++c) {
+              tc::ld_wait(x[c & 1]);
+              if (c + 1 < N / 16) tc::tmem_ld(s_tm + 16 * (c + 1), x[(c + 1) & 1]);
+              fn(c, x[c & 1]);
+            }
+          }
+        };
+        const float4* mr = reinterpret_cast<const float4*>(sh.mrow);
+        bool raise = true;
+        if (t > w.t0) {
+          float mx[2] = {-INFINITY, -INFINITY};
+          columns([&](int c, uint32_t(&v)[16]) {
+#pragma unroll
+            for (int i = 0; i < 16; i += 4) {
+              const float4 m = mr[4 * c + (i >> 2)];
+              float2 y0 = fms2(v[i], v[i + 1], f, m.x, m.y), y1 = fms2(v[i + 2], v[i + 3], f, m.z, m.w);
+              if (masked) {
+                if (!seen(16 * c + i)) y0.x = -INFINITY;
+                if (!seen(16 * c + i + 1)) y0.y = -INFINITY;
+                if (!seen(16 * c + i + 2)) y1.x = -INFINITY;
+                if (!seen(16 * c + i + 3)) y1.y = -INFINITY;
+              }
+              mx[0] = fmaxf(mx[0], fmaxf(y0.x, y0.y));
+              mx[1] = fmaxf(mx[1], fmaxf(y1.x, y1.y));
+            }
+          });
+          raise = vote_any(fmaxf(mx[0], mx[1]) > RAISE);
+        }
+        if (raise) {
+          // every row's maximum over the tile: within the warp as ordered integers, then over the warps
+          columns([&](int c, uint32_t(&v)[16]) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              float y = fmaxf(__uint_as_float(v[i]) * f, -INFINITY);  // a NaN sets no maximum
+              if (!seen(16 * c + i)) y = -INFINITY;
+              const int o = __float_as_int(y) ^ ((__float_as_int(y) >> 31) & 0x7fffffff);
+              const int mo = __reduce_max_sync(FULL_MASK, o);
+              if (lane == i) sh.red[warp][16 * c + i] = __int_as_float(mo ^ ((mo >> 31) & 0x7fffffff));
+            }
+          });
+          asm volatile("bar.sync 1, 128;" ::: "memory");
+          if (kq < N) {
+            const float top = fmaxf(fmaxf(sh.red[0][kq], sh.red[1][kq]), fmaxf(sh.red[2][kq], sh.red[3][kq]));
+            // a row that has seen nothing yet has a maximum that any score passes
+            const float old = t > w.t0 ? sh.mrow[kq] : NOTHING, nm = fmaxf(old, top);
+            sh.mrow[kq] = nm;
+            sh.red[0][kq] = ex2(old - nm);  // what the sums so far are multiplied by
+          }
+          asm volatile("bar.sync 1, 128;" ::: "memory");
+          if (t > w.t0) {
+            wait(sh.o_done[(cnt - 1) & 1], ((cnt - 1) >> 1) & 1, 11);
+            tc::fence_after();
+            const uint32_t o_tm = tmem + 128u + 64u * (items & 1) + lanes;
+#pragma unroll
+            for (int c = 0; c < N / 16; ++c) {
+              uint32_t o[16];
+              tc::tmem_ld(o_tm + 16 * c, o);
+              tc::ld_wait(o);
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                const float g = sh.red[0][16 * c + i];
+                o[i] = g == 0.f ? 0u : __float_as_uint(__uint_as_float(o[i]) * g);
+                l[16 * c + i] = g == 0.f ? 0.f : l[16 * c + i] * g;
+              }
+              tc::tmem_st(o_tm + 16 * c, o);
+            }
+            tc::st_wait();
+          }
+          asm volatile("bar.sync 1, 128;" ::: "memory");  // red has been read
+        }
+        // weights: rounded to bf16 (2^-9 of each at most; e4m3: times V's scale), their sums taken as they were
+        uint32_t p[N / 2];
+        columns([&](int c, uint32_t(&v)[16]) {
+#pragma unroll
+          for (int i = 0; i < 16; i += 2) {
+            const float2 m = reinterpret_cast<const float2*>(sh.mrow)[8 * c + (i >> 1)];
+            float2 y = fms2(v[i], v[i + 1], f, m.x, m.y);
+            if (masked) {
+              if (!seen(16 * c + i)) y.x = -INFINITY;
+              if (!seen(16 * c + i + 1)) y.y = -INFINITY;
+            }
+            y = make_float2(ex2(y.x), ex2(y.y));
+            const float2 ls = add2(make_float2(l[16 * c + i], l[16 * c + i + 1]), y);
+            l[16 * c + i] = ls.x;
+            l[16 * c + i + 1] = ls.y;
+            p[8 * c + (i >> 1)] = FP8 ? pack_bf16(y.x * vs, y.y * vs) : pack_bf16(y.x, y.y);
+          }
+        });
+        if (cnt >= 2) wait(sh.o_done[buf], ((cnt >> 1) - 1) & 1, 17);  // the product that read this buffer
+        uint8_t* pb = pbuf + buf * HALF;
+#pragma unroll
+        for (int c = 0; c < N / 8; ++c)
+          *reinterpret_cast<uint4*>(pb + tile_at(kq, c)) = make_uint4(p[4 * c], p[4 * c + 1], p[4 * c + 2], p[4 * c + 3]);
+        if (masked) {
+          // positions behind the context hold any bits, and a node's infinities and NaN go to the rows that
+          // see it at the end
+          const int c = 2 * cnt + 1;
+          wait(sh.full[c % S], (c / S) & 1, 12);
+          uint8_t* v = ring + (c % S) * TILE;
+          if (pos >= base) {
+            bool odd = false;
+#pragma unroll 4
+            for (int i = 0; i < 16; ++i) {
+              uint4& q = *reinterpret_cast<uint4*>(v + tile_at(kq, i));
+              if (pos >= k_len) {
+                q = make_uint4(0, 0, 0, 0);
+                continue;
+              }
+              uint4 y = q;
+              const uint32_t o[4] = {odd_halves(y.x), odd_halves(y.y), odd_halves(y.z), odd_halves(y.w)};
+              if (o[0] | o[1] | o[2] | o[3]) {
+                odd = true;
+                y.x &= ~((o[0] >> 15) * 0xffffu);
+                y.y &= ~((o[1] >> 15) * 0xffffu);
+                y.z &= ~((o[2] >> 15) * 0xffffu);
+                y.w &= ~((o[3] >> 15) * 0xffffu);
+                q = y;
+              }
+            }
+            const int nd = pos - base;
+            if (odd && nd >= 0 && nd < TREE_MAX_NODES) atomicOr(&sh.bad[items & 1][nd >> 5], 1u << (nd & 31));
+          }
+        }
+        tc::fence_proxy_async();
+        tc::fence_before();
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive_release(bar(sh.p_ready[buf]));
+      }
+      // ---- sums over the threads: each exchange halves what a lane holds
+      int at = 0, held = N;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) {
+        if (held > 1) {
+          const bool up = lane & o;
+          held >>= 1;
+          at += up ? held : 0;
+#pragma unroll
+          for (int i = 0; i < N / 2; ++i)
+            if (i < held) {
+              const float keep = up ? l[i + held] : l[i], give = up ? l[i] : l[i + held];
+              l[i] = keep + __shfl_xor_sync(FULL_MASK, give, o);
+            }
+        } else {
+          l[0] += __shfl_xor_sync(FULL_MASK, l[0], o);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < (N > 32 ? N / 32 : 1); ++i) sh.red[warp][at + i] = l[i];
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+      const bool whole = w.t0 == 0 && w.t1 == w.tiles;
+      float* slot = slot_o(a, blockIdx.x, w.t0 == 0);
+      if (kq < N) {
+        const float L = (sh.red[0][kq] + sh.red[1][kq]) + (sh.red[2][kq] + sh.red[3][kq]);
+        sh.inv[kq] = !whole ? 1.f : L == 0.f ? 0.f : 1.f / L;
+        if (!whole && kq < rows)
+          *reinterpret_cast<float2*>(slot + (int64_t)a.rows_cap * AD + kq * 2) = make_float2(L == 0.f ? -INFINITY : sh.mrow[kq], L);
+      }
+      wait(sh.o_done[(cnt - 1) & 1], ((cnt - 1) >> 1) & 1, 13);
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+      tc::fence_after();
+      uint32_t any = 0;
+#pragma unroll
+      for (int i = 0; i < BAD_WORDS; ++i) any |= sh.bad[items & 1][i];
+      if (kq < BAD_WORDS) sh.bad[(items + 1) & 1][kq] = 0;
+      const uint32_t o_tm = tmem + 128u + 64u * (items & 1) + lanes;
+      {
+        // eight rows at a time: a warp writes 32 dims of each
+        __nv_bfloat16* op = static_cast<__nv_bfloat16*>(a.t.out) + ((int64_t)qrow * a.t.nq + w.h * a.G) * AD + kq;
+        float* po = slot + kq;
+        const int64_t jump = (int64_t)(a.t.nq - a.G) * AD;
+        int gh = 0;
+#pragma unroll 1
+        for (int r = 0; r < rows; r += 8) {
+          uint32_t o[8];
+          tc::tmem_ld(o_tm + r, o);
+          const float4 i0 = *reinterpret_cast<const float4*>(sh.inv + r), i1 = *reinterpret_cast<const float4*>(sh.inv + r + 4);
+          const float inv[8] = {i0.x, i0.y, i0.z, i0.w, i1.x, i1.y, i1.z, i1.w};
+          tc::ld_wait(o);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            if (r + i < rows) {
+              const float v = inv[i] == 0.f ? 0.f : __uint_as_float(o[i]) * inv[i];
+              if (whole)
+                *op = __float2bfloat16_rn(v);
+              else
+                *po = v;
+            }
+            po += AD;
+            op += AD;
+            if (++gh == a.G) {
+              gh = 0;
+              op += jump;
+            }
+          }
+        }
+        if (any && k_len > 0)
+          for (int r = 0; r < rows; ++r) {
+            if (whole)
+              add_bad<FP8>(a, w, sh.bad[items & 1], r / a.G, kq, 1,
+                           static_cast<__nv_bfloat16*>(a.t.out) + ((int64_t)(qrow + r / a.G) * a.t.nq + w.h * a.G + r % a.G) * AD + kq);
+            else
+              add_bad<FP8>(a, w, sh.bad[items & 1], r / a.G, kq, 1, slot + (int64_t)r * AD + kq);
+          }
+      }
+      tc::fence_before();
+      asm volatile("bar.sync 1, 128;" ::: "memory");  // mrow, inv, red and bad have been read
+      if (lane == 0) tc::mbar_arrive_release(bar(sh.o_empty[items & 1]));
+    }
+    tc::fence_before();
+  } else if (warp == F_TMA) {
+    // ------------------------------------------------------------------ TMA producer
+    if (lane == 0) {
+      tc::prefetch_map(&kmap);
+      tc::prefetch_map(&vmap);
+    }
+    const int depth = FP8 ? RS : S;
+    Place at;
+    int c = 0;  // tiles so far (K and V in turn)
+    bool ok = true;
+    for (Walk w(a, sh.spot); w.more() && ok; w.next(a)) {
+      const int* bt = a.t.block_tables + w.b * a.t.bt_stride;
+      for (int t = w.t0; t < w.t1 && ok; ++t) {
+        // one lane per box
+        int row = a.oob_row;
+        const int r = lane << (a.bs_shift < 7 ? a.bs_shift : 7);
+        if (r < KT) {
+          const int tok = t * KT + r, bi = tok >> a.bs_shift;
+          if (bi < a.t.W) {
+            const int blk = bt[bi];
+            if (blk >= 0 && blk < a.t.num_blocks) row = ((blk * a.t.nkv + w.h) << a.bs_shift) + (tok & (a.t.block_size - 1));
+          }
+        }
+        for (int kv = 0; kv < 2 && ok; ++kv, ++c) {
+          if (!wait(FP8 ? sh.raw_empty[at.s] : sh.empty[at.s], at.ph ^ 1, 1)) {
+            ok = false;
+            break;
+          }
+          const uint32_t full = bar(FP8 ? sh.raw_full[at.s] : sh.full[at.s]);
+          const uint32_t dst = FP8 ? smem_u32(rawr + at.s * RAW_TILE) : smem_u32(ring + at.s * TILE);
+          const CUtensorMap* map = kv ? &vmap : &kmap;
+          if (lane == 0) tc::mbar_arrive_expect_tx(full, FP8 ? RAW_TILE : TILE);
+          __syncwarp();
+          if (r < KT) {
+            tc::tma_load_2d(dst + r * 128, map, full, 0, row);
+            if (!FP8) tc::tma_load_2d(dst + HALF + r * 128, map, full, 64, row);
+          }
+          at.step(1, depth);
         }
       }
     }
-    float acc[16][4];
-#pragma unroll
-    for (int j = 0; j < 16; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-    float unit = 1.f;  // e4m3: V's scale that the sums are in units of
-
-    for (int t = w.t0; t < w.t1; ++t, ++i) {
-      if (TG > 1 && i % TG != tg) continue;
-      const int s = i % C::RING;
-      wait(full(s), (i / C::RING) & 1, 4);
-      const uint32_t kb = smem_u32(ring + s * C::STAGE), vb = kb + C::KV_BYTES;
-      if (rg * 16 < rows) {
-        float sc[NT][4];
-#pragma unroll
-        for (int j = 0; j < NT; ++j) sc[j][0] = sc[j][1] = sc[j][2] = sc[j][3] = 0.f;
-#pragma unroll
-        for (int kk = 0; kk < 8; ++kk)
-#pragma unroll
-          for (int np = 0; np < NT / 2; ++np) {
-            uint32_t kf[4];
-            const int r = key0 + np * 16 + (lane & 7) + ((lane >> 4) << 3), c = kk * 2 + ((lane >> 3) & 1);
-            ldsm4(kb + tile_at(r, c), kf);
-            mma<FP8>(sc[2 * np], qf[kk], kf[0], kf[1]);
-            mma<FP8>(sc[2 * np + 1], qf[kk], kf[2], kf[3]);
-          }
-        // scores in units of log2; keys that a row does not see: -inf
-        const bool masked = t * KT + KT > base;
-        uint64_t see[2] = {~0ull, ~0ull};
-        if (masked) {
-          const int d = base - t * KT;  // keys of this tile before the tree (below 0: nodes in earlier tiles)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int64_t* mw = a.t.mask + (int64_t)(qrow + node[e]) * a.t.mask_stride;
-            if (d > 0) {
-              see[e] = (1ull << d) - 1 | (uint64_t)mw[0] << d;
-            } else {
-              const int word = -d >> 6, sh = -d & 63;
-              const uint64_t lo = word < a.t.words ? (uint64_t)mw[word] : 0, hi = word + 1 < a.t.words ? (uint64_t)mw[word + 1] : 0;
-              see[e] = sh ? lo >> sh | hi << (64 - sh) : lo;
-            }
-            const int valid = k_len - t * KT;
-            if (valid < KT) see[e] &= valid > 0 ? (1ull << valid) - 1 : 0ull;
-            see[e] >>= key0;
-          }
+    if (*gave_up)  // copies that nobody waited for may still be landing
+      for (int k = max(0, c - depth); k < c; ++k)
+        tc::mbar_drain(bar(FP8 ? sh.raw_full[k % depth] : sh.full[k % depth]), (k / depth) & 1);
+  } else if (warp == F_Q) {
+    // ------------------------------------------------------------------ Q, two buffers
+    int items = 0;
+    for (Walk w(a, sh.spot); w.more(); w.next(a), ++items) {
+      const int qb = items & 1;
+      if (items > 1) wait(sh.q_empty[qb], ((items >> 1) - 1) & 1, 14);
+      const int rows = w.rows(a), c = lane & 15;
+      int r = lane >> 4, node = r / a.G, gh = r % a.G;
+      const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(a.t.q) + (int64_t)seq_begin(a.t, w.b) * a.t.q_stride + (int64_t)w.h * a.G * AD + c * 8;
+#pragma unroll 1
+      for (; r < N; r += 2) {
+        uint8_t* dst = sq + qb * QT + (c >> 3) * QHALF + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+        if (r >= rows) {  // no row: scores of 0
+          *reinterpret_cast<uint4*>(dst) = make_uint4(0, 0, 0, 0);
+          continue;
         }
-        float mx[2] = {-INFINITY, -INFINITY};
+        const __nv_bfloat16* src = q + (int64_t)node * a.t.q_stride + gh * AD;
+        for (gh += 2; gh >= a.G; gh -= a.G) ++node;
+        if (a.q16) {
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+        } else {
 #pragma unroll
-        for (int j = 0; j < NT; ++j)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float f = qmul[e >> 1];
-            if constexpr (FP8) f *= unit_scale[s][(key0 + j * 8) >> 4].x;
-            sc[j][e] *= f;
-            if (masked && !(see[e >> 1] >> (j * 8 + c2 + (e & 1)) & 1)) sc[j][e] = -INFINITY;
-            mx[e >> 1] = fmaxf(mx[e >> 1], sc[j][e]);
-          }
-        float al[2], bs[2];
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          mx[e] = fmaxf(mx[e], __shfl_xor_sync(FULL_MASK, mx[e], 1));
-          mx[e] = fmaxf(mx[e], __shfl_xor_sync(FULL_MASK, mx[e], 2));
-          mx[e] = fmaxf(mx[e], m[e]);
-          bs[e] = mx[e] == -INFINITY ? 0.f : mx[e];
-          al[e] = ex2(m[e] - bs[e]);
-          // f16: weights up to 2^15, so that those down to 2^-29 of the largest keep 11 bits; the sums share the factor
-          if constexpr (FP8) bs[e] -= 15.f;
-          m[e] = mx[e];
-          l[e] *= al[e];
+          for (int e = 0; e < 4; ++e)
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(dst) + 4 * e), "l"(src + 2 * e) : "memory");
         }
+      }
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      tc::fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive_release(bar(sh.q_full[qb]));
+    }
+  } else if (warp == F_MMA) {
+    // ------------------------------------------------------------------ MMA issuer
+    constexpr uint32_t id_s = tc::idesc_bf16(128, N, false), id_o = tc::idesc_bf16(128, N, true) | (1u << 15);
+    const uint64_t ring_k = tc::sdesc(smem_u32(ring)), ring_v = tc::sdesc_mn(smem_u32(ring), HALF);
+    const uint64_t p0 = tc::sdesc_mn(smem_u32(pbuf), HALF), q0 = tc::sdesc(smem_u32(sq));
+    bool ok = true;
+    uint32_t cnt = 0;
+    int items = 0;
+    Place at;  // of the next K
+    // the product with V that is still to come: its tile's number, V's place, the item
+    bool pending = false, p_first = false;
+    uint32_t p_cnt = 0;
+    int p_item = 0;
+    Place p_at;
+    auto product = [&]() {
+      const int buf = p_cnt & 1, ob = p_item & 1;
+      pending = false;
+      ok = wait(sh.p_ready[buf], (p_cnt >> 1) & 1, 3) && wait(sh.full[p_at.s], p_at.ph, 4) &&
+           // the outputs of the item before last have been read
+           (!p_first || p_item < 2 || wait(sh.o_empty[ob], ((p_item >> 1) - 1) & 1, 5));
+      if (!ok) return;
+      tc::fence_after();
+      if (elect_one()) {
+        const uint64_t vd = ring_v + (uint64_t)p_at.s * (TILE >> 4), pd = p0 + (uint64_t)buf * (HALF >> 4);
 #pragma unroll
-        for (int j = 0; j < NT; ++j)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            sc[j][e] = ex2(sc[j][e] - bs[e >> 1]);
-            l[e >> 1] += sc[j][e];
-          }
-#pragma unroll
-        for (int ks = 0; ks < KW / 16; ++ks) {  // 16 keys at a time
-          float f[2] = {1.f, 1.f};
-          if (ks == 0) {
-            f[0] = al[0];
-            f[1] = al[1];
-          }
-          bool gone = false;
-          if constexpr (FP8) {
-            const float vs = unit_scale[s][(key0 >> 4) + ks].y;
-            gone = vs == 0.f;  // no block, or one of zeros
-            if (!gone) {
-              f[0] *= unit / vs;
-              f[1] *= unit / vs;
-              unit = vs;
-            }
-          }
-          if (__any_sync(FULL_MASK, f[0] != 1.f || f[1] != 1.f)) {
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-              acc[j][0] *= f[0];
-              acc[j][1] *= f[0];
-              acc[j][2] *= f[1];
-              acc[j][3] *= f[1];
-            }
-          }
-          if (gone) continue;
-          // P is rounded to the type of V: 2^-9 (bf16) or 2^-12 (f16) of each weight at most; the sum l is not
-          const uint32_t pf[4] = {pack<FP8>(sc[2 * ks][0], sc[2 * ks][1]), pack<FP8>(sc[2 * ks][2], sc[2 * ks][3]),
-                                  pack<FP8>(sc[2 * ks + 1][0], sc[2 * ks + 1][1]),
-                                  pack<FP8>(sc[2 * ks + 1][2], sc[2 * ks + 1][3])};
-          uint32_t keep0 = ~0u, keep1 = ~0u, odd = 0;
-          if (masked) {
-            // positions behind the context hold any bits
-            const int k = t * KT + key0 + ks * 16 + c2;
-            keep0 = (k < k_len ? 0xffffu : 0u) | (k + 1 < k_len ? 0xffff0000u : 0u);
-            keep1 = (k + 8 < k_len ? 0xffffu : 0u) | (k + 9 < k_len ? 0xffff0000u : 0u);
-          }
-#pragma unroll
-          for (int np = 0; np < 8; ++np) {
-            uint32_t vf[4];
-            const int r = key0 + ks * 16 + (lane & 7) + ((lane >> 3) & 1) * 8, c = np * 2 + (lane >> 4);
-            ldsm4t(vb + tile_at(r, c), vf);
-            if (masked) {
-              vf[0] &= keep0;
-              vf[2] &= keep0;
-              vf[1] &= keep1;
-              vf[3] &= keep1;
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const uint32_t o = odd_halves<FP8>(vf[e]);
-                odd |= o;
-                vf[e] &= ~((o >> 15) * 0xffffu);  // to 0: added below where it is seen
-              }
-            }
-            mma<FP8>(acc[2 * np], pf, vf[0], vf[1]);
-            mma<FP8>(acc[2 * np + 1], pf, vf[2], vf[3]);
-          }
-          if (masked && __any_sync(FULL_MASK, odd != 0)) {
-            // infinities and NaN, for the rows that see them
-            for (int kx = 0; kx < 16; ++kx) {
-              const int key = key0 + ks * 16 + kx;
-              if (t * KT + key >= k_len) break;
-              const int from = (lane & 28) | ((kx & 7) >> 1);
-              float p[2];
-#pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                const float x0 = __shfl_sync(FULL_MASK, sc[2 * ks][2 * e], from), x1 = __shfl_sync(FULL_MASK, sc[2 * ks][2 * e + 1], from);
-                const float y0 = __shfl_sync(FULL_MASK, sc[2 * ks + 1][2 * e], from), y1 = __shfl_sync(FULL_MASK, sc[2 * ks + 1][2 * e + 1], from);
-                p[e] = kx < 8 ? (kx & 1 ? x1 : x0) : (kx & 1 ? y1 : y0);
-              }
-#pragma unroll
-              for (int j = 0; j < 16; ++j) {
-                uint32_t x;
-                asm volatile("ld.shared.b32 %0, [%1];" : "=r"(x) : "r"(vb + tile_at(key, j) + (lane & 3) * 4) : "memory");
-                const uint32_t o = odd_halves<FP8>(x);
-                const float2 v = unpack<FP8>(x);
-#pragma unroll
-                for (int e = 0; e < 2; ++e)
-                  if (see[e] >> (ks * 16 + kx) & 1) {
-                    if (o & 0x8000u) acc[j][2 * e] += p[e] * v.x;
-                    if (o & 0x80000000u) acc[j][2 * e + 1] += p[e] * v.y;
-                  }
-              }
-            }
-          }
-        }
+        for (int k = 0; k < 8; ++k)  // 16 keys
+          tc::mma_bf16_ss(tmem + 128u + 64u * ob, vd + k * (16 * 128 >> 4), pd + k * (16 * 128 >> 4), id_o, !p_first || k > 0);
+        tc::commit<1>(bar(sh.o_done[buf]));
+        tc::commit<1>(bar(sh.empty[p_at.s]));
       }
       __syncwarp();
-      if (lane == 0) tc::mbar_arrive_release(empty(s));
-    }
-
-    // ---- join the warps of each row group
+    };
+    for (Walk w(a, sh.spot); w.more() && ok; w.next(a), ++items) {
+      const int qb = items & 1;
+      for (int t = w.t0; t < w.t1 && ok; ++t, ++cnt) {
+        const int buf = cnt & 1;
+        // the last tile's product goes first unless this tile's keys are there already
+        int ready = 0;
+        if (lane == 0) ready = tc::mbar_try(bar(sh.full[at.s]), at.ph);
+        if (pending && !__shfl_sync(FULL_MASK, ready, 0)) product();
+        if (!ok) break;
+        if (t == w.t0) ok = wait(sh.q_full[qb], (items >> 1) & 1, 2);
+        ok = ok && wait(sh.full[at.s], at.ph, 6);
+        if (!ok) break;
+        if (cnt >= 2) tc::fence_after();  // the buffer's last reader has announced its weights
+        if constexpr (FP8) tc::fence_after();
+        if (elect_one()) {
+          const uint64_t kd = ring_k + (uint64_t)at.s * (TILE >> 4), qd = q0 + (uint64_t)qb * (QT >> 4);
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      l[e] += __shfl_xor_sync(FULL_MASK, l[e], 1);
-      l[e] += __shfl_xor_sync(FULL_MASK, l[e], 2);
-    }
-    // this warp's 16 x 128 outputs; columns are moved by the row so that a store's rows meet no bank twice
-    float* mo = merge_o + warp * 16 * AD;
-    const int r0 = lane >> 2;
-    if ((lane & 3) == 0) {
-      merge_ml[warp * 16 + r0] = make_float2(m[0], l[0]);
-      merge_ml[warp * 16 + r0 + 8] = make_float2(m[1], l[1]);
-    }
-#pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      const int c = (j * 8 + c2) ^ ((r0 & 3) << 3);
-      *reinterpret_cast<float2*>(mo + r0 * AD + c) = make_float2(acc[j][0] * unit, acc[j][1] * unit);
-      *reinterpret_cast<float2*>(mo + (r0 + 8) * AD + c) = make_float2(acc[j][2] * unit, acc[j][3] * unit);
-    }
-    asm volatile("bar.sync 1, %0;" ::"n"(NWARP * 32) : "memory");
-    const bool whole = w.t0 == 0 && w.t1 == w.tiles;
-    float* po = slot_o(a, ROWS, blockIdx.x, w.t0 == 0);
-    // a thread takes 4 columns of a row
-    for (int x = threadIdx.x; x < rows * (AD / 4); x += NWARP * 32) {
-      const int r = x / (AD / 4), c = x % (AD / 4) * 4, g = r >> 4, q = r & 15;
-      float M = -INFINITY;
-#pragma unroll
-      for (int k = 0; k < SH; ++k) M = fmaxf(M, merge_ml[(k * RG + g) * 16 + q].x);
-      const float mb = M == -INFINITY ? 0.f : M;
-      float L = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int k = 0; k < SH; ++k) {
-        const float2 ml = merge_ml[(k * RG + g) * 16 + q];
-        if (ml.x == -INFINITY && ml.y == 0.f) continue;  // saw nothing
-        const float f = ex2(ml.x - mb);
-        const float4 v = *reinterpret_cast<const float4*>(merge_o + ((k * RG + g) * 16 + q) * AD + (c ^ ((q & 3) << 3)));
-        L += f * ml.y;
-        o[0] += f * v.x;
-        o[1] += f * v.y;
-        o[2] += f * v.z;
-        o[3] += f * v.w;
-      }
-      if (whole) {
-        const float inv = L != 0.f ? 1.f / L : 0.f;
-        const int R = rt * ROWS + r;
-        __nv_bfloat16* op = static_cast<__nv_bfloat16*>(a.t.out) +
-                            ((int64_t)(qrow + R / a.G) * a.t.nq + w.h * a.G + R % a.G) * AD + c;
-        float v[4] = {o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};
-        if (L == 0.f) v[0] = v[1] = v[2] = v[3] = 0.f;
-        *reinterpret_cast<uint2*>(op) = f32_to_bf16x4(v);
-      } else {
-        *reinterpret_cast<float4*>(po + r * AD + c) = make_float4(o[0], o[1], o[2], o[3]);
-        if (c == 0) *reinterpret_cast<float2*>(po + ROWS * AD + r * 2) = make_float2(M, L);
+          for (int k = 0; k < 8; ++k)
+            tc::mma_bf16_ss(tmem + 64u * buf, kd + (((k >> 2) * HALF + (k & 3) * 32) >> 4), qd + (((k >> 2) * QHALF + (k & 3) * 32) >> 4), id_s, k > 0);
+          tc::commit<1>(bar(sh.s_full[buf]));
+          tc::commit<1>(bar(sh.empty[at.s]));
+          if (t == w.t1 - 1) tc::commit<1>(bar(sh.q_empty[qb]));
+        }
+        __syncwarp();
+        if (pending) product();
+        pending = true;
+        p_first = t == w.t0;
+        p_cnt = cnt;
+        p_item = items;
+        at.step(1, S);
+        p_at = at;
+        at.step(1, S);
       }
     }
-    asm volatile("bar.sync 1, %0;" ::"n"(NWARP * 32) : "memory");  // the outputs are read
+    if (ok && pending) product();
+    if (elect_one()) tc::commit<1>(bar(sh.drain));  // every MMA of this thread
+    __syncwarp();
+    if (lane == 0) tc::mbar_drain(bar(sh.drain), 0);
+    __syncwarp();
+  } else if (FP8 && warp >= F_CONV) {
+    // ------------------------------------------------------------------ e4m3 -> bf16 tiles
+    const int tid = threadIdx.x - F_CONV * 32;
+    Place from, to;
+    int tile = 0;
+    for (Walk w(a, sh.spot); w.more(); w.next(a)) {
+      const int* bt = a.t.block_tables + w.b * a.t.bt_stride;
+      for (int t = w.t0; t < w.t1; ++t, ++tile)
+        for (int kv = 0; kv < 2; ++kv) {
+          float2 sc = make_float2(0.f, 0.f);
+          if (kv == 0 && tid < KT / 16) {
+            const int bi = (t * KT + tid * 16) >> a.bs_shift;
+            const int blk = bi < a.t.W ? bt[bi] : -1;
+            if (blk >= 0 && blk < a.t.num_blocks) {
+              const int64_t k = (int64_t)blk * a.t.nkv + w.h;
+              sc = make_float2(a.t.k_scale[k], a.t.v_scale[k]);
+            }
+          }
+          wait(sh.raw_full[from.s], from.ph, 15);
+          wait(sh.empty[to.s], to.ph ^ 1, 16);
+          if (kv == 0 && tid < 32) {
+            if (tid < KT / 16) sh.scale[tile & 3][tid] = sc;
+            __syncwarp();
+            if (tid == 0) tc::mbar_arrive_release(bar(sh.scale_full[tile & 3]));
+          }
+          convert_tile(rawr + from.s * RAW_TILE, ring + to.s * TILE, tid);
+          tc::fence_proxy_async();
+          __syncwarp();
+          if (lane == 0) {
+            tc::mbar_arrive_release(bar(sh.full[to.s]));
+            tc::mbar_arrive_release(bar(sh.raw_empty[from.s]));
+          }
+          from.step(1, RS);
+          to.step(1, S);
+        }
+    }
+  }
+  __syncthreads();
+  if (warp == F_MMA) {
+    tc::fence_after();
+    tc::tmem_dealloc<1>(tmem, 256);
   }
 }
 
 // ---------------------------------------------------------------------------- joining
-// CTA (chunk, row tile, 16 rows) joins the pair that begins in its chunk and ends in a later one.
-__global__ void __launch_bounds__(128) tree_join_kernel(Args a, int ROWS) {
+// CTA (chunk, 4 rows) joins the item that begins in its chunk and ends in a later one.
+__global__ void __launch_bounds__(128) tree_join_kernel(Args a) {
   pdl_wait();     // the partial sums come from the previous kernel in the stream
   pdl_trigger();  // the next kernel may start its prologue
   __shared__ Spot spot;
-  const int rt = blockIdx.x % a.row_tiles, chunk = blockIdx.x / a.row_tiles;
-  find_chunk(a, chunk, &spot);
+  __shared__ int64_t part[4];
+  const int chunk = blockIdx.x;
+  find_chunk(a, chunk, &spot, part);
   const int64_t lo = spot.lo, hi = spot.hi;
   if (hi <= lo || hi >= spot.total) return;
-  const int b = spot.at_hi.b, tiles = seq_tiles(a.t, b);
-  const int h = (int)(spot.at_hi.rem / tiles), t = (int)(spot.at_hi.rem % tiles);
+  const int b = spot.hi_seq, tiles = seq_tiles(a.t, b), per = tiles * a.t.nkv;
+  const int rt = (int)(spot.hi_rem / per), r0 = (int)(spot.hi_rem % per), h = r0 / tiles, t = r0 % tiles;
   const int64_t begin = hi - t, end = begin + tiles;
-  if (t == 0 || begin < lo) return;  // nothing is cut here, or the pair begins in an earlier chunk
-  const int rows = min(ROWS, min(seq_nodes(a.t, b), a.t.max_nodes) * a.G - rt * ROWS);
-  const int qrow = seq_begin(a.t, b);
+  if (t == 0 || begin < lo) return;  // nothing is cut here, or the item begins in an earlier chunk
+  const int rows = min(a.rows_cap, seq_rows(a, b) - rt * a.rows_cap);
   const int r = blockIdx.y * 4 + (threadIdx.x >> 5), c = (threadIdx.x & 31) * 4;
   if (r >= rows) return;
   float M = -INFINITY, L = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
   int64_t from = lo, upto = hi;
   for (int k = chunk;; ++k) {
     if (upto > from) {  // with fewer tiles than chunks, some have none
-      const float* po = slot_o(a, ROWS, k * a.row_tiles + rt, k == chunk);
-      const float2 ml = *reinterpret_cast<const float2*>(po + ROWS * AD + r * 2);
-      const float4 v = *reinterpret_cast<const float4*>(po + r * AD + c);
+      const float* po = slot_o(a, k, k == chunk);
+      const float2 ml = *reinterpret_cast<const float2*>(po + (int64_t)a.rows_cap * AD + r * 2);
+      const float4 v = *reinterpret_cast<const float4*>(po + (int64_t)r * AD + c);
       if (!(ml.x == -INFINITY && ml.y == 0.f)) {
         const float nm = fmaxf(M, ml.x), nb = nm == -INFINITY ? 0.f : nm;
         const float f = L == 0.f && M == -INFINITY ? 0.f : ex2(M - nb), g = ex2(ml.x - nb);
@@ -690,9 +1442,10 @@ __global__ void __launch_bounds__(128) tree_join_kernel(Args a, int ROWS) {
   const float inv = L != 0.f ? 1.f / L : 0.f;
   float v[4] = {o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};
   if (L == 0.f) v[0] = v[1] = v[2] = v[3] = 0.f;
-  const int R = rt * ROWS + r;
+  const int R = rt * a.rows_cap + r;
   *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(a.t.out) +
-                            ((int64_t)(qrow + R / a.G) * a.t.nq + h * a.G + R % a.G) * AD + c) = f32_to_bf16x4(v);
+                            ((int64_t)(seq_begin(a.t, b) + R / a.G) * a.t.nq + h * a.G + R % a.G) * AD + c) =
+      f32_to_bf16x4(v);
 }
 
 PFN_cuTensorMapEncodeTiled_v12000 encoder() {
@@ -722,28 +1475,58 @@ bool pool_map(CUtensorMap* m, const void* base, int64_t rows, bool fp8, int box_
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <bool FP8, int RG>
-cudaError_t launch_main(const CUtensorMap& km, const CUtensorMap& vm, const Args& a, cudaStream_t stream) {
-  static std::atomic<uint64_t> done{0};
-  cudaError_t e = smem_opt_in(done, tree_attn_kernel<FP8, RG>, Cfg<FP8>::SMEM);
-  if (e != cudaSuccess) return e;
-  return launch_pdl(tree_attn_kernel<FP8, RG>, dim3(a.chunks * a.row_tiles), dim3(Cfg<FP8>::THREADS), Cfg<FP8>::SMEM,
-                    stream, km, vm, a);
-}
-
 }  // namespace
 
-// Row groups by the rows of the largest tree; one CTA per SM (shared memory allows one).
-TreeAttnPlan tree_attn_plan(int num_seqs, int max_nodes, int nq, int nkv, int num_sms) {
+// Rows per CTA by the largest tree: the kernel for few rows up to 64.  One CTA per SM (shared memory allows one).
+TreeAttnPlan tree_attn_plan(int max_nodes, int nq, int nkv, int num_sms) {
   TreeAttnPlan p;
   const int rows = max_nodes * (nq / nkv);
-  p.rg = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
-  p.row_tiles = (rows + p.rg * 16 - 1) / (p.rg * 16);
-  p.chunks = num_sms / p.row_tiles > 1 ? num_sms / p.row_tiles : 1;
-  p.ws_floats = 2LL * p.chunks * p.row_tiles * p.rg * 16 * (AD + 2);
-  (void)num_seqs;
+  p.rows_cap = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : rows <= 128 ? 128 : 256;
+  p.chunks = num_sms;
+  p.ws_floats = 2LL * p.chunks * p.rows_cap * (AD + 2);
   return p;
 }
+
+namespace {
+constexpr int SMEM_MOST = 232448;  // 227 KB
+
+template <typename K>
+cudaError_t launch_main(K kern, int threads, int smem, std::atomic<uint64_t>& done, const CUtensorMap& km,
+                        const CUtensorMap& vm, const Args& a, cudaStream_t stream) {
+  cudaError_t e = smem_opt_in(done, kern, SMEM_MOST);
+  if (e != cudaSuccess) return e;
+  return launch_pdl(kern, dim3(a.chunks), dim3(threads), smem, stream, km, vm, a);
+}
+
+template <bool FP8, int N>
+cudaError_t launch_few(const CUtensorMap& km, const CUtensorMap& vm, Args& a, cudaStream_t stream) {
+  static std::atomic<uint64_t> done{0};
+  // the rest of shared memory: K and V tiles (e4m3: three of them, and 8-bit ones)
+  const int left = SMEM_MOST - few_bytes(N, 0, 0);
+  a.slots = FP8 ? 3 : std::min(left / TILE, 8);
+  a.raw_slots = FP8 ? std::min((left - 3 * TILE) / RAW_TILE, 8) : 0;
+  return launch_main(tree_attn_few_kernel<FP8, N>, FP8 ? 384 : 256, few_bytes(N, a.slots, a.raw_slots), done, km, vm, a, stream);
+}
+
+template <bool FP8>
+cudaError_t launch_wide(const CUtensorMap& km, const CUtensorMap& vm, Args& a, cudaStream_t stream) {
+  static std::atomic<uint64_t> done{0};
+  const int qt = a.rows_cap / 128;
+  a.slots = FP8 ? 4 : 7 - qt;
+  a.raw_slots = FP8 ? (qt == 1 ? 4 : 2) : 0;
+  return launch_main(tree_attn_kernel<FP8>, FP8 ? 512 : 384, smem_bytes(qt, a.slots, a.raw_slots), done, km, vm, a, stream);
+}
+
+template <bool FP8>
+cudaError_t launch_rows(const CUtensorMap& km, const CUtensorMap& vm, Args& a, cudaStream_t stream) {
+  switch (a.rows_cap) {
+    case 16: return launch_few<FP8, 16>(km, vm, a, stream);
+    case 32: return launch_few<FP8, 32>(km, vm, a, stream);
+    case 64: return launch_few<FP8, 64>(km, vm, a, stream);
+    default: return launch_wide<FP8>(km, vm, a, stream);
+  }
+}
+}  // namespace
 
 cudaError_t launch_tree_attention(const TreeAttn& t, const TreeAttnPlan& p, cudaStream_t stream) {
   const int64_t rows = (int64_t)t.num_blocks * t.nkv * t.block_size;
@@ -753,24 +1536,20 @@ cudaError_t launch_tree_attention(const TreeAttn& t, const TreeAttnPlan& p, cuda
   Args a;
   a.t = t;
   a.G = t.nq / t.nkv;
-  a.row_tiles = p.row_tiles;
   a.chunks = p.chunks;
+  a.rows_cap = p.rows_cap;
+  a.slots = a.raw_slots = 0;
   a.bs_shift = __builtin_ctz((unsigned)t.block_size);
   a.box_rows = t.block_size < KT ? t.block_size : KT;
   a.oob_row = (int)rows;
+  a.q16 = t.q_stride % 8 == 0 && (reinterpret_cast<uintptr_t>(t.q) & 15) == 0;
   a.scale_log2 = t.softmax_scale * LOG2E;
   CUtensorMap km, vm;
   if (!pool_map(&km, t.k_cache, rows, t.kv_fp8, a.box_rows) || !pool_map(&vm, t.v_cache, rows, t.kv_fp8, a.box_rows))
     return cudaErrorInvalidValue;
-  cudaError_t e;
-  if (t.kv_fp8)
-    e = p.rg == 1 ? launch_main<true, 1>(km, vm, a, stream)
-                  : p.rg == 2 ? launch_main<true, 2>(km, vm, a, stream) : launch_main<true, 4>(km, vm, a, stream);
-  else
-    e = p.rg == 1 ? launch_main<false, 1>(km, vm, a, stream)
-                  : p.rg == 2 ? launch_main<false, 2>(km, vm, a, stream) : launch_main<false, 4>(km, vm, a, stream);
+  cudaError_t e = t.kv_fp8 ? launch_rows<true>(km, vm, a, stream) : launch_rows<false>(km, vm, a, stream);
   if (e != cudaSuccess) return e;
-  return launch_pdl(tree_join_kernel, dim3(a.chunks * a.row_tiles, p.rg * 4), dim3(128), 0, stream, a, p.rg * 16);
+  return launch_pdl(tree_join_kernel, dim3(a.chunks, a.rows_cap / 4), dim3(128), 0, stream, a);
 }
 
 int tree_attn_error_code(int reset) {

@@ -73,14 +73,6 @@ std::tuple<at::Tensor, at::Tensor> tree_mask(const at::Tensor& parents, const at
   return {mask, depth};
 }
 
-std::vector<int64_t> tree_attention_plan(int64_t num_seqs, int64_t max_nodes, int64_t nq, int64_t nkv, int64_t num_sms) {
-  TORCH_CHECK(num_seqs >= 0 && max_nodes >= 1 && max_nodes <= nvb::TREE_MAX_NODES && nkv > 0 && nq > 0 && nq % nkv == 0 &&
-                  nq <= 65536 && num_sms > 0 && num_sms < 4096,
-              "tree_attention_plan: up to ", nvb::TREE_MAX_NODES, " nodes, KV heads that divide the query heads, SMs");
-  const auto p = nvb::tree_attn_plan((int)num_seqs, (int)max_nodes, (int)nq, (int)nkv, (int)num_sms);
-  return {p.rg, p.row_tiles, p.chunks, p.ws_floats};
-}
-
 at::Tensor tree_attention(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache,
                           const Opt& k_scale, const Opt& v_scale, const at::Tensor& mask, const at::Tensor& block_tables,
                           const at::Tensor& cu_q, const at::Tensor& ctx_lens, int64_t num_seqs, int64_t max_nodes,
@@ -123,7 +115,7 @@ at::Tensor tree_attention(const at::Tensor& q, const at::Tensor& k_cache, const 
   at::Tensor out = new_cuda({T, nq * D}, at::kBFloat16, q);
   if (T == 0 || num_seqs == 0) return out;
   const int sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
-  const nvb::TreeAttnPlan p = nvb::tree_attn_plan((int)num_seqs, (int)max_nodes, (int)nq, (int)nkv, sms);
+  const nvb::TreeAttnPlan p = nvb::tree_attn_plan((int)max_nodes, (int)nq, (int)nkv, sms);
   at::Tensor ws = new_cuda({p.ws_floats}, at::kFloat, q);
   nvb::TreeAttn a{};
   a.q = q.data_ptr();
@@ -274,7 +266,6 @@ int64_t tree_error(bool reset) { return nvb::tree_attn_error_code(reset ? 1 : 0)
 void register_tree(pybind11::module& m) {
   m.def("tree_mask", &tree_mask);
   m.def("tree_attention", &tree_attention);
-  m.def("tree_attention_plan", &tree_attention_plan);
   m.def("tree_verify", &tree_verify);
   m.def("tree_commit", &tree_commit);
   m.def("tree_error", &tree_error, pybind11::arg("reset") = false);

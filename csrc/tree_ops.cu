@@ -173,13 +173,24 @@ __global__ void __launch_bounds__(CT) tree_commit_kernel(TreeCommit a) {
           // the block begins with this row: its scale, as the store of a first token sets it
 #pragma unroll
           for (int o = 4; o; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(group, amax, o, 8));
-          now = fmaxf(__fdiv_rn(__fmul_rn(amax, 4.f), 448.f), 1e-8f);
+          now = fmaxf(__fmul_rn(amax, 4.0f / 448.0f), 1e-8f);
           if (lane == 0) scales[s_dst[j] / per_block * a.nkv] = now;
         }
         if (now != from) {  // rounded to 8 bits again, to within half a step of e4m3
           uint32_t y[4];
+          if (fminf(now, from) > 1e-20f && fmaxf(now, from) < 1e20f) {
+            // f / now, correctly rounded, from the correctly rounded reciprocal: the remainder of f * r is exact and
+            // corrects it (P. Markstein, 1990); the bounds keep the remainder above fp32's smallest
+            const float r = __frcp_rn(now);
 #pragma unroll
-          for (int k = 0; k < 16; ++k) f[k] = __fdiv_rn(f[k], now);
+            for (int k = 0; k < 16; ++k) {
+              const float q = __fmul_rn(f[k], r);
+              f[k] = q == 0.f ? q : fmaf(fmaf(-q, now, f[k]), r, q);  // (a zero keeps its sign)
+            }
+          } else {
+#pragma unroll
+            for (int k = 0; k < 16; ++k) f[k] = __fdiv_rn(f[k], now);
+          }
 #pragma unroll
           for (int k = 0; k < 4; ++k) y[k] = f32x4_to_e4m3(f + 4 * k);
           x[u] = make_uint4(y[0], y[1], y[2], y[3]);

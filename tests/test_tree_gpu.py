@@ -101,10 +101,11 @@ class Case:
                 a = torch.softmax(s, -1).nan_to_num(0.0)
                 out[at:at + n] = torch.einsum("hgnk,hkd->nhgd", a, v).reshape(n, self.nq, 128)
                 aabs = torch.einsum("hgnk,hkd->nhgd", a, v.abs()).reshape(n, self.nq, 128)
-                # a score: 128 rounded sums and 4 products of it, exp2 to 2^-22, each weight rounded to bf16 (2^-8
-                # with half a step) or f16 (2^-11), the sums over at most 2^15 keys in tiles: 600 roundings
+                # a score: 128 rounded sums and 4 products of it, exp2 to 2^-22, the sums over at most 2^15 keys in
+                # tiles: 600 roundings; each weight (8-bit caches: times V's scale) is rounded to bf16, half a step
+                # of which is 2^-8 of it
                 e = 2 * (float(size) * 132 * 2.0 ** -24 + 2.0 ** -21) + 600 * 2.0 ** -24
-                bound[at:at + n] = aabs * (e + (2.0 ** -11 if self.dtype == F8 else 2.0 ** -8))
+                bound[at:at + n] = aabs * (e + 2.0 ** -8)
             at += n
         return out, bound + out.abs() * 2.0 ** -8 + 1e-30
 
@@ -497,11 +498,12 @@ def _commit_case(ns, ks, bs, dtype, L=3, nkv=2, seed=0, width=None):
 
 
 def _check_commit(ops, ctx, kv, s, path, length):
-    kv2, s2 = kv.cpu(), None if s is None else s.cpu()
+    # the oracle on the GPU too: there a division by 448 is a product with its reciprocal, as where K/V is stored
+    kv2, s2 = kv.clone(), None if s is None else s.clone()
     R.tree_commit(kv2, ctx.host_q_lens, ctx.host_k_lens, ctx.block_tables.tolist(), path.cpu(), length.cpu(), s2)
     ops.commit_tree(kv, ctx, path, length, s)
-    assert torch.equal(kv.cpu().view(torch.uint8), kv2.view(torch.uint8))  # the same fp32 operations: bit for bit
-    assert s is None or torch.equal(s.cpu(), s2)
+    assert torch.equal(kv.view(torch.uint8), kv2.view(torch.uint8))  # the same fp32 operations: bit for bit
+    assert s is None or torch.equal(s, s2)
 
 
 @KV
@@ -531,6 +533,14 @@ def test_commit_paths_that_end_early_and_bad_blocks(ops, dtype):
     ctx, kv, s, path, length = _commit_case([9], [40], 16, dtype)
     ctx.context_lens[0], ctx.host_k_lens[0] = 4, 4
     _check_commit(ops, ctx, kv, s, path, length)
+
+
+def test_commit_scales_of_any_size(ops):
+    """Quotients by scales far from 1, where the remainder of a quotient would fall below fp32's smallest."""
+    for size in (1e-30, 1e-12, 1e12, 1e30):
+        ctx, kv, s, path, length = _commit_case([16, 9], [40, 30], 16, F8, seed=4)
+        s *= size
+        _check_commit(ops, ctx, kv, s, path, length)
 
 
 @KV
