@@ -80,14 +80,31 @@ __device__ __forceinline__ int seq_begin(const TreeAttn& t, int b) { return min(
 __device__ __forceinline__ int seq_nodes(const TreeAttn& t, int b) { return min(t.cu_q[b + 1], t.T) - seq_begin(t, b); }
 __device__ __forceinline__ int seq_rows(const Args& a, int b) { return min(seq_nodes(a.t, b), a.t.max_nodes) * a.G; }
 __device__ __forceinline__ int seq_tiles(const TreeAttn& t, int b) { return max(1, (t.ctx_lens[b] + KT - 1) / KT); }
-__device__ __forceinline__ int64_t seq_count(const Args& a, int b) {
+// Its work: a tile counts twice where it meets more than 128 rows.
+__device__ __forceinline__ int64_t seq_work(const Args& a, int b) {
   const int rows = seq_rows(a, b);
-  return rows > 0 ? (int64_t)seq_tiles(a.t, b) * a.t.nkv * ((rows + a.rows_cap - 1) / a.rows_cap) : 0;
+  if (rows <= 0) return 0;
+  const int rts = (rows + a.rows_cap - 1) / a.rows_cap, last = rows - (rts - 1) * a.rows_cap;
+  return (int64_t)seq_tiles(a.t, b) * a.t.nkv * ((a.rows_cap > 128 ? 2 : 1) * (rts - 1) + (last > 128 ? 2 : 1));
+}
+// The tile (of sequence b's part of the list) in which its work unit `w` lies, and the units ahead of tile `i`.
+__device__ __forceinline__ int64_t work_tile(const Args& a, int b, int64_t w) {
+  if (a.rows_cap <= 128) return w;
+  const int rows = seq_rows(a, b);
+  const int64_t twice = (int64_t)seq_tiles(a.t, b) * a.t.nkv * (rows / 256 + (rows % 256 > 128 ? 1 : 0));
+  return w < 2 * twice ? w / 2 : w - twice;
+}
+__device__ __forceinline__ int64_t tile_work(const Args& a, int b, int64_t i) {
+  if (a.rows_cap <= 128) return i;
+  const int rows = seq_rows(a, b);
+  const int64_t twice = (int64_t)seq_tiles(a.t, b) * a.t.nkv * (rows / 256 + (rows % 256 > 128 ? 1 : 0));
+  return i < twice ? 2 * i : i + twice;
 }
 
-// Stretch [lo, hi) of the list, and the sequences in which its ends lie, with the tiles before them in it.
+// Stretch c of the list: from tile lo_tile of sequence lo_seq to ahead of tile hi_tile of hi_seq.  In units of work:
+// the whole list's, and those ahead of hi_seq.
 struct Spot {
-  int64_t total, lo, hi, lo_rem, hi_rem;
+  int64_t total, hi_ahead, lo_tile, hi_tile;
   int lo_seq, hi_seq;
 };
 
@@ -97,7 +114,7 @@ __device__ void find_chunk(const Args& a, int c, Spot* out, int64_t* part) {
   const int per = (a.t.num_seqs + nt - 1) / nt;
   const int b0 = min(a.t.num_seqs, (int)threadIdx.x * per), b1 = min(a.t.num_seqs, b0 + per);
   int64_t sum = 0;
-  for (int b = b0; b < b1; ++b) sum += seq_count(a, b);
+  for (int b = b0; b < b1; ++b) sum += seq_work(a, b);
   int64_t incl = sum;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -105,6 +122,10 @@ __device__ void find_chunk(const Args& a, int c, Spot* out, int64_t* part) {
     if (lane >= o) incl += up;
   }
   if (lane == 31) part[warp] = incl;
+  if (threadIdx.x == 0) {
+    out->lo_seq = out->hi_seq = a.t.num_seqs;
+    out->lo_tile = out->hi_tile = 0;
+  }
   __syncthreads();
   int64_t before = 0, total = 0;
   for (int w = 0; w < nw; ++w) {
@@ -112,64 +133,75 @@ __device__ void find_chunk(const Args& a, int c, Spot* out, int64_t* part) {
     total += part[w];
   }
   const int64_t lo = total * c / a.chunks, hi = total * (c + 1) / a.chunks;
-  if (threadIdx.x == 0) {
-    out->total = total;
-    out->lo = lo;
-    out->hi = hi;
-  }
+  if (threadIdx.x == 0) out->total = total;
   int64_t at = before + incl - sum;
   for (int b = b0; b < b1; ++b) {
-    const int64_t n = seq_count(a, b);
+    const int64_t n = seq_work(a, b);
     if (lo >= at && lo < at + n) {
       out->lo_seq = b;
-      out->lo_rem = lo - at;
+      out->lo_tile = work_tile(a, b, lo - at);
     }
     if (hi >= at && hi < at + n) {
       out->hi_seq = b;
-      out->hi_rem = hi - at;
+      out->hi_tile = work_tile(a, b, hi - at);
+      out->hi_ahead = at;
     }
     at += n;
   }
   __syncthreads();
 }
 
-// Walks the items of a stretch: tiles [t0, t1) of KV head h and rows [row0, row0 + rows) of sequence b.
+// Walks the items of a stretch: tiles [t0, t1) of KV head h and rows [rt * rows_cap, ...) of sequence b.
 struct Walk {
-  int b, rt, h, t0, t1, tiles, rts;
-  int64_t left;
+  int b, rt, h, t0, t1, tiles, rts, hi_seq;
+  int64_t at, hi_tile;  // the item's first tile in the sequence's part of the list; the stretch's end in hi_seq's
   __device__ __forceinline__ void enter(const Args& a) {
     tiles = seq_tiles(a.t, b);
     rts = (seq_rows(a, b) + a.rows_cap - 1) / a.rows_cap;
   }
+  __device__ __forceinline__ void to_end() {
+    t1 = b == hi_seq ? (int)min((int64_t)tiles, hi_tile - at) : tiles;
+  }
   __device__ __forceinline__ Walk(const Args& a, const Spot& s) {
-    left = s.hi - s.lo;
-    b = rt = h = t0 = t1 = tiles = rts = 0;
-    if (left > 0) {
-      b = s.lo_seq;
+    b = s.lo_seq;
+    hi_seq = s.hi_seq;
+    hi_tile = s.hi_tile;
+    rt = h = t0 = t1 = tiles = rts = 0;
+    at = 0;
+    if (b < a.t.num_seqs) {
       enter(a);
       const int per = tiles * a.t.nkv;  // below 2^31: k_len / 128 x nkv
-      rt = (int)(s.lo_rem / per);
-      const int r = (int)(s.lo_rem % per);
+      rt = (int)(s.lo_tile / per);
+      const int r = (int)(s.lo_tile % per);
       h = r / tiles;
       t0 = r % tiles;
-      t1 = (int)min((int64_t)tiles, t0 + left);
+      at = s.lo_tile - t0;
+      to_end();
     }
   }
-  __device__ __forceinline__ bool more() const { return left > 0; }
+  __device__ __forceinline__ bool more() const { return t1 > t0; }
   __device__ __forceinline__ void next(const Args& a) {
-    left -= t1 - t0;
-    if (left <= 0) return;
-    if (t1 == tiles && ++h == a.t.nkv) {
+    if (t1 < tiles) {
+      t0 = t1;  // the stretch's end
+      return;
+    }
+    at += tiles;
+    if (++h == a.t.nkv) {
       h = 0;
       if (++rt == rts) {
         rt = 0;
+        at = 0;
         do ++b;
-        while (seq_rows(a, b) <= 0);
+        while (b < a.t.num_seqs && seq_rows(a, b) <= 0);
+        if (b >= a.t.num_seqs) {
+          t0 = t1 = 0;
+          return;
+        }
         enter(a);
       }
     }
     t0 = 0;
-    t1 = (int)min((int64_t)tiles, left);
+    to_end();
   }
   __device__ __forceinline__ int rows(const Args& a) const { return min(a.rows_cap, seq_rows(a, b) - rt * a.rows_cap); }
 };
@@ -1408,20 +1440,27 @@ __global__ void __launch_bounds__(128) tree_join_kernel(Args a) {
   __shared__ int64_t part[4];
   const int chunk = blockIdx.x;
   find_chunk(a, chunk, &spot, part);
-  const int64_t lo = spot.lo, hi = spot.hi;
-  if (hi <= lo || hi >= spot.total) return;
-  const int b = spot.hi_seq, tiles = seq_tiles(a.t, b), per = tiles * a.t.nkv;
-  const int rt = (int)(spot.hi_rem / per), r0 = (int)(spot.hi_rem % per), h = r0 / tiles, t = r0 % tiles;
-  const int64_t begin = hi - t, end = begin + tiles;
-  if (t == 0 || begin < lo) return;  // nothing is cut here, or the item begins in an earlier chunk
+  const int b = spot.hi_seq;
+  if (b >= a.t.num_seqs) return;  // the list's end
+  const int tiles = seq_tiles(a.t, b), per = tiles * a.t.nkv;
+  const int rt = (int)(spot.hi_tile / per), r0 = (int)(spot.hi_tile % per), h = r0 / tiles, t = r0 % tiles;
+  // the item that this chunk's end cuts: its first tile and its work
+  const int64_t first = spot.hi_tile - t, begin = spot.hi_ahead + tile_work(a, b, first),
+                end = spot.hi_ahead + tile_work(a, b, first + tiles), unit = (end - begin) / tiles;
+  // tiles of it ahead of a place in the list
+  auto ahead = [&](int64_t w) { return w <= begin ? (int64_t)0 : w >= end ? (int64_t)tiles : (w - begin) / unit; };
+  auto edge = [&](int k) { return spot.total * k / a.chunks; };
+  // (a chunk whose place lies inside the item's first tile begins with it)
+  if (t == 0 || edge(chunk) >= begin + unit) return;  // nothing is cut here, or the item begins in an earlier chunk
   const int rows = min(a.rows_cap, seq_rows(a, b) - rt * a.rows_cap);
   const int r = blockIdx.y * 4 + (threadIdx.x >> 5), c = (threadIdx.x & 31) * 4;
   if (r >= rows) return;
   float M = -INFINITY, L = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-  int64_t from = lo, upto = hi;
-  for (int k = chunk;; ++k) {
-    if (upto > from) {  // with fewer tiles than chunks, some have none
-      const float* po = slot_o(a, k, k == chunk);
+  int64_t from = 0;
+  for (int k = chunk; from < tiles; ++k) {
+    const int64_t upto = ahead(edge(k + 1));
+    if (upto > from) {  // with less work than chunks, some have none
+      const float* po = slot_o(a, k, from == 0);
       const float2 ml = *reinterpret_cast<const float2*>(po + (int64_t)a.rows_cap * AD + r * 2);
       const float4 v = *reinterpret_cast<const float4*>(po + (int64_t)r * AD + c);
       if (!(ml.x == -INFINITY && ml.y == 0.f)) {
@@ -1434,10 +1473,8 @@ __global__ void __launch_bounds__(128) tree_join_kernel(Args a) {
         o[2] = (f == 0.f ? 0.f : o[2] * f) + g * v.z;
         o[3] = (f == 0.f ? 0.f : o[3] * f) + g * v.w;
       }
+      from = upto;
     }
-    if (upto >= end) break;
-    from = upto;
-    upto = spot.total * (k + 2) / a.chunks;
   }
   const float inv = L != 0.f ? 1.f / L : 0.f;
   float v[4] = {o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};

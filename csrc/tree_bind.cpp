@@ -158,7 +158,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> tree_verify(const at::Tensor& log
   TORCH_CHECK(logits.dim() == 2 && logits.size(1) > 0 && (logits.stride(1) == 1 || logits.size(1) == 1), op,
               ": logits must be [tokens, vocabulary] with unit inner stride");
   const int64_t T = logits.size(0), V = logits.size(1);
-  TORCH_CHECK(V < (1LL << 30) && T < (1LL << 31) - 65536, op, ": too large");
+  TORCH_CHECK(V < (1 << 22) && T < (1LL << 31) - 65536, op, ": vocabularies of up to 4194303 tokens, got ", V);
   check_batch(cu_q, num_seqs, max_nodes, logits, op);
   check_vec(tokens, T, at::kInt, logits, op, "tokens");
   check_vec(parents, T, at::kInt, logits, op, "parents");

@@ -68,135 +68,121 @@ __global__ void tree_mask_kernel(const int* __restrict__ parents, const int* __r
 constexpr int CT = 256;   // threads per CTA
 constexpr int BATCH = 8;  // rows in flight per group
 
-__device__ __forceinline__ int64_t page_row(const TreeCommit& a, int b, int pos) {
-  const int bi = pos / a.block_size;
-  if (bi >= a.W) return -1;
-  const int blk = a.block_tables[(int64_t)b * a.bt_stride + bi];
-  if (blk < 0 || blk >= a.num_blocks) return -1;
-  return (int64_t)blk * a.nkv * a.block_size + pos % a.block_size;
-}
-
 template <bool FP8>
-__global__ void __launch_bounds__(CT) tree_commit_kernel(TreeCommit a) {
+__global__ void __launch_bounds__(CT, FP8 ? 3 : 4) tree_commit_kernel(TreeCommit a) {
   pdl_wait();     // inputs come from the previous kernel in the stream
   pdl_trigger();  // the next kernel may start its prologue
   constexpr int LANES = FP8 ? 8 : 16;  // lanes of 16 bytes per row
   constexpr int UNITS = CT / LANES;
-  __shared__ int64_t s_src[TREE_MAX_NODES], s_dst[TREE_MAX_NODES];
-  __shared__ int s_off[TREE_MAX_NODES];  // destination's offset in its block; -1: nothing moves
+  constexpr int ROW = FP8 ? 128 : 256;  // bytes
+  // The rows to move, in the order of their destinations, and the tree's blocks (ids; -1: none).
+  __shared__ int s_block[TREE_MAX_NODES + 1];
+  __shared__ uint32_t s_src[TREE_MAX_NODES], s_dst[TREE_MAX_NODES];  // (block of the tree) << 24 | offset in it
   __shared__ int s_first, s_len;
-  extern __shared__ float s_scale[];     // e4m3: [UNITS][blocks of the tree]
-  const int b = blockIdx.y;
-  const int n = a.cu_q[b + 1] - a.cu_q[b], base = a.ctx_lens[b] - n;
+  extern __shared__ float s_scale[];  // e4m3: [UNITS][blocks of the tree]
+  const int b = blockIdx.y, bs = a.block_size;
+  const int n = min(a.cu_q[b + 1] - a.cu_q[b], a.max_nodes), base = a.ctx_lens[b] - (a.cu_q[b + 1] - a.cu_q[b]);
   const int want = min(min(a.length[b], a.max_path), TREE_MAX_NODES);
   if (base < 0 || want <= 1) return;
   const int* path = a.path + (int64_t)b * a.path_stride;
-  if (threadIdx.x == 0) {
-    s_first = want;
-    s_len = want;
+  const int block0 = base / bs, blocks = (base + n - 1) / bs - block0 + 1;
+  if (threadIdx.x == 0) s_first = s_len = want;
+  for (int i = threadIdx.x; i < blocks; i += CT) {
+    const int id = block0 + i < a.W ? a.block_tables[(int64_t)b * a.bt_stride + block0 + i] : -1;
+    s_block[i] = id >= 0 && id < a.num_blocks ? id : -1;
   }
   __syncthreads();
   for (int j = threadIdx.x; j < want; j += CT) {
     const int node = path[j], before = j ? path[j - 1] : -1;
-    if (!(node > before && node < min(n, a.max_nodes))) atomicMin(&s_len, j);
+    if (!(node > before && node < n)) {
+      atomicMin(&s_len, j);  // the path ends where it does not increase, or leaves the tree
+    } else {
+      const int src = base + node, dst = base + j;
+      s_src[j] = (uint32_t)(src / bs - block0) << 24 | src % bs;
+      s_dst[j] = (uint32_t)(dst / bs - block0) << 24 | dst % bs;
+      if (node != j) atomicMin(&s_first, j);
+    }
   }
   __syncthreads();
-  const int len = s_len;
-  for (int j = threadIdx.x; j < len; j += CT) {
-    const int node = path[j];
-    const int64_t src = page_row(a, b, base + node), dst = page_row(a, b, base + j);
-    const bool moves = node != j && src >= 0 && dst >= 0;
-    s_src[j] = src;
-    s_dst[j] = dst;
-    s_off[j] = moves ? (base + j) % a.block_size : -1;
-    if (node != j) atomicMin(&s_first, j);
-  }
-  __syncthreads();
-  const int first = s_first;
-  if (first >= len) return;
-  const int unit = blockIdx.x * UNITS + threadIdx.x / LANES, lane = threadIdx.x % LANES;
-  if (unit >= 2 * a.layers * a.nkv) return;
-  const int h = unit % a.nkv, layer = unit / a.nkv % a.layers, kv = unit / a.nkv / a.layers;
-  const int row_bytes = FP8 ? 128 : 256;
-  uint8_t* pool = static_cast<uint8_t*>(a.kv) + kv * a.stride_kv + layer * a.stride_layer +
-                  (int64_t)h * a.block_size * row_bytes + lane * 16;
-  if constexpr (!FP8) {
-    for (int j0 = first; j0 < len; j0 += BATCH) {
-      uint4 x[BATCH];
+  const int first = s_first, len = s_len;
+  const int lane = threadIdx.x % LANES;
+  for (int unit = blockIdx.x * UNITS + threadIdx.x / LANES; unit < 2 * a.layers * a.nkv && first < len; unit += gridDim.x * UNITS) {
+    const int h = unit % a.nkv, layer = unit / a.nkv % a.layers, kv = unit / a.nkv / a.layers;
+    uint8_t* pool = static_cast<uint8_t*>(a.kv) + kv * a.stride_kv + layer * a.stride_layer + lane * 16;
+    auto at = [&](uint32_t where) {
+      return reinterpret_cast<uint4*>(pool + (((int64_t)s_block[where >> 24] * a.nkv + h) * bs + (where & 0xffffff)) * ROW);
+    };
+    auto moves = [&](int j) { return j < len && s_block[s_src[j] >> 24] >= 0 && s_block[s_dst[j] >> 24] >= 0; };
+    if constexpr (!FP8) {
+      for (int j0 = first; j0 < len; j0 += BATCH) {
+        uint4 x[BATCH];
 #pragma unroll
-      for (int u = 0; u < BATCH; ++u)
-        if (j0 + u < len && s_off[j0 + u] >= 0) x[u] = *reinterpret_cast<const uint4*>(pool + s_src[j0 + u] * row_bytes);
+        for (int u = 0; u < BATCH; ++u)
+          if (moves(j0 + u)) x[u] = *at(s_src[j0 + u]);
 #pragma unroll
-      for (int u = 0; u < BATCH; ++u)
-        if (j0 + u < len && s_off[j0 + u] >= 0) *reinterpret_cast<uint4*>(pool + s_dst[j0 + u] * row_bytes) = x[u];
-    }
-  } else {
-    float* scales = a.scale + kv * a.scale_stride_kv + layer * a.scale_stride_layer + h;
-    const int64_t per_block = (int64_t)a.nkv * a.block_size;
-    const unsigned group = 0xffu << (threadIdx.x & 24);
-    // the scales of the tree's blocks as they were: a moved first row replaces its block's
-    const int blk0 = (base + first) / a.block_size;
-    const int blocks = (base + min(n, a.max_nodes) - 1) / a.block_size - blk0 + 1;
-    const int ld = (a.max_nodes - 1) / a.block_size + 2;
-    float* old = s_scale + threadIdx.x / LANES * ld;
-    for (int i = lane; i < blocks; i += LANES) {
-      const int64_t r = page_row(a, b, (blk0 + i) * a.block_size);
-      old[i] = r >= 0 ? scales[r / per_block * a.nkv] : 1.f;
-    }
-    __syncwarp(group);
-    float now = old[0];  // of the destination's block
-    int now_blk = 0;
-    for (int j0 = first; j0 < len; j0 += BATCH) {
-      uint4 x[BATCH];
-#pragma unroll
-      for (int u = 0; u < BATCH; ++u)
-        if (j0 + u < len && s_off[j0 + u] >= 0) x[u] = *reinterpret_cast<const uint4*>(pool + s_src[j0 + u] * row_bytes);
-#pragma unroll
-      for (int u = 0; u < BATCH; ++u) {
-        const int j = j0 + u;
-        if (j >= len || s_off[j] < 0) continue;
-        const float from = old[(base + path[j]) / a.block_size - blk0];
-        const int blk = (base + j) / a.block_size - blk0;
-        if (blk != now_blk) now = old[blk];
-        now_blk = blk;
-        float f[16];
-        const uint32_t w[4] = {x[u].x, x[u].y, x[u].z, x[u].w};
-#pragma unroll
-        for (int k = 0; k < 4; ++k) e4m3x4_to_f32(w[k], f + 4 * k);
-        float amax = 0.f;
-#pragma unroll
-        for (int k = 0; k < 16; ++k) {
-          f[k] = __fmul_rn(f[k], from);
-          amax = fmaxf(amax, fabsf(f[k]));
-        }
-        if (s_off[j] == 0) {
-          // the block begins with this row: its scale, as the store of a first token sets it
-#pragma unroll
-          for (int o = 4; o; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(group, amax, o, 8));
-          now = fmaxf(__fmul_rn(amax, 4.0f / 448.0f), 1e-8f);
-          if (lane == 0) scales[s_dst[j] / per_block * a.nkv] = now;
-        }
-        if (now != from) {  // rounded to 8 bits again, to within half a step of e4m3
-          uint32_t y[4];
-          if (fminf(now, from) > 1e-20f && fmaxf(now, from) < 1e20f) {
-            // f / now, correctly rounded, from the correctly rounded reciprocal: the remainder of f * r is exact and
-            // corrects it (P. Markstein, 1990); the bounds keep the remainder above fp32's smallest
-            const float r = __frcp_rn(now);
-#pragma unroll
-            for (int k = 0; k < 16; ++k) {
-              const float q = __fmul_rn(f[k], r);
-              f[k] = q == 0.f ? q : fmaf(fmaf(-q, now, f[k]), r, q);  // (a zero keeps its sign)
-            }
-          } else {
-#pragma unroll
-            for (int k = 0; k < 16; ++k) f[k] = __fdiv_rn(f[k], now);
-          }
-#pragma unroll
-          for (int k = 0; k < 4; ++k) y[k] = f32x4_to_e4m3(f + 4 * k);
-          x[u] = make_uint4(y[0], y[1], y[2], y[3]);
-        }
-        *reinterpret_cast<uint4*>(pool + s_dst[j] * row_bytes) = x[u];
+        for (int u = 0; u < BATCH; ++u)
+          if (moves(j0 + u)) *at(s_dst[j0 + u]) = x[u];
       }
+    } else {
+      float* scales = a.scale + kv * a.scale_stride_kv + layer * a.scale_stride_layer + h;
+      const unsigned group = 0xffu << (threadIdx.x & 24);
+      // the scales of the tree's blocks as they were: a moved first row replaces its block's
+      float* old = s_scale + threadIdx.x / LANES * ((a.max_nodes - 1) / bs + 2);
+      for (int i = lane; i < blocks; i += LANES) old[i] = s_block[i] >= 0 ? scales[(int64_t)s_block[i] * a.nkv] : 1.f;
+      __syncwarp(group);
+      float now = 1.f;  // of the destination's block
+      int now_block = -1;
+      for (int j0 = first; j0 < len; j0 += BATCH) {
+        uint4 x[BATCH];
+#pragma unroll
+        for (int u = 0; u < BATCH; ++u)
+          if (moves(j0 + u)) x[u] = *at(s_src[j0 + u]);
+#pragma unroll
+        for (int u = 0; u < BATCH; ++u) {
+          if (!moves(j0 + u)) continue;
+          const uint32_t dst = s_dst[j0 + u];
+          const float from = old[s_src[j0 + u] >> 24];
+          if ((int)(dst >> 24) != now_block) now = old[dst >> 24];
+          now_block = dst >> 24;
+          float f[16];
+          const uint32_t w[4] = {x[u].x, x[u].y, x[u].z, x[u].w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) e4m3x4_to_f32(w[k], f + 4 * k);
+#pragma unroll
+          for (int k = 0; k < 16; ++k) f[k] = __fmul_rn(f[k], from);
+          if ((dst & 0xffffff) == 0) {
+            // the block begins with this row: its scale, as the store of a first token sets it
+            float amax = 0.f;
+#pragma unroll
+            for (int k = 0; k < 16; ++k) amax = fmaxf(amax, fabsf(f[k]));
+#pragma unroll
+            for (int o = 4; o; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(group, amax, o, 8));
+            now = fmaxf(__fmul_rn(amax, 4.0f / 448.0f), 1e-8f);
+            if (lane == 0) scales[(int64_t)s_block[now_block] * a.nkv] = now;
+          }
+          if (now != from) {  // rounded to 8 bits again, to within half a step of e4m3
+            uint32_t y[4];
+            if (fminf(now, from) > 1e-20f && fmaxf(now, from) < 1e20f) {
+              // f / now, correctly rounded, from the correctly rounded reciprocal: the remainder of f * r is exact
+              // and corrects it (P. Markstein, 1990); the bounds keep the remainder above fp32's smallest
+              const float r = __frcp_rn(now);
+#pragma unroll
+              for (int k = 0; k < 16; ++k) {
+                const float q = __fmul_rn(f[k], r);
+                f[k] = q == 0.f ? q : fmaf(fmaf(-q, now, f[k]), r, q);  // (a zero keeps its sign)
+              }
+            } else {
+#pragma unroll
+              for (int k = 0; k < 16; ++k) f[k] = __fdiv_rn(f[k], now);
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) y[k] = f32x4_to_e4m3(f + 4 * k);
+            x[u] = make_uint4(y[0], y[1], y[2], y[3]);
+          }
+          *at(dst) = x[u];
+        }
+      }
+      __syncwarp(group);  // `old` is filled anew
     }
   }
 }
@@ -222,8 +208,11 @@ cudaError_t launch_tree_commit(const TreeCommit& a, cudaStream_t stream) {
   if (a.num_seqs <= 0 || a.num_seqs > 65535 || a.layers <= 0 || a.nkv <= 0 || a.block_size <= 0 || a.max_path <= 0 ||
       a.max_nodes <= 0 || a.max_nodes > TREE_MAX_NODES)
     return cudaErrorInvalidValue;
-  const int units = CT / (a.kv_fp8 ? 8 : 16);
-  const dim3 grid((2 * a.layers * a.nkv + units - 1) / units, a.num_seqs);
+  // a CTA's way to its first row takes some microseconds: no more CTAs than run at a time, about four per SM, each
+  // for several units
+  const int units = CT / (a.kv_fp8 ? 8 : 16), most = (2 * a.layers * a.nkv + units - 1) / units;
+  const int share = (4 * 148 + a.num_seqs - 1) / a.num_seqs;
+  const dim3 grid(share < most ? share : most, a.num_seqs);
   if (a.kv_fp8)
     launch_pdl(tree_commit_kernel<true>, grid, dim3(CT), units * ((a.max_nodes - 1) / a.block_size + 2) * sizeof(float),
                stream, a);

@@ -5,26 +5,27 @@
 // child the next token is the first x whose cumulative sum of p is above u_draw times the total.
 //
 // A cumulative sum over a vocabulary of 1.5e5 tokens has tokens narrower than fp32's rounding next to every border,
-// so weights and sums are 64-bit: decisions are those of exact arithmetic but for random numbers within some 1e-12 of
-// a border, and do not depend on how many CTAs share a row.  exp2 in 64 bits costs 9 fp64 instructions here: the
-// argument is taken apart into a multiple of 1/256 (a table entry, and an exponent by integer addition) and a rest
-// |r| <= 1/512 with 2^r = 1 + t + t^2/2 + t^3/6, t = r ln 2 (next term: 1.4e-13).
+// so weights and sums are 64-bit: decisions are those of exact arithmetic but for random numbers within some 1e-11 of
+// a border, and do not depend on how many CTAs share a row.  exp2 in 64 bits costs 9 fp64 instructions here, which
+// bound the kernel (an SM does 64 a clock): the argument is taken apart into a multiple of 1/32 (a table entry, and
+// an exponent by integer addition) and a rest |r| <= 1/64 with 2^r = 1 + t + t^2/2 + t^3/6 + t^4/24, t = r ln 2 (next
+// term: at most 1.3e-12).  The table's halves are read as words: 32 entries, a bank each.
 //
 // One cluster of CTAs walks one tree, so only the rows of visited nodes are read.  A row is cut into chunks of
-// 1024 tokens; a warp sums a chunk relative to the chunk's maximum and sends (sum, maximum) to every CTA of the
+// 512 tokens; a warp sums a chunk relative to the chunk's maximum and sends (sum, maximum) to every CTA of the
 // cluster, whose first warps then take the same decisions from the same numbers: one cluster barrier per row.
 #include "common.cuh"
 #include "tcgen05.cuh"
 #include "tree.h"
+#include <cstdlib>
 
 namespace nvb {
 namespace {
 
-constexpr int VT = 512;            // threads per CTA
-constexpr int VWARPS = VT / 32;
-constexpr int BLOCK = 1024;        // tokens of a warp's step: 32 per lane
+constexpr int BLOCK = 512;         // tokens of a warp's step: 16 per lane
 constexpr int MAX_CHUNKS = 512;    // longer vocabularies have longer chunks
 constexpr float NEG = -INFINITY;
+constexpr unsigned SPAN = 0xC0DC2000u;  // upper word of -28800 = -32 x 900: weights below 2^-900 of the largest are none
 
 struct ChunkSum {
   double sum;  // relative to max (walk over the logits), or as it is (residuals)
@@ -32,29 +33,71 @@ struct ChunkSum {
   int first;   // token of the first maximum
 };
 
-struct Exp2 {
-  const double* table;  // 2^(j / 256)
-  // 2^(z / 256) p + acc for z <= 0 (or a rounding above it); z below -256000 counts as that
-  __device__ __forceinline__ double fma_to(double z, double acc) const {
-    const unsigned hi = min((unsigned)__double2hiint(z), 0xC10F4000u);  // -256000 and its low word's worth
-    z = __hiloint2double((int)hi, __double2loint(z));
-    const double t = z + 6755399441055744.0;  // 1.5 * 2^52: the low word is the nearest integer
-    const int j = __double2loint(t);
-    const double r = z - (t - 6755399441055744.0);
-    constexpr double A = 0.69314718055994530942 / 256.0;
-    const double p = fma(fma(fma(A * A * A / 6.0, r, A * A / 2.0), r, A), r, 1.0);
-    const double e = table[j & 255];
-    const double s = __hiloint2double(__double2hiint(e) + (j >> 8) * (1 << 20), __double2loint(e));
-    return fma(s, p, acc);
-  }
+// 2^(z / 32) for z <= 0 (or a rounding above it) from a table of 2^(j / 32), possibly times a factor, as words;
+// z below -28800 counts as that.  The two factors of the result.
+struct Power {
+  double scale, poly;
 };
+__device__ __forceinline__ Power power(double z, const uint32_t* hi32, const uint32_t* lo32) {
+  z = __hiloint2double((int)min((unsigned)__double2hiint(z), SPAN), __double2loint(z));
+  const double t = z + 6755399441055744.0;  // 1.5 * 2^52: the low word is the nearest integer
+  const int j = __double2loint(t);
+  const double r = z - (t - 6755399441055744.0);
+  constexpr double A = 0.69314718055994530942 / 32.0;
+  Power p;
+  p.poly = fma(fma(fma(fma(A * A * A * A / 24.0, r, A * A * A / 6.0), r, A * A / 2.0), r, A), r, 1.0);
+  p.scale = __hiloint2double((int)hi32[j & 31] + (j >> 5) * (1 << 20), (int)lo32[j & 31]);
+  return p;
+}
+
+// The same for four at a time, step by step: one alone waits for its own last instruction most of the time.
+__device__ __forceinline__ void power4(double (&z)[4], const uint32_t* hi32, const uint32_t* lo32, double (&scale)[4],
+                                       double (&poly)[4]) {
+  constexpr double A = 0.69314718055994530942 / 32.0;
+  double t[4];
+  int j[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) z[i] = __hiloint2double((int)min((unsigned)__double2hiint(z[i]), SPAN), __double2loint(z[i]));
+#pragma unroll
+  for (int i = 0; i < 4; ++i) t[i] = z[i] + 6755399441055744.0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    j[i] = __double2loint(t[i]);
+    t[i] -= 6755399441055744.0;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) z[i] -= t[i];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    scale[i] = __hiloint2double((int)hi32[j[i] & 31] + (j[i] >> 5) * (1 << 20), (int)lo32[j[i] & 31]);
+    poly[i] = fma(A * A * A * A / 24.0, z[i], A * A * A / 6.0);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) poly[i] = fma(poly[i], z[i], A * A / 2.0);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) poly[i] = fma(poly[i], z[i], A);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) poly[i] = fma(poly[i], z[i], 1.0);
+}
+
+// The 64-bit value of an fp32 one by its bits (no conversion instruction: those are a quarter as many a clock).
+// 0 and subnormals become about 2^-127, infinities 2^128.
+__device__ __forceinline__ double wide(uint32_t f) {
+  return __hiloint2double((int)((((int)f >> 3) & 0x8fffffff) + 0x38000000), (int)(f << 29));
+}
 
 // What a token's weight is made of, at the node at hand.
 struct Dist {
-  double c256;     // 256 log2(e) / T
+  double c;        // 32 log2(e) / T
   double inv_sum;  // 1 / sum of the weights
   float max;       // the row's maximum (a NaN counts as -inf)
   bool greedy;
+  // Whether l c - max c in one instruction is exact enough (2^-35 of 1/32), and -inf far enough off.
+  __device__ __forceinline__ bool plain(float top) const { return c > 1e-9 && fabs((double)top) * c < 262144.0; }
+};
+
+struct Tables {
+  const uint32_t *hi, *lo;  // 2^(j / 32)
 };
 
 template <bool BF16>
@@ -67,55 +110,78 @@ __device__ __forceinline__ float logit_at(const void* row, int64_t x) {
   return fmaxf(v, NEG);  // a NaN counts as -inf
 }
 
-// exp((l - max) / T), 0 for -inf and below 2^-1000; an infinite maximum leaves its own tokens alone.
-__device__ __forceinline__ double weight(float l, const Dist& d, const Exp2& ex) {
+template <bool BF16>
+__device__ __forceinline__ float raw_logit(uint32_t raw) {
+  return fmaxf(__uint_as_float(BF16 ? raw << 16 : raw), NEG);
+}
+
+// exp((l - top) / T), 0 for -inf and below 2^-900; an infinite maximum leaves its own tokens alone.
+__device__ __forceinline__ double weight(float l, float top, double c, const Tables& tb) {
   if (l == NEG) return 0.0;
-  if (d.max == INFINITY) return l == INFINITY ? 1.0 : 0.0;
-  const double z = ((double)l - (double)d.max) * d.c256;
-  return z < -256000.0 ? 0.0 : ex.fma_to(z, 0.0);
+  if (top == INFINITY) return l == INFINITY ? 1.0 : 0.0;
+  const double z = ((double)l - (double)top) * c;
+  if ((unsigned)__double2hiint(z) > SPAN) return 0.0;
+  const Power p = power(z, tb.hi, tb.lo);
+  return p.scale * p.poly;
 }
 
-// Token of value i of a lane's 32 in a block.
+// 16 logits of a lane in a block of 512: fp32 bits.
 template <bool BF16>
-__device__ __forceinline__ int place(int i, int lane) {
-  return BF16 ? ((i >> 3) * 32 + lane) * 8 + (i & 7) : ((i >> 2) * 32 + lane) * 4 + (i & 3);
-}
-
-// 32 logits of the block [s, s + BLOCK) per lane; tokens from `end` on are -inf.
-template <bool BF16>
-__device__ __forceinline__ void load_block(const void* row, int s, int end, bool aligned, int lane, float (&v)[32]) {
-  if (aligned && s + BLOCK <= end) {
+struct Lane {
+  static constexpr int VECS = BF16 ? 2 : 4;
+  uint4 v[VECS];
+  __device__ __forceinline__ void load(const void* row, int s, int lane) {
+    const uint4* p = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(row) + (int64_t)s * (BF16 ? 2 : 4)) + lane;
+#pragma unroll
+    for (int i = 0; i < VECS; ++i) v[i] = __ldg(p + i * 32);
+  }
+  // fp32 bits of value i
+  __device__ __forceinline__ uint32_t bits(int i) const {
     if constexpr (BF16) {
-      const uint4* p = reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(row) + s) + lane;
-      uint4 x[4];
-#pragma unroll
-      for (int q = 0; q < 4; ++q) x[q] = __ldg(p + q * 32);
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        float f[8];
-        bf16x8_to_f32(x[q], f);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[q * 8 + e] = fmaxf(f[e], NEG);
-      }
+      const uint4& q = v[i >> 3];
+      const uint32_t w = (i & 7) < 2 ? q.x : (i & 7) < 4 ? q.y : (i & 7) < 6 ? q.z : q.w;
+      return i & 1 ? w & 0xffff0000u : w << 16;
     } else {
-      const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(row) + s) + lane;
-#pragma unroll
-      for (int q = 0; q < 8; ++q) {
-        const float4 x = __ldg(p + q * 32);
-        v[q * 4] = fmaxf(x.x, NEG);
-        v[q * 4 + 1] = fmaxf(x.y, NEG);
-        v[q * 4 + 2] = fmaxf(x.z, NEG);
-        v[q * 4 + 3] = fmaxf(x.w, NEG);
-      }
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 32; ++i) {
-      const int x = s + place<BF16>(i, lane);
-      v[i] = x < end ? logit_at<BF16>(row, x) : NEG;
+      const uint4& q = v[i >> 2];
+      return (i & 3) == 0 ? q.x : (i & 3) == 1 ? q.y : (i & 3) == 2 ? q.z : q.w;
     }
   }
-}
+  __device__ __forceinline__ static int place(int i, int lane) {  // token of value i in the block
+    return BF16 ? ((i >> 3) * 32 + lane) * 8 + (i & 7) : ((i >> 2) * 32 + lane) * 4 + (i & 3);
+  }
+  // NaN to -inf
+  __device__ __forceinline__ void clean() {
+#pragma unroll
+    for (int k = 0; k < VECS; ++k) {
+      uint32_t* w = reinterpret_cast<uint32_t*>(&v[k]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if constexpr (BF16) {
+          const uint32_t neg = 0xff80ff80u;
+          __nv_bfloat162 m = __hmax2(*reinterpret_cast<__nv_bfloat162*>(&w[e]), *reinterpret_cast<const __nv_bfloat162*>(&neg));
+          w[e] = *reinterpret_cast<uint32_t*>(&m);
+        } else {
+          w[e] = __float_as_uint(fmaxf(__uint_as_float(w[e]), NEG));
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ float max() const {
+    if constexpr (BF16) {
+      __nv_bfloat162 m[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        m[e] = __hmax2(reinterpret_cast<const __nv_bfloat162*>(&v[0])[e], reinterpret_cast<const __nv_bfloat162*>(&v[1])[e]);
+      m[0] = __hmax2(__hmax2(m[0], m[1]), __hmax2(m[2], m[3]));
+      return fmaxf(__low2float(m[0]), __high2float(m[0]));
+    } else {
+      float m = NEG;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) m = fmaxf(m, __uint_as_float(bits(i)));
+      return m;
+    }
+  }
+};
 
 __device__ __forceinline__ double warp_sum64(double v) {
 #pragma unroll
@@ -128,65 +194,73 @@ struct Cut {
   int head, len, count, V;
   __device__ __forceinline__ int begin(int k) const { return k ? head + k * len : 0; }
   __device__ __forceinline__ int end(int k) const { return min(V, head + (k + 1) * len); }
+  // one aligned block
+  __device__ __forceinline__ bool block(int k) const { return len == BLOCK && (k || !head) && begin(k) + BLOCK <= V; }
 };
 
-// f(block start, block end, aligned) over the blocks of chunk k.
-template <typename F>
-__device__ __forceinline__ void blocks_of(const Cut& cut, int k, F&& f) {
-  int s = cut.begin(k);
-  const int end = cut.end(k);
-  if (k == 0 && cut.head) {
-    f(0, min(cut.head, end), false);
-    s = cut.head;
+// Sum over an aligned block of exp((l - m) / T) and m, its maximum; at T <= 0 the first maximum alone.
+template <bool BF16>
+__device__ __forceinline__ ChunkSum sum_block(Lane<BF16>& x, int s, const Dist& d, const Tables& tb, int lane) {
+  x.clean();
+  ChunkSum out;
+  out.max = warp_max(x.max());
+  out.sum = 0.0;
+  out.first = 0x7fffffff;
+  if (out.max == NEG) return out;
+  if (d.greedy) {
+    int at = 0x7fffffff;
+#pragma unroll
+    for (int i = 15; i >= 0; --i)
+      if (__uint_as_float(x.bits(i)) == out.max) at = s + Lane<BF16>::place(i, lane);
+    out.first = __reduce_min_sync(FULL_MASK, at);
+    return out;
   }
-  for (; s < end; s += BLOCK) f(s, end, true);
+  double sum[4] = {0.0, 0.0, 0.0, 0.0};
+  if (out.max < INFINITY && d.plain(out.max)) {
+    const double mc = -(double)out.max * d.c;
+#pragma unroll
+    for (int i = 0; i < 16; i += 4) {
+      double z[4], scale[4], poly[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) z[e] = fma(wide(x.bits(i + e)), d.c, mc);
+      power4(z, tb.hi, tb.lo, scale, poly);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sum[e] = fma(scale[e], poly[e], sum[e]);
+    }
+  } else {
+#pragma unroll 1
+    for (int i = 0; i < 16; ++i) {
+      uint32_t b = 0;
+#pragma unroll
+      for (int k = 0; k < 16; ++k)
+        if (k == i) b = x.bits(k);
+      sum[0] += weight(__uint_as_float(b), out.max, d.c, tb);
+    }
+  }
+  out.sum = warp_sum64((sum[0] + sum[1]) + (sum[2] + sum[3]));
+  return out;
 }
 
-// Sum over chunk k of exp((l - m) / T) and m, its maximum; at T <= 0 the first maximum alone.
+// The same for a chunk of any place and length, token by token.
 template <bool BF16>
-__device__ ChunkSum sum_chunk(const void* row, const Cut& cut, int k, const Dist& d, const Exp2& ex, int lane) {
-  float m = NEG;
-  double sum = 0.0;
-  int first = 0x7fffffff;
-  blocks_of(cut, k, [&](int s, int end, bool aligned) {
-    float v[32];
-    load_block<BF16>(row, s, end, aligned, lane, v);
-    float bm = v[0];
-#pragma unroll
-    for (int i = 1; i < 32; ++i) bm = fmaxf(bm, v[i]);
-    bm = warp_max(bm);
-    const float nm = fmaxf(m, bm);
-    if (nm == NEG) return;
-    if (d.greedy) {
-      if (bm > m) {  // an earlier block keeps an equal maximum
-        int at = 0x7fffffff;
-#pragma unroll
-        for (int i = 31; i >= 0; --i)
-          if (v[i] == bm) at = s + place<BF16>(i, lane);
-        first = __reduce_min_sync(FULL_MASK, at);
-      }
-      m = nm;
-      return;
-    }
-    if (nm == INFINITY) {
-      if (m < nm) sum = 0.0;
-#pragma unroll
-      for (int i = 0; i < 32; ++i) sum += v[i] == INFINITY ? 1.0 : 0.0;
-      m = nm;
-      return;
-    }
-    const double top = (double)nm;
-    if (m != NEG && nm > m) sum = ex.fma_to(((double)m - top) * d.c256, 0.0) * sum;
-    double part = 0.0;
-#pragma unroll
-    for (int i = 0; i < 32; ++i) part = ex.fma_to(((double)v[i] - top) * d.c256, part);
-    sum += part;
-    m = nm;
-  });
+__device__ ChunkSum sum_tokens(const void* row, int s, int end, const Dist& d, const Tables& tb, int lane) {
   ChunkSum out;
-  out.sum = d.greedy ? 0.0 : warp_sum64(sum);
-  out.max = m;
-  out.first = first;
+  float m = NEG;
+  for (int x = s + lane; x < end; x += 32) m = fmaxf(m, logit_at<BF16>(row, x));
+  out.max = m = warp_max(m);
+  int at = 0x7fffffff;
+  double sum = 0.0;
+  if (m > NEG)
+    for (int x = s + lane; x < end; x += 32) {
+      const float l = logit_at<BF16>(row, x);
+      if (d.greedy) {
+        if (l == m) at = min(at, x);
+      } else {
+        sum += weight(l, m, d.c, tb);
+      }
+    }
+  out.first = __reduce_min_sync(FULL_MASK, at);
+  out.sum = warp_sum64(sum);
   return out;
 }
 
@@ -212,8 +286,8 @@ __device__ __forceinline__ double left_of(double p, double q, const Residual& r)
 }
 
 template <bool BF16>
-__device__ double left_at(const void* row, int x, const Dist& d, const Exp2& ex, const Residual& r) {
-  const double p = weight(logit_at<BF16>(row, x), d, ex) * d.inv_sum;
+__device__ double left_at(const void* row, int x, const Dist& d, const Tables& tb, const Residual& r) {
+  const double p = weight(logit_at<BF16>(row, x), d.max, d.c, tb) * d.inv_sum;
   if (!r.draft) {
     for (int i = 0; i < r.k; ++i)
       if (r.gone[i] == x) return 0.0;
@@ -223,54 +297,80 @@ __device__ double left_at(const void* row, int x, const Dist& d, const Exp2& ex,
 }
 
 template <bool BF16>
-__device__ ChunkSum sum_residual(const void* row, const Cut& cut, int k, const Dist& d, const Exp2& ex,
-                                 const Residual& r, int lane) {
+__device__ double left_tokens(const void* row, int s, int end, const Dist& d, const Tables& tb, const Residual& r, int lane) {
   double sum = 0.0;
-  blocks_of(cut, k, [&](int s, int end, bool aligned) {
-    float v[32];
-    load_block<BF16>(row, s, end, aligned, lane, v);
-#pragma unroll 8
-    for (int i = 0; i < 32; ++i) {
-      const int x = s + place<BF16>(i, lane);
-      if (x < end) sum += left_of(weight(v[i], d, ex) * d.inv_sum, draft_at(r, x), r);
+  for (int x = s + lane; x < end; x += 32) sum += left_at<BF16>(row, x, d, tb, r);
+  return warp_sum64(sum);
+}
+
+// Mass of the residual over an aligned block; tb: the table times 1 / sum.
+template <bool BF16>
+__device__ __forceinline__ double left_block(Lane<BF16>& x, const float (&q)[16], const Dist& d, const Tables& tb,
+                                             const Residual& r) {
+  x.clean();
+  const double mc = -(double)d.max * d.c;
+  double sum[4] = {0.0, 0.0, 0.0, 0.0};
+#pragma unroll
+  for (int i = 0; i < 16; i += 4) {
+    double z[4], scale[4], poly[4], qd[4];
+    bool none[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      z[e] = fma(wide(x.bits(i + e)), d.c, mc);
+      none[e] = (unsigned)__double2hiint(z[e]) > SPAN;
+      qd[e] = q[i + e] > 0.f ? wide(__float_as_uint(q[i + e])) : 0.0;
     }
-  });
-  ChunkSum out;
-  out.sum = warp_sum64(sum);
-  out.max = 0.f;
-  out.first = 0;
-  return out;
+    power4(z, tb.hi, tb.lo, scale, poly);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      scale[e] = fma(scale[e], poly[e], -qd[e]);
+      scale[e] = __double2hiint(scale[e]) < 0 || none[e] ? 0.0 : scale[e];
+    }
+    for (int k = 1; k < r.k; ++k) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        scale[e] = fma(scale[e], r.inv_mass[k - 1], -qd[e]);
+        scale[e] = __double2hiint(scale[e]) < 0 ? 0.0 : scale[e];
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sum[e] += scale[e];
+  }
+  return (sum[0] + sum[1]) + (sum[2] + sum[3]);
 }
 
 enum Action { DRAW = 0, GO = 1, RESIDUAL = 2 };
 
 struct Shared {
   ChunkSum chunk[2][MAX_CHUNKS];
-  double table[256];
+  uint32_t hi[32], lo[32];      // 2^(j / 32)
+  uint32_t r_hi[32], r_lo[32];  // times 1 / sum
   double mass[TREE_MAX_NODES];      // of the residual after i rejections (0: the distribution itself, 1)
   double inv_mass[TREE_MAX_NODES];  // [i]: 1 / mass[i + 1]
-  double scan[VWARPS];
+  double scan[16];
   double now;    // mass at hand
-  double share;  // of the draw: what the cumulative sum has to pass
-  Dist dist;
-  int parent[TREE_MAX_NODES], token[TREE_MAX_NODES], gone[TREE_MAX_NODES];
+  double share, ahead;  // of the draw: what the cumulative sum has to pass, and the sum ahead of the chunk
+  float wmax[16];
+  int wfirst[16];
+  int parent[TREE_MAX_NODES], token[TREE_MAX_NODES], gone[TREE_MAX_NODES], kid[TREE_MAX_NODES];
   float u[TREE_MAX_NODES];
   int action, child, rejected;
+  int at;        // the next child to try
   int summed;  // rejections that the chunk sums at hand stand for
   int best;    // first maximum of the row
   int found, held, drawn_chunk;
 };
 
 // Sum of a chunk in units of the row's maximum.
-__device__ __forceinline__ double scaled(const ChunkSum& c, const Dist& d, const Exp2& ex) {
-  if (c.max == NEG) return 0.0;
-  if (c.max == d.max) return c.sum;
-  if (d.max == INFINITY) return 0.0;
-  return ex.fma_to(((double)c.max - (double)d.max) * d.c256, 0.0) * c.sum;
+__device__ __forceinline__ double scaled(const ChunkSum& c, const Dist& d, const Tables& tb) {
+  if (c.max == d.max) return c.sum;  // (an empty row's, too)
+  return weight(c.max, d.max, d.c, tb) * c.sum;
 }
 
-template <bool BF16>
-__global__ void __launch_bounds__(VT, 2) tree_verify_kernel(TreeVerify a, int len) {
+// 512 threads and one CTA per SM while the trees are fewer than the SMs, else 256 threads and two or three CTAs.
+template <bool BF16, int VT>
+__global__ void __launch_bounds__(VT, VT == 512 ? 1 : BF16 ? 3 : 2) tree_verify_kernel(TreeVerify a, int len) {
+  constexpr int VWARPS = VT / 32;
   pdl_wait();     // inputs come from the previous kernel in the stream
   pdl_trigger();  // the next kernel may start its prologue
   extern __shared__ __align__(16) uint8_t vsm[];
@@ -297,13 +397,17 @@ __global__ void __launch_bounds__(VT, 2) tree_verify_kernel(TreeVerify a, int le
     sh.token[i] = a.tokens[t0 + i];
     sh.u[i] = a.u[t0 + i];
   }
-  for (int i = threadIdx.x; i < 256; i += VT) sh.table[i] = exp2(i / 256.0);
-  const Exp2 ex{sh.table};
+  if (threadIdx.x < 32) {
+    const double e = exp2(threadIdx.x / 32.0);
+    sh.hi[threadIdx.x] = (uint32_t)__double2hiint(e);
+    sh.lo[threadIdx.x] = (uint32_t)__double2loint(e);
+  }
+  const Tables tb{sh.hi, sh.lo}, scaled_tb{sh.r_hi, sh.r_lo};
   const float temp = a.temps[b];
   Dist d;
   d.greedy = !(temp > 0.f);
   // above 0 at an infinite temperature too, where -inf still has no weight
-  d.c256 = d.greedy ? 0.0 : fmax(256.0 * 1.4426950408889634074 / (double)temp, 1e-300);
+  d.c = d.greedy ? 0.0 : fmax(32.0 * 1.4426950408889634074 / (double)temp, 1e-300);
   d.inv_sum = 0.0;
   d.max = NEG;
   Residual left;
@@ -318,16 +422,49 @@ __global__ void __launch_bounds__(VT, 2) tree_verify_kernel(TreeVerify a, int le
   cut.V = a.V;
   cut.len = len;
 
-  // The chunk sums, in the shared memory of every CTA.
+  // The chunk sums, in the shared memory of every CTA.  A warp's next block is on its way while it works on one.
   auto pass = [&](bool residual) -> ChunkSum* {
     ChunkSum* to = sh.chunk[phase & 1];
-    for (int k = cta * VWARPS + warp; k < cut.count; k += ctas * VWARPS) {
-      const ChunkSum c =
-          residual ? sum_residual<BF16>(row, cut, k, d, ex, left, lane) : sum_chunk<BF16>(row, cut, k, d, ex, lane);
+    const int stride = ctas * VWARPS;
+    const bool fast_q = residual && d.plain(d.max) && d.max < INFINITY;
+    Lane<BF16> x, nx;
+    int k = cta * VWARPS + warp;
+    if (k < cut.count && cut.block(k)) x.load(row, cut.begin(k), lane);
+    for (; k < cut.count; k += stride) {
+      const int s = cut.begin(k), end = cut.end(k), nk = k + stride;
+      if (nk < cut.count && cut.block(nk)) nx.load(row, cut.begin(nk), lane);
+      ChunkSum c;
+      if (!residual) {
+        c = cut.block(k) ? sum_block<BF16>(x, s, d, tb, lane) : sum_tokens<BF16>(row, s, end, d, tb, lane);
+      } else {
+        if (fast_q && cut.block(k)) {
+          float q[16];
+          const float* qr = left.draft + s;
+          if ((reinterpret_cast<uintptr_t>(qr) & 15) == 0) {
+#pragma unroll
+            for (int i = 0; i < 16; i += 4) {
+              const float4 f = __ldg(reinterpret_cast<const float4*>(qr + Lane<BF16>::place(i, lane)));
+              q[i] = f.x;
+              q[i + 1] = f.y;
+              q[i + 2] = f.z;
+              q[i + 3] = f.w;
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) q[i] = __ldg(qr + Lane<BF16>::place(i, lane));
+          }
+          c.sum = warp_sum64(left_block<BF16>(x, q, d, scaled_tb, left));
+        } else {
+          c.sum = left_tokens<BF16>(row, s, end, d, tb, left, lane);
+        }
+        c.max = 0.f;
+        c.first = 0;
+      }
       if (lane < (int)ctas)
         asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(tc::cluster_map(smem_u32(to + k), lane)),
                      "r"(__double2loint(c.sum)), "r"(__double2hiint(c.sum)), "r"(__float_as_int(c.max)), "r"(c.first)
                      : "memory");
+      x = nx;
     }
     // the other buffer is written from here on, which every CTA has read before it came to this barrier
     tc::cluster_arrive();
@@ -335,22 +472,38 @@ __global__ void __launch_bounds__(VT, 2) tree_verify_kernel(TreeVerify a, int le
     ++phase;
     return to;
   };
-  // The first child of `node` from index `from` on, or n.  All lanes of a warp.
-  auto next_child = [&](int from) {
-    for (int i = from; i < n; i += 32) {
-      const unsigned hit = __ballot_sync(FULL_MASK, i + lane < n && sh.parent[i + lane] == node);
-      if (hit) return i + __ffs(hit) - 1;
+  // First warp: the children of `node` in sh.kid; lane i holds child i's logit and draft probability, whose loads run
+  // beside the pass over the row, and later its probability.
+  int kids = 0;
+  uint32_t kid_raw = 0;  // as loaded: nothing waits for it before it is used
+  float kid_draft = 0.f;
+  bool kid_in = false;
+  double kid_p = 0.0;
+  auto find_children = [&]() {
+    kids = 0;
+    for (int i = (node + 1) & ~31; i < n; i += 32) {
+      const bool hit = i + lane > node && i + lane < n && sh.parent[i + lane] == node;
+      const unsigned all = __ballot_sync(FULL_MASK, hit);
+      if (hit) sh.kid[kids + __popc(all & ((1u << lane) - 1))] = i + lane;
+      kids += __popc(all);
     }
-    return n;
+    __syncwarp();
+    kid_draft = 0.f;
+    const int x = lane < kids ? sh.token[sh.kid[lane]] : -1;
+    kid_in = x >= 0 && x < a.V;
+    if (kid_in) {
+      kid_raw = BF16 ? __ldg(static_cast<const unsigned short*>(row) + x) : __ldg(static_cast<const unsigned*>(row) + x);
+      if (left.draft) kid_draft = __ldg(left.draft + x);
+    }
   };
-  // Tries children from sh.child on until one is taken, a residual is needed or none is left (first warp, with
-  // the same numbers in every lane and every CTA).
+  // First warp: tries children from sh.at on until one is taken, a residual is needed or none is left (with the same
+  // numbers in every lane and every CTA).
   auto try_children = [&]() {
-    int child = sh.child, rejected = sh.rejected, action = DRAW;
+    int at = sh.at, rejected = sh.rejected, action = DRAW;
     double mass = sh.now;
     __syncwarp();
-    for (child = next_child(child); child < n; child = next_child(child + 1)) {
-      const int x = sh.token[child];
+    for (; at < kids; ++at) {
+      const int child = sh.kid[at], x = sh.token[child];
       const bool in = x >= 0 && x < a.V;
       if (d.greedy) {
         if (in && x == sh.best) {
@@ -359,9 +512,21 @@ __global__ void __launch_bounds__(VT, 2) tree_verify_kernel(TreeVerify a, int le
         }
         continue;
       }
+      double p = 0.0, q = 1.0;
+      if (at < 32) {
+        p = __shfl_sync(FULL_MASK, kid_p, at);
+        const float f = __shfl_sync(FULL_MASK, kid_draft, at);
+        if (left.draft) q = f > 0.f ? (double)f : 0.0;
+      } else if (in) {
+        p = weight(logit_at<BF16>(row, x), d.max, d.c, tb) * d.inv_sum;
+        if (left.draft) q = draft_at(left, x);
+      }
       left.k = rejected;
-      const double p = in ? left_at<BF16>(row, x, d, ex, left) : 0.0;
-      const double q = !left.draft ? 1.0 : in ? draft_at(left, x) : 0.0;
+      if (left.draft)
+        p = left_of(p, q, left);
+      else
+        for (int i = 0; i < rejected; ++i)
+          if (sh.gone[i] == x) p = 0.0;
       if (in && (double)sh.u[child] * q * mass < p) {
         action = GO;
         break;
@@ -369,7 +534,7 @@ __global__ void __launch_bounds__(VT, 2) tree_verify_kernel(TreeVerify a, int le
       if (left.draft) {
         if (mass > 0.0) {  // nothing is left to take q from otherwise
           ++rejected;
-          ++child;
+          ++at;
           action = RESIDUAL;
           break;
         }
@@ -381,7 +546,8 @@ __global__ void __launch_bounds__(VT, 2) tree_verify_kernel(TreeVerify a, int le
       }
     }
     if (lane == 0) {
-      sh.child = child;
+      sh.at = at;
+      sh.child = action == GO ? sh.kid[at] : -1;
       sh.rejected = rejected;
       sh.now = mass;
       sh.action = action;
@@ -398,42 +564,65 @@ __global__ void __launch_bounds__(VT, 2) tree_verify_kernel(TreeVerify a, int le
     cut.head = (int)((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / E;
     cut.count = a.V <= cut.head + len ? 1 : (a.V - cut.head + len - 1) / len;
     __syncthreads();  // the table (first node); every thread has read the last node's decision
+    if (warp == 0) find_children();
     sums = pass(false);
+    // the row's maximum and sum, by all threads, the same numbers in each
+    float m = NEG;
+    for (int k = threadIdx.x; k < cut.count; k += VT) m = fmaxf(m, sums[k].max);
+    m = warp_max(m);
+    if (lane == 0) sh.wmax[warp] = m;
+    __syncthreads();
+    d.max = NEG;
+#pragma unroll
+    for (int w = 0; w < VWARPS; ++w) d.max = fmaxf(d.max, sh.wmax[w]);
+    double total = 0.0;
+    int first = 0x7fffffff;
+    for (int k = threadIdx.x; k < cut.count; k += VT) {
+      total += scaled(sums[k], d, tb);
+      if (sums[k].max == d.max) first = min(first, sums[k].first);
+    }
+    total = warp_sum64(total);
+    first = __reduce_min_sync(FULL_MASK, first);
+    if (lane == 0) {
+      sh.scan[warp] = total;
+      sh.wfirst[warp] = first;
+    }
+    __syncthreads();
+    total = 0.0;
+#pragma unroll
+    for (int w = 0; w < VWARPS; ++w) {
+      total += sh.scan[w];
+      first = min(first, sh.wfirst[w]);
+    }
+    d.inv_sum = total > 0.0 ? 1.0 / total : 0.0;
     if (warp == 0) {
-      float m = NEG;
-      int first = 0x7fffffff;
-      for (int k = lane; k < cut.count; k += 32) {
-        const ChunkSum c = sums[k];
-        if (c.max > m) {
-          m = c.max;
-          first = c.first;
-        }
-      }
-      d.max = warp_max(m);
-      first = __reduce_min_sync(FULL_MASK, m == d.max ? first : 0x7fffffff);
-      double total = 0.0;
-      for (int k = lane; k < cut.count; k += 32) total += scaled(sums[k], d, ex);
-      total = warp_sum64(total);
-      d.inv_sum = total > 0.0 ? 1.0 / total : 0.0;
       if (lane == 0) {
-        sh.dist = d;
         sh.best = d.max == NEG ? -1 : first;
         sh.now = sh.mass[0] = total > 0.0 ? 1.0 : 0.0;
-        sh.rejected = sh.summed = 0;
-        sh.child = node + 1;
+        sh.rejected = sh.summed = sh.at = 0;
+      }
+      if (!d.greedy) kid_p = weight(kid_in ? raw_logit<BF16>(kid_raw) : NEG, d.max, d.c, tb) * d.inv_sum;
+      if (left.draft) {
+        const double e = __hiloint2double((int)tb.hi[lane], (int)tb.lo[lane]) * d.inv_sum;
+        sh.r_hi[lane] = (uint32_t)__double2hiint(e);
+        sh.r_lo[lane] = (uint32_t)__double2loint(e);
       }
       __syncwarp();
       try_children();
     }
     __syncthreads();
-    d = sh.dist;
     while (sh.action == RESIDUAL) {
       left.k = sh.rejected;
       sums = pass(true);
+      double part = 0.0;
+      for (int k = threadIdx.x; k < cut.count; k += VT) part += sums[k].sum;
+      part = warp_sum64(part);
+      if (lane == 0) sh.scan[warp] = part;
+      __syncthreads();
       if (warp == 0) {
         double m = 0.0;
-        for (int k = lane; k < cut.count; k += 32) m += sums[k].sum;
-        m = warp_sum64(m);
+#pragma unroll
+        for (int w = 0; w < VWARPS; ++w) m += sh.scan[w];
         if (lane == 0) {
           const int k = left.k;
           if (m > 0.0) {
@@ -468,63 +657,66 @@ __global__ void __launch_bounds__(VT, 2) tree_verify_kernel(TreeVerify a, int le
     return;
   }
   // ---- the draw: the chunk in which the cumulative sum passes the share, then the token in it
+  if (!left.draft || left.k == 0)
+    for (int k = threadIdx.x; k < cut.count; k += VT) sums[k].sum = scaled(sums[k], d, tb) * d.inv_sum;
+  __syncthreads();
+  if (!left.draft) {
+    for (int i = warp; i < left.k; i += VWARPS) {  // a rejected token's chunk is summed again without it
+      const int k = sh.gone[i] < cut.head ? 0 : (sh.gone[i] - cut.head) / len;
+      const double part = left_tokens<BF16>(row, cut.begin(k), cut.end(k), d, tb, left, lane);
+      if (lane == 0) sums[k].sum = part;
+    }
+    __syncthreads();
+  }
   if (warp == 0) {
-    if (!left.draft || left.k == 0)
-      for (int k = lane; k < cut.count; k += 32) sums[k].sum = scaled(sums[k], d, ex) * d.inv_sum;
-    __syncwarp();
-    if (!left.draft)
-      for (int i = 0; i < left.k; ++i) {  // a rejected token's chunk is summed again without it
-        const int k = sh.gone[i] < cut.head ? 0 : (sh.gone[i] - cut.head) / len;
-        double part = 0.0;
-        for (int x = cut.begin(k) + lane; x < cut.end(k); x += 32) part += left_at<BF16>(row, x, d, ex, left);
-        part = warp_sum64(part);
-        if (lane == 0) sums[k].sum = part;
-        __syncwarp();
-      }
-    double carry = 0.0;
-    for (int k0 = 0; k0 < cut.count; k0 += 32) {
-      double v = k0 + lane < cut.count ? sums[k0 + lane].sum : 0.0;
+    // a lane takes consecutive chunks
+    const int per = (cut.count + 31) / 32, k0 = min(cut.count, lane * per), k1 = min(cut.count, k0 + per);
+    double mine = 0.0;
+    for (int k = k0; k < k1; ++k) mine += sums[k].sum;
+    double upto = mine;
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const double up = __shfl_up_sync(FULL_MASK, v, o);
-        if (lane >= o) v += up;
-      }
-      v += carry;
-      if (k0 + lane < cut.count) sums[k0 + lane].sum = v;
-      carry = __shfl_sync(FULL_MASK, v, 31);
+    for (int o = 1; o < 32; o <<= 1) {
+      const double up = __shfl_up_sync(FULL_MASK, upto, o);
+      if (lane >= o) upto += up;
     }
-    __syncwarp();
+    const double total = __shfl_sync(FULL_MASK, upto, 31);
     const float u = a.u_draw[b];
-    const double share = (double)(u > 0.f ? fminf(u, 1.f) : 0.f) * carry;
-    int at = -1, held = -1;
-    for (int k0 = 0; k0 < cut.count && at < 0; k0 += 32) {
-      const int k = k0 + lane;
-      const double v = k < cut.count ? sums[k].sum : 0.0, before = k && k < cut.count ? sums[k - 1].sum : 0.0;
-      const unsigned above = __ballot_sync(FULL_MASK, k < cut.count && v > share);
-      const unsigned any = __ballot_sync(FULL_MASK, k < cut.count && v > before);
-      if (any) held = k0 + 31 - __clz(any);
-      if (above) at = k0 + __ffs(above) - 1;
-    }
+    const double share = (double)(u > 0.f ? fminf(u, 1.f) : 0.f) * total;
+    const unsigned above = __ballot_sync(FULL_MASK, mine > 0.0 && upto > share), any = __ballot_sync(FULL_MASK, mine > 0.0);
     if (lane == 0) {
-      sh.share = share;
-      sh.drawn_chunk = at >= 0 ? at : held;
       sh.found = 0x7fffffff;
       sh.held = -1;
+      if (!any) sh.drawn_chunk = -1;  // no logit above -inf
+    }
+    if (any && lane == (above ? __ffs(above) - 1 : 31 - __clz(any))) {
+      double sum = upto - mine;
+      int at = -1;
+      double ahead = 0.0;
+      for (int k = k0; k < k1; ++k) {
+        if (sums[k].sum > 0.0) {
+          at = k;  // the last one with any mass where rounding leaves none above the share
+          ahead = sum;
+        }
+        sum += sums[k].sum;
+        if (above && sums[k].sum > 0.0 && sum > share) break;
+      }
+      sh.drawn_chunk = at;
+      sh.ahead = ahead;
+      sh.share = share;
     }
   }
   __syncthreads();
   const int k = sh.drawn_chunk;
-  if (k < 0) {  // no logit above -inf
+  if (k < 0) {
     if (threadIdx.x == 0) a.next_token[b] = 0;
     return;
   }
-  double before = k ? sums[k - 1].sum : 0.0;
+  double before = sh.ahead;
   const double share = sh.share;
-  for (int s = cut.begin(k); s < cut.end(k); s += 2 * VT) {
-    const int x = s + 2 * threadIdx.x, end = cut.end(k);
-    const double v0 = x < end ? left_at<BF16>(row, x, d, ex, left) : 0.0;
-    const double v1 = x + 1 < end ? left_at<BF16>(row, x + 1, d, ex, left) : 0.0;
-    double sum = v0 + v1;
+  for (int s = cut.begin(k); s < cut.end(k); s += VT) {
+    const int x = s + threadIdx.x;
+    const double v = x < cut.end(k) ? left_at<BF16>(row, x, d, tb, left) : 0.0;
+    double sum = v;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const double up = __shfl_up_sync(FULL_MASK, sum, o);
@@ -537,14 +729,8 @@ __global__ void __launch_bounds__(VT, 2) tree_verify_kernel(TreeVerify a, int le
       if (w < warp) ahead += sh.scan[w];
       before += sh.scan[w];
     }
-    const double c1 = ahead + sum, c0 = c1 - v1;
-    int at = 0x7fffffff, held = -1;
-    if (v1 > 0.0 && c1 > share) at = x + 1;
-    if (v0 > 0.0 && c0 > share) at = x;
-    if (v0 > 0.0) held = x;
-    if (v1 > 0.0) held = x + 1;
-    at = __reduce_min_sync(FULL_MASK, at);
-    held = __reduce_max_sync(FULL_MASK, held);
+    const int at = __reduce_min_sync(FULL_MASK, v > 0.0 && ahead + sum > share ? x : 0x7fffffff);
+    const int held = __reduce_max_sync(FULL_MASK, v > 0.0 ? x : -1);
     if (lane == 0) {
       atomicMin(&sh.found, at);
       atomicMax(&sh.held, held);
@@ -553,27 +739,33 @@ __global__ void __launch_bounds__(VT, 2) tree_verify_kernel(TreeVerify a, int le
     if (sh.found != 0x7fffffff) break;  // the same in every thread: written ahead of the barrier only
     __syncthreads();
   }
-  // the sums of the whole chunk may have been a rounding above those of its tokens
+  // the chunk's sum may have been a rounding above that of its tokens
   if (threadIdx.x == 0) a.next_token[b] = sh.found != 0x7fffffff ? sh.found : max(sh.held, 0);
 }
 
 }  // namespace
 
+static int tree_ctas = getenv("TREE_CTAS") ? atoi(getenv("TREE_CTAS")) : 0;
 cudaError_t launch_tree_verify(const TreeVerify& a, cudaStream_t stream) {
   if (a.num_seqs <= 0 || a.V <= 0 || a.max_nodes < 1 || a.max_nodes > TREE_MAX_NODES) return cudaErrorInvalidValue;
   int len = BLOCK;
   while ((int64_t)len * (MAX_CHUNKS - 1) < a.V) len *= 2;
-  // CTAs per tree: as many as keep every cluster resident at two CTAs per SM, at least eight chunks for each
+  // CTAs per tree, no more than have a chunk per warp.  Few trees: all SMs, one CTA of 512 threads on each.  Many:
+  // eight smaller CTAs, although that takes several rounds of clusters: walks differ in length, and the longest one of
+  // 256 trees on a CTA each was what the call took (256 x 8 nodes, 151936 tokens: 470 us; 2, 4, 8 CTAs: see below).
+  const bool many = a.num_seqs * 16 > 148;
+  const int vt = many ? 256 : 512, most = tree_ctas > 0 ? tree_ctas : many ? 8 : 16;
   const int chunks = (a.V + len - 1) / len;
   int ctas = 1;
-  while (ctas < 16 && (int64_t)a.num_seqs * ctas * 2 <= 2 * 148 && ctas * 2 * 8 <= chunks) ctas *= 2;
-  auto kern = a.logits_bf16 ? tree_verify_kernel<true> : tree_verify_kernel<false>;
-  static std::atomic<uint64_t> done[2] = {{0}, {0}};
-  cudaError_t e = smem_opt_in(done[a.logits_bf16 ? 1 : 0], kern, (int)sizeof(Shared), true);
+  while (ctas < most && ctas * (vt / 32) < chunks) ctas *= 2;
+  auto kern = a.logits_bf16 ? (many ? tree_verify_kernel<true, 256> : tree_verify_kernel<true, 512>)
+                            : (many ? tree_verify_kernel<false, 256> : tree_verify_kernel<false, 512>);
+  static std::atomic<uint64_t> done[4] = {{0}, {0}, {0}, {0}};
+  cudaError_t e = smem_opt_in(done[(a.logits_bf16 ? 1 : 0) + (many ? 2 : 0)], kern, (int)sizeof(Shared), true);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)a.num_seqs * ctas);
-  cfg.blockDim = dim3(VT);
+  cfg.blockDim = dim3(vt);
   cfg.dynamicSmemBytes = sizeof(Shared);
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];

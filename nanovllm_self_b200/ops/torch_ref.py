@@ -343,7 +343,7 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
 
 def _tree_probs(row: torch.Tensor, temperature: float) -> torch.Tensor:
     """float64 probabilities of a row of logits; all zero where no logit is above -inf (a NaN counts as -inf; less than
-    2^-1000 of the largest as nothing).  A temperature that is not above 0 puts all of it on the first maximum."""
+    2^-900 of the largest as nothing).  A temperature that is not above 0 puts all of it on the first maximum."""
     z = row.double()
     z = torch.where(torch.isnan(z), float("-inf"), z)
     top = z.max()
@@ -354,7 +354,7 @@ def _tree_probs(row: torch.Tensor, temperature: float) -> torch.Tensor:
         p[int((z == top).int().argmax())] = 1.0
         return p
     w = (z == top).double() if top == float("inf") else torch.exp((z - top) / temperature)
-    w = torch.where(w < 2.0 ** -1000, 0.0, w)
+    w = torch.where(w < 2.0 ** -900, 0.0, w)
     return w / w.sum()
 
 
