@@ -234,14 +234,12 @@ __host__ __device__ constexpr int smem_bytes(int q_tiles, int slots, int raw_slo
   return q_tiles * TILE + slots * TILE + raw_slots * RAW_TILE + (int)sizeof(Small);
 }
 
-// e4m3 x 4 -> bf16 x 4, exactly: the bits of exponent and mantissa are shifted into place, and a product with 2^120
-// makes up for the exponents' difference (subnormals too).  A NaN becomes 480, which no e4m3 value is.
+// e4m3 x 4 -> bf16 x 4, exactly (4 significant bits; a NaN stays one), by f16 and fp32.
 __device__ __forceinline__ void e4m3x4_to_bf16(uint32_t x, uint32_t& lo, uint32_t& hi) {
-  uint32_t a = __byte_perm(x, 0, 0x1404), b = __byte_perm(x, 0, 0x3424);
-  a = (a & 0x80008000u) | ((a >> 4) & 0x07f007f0u);
-  b = (b & 0x80008000u) | ((b >> 4) & 0x07f007f0u);
-  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(lo) : "r"(a), "r"(0x7b807b80u));
-  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(hi) : "r"(b), "r"(0x7b807b80u));
+  float f[4];
+  e4m3x4_to_f32(x, f);
+  lo = pack_bf16(f[0], f[1]);
+  hi = pack_bf16(f[2], f[3]);
 }
 
 // A tile of e4m3 values (rows of 128 bytes) -> bf16 in a swizzled tile.  128 threads.
@@ -253,21 +251,15 @@ __device__ __forceinline__ void convert_tile(const uint8_t* src, uint8_t* dst, i
   for (int u = 0; u < 8; ++u) {
     const int idx = tid + u * 128, r = idx >> 3, i = idx & 7;  // 16 values of row r
     const uint32_t in[4] = {x[u].x, x[u].y, x[u].z, x[u].w};
-    uint32_t h[8], nan = 0;
+    uint32_t h[8];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      e4m3x4_to_bf16(in[e], h[2 * e], h[2 * e + 1]);
-      nan |= (in[e] & 0x7f7f7f7fu) + 0x01010101u;
-    }
-    if (nan & 0x80808080u) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        if ((h[e] & 0x7fffu) == 0x43f0u) h[e] |= 0x7fffu;  // 480
-        if ((h[e] & 0x7fff0000u) == 0x43f00000u) h[e] |= 0x7fff0000u;
-      }
-    }
-    *reinterpret_cast<uint4*>(dst + tile_at(r, 2 * i)) = make_uint4(h[0], h[1], h[2], h[3]);
-    *reinterpret_cast<uint4*>(dst + tile_at(r, 2 * i + 1)) = make_uint4(h[4], h[5], h[6], h[7]);
+    for (int e = 0; e < 4; ++e) e4m3x4_to_bf16(in[e], h[2 * e], h[2 * e + 1]);
+    // half of a row's eight lanes store their second 16 bytes first: the two halves of 64 dims lie in the same banks
+    // (a tile: 645 -> 400 clocks of stores and loads)
+    const int late = i >> 2;
+    uint4 v0 = make_uint4(h[0], h[1], h[2], h[3]), v1 = make_uint4(h[4], h[5], h[6], h[7]);
+    *reinterpret_cast<uint4*>(dst + tile_at(r, 2 * i + late)) = late ? v1 : v0;
+    *reinterpret_cast<uint4*>(dst + tile_at(r, 2 * i + 1 - late)) = late ? v0 : v1;
   }
 }
 
@@ -907,9 +899,14 @@ struct Few {  // shared memory besides the tiles
   int gave_up;
 };
 
-__host__ __device__ constexpr int few_bytes(int n, int slots, int raw_slots) {
-  return 2 * n * 256 + 2 * HALF + slots * TILE + raw_slots * RAW_TILE + (int)sizeof(Few);
-}
+// Buffers of Q and P: two each; e4m3, which needs the room for its 8-bit tiles: one of P, and with 64 rows one of Q.
+template <bool FP8, int N>
+struct Bufs {
+  static constexpr int Q = FP8 && N == 64 ? 1 : 2, P = FP8 ? 1 : 2;
+  __host__ __device__ static constexpr int bytes(int slots, int raw_slots) {
+    return Q * N * 256 + P * HALF + slots * TILE + raw_slots * RAW_TILE + (int)sizeof(Few);
+  }
+};
 
 __device__ __forceinline__ bool vote_any(bool p) {  // over the 128 softmax threads
   uint32_t r;
@@ -931,7 +928,7 @@ __device__ __forceinline__ float2 fms2(uint32_t a, uint32_t b, float f, float c,
 }
 
 template <bool FP8, int N>
-__global__ void __launch_bounds__(FP8 ? 384 : 256, 1)
+__global__ void __launch_bounds__(FP8 ? 512 : 256, 1)
     tree_attn_few_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, Args a) {
   pdl_wait();     // inputs come from the previous kernel in the stream
   pdl_trigger();  // the next kernel may start its prologue
@@ -941,9 +938,10 @@ __global__ void __launch_bounds__(FP8 ? 384 : 256, 1)
   const int S = a.slots, RS = a.raw_slots;
   uint8_t* ring = sm;
   uint8_t* pbuf = ring + S * TILE;
-  uint8_t* rawr = pbuf + 2 * HALF;
+  constexpr int QB = Bufs<FP8, N>::Q, PB = Bufs<FP8, N>::P;
+  uint8_t* rawr = pbuf + PB * HALF;
   uint8_t* sq = rawr + RS * RAW_TILE;
-  Few& sh = *reinterpret_cast<Few*>(sq + 2 * QT);
+  Few& sh = *reinterpret_cast<Few*>(sq + QB * QT);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   auto bar = [](uint64_t& b) { return smem_u32(&b); };
   if (smem_u32(sm) & 1023) {  // the swizzle goes by the address
@@ -979,6 +977,15 @@ __global__ void __launch_bounds__(FP8 ? 384 : 256, 1)
   volatile int* gave_up = &sh.gave_up;
   auto wait = [&](uint64_t& b, uint32_t parity, int code) { return warp_wait(bar(b), parity, &sh.gave_up, code); };
 
+  // e4m3: 512 threads begin with 128 registers each, of which the softmax warps take more: 216 + 72 + 2 x 104 < 4 x 128
+  if constexpr (FP8) {
+    if (warp < F_TMA)
+      regs_inc<216>();
+    else if (warp < F_CONV)
+      regs_dec<72>();
+    else
+      regs_dec<104>();
+  }
   if (warp < F_TMA) {
     // ------------------------------------------------------------------ softmax, outputs
     const int kq = threadIdx.x;  // TMEM lane: a key of the tile, a dim of the outputs
@@ -1120,8 +1127,9 @@ __global__ void __launch_bounds__(FP8 ? 384 : 256, 1)
             p[8 * c + (i >> 1)] = FP8 ? pack_bf16(y.x * vs, y.y * vs) : pack_bf16(y.x, y.y);
           }
         });
-        if (cnt >= 2) wait(sh.o_done[buf], ((cnt >> 1) - 1) & 1, 17);  // the product that read this buffer
-        uint8_t* pb = pbuf + buf * HALF;
+        // the product that read this buffer
+        if (cnt >= (uint32_t)PB) wait(sh.o_done[(cnt - PB) & 1], ((cnt - PB) >> 1) & 1, 17);
+        uint8_t* pb = pbuf + (PB == 2 ? buf : 0) * HALF;
 #pragma unroll
         for (int c = 0; c < N / 8; ++c)
           *reinterpret_cast<uint4*>(pb + tile_at(kq, c)) = make_uint4(p[4 * c], p[4 * c + 1], p[4 * c + 2], p[4 * c + 3]);
@@ -1289,8 +1297,8 @@ __global__ void __launch_bounds__(FP8 ? 384 : 256, 1)
     // ------------------------------------------------------------------ Q, two buffers
     int items = 0;
     for (Walk w(a, sh.spot); w.more(); w.next(a), ++items) {
-      const int qb = items & 1;
-      if (items > 1) wait(sh.q_empty[qb], ((items >> 1) - 1) & 1, 14);
+      const int qb = items % QB;
+      if (items >= QB) wait(sh.q_empty[qb], (items / QB - 1) & 1, 14);
       const int rows = w.rows(a), c = lane & 15;
       int r = lane >> 4, node = r / a.G, gh = r % a.G;
       const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(a.t.q) + (int64_t)seq_begin(a.t, w.b) * a.t.q_stride + (int64_t)w.h * a.G * AD + c * 8;
@@ -1339,7 +1347,7 @@ __global__ void __launch_bounds__(FP8 ? 384 : 256, 1)
       if (!ok) return;
       tc::fence_after();
       if (elect_one()) {
-        const uint64_t vd = ring_v + (uint64_t)p_at.s * (TILE >> 4), pd = p0 + (uint64_t)buf * (HALF >> 4);
+        const uint64_t vd = ring_v + (uint64_t)p_at.s * (TILE >> 4), pd = p0 + (uint64_t)(PB == 2 ? buf : 0) * (HALF >> 4);
 #pragma unroll
         for (int k = 0; k < 8; ++k)  // 16 keys
           tc::mma_bf16_ss(tmem + 128u + 64u * ob, vd + k * (16 * 128 >> 4), pd + k * (16 * 128 >> 4), id_o, !p_first || k > 0);
@@ -1349,7 +1357,7 @@ __global__ void __launch_bounds__(FP8 ? 384 : 256, 1)
       __syncwarp();
     };
     for (Walk w(a, sh.spot); w.more() && ok; w.next(a), ++items) {
-      const int qb = items & 1;
+      const int qb = items % QB;
       for (int t = w.t0; t < w.t1 && ok; ++t, ++cnt) {
         const int buf = cnt & 1;
         // the last tile's product goes first unless this tile's keys are there already
@@ -1357,7 +1365,7 @@ __global__ void __launch_bounds__(FP8 ? 384 : 256, 1)
         if (lane == 0) ready = tc::mbar_try(bar(sh.full[at.s]), at.ph);
         if (pending && !__shfl_sync(FULL_MASK, ready, 0)) product();
         if (!ok) break;
-        if (t == w.t0) ok = wait(sh.q_full[qb], (items >> 1) & 1, 2);
+        if (t == w.t0) ok = wait(sh.q_full[qb], (items / QB) & 1, 2);
         ok = ok && wait(sh.full[at.s], at.ph, 6);
         if (!ok) break;
         if (cnt >= 2) tc::fence_after();  // the buffer's last reader has announced its weights
@@ -1388,40 +1396,48 @@ __global__ void __launch_bounds__(FP8 ? 384 : 256, 1)
     if (lane == 0) tc::mbar_drain(bar(sh.drain), 0);
     __syncwarp();
   } else if (FP8 && warp >= F_CONV) {
-    // ------------------------------------------------------------------ e4m3 -> bf16 tiles
-    const int tid = threadIdx.x - F_CONV * 32;
+    // ------------------------------------------------------------------ e4m3 -> bf16 tiles: four warps for K, four for V
+    const int tid = (threadIdx.x - F_CONV * 32) & 127, kv = (warp - F_CONV) >> 2;
     Place from, to;
+    from.step(kv, RS);
+    to.step(kv, S);
     int tile = 0;
-    for (Walk w(a, sh.spot); w.more(); w.next(a)) {
-      const int* bt = a.t.block_tables + w.b * a.t.bt_stride;
-      for (int t = w.t0; t < w.t1; ++t, ++tile)
-        for (int kv = 0; kv < 2; ++kv) {
-          float2 sc = make_float2(0.f, 0.f);
-          if (kv == 0 && tid < KT / 16) {
-            const int bi = (t * KT + tid * 16) >> a.bs_shift;
-            const int blk = bi < a.t.W ? bt[bi] : -1;
-            if (blk >= 0 && blk < a.t.num_blocks) {
-              const int64_t k = (int64_t)blk * a.t.nkv + w.h;
-              sc = make_float2(a.t.k_scale[k], a.t.v_scale[k]);
-            }
-          }
-          wait(sh.raw_full[from.s], from.ph, 15);
-          wait(sh.empty[to.s], to.ph ^ 1, 16);
-          if (kv == 0 && tid < 32) {
-            if (tid < KT / 16) sh.scale[tile & 3][tid] = sc;
-            __syncwarp();
-            if (tid == 0) tc::mbar_arrive_release(bar(sh.scale_full[tile & 3]));
-          }
-          convert_tile(rawr + from.s * RAW_TILE, ring + to.s * TILE, tid);
-          tc::fence_proxy_async();
-          __syncwarp();
-          if (lane == 0) {
-            tc::mbar_arrive_release(bar(sh.full[to.s]));
-            tc::mbar_arrive_release(bar(sh.raw_empty[from.s]));
-          }
-          from.step(1, RS);
-          to.step(1, S);
+    // the scales of a tile, asked for while the one before is converted
+    auto scales = [&](const Walk& w, int t) {
+      float2 sc = make_float2(0.f, 0.f);
+      if (kv == 0 && tid < KT / 16) {
+        const int bi = (t * KT + tid * 16) >> a.bs_shift;
+        const int blk = bi < a.t.W ? a.t.block_tables[w.b * a.t.bt_stride + bi] : -1;
+        if (blk >= 0 && blk < a.t.num_blocks) {
+          const int64_t k = (int64_t)blk * a.t.nkv + w.h;
+          sc = make_float2(a.t.k_scale[k], a.t.v_scale[k]);
         }
+      }
+      return sc;
+    };
+    for (Walk w(a, sh.spot); w.more(); w.next(a)) {
+      float2 next = scales(w, w.t0);
+      for (int t = w.t0; t < w.t1; ++t, ++tile) {
+        const float2 sc = next;
+        wait(sh.raw_full[from.s], from.ph, 15);
+        if (t + 1 < w.t1) next = scales(w, t + 1);
+        wait(sh.empty[to.s], to.ph ^ 1, 16);
+        if (kv == 0 && tid < 32) {
+          // (K's slot is free: the weights of the fourth tile before this one are done, and with them its scales)
+          if (tid < KT / 16) sh.scale[tile & 3][tid] = sc;
+          __syncwarp();
+          if (tid == 0) tc::mbar_arrive_release(bar(sh.scale_full[tile & 3]));
+        }
+        convert_tile(rawr + from.s * RAW_TILE, ring + to.s * TILE, tid);
+        tc::fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) {
+          tc::mbar_arrive_release(bar(sh.full[to.s]));
+          tc::mbar_arrive_release(bar(sh.raw_empty[from.s]));
+        }
+        from.step(2, RS);
+        to.step(2, S);
+      }
     }
   }
   __syncthreads();
@@ -1538,11 +1554,13 @@ cudaError_t launch_main(K kern, int threads, int smem, std::atomic<uint64_t>& do
 template <bool FP8, int N>
 cudaError_t launch_few(const CUtensorMap& km, const CUtensorMap& vm, Args& a, cudaStream_t stream) {
   static std::atomic<uint64_t> done{0};
-  // the rest of shared memory: K and V tiles (e4m3: three of them, and 8-bit ones)
-  const int left = SMEM_MOST - few_bytes(N, 0, 0);
-  a.slots = FP8 ? 3 : std::min(left / TILE, 8);
-  a.raw_slots = FP8 ? std::min((left - 3 * TILE) / RAW_TILE, 8) : 0;
-  return launch_main(tree_attn_few_kernel<FP8, N>, FP8 ? 384 : 256, few_bytes(N, a.slots, a.raw_slots), done, km, vm, a, stream);
+  // The rest of shared memory: K and V tiles.  e4m3: four of them, and four 8-bit ones - even numbers, so that K and V,
+  // which are converted by warps of their own, have slots of their own.
+  const int left = SMEM_MOST - Bufs<FP8, N>::bytes(0, 0);
+  a.slots = FP8 ? 4 : std::min(left / TILE, 8);
+  a.raw_slots = FP8 ? 4 : 0;
+  static_assert(Bufs<true, N>::bytes(4, 4) <= SMEM_MOST, "");
+  return launch_main(tree_attn_few_kernel<FP8, N>, FP8 ? 512 : 256, Bufs<FP8, N>::bytes(a.slots, a.raw_slots), done, km, vm, a, stream);
 }
 
 template <bool FP8>
