@@ -17,7 +17,6 @@
 #include "common.cuh"
 #include "tcgen05.cuh"
 #include "tree.h"
-#include <cstdlib>
 
 namespace nvb {
 namespace {
@@ -745,16 +744,18 @@ __global__ void __launch_bounds__(VT, VT == 512 ? 1 : BF16 ? 3 : 2) tree_verify_
 
 }  // namespace
 
-static int tree_ctas = getenv("TREE_CTAS") ? atoi(getenv("TREE_CTAS")) : 0;
 cudaError_t launch_tree_verify(const TreeVerify& a, cudaStream_t stream) {
   if (a.num_seqs <= 0 || a.V <= 0 || a.max_nodes < 1 || a.max_nodes > TREE_MAX_NODES) return cudaErrorInvalidValue;
   int len = BLOCK;
   while ((int64_t)len * (MAX_CHUNKS - 1) < a.V) len *= 2;
   // CTAs per tree, no more than have a chunk per warp.  Few trees: all SMs, one CTA of 512 threads on each.  Many:
   // eight smaller CTAs, although that takes several rounds of clusters: walks differ in length, and the longest one of
-  // 256 trees on a CTA each was what the call took (256 x 8 nodes, 151936 tokens: 470 us; 2, 4, 8 CTAs: see below).
+  // 256 trees on a CTA each was what the call took.  Measured (us) at 1, 2, 4, 8, 16 CTAs:
+  //   256 trees of 8 nodes, 151936 tokens             477  266  213  214  319
+  //   64 of 16, with a draft                             -  365  240  171  203
+  //   17 of up to 64, 37987 tokens, fp32, with a draft   -    -    -   64   60   (1 of 8, 151936 tokens: 26, 24)
   const bool many = a.num_seqs * 16 > 148;
-  const int vt = many ? 256 : 512, most = tree_ctas > 0 ? tree_ctas : many ? 8 : 16;
+  const int vt = many ? 256 : 512, most = many ? 8 : 16;
   const int chunks = (a.V + len - 1) / len;
   int ctas = 1;
   while (ctas < most && ctas * (vt / 32) < chunks) ctas *= 2;
