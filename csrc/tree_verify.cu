@@ -129,10 +129,36 @@ template <bool BF16>
 struct Lane {
   static constexpr int VECS = BF16 ? 2 : 4;
   uint4 v[VECS];
-  __device__ __forceinline__ void load(const void* row, int s, int lane) {
-    const uint4* p = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(row) + (int64_t)s * (BF16 ? 2 : 4)) + lane;
+  // Tokens s .. s + 511 of the row (row + s: on 16 bytes), -inf outside 0 .. V - 1.
+  __device__ __forceinline__ void load(const void* row, int s, int V, int lane) {
+    constexpr int E = BF16 ? 2 : 4, N = 16 / E;
+    const uint4* p = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(row) + (int64_t)s * E) + lane;
+    if (s >= 0 && s + BLOCK <= V) {
 #pragma unroll
-    for (int i = 0; i < VECS; ++i) v[i] = __ldg(p + i * 32);
+      for (int i = 0; i < VECS; ++i) v[i] = __ldg(p + i * 32);
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < VECS; ++i) {
+      const int t = s + (i * 32 + lane) * N;
+      if (t >= 0 && t + N <= V) {
+        v[i] = __ldg(p + i * 32);
+      } else {
+        uint32_t w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if constexpr (BF16) {
+            const unsigned short* h = static_cast<const unsigned short*>(row) + t + 2 * e;
+            const uint32_t lo = (unsigned)(t + 2 * e) < (unsigned)V ? __ldg(h) : 0xff80;
+            const uint32_t hi = (unsigned)(t + 2 * e + 1) < (unsigned)V ? __ldg(h + 1) : 0xff80;
+            w[e] = hi << 16 | lo;
+          } else {
+            w[e] = (unsigned)(t + e) < (unsigned)V ? __ldg(static_cast<const uint32_t*>(row) + t + e) : 0xff800000u;
+          }
+        }
+        v[i] = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+    }
   }
   // fp32 bits of value i
   __device__ __forceinline__ uint32_t bits(int i) const {
@@ -188,16 +214,37 @@ __device__ __forceinline__ double warp_sum64(double v) {
   return v;
 }
 
-// The row's chunks: the first ends at a 16-byte boundary (`head` tokens in) plus `len`, the others have `len` tokens.
+// The row's chunks: every `len` tokens from the 16-byte boundary at or before it, `shift` tokens ahead of it.
 struct Cut {
-  int head, len, count, V;
-  __device__ __forceinline__ int begin(int k) const { return k ? head + k * len : 0; }
-  __device__ __forceinline__ int end(int k) const { return min(V, head + (k + 1) * len); }
-  // one aligned block
-  __device__ __forceinline__ bool block(int k) const { return len == BLOCK && (k || !head) && begin(k) + BLOCK <= V; }
+  int shift, len, count, V;
+  __device__ __forceinline__ int start(int k) const { return k * len - shift; }  // of the first: may be below 0
+  __device__ __forceinline__ int begin(int k) const { return max(0, start(k)); }
+  __device__ __forceinline__ int end(int k) const { return min(V, start(k + 1)); }
 };
 
-// Sum over an aligned block of exp((l - m) / T) and m, its maximum; at T <= 0 the first maximum alone.
+// 16 draft probabilities of a lane in a block of 512 tokens, 0 outside 0 .. V - 1.
+template <bool BF16>
+__device__ __forceinline__ void load_draft(float (&q)[16], const float* draft, int s, int V, int lane) {
+  const float* at = draft + s;
+  if (s >= 0 && s + BLOCK <= V && (reinterpret_cast<uintptr_t>(at) & 15) == 0) {
+#pragma unroll
+    for (int i = 0; i < 16; i += 4) {
+      const float4 f = __ldg(reinterpret_cast<const float4*>(at + Lane<BF16>::place(i, lane)));
+      q[i] = f.x;
+      q[i + 1] = f.y;
+      q[i + 2] = f.z;
+      q[i + 3] = f.w;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int t = Lane<BF16>::place(i, lane);
+      q[i] = (unsigned)(s + t) < (unsigned)V ? __ldg(at + t) : 0.f;
+    }
+  }
+}
+
+// Sum over a block of exp((l - m) / T) and m, its maximum; at T <= 0 the first maximum alone.
 template <bool BF16>
 __device__ __forceinline__ ChunkSum sum_block(Lane<BF16>& x, int s, const Dist& d, const Tables& tb, int lane) {
   x.clean();
@@ -240,7 +287,7 @@ __device__ __forceinline__ ChunkSum sum_block(Lane<BF16>& x, int s, const Dist& 
   return out;
 }
 
-// The same for a chunk of any place and length, token by token.
+// The same for a chunk of any length, token by token.
 template <bool BF16>
 __device__ ChunkSum sum_tokens(const void* row, int s, int end, const Dist& d, const Tables& tb, int lane) {
   ChunkSum out;
@@ -302,7 +349,7 @@ __device__ double left_tokens(const void* row, int s, int end, const Dist& d, co
   return warp_sum64(sum);
 }
 
-// Mass of the residual over an aligned block; tb: the table times 1 / sum.
+// Mass of the residual over a block; tb: the table times 1 / sum.
 template <bool BF16>
 __device__ __forceinline__ double left_block(Lane<BF16>& x, const float (&q)[16], const Dist& d, const Tables& tb,
                                              const Residual& r) {
@@ -421,56 +468,6 @@ __global__ void __launch_bounds__(VT, VT == 512 ? 1 : BF16 ? 3 : 2) tree_verify_
   cut.V = a.V;
   cut.len = len;
 
-  // The chunk sums, in the shared memory of every CTA.  A warp's next block is on its way while it works on one.
-  auto pass = [&](bool residual) -> ChunkSum* {
-    ChunkSum* to = sh.chunk[phase & 1];
-    const int stride = ctas * VWARPS;
-    const bool fast_q = residual && d.plain(d.max) && d.max < INFINITY;
-    Lane<BF16> x, nx;
-    int k = cta * VWARPS + warp;
-    if (k < cut.count && cut.block(k)) x.load(row, cut.begin(k), lane);
-    for (; k < cut.count; k += stride) {
-      const int s = cut.begin(k), end = cut.end(k), nk = k + stride;
-      if (nk < cut.count && cut.block(nk)) nx.load(row, cut.begin(nk), lane);
-      ChunkSum c;
-      if (!residual) {
-        c = cut.block(k) ? sum_block<BF16>(x, s, d, tb, lane) : sum_tokens<BF16>(row, s, end, d, tb, lane);
-      } else {
-        if (fast_q && cut.block(k)) {
-          float q[16];
-          const float* qr = left.draft + s;
-          if ((reinterpret_cast<uintptr_t>(qr) & 15) == 0) {
-#pragma unroll
-            for (int i = 0; i < 16; i += 4) {
-              const float4 f = __ldg(reinterpret_cast<const float4*>(qr + Lane<BF16>::place(i, lane)));
-              q[i] = f.x;
-              q[i + 1] = f.y;
-              q[i + 2] = f.z;
-              q[i + 3] = f.w;
-            }
-          } else {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) q[i] = __ldg(qr + Lane<BF16>::place(i, lane));
-          }
-          c.sum = warp_sum64(left_block<BF16>(x, q, d, scaled_tb, left));
-        } else {
-          c.sum = left_tokens<BF16>(row, s, end, d, tb, left, lane);
-        }
-        c.max = 0.f;
-        c.first = 0;
-      }
-      if (lane < (int)ctas)
-        asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(tc::cluster_map(smem_u32(to + k), lane)),
-                     "r"(__double2loint(c.sum)), "r"(__double2hiint(c.sum)), "r"(__float_as_int(c.max)), "r"(c.first)
-                     : "memory");
-      x = nx;
-    }
-    // the other buffer is written from here on, which every CTA has read before it came to this barrier
-    tc::cluster_arrive();
-    tc::cluster_wait();
-    ++phase;
-    return to;
-  };
   // First warp: the children of `node` in sh.kid; lane i holds child i's logit and draft probability, whose loads run
   // beside the pass over the row, and later its probability.
   int kids = 0;
@@ -494,6 +491,44 @@ __global__ void __launch_bounds__(VT, VT == 512 ? 1 : BF16 ? 3 : 2) tree_verify_
       kid_raw = BF16 ? __ldg(static_cast<const unsigned short*>(row) + x) : __ldg(static_cast<const unsigned*>(row) + x);
       if (left.draft) kid_draft = __ldg(left.draft + x);
     }
+  };
+  // The chunk sums, in the shared memory of every CTA.  A warp's next block is on its way while it works on one.
+  auto pass = [&](bool residual) -> ChunkSum* {
+    ChunkSum* to = sh.chunk[phase & 1];
+    const int stride = ctas * VWARPS;
+    const bool blocks = len == BLOCK && (!residual || (d.plain(d.max) && d.max < INFINITY));
+    Lane<BF16> x, nx;
+    int k = cta * VWARPS + warp;
+    if (blocks && k < cut.count) x.load(row, cut.start(k), cut.V, lane);
+    if (!residual && warp == 0) find_children();
+    for (; k < cut.count; k += stride) {
+      const int s = cut.start(k), nk = k + stride;
+      if (blocks && nk < cut.count) nx.load(row, cut.start(nk), cut.V, lane);
+      ChunkSum c;
+      if (!residual) {
+        c = blocks ? sum_block<BF16>(x, s, d, tb, lane) : sum_tokens<BF16>(row, cut.begin(k), cut.end(k), d, tb, lane);
+      } else {
+        if (blocks) {
+          float q[16];
+          load_draft<BF16>(q, left.draft, s, cut.V, lane);
+          c.sum = warp_sum64(left_block<BF16>(x, q, d, scaled_tb, left));
+        } else {
+          c.sum = left_tokens<BF16>(row, cut.begin(k), cut.end(k), d, tb, left, lane);
+        }
+        c.max = 0.f;
+        c.first = 0;
+      }
+      if (lane < (int)ctas)
+        asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(tc::cluster_map(smem_u32(to + k), lane)),
+                     "r"(__double2loint(c.sum)), "r"(__double2hiint(c.sum)), "r"(__float_as_int(c.max)), "r"(c.first)
+                     : "memory");
+      x = nx;
+    }
+    // the other buffer is written from here on, which every CTA has read before it came to this barrier
+    tc::cluster_arrive();
+    tc::cluster_wait();
+    ++phase;
+    return to;
   };
   // First warp: tries children from sh.at on until one is taken, a residual is needed or none is left (with the same
   // numbers in every lane and every CTA).
@@ -560,10 +595,9 @@ __global__ void __launch_bounds__(VT, VT == 512 ? 1 : BF16 ? 3 : 2) tree_verify_
     row = static_cast<const uint8_t*>(a.logits) + r * a.ld * E;
     left.draft = a.draft && !d.greedy ? a.draft + r * a.ld_draft : nullptr;
     left.k = 0;
-    cut.head = (int)((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / E;
-    cut.count = a.V <= cut.head + len ? 1 : (a.V - cut.head + len - 1) / len;
+    cut.shift = (int)(reinterpret_cast<uintptr_t>(row) & 15) / E;
+    cut.count = (a.V + cut.shift + len - 1) / len;
     __syncthreads();  // the table (first node); every thread has read the last node's decision
-    if (warp == 0) find_children();
     sums = pass(false);
     // the row's maximum and sum, by all threads, the same numbers in each
     float m = NEG;
@@ -661,7 +695,7 @@ __global__ void __launch_bounds__(VT, VT == 512 ? 1 : BF16 ? 3 : 2) tree_verify_
   __syncthreads();
   if (!left.draft) {
     for (int i = warp; i < left.k; i += VWARPS) {  // a rejected token's chunk is summed again without it
-      const int k = sh.gone[i] < cut.head ? 0 : (sh.gone[i] - cut.head) / len;
+      const int k = (sh.gone[i] + cut.shift) / len;
       const double part = left_tokens<BF16>(row, cut.begin(k), cut.end(k), d, tb, left, lane);
       if (lane == 0) sums[k].sum = part;
     }
@@ -747,7 +781,7 @@ __global__ void __launch_bounds__(VT, VT == 512 ? 1 : BF16 ? 3 : 2) tree_verify_
 cudaError_t launch_tree_verify(const TreeVerify& a, cudaStream_t stream) {
   if (a.num_seqs <= 0 || a.V <= 0 || a.max_nodes < 1 || a.max_nodes > TREE_MAX_NODES) return cudaErrorInvalidValue;
   int len = BLOCK;
-  while ((int64_t)len * (MAX_CHUNKS - 1) < a.V) len *= 2;
+  while ((int64_t)len * (MAX_CHUNKS - 1) < a.V) len *= 2;  // (one chunk more for a row off a 16-byte boundary)
   // CTAs per tree, no more than have a chunk per warp.  Few trees: all SMs, one CTA of 512 threads on each.  Many:
   // eight smaller CTAs, although that takes several rounds of clusters: walks differ in length, and the longest one of
   // 256 trees on a CTA each was what the call took.  Measured (us) at 1, 2, 4, 8, 16 CTAs:
