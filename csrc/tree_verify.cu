@@ -413,7 +413,7 @@ __device__ __forceinline__ double scaled(const ChunkSum& c, const Dist& d, const
   return weight(c.max, d.max, d.c, tb) * c.sum;
 }
 
-// 512 threads and one CTA per SM while the trees are fewer than the SMs, else 256 threads and two or three CTAs.
+// 512 threads and one CTA per SM while there are SMs for all, else 256 threads and two or three CTAs.
 template <bool BF16, int VT>
 __global__ void __launch_bounds__(VT, VT == 512 ? 1 : BF16 ? 3 : 2) tree_verify_kernel(TreeVerify a, int len) {
   constexpr int VWARPS = VT / 32;
@@ -782,21 +782,25 @@ cudaError_t launch_tree_verify(const TreeVerify& a, cudaStream_t stream) {
   if (a.num_seqs <= 0 || a.V <= 0 || a.max_nodes < 1 || a.max_nodes > TREE_MAX_NODES) return cudaErrorInvalidValue;
   int len = BLOCK;
   while ((int64_t)len * (MAX_CHUNKS - 1) < a.V) len *= 2;  // (one chunk more for a row off a 16-byte boundary)
-  // CTAs per tree, no more than have a chunk per warp.  Few trees: all SMs, one CTA of 512 threads on each.  Many:
-  // eight smaller CTAs, although that takes several rounds of clusters: walks differ in length, and the longest one of
-  // 256 trees on a CTA each was what the call took.  Measured (us) at 1, 2, 4, 8, 16 CTAs:
-  //   256 trees of 8 nodes, 151936 tokens             477  266  213  214  319
-  //   64 of 16, with a draft                             -  365  240  171  203
-  //   17 of up to 64, 37987 tokens, fp32, with a draft   -    -    -   64   60   (1 of 8, 151936 tokens: 26, 24)
-  const bool many = a.num_seqs * 16 > 148;
-  const int vt = many ? 256 : 512, most = many ? 8 : 16;
+  // CTAs per tree.  Few trees: all SMs, one CTA of 512 threads on each, no more than have a chunk per warp.  More:
+  // smaller CTAs, three to an SM.  Behind some 32 trees eight of them, no more than have two chunks per warp, although
+  // that takes several rounds of clusters: walks differ in length, and the longest one of 256 trees on a CTA each was
+  // what the call took.  Measured (us, 256 threads unless noted) at 1, 4, 8, 16 CTAs:
+  //   256 trees of 8 nodes, 151936 tokens                    362  178  178  252
+  //   64 of 16, with a draft                                 485  184  134  149
+  //   120 of 8, 32000 tokens, with a draft                    95   55   66  121
+  //   32 of 16, 151936 tokens                                325  110   79   69   (512 threads: 236, 84, 73, 93)
+  //   20 of 16, with a draft                                 339  109   79   64   (237, 81, 68, 85)
+  //   8 of 8, with a draft; 1 of 8: 512 threads              188, 63;  65, 28;  47, 23;  43, 20
+  const bool few = a.num_seqs * 16 <= 148, crowded = a.num_seqs > 32;
+  const int vt = few ? 512 : 256, most = crowded ? 8 : 16;
   const int chunks = (a.V + len - 1) / len;
   int ctas = 1;
-  while (ctas < most && ctas * (vt / 32) < chunks) ctas *= 2;
-  auto kern = a.logits_bf16 ? (many ? tree_verify_kernel<true, 256> : tree_verify_kernel<true, 512>)
-                            : (many ? tree_verify_kernel<false, 256> : tree_verify_kernel<false, 512>);
+  while (ctas < most && (crowded ? 2 * ctas * (vt / 32) <= chunks : ctas * (vt / 32) < chunks)) ctas *= 2;
+  auto kern = a.logits_bf16 ? (few ? tree_verify_kernel<true, 512> : tree_verify_kernel<true, 256>)
+                            : (few ? tree_verify_kernel<false, 512> : tree_verify_kernel<false, 256>);
   static std::atomic<uint64_t> done[4] = {{0}, {0}, {0}, {0}};
-  cudaError_t e = smem_opt_in(done[(a.logits_bf16 ? 1 : 0) + (many ? 2 : 0)], kern, (int)sizeof(Shared), true);
+  cudaError_t e = smem_opt_in(done[(a.logits_bf16 ? 1 : 0) + (few ? 2 : 0)], kern, (int)sizeof(Shared), true);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)a.num_seqs * ctas);

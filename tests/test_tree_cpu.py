@@ -349,6 +349,7 @@ def test_the_kernels_refuse_bad_arguments():
     assert "temperatures" in verify(temps=torch.ones(3)) and "uniforms" in verify(u=torch.rand(5).double())
     assert "draw_uniforms" in verify(ud=torch.rand(1)) and "draft_probs" in verify(draft=torch.zeros(5, 51))
     assert "draft_probs" in verify(draft=torch.zeros(5, 50).bfloat16()) and "nodes" in verify(m=257)
+    assert "4194303" in verify(logits=torch.empty(5, 1 << 22, dtype=torch.bfloat16))
 
     def commit(**kw):
         a = dict(kv=torch.zeros(2, 3, nb, 2, 16, 128, **bf16), path=torch.zeros(2, 3, **i32),

@@ -368,9 +368,9 @@ def test_walk(ops, draft, dtype, ns, v):
 
 
 @pytest.mark.parametrize("draft", [False, True])
-@pytest.mark.parametrize("b", [1, 5, 20, 80, 170])
+@pytest.mark.parametrize("b", [1, 5, 20, 32, 33, 80, 170])
 def test_walk_over_cluster_sizes(ops, draft, b):
-    """One tree takes up to 16 CTAs; 150 trees and more one each."""
+    """A tree takes up to 16 CTAs where trees are few, up to 8 smaller ones where they are many."""
     Walk([3] * b, 20001, torch.bfloat16, draft, seed=b).check(ops)
 
 
