@@ -5,11 +5,12 @@
 // child the next token is the first x whose cumulative sum of p is above u_draw times the total.
 //
 // A cumulative sum over a vocabulary of 1.5e5 tokens has tokens narrower than fp32's rounding next to every border,
-// so weights and sums are 64-bit: decisions are those of exact arithmetic but for random numbers within some 1e-11 of
-// a border, and do not depend on how many CTAs share a row.  exp2 in 64 bits costs 9 fp64 instructions here, which
-// bound the kernel (an SM does 64 a clock): the argument is taken apart into a multiple of 1/32 (a table entry, and
-// an exponent by integer addition) and a rest |r| <= 1/64 with 2^r = 1 + t + t^2/2 + t^3/6 + t^4/24, t = r ln 2 (next
-// term: at most 1.3e-12).  The table's halves are read as words: 32 entries, a bank each.
+// so decisions rest on 64-bit weights and sums, or on fp32 ones where their error cannot matter: they are those of
+// exact arithmetic but for random numbers within some 1e-11 of a border, and do not depend on how many CTAs share a
+// row.  exp2 in 64 bits costs 9 fp64 instructions here (an SM does 64 a clock) of some 30 in all: the argument is taken
+// apart into a multiple of 1/32 (a table entry, and an exponent by integer addition) and a rest |r| <= 1/64 with
+// 2^r = 1 + t + t^2/2 + t^3/6 + t^4/24, t = r ln 2 (next term: at most 1.3e-12).  The table's halves are read as
+// words: 32 entries, a bank each.
 //
 // One cluster of CTAs walks one tree, so only the rows of visited nodes are read.  A row is cut into chunks of
 // 512 tokens; a warp sums a chunk relative to the chunk's maximum and sends (sum, maximum) to every CTA of the
@@ -24,7 +25,14 @@ namespace {
 constexpr int BLOCK = 512;         // tokens of a warp's step: 16 per lane
 constexpr int MAX_CHUNKS = 512;    // longer vocabularies have longer chunks
 constexpr float NEG = -INFINITY;
+constexpr double SLACK = 1.0 / 262144.0;  // 2^-18: bounds the fp32 sums' relative error (sum_block_fast)
 constexpr unsigned SPAN = 0xC0DC2000u;  // upper word of -28800 = -32 x 900: weights below 2^-900 of the largest are none
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 
 struct ChunkSum {
   double sum;  // relative to max (walk over the logits), or as it is (residuals)
@@ -90,7 +98,10 @@ struct Dist {
   double c;        // 32 log2(e) / T
   double inv_sum;  // 1 / sum of the weights
   float max;       // the row's maximum (a NaN counts as -inf)
+  float cf;        // log2(e) / T
   bool greedy;
+  // Whether fp32's range holds log2(e) / T, with room.
+  __device__ __forceinline__ bool moderate() const { return cf > 1e-6f && cf < 1e6f; }
   // Whether l c - max c in one instruction is exact enough (2^-35 of 1/32), and -inf far enough off.
   __device__ __forceinline__ bool plain(float top) const { return c > 1e-9 && fabs((double)top) * c < 262144.0; }
 };
@@ -287,6 +298,31 @@ __device__ __forceinline__ ChunkSum sum_block(Lane<BF16>& x, int s, const Dist& 
   return out;
 }
 
+// The same in fp32.  y = (l - m) log2(e) / T has a relative error of 3 x 2^-24 (cf, difference, product), exp2 one of
+// 2^-22; the sum of w |y| over a block is at most 9 times that of w (the entropy of 512 values is at most 9 bits), so
+// the weights' errors come to 9 ln 2 x 3 x 2^-24 + 2^-22 = 23 x 2^-24 of the sum; with 11 roundings in the sum it is
+// within 34 x 2^-24, about half of SLACK.  (What exp2 flushes to 0 is below 2^-126 of the maximum.)
+template <bool BF16>
+__device__ __forceinline__ ChunkSum sum_block_fast(Lane<BF16>& x, int s, const Dist& d, const Tables& tb, int lane) {
+  if (d.greedy) return sum_block<BF16>(x, s, d, tb, lane);
+  x.clean();
+  ChunkSum out;
+  out.max = warp_max(x.max());
+  out.sum = 0.0;
+  out.first = 0x7fffffff;
+  if (out.max == NEG) return out;
+  float sum[4] = {0.f, 0.f, 0.f, 0.f};
+  if (out.max < INFINITY) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) sum[i & 3] += ex2((__uint_as_float(x.bits(i)) - out.max) * d.cf);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) sum[i & 3] += __uint_as_float(x.bits(i)) == INFINITY ? 1.f : 0.f;
+  }
+  out.sum = (double)warp_sum((sum[0] + sum[1]) + (sum[2] + sum[3]));
+  return out;
+}
+
 // The same for a chunk of any length, token by token.
 template <bool BF16>
 __device__ ChunkSum sum_tokens(const void* row, int s, int end, const Dist& d, const Tables& tb, int lane) {
@@ -385,7 +421,8 @@ __device__ __forceinline__ double left_block(Lane<BF16>& x, const float (&q)[16]
   return (sum[0] + sum[1]) + (sum[2] + sum[3]);
 }
 
-enum Action { DRAW = 0, GO = 1, RESIDUAL = 2 };
+// REDO: fp32's roundings could have decided.
+enum Action { DRAW = 0, GO = 1, RESIDUAL = 2, REDO = 3 };
 
 struct Shared {
   ChunkSum chunk[2][MAX_CHUNKS];
@@ -404,7 +441,7 @@ struct Shared {
   int at;        // the next child to try
   int summed;  // rejections that the chunk sums at hand stand for
   int best;    // first maximum of the row
-  int found, held, drawn_chunk;
+  int found, held, drawn_chunk, sure;
 };
 
 // Sum of a chunk in units of the row's maximum.
@@ -413,9 +450,39 @@ __device__ __forceinline__ double scaled(const ChunkSum& c, const Dist& d, const
   return weight(c.max, d.max, d.c, tb) * c.sum;
 }
 
+__device__ __forceinline__ void send(ChunkSum* to, const ChunkSum& c, int ctas, int lane) {
+  if (lane < ctas)
+    asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(tc::cluster_map(smem_u32(to), lane)),
+                 "r"(__double2loint(c.sum)), "r"(__double2hiint(c.sum)), "r"(__float_as_int(c.max)), "r"(c.first)
+                 : "memory");
+}
+
+// A warp's chunks in 64 bits behind an fp32 walk: few nodes come to it, and its registers are not that walk's.
+template <bool BF16>
+__device__ __noinline__ void sum_again(const void* row, const Cut& cut, const Dist& d, const Tables& tb, ChunkSum* to, int k,
+                                       int stride, int ctas) {
+  const int lane = threadIdx.x & 31;
+  for (; k < cut.count; k += stride) {
+    ChunkSum c;
+    if (cut.len == BLOCK) {
+      Lane<BF16> x;
+      x.load(row, cut.start(k), cut.V, lane);
+      c = sum_block<BF16>(x, cut.start(k), d, tb, lane);
+    } else {
+      c = sum_tokens<BF16>(row, cut.begin(k), cut.end(k), d, tb, lane);
+    }
+    send(to + k, c, ctas, lane);
+  }
+}
+
 // 512 threads and one CTA per SM while there are SMs for all, else 256 threads and two or three CTAs.
-template <bool BF16, int VT>
-__global__ void __launch_bounds__(VT, VT == 512 ? 1 : BF16 ? 3 : 2) tree_verify_kernel(TreeVerify a, int len) {
+// FAST (no draft): nodes are summed in fp32 first, and again in 64 bits where its roundings could decide: a draw of a
+// token of less than some 1e-5, a number that close to a border.  In 64 bits a token costs some 30 instructions, which
+// bound a call of many trees, in fp32 8 (256 trees of 8 nodes, 151936 tokens: 174 us all in 64 bits, 127 so).
+// Few trees wait for their longest walk, where a node walked twice costs more than fp32 gains (17 of up to 64: 64 -> 102),
+// and with a draft a rejection's chain of residuals multiplies the error (64 of 16: 171 -> 204).
+template <bool BF16, int VT, bool FAST>
+__global__ void __launch_bounds__(VT, VT == 512 ? 1 : FAST || BF16 ? 3 : 2) tree_verify_kernel(TreeVerify a, int len) {
   constexpr int VWARPS = VT / 32;
   pdl_wait();     // inputs come from the previous kernel in the stream
   pdl_trigger();  // the next kernel may start its prologue
@@ -454,6 +521,7 @@ __global__ void __launch_bounds__(VT, VT == 512 ? 1 : BF16 ? 3 : 2) tree_verify_
   d.greedy = !(temp > 0.f);
   // above 0 at an infinite temperature too, where -inf still has no weight
   d.c = d.greedy ? 0.0 : fmax(32.0 * 1.4426950408889634074 / (double)temp, 1e-300);
+  d.cf = (float)(d.c / 32.0);
   d.inv_sum = 0.0;
   d.max = NEG;
   Residual left;
@@ -462,6 +530,8 @@ __global__ void __launch_bounds__(VT, VT == 512 ? 1 : BF16 ? 3 : 2) tree_verify_
   left.gone = sh.gone;
   left.k = 0;
   int node = 0, length = 1;
+  const bool slow = !FAST || d.greedy || !d.moderate();
+  bool exact = slow;  // this node in 64 bits
   uint32_t phase = 0;
   const void* row = nullptr;
   Cut cut;
@@ -499,6 +569,11 @@ __global__ void __launch_bounds__(VT, VT == 512 ? 1 : BF16 ? 3 : 2) tree_verify_
     const bool blocks = len == BLOCK && (!residual || (d.plain(d.max) && d.max < INFINITY));
     Lane<BF16> x, nx;
     int k = cta * VWARPS + warp;
+    if (FAST && exact && !d.greedy) {
+      if (warp == 0) find_children();
+      sum_again<BF16>(row, cut, d, tb, to, k, stride, ctas);
+      k = cut.count;
+    }
     if (blocks && k < cut.count) x.load(row, cut.start(k), cut.V, lane);
     if (!residual && warp == 0) find_children();
     for (; k < cut.count; k += stride) {
@@ -506,7 +581,8 @@ __global__ void __launch_bounds__(VT, VT == 512 ? 1 : BF16 ? 3 : 2) tree_verify_
       if (blocks && nk < cut.count) nx.load(row, cut.start(nk), cut.V, lane);
       ChunkSum c;
       if (!residual) {
-        c = blocks ? sum_block<BF16>(x, s, d, tb, lane) : sum_tokens<BF16>(row, cut.begin(k), cut.end(k), d, tb, lane);
+        c = blocks ? (FAST ? sum_block_fast<BF16>(x, s, d, tb, lane) : sum_block<BF16>(x, s, d, tb, lane))
+                   : sum_tokens<BF16>(row, cut.begin(k), cut.end(k), d, tb, lane);
       } else {
         if (blocks) {
           float q[16];
@@ -518,10 +594,7 @@ __global__ void __launch_bounds__(VT, VT == 512 ? 1 : BF16 ? 3 : 2) tree_verify_
         c.max = 0.f;
         c.first = 0;
       }
-      if (lane < (int)ctas)
-        asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(tc::cluster_map(smem_u32(to + k), lane)),
-                     "r"(__double2loint(c.sum)), "r"(__double2hiint(c.sum)), "r"(__float_as_int(c.max)), "r"(c.first)
-                     : "memory");
+      send(to + k, c, ctas, lane);
       x = nx;
     }
     // the other buffer is written from here on, which every CTA has read before it came to this barrier
@@ -561,6 +634,12 @@ __global__ void __launch_bounds__(VT, VT == 512 ? 1 : BF16 ? 3 : 2) tree_verify_
       else
         for (int i = 0; i < rejected; ++i)
           if (sh.gone[i] == x) p = 0.0;
+      // p is within SLACK of itself, the mass (1 less the rejected tokens) within SLACK
+      if (FAST && !exact && in && p > 0.0 &&
+          (!(fabs(p - (double)sh.u[child] * mass) > SLACK * (p + fabs((double)sh.u[child]))) || mass - p < 8.0 * SLACK)) {
+        action = REDO;
+        break;
+      }
       if (in && (double)sh.u[child] * q * mass < p) {
         action = GO;
         break;
@@ -588,12 +667,111 @@ __global__ void __launch_bounds__(VT, VT == 512 ? 1 : BF16 ? 3 : 2) tree_verify_
     }
   };
 
+  // The draw: the chunk in which the cumulative sum passes the share, then the token in it.  False where fp32's
+  // roundings could have decided: with every chunk within SLACK of its sum, so is the cumulative sum's share of the
+  // total.  (At most one thread is sure of its token.)  FAST: in every CTA of the cluster, which all learn by it
+  // whether the node is walked again.
+  int next = 0;
+  auto draw = [&](ChunkSum* sums) -> bool {
+    if (d.greedy) {
+      next = max(sh.best, 0);
+      return true;
+    }
+    if (!left.draft || left.k == 0)
+      for (int k = threadIdx.x; k < cut.count; k += VT) sums[k].sum = scaled(sums[k], d, tb) * d.inv_sum;
+    __syncthreads();
+    if (!left.draft) {
+      for (int i = warp; i < left.k; i += VWARPS) {  // a rejected token's chunk is summed again without it
+        const int k = (sh.gone[i] + cut.shift) / len;
+        const double part = left_tokens<BF16>(row, cut.begin(k), cut.end(k), d, tb, left, lane);
+        if (lane == 0) sums[k].sum = part;
+      }
+      __syncthreads();
+    }
+    if (warp == 0) {
+      // a lane takes consecutive chunks
+      const int per = (cut.count + 31) / 32, k0 = min(cut.count, lane * per), k1 = min(cut.count, k0 + per);
+      double mine = 0.0;
+      for (int k = k0; k < k1; ++k) mine += sums[k].sum;
+      double upto = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const double up = __shfl_up_sync(FULL_MASK, upto, o);
+        if (lane >= o) upto += up;
+      }
+      const double total = __shfl_sync(FULL_MASK, upto, 31);
+      const float u = a.u_draw[b];
+      const double share = (double)(u > 0.f ? fminf(u, 1.f) : 0.f) * total;
+      const unsigned above = __ballot_sync(FULL_MASK, mine > 0.0 && upto > share), any = __ballot_sync(FULL_MASK, mine > 0.0);
+      if (lane == 0) {
+        sh.found = 0x7fffffff;
+        sh.sure = 0;
+        sh.held = -1;
+        if (!any) sh.drawn_chunk = -1;  // no logit above -inf
+      }
+      if (any && lane == (above ? __ffs(above) - 1 : 31 - __clz(any))) {
+        double sum = upto - mine;
+        int at = -1;
+        double ahead = 0.0;
+        for (int k = k0; k < k1; ++k) {
+          if (sums[k].sum > 0.0) {
+            at = k;  // the last one with any mass where rounding leaves none above the share
+            ahead = sum;
+          }
+          sum += sums[k].sum;
+          if (above && sums[k].sum > 0.0 && sum > share) break;
+        }
+        sh.drawn_chunk = at;
+        sh.ahead = ahead;
+        sh.share = share;
+      }
+    }
+    __syncthreads();
+    const int k = sh.drawn_chunk;
+    if (k < 0) {
+      next = 0;
+      return true;
+    }
+    double before = sh.ahead;
+    const double share = sh.share;
+    for (int s = cut.begin(k); s < cut.end(k); s += VT) {
+      const int x = s + threadIdx.x;
+      const double v = x < cut.end(k) ? left_at<BF16>(row, x, d, tb, left) : 0.0;
+      double sum = v;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const double up = __shfl_up_sync(FULL_MASK, sum, o);
+        if (lane >= o) sum += up;
+      }
+      if (lane == 31) sh.scan[warp] = sum;
+      __syncthreads();
+      double ahead = before;
+      for (int w = 0; w < VWARPS; ++w) {
+        if (w < warp) ahead += sh.scan[w];
+        before += sh.scan[w];
+      }
+      const int at = __reduce_min_sync(FULL_MASK, v > 0.0 && ahead + sum > share ? x : 0x7fffffff);
+      if (FAST && !exact && v > 0.0 && ahead + sum - v + 2.0 * SLACK <= share && share <= ahead + sum - 2.0 * SLACK) sh.sure = 1;
+      const int held = __reduce_max_sync(FULL_MASK, v > 0.0 ? x : -1);
+      if (lane == 0) {
+        atomicMin(&sh.found, at);
+        atomicMax(&sh.held, held);
+      }
+      __syncthreads();
+      if (sh.found != 0x7fffffff) break;  // the same in every thread: written ahead of the barrier only
+      __syncthreads();
+    }
+    // the chunk's sum may have been a rounding above that of its tokens
+    next = sh.found != 0x7fffffff ? sh.found : max(sh.held, 0);
+    return exact || sh.sure != 0;
+  };
+
   ChunkSum* sums = nullptr;
   while (true) {
     const int64_t r = (int64_t)t0 + node;
     constexpr int E = BF16 ? 2 : 4;
     row = static_cast<const uint8_t*>(a.logits) + r * a.ld * E;
-    left.draft = a.draft && !d.greedy ? a.draft + r * a.ld_draft : nullptr;
+    left.draft = !FAST && a.draft && !d.greedy ? a.draft + r * a.ld_draft : nullptr;
     left.k = 0;
     cut.shift = (int)(reinterpret_cast<uintptr_t>(row) & 15) / E;
     cut.count = (a.V + cut.shift + len - 1) / len;
@@ -644,7 +822,7 @@ __global__ void __launch_bounds__(VT, VT == 512 ? 1 : BF16 ? 3 : 2) tree_verify_
       try_children();
     }
     __syncthreads();
-    while (sh.action == RESIDUAL) {
+    while (!FAST && sh.action == RESIDUAL) {
       left.k = sh.rejected;
       sums = pass(true);
       double part = 0.0;
@@ -673,107 +851,30 @@ __global__ void __launch_bounds__(VT, VT == 512 ? 1 : BF16 ? 3 : 2) tree_verify_
       }
       __syncthreads();
     }
-    if (sh.action != GO) break;
+    if (FAST && sh.action == REDO) {
+      exact = true;
+      continue;
+    }
+    if (sh.action != GO) {
+      left.k = sh.rejected;
+      if (left.draft && sh.summed != left.k) sums = pass(left.k > 0);
+      if ((!FAST && cta != 0) || draw(sums)) break;
+      exact = true;
+      continue;
+    }
+    exact = slow;
     node = sh.child;
     if (cta == 0 && threadIdx.x == 0) path[length] = node;
     ++length;
   }
 
-  left.k = sh.rejected;
-  if (left.draft && sh.summed != left.k) sums = pass(left.k > 0);
   if (cta != 0) return;
   for (int i = threadIdx.x; i < a.max_nodes; i += VT)
     if (i == 0 || i >= length) path[i] = i ? -1 : 0;
-  if (threadIdx.x == 0) a.length[b] = length;
-  if (d.greedy) {
-    if (threadIdx.x == 0) a.next_token[b] = max(sh.best, 0);
-    return;
+  if (threadIdx.x == 0) {
+    a.length[b] = length;
+    a.next_token[b] = next;
   }
-  // ---- the draw: the chunk in which the cumulative sum passes the share, then the token in it
-  if (!left.draft || left.k == 0)
-    for (int k = threadIdx.x; k < cut.count; k += VT) sums[k].sum = scaled(sums[k], d, tb) * d.inv_sum;
-  __syncthreads();
-  if (!left.draft) {
-    for (int i = warp; i < left.k; i += VWARPS) {  // a rejected token's chunk is summed again without it
-      const int k = (sh.gone[i] + cut.shift) / len;
-      const double part = left_tokens<BF16>(row, cut.begin(k), cut.end(k), d, tb, left, lane);
-      if (lane == 0) sums[k].sum = part;
-    }
-    __syncthreads();
-  }
-  if (warp == 0) {
-    // a lane takes consecutive chunks
-    const int per = (cut.count + 31) / 32, k0 = min(cut.count, lane * per), k1 = min(cut.count, k0 + per);
-    double mine = 0.0;
-    for (int k = k0; k < k1; ++k) mine += sums[k].sum;
-    double upto = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const double up = __shfl_up_sync(FULL_MASK, upto, o);
-      if (lane >= o) upto += up;
-    }
-    const double total = __shfl_sync(FULL_MASK, upto, 31);
-    const float u = a.u_draw[b];
-    const double share = (double)(u > 0.f ? fminf(u, 1.f) : 0.f) * total;
-    const unsigned above = __ballot_sync(FULL_MASK, mine > 0.0 && upto > share), any = __ballot_sync(FULL_MASK, mine > 0.0);
-    if (lane == 0) {
-      sh.found = 0x7fffffff;
-      sh.held = -1;
-      if (!any) sh.drawn_chunk = -1;  // no logit above -inf
-    }
-    if (any && lane == (above ? __ffs(above) - 1 : 31 - __clz(any))) {
-      double sum = upto - mine;
-      int at = -1;
-      double ahead = 0.0;
-      for (int k = k0; k < k1; ++k) {
-        if (sums[k].sum > 0.0) {
-          at = k;  // the last one with any mass where rounding leaves none above the share
-          ahead = sum;
-        }
-        sum += sums[k].sum;
-        if (above && sums[k].sum > 0.0 && sum > share) break;
-      }
-      sh.drawn_chunk = at;
-      sh.ahead = ahead;
-      sh.share = share;
-    }
-  }
-  __syncthreads();
-  const int k = sh.drawn_chunk;
-  if (k < 0) {
-    if (threadIdx.x == 0) a.next_token[b] = 0;
-    return;
-  }
-  double before = sh.ahead;
-  const double share = sh.share;
-  for (int s = cut.begin(k); s < cut.end(k); s += VT) {
-    const int x = s + threadIdx.x;
-    const double v = x < cut.end(k) ? left_at<BF16>(row, x, d, tb, left) : 0.0;
-    double sum = v;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const double up = __shfl_up_sync(FULL_MASK, sum, o);
-      if (lane >= o) sum += up;
-    }
-    if (lane == 31) sh.scan[warp] = sum;
-    __syncthreads();
-    double ahead = before;
-    for (int w = 0; w < VWARPS; ++w) {
-      if (w < warp) ahead += sh.scan[w];
-      before += sh.scan[w];
-    }
-    const int at = __reduce_min_sync(FULL_MASK, v > 0.0 && ahead + sum > share ? x : 0x7fffffff);
-    const int held = __reduce_max_sync(FULL_MASK, v > 0.0 ? x : -1);
-    if (lane == 0) {
-      atomicMin(&sh.found, at);
-      atomicMax(&sh.held, held);
-    }
-    __syncthreads();
-    if (sh.found != 0x7fffffff) break;  // the same in every thread: written ahead of the barrier only
-    __syncthreads();
-  }
-  // the chunk's sum may have been a rounding above that of its tokens
-  if (threadIdx.x == 0) a.next_token[b] = sh.found != 0x7fffffff ? sh.found : max(sh.held, 0);
 }
 
 }  // namespace
@@ -785,22 +886,25 @@ cudaError_t launch_tree_verify(const TreeVerify& a, cudaStream_t stream) {
   // CTAs per tree.  Few trees: all SMs, one CTA of 512 threads on each, no more than have a chunk per warp.  More:
   // smaller CTAs, three to an SM.  Behind some 32 trees eight of them, no more than have two chunks per warp, although
   // that takes several rounds of clusters: walks differ in length, and the longest one of 256 trees on a CTA each was
-  // what the call took.  Measured (us, 256 threads unless noted) at 1, 4, 8, 16 CTAs:
-  //   256 trees of 8 nodes, 151936 tokens                    362  178  178  252
-  //   64 of 16, with a draft                                 485  184  134  149
+  // what the call took.  In fp32 four are enough for many.  Measured (us, 256 threads unless noted) at 1, 4, 8, 16 CTAs:
+  //   256 trees of 8 nodes, 151936 tokens, fp32 first        199  127  168  293   (all in 64 bits 362, 178, 178, 252)
+  //   64 of 16, fp32 first                                   236   91   74   99
+  //   120 of 8, 32000 tokens, fp32 first                      55   43   58  108
+  //   64 of 16, 151936 tokens, with a draft                  485  184  134  149
   //   120 of 8, 32000 tokens, with a draft                    95   55   66  121
   //   32 of 16, 151936 tokens                                325  110   79   69   (512 threads: 236, 84, 73, 93)
   //   20 of 16, with a draft                                 339  109   79   64   (237, 81, 68, 85)
   //   8 of 8, with a draft; 1 of 8: 512 threads              188, 63;  65, 28;  47, 23;  43, 20
-  const bool few = a.num_seqs * 16 <= 148, crowded = a.num_seqs > 32;
-  const int vt = few ? 512 : 256, most = crowded ? 8 : 16;
+  const bool few = a.num_seqs * 16 <= 148, crowded = a.num_seqs > 32, fast = crowded && !a.draft;
+  const int vt = few ? 512 : 256, most = !crowded ? 16 : fast && a.num_seqs > 128 ? 4 : 8;
   const int chunks = (a.V + len - 1) / len;
   int ctas = 1;
   while (ctas < most && (crowded ? 2 * ctas * (vt / 32) <= chunks : ctas * (vt / 32) < chunks)) ctas *= 2;
-  auto kern = a.logits_bf16 ? (few ? tree_verify_kernel<true, 512> : tree_verify_kernel<true, 256>)
-                            : (few ? tree_verify_kernel<false, 512> : tree_verify_kernel<false, 256>);
-  static std::atomic<uint64_t> done[4] = {{0}, {0}, {0}, {0}};
-  cudaError_t e = smem_opt_in(done[(a.logits_bf16 ? 1 : 0) + (few ? 2 : 0)], kern, (int)sizeof(Shared), true);
+  auto kern = fast ? (a.logits_bf16 ? tree_verify_kernel<true, 256, true> : tree_verify_kernel<false, 256, true>)
+              : few ? (a.logits_bf16 ? tree_verify_kernel<true, 512, false> : tree_verify_kernel<false, 512, false>)
+                    : (a.logits_bf16 ? tree_verify_kernel<true, 256, false> : tree_verify_kernel<false, 256, false>);
+  static std::atomic<uint64_t> done[6] = {{0}, {0}, {0}, {0}, {0}, {0}};
+  cudaError_t e = smem_opt_in(done[(a.logits_bf16 ? 1 : 0) + (fast ? 4 : few ? 2 : 0)], kern, (int)sizeof(Shared), true);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)a.num_seqs * ctas);

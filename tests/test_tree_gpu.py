@@ -374,6 +374,27 @@ def test_walk_over_cluster_sizes(ops, draft, b):
     Walk([3] * b, 20001, torch.bfloat16, draft, seed=b).check(ops)
 
 
+@pytest.mark.parametrize("draft", [False, True])
+@pytest.mark.parametrize("b", [3, 40])
+def test_walk_with_numbers_next_to_the_borders(ops, b, draft):
+    """Random numbers that are the fp32 values next to a probability (tests) or to a border of the cumulative sum (draws),
+    on either side: within 1e-7 of it, and by the widths of these distributions never within the 1e-11 of 64-bit sums."""
+    for seed in range(4):
+        w = Walk([4] * b, 20011, torch.float32, draft, seed, temps=(1.0, 0.6, 1.4), spread=1.0)
+        start = torch.arange(b).repeat_interleave(4) * 4
+        above = start + w.parents.clamp(min=0)
+        p = torch.softmax(w.logits.double() / w.temps.double().repeat_interleave(4)[:, None], -1)
+        tok = w.tokens.long()
+        near = p[above, tok] / (w.draft[above, tok].double() if draft else 1.0)
+        w.u = near.clamp(max=1.0).float()
+        pick = torch.randint(0, 20011, (b,), generator=torch.Generator().manual_seed(seed))
+        w.ud = p[::4].cumsum(-1)[torch.arange(b), pick].float()  # of the root, where its children are rejected or none
+        if seed % 2:
+            w.u, w.ud = torch.nextafter(w.u, torch.ones(())), torch.nextafter(w.ud, torch.zeros(()))
+        w.parents[torch.arange(0, 4 * b, 4 * 3)[:, None] + torch.arange(1, 4)] = -1  # every third tree: the draw alone
+        w.check(ops)
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_walk_full_vocabulary_flat_and_peaked(ops, dtype):
     for spread, seed in ((0.0, 1), (0.1, 2), (8.0, 3)):
