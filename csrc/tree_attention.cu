@@ -42,7 +42,7 @@ constexpr float LOG2E = 1.4426950408889634f;
 constexpr float RAISE = 8.f;            // the running maximum follows once a row's grows by 2^8
 // First warp of each role; 0-7: softmax, whose rows up to 64 are with warps 0, 1, 4 and 5: the polling MMA warps share
 // the other warps' schedulers.
-constexpr int W_TMA = 8, W_Q = 9, W_MMA = 10, W_CONV = 12;
+constexpr int W_TMA = 8, W_MMA = 10, W_CONV = 12;
 constexpr int BAD_WORDS = TREE_MAX_NODES / 32;
 constexpr float NOTHING = -3e38f;       // below any score
 
@@ -80,25 +80,41 @@ __device__ __forceinline__ int seq_begin(const TreeAttn& t, int b) { return min(
 __device__ __forceinline__ int seq_nodes(const TreeAttn& t, int b) { return min(t.cu_q[b + 1], t.T) - seq_begin(t, b); }
 __device__ __forceinline__ int seq_rows(const Args& a, int b) { return min(seq_nodes(a.t, b), a.t.max_nodes) * a.G; }
 __device__ __forceinline__ int seq_tiles(const TreeAttn& t, int b) { return max(1, (t.ctx_lens[b] + KT - 1) / KT); }
-// Its work: a tile counts twice where it meets more than 128 rows.
+// Its work, in units of some 1000 clocks: a tile that meets more than 128 rows takes ALL_ROWS (the exponentials), one
+// that meets fewer takes FEW_ROWS (its bytes, or up to 64 rows a tile's round), and an item (a sequence, a stretch of
+// rows, a KV head) ITEM_WORK whatever its tiles (queries, first maximum, outputs).  With stretches of equal products the
+// slowest CTA took 470000 clocks where most took 335000, with ITEM_WORK 0 more (24 x up to 64 nodes, 64 heads, 600 to
+// 8000 tokens).
+constexpr int ALL_ROWS = 4, FEW_ROWS = 3, ITEM_WORK = 12;
+struct Work {
+  int tiles;
+  int64_t twice;  // items of more than 128 rows, which come first
+  int64_t per2, per1;  // work of an item
+  __device__ __forceinline__ Work(const Args& a, int b) {
+    const int rows = seq_rows(a, b);
+    tiles = seq_tiles(a.t, b);
+    twice = a.rows_cap > 128 ? (int64_t)a.t.nkv * (rows / 256 + (rows % 256 > 128 ? 1 : 0)) : 0;
+    per2 = ITEM_WORK + (int64_t)ALL_ROWS * tiles;
+    per1 = ITEM_WORK + (int64_t)FEW_ROWS * tiles;
+  }
+  // the tile (of sequence b's part of the list) in which its work unit `w` lies; the first one takes the item's own
+  __device__ __forceinline__ int64_t tile(int64_t w) const {
+    const bool two = w < twice * per2;
+    if (!two) w -= twice * per2;
+    const int64_t item = w / (two ? per2 : per1), at = w % (two ? per2 : per1) - ITEM_WORK;
+    return (item + (two ? 0 : twice)) * tiles + (at <= 0 ? 0 : at / (two ? ALL_ROWS : FEW_ROWS));
+  }
+  // the units ahead of the item that begins with tile i
+  __device__ __forceinline__ int64_t ahead(int64_t i) const {
+    const int64_t item = i / tiles;
+    return item <= twice ? item * per2 : twice * per2 + (item - twice) * per1;
+  }
+};
 __device__ __forceinline__ int64_t seq_work(const Args& a, int b) {
   const int rows = seq_rows(a, b);
   if (rows <= 0) return 0;
-  const int rts = (rows + a.rows_cap - 1) / a.rows_cap, last = rows - (rts - 1) * a.rows_cap;
-  return (int64_t)seq_tiles(a.t, b) * a.t.nkv * ((a.rows_cap > 128 ? 2 : 1) * (rts - 1) + (last > 128 ? 2 : 1));
-}
-// The tile (of sequence b's part of the list) in which its work unit `w` lies, and the units ahead of tile `i`.
-__device__ __forceinline__ int64_t work_tile(const Args& a, int b, int64_t w) {
-  if (a.rows_cap <= 128) return w;
-  const int rows = seq_rows(a, b);
-  const int64_t twice = (int64_t)seq_tiles(a.t, b) * a.t.nkv * (rows / 256 + (rows % 256 > 128 ? 1 : 0));
-  return w < 2 * twice ? w / 2 : w - twice;
-}
-__device__ __forceinline__ int64_t tile_work(const Args& a, int b, int64_t i) {
-  if (a.rows_cap <= 128) return i;
-  const int rows = seq_rows(a, b);
-  const int64_t twice = (int64_t)seq_tiles(a.t, b) * a.t.nkv * (rows / 256 + (rows % 256 > 128 ? 1 : 0));
-  return i < twice ? 2 * i : i + twice;
+  const Work w(a, b);
+  return w.ahead((int64_t)a.t.nkv * ((rows + a.rows_cap - 1) / a.rows_cap) * w.tiles);
 }
 
 // Stretch c of the list: from tile lo_tile of sequence lo_seq to ahead of tile hi_tile of hi_seq.  In units of work:
@@ -139,11 +155,11 @@ __device__ void find_chunk(const Args& a, int c, Spot* out, int64_t* part) {
     const int64_t n = seq_work(a, b);
     if (lo >= at && lo < at + n) {
       out->lo_seq = b;
-      out->lo_tile = work_tile(a, b, lo - at);
+      out->lo_tile = Work(a, b).tile(lo - at);
     }
     if (hi >= at && hi < at + n) {
       out->hi_seq = b;
-      out->hi_tile = work_tile(a, b, hi - at);
+      out->hi_tile = Work(a, b).tile(hi - at);
       out->hi_ahead = at;
     }
     at += n;
@@ -219,7 +235,7 @@ __device__ __forceinline__ uint32_t tile_at(int r, int c16) {
 
 struct Small {  // shared memory besides the tiles
   uint64_t full[8], empty[8], raw_full[8], raw_empty[8];
-  uint64_t q_full, q_empty, s_full[2], p_ready[2], o_done[2], o_empty, drain[2];
+  uint64_t q_full, s_full[2], p_ready[2], o_done[2], o_empty, drain[2];
   uint64_t scale_full[4];
   float2 ml[2][128];        // (maximum, sum) of the groups' rows
   float2 scale[4][KT / 16];  // e4m3: (K, V) scales of 16 keys, of the last four tiles
@@ -263,6 +279,69 @@ __device__ __forceinline__ void convert_tile(const uint8_t* src, uint8_t* dst, i
   }
 }
 
+// One warp: queries of rows R .. R + rows - 1 (at most 128) of KV head h as a tile of the products (dims 64.. `half` bytes
+// on).  Two rows a step, four steps at a time, whose places in the tile repeat every 1024 bytes.
+__device__ __forceinline__ void load_q(const Args& a, int b, int h, int R, int rows, uint32_t dst, int half, int lane) {
+  const int c = lane & 15, r0 = lane >> 4, two_gh = 2 % a.G;
+  const int64_t stride = a.t.q_stride, two = 2 / a.G * stride;
+  int gh = (R + r0) % a.G;
+  const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(a.t.q) + (seq_begin(a.t, b) + (R + r0) / a.G) * stride +
+                           (int64_t)h * a.G * AD + c * 8;
+  dst += (c >> 3) * half + r0 * 128;
+  for (int r = r0; r < rows; r += 8, dst += 1024) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const __nv_bfloat16* src = q + gh * AD;
+      const uint32_t to = dst + j * 256 + (((c & 7) ^ (r0 + 2 * j)) << 4);
+      if (r + 2 * j < rows) {
+        if (a.q16) {
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(src) : "memory");
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to + 4 * e), "l"(src + 2 * e) : "memory");
+        }
+      }
+      gh += two_gh;
+      q += two;
+      if (gh >= a.G) {
+        gh -= a.G;
+        q += stride;
+      }
+    }
+  }
+}
+
+// Row r of a V tile without its infinities and NaN, all zeros `behind` the context; whether there were any.
+__device__ __forceinline__ bool clean_row(uint8_t* v, int r, bool behind) {
+  uint32_t any = 0;
+#pragma unroll
+  for (int h = 0; h < 16 && !behind; h += 8) {  // eight loads on their way: nearly all rows are left as they are
+    uint4 x[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = *reinterpret_cast<const uint4*>(v + tile_at(r, h + i));
+#pragma unroll
+    for (int i = 0; i < 8; ++i) any |= odd_halves(x[i].x) | odd_halves(x[i].y) | odd_halves(x[i].z) | odd_halves(x[i].w);
+  }
+  if (behind) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) *reinterpret_cast<uint4*>(v + tile_at(r, i)) = make_uint4(0, 0, 0, 0);
+  }
+  if (any) {
+#pragma unroll 1
+    for (int i = 0; i < 16; ++i) {
+      uint4& at = *reinterpret_cast<uint4*>(v + tile_at(r, i));
+      uint4 x = at;
+      x.x &= ~((odd_halves(x.x) >> 15) * 0xffffu);
+      x.y &= ~((odd_halves(x.y) >> 15) * 0xffffu);
+      x.z &= ~((odd_halves(x.z) >> 15) * 0xffffu);
+      x.w &= ~((odd_halves(x.w) >> 15) * 0xffffu);
+      at = x;
+    }
+  }
+  return any != 0;
+}
+
 // Keys [key0, key0 + 64) that a row sees, as bits: those before the tree and its mask's, within the context.
 __device__ __forceinline__ uint64_t visible(const uint64_t (&mask)[TREE_WORDS], int key0, int base, int k_len) {
   const int d = base - key0;
@@ -293,8 +372,8 @@ __device__ __forceinline__ void st32(void* p, const uint32_t (&v)[8]) {
                : "memory");
 }
 
-// With 512 threads (e4m3) the block starts with 128 registers per thread; the softmax warps take more from the other
-// warpgroups: 2 x 176 + 56 + 104 = 4 x 128.
+// The block starts with 128 (e4m3: 512 threads) or 168 registers per thread; the softmax warps take more from the
+// other warpgroups: 2 x 176 + 56 + 104 = 4 x 128, 2 x 208 + 88 = 3 x 168.
 template <int N>
 __device__ __forceinline__ void regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N>
@@ -411,8 +490,7 @@ __global__ void __launch_bounds__(FP8 ? 512 : 384, 1)
       tc::mbar_init(bar(sh.raw_full[s]), 1);
       tc::mbar_init(bar(sh.raw_empty[s]), 4);
     }
-    tc::mbar_init(bar(sh.q_full), 1);
-    tc::mbar_init(bar(sh.q_empty), 2);
+    tc::mbar_init(bar(sh.q_full), 8);
     for (int g = 0; g < 2; ++g) {
       tc::mbar_init(bar(sh.s_full[g]), 1);
       tc::mbar_init(bar(sh.p_ready[g]), 4);
@@ -436,7 +514,7 @@ __global__ void __launch_bounds__(FP8 ? 512 : 384, 1)
 
   if (warp < W_TMA) {
     // ------------------------------------------------------------------ softmax, outputs
-    if constexpr (FP8) regs_inc<176>();
+    regs_inc<FP8 ? 176 : 208>();
     const int g = warp >> 2, q4 = warp & 3, lr = q4 * 32 + lane;  // TMEM lane = row of the group
     const uint32_t lanes = (uint32_t)(q4 * 32) << 16;
     const uint32_t s_tm = tmem + g * 128u + lanes, o_tm = tmem + 256u + lanes;  // O of group k: + 128 k
@@ -447,16 +525,49 @@ __global__ void __launch_bounds__(FP8 ? 512 : 384, 1)
     auto turn_pass = [&]() { asm volatile("bar.arrive %0, 256;" ::"r"(3 - g) : "memory"); };
     if (g == 1) turn_pass();
     int tile0 = 0, items = 0;  // tiles before this item
-    for (Walk w(a, sh.spot); w.more(); w.next(a), ++items) {
-      const int n = w.t1 - w.t0, rows = w.rows(a), two = rows > 128, steps = two ? 2 * n : n;
-      const int row = two ? g * 128 + lr : lr, R = w.rt * a.rows_cap + row;
-      const bool live = row < rows, work = __any_sync(FULL_MASK, live);
-      const int qrow = seq_begin(a.t, w.b), nodes = seq_nodes(a.t, w.b), k_len = a.t.ctx_lens[w.b], base = k_len - nodes;
-      const int node = live ? R / a.G : 0, head = w.h * a.G + (live ? R % a.G : 0);
-      uint64_t bits[TREE_WORDS];  // the row's mask
+    // An item's queries, by the eight warps: one alone took 20000 clocks for 256 rows.  The next item's are on their way
+    // while this one's outputs are written.
+    auto fetch_q = [&](const Walk& w) {
+      const int rows = w.rows(a), per = rows > 128 ? 32 : 16, r = warp * per;
+      load_q(a, w.b, w.h, w.rt * a.rows_cap + r, min(per, rows - r), smem_u32(sq) + (r >> 7) * TILE + (r & 127) * 128, HALF, lane);
+    };
+    struct Row {  // what a thread has to know of its row
+      int row, qrow, nodes, k_len, node, gh;
+      uint64_t bits[TREE_WORDS];  // the mask
+    };
+    auto row_of = [&](const Walk& w) {
+      Row r;
+      const int rows = w.rows(a);
+      r.row = rows > 128 ? g * 128 + lr : lr;
+      const int R = w.rt * a.rows_cap + r.row;
+      const bool live = r.row < rows;
+      r.qrow = seq_begin(a.t, w.b);
+      r.nodes = seq_nodes(a.t, w.b);
+      r.k_len = a.t.ctx_lens[w.b];
+      r.node = live ? R / a.G : 0;
+      r.gh = live ? R % a.G : 0;
 #pragma unroll
       for (int i = 0; i < TREE_WORDS; ++i)
-        bits[i] = i < a.t.words ? (uint64_t)a.t.mask[(int64_t)(qrow + node) * a.t.mask_stride + i] : 0ull;
+        r.bits[i] = i < a.t.words ? (uint64_t)a.t.mask[(int64_t)(r.qrow + r.node) * a.t.mask_stride + i] : 0ull;
+      return r;
+    };
+    Walk next(a, sh.spot);
+    Row next_row;
+    if (next.more()) {
+      fetch_q(next);
+      next_row = row_of(next);
+    }
+    for (; next.more(); ++items) {
+      const Walk w = next;
+      next.next(a);
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      tc::fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive_release(bar(sh.q_full));
+      const int n = w.t1 - w.t0, rows = w.rows(a), two = rows > 128, steps = two ? 2 * n : n;
+      const Row me = next_row;
+      const int row = me.row, qrow = me.qrow, k_len = me.k_len, base = k_len - me.nodes, node = me.node, head = w.h * a.G + me.gh;
+      const bool live = row < rows, work = __any_sync(FULL_MASK, live);
       float m = -INFINITY, l = 0.f;
       int mine = 0;
       for (int st = g; st < steps; st += 2, ++mine, ++n_done) {
@@ -472,7 +583,7 @@ __global__ void __launch_bounds__(FP8 ? 512 : 384, 1)
           constexpr bool MASK = decltype(with_mask)::value;
           uint32_t see[4] = {~0u, ~0u, ~0u, ~0u}, x[2][16], p[64];
           if constexpr (MASK) {
-            const uint64_t s0 = visible(bits, t * KT, base, k_len), s1 = visible(bits, t * KT + 64, base, k_len);
+            const uint64_t s0 = visible(me.bits, t * KT, base, k_len), s1 = visible(me.bits, t * KT + 64, base, k_len);
             see[0] = (uint32_t)s0;
             see[1] = (uint32_t)(s0 >> 32);
             see[2] = (uint32_t)s1;
@@ -550,6 +661,7 @@ __global__ void __launch_bounds__(FP8 ? 512 : 384, 1)
             m = nm;
             weights(m == -INFINITY ? 0.f : m);
           }
+          turn_pass();
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
             uint32_t(&pc)[16] = *reinterpret_cast<uint32_t(*)[16]>(p + 16 * c);
@@ -565,8 +677,9 @@ __global__ void __launch_bounds__(FP8 ? 512 : 384, 1)
             softmax(std::true_type());
           else
             softmax(std::false_type());
+        } else {
+          turn_pass();
         }
-        turn_pass();
         if (masked) {
           // this group's threads look through V, a key each: positions behind the context hold any bits, and
           // a node's infinities and NaN go to the rows that see it at the end.  (Where both groups use the tile, both
@@ -575,25 +688,7 @@ __global__ void __launch_bounds__(FP8 ? 512 : 384, 1)
           wait(sh.full[c % S], (c / S) & 1, 12);
           uint8_t* v = ring + (c % S) * TILE;
           if (pos >= base) {
-            bool odd = false;
-#pragma unroll 4
-            for (int i = 0; i < 16; ++i) {
-              uint4& x = *reinterpret_cast<uint4*>(v + tile_at(lr, i));
-              if (pos >= k_len) {
-                x = make_uint4(0, 0, 0, 0);
-                continue;
-              }
-              uint4 y = x;
-              const uint32_t o[4] = {odd_halves(y.x), odd_halves(y.y), odd_halves(y.z), odd_halves(y.w)};
-              if (o[0] | o[1] | o[2] | o[3]) {
-                odd = true;
-                y.x &= ~((o[0] >> 15) * 0xffffu);
-                y.y &= ~((o[1] >> 15) * 0xffffu);
-                y.z &= ~((o[2] >> 15) * 0xffffu);
-                y.w &= ~((o[3] >> 15) * 0xffffu);
-                x = y;
-              }
-            }
+            const bool odd = clean_row(v, lr, pos >= k_len);
             const int nd = pos - base;
             if (odd && nd >= 0 && nd < TREE_MAX_NODES) atomicOr(&sh.bad[items & 1][nd >> 5], 1u << (nd & 31));
           }
@@ -613,6 +708,10 @@ __global__ void __launch_bounds__(FP8 ? 512 : 384, 1)
       tc::fence_before();
       asm volatile("bar.sync 1, 256;" ::: "memory");
       tc::fence_after();
+      if (next.more()) {  // every product with this item's queries has been waited for
+        fetch_q(next);
+        next_row = row_of(next);
+      }
       const float2 ml0 = sh.ml[0][lr], ml1 = sh.ml[1][lr];
       uint32_t any = 0;
 #pragma unroll
@@ -692,7 +791,7 @@ __global__ void __launch_bounds__(FP8 ? 512 : 384, 1)
     }
     tc::fence_before();
   } else if (warp < W_CONV) {
-    if constexpr (FP8) regs_dec<56>();
+    regs_dec<FP8 ? 56 : 88>();
     if (warp == W_TMA) {
       // ---------------------------------------------------------------- TMA producer
       if (lane == 0) {
@@ -794,10 +893,6 @@ __global__ void __launch_bounds__(FP8 ? 512 : 384, 1)
             k_at.step(by, S);
             ++done;
           }
-          if (i == mine - 1 || mine == 0) {  // Q has been read
-            if (elect_one()) tc::commit<1>(bar(sh.q_empty));
-            __syncwarp();
-          }
         }
         const int on = begin.s + 2 * n;
         begin.ph ^= (uint32_t)(on / S) & 1;
@@ -807,31 +902,6 @@ __global__ void __launch_bounds__(FP8 ? 512 : 384, 1)
       __syncwarp();
       if (lane == 0) tc::mbar_drain(bar(sh.drain[g]), 0);
       __syncwarp();
-    } else {
-      static_assert(W_Q == W_TMA + 1 && W_MMA == W_Q + 1, "");
-      // ---------------------------------------------------------------- Q
-      int items = 0;
-      for (Walk w(a, sh.spot); w.more(); w.next(a), ++items) {
-        if (items > 0) wait(sh.q_empty, (items - 1) & 1, 14);  // the products of the item before have read theirs
-        const int rows = w.rows(a), R0 = w.rt * a.rows_cap;
-        const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(a.t.q) + (int64_t)seq_begin(a.t, w.b) * a.t.q_stride + (int64_t)w.h * a.G * AD;
-        for (int i = lane; i < rows * 16; i += 32) {
-          const int r = i >> 4, c = i & 15, R = R0 + r;
-          const __nv_bfloat16* src = q + (int64_t)(R / a.G) * a.t.q_stride + (R % a.G) * AD + c * 8;
-          const uint32_t dst = smem_u32(sq + (r >> 7) * TILE) + tile_at(r & 127, c);
-          if (a.q16) {
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-          } else {
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst + 4 * e), "l"(src + 2 * e) : "memory");
-          }
-        }
-        asm volatile("cp.async.wait_all;" ::: "memory");
-        tc::fence_proxy_async();
-        __syncwarp();
-        if (lane == 0) tc::mbar_arrive_release(bar(sh.q_full));
-      }
     }
   } else if constexpr (FP8) {
     // ------------------------------------------------------------------ e4m3 -> bf16 tiles
@@ -1140,25 +1210,7 @@ __global__ void __launch_bounds__(FP8 ? 512 : 256, 1)
           wait(sh.full[c % S], (c / S) & 1, 12);
           uint8_t* v = ring + (c % S) * TILE;
           if (pos >= base) {
-            bool odd = false;
-#pragma unroll 4
-            for (int i = 0; i < 16; ++i) {
-              uint4& q = *reinterpret_cast<uint4*>(v + tile_at(kq, i));
-              if (pos >= k_len) {
-                q = make_uint4(0, 0, 0, 0);
-                continue;
-              }
-              uint4 y = q;
-              const uint32_t o[4] = {odd_halves(y.x), odd_halves(y.y), odd_halves(y.z), odd_halves(y.w)};
-              if (o[0] | o[1] | o[2] | o[3]) {
-                odd = true;
-                y.x &= ~((o[0] >> 15) * 0xffffu);
-                y.y &= ~((o[1] >> 15) * 0xffffu);
-                y.z &= ~((o[2] >> 15) * 0xffffu);
-                y.w &= ~((o[3] >> 15) * 0xffffu);
-                q = y;
-              }
-            }
+            const bool odd = clean_row(v, kq, pos >= k_len);
             const int nd = pos - base;
             if (odd && nd >= 0 && nd < TREE_MAX_NODES) atomicOr(&sh.bad[items & 1][nd >> 5], 1u << (nd & 31));
           }
@@ -1300,25 +1352,9 @@ __global__ void __launch_bounds__(FP8 ? 512 : 256, 1)
       const int qb = items % QB;
       if (items >= QB) wait(sh.q_empty[qb], (items / QB - 1) & 1, 14);
       const int rows = w.rows(a), c = lane & 15;
-      int r = lane >> 4, node = r / a.G, gh = r % a.G;
-      const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(a.t.q) + (int64_t)seq_begin(a.t, w.b) * a.t.q_stride + (int64_t)w.h * a.G * AD + c * 8;
-#pragma unroll 1
-      for (; r < N; r += 2) {
-        uint8_t* dst = sq + qb * QT + (c >> 3) * QHALF + r * 128 + (((c & 7) ^ (r & 7)) << 4);
-        if (r >= rows) {  // no row: scores of 0
-          *reinterpret_cast<uint4*>(dst) = make_uint4(0, 0, 0, 0);
-          continue;
-        }
-        const __nv_bfloat16* src = q + (int64_t)node * a.t.q_stride + gh * AD;
-        for (gh += 2; gh >= a.G; gh -= a.G) ++node;
-        if (a.q16) {
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(dst) + 4 * e), "l"(src + 2 * e) : "memory");
-        }
-      }
+      load_q(a, w.b, w.h, 0, rows, smem_u32(sq + qb * QT), QHALF, lane);
+      for (int r = rows + (lane >> 4); r < N; r += 2)  // no row: scores of 0
+        *reinterpret_cast<uint4*>(sq + qb * QT + (c >> 3) * QHALF + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = make_uint4(0, 0, 0, 0);
       asm volatile("cp.async.wait_all;" ::: "memory");
       tc::fence_proxy_async();
       __syncwarp();
@@ -1448,7 +1484,9 @@ __global__ void __launch_bounds__(FP8 ? 512 : 256, 1)
 }
 
 // ---------------------------------------------------------------------------- joining
-// CTA (chunk, 4 rows) joins the item that begins in its chunk and ends in a later one.
+// CTA (chunk, JOIN_ROWS rows) joins the item that begins in its chunk and ends in a later one, a warp four rows at a
+// time: their loads are independent.
+constexpr int JOIN_ROWS = 16;
 __global__ void __launch_bounds__(128) tree_join_kernel(Args a) {
   pdl_wait();     // the partial sums come from the previous kernel in the stream
   pdl_trigger();  // the next kernel may start its prologue
@@ -1461,44 +1499,66 @@ __global__ void __launch_bounds__(128) tree_join_kernel(Args a) {
   const int tiles = seq_tiles(a.t, b), per = tiles * a.t.nkv;
   const int rt = (int)(spot.hi_tile / per), r0 = (int)(spot.hi_tile % per), h = r0 / tiles, t = r0 % tiles;
   // the item that this chunk's end cuts: its first tile and its work
-  const int64_t first = spot.hi_tile - t, begin = spot.hi_ahead + tile_work(a, b, first),
-                end = spot.hi_ahead + tile_work(a, b, first + tiles), unit = (end - begin) / tiles;
+  const Work work(a, b);
+  const int64_t first = spot.hi_tile - t, begin = spot.hi_ahead + work.ahead(first);
+  const int unit = first < work.twice * tiles ? ALL_ROWS : FEW_ROWS;
   // tiles of it ahead of a place in the list
-  auto ahead = [&](int64_t w) { return w <= begin ? (int64_t)0 : w >= end ? (int64_t)tiles : (w - begin) / unit; };
+  auto ahead = [&](int64_t w) {
+    w -= begin + ITEM_WORK;
+    return w <= 0 ? (int64_t)0 : min((int64_t)tiles, w / unit);
+  };
   auto edge = [&](int k) { return spot.total * k / a.chunks; };
   // (a chunk whose place lies inside the item's first tile begins with it)
-  if (t == 0 || edge(chunk) >= begin + unit) return;  // nothing is cut here, or the item begins in an earlier chunk
+  if (t == 0 || edge(chunk) >= begin + ITEM_WORK + unit) return;  // nothing is cut here, or it begins in an earlier chunk
   const int rows = min(a.rows_cap, seq_rows(a, b) - rt * a.rows_cap);
-  const int r = blockIdx.y * 4 + (threadIdx.x >> 5), c = (threadIdx.x & 31) * 4;
-  if (r >= rows) return;
-  float M = -INFINITY, L = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+  constexpr int N = JOIN_ROWS / 4;
+  const int row0 = blockIdx.y * JOIN_ROWS + (threadIdx.x >> 5) * N, c = (threadIdx.x & 31) * 4;
+  if (row0 >= rows) return;
+  float M[N], L[N], o[N][4];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    M[i] = -INFINITY;
+    L[i] = o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+  }
   int64_t from = 0;
   for (int k = chunk; from < tiles; ++k) {
     const int64_t upto = ahead(edge(k + 1));
     if (upto > from) {  // with less work than chunks, some have none
       const float* po = slot_o(a, k, from == 0);
-      const float2 ml = *reinterpret_cast<const float2*>(po + (int64_t)a.rows_cap * AD + r * 2);
-      const float4 v = *reinterpret_cast<const float4*>(po + (int64_t)r * AD + c);
-      if (!(ml.x == -INFINITY && ml.y == 0.f)) {
-        const float nm = fmaxf(M, ml.x), nb = nm == -INFINITY ? 0.f : nm;
-        const float f = L == 0.f && M == -INFINITY ? 0.f : ex2(M - nb), g = ex2(ml.x - nb);
-        M = nm;
-        L = L * f + g * ml.y;
-        o[0] = (f == 0.f ? 0.f : o[0] * f) + g * v.x;
-        o[1] = (f == 0.f ? 0.f : o[1] * f) + g * v.y;
-        o[2] = (f == 0.f ? 0.f : o[2] * f) + g * v.z;
-        o[3] = (f == 0.f ? 0.f : o[3] * f) + g * v.w;
+      float2 ml[N];
+      float4 v[N];
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int r = min(row0 + i, rows - 1);
+        ml[i] = *reinterpret_cast<const float2*>(po + (int64_t)a.rows_cap * AD + r * 2);
+        v[i] = *reinterpret_cast<const float4*>(po + (int64_t)r * AD + c);
+      }
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        if (ml[i].x == -INFINITY && ml[i].y == 0.f) continue;
+        const float nm = fmaxf(M[i], ml[i].x), nb = nm == -INFINITY ? 0.f : nm;
+        const float f = L[i] == 0.f && M[i] == -INFINITY ? 0.f : ex2(M[i] - nb), g = ex2(ml[i].x - nb);
+        M[i] = nm;
+        L[i] = L[i] * f + g * ml[i].y;
+        o[i][0] = (f == 0.f ? 0.f : o[i][0] * f) + g * v[i].x;
+        o[i][1] = (f == 0.f ? 0.f : o[i][1] * f) + g * v[i].y;
+        o[i][2] = (f == 0.f ? 0.f : o[i][2] * f) + g * v[i].z;
+        o[i][3] = (f == 0.f ? 0.f : o[i][3] * f) + g * v[i].w;
       }
       from = upto;
     }
   }
-  const float inv = L != 0.f ? 1.f / L : 0.f;
-  float v[4] = {o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};
-  if (L == 0.f) v[0] = v[1] = v[2] = v[3] = 0.f;
-  const int R = rt * a.rows_cap + r;
-  *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(a.t.out) +
-                            ((int64_t)(seq_begin(a.t, b) + R / a.G) * a.t.nq + h * a.G + R % a.G) * AD + c) =
-      f32_to_bf16x4(v);
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    if (row0 + i >= rows) return;
+    const float inv = L[i] != 0.f ? 1.f / L[i] : 0.f;
+    float v[4] = {o[i][0] * inv, o[i][1] * inv, o[i][2] * inv, o[i][3] * inv};
+    if (L[i] == 0.f) v[0] = v[1] = v[2] = v[3] = 0.f;
+    const int R = rt * a.rows_cap + row0 + i;
+    *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(a.t.out) +
+                              ((int64_t)(seq_begin(a.t, b) + R / a.G) * a.t.nq + h * a.G + R % a.G) * AD + c) =
+        f32_to_bf16x4(v);
+  }
 }
 
 PFN_cuTensorMapEncodeTiled_v12000 encoder() {
@@ -1604,7 +1664,7 @@ cudaError_t launch_tree_attention(const TreeAttn& t, const TreeAttnPlan& p, cuda
     return cudaErrorInvalidValue;
   cudaError_t e = t.kv_fp8 ? launch_rows<true>(km, vm, a, stream) : launch_rows<false>(km, vm, a, stream);
   if (e != cudaSuccess) return e;
-  return launch_pdl(tree_join_kernel, dim3(a.chunks, a.rows_cap / 4), dim3(128), 0, stream, a);
+  return launch_pdl(tree_join_kernel, dim3(a.chunks, a.rows_cap / JOIN_ROWS), dim3(128), 0, stream, a);
 }
 
 int tree_attn_error_code(int reset) {
