@@ -66,10 +66,10 @@ __global__ void tree_mask_kernel(const int* __restrict__ parents, const int* __r
 // before it writes them needs no other order.  Every byte is read and written once; a call for one sequence is
 // bound by the launch and two dependent reads (path, then rows).
 constexpr int CT = 256;   // threads per CTA
-constexpr int BATCH = 8;  // rows in flight per group
+constexpr int BATCH = 4;  // rows in flight per group: four CTAs per SM, with eight three
 
 template <bool FP8>
-__global__ void __launch_bounds__(CT, FP8 ? 3 : 4) tree_commit_kernel(TreeCommit a) {
+__global__ void __launch_bounds__(CT, 4) tree_commit_kernel(TreeCommit a) {
   pdl_wait();     // inputs come from the previous kernel in the stream
   pdl_trigger();  // the next kernel may start its prologue
   constexpr int LANES = FP8 ? 8 : 16;  // lanes of 16 bytes per row
@@ -208,10 +208,11 @@ cudaError_t launch_tree_commit(const TreeCommit& a, cudaStream_t stream) {
   if (a.num_seqs <= 0 || a.num_seqs > 65535 || a.layers <= 0 || a.nkv <= 0 || a.block_size <= 0 || a.max_path <= 0 ||
       a.max_nodes <= 0 || a.max_nodes > TREE_MAX_NODES)
     return cudaErrorInvalidValue;
-  // a CTA's way to its first row takes some microseconds: no more CTAs than run at a time, about four per SM, each
-  // for several units
+  // CTAs per sequence: in all as many as four rounds of four per SM, since paths differ in length; a group of lanes
+  // then has a few units, and a CTA's way to its first row is paid a few times only.  128 trees of 16 nodes, 64
+  // layers, e4m3, at 1, 2, 4, 8, 16, 32 CTAs each: 183, 106, 66, 49, 44, 46 us (115 MB in rows of 128 bytes: 2.6 TB/s).
   const int units = CT / (a.kv_fp8 ? 8 : 16), most = (2 * a.layers * a.nkv + units - 1) / units;
-  const int share = (4 * 148 + a.num_seqs - 1) / a.num_seqs;
+  const int share = (16 * 148 + a.num_seqs - 1) / a.num_seqs;
   const dim3 grid(share < most ? share : most, a.num_seqs);
   if (a.kv_fp8)
     launch_pdl(tree_commit_kernel<true>, grid, dim3(CT), units * ((a.max_nodes - 1) / a.block_size + 2) * sizeof(float),

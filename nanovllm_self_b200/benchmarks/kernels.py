@@ -30,7 +30,8 @@ CASES = ("attn_decode", "attn_decode_fp8", "attn_prefill", "attn_prefill_mma", "
          "attn_prefill_flash_attn", "gemm_prefill", "gemm_decode", "gemm_decode256", "gemm_gate_up_silu256", "qkv_post",
          "qkv_post_fp8", "add_rmsnorm", "silu_mul", "sample", "qkv_post256", "lm_head_sample256", "lm_head_logits_sample256",
          "lm_head_sample256_t", "lm_head_logits_sample256_t", "lm_head_logits256", "fp8_quant", "fp8_norm",
-         "fp8_linear1", "fp8_linear256", "fp8_linear4096", "fp8_linear_silu1", "fp8_linear_silu256", "fp8_linear_silu4096")
+         "fp8_linear1", "fp8_linear256", "fp8_linear4096", "fp8_linear_silu1", "fp8_linear_silu256", "fp8_linear_silu4096",
+         "tree_attn", "tree_attn_fp8", "tree_attn_wide", "tree_verify", "tree_verify_draft", "tree_commit")
 # Qwen3-8B decode GEMM shapes (n, k) for gemm_sweep: qkv, o_proj, gate_up, down_proj, lm_head
 DECODE_SHAPES = {"qkv": ((NQ + 2 * NKV) * D, HID), "o_proj": (HID, NQ * D), "gate_up": (2 * INTER, HID),
                  "down_proj": (HID, INTER), "lm_head": (VOCAB, HID)}
@@ -165,6 +166,32 @@ def build_case(name: str, ops: CudaOps, dev="cuda"):
         if silu:
             return (lambda: ops.linear_silu_fp8(x, w, INTER)), m * k + n * k + m * INTER, 2 * m * n * k
         return (lambda: ops.linear_fp8(x, w)), m * k + n * k + 2 * m * n, 2 * m * n * k
+    if name.startswith("tree"):
+        # 64 trees of 16 drafted tokens ("_wide": 48) over 2048 positions, half of the nodes children of the root
+        B, L = 64, 2048
+        n = 48 if name == "tree_attn_wide" else 16
+        q, kc, vc, ks, vs, c = _paged(B, L, n, name.endswith("fp8"), dev)
+        parents = torch.tensor([-1] + [0] * (n // 2) + list(range(1, n - n // 2)), dtype=torch.int32, device=dev).repeat(B)
+        if name.startswith("tree_attn"):
+            mask, _ = ops.tree_mask(parents, c)
+            kv_bytes = 2 * B * NKV * L * D * kc.element_size()
+            return (lambda: ops.attention_tree(q, kc, vc, c, mask, D ** -0.5, ks, vs)), kv_bytes + 2 * q.numel() * 2, \
+                4 * B * n * NQ * L * D
+        if name.startswith("tree_verify"):
+            # bytes: the roots' rows, which every walk reads; without a draft few go further, since the tokens are
+            # the target's tail
+            logits = 2.0 * torch.randn(B * n, VOCAB, device=dev)
+            draft = torch.softmax(logits + torch.randn_like(logits), -1) if name.endswith("draft") else None
+            logits = logits.to(torch.bfloat16)
+            tokens = torch.randint(0, VOCAB, (B * n,), dtype=torch.int32, device=dev)
+            u, ud, t = torch.rand(B * n, device=dev), torch.rand(B, device=dev), torch.ones(B, device=dev)
+            return (lambda: ops.verify_tree(logits, tokens, parents, c, t, u, ud, draft)), \
+                B * VOCAB * (2 if draft is None else 6), None
+        pool = torch.randn(2, 4, kc.shape[0], NKV, kc.shape[2], D, device=dev).to(torch.bfloat16)
+        path = torch.full((B, n), -1, dtype=torch.int32, device=dev)
+        path[:, :3] = torch.tensor([0, n // 2 - 1, n - 1], device=dev)  # a child of the root, and its child
+        lengths = torch.full((B,), 3, dtype=torch.int32, device=dev)
+        return (lambda: ops.commit_tree(pool, c, path, lengths)), 2 * 2 * B * 2 * 4 * NKV * D * 2, None
     raise ValueError(f"unknown case {name!r}; one of {', '.join(CASES)}")
 
 
