@@ -431,11 +431,12 @@ def test_walk_where_the_draft_is_the_target(ops):
     assert w.want()[1][0] == 1
 
 
+@pytest.mark.parametrize("b", [12, 40])  # 40: summed in fp32 first
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
-def test_walk_infinities_nan_and_odd_numbers(ops, dtype):
+def test_walk_infinities_nan_and_odd_numbers(ops, dtype, b):
     inf, nan = float("inf"), float("nan")
     for v in (5, 3001):
-        w = Walk([3] * 12, v, dtype, False, v, (1.0,))
+        w = Walk([3] * b, v, dtype, False, v, (1.0,))
         x = w.logits
         x[0] = -inf
         x[3, ::2] = nan
@@ -444,7 +445,7 @@ def test_walk_infinities_nan_and_odd_numbers(ops, dtype):
         x[12, 1:] = -inf
         x[15, : v // 2] = -inf
         x[18] = x[18].abs() * 1e30
-        w.temps = torch.tensor([1.0, 1, 1, 1, 1, 1, 1, 1e-30, 1e30, inf, nan, -1])
+        w.temps[:12] = torch.tensor([1.0, 1, 1, 1, 1, 1, 1, 1e-30, 1e30, inf, nan, -1])
         w.tokens[1:3] = torch.tensor([-1, v])
         w.tokens[9:12] = torch.tensor([0, 2, 3])
         w.ud[:7] = torch.tensor([0.5, 1.0, nan, 0.7, -2.0, 1.0, 3.0])
@@ -480,6 +481,13 @@ def test_walk_rows_of_any_alignment(ops):
             d.copy_(w.draft)
             got = ops.verify_tree(big, w.tokens.to(DEV), w.parents.to(DEV), w.ctx, w.temps.to(DEV), w.u.to(DEV), w.ud.to(DEV), d)
             assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+
+@pytest.mark.parametrize("draft", [False, True])
+def test_walk_many_trees_in_rows_of_any_alignment(ops, draft):
+    """More trees than get a CTA of 512 threads, rows of an odd length; a vocabulary in chunks longer than 512 tokens."""
+    Walk([2] * 70, 9001, torch.bfloat16, draft, 3, (1.0, 0.5, 2.0), spread=3.0).check(ops)
+    Walk([1] * 34, 270001, torch.bfloat16, draft, 4, (1.0, 0.5), spread=3.0).check(ops)
 
 
 def test_walk_in_a_graph(ops):
