@@ -13,13 +13,21 @@
 // An e4m3 cache is converted once per value by four more warps, to bf16 (exact); K's scale multiplies the scores, V's
 // the weights before they are rounded.
 //
-// Balance: the tiles of all (sequence, 256 rows, KV head) are laid end to end and cut into equal stretches, one per
-// CTA, whatever the sequences' lengths.  One that is cut leaves partial sums (at most two per CTA), which a second
+// Up to 64 rows (nodes x query heads of a KV head) the roles of the product's sides are exchanged: tree_attn_few_kernel.
+//
+// Balance: the tiles of all (sequence, 256 rows, KV head) are laid end to end and cut into stretches of equal work, one
+// per CTA, whatever the sequences' lengths.  One that is cut leaves partial sums (at most two per CTA), which a second
 // kernel joins in the order of the keys: no atomics, the same bits on every run.
 //
 // Masks: only tiles that reach into the tree look at them.  What a row does not see takes no part in it: its score is
 // -inf, and a value that is infinite or NaN (0 x inf) is taken out of such a tile in shared memory and added at the
 // end to the rows that see it.
+//
+// What bounds it.  Up to 64 rows the bytes of K and V should: 64 trees of 16 nodes, 32 query and 8 KV heads, 2048
+// tokens, bf16: 138 us, 4.0 TB/s (a tile's round of product, maximum, weights and store is longer than its bytes take);
+// 128 trees of 8 on e4m3: 305 us, 1.8 TB/s (a round takes twice as long beside the eight warps that convert).  Beyond, the
+// exponentials: 24 trees of up to 64 nodes, 64 and 8 heads, up to 8191 tokens: 250-270 us, 520-560 TFLOP/s; two groups'
+// weights of a tile take 3800 clocks in turn, the products 2048.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
@@ -40,8 +48,8 @@ constexpr int TILE = 2 * HALF;          // a 128 x 128 tile of 16-bit values
 constexpr int RAW_TILE = KT * AD;       // of 8-bit values
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float RAISE = 8.f;            // the running maximum follows once a row's grows by 2^8
-// First warp of each role; 0-7: softmax, whose rows up to 64 are with warps 0, 1, 4 and 5: the polling MMA warps share
-// the other warps' schedulers.
+// First warp of each role; 0-7: softmax (the polling MMA warps share the schedulers of warps 2, 3, 6 and 7, whose rows are
+// the last); 9 has none: registers are moved between whole warpgroups.
 constexpr int W_TMA = 8, W_MMA = 10, W_CONV = 12;
 constexpr int BAD_WORDS = TREE_MAX_NODES / 32;
 constexpr float NOTHING = -3e38f;       // below any score
@@ -64,7 +72,7 @@ __device__ __forceinline__ uint32_t odd_halves(uint32_t x) { return ((x & 0x7fff
 struct Args {
   TreeAttn t;
   int G, chunks, bs_shift;
-  int rows_cap;     // rows of a CTA: 128 or 256
+  int rows_cap;     // rows of a CTA: 16 to 256
   int slots;        // tiles of the 16-bit ring (K and V in turn)
   int raw_slots;    // and of the e4m3 ring
   int box_rows;     // rows per TMA box: min(128, block size)
@@ -225,6 +233,10 @@ struct Walk {
 // Partial sums of slot s (2 per CTA): rows x 128 outputs (not divided by the sum), then rows x (maximum, sum).
 __device__ __forceinline__ float* slot_o(const Args& a, int cta, int slot) {
   return a.t.ws + (int64_t)(cta * 2 + slot) * a.rows_cap * (AD + 2);
+}
+// Behind them each CTA's end in the list, for the join.
+__device__ __forceinline__ Spot* spot_of(const Args& a, int cta) {
+  return reinterpret_cast<Spot*>(a.t.ws + 2LL * a.chunks * a.rows_cap * (AD + 2)) + cta;
 }
 
 // ------------------------------------------------------------------------ main kernel
@@ -480,7 +492,10 @@ __global__ void __launch_bounds__(FP8 ? 512 : 384, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   auto bar = [](uint64_t& b) { return smem_u32(&b); };
   if (smem_u32(sm) & 1023) {  // the swizzle goes by the address
-    if (threadIdx.x == 0) atomicCAS(&g_tree_error, 0, 9);
+    if (threadIdx.x == 0) {
+      atomicCAS(&g_tree_error, 0, 9);
+      spot_of(a, blockIdx.x)->hi_seq = a.t.num_seqs;  // nothing to join
+    }
     return;
   }
   if (threadIdx.x == 0) {
@@ -506,6 +521,7 @@ __global__ void __launch_bounds__(FP8 ? 512 : 384, 1)
   if (warp == W_MMA) tc::tmem_alloc<1>(smem_u32(&sh.tmem), 512);
   tc::fence_before();
   find_chunk(a, blockIdx.x, &sh.spot, sh.part);  // ends with a barrier
+  if (threadIdx.x == 0) *spot_of(a, blockIdx.x) = sh.spot;
   tc::fence_after();
   const uint32_t tmem = sh.tmem;
   volatile int* gave_up = &sh.gave_up;
@@ -1015,7 +1031,10 @@ __global__ void __launch_bounds__(FP8 ? 512 : 256, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   auto bar = [](uint64_t& b) { return smem_u32(&b); };
   if (smem_u32(sm) & 1023) {  // the swizzle goes by the address
-    if (threadIdx.x == 0) atomicCAS(&g_tree_error, 0, 9);
+    if (threadIdx.x == 0) {
+      atomicCAS(&g_tree_error, 0, 9);
+      spot_of(a, blockIdx.x)->hi_seq = a.t.num_seqs;  // nothing to join
+    }
     return;
   }
   if (threadIdx.x == 0) {
@@ -1042,6 +1061,7 @@ __global__ void __launch_bounds__(FP8 ? 512 : 256, 1)
   if (warp == F_MMA) tc::tmem_alloc<1>(smem_u32(&sh.tmem), 256);
   tc::fence_before();
   find_chunk(a, blockIdx.x, &sh.spot, sh.part);  // ends with a barrier
+  if (threadIdx.x == 0) *spot_of(a, blockIdx.x) = sh.spot;
   tc::fence_after();
   const uint32_t tmem = sh.tmem;  // S^T at 0 and 64, O^T at 128 and 192
   volatile int* gave_up = &sh.gave_up;
@@ -1490,10 +1510,8 @@ constexpr int JOIN_ROWS = 16;
 __global__ void __launch_bounds__(128) tree_join_kernel(Args a) {
   pdl_wait();     // the partial sums come from the previous kernel in the stream
   pdl_trigger();  // the next kernel may start its prologue
-  __shared__ Spot spot;
-  __shared__ int64_t part[4];
   const int chunk = blockIdx.x;
-  find_chunk(a, chunk, &spot, part);
+  const Spot spot = *spot_of(a, chunk);
   const int b = spot.hi_seq;
   if (b >= a.t.num_seqs) return;  // the list's end
   const int tiles = seq_tiles(a.t, b), per = tiles * a.t.nkv;
@@ -1596,7 +1614,7 @@ TreeAttnPlan tree_attn_plan(int max_nodes, int nq, int nkv, int num_sms) {
   const int rows = max_nodes * (nq / nkv);
   p.rows_cap = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : rows <= 128 ? 128 : 256;
   p.chunks = num_sms;
-  p.ws_floats = 2LL * p.chunks * p.rows_cap * (AD + 2);
+  p.ws_floats = 2LL * p.chunks * p.rows_cap * (AD + 2) + p.chunks * (int64_t)(sizeof(Spot) / sizeof(float));
   return p;
 }
 
