@@ -24,9 +24,9 @@
 // end to the rows that see it.
 //
 // What bounds it.  Up to 64 rows the bytes of K and V should: 64 trees of 16 nodes, 32 query and 8 KV heads, 2048
-// tokens, bf16: 138 us, 4.0 TB/s (a tile's round of product, maximum, weights and store is longer than its bytes take);
-// 128 trees of 8 on e4m3: 305 us, 1.8 TB/s (a round takes twice as long beside the eight warps that convert).  Beyond, the
-// exponentials: 24 trees of up to 64 nodes, 64 and 8 heads, up to 8191 tokens: 250-270 us, 520-560 TFLOP/s; two groups'
+// tokens, bf16: 131 us, 4.2 TB/s (a tile's round of product, maximum, weights and store is longer than its bytes take);
+// 128 trees of 8 on e4m3: 300 us, 1.8 TB/s (a round takes twice as long beside the eight warps that convert).  Beyond, the
+// exponentials: 24 trees of up to 64 nodes, 64 and 8 heads, up to 8191 tokens: 241-262 us, 530-580 TFLOP/s; two groups'
 // weights of a tile take 3800 clocks in turn, the products 2048.
 #include <cuda.h>
 #include <cudaTypedefs.h>
