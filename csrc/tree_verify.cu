@@ -14,7 +14,8 @@
 //
 // One cluster of CTAs walks one tree, so only the rows of visited nodes are read.  A row is cut into chunks of
 // 512 tokens; a warp sums a chunk relative to the chunk's maximum and sends (sum, maximum) to every CTA of the
-// cluster, whose first warps then take the same decisions from the same numbers: one cluster barrier per row.
+// cluster, whose first warps then take the same decisions from the same numbers: one cluster barrier per row, and one
+// ahead of the first, since a CTA's shared memory may be written to from outside only once it has started.
 #include "common.cuh"
 #include "tcgen05.cuh"
 #include "tree.h"
@@ -484,6 +485,7 @@ __device__ __noinline__ void sum_again(const void* row, const Cut& cut, const Di
 template <bool BF16, int VT, bool FAST>
 __global__ void __launch_bounds__(VT, VT == 512 ? 1 : FAST || BF16 ? 3 : 2) tree_verify_kernel(TreeVerify a, int len) {
   constexpr int VWARPS = VT / 32;
+  tc::cluster_arrive();  // this CTA has started; waited for below, ahead of the first store to another CTA
   pdl_wait();     // inputs come from the previous kernel in the stream
   pdl_trigger();  // the next kernel may start its prologue
   extern __shared__ __align__(16) uint8_t vsm[];
@@ -503,6 +505,7 @@ __global__ void __launch_bounds__(VT, VT == 512 ? 1 : FAST || BF16 ? 3 : 2) tree
         a.next_token[b] = -1;
       }
     }
+    tc::cluster_wait();
     return;
   }
   for (int i = threadIdx.x; i < n; i += VT) {
@@ -767,6 +770,7 @@ __global__ void __launch_bounds__(VT, VT == 512 ? 1 : FAST || BF16 ? 3 : 2) tree
   };
 
   ChunkSum* sums = nullptr;
+  tc::cluster_wait();  // every CTA of the cluster has started
   while (true) {
     const int64_t r = (int64_t)t0 + node;
     constexpr int E = BF16 ? 2 : 4;
