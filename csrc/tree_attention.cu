@@ -247,7 +247,10 @@ __device__ __forceinline__ uint32_t tile_at(int r, int c16) {
 
 struct Small {  // shared memory besides the tiles
   uint64_t full[8], empty[8], raw_full[8], raw_empty[8];
-  uint64_t q_full, s_full[2], p_ready[2], o_done[2], o_empty, drain[2];
+  // q_full: one per group, and only items in which the group has steps arrive at it.  With one barrier for both, an item
+  // of a single step, which group 1 takes no part in, could be over before group 1's MMA warp had looked: two such
+  // items on, the barrier's parity is what it was and the warp waits for an item that it is already behind.
+  uint64_t q_full[2], s_full[2], p_ready[2], o_done[2], o_empty, drain[2];
   uint64_t scale_full[4];
   float2 ml[2][128];        // (maximum, sum) of the groups' rows
   float2 scale[4][KT / 16];  // e4m3: (K, V) scales of 16 keys, of the last four tiles
@@ -505,8 +508,8 @@ __global__ void __launch_bounds__(FP8 ? 512 : 384, 1)
       tc::mbar_init(bar(sh.raw_full[s]), 1);
       tc::mbar_init(bar(sh.raw_empty[s]), 4);
     }
-    tc::mbar_init(bar(sh.q_full), 8);
     for (int g = 0; g < 2; ++g) {
+      tc::mbar_init(bar(sh.q_full[g]), 8);
       tc::mbar_init(bar(sh.s_full[g]), 1);
       tc::mbar_init(bar(sh.p_ready[g]), 4);
       tc::mbar_init(bar(sh.o_done[g]), 1);
@@ -579,8 +582,11 @@ __global__ void __launch_bounds__(FP8 ? 512 : 384, 1)
       asm volatile("cp.async.wait_all;" ::: "memory");
       tc::fence_proxy_async();
       __syncwarp();
-      if (lane == 0) tc::mbar_arrive_release(bar(sh.q_full));
       const int n = w.t1 - w.t0, rows = w.rows(a), two = rows > 128, steps = two ? 2 * n : n;
+      if (lane == 0) {
+        tc::mbar_arrive_release(bar(sh.q_full[0]));
+        if (steps > 1) tc::mbar_arrive_release(bar(sh.q_full[1]));
+      }
       const Row me = next_row;
       const int row = me.row, qrow = me.qrow, k_len = me.k_len, base = k_len - me.nodes, node = me.node, head = w.h * a.G + me.gh;
       const bool live = row < rows, work = __any_sync(FULL_MASK, live);
@@ -861,6 +867,7 @@ __global__ void __launch_bounds__(FP8 ? 512 : 384, 1)
       bool ok = true;
       uint32_t done = 0;  // steps so far
       int items = 0;
+      uint32_t q_items = 0;  // of them with steps of this group
       Place begin;  // of the item's first K
       for (Walk w(a, sh.spot); w.more() && ok; w.next(a), ++items) {
         const int n = w.t1 - w.t0, two = w.rows(a) > 128;
@@ -870,7 +877,7 @@ __global__ void __launch_bounds__(FP8 ? 512 : 384, 1)
         if (!two && g) k_at.step(2, S);
         v_at = k_at;
         v_at.step(1, S);
-        ok = wait(sh.q_full, items & 1, 2);
+        if (mine > 0) ok = wait(sh.q_full[g], q_items++ & 1, 2);
         for (int i = 0; i <= mine && ok; ++i) {
           if (i > 0) {  // P V of the step before
             ok = wait(sh.p_ready[g], (done - 1) & 1, 3) && wait(sh.full[v_at.s], v_at.ph, 4) &&
@@ -1645,6 +1652,7 @@ template <bool FP8>
 cudaError_t launch_wide(const CUtensorMap& km, const CUtensorMap& vm, Args& a, cudaStream_t stream) {
   static std::atomic<uint64_t> done{0};
   const int qt = a.rows_cap / 128;
+  static_assert(smem_bytes(2, FP8 ? 4 : 5, FP8 ? 2 : 0) <= SMEM_MOST && smem_bytes(1, FP8 ? 4 : 6, FP8 ? 4 : 0) <= SMEM_MOST, "");
   a.slots = FP8 ? 4 : 7 - qt;
   a.raw_slots = FP8 ? (qt == 1 ? 4 : 2) : 0;
   return launch_main(tree_attn_kernel<FP8>, FP8 ? 512 : 384, smem_bytes(qt, a.slots, a.raw_slots), done, km, vm, a, stream);

@@ -160,6 +160,23 @@ def test_attention_long_context_and_no_context(ops, dtype):
 
 
 @KV
+@pytest.mark.parametrize("longer", [0, 1, 7])
+def test_attention_many_items_of_one_tile(ops, dtype, longer):
+    """Between 64 and 128 rows over contexts of up to a tile, some ten items per CTA: one of the two groups has no step
+    in them, but in the contexts of a few tiles among them."""
+    g = torch.Generator().manual_seed(longer)
+    ns = torch.randint(17, 33, (200,), generator=g).tolist()
+    ks = [n + int(torch.randint(0, 128 - n + 1, (), generator=g)) for n in ns]
+    for i in range(longer):
+        ks[29 * i + 3] = 128 * (i + 1) + 1
+    c = Case(ns, ks, 32, 8, 16, dtype, seed=longer)
+    first = c.run(ops)
+    c.check(first)
+    for _ in range(5):
+        assert torch.equal(c.run(ops), first)
+
+
+@KV
 def test_attention_is_the_same_on_every_run(ops, dtype):
     """Fewer tiles than CTAs, and more; memory that the allocator hands out again holds other sums, or NaN."""
     for c in (Case([8], [600], 8, 2, 16, dtype), Case([8, 3, 16], [2000, 70, 512], 32, 8, 64, dtype)):
