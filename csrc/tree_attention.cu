@@ -20,12 +20,12 @@
 // kernel joins in the order of the keys: no atomics, the same bits on every run.
 //
 // Masks: only tiles that reach into the tree look at them.  What a row does not see takes no part in it: its score is
-// -inf, and a value that is infinite or NaN (0 x inf) is taken out of such a tile in shared memory and added at the
-// end to the rows that see it.
+// -inf, and a value that is infinite or NaN (0 x inf), of itself or by its scale, is taken out of such a tile in shared
+// memory and added at the end to the rows that see it.
 //
 // What bounds it.  Up to 64 rows the bytes of K and V should: 64 trees of 16 nodes, 32 query and 8 KV heads, 2048
 // tokens, bf16: 131 us, 4.2 TB/s (a tile's round of product, maximum, weights and store is longer than its bytes take);
-// 128 trees of 8 on e4m3: 300 us, 1.8 TB/s (a round takes twice as long beside the eight warps that convert).  Beyond, the
+// 128 trees of 8 on e4m3: 308 us, 1.8 TB/s (a round takes twice as long beside the eight warps that convert).  Beyond, the
 // exponentials: 24 trees of up to 64 nodes, 64 and 8 heads, up to 8191 tokens: 241-262 us, 530-580 TFLOP/s; two groups'
 // weights of a tile take 3800 clocks in turn, the products 2048.
 #include <cuda.h>
@@ -51,7 +51,7 @@ constexpr float RAISE = 8.f;            // the running maximum follows once a ro
 // First warp of each role; 0-7: softmax (the polling MMA warps share the schedulers of warps 2, 3, 6 and 7, whose rows are
 // the last); 9 has none: registers are moved between whole warpgroups.
 constexpr int W_TMA = 8, W_MMA = 10, W_CONV = 12;
-constexpr int BAD_WORDS = TREE_MAX_NODES / 32;
+constexpr int BAD_WORDS = TREE_MAX_NODES / 32 + 1;  // the nodes, and keys ahead of them (bad_from)
 constexpr float NOTHING = -3e38f;       // below any score
 
 __device__ int g_tree_error = 0;
@@ -254,7 +254,7 @@ struct Small {  // shared memory besides the tiles
   uint64_t scale_full[4];
   float2 ml[2][128];        // (maximum, sum) of the groups' rows
   float2 scale[4][KT / 16];  // e4m3: (K, V) scales of 16 keys, of the last four tiles
-  uint32_t bad[2][BAD_WORDS];  // nodes whose values are not finite
+  uint32_t bad[2][BAD_WORDS];  // keys from bad_from() on whose values are not finite
   int64_t part[16];
   Spot spot;
   uint32_t tmem;
@@ -325,6 +325,20 @@ __device__ __forceinline__ void load_q(const Args& a, int b, int h, int R, int r
       }
     }
   }
+}
+
+// The first key that is looked at for values that are not finite: the tree's, or of an 8-bit cache the first of the 16
+// (of one scale) in which the tree begins.
+template <bool FP8>
+__device__ __forceinline__ int bad_from(int base) {
+  return FP8 ? base & ~15 : base;
+}
+
+// V's scale of a key is not finite, and not every row sees the 16 keys that share it (or they lie behind the context,
+// where the block may be anybody's): their weights are 0, and their values count as not finite.
+template <bool FP8>
+__device__ __forceinline__ bool odd_scale(int key, int base, float vs) {
+  return key >= bad_from<FP8>(base) && !(fabsf(vs) < INFINITY);
 }
 
 // Row r of a V tile without its infinities and NaN, all zeros `behind` the context; whether there were any.
@@ -439,25 +453,29 @@ __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatil
   return warp_poll(bar, parity, gave_up, code);
 }
 
-// The part of nodes whose values were taken out of the products in a row that sees them, from the cache: the values
+// The part of keys whose values were taken out of the products in a row that sees them, from the cache: the values
 // themselves (infinite or NaN), added to the row's outputs [d0, d0 + n) at `out`.
 template <bool FP8, typename T>
 __device__ __forceinline__ void add_bad(const Args& a, const Walk& w, const uint32_t* bad, int node, int d0, int n, T* out) {
   const int qrow = seq_begin(a.t, w.b), nodes = seq_nodes(a.t, w.b), base = a.t.ctx_lens[w.b] - nodes;
-  for (int nd = 0; nd < min(nodes, min(TREE_WORDS, a.t.words) * 64); ++nd) {
-    if (!(bad[nd >> 5] >> (nd & 31) & 1) || !(a.t.mask[(int64_t)(qrow + node) * a.t.mask_stride + (nd >> 6)] >> (nd & 63) & 1))
+  const int from = bad_from<FP8>(base), last = base + min(nodes, min(TREE_WORDS, a.t.words) * 64);
+  for (int pos = from; pos < last; ++pos) {
+    const int nd = pos - base;
+    if (!(bad[(pos - from) >> 5] >> ((pos - from) & 31) & 1) ||
+        (nd >= 0 && !(a.t.mask[(int64_t)(qrow + node) * a.t.mask_stride + (nd >> 6)] >> (nd & 63) & 1)))
       continue;
-    const int pos = base + nd;
     if (pos < w.t0 * KT || pos >= w.t1 * KT || (pos >> a.bs_shift) >= a.t.W) continue;
     const int blk = a.t.block_tables[w.b * a.t.bt_stride + (pos >> a.bs_shift)];
     if (blk < 0 || blk >= a.t.num_blocks) continue;
-    const int64_t at = ((((int64_t)blk * a.t.nkv + w.h) << a.bs_shift) + (pos & (a.t.block_size - 1))) * AD + d0;
+    const int64_t row = (int64_t)blk * a.t.nkv + w.h, at = ((row << a.bs_shift) + (pos & (a.t.block_size - 1))) * AD + d0;
     for (int i = 0; i < n; ++i) {
       float z;
-      if constexpr (FP8)
-        z = (static_cast<const uint8_t*>(a.t.v_cache)[at + i] & 0x7f) == 0x7f ? NAN : 0.f;
-      else
+      if constexpr (FP8) {
+        __half_raw x = __nv_cvt_fp8_to_halfraw(static_cast<const uint8_t*>(a.t.v_cache)[at + i], __NV_E4M3);
+        z = __half2float(*reinterpret_cast<__half*>(&x)) * a.t.v_scale[row];
+      } else {
         z = __bfloat162float(static_cast<const __nv_bfloat16*>(a.t.v_cache)[at + i]);
+      }
       if (!(fabsf(z) < INFINITY)) {
         if constexpr (sizeof(T) == 2)
           out[i] = __float2bfloat16_rn(__bfloat162float(out[i]) + z);
@@ -632,6 +650,11 @@ __global__ void __launch_bounds__(FP8 ? 512 : 384, 1)
             float mx[2] = {-INFINITY, -INFINITY};
             columns([&](int c, uint32_t(&v)[16]) {
               const float f = factor(c);
+              [[maybe_unused]] float vs = 1.f;
+              if constexpr (FP8) {
+                vs = scl[c].y;
+                if (MASK && odd_scale<FP8>(t * KT + 16 * c, base, vs)) vs = 0.f;
+              }
 #pragma unroll
               for (int i = 0; i < 16; i += 2) {
                 float2 y = fma2(v[i], v[i + 1], f, -sub);
@@ -642,8 +665,8 @@ __global__ void __launch_bounds__(FP8 ? 512 : 384, 1)
                 y = make_float2(ex2(y.x), ex2(y.y));
                 ls[i >> 1 & 1] = add2(ls[i >> 1 & 1], y);
                 if constexpr (FP8) {
-                  y.x *= scl[c].y;
-                  y.y *= scl[c].y;
+                  y.x *= vs;
+                  y.y *= vs;
                 }
                 // rounded by 2^-9 of a weight at most; the sum takes the weights as they were
                 p[8 * c + (i >> 1)] = pack_bf16(y.x, y.y);
@@ -709,10 +732,11 @@ __global__ void __launch_bounds__(FP8 ? 512 : 384, 1)
           const int c = 2 * (tile0 + j) + 1, pos = t * KT + lr;
           wait(sh.full[c % S], (c / S) & 1, 12);
           uint8_t* v = ring + (c % S) * TILE;
-          if (pos >= base) {
-            const bool odd = clean_row(v, lr, pos >= k_len);
-            const int nd = pos - base;
-            if (odd && nd >= 0 && nd < TREE_MAX_NODES) atomicOr(&sh.bad[items & 1][nd >> 5], 1u << (nd & 31));
+          if (pos >= bad_from<FP8>(base)) {
+            bool odd = clean_row(v, lr, pos >= k_len);
+            if constexpr (FP8) odd |= pos < k_len && odd_scale<FP8>(pos, base, scl[lr >> 4].y);
+            const int i = pos - bad_from<FP8>(base);
+            if (odd && i < BAD_WORDS * 32) atomicOr(&sh.bad[items & 1][i >> 5], 1u << (i & 31));
           }
           tc::fence_proxy_async();
         }
@@ -1236,10 +1260,16 @@ __global__ void __launch_bounds__(FP8 ? 512 : 256, 1)
           const int c = 2 * cnt + 1;
           wait(sh.full[c % S], (c / S) & 1, 12);
           uint8_t* v = ring + (c % S) * TILE;
-          if (pos >= base) {
-            const bool odd = clean_row(v, kq, pos >= k_len);
-            const int nd = pos - base;
-            if (odd && nd >= 0 && nd < TREE_MAX_NODES) atomicOr(&sh.bad[items & 1][nd >> 5], 1u << (nd & 31));
+          if (pos >= bad_from<FP8>(base)) {
+            bool odd = clean_row(v, kq, pos >= k_len);
+            if constexpr (FP8)
+              if (odd_scale<FP8>(pos, base, sh.scale[cnt & 3][kq >> 4].y)) {
+                odd = pos < k_len;
+#pragma unroll 1
+                for (int c = 0; c < N / 8; ++c) *reinterpret_cast<uint4*>(pb + tile_at(kq, c)) = make_uint4(0, 0, 0, 0);
+              }
+            const int i = pos - bad_from<FP8>(base);
+            if (odd && i < BAD_WORDS * 32) atomicOr(&sh.bad[items & 1][i >> 5], 1u << (i & 31));
           }
         }
         tc::fence_proxy_async();

@@ -244,6 +244,59 @@ def test_attention_visible_infinite_values_reach_their_rows(ops, dtype):
     assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.nan_to_num(0), want.nan_to_num(0))
 
 
+@pytest.mark.parametrize("bad", [float("inf"), float("nan")])
+@pytest.mark.parametrize("ns,ks,nq,nkv", [([20, 3], [52, 40], 2, 2), ([20], [308], 4, 2), ([20, 9], [52, 300], 6, 2),
+                                          ([20, 7], [52, 800], 32, 4), ([200], [232], 2, 2)])
+def test_attention_masked_scales_take_no_part(ops, ns, ks, nq, nkv, bad):
+    """Scales of blocks behind the contexts, and of blocks that hold nodes which some rows do not see."""
+    c = Case(ns, ks, nq, nkv, 16, F8)
+    c.mask[:16, 0] &= 0xffff                    # the first tree's first 16 nodes see none of the others, which
+    base, nb = ks[0] - ns[0], c.k.shape[0]      # lie in blocks of their own
+    assert base % 16 == 0
+    # behind the contexts the tables name a block that nobody owns
+    extra = torch.full((1, nkv, 16, 128), 0x38, dtype=torch.uint8, device=DEV)
+    c.k, c.v = (torch.cat([x.view(torch.uint8), extra]).view(F8) for x in (c.k, c.v))
+    c.ks_, c.vs_ = (torch.cat([s, torch.ones(1, nkv, device=DEV)]) for s in (c.ks_, c.vs_))
+    t = torch.full((len(ns), c.ctx.block_tables.shape[1] + 8), nb, dtype=torch.int32, device=DEV)
+    for b, k in enumerate(ks):
+        t[b, :-(-k // 16)] = c.ctx.block_tables[b, :-(-k // 16)]
+    c.ctx.block_tables = t
+    clean = c.run(ops)
+    c.check(clean)
+    for s in (c.ks_, c.vs_):
+        s[nb] = bad
+    assert torch.equal(c.run(ops), clean)
+    late = t[0, (base + 16) // 16:-(-ks[0] // 16)].long()
+    sees = torch.zeros(c.T, dtype=torch.bool, device=DEV)
+    sees[:ns[0]] = torch.stack([(c.mask[:ns[0], i // 64] >> (i % 64) & 1).bool() for i in range(16, ns[0])]).any(0)
+    assert sees.any() and not sees[:16].any()
+    for s in (c.vs_, c.ks_):
+        keep = s.clone()
+        s[late] = bad
+        got = c.run(ops)
+        s.copy_(keep)
+        assert torch.equal(got[~sees], clean[~sees])
+        assert s is c.ks_ or not got[sees].isfinite().any()
+
+
+@pytest.mark.parametrize("bad", [float("inf"), float("nan")])
+@pytest.mark.parametrize("nq,nkv", [(2, 2), (16, 4)])
+def test_attention_visible_scales_reach_their_rows(ops, nq, nkv, bad):
+    """A scale that is not finite over the last cached tokens and the first nodes, or over the last nodes: infinite or NaN
+    where the values times their scale, added up over what a row sees, are."""
+    c = Case([20], [53], nq, nkv, 16, F8)
+    for place in (2, 3):
+        keep = c.vs_.clone()
+        c.vs_[int(c.ctx.block_tables[0, place])] = bad
+        got = c.run(ops).view(20, nq, 128)
+        want = R.tree_attention(c.q.view(20, nq, 128), c.k, c.v, c.ns, c.ks, c.ctx.block_tables.tolist(), c.mask, c.scale,
+                                c.ks_, c.vs_)
+        c.vs_.copy_(keep)
+        assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.isinf(), want.isinf())
+        assert torch.equal(got[got.isinf()], want[want.isinf()]) and (want.isinf().any() or bad != bad)
+        assert not want[0].isfinite().any() if place == 2 else want[0].isfinite().all()
+
+
 def test_attention_bad_blocks_read_as_zeros(ops):
     c = Case([5], [200], 8, 2, 16)
     t = c.ctx.block_tables
