@@ -162,7 +162,8 @@ __global__ void __launch_bounds__(CT, 4) tree_commit_kernel(TreeCommit a) {
           }
           if (now != from) {  // rounded to 8 bits again, to within half a step of e4m3
             uint32_t y[4];
-            if (fminf(now, from) > 1e-20f && fmaxf(now, from) < 1e20f) {
+            // (|f| <= 448 from: with from <= 1e30 now the quotient is far from fp32's largest)
+            if (fminf(now, from) > 1e-20f && fmaxf(now, from) < 1e20f && from <= __fmul_rn(1e30f, now)) {
               // f / now, correctly rounded, from the correctly rounded reciprocal: the remainder of f * r is exact
               // and corrects it (P. Markstein, 1990); the bounds keep the remainder above fp32's smallest
               const float r = __frcp_rn(now);

@@ -642,6 +642,17 @@ def test_commit_scales_of_any_size(ops):
         _check_commit(ops, ctx, kv, s, path, length)
 
 
+@pytest.mark.parametrize("bs", [4, 16])
+def test_commit_between_scales_of_different_sizes(ops, bs):
+    """Every pair of sizes as source and destination: quotients past fp32's range saturate, ones below the format vanish."""
+    sizes = torch.tensor([1e-38, 2e-20, 1e-8, 1.0, 5e19, 1e30], device=DEV)
+    for seed in range(4):
+        ctx, kv, s, path, length = _commit_case([16] * 12, [37 + i for i in range(12)], bs, F8, L=4, seed=seed)
+        pick = torch.randint(0, len(sizes), s.shape, device=DEV, generator=_gen(seed))
+        s = sizes[pick] * (1 + torch.rand(s.shape, device=DEV, generator=_gen(seed)))
+        _check_commit(ops, ctx, kv, s, path, length)
+
+
 @KV
 def test_commit_of_a_range_of_layers(ops, dtype):
     ctx, kv, s, path, length = _commit_case([12, 12], [40, 29], 16, dtype, L=6)
