@@ -677,12 +677,12 @@ __global__ void __launch_bounds__(FP8 ? 512 : 384, 1)
           if (mine == 0) {  // the first tile's maximum; later ones mostly stay within 2^RAISE of it
             top = -INFINITY;
             columns([&](int c, uint32_t(&v)[16]) {
+              const float f = factor(c);  // of either sign
               float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
               for (int i = 0; i < 16; ++i)
-                if (seen(c, i)) mx[i & 1] = fmaxf(mx[i & 1], __uint_as_float(v[i]));
-              const float mc = fmaxf(mx[0], mx[1]);
-              if (mc > -INFINITY) top = fmaxf(top, mc * factor(c));
+                if (seen(c, i)) mx[i & 1] = fmaxf(mx[i & 1], __uint_as_float(v[i]) * f);
+              top = fmaxf(top, fmaxf(mx[0], mx[1]));
             });
             m = top;
           }

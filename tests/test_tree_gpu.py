@@ -330,6 +330,14 @@ def test_attention_large_and_small_magnitudes(ops, dtype):
         c.check(c.run(ops))
 
 
+@KV
+@pytest.mark.parametrize("ns,ks,nq,nkv", [([256], [700], 2, 2), ([40, 9], [300, 77], 16, 4), ([8, 5], [300, 500], 8, 2)])
+def test_attention_with_a_negative_scale(ops, dtype, ns, ks, nq, nkv):
+    """Scores of some hundreds of both signs: weights are relative to the largest of scale q k, not of q k."""
+    c = Case(ns, ks, nq, nkv, 16, dtype, spread=40.0)
+    c.check(ops.attention_tree(-c.q, c.k, c.v, c.ctx, c.mask, -c.scale, c.ks_, c.vs_))
+
+
 def test_attention_strided_operands(ops):
     c = Case([8, 5], [300, 77], 8, 2, 16)
     want = c.run(ops)
