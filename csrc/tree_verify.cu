@@ -5,12 +5,16 @@
 // child the next token is the first x whose cumulative sum of p is above u_draw times the total.
 //
 // A cumulative sum over a vocabulary of 1.5e5 tokens has tokens narrower than fp32's rounding next to every border,
-// so decisions rest on 64-bit weights and sums, or on fp32 ones where their error cannot matter: they are those of
-// exact arithmetic but for random numbers within some 1e-11 of a border, and do not depend on how many CTAs share a
-// row.  exp2 in 64 bits costs 9 fp64 instructions here (an SM does 64 a clock) of some 30 in all: the argument is taken
-// apart into a multiple of 1/32 (a table entry, and an exponent by integer addition) and a rest |r| <= 1/64 with
-// 2^r = 1 + t + t^2/2 + t^3/6 + t^4/24, t = r ln 2 (next term: at most 1.3e-12).  The table's halves are read as
-// words: 32 entries, a bank each.
+// so decisions rest on 64-bit weights and sums, or on fp32 ones where their error cannot matter.  exp2 in 64 bits costs 9
+// fp64 instructions here (an SM does 64 a clock) of some 30 in all: the argument is taken apart into a multiple of 1/32
+// (a table entry, and an exponent by integer addition) and a rest |r| <= 1/64, and 2^r = exp(t), t = r ln 2, |t| <= h, is
+// 1 + t + .. + t^4/24 with t^5/120 spread over t and t^3 as (h^5/120) (20 (t/h)^3 - 5 t/h) / 16, off by Chebyshev's
+// h^5/1920 = 7.9e-14 at most (left out it would be 1.3e-12), and by nothing at t = 0.  The table's halves are read as
+// words: 32 entries, a bank each.  A weight w is within 8e-14 + 2^-52 |ln w| + 2^-53 |m| / T of itself (m: the chunk's
+// largest logit, whose product with 1 / T is rounded), p within 1e-13 with the roundings of sums and products (|m| / T up to
+// 50, weights above 2^-40 of the largest).  So the decisions are those of exact arithmetic but for random numbers that
+// close to a border; behind rejections 1e-13 over the product of the masses that they left, since max(p - q, 0) keeps p's
+// error and loses most of p where q is near it.  They do not depend on how many CTAs share a row.
 //
 // One cluster of CTAs walks one tree, so only the rows of visited nodes are read.  A row is cut into chunks of
 // 512 tokens; a warp sums a chunk relative to the chunk's maximum and sends (sum, maximum) to every CTA of the
@@ -41,6 +45,10 @@ struct ChunkSum {
   int first;   // token of the first maximum
 };
 
+// exp(A r), |r| <= 1/2: coefficients of r .. r^4 (above: A = ln 2 / 32, h = A / 2)
+constexpr double A = 0.69314718055994530942 / 32.0, H2 = A * A / 4.0;
+constexpr double E1 = A * (1.0 - H2 * H2 / 384.0), E2 = A * A / 2.0, E3 = A * A * A * (1.0 / 6.0 + H2 / 96.0), E4 = A * A * A * A / 24.0;
+
 // 2^(z / 32) for z <= 0 (or a rounding above it) from a table of 2^(j / 32), possibly times a factor, as words;
 // z below -28800 counts as that.  The two factors of the result.
 struct Power {
@@ -51,9 +59,8 @@ __device__ __forceinline__ Power power(double z, const uint32_t* hi32, const uin
   const double t = z + 6755399441055744.0;  // 1.5 * 2^52: the low word is the nearest integer
   const int j = __double2loint(t);
   const double r = z - (t - 6755399441055744.0);
-  constexpr double A = 0.69314718055994530942 / 32.0;
   Power p;
-  p.poly = fma(fma(fma(fma(A * A * A * A / 24.0, r, A * A * A / 6.0), r, A * A / 2.0), r, A), r, 1.0);
+  p.poly = fma(fma(fma(fma(E4, r, E3), r, E2), r, E1), r, 1.0);
   p.scale = __hiloint2double((int)hi32[j & 31] + (j >> 5) * (1 << 20), (int)lo32[j & 31]);
   return p;
 }
@@ -61,7 +68,6 @@ __device__ __forceinline__ Power power(double z, const uint32_t* hi32, const uin
 // The same for four at a time, step by step: one alone waits for its own last instruction most of the time.
 __device__ __forceinline__ void power4(double (&z)[4], const uint32_t* hi32, const uint32_t* lo32, double (&scale)[4],
                                        double (&poly)[4]) {
-  constexpr double A = 0.69314718055994530942 / 32.0;
   double t[4];
   int j[4];
 #pragma unroll
@@ -78,12 +84,12 @@ __device__ __forceinline__ void power4(double (&z)[4], const uint32_t* hi32, con
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     scale[i] = __hiloint2double((int)hi32[j[i] & 31] + (j[i] >> 5) * (1 << 20), (int)lo32[j[i] & 31]);
-    poly[i] = fma(A * A * A * A / 24.0, z[i], A * A * A / 6.0);
+    poly[i] = fma(E4, z[i], E3);
   }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) poly[i] = fma(poly[i], z[i], A * A / 2.0);
+  for (int i = 0; i < 4; ++i) poly[i] = fma(poly[i], z[i], E2);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) poly[i] = fma(poly[i], z[i], A);
+  for (int i = 0; i < 4; ++i) poly[i] = fma(poly[i], z[i], E1);
 #pragma unroll
   for (int i = 0; i < 4; ++i) poly[i] = fma(poly[i], z[i], 1.0);
 }
@@ -103,7 +109,7 @@ struct Dist {
   bool greedy;
   // Whether fp32's range holds log2(e) / T, with room.
   __device__ __forceinline__ bool moderate() const { return cf > 1e-6f && cf < 1e6f; }
-  // Whether l c - max c in one instruction is exact enough (2^-35 of 1/32), and -inf far enough off.
+  // Whether l c - top c in one instruction, with top c rounded, is exact enough (2^-35 of 1/32), and -inf far enough off.
   __device__ __forceinline__ bool plain(float top) const { return c > 1e-9 && fabs((double)top) * c < 262144.0; }
 };
 

@@ -509,6 +509,36 @@ def test_walk_where_the_draft_is_the_target(ops):
     assert w.want()[1][0] == 1
 
 
+@pytest.mark.parametrize("v", [301, 1303])
+@pytest.mark.parametrize("b", [9, 24, 40])
+def test_walk_behind_rejections_of_a_draft_near_the_target(ops, b, v):
+    """q = p (1 +- 2^-21): a rejection leaves 2.4e-7 of p and multiplies its relative error by 2^21, a second one by 2.
+    p is within 1e-13 of itself, so the cumulative shares within 1e-13 2^22 / 2 = 2.1e-7 (an error e of each term moves
+    a share c by 2 c (1 - c) e at most); the draws are 2.4e-7 and more from a border, the tests 3e-7 of p."""
+    w = Walk([3] * b, v, torch.float32, True, b, temps=(1.0, 0.6, 1.4), spread=1.0)
+    g = torch.Generator().manual_seed(b)
+    p = torch.softmax(w.logits.double() / w.temps.double().repeat_interleave(3)[:, None], -1)
+    more = torch.rand(3 * b, v, generator=g) < 0.5
+    w.draft = (p * torch.where(more, 1 + 2.0 ** -21, 1 - 2.0 ** -21)).float()
+    w.parents = torch.tensor([-1, 0, 0] * b, dtype=torch.int32)
+    w.parents[2::6] = -1                                  # one rejection in every other tree, two in the rest
+    above = (torch.arange(b) * 3).repeat_interleave(3)
+    w.tokens = torch.multinomial(p[above] * more[above], 1, generator=g)[:, 0].int()
+    w.u = torch.full_like(w.u, 1 - 2.0 ** -24)            # u q is above p
+    for i in range(b):
+        r, q = p[3 * i], w.draft[3 * i].double()
+        for _ in range(1 + int(w.parents[3 * i + 2] == 0)):
+            r = (r - q).clamp(min=0.0)
+            r = r / r.sum()
+        c = r.cumsum(0)
+        # next to a border below a quarter, where fp32 numbers are 1.5e-8 apart at most, on either side of it
+        at = int(torch.randint(0, int((c < 0.25).sum()), (), generator=g))
+        share = float(c[at]) + (1 if i % 2 else -1) * (2.5e-7 + 5e-8 * int(torch.randint(0, 3, (), generator=g)))
+        w.ud[i] = max(share, 0.0)
+    w.check(ops)
+    assert (w.want()[1] == 1).all()
+
+
 @pytest.mark.parametrize("b", [12, 40])  # 40: summed in fp32 first
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_walk_infinities_nan_and_odd_numbers(ops, dtype, b):
