@@ -49,11 +49,7 @@ struct Fp8Plan {
 Fp8Plan fp8_plan(int T, int N, int K, int act, int num_sms);
 cudaError_t gemm_fp8(const Fp8Gemm& g, const Fp8Plan& plan, int num_sms, cudaStream_t stream);
 
-// Error word written by a product that gave up on a bounded wait (0 = none; the last code wins): its output is
-// not valid.  One word for all GPUs of the process, in host memory: what a launch wrote is seen once its stream
-// has been synchronised.
-int gemm_fp8_error_code(int reset);
-// Runs a wait that nothing ends, for at most budget_ns (up to 2 s), through the same path: error code 599.
+// Runs a wait that nothing ends, for at most budget_ns (up to 2 s), as a product waits: error code 599.
 cudaError_t gemm_fp8_wait_check(uint64_t budget_ns, cudaStream_t stream);
 
 }  // namespace nvb

@@ -5,6 +5,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
+#include "device_error.h"
 #include "fp8.h"
 
 namespace {
@@ -195,7 +196,7 @@ Pair linear_silu_fp8(const at::Tensor& xq, const at::Tensor& xs, const at::Tenso
   return {q, s};
 }
 
-int64_t fp8_error(bool reset) { return nvb::gemm_fp8_error_code(reset ? 1 : 0); }
+int64_t fp8_error(bool reset) { return nvb::device_error_code(reset ? 1 : 0); }
 
 void fp8_wait_check(int64_t budget_ns) {
   TORCH_CHECK(budget_ns >= 0, "fp8_wait_check: the budget must not be negative");

@@ -45,15 +45,15 @@
 // two rings deep cost 2%, four 8%.
 //
 // Neither kernel uses a global workspace.  Every wait on an mbarrier is bounded; on expiry the kernel records
-// an error code in a word of host memory, drains its copies, frees TMEM and returns, with an output that is
+// an error code in the process's error word (device_error.h), drains its copies, frees TMEM and returns, with an output that is
 // not valid: whoever reads the output back checks the word (fp8_error).  Cluster barriers, TMEM allocation and
 // the wait for the previous kernel have no bound of their own; every thread reaches them, on the error path too.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
 #include <algorithm>
-#include <mutex>
 
+#include "device_error.h"
 #include "fp8_quant.cuh"
 #include "tcgen05.cuh"
 
@@ -857,31 +857,6 @@ __global__ void __launch_bounds__(WeightsCfg<NP, MW>::THREADS, 2)
   }
 }
 
-// The error word: pinned host memory that every GPU of the process can write, so that reading it after a
-// synchronisation costs no copy and covers all of them.  Null where it cannot be had.
-std::atomic<int*> g_error_word{nullptr};
-int* error_word() {
-  int* w = g_error_word.load(std::memory_order_acquire);
-  if (w) return w;
-  static std::mutex mu;
-  std::lock_guard<std::mutex> lock(mu);
-  if ((w = g_error_word.load(std::memory_order_acquire))) return w;
-  // the first call may lie inside a stream capture, which this allocation does not concern
-  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
-  if (cudaThreadExchangeStreamCaptureMode(&mode) != cudaSuccess) return nullptr;
-  void* m = nullptr;
-  const cudaError_t e = cudaHostAlloc(&m, sizeof(int), cudaHostAllocPortable | cudaHostAllocMapped);
-  cudaThreadExchangeStreamCaptureMode(&mode);
-  if (e != cudaSuccess) {
-    cudaGetLastError();
-    return nullptr;
-  }
-  w = static_cast<int*>(m);
-  *w = 0;
-  g_error_word.store(w, std::memory_order_release);
-  return w;
-}
-
 // A wait that nothing ends, given up after budget_ns.
 __global__ void wait_check_kernel(int* word, uint64_t budget_ns) {
   __shared__ uint64_t bar;
@@ -1098,7 +1073,7 @@ Fp8Plan fp8_plan(int T, int N, int K, int act, int num_sms) {
 cudaError_t gemm_fp8(const Fp8Gemm& g, const Fp8Plan& pl, int num_sms, cudaStream_t stream) {
   if (g.T == 0 || g.N == 0) return cudaSuccess;
   Params p{};
-  p.error = error_word();
+  p.error = device_error_word();
   if (!p.error) return cudaErrorMemoryAllocation;
   p.ws = g.ws;
   p.ldws = g.ldws;
@@ -1124,14 +1099,8 @@ cudaError_t gemm_fp8(const Fp8Gemm& g, const Fp8Plan& pl, int num_sms, cudaStrea
   }
 }
 
-int gemm_fp8_error_code(int reset) {
-  int* w = g_error_word.load(std::memory_order_acquire);
-  if (!w) return 0;  // no product was ever launched
-  return reset ? __atomic_exchange_n(w, 0, __ATOMIC_ACQ_REL) : __atomic_load_n(w, __ATOMIC_ACQUIRE);
-}
-
 cudaError_t gemm_fp8_wait_check(uint64_t budget_ns, cudaStream_t stream) {
-  int* w = error_word();
+  int* w = device_error_word();
   if (!w) return cudaErrorMemoryAllocation;
   wait_check_kernel<<<1, 1, 0, stream>>>(w, std::min<uint64_t>(budget_ns, WAIT_BUDGET_NS));
   return cudaGetLastError();

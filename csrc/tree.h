@@ -40,8 +40,8 @@ struct TreeAttnPlan {
 };
 TreeAttnPlan tree_attn_plan(int max_nodes, int nq, int nkv, int num_sms);
 cudaError_t launch_tree_attention(const TreeAttn& a, const TreeAttnPlan& p, cudaStream_t stream);
-// Error word of a kernel that gave up on a bounded wait (0 = none).
-int tree_attn_error_code(int reset);
+// Runs a wait that nothing ends, for at most budget_ns (up to 2 s), as attention waits: error code 699.
+cudaError_t launch_tree_wait_check(uint64_t budget_ns, cudaStream_t stream);
 
 struct TreeVerify {
   const void* logits;  // [T, V]

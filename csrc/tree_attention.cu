@@ -24,14 +24,15 @@
 // memory and added at the end to the rows that see it.
 //
 // What bounds it.  Up to 64 rows the bytes of K and V should: 64 trees of 16 nodes, 32 query and 8 KV heads, 2048
-// tokens, bf16: 131 us, 4.2 TB/s (a tile's round of product, maximum, weights and store is longer than its bytes take);
-// 128 trees of 8 on e4m3: 308 us, 1.8 TB/s (a round takes twice as long beside the eight warps that convert).  Beyond, the
-// exponentials: 24 trees of up to 64 nodes, 64 and 8 heads, up to 8191 tokens: 241-262 us, 530-580 TFLOP/s; two groups'
+// tokens, bf16: 126 us, 4.4 TB/s (a tile's round of product, maximum, weights and store is longer than its bytes take);
+// 128 trees of 8 on e4m3: 298 us, 1.8 TB/s (a round takes twice as long beside the eight warps that convert).  Beyond, the
+// exponentials: 24 trees of up to 64 nodes, 64 and 8 heads, up to 8191 tokens: 252-261 us, 530-550 TFLOP/s; two groups'
 // weights of a tile take 3800 clocks in turn, the products 2048.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
 #include "common.cuh"
+#include "device_error.h"
 #include "tcgen05.cuh"
 #include "tree.h"
 
@@ -54,7 +55,7 @@ constexpr int W_TMA = 8, W_MMA = 10, W_CONV = 12;
 constexpr int BAD_WORDS = TREE_MAX_NODES / 32 + 1;  // the nodes, and keys ahead of them (bad_from)
 constexpr float NOTHING = -3e38f;       // below any score
 
-__device__ int g_tree_error = 0;
+constexpr int ERROR_BASE = 600;         // of the codes in the process's error word
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -79,6 +80,7 @@ struct Args {
   int oob_row;      // a row behind the pool: reads as zeros
   int q16;          // q's rows are 16-byte aligned
   float scale_log2;
+  int* error;       // the process's error word
 };
 
 // ------------------------------------------------------------------- the list of tiles
@@ -425,9 +427,16 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
   return r;
 }
 
-// Bounded wait of a whole warp; on expiry every role goes on without waiting, and the outputs are not valid.  The same
-// answer in every lane.  One lane polls.
-__device__ __forceinline__ bool warp_poll(uint32_t bar, uint32_t parity, volatile int* gave_up, int code) {
+// An error, in the process's error word: the outputs are not valid.
+__device__ __forceinline__ void give_up(int* word, int code) {
+  *reinterpret_cast<volatile int*>(word) = ERROR_BASE + code;
+  __threadfence_system();
+}
+
+// Bounded wait of a whole warp; on expiry every role goes on without waiting, and the kernel's end reports the code that
+// it finds in *gave_up.  The same answer in every lane.  One lane polls.
+__device__ __forceinline__ bool warp_poll(uint32_t bar, uint32_t parity, volatile int* gave_up, int code,
+                                          uint64_t budget_ns = tc::WAIT_BUDGET_NS) {
   int ok = 1;
   if ((threadIdx.x & 31) == 0) {
     SpinBudget sb;
@@ -436,9 +445,8 @@ __device__ __forceinline__ bool warp_poll(uint32_t bar, uint32_t parity, volatil
         ok = 0;
         break;
       }
-      if (sb.expired(tc::WAIT_BUDGET_NS)) {
-        atomicCAS(&g_tree_error, 0, code);
-        *gave_up = 1;
+      if (sb.expired(budget_ns)) {
+        *gave_up = code;
         ok = 0;
         break;
       }
@@ -451,6 +459,21 @@ __device__ __forceinline__ bool warp_poll(uint32_t bar, uint32_t parity, volatil
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* gave_up, int code) {
   if (__all_sync(FULL_MASK, tc::mbar_try(bar, parity))) return true;
   return warp_poll(bar, parity, gave_up, code);
+}
+
+// A wait that nothing ends, given up after budget_ns.
+__global__ void tree_wait_check_kernel(int* word, uint64_t budget_ns) {
+  __shared__ uint64_t bar;
+  __shared__ int gave_up;
+  if (threadIdx.x == 0) {
+    tc::mbar_init(smem_u32(&bar), 1);
+    gave_up = 0;
+    tc::fence_barrier_init();
+  }
+  __syncthreads();
+  warp_poll(smem_u32(&bar), 0, &gave_up, 99, budget_ns);
+  __syncthreads();
+  if (threadIdx.x == 0 && gave_up) give_up(word, gave_up);
 }
 
 // The part of keys whose values were taken out of the products in a row that sees them, from the cache: the values
@@ -514,7 +537,7 @@ __global__ void __launch_bounds__(FP8 ? 512 : 384, 1)
   auto bar = [](uint64_t& b) { return smem_u32(&b); };
   if (smem_u32(sm) & 1023) {  // the swizzle goes by the address
     if (threadIdx.x == 0) {
-      atomicCAS(&g_tree_error, 0, 9);
+      give_up(a.error, 9);
       spot_of(a, blockIdx.x)->hi_seq = a.t.num_seqs;  // nothing to join
     }
     return;
@@ -989,6 +1012,7 @@ __global__ void __launch_bounds__(FP8 ? 512 : 384, 1)
     }
   }
   __syncthreads();
+  if (threadIdx.x == 0 && sh.gave_up) give_up(a.error, sh.gave_up);
   if (warp == W_MMA) {
     tc::fence_after();
     tc::tmem_dealloc<1>(tmem, 512);
@@ -1063,7 +1087,7 @@ __global__ void __launch_bounds__(FP8 ? 512 : 256, 1)
   auto bar = [](uint64_t& b) { return smem_u32(&b); };
   if (smem_u32(sm) & 1023) {  // the swizzle goes by the address
     if (threadIdx.x == 0) {
-      atomicCAS(&g_tree_error, 0, 9);
+      give_up(a.error, 9);
       spot_of(a, blockIdx.x)->hi_seq = a.t.num_seqs;  // nothing to join
     }
     return;
@@ -1534,6 +1558,7 @@ __global__ void __launch_bounds__(FP8 ? 512 : 256, 1)
     }
   }
   __syncthreads();
+  if (threadIdx.x == 0 && sh.gave_up) give_up(a.error, sh.gave_up);
   if (warp == F_MMA) {
     tc::fence_after();
     tc::tmem_dealloc<1>(tmem, 256);
@@ -1715,6 +1740,8 @@ cudaError_t launch_tree_attention(const TreeAttn& t, const TreeAttnPlan& p, cuda
   a.oob_row = (int)rows;
   a.q16 = t.q_stride % 8 == 0 && (reinterpret_cast<uintptr_t>(t.q) & 15) == 0;
   a.scale_log2 = t.softmax_scale * LOG2E;
+  a.error = device_error_word();
+  if (!a.error) return cudaErrorMemoryAllocation;
   CUtensorMap km, vm;
   if (!pool_map(&km, t.k_cache, rows, t.kv_fp8, a.box_rows) || !pool_map(&vm, t.v_cache, rows, t.kv_fp8, a.box_rows))
     return cudaErrorInvalidValue;
@@ -1723,14 +1750,11 @@ cudaError_t launch_tree_attention(const TreeAttn& t, const TreeAttnPlan& p, cuda
   return launch_pdl(tree_join_kernel, dim3(a.chunks, a.rows_cap / JOIN_ROWS), dim3(128), 0, stream, a);
 }
 
-int tree_attn_error_code(int reset) {
-  int v = 0;
-  cudaMemcpyFromSymbol(&v, g_tree_error, sizeof(int));
-  if (reset) {
-    const int z = 0;
-    cudaMemcpyToSymbol(g_tree_error, &z, sizeof(int));
-  }
-  return v;
+cudaError_t launch_tree_wait_check(uint64_t budget_ns, cudaStream_t stream) {
+  int* word = device_error_word();
+  if (!word) return cudaErrorMemoryAllocation;
+  tree_wait_check_kernel<<<1, 32, 0, stream>>>(word, std::min<uint64_t>(budget_ns, tc::WAIT_BUDGET_NS));
+  return cudaGetLastError();
 }
 
 }  // namespace nvb

@@ -6,6 +6,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
+#include "device_error.h"
 #include "tree.h"
 
 namespace {
@@ -259,7 +260,12 @@ void tree_commit(const at::Tensor& kv, const at::Tensor& path, const at::Tensor&
   ok(nvb::launch_tree_commit(a, stream()), op);
 }
 
-int64_t tree_error(bool reset) { return nvb::tree_attn_error_code(reset ? 1 : 0); }
+int64_t tree_error(bool reset) { return nvb::device_error_code(reset ? 1 : 0); }
+
+void tree_wait_check(int64_t budget_ns) {
+  TORCH_CHECK(budget_ns >= 0, "tree_wait_check: the budget must not be negative");
+  ok(nvb::launch_tree_wait_check((uint64_t)budget_ns, stream()), "tree_wait_check");
+}
 
 }  // namespace
 
@@ -269,4 +275,5 @@ void register_tree(pybind11::module& m) {
   m.def("tree_verify", &tree_verify);
   m.def("tree_commit", &tree_commit);
   m.def("tree_error", &tree_error, pybind11::arg("reset") = false);
+  m.def("tree_wait_check", &tree_wait_check, pybind11::arg("budget_ns") = 1000000);
 }

@@ -428,11 +428,11 @@ class ModelRunner:
         return out
 
     def _check_device_error(self) -> None:
-        """An fp8 product that gave up on a bounded wait leaves an output that is not valid: no token made
-        from it is returned, in this step or a later one (the KV cache may hold what came of it)."""
+        """A kernel that gave up on a bounded wait leaves an output that is not valid: no token made from it is
+        returned, in this step or a later one (the KV cache may hold what came of it)."""
         code = self.ops.device_error()
         if code:
-            raise RuntimeError(f"an fp8 product gave up on a bounded wait (code {code}): this step's tokens and the "
+            raise RuntimeError(f"a kernel gave up on a bounded wait (code {code}): this step's tokens and the "
                                "KV cache are not valid")
 
     # ----------------------------------------------------------- cuda graphs

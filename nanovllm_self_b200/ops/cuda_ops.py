@@ -140,8 +140,8 @@ class CudaOps:
                                       w[0].shape[0] // 2 if features is None else features)
 
     def device_error(self) -> int:
-        """Code of an fp8 product that gave up on a bounded wait since the process began (0: none); its output
-        was not valid.  Reads host memory: call it once the product's stream has been synchronised.
+        """Code of an fp8 product (501 and up) or an ``attention_tree`` (601 and up) that gave up on a bounded wait since
+        the process began (0: none); its output was not valid.  Reads host memory: call it once the stream has been synchronised.
         ``C.fp8_error(True)`` clears it."""
         return self.C.fp8_error(False)
 

@@ -13,7 +13,7 @@ from torch.utils.cpp_extension import BuildExtension, CUDAExtension
 ROOT = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(ROOT, "csrc")
 SOURCES = [
-    "bindings.cpp", "gemm_bind.cpp", "comm_bind.cpp",
+    "bindings.cpp", "device_error.cpp", "gemm_bind.cpp", "comm_bind.cpp",
     "norm_act.cu", "qkv_rope_kv.cu", "attention.cu", "sampling.cu", "gemm_tcgen05.cu", "comm.cu",
     "attn_decode_noalloc.cu", "fp8_bind.cpp", "fp8_quant.cu", "gemm_fp8.cu",
     "tree_bind.cpp", "tree_ops.cu", "tree_attention.cu", "tree_verify.cu",

@@ -365,3 +365,11 @@ def test_the_kernels_refuse_bad_arguments():
     kv8 = torch.zeros(2, 3, nb, 2, 16, 128, **f8)
     assert "scales" in commit(kv=kv8) and "scales" in commit(kv=kv8, scale=torch.ones(2, 3, nb, 1))
     assert "CUDA" in commit(kv=kv8, scale=torch.ones(2, 3, nb, 2))
+
+
+def test_an_expired_wait_of_a_tree_ends_the_engines_step(monkeypatch):
+    from nanovllm_self_b200 import SamplingParams
+    llm = LLM("tiny", device="cpu", dtype="fp32", block_size=16, max_model_len=128, num_blocks=16, weight_quant_mode="fp8")
+    monkeypatch.setattr(llm.model_runner.ops, "device_error", lambda: 613)
+    with pytest.raises(RuntimeError, match="a kernel gave up on a bounded wait .code 613"):
+        llm.generate([[1, 2, 3]], SamplingParams(temperature=0, max_tokens=2, ignore_eos=True))

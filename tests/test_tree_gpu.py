@@ -399,6 +399,20 @@ def test_attention_on_a_side_stream_and_in_graphs(ops):
     c.check(graphs[0][1])
 
 
+def test_an_expired_wait_reaches_the_caller(ops):
+    """The code of a wait that runs out is what device_error gives once the stream is synchronised, and only until it is
+    cleared; calls behind it are as they were."""
+    c = Case([8], [600], 8, 2, 16)
+    want = c.run(ops)
+    torch.cuda.synchronize()
+    assert ops.device_error() == 0
+    ops.C.tree_wait_check(1000000)     # nothing ends this wait: given up after a millisecond
+    got = c.run(ops)
+    torch.cuda.synchronize()
+    assert ops.device_error() == 699 and ops.C.tree_error() == 699 and torch.equal(got, want)
+    assert ops.C.tree_error(True) == 699 and ops.device_error() == 0
+
+
 # ------------------------------------------------------------------------------ verification
 class Walk:
     def __init__(self, ns, v, dtype=torch.bfloat16, draft=False, seed=0, temps=(1.0, 0.7, 0.0), spread=2.0):
