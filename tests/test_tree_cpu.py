@@ -163,6 +163,31 @@ def test_walk_keeps_the_target_distribution():
         assert ((got - p).abs() <= 5 * (p * (1 - p) / (trials // 10)).sqrt()).all()
 
 
+@pytest.mark.parametrize("draft", [True, False])
+def test_walk_keeps_the_distribution_of_the_second_token(draft):
+    """Behind an accepted child the next token, taken from the tree or drawn, is distributed as the target's
+    probabilities behind that child's token."""
+    torch.manual_seed(1)
+    v, trials = 3, 4000
+    first, second = torch.randn(v), torch.randn(v, v)         # the target's logits: of the first token, and behind each
+    q0, q1 = torch.softmax(torch.randn(v), 0), torch.softmax(torch.randn(v, v), -1)
+    parents = torch.tensor([-1, 0, 1], dtype=torch.int32)
+    counts = torch.zeros(v, v)
+    for _ in range(trials):
+        x = int(torch.multinomial(q0, 1)) if draft else int(torch.randint(0, v, ()))
+        y = int(torch.multinomial(q1[x], 1)) if draft else 1
+        path, n, nxt = R.tree_verify(torch.stack([first, second[x], second[x]]), torch.tensor([0, x, y], dtype=torch.int32),
+                                     parents, [3], 3, torch.ones(1), torch.rand(3), torch.rand(1),
+                                     torch.stack([q0, q1[x], q1[x]]) if draft else None)
+        if n[0] > 1:
+            counts[x, y if n[0] > 2 else int(nxt[0])] += 1
+    for x in range(v):
+        p, k = torch.softmax(second[x].double(), 0), float(counts[x].sum())
+        assert k > 200
+        # five standard deviations of a share of k draws
+        assert ((counts[x].double() / k - p).abs() <= 5 * (p * (1 - p) / k).sqrt()).all()
+
+
 def test_greedy_walk_follows_the_first_maximum():
     logits = torch.tensor([[0.0, 2, 2, 1], [5, 0, 0, 0], [0, 0, 0, 9], [0, 0, 7, 7]])
     parents = torch.tensor([-1, 0, 0, 2], dtype=torch.int32)

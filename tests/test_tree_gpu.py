@@ -773,3 +773,116 @@ def test_steps_of_drafted_trees_equal_steps_of_single_tokens(kv):
         path = torch.tensor([[0, 2, 4]], dtype=torch.int32, device=DEV)
         ops.commit_tree(run.kv_cache, ctx, path, torch.tensor([3], dtype=torch.int32, device=DEV), run.kv_scale_cache)
         tokens += taken
+
+
+@pytest.mark.parametrize("captured", [False, True])
+@pytest.mark.parametrize("kv", ["none", "fp8"])
+def test_whole_steps_of_several_sequences(kv, captured):
+    """Masks, forward pass, walk and commit in a row, of three sequences at once, eagerly or as one graph that is replayed
+    with new inputs: what each operator leaves is what its plain form makes of what the one before left, and the cache
+    behind the last commit is that of the tokens that the steps added."""
+    from nanovllm_self_b200 import LLM
+    from nanovllm_self_b200.utils.context import Context
+    llm = LLM("tiny-gpu", block_size=16, max_model_len=512, num_blocks=64, kv_cache_quant_mode=kv, enforce_eager=True)
+    run, ops = llm.model_runner, llm.model_runner.ops
+    i32 = dict(dtype=torch.int32, device=DEV)
+    ns, B, T = [7, 4, 1], 3, 12
+    par = torch.tensor([-1, 0, 0, 1, 2, 2, 4, -1, 0, 1, 2, -1], **i32)
+    tables = torch.randperm(48, generator=torch.Generator().manual_seed(1)).int().view(6, 8).to(DEV)  # the last 3: see below
+    g = torch.Generator().manual_seed(0)
+    lines = [torch.randint(3, 2000, (n,), generator=g).tolist() for n in (27, 40, 5)]
+
+    def slots(row, start, n):
+        pos = torch.arange(start, start + n)
+        return tables[row].cpu()[pos // 16] * 16 + pos % 16
+
+    def forward(rows, tokens, starts, mask=None, decode=0):
+        """New tokens per sequence behind `starts` cached ones, in the blocks of the tables' `rows`."""
+        n = [len(t) for t in tokens]
+        ctx, _ = make_ctx(n, [s + k for s, k in zip(starts, n)], device=DEV, tables=tables[rows].cpu())
+        ctx.num_decode_seqs, ctx.tree_mask = decode, mask
+        ctx.slot_mapping = torch.cat([slots(r, s, k) for r, s, k in zip(rows, starts, n)]).int().to(DEV)
+        ctx.logits_indices = torch.arange(sum(n), **i32)
+        pos = torch.cat([torch.arange(s, s + k) for s, k in zip(starts, n)]).int().to(DEV)
+        return run.model.forward(torch.tensor(sum(tokens, []), **i32), pos, ctx, run.kv_layers, run.kv_scale_layers)
+
+    # what single greedy steps of the first sequence choose, to draft from
+    for r in range(B):
+        forward([r], [lines[r][:-1]], [0])
+    good = list(lines[0])
+    for _ in range(12):
+        good.append(int(forward([0], [[good[-1]]], [len(good) - 1], decode=1)[0].argmax()))
+    for r in range(B):
+        forward([r], [lines[r][:-1]], [0])
+
+    tokens, u, base = torch.zeros(T, **i32), torch.zeros(T, device=DEV), torch.zeros(T, **i32)
+    ud, temps = torch.zeros(B, device=DEV), torch.tensor([0.0, 0.8, 0.9], device=DEV)
+    ctx, _ = make_ctx(ns, [64] * B, device=DEV, tables=tables[:B].cpu())
+    ctx.slot_mapping, ctx.logits_indices = torch.zeros(T, **i32), torch.arange(T, **i32)
+
+    def pass_through(x):
+        ctx.tree_mask = x["mask"]
+        return run.model.forward(tokens, base + x["depth"], ctx, run.kv_layers, run.kv_scale_layers)
+
+    def step():
+        x = dict(zip(("mask", "depth"), ops.tree_mask(par, ctx)))
+        x["logits"] = pass_through(x)
+        x["path"], x["length"], x["next"] = ops.verify_tree(x["logits"], tokens, par, ctx, temps, u, ud)
+        ops.commit_tree(run.kv_cache, ctx, x["path"], x["length"], run.kv_scale_cache)
+        return x
+
+    pool = [t for t in (run.kv_cache, run.kv_scale_cache) if t is not None]
+    graph, x = None, None
+    lengths = []
+    for number in range(4):
+        starts = [len(l) - 1 for l in lines]
+        nxt = good[starts[0] + 1:starts[0] + 4]
+        trees = [[lines[0][-1], nxt[0] ^ 1, nxt[0], 11, nxt[1], nxt[1] ^ 1, 12],
+                 [lines[1][-1]] + torch.randint(3, 2000, (3,), generator=g).tolist(), [lines[2][-1]]]
+        tokens.copy_(torch.tensor(sum(trees, [])))
+        base.copy_(torch.repeat_interleave(torch.tensor(starts), torch.tensor(ns)))
+        ctx.host_k_lens = [s + n for s, n in zip(starts, ns)]
+        ctx.context_lens.copy_(torch.tensor(ctx.host_k_lens))
+        ctx.slot_mapping.copy_(torch.cat([slots(r, s, n) for r, (s, n) in enumerate(zip(starts, ns))]))
+        # the second sequence's chain is taken up to node `number`: a child at u = 0 is, at u = 1 - 2^-24 it is not
+        u.copy_(torch.rand(T, generator=g))
+        u[7:11] = torch.tensor([0.0 if i <= number else 1 - 2.0 ** -24 for i in range(4)])
+        ud.copy_(torch.rand(B, generator=g))
+        before = [t.clone() for t in pool]
+        if not captured:
+            x = step()
+        else:
+            if graph is None:
+                step()                      # plans and workspaces
+                torch.cuda.synchronize()
+                for t, b in zip(pool, before):
+                    t.copy_(b)
+                graph = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(graph):
+                    x = step()
+            graph.replay()
+        torch.cuda.synchronize()
+        after = [t.clone() for t in pool]
+        # each operator by its plain form
+        mask, depth = R.tree_mask(par.cpu(), [0, 7, 11, 12], 7)
+        assert torch.equal(x["mask"].cpu(), mask) and torch.equal(x["depth"].cpu(), depth)
+        for t, b in zip(pool, before):
+            t.copy_(b)
+        assert torch.equal(pass_through(x), x["logits"])
+        path, length, token = R.tree_verify(x["logits"].cpu(), tokens.cpu(), par.cpu(), ns, 7, temps.cpu(), u.cpu(), ud.cpu())
+        assert torch.equal(x["path"].cpu(), path) and torch.equal(x["length"].cpu(), length) and torch.equal(x["next"].cpu(), token)
+        R.tree_commit(run.kv_cache, ns, ctx.host_k_lens, tables[:B].tolist(), path, length, run.kv_scale_cache)
+        for t, a in zip(pool, after):
+            assert torch.equal(t.view(torch.uint8) if t.element_size() == 1 else t, a.view(torch.uint8) if a.element_size() == 1 else a)
+        lengths.append(length.tolist())
+        for b in range(B):
+            lines[b] += [trees[b][i] for i in path[b, 1:length[b]].tolist()] + [int(token[b])]
+    assert [n[1:] for n in lengths] == [[min(i, 3) + 1, 1] for i in range(4)]
+    if kv == "none":
+        assert lines[0] == good[:len(lines[0])] and [n[0] for n in lengths] == [3] * 4
+    # the next tokens' logits behind the committed cache, and behind a cache that the whole lines are written to at once:
+    # bf16 activations, and an 8-bit cache that rounds rows again where they change blocks
+    got = forward([0, 1, 2], [[l[-1]] for l in lines], [len(l) - 1 for l in lines], decode=3)
+    for b in range(B):
+        want = forward([3 + b], [lines[b]], [0])[-1].float()
+        assert (got[b].float() - want).abs().max() <= (0.05 if kv == "none" else 0.3) * want.std()
