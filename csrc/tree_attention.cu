@@ -24,8 +24,8 @@
 // memory and added at the end to the rows that see it.
 //
 // What bounds it.  Up to 64 rows the bytes of K and V should: 64 trees of 16 nodes, 32 query and 8 KV heads, 2048
-// tokens, bf16: 126 us, 4.4 TB/s (a tile's round of product, maximum, weights and store is longer than its bytes take);
-// 128 trees of 8 on e4m3: 298 us, 1.8 TB/s (a round takes twice as long beside the eight warps that convert).  Beyond, the
+// tokens, bf16: 127 us, 4.35 TB/s (a tile's round of product, maximum, weights and store is longer than its bytes take);
+// 128 trees of 8 on e4m3: 295 us, 1.9 TB/s (a round takes twice as long beside the eight warps that convert).  Beyond, the
 // exponentials: 24 trees of up to 64 nodes, 64 and 8 heads, up to 8191 tokens: 252-261 us, 530-550 TFLOP/s; two groups'
 // weights of a tile take 3800 clocks in turn, the products 2048.
 #include <cuda.h>
@@ -691,7 +691,7 @@ __global__ void __launch_bounds__(FP8 ? 512 : 384, 1)
                   y.x *= vs;
                   y.y *= vs;
                 }
-                // rounded by 2^-9 of a weight at most; the sum takes the weights as they were
+                // rounded by 2^-8 of a weight at most; the sum takes the weights as they were
                 p[8 * c + (i >> 1)] = pack_bf16(y.x, y.y);
               }
             });
@@ -1254,7 +1254,7 @@ __global__ void __launch_bounds__(FP8 ? 512 : 256, 1)
           }
           asm volatile("bar.sync 1, 128;" ::: "memory");  // red has been read
         }
-        // weights: rounded to bf16 (2^-9 of each at most; e4m3: times V's scale), their sums taken as they were
+        // weights: rounded to bf16 (2^-8 of each at most; e4m3: times V's scale), their sums taken as they were
         uint32_t p[N / 2];
         columns([&](int c, uint32_t(&v)[16]) {
 #pragma unroll

@@ -211,8 +211,8 @@ cudaError_t launch_tree_commit(const TreeCommit& a, cudaStream_t stream) {
     return cudaErrorInvalidValue;
   // CTAs per sequence: in all as many as four rounds of four per SM, since paths differ in length; a group of lanes
   // then has a few units, and a CTA's way to its first row is paid a few times only.  128 trees of 16 nodes, 64
-  // layers, e4m3, at 1, 2, 4, 8, 16, 32 CTAs each: 183, 106, 66, 49, 44, 46 us (115 MB in rows of 128 bytes: 2.6 TB/s;
-  // on many caches in turn 60 us).
+  // layers, e4m3, at 1, 2, 4, 8, 16, 32 CTAs each: 183, 106, 66, 49, 44, 46 us (115 MB in rows of 128 bytes on one pair of
+  // caches, most of which stays in the L2: 2.6 TB/s; on caches in turn, as in a step, 60 us at 16: 1.9 TB/s).
   const int units = CT / (a.kv_fp8 ? 8 : 16), most = (2 * a.layers * a.nkv + units - 1) / units;
   const int share = (16 * 148 + a.num_seqs - 1) / a.num_seqs;
   const dim3 grid(share < most ? share : most, a.num_seqs);

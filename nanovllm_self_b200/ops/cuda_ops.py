@@ -202,7 +202,7 @@ class CudaOps:
     def verify_tree(self, logits, tokens, parents, ctx, temperatures, uniforms, draw_uniforms, draft_probs=None):
         """(path int32 [B, max_seqlen_q], length int32 [B], next token int32 [B]): the walk through each tree by
         rejection sampling from these random numbers (``torch_ref.tree_verify`` has the formulas).  logits [T, V]
-        bf16 or fp32, one row per node; tokens, parents int32 [T]; temperatures fp32 [B] (0 and below: greedy);
+        bf16 or fp32, one row per node (whole rows: the shards of tensor-parallel ranks gathered); tokens, parents int32 [T]; temperatures fp32 [B] (0 and below: greedy);
         uniforms fp32 [T], draw_uniforms fp32 [B] in [0, 1); draft_probs fp32 [T, V], row i what i's children were
         drawn from, or None where they were not drawn."""
         self.launches += 1
